@@ -41,7 +41,7 @@ extern "C" {
 #define LFFN_ERR_LAUNCH      -3   /* hipGetLastError() after the launch was not hipSuccess */
 #define LFFN_ERR_SCRATCH     -4   /* an entry point that allocates nothing: the shape exceeds its static scratch */
 
-#define LFFN_ABI_VERSION 15
+#define LFFN_ABI_VERSION 16
 
 /* ABI version of the loaded library (LFFN_ABI_VERSION at build time). */
 int lffn_version(void);
@@ -888,6 +888,72 @@ int lffn_linear_norm_f32(const float *x, const float *norm_weight, const float *
 #define LFFN_ATTENTION_MAX_KEYS 2048
 int lffn_attention_f32(const float *q, const float *k, const float *v, const float *mask, float *out, int64_t B,
                        int64_t L, int64_t heads, void *stream);
+
+/* ------------------------------------------------- attention to an encoder's states */
+
+/* Formats of the two operators below: those of the gather's rows, 0 float, 1 bfloat16, 2 half. */
+
+/*
+ * Norms of queries and keys for each head and the rotation to their positions, one launch:
+ *   y = x / sqrt(mean(x^2) + eps) * weight over the columns of a head; then of the first `rotary` columns every pair (a, b) becomes
+ *   (a cos - b sin, b cos + a sin), pairs (i, i + rotary / 2), or (2 i, 2 i + 1) where `interleaved` is not 0.
+ * table: [table_rows, rotary] float, the cosines of a position's rotary / 2 angles and then their sines; rotary 0: no rotation.
+ * positions: [B, len] with a batch stride (0: the same for every sequence), int32 or int64 (positions_64), or NULL: 0, 1, 2 ...; a
+ * position outside the table is clamped into it.
+ * x: rows of `columns` numbers that lie together; strides in elements of batch, token and head, multiples of 16 bytes, as are the addresses.
+ * q_weight, k_weight: [columns] float, 16-byte aligned, or NULL.  k NULL: queries alone.  columns a multiple of 8, at most 256;
+ * rotary a multiple of 16, at most columns.  Sums in fp32, one rounding.  q_out, k_out: [B, len, heads, columns], no input's memory.
+ */
+typedef struct lffn_qk_norm_rotary {
+    const void *q, *k;
+    const float *q_weight, *k_weight, *table;
+    const void *q_positions, *k_positions;
+    int64_t B, q_len, k_len, q_heads, k_heads, columns, rotary, table_rows;
+    int64_t q_strides[3], k_strides[3];
+    int64_t q_positions_stride, k_positions_stride;
+    float eps;
+    int32_t format, positions_64, interleaved;
+} lffn_qk_norm_rotary;
+int lffn_qk_norm_rotary_fwd(const lffn_qk_norm_rotary *a, void *q_out, void *k_out, void *stream);
+
+/*
+ * Its backward.  g_q, g_k and grad_q, grad_k: [B, len, heads, columns] (k's NULL where k is); grad_q_weight, grad_k_weight: [columns]
+ * float or NULL (not wanted, or no weight).  workspace: 16-byte aligned, of lffn_qk_norm_rotary_bwd_workspace_bytes.  Sums of the weights'
+ * gradients in a fixed order: the same bits on every call.
+ */
+int lffn_qk_norm_rotary_bwd_workspace_bytes(const lffn_qk_norm_rotary *a, int64_t *bytes);
+int lffn_qk_norm_rotary_bwd(const lffn_qk_norm_rotary *a, const void *g_q, const void *g_k, void *grad_q, void *grad_k,
+                            float *grad_q_weight, float *grad_k_weight, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Attention of queries to keys and values of another length, key_heads <= heads (heads / key_heads neighbouring query heads share a key head):
+ *   out[b, i, h] = sum_j p_j v[b, j, h'],  p = softmax_j(scale q[b, i, h] . k[b, j, h'])  over the keys that take part.
+ * q: [B, q_len, heads, columns], k, v: [B, k_len, key_heads, columns], by strides (elements) of batch, token and head, multiples of 16 bytes,
+ * as are the addresses; columns lie together, a multiple of 8, at most 128.  key_mask: [B, k_len] bytes, not 0 where a key takes part, with a
+ * batch stride, or NULL.  Keys and values that take no part are not read.  A query without keys gets zeros.  scale: positive, finite.
+ * format 0: fp32 accuracy, 1 and 2: products of 16 bits, sums in fp32, softmax weights rounded to the format.
+ * out: [B, q_len, heads, columns], in the format.  lse: [B, key_heads, q_len * heads / key_heads] or NULL, what the backward needs of a row
+ * (private to it).  workspace: 16-byte aligned, of lffn_cross_attention_workspace_bytes (0: may be NULL).
+ */
+typedef struct lffn_cross_attention {
+    const void *q, *k, *v;
+    const uint8_t *key_mask;
+    int64_t B, q_len, k_len, heads, key_heads, columns;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    int64_t mask_stride;
+    float scale;
+    int32_t format;
+} lffn_cross_attention;
+int lffn_cross_attention_workspace_bytes(const lffn_cross_attention *a, int64_t *bytes);
+int lffn_cross_attention_fwd(const lffn_cross_attention *a, void *out, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Its backward: from out and lse of the forward and the gradient of out, the gradients of q, k and v, all contiguous as out (k's and v's
+ * [B, k_len, key_heads, columns]); zeros for keys that take no part.  No atomics: the same bits on every call.
+ */
+int lffn_cross_attention_bwd_workspace_bytes(const lffn_cross_attention *a, int64_t *bytes);
+int lffn_cross_attention_bwd(const lffn_cross_attention *a, const void *out, const float *lse, const void *g_out, void *grad_q, void *grad_k,
+                             void *grad_v, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,7 @@ from .bh4 import (FastHadamardTransform, FastHadamardTransformDim512, FastHadama
 from .compute_code_score import ComputeCodeScore, bin2dec, compute_code_score, compute_code_score_torch
 from .gather import (LookupGather, WeightedVectorGatherAdd, gather, indexed_inner_product, lookup_gather,
                      weighted_gather_add, weighted_vector_gather_add, weighted_vector_scatter_add)
+from .cross_attention import CrossAttentionFunction, QkNormRotary, cross_attention, qk_norm_rotary, rotary_table
 from .lookup import BH4, Hashing, LookupFFN
 from .encoder import Attention, Encoder, EncoderLayer, Lookup, RobertaEmbeddings
 
@@ -21,4 +22,5 @@ __all__ = [
     "compute_code_score", "compute_code_score_torch", "bin2dec", "ComputeCodeScore",
     "gather", "weighted_gather_add", "weighted_vector_gather_add", "indexed_inner_product",
     "weighted_vector_scatter_add", "WeightedVectorGatherAdd", "LookupGather", "lookup_gather",
+    "cross_attention", "qk_norm_rotary", "rotary_table", "CrossAttentionFunction", "QkNormRotary",
 ]

@@ -16,7 +16,7 @@ _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 # LOOKUPFFN_HIP_LIB points at another build of the same ABI (e.g. a tuning build)
 LIB_PATH = os.environ.get("LOOKUPFFN_HIP_LIB") or os.path.join(_PKG_DIR, "liblookupffn_hip.so")
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 LFFN_OK = 0
 LFFN_ERR_BAD_ARG = -1
@@ -145,6 +145,28 @@ class Sum(ctypes.Structure):
     _fields_ = [("parts", _vp), ("out", _vp), ("n", _i64), ("num_partials", _i64)]
 
 
+class QkNormRotary(ctypes.Structure):
+    """struct lffn_qk_norm_rotary of include/lookupffn_hip.h."""
+    _fields_ = [("q", _vp), ("k", _vp), ("q_weight", _vp), ("k_weight", _vp), ("table", _vp), ("q_positions", _vp), ("k_positions", _vp),
+                ("B", _i64), ("q_len", _i64), ("k_len", _i64), ("q_heads", _i64), ("k_heads", _i64), ("columns", _i64), ("rotary", _i64),
+                ("table_rows", _i64), ("q_strides", _i64 * 3), ("k_strides", _i64 * 3), ("q_positions_stride", _i64),
+                ("k_positions_stride", _i64), ("eps", _f32), ("format", _i32), ("positions_64", _i32), ("interleaved", _i32)]
+
+
+class CrossAttention(ctypes.Structure):
+    """struct lffn_cross_attention of include/lookupffn_hip.h."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("key_mask", _vp), ("B", _i64), ("q_len", _i64), ("k_len", _i64), ("heads", _i64),
+                ("key_heads", _i64), ("columns", _i64), ("q_strides", _i64 * 3), ("k_strides", _i64 * 3), ("v_strides", _i64 * 3),
+                ("mask_stride", _i64), ("scale", _f32), ("format", _i32)]
+
+
+SIGNATURES["lffn_qk_norm_rotary_fwd"] = [ctypes.POINTER(QkNormRotary), _vp, _vp, _vp]
+SIGNATURES["lffn_qk_norm_rotary_bwd_workspace_bytes"] = [ctypes.POINTER(QkNormRotary), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_qk_norm_rotary_bwd"] = [ctypes.POINTER(QkNormRotary), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
+SIGNATURES["lffn_cross_attention_workspace_bytes"] = [ctypes.POINTER(CrossAttention), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_cross_attention_fwd"] = [ctypes.POINTER(CrossAttention), _vp, _vp, _vp, _i64, _vp]
+SIGNATURES["lffn_cross_attention_bwd_workspace_bytes"] = [ctypes.POINTER(CrossAttention), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_cross_attention_bwd"] = [ctypes.POINTER(CrossAttention), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
 SIGNATURES["lffn_sum_many_f32"] = [ctypes.POINTER(Sum), _i32, _vp]
 SIGNATURES["lffn_lookup_backward_sums_f32"] = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp]
 SIGNATURES["lffn_lookup_backward_sums_rows"] = [_i64, ctypes.POINTER(_i64)]

@@ -1,0 +1,322 @@
+// softmax(scale q k^T) v of queries against an encoder's states: the forward kernels (cross_attention.h: operands and tiles).
+//
+// A workgroup has 128 rows (queries of the heads that share a key head), 32 a wavefront, and walks the keys 64 at a time with the running maximum and
+// sum of a softmax taken in one pass.  Keys and values are fetched a step ahead and lie in LDS as in memory, in two buffers; scores are
+// formed as keys x queries, weights times values as (values turned round) x weights.  Steps without a key that takes part are left out, masked
+// keys and values are zeros that nobody fetched.  Where there are too few rows to fill the chip the keys are shared out over several workgroups,
+// whose results a second kernel joins.
+#include "cross_attention.h"
+
+using namespace cross_attention;
+
+namespace {
+
+struct FwdArgs {
+    const char *q, *k, *v;
+    const uint8_t *mask;
+    char *out;
+    float *lse, *part, *part_lse;         // parts: [splits, B, key heads, rows(, columns)]
+    int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, mask_stride;         // strides in bytes
+    int64_t keys, steps, split_steps;
+    int key_heads, group, rows, row_tiles, splits, columns;
+    int64_t q_len, units;
+    float c;                              // scale log2 e
+};
+
+constexpr float SLACK = 6.f;              // how far (powers of two) a row's largest score may outgrow the one that its sums go by
+
+template <typename F, int DP, int KT>
+__global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1 || DP <= 64 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
+    typedef Tile<F, DP, KT> T;
+    typedef Frag<F::PLANES> Op;
+    constexpr int CHUNKS = DP / 16, KB = KT / 32, DB = DP / 32;
+    extern __shared__ __attribute__((aligned(16))) uint4 lds[];           // [2][keys, values], words
+    uint64_t *const words = reinterpret_cast<uint64_t *>(lds + 4 * T::SIZE);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, half = lane >> 5;
+    const int64_t unit = unit_of(blockIdx.x, a.units);
+    const int tile = unit % a.row_tiles, split = unit / a.row_tiles % a.splits;
+    const int64_t bh = unit / a.row_tiles / a.splits, b = bh / a.key_heads, kh = bh - b * a.key_heads;
+    const int pieces = a.columns / 8;
+    const Rows rows{a.q + b * a.qb + kh * a.group * a.qh, a.qt, a.qh, a.group};
+    const char *const kp = a.k + b * a.kb + kh * a.kh, *const vp = a.v + b * a.vb + kh * a.vh;
+    const uint8_t *const mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+    const int row = tile * TILE + wave * ROWS + r;
+
+    typename F::Raw rk[T::SHARE], rv[T::SHARE];
+    auto fetch = [&](int64_t step, uint64_t word) {
+#pragma unroll
+        for (int i = 0; i < T::SHARE; ++i) {
+            const int p = tid + WG * i, key = p / T::PIECES, piece = p % T::PIECES;
+            const bool live = (word >> key & 1) && piece < pieces;
+            const int64_t at = step * KT + key;
+            rk[i] = live ? F::load(kp + at * a.kt + piece * 8 * F::BYTES) : F::zero();
+            rv[i] = live ? F::load(vp + at * a.vt + piece * 8 * F::BYTES) : F::zero();
+        }
+    };
+    auto place = [&](int buf) {
+        uint4 *const to = lds + buf * 2 * T::SIZE;
+#pragma unroll
+        for (int i = 0; i < T::SHARE; ++i) {
+            const int p = tid + WG * i, key = p / T::PIECES, piece = p % T::PIECES;
+            T::put(to, key, piece, rk[i]);
+            T::put(to + T::SIZE, key, piece, rv[i]);
+        }
+    };
+
+    Op fq[CHUNKS];
+    {
+        const bool live = row < a.rows;
+        const char *const p = rows.at(live ? row : 0);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) fq[c] = own_rows<F>(p, live, c, half, pieces);
+    }
+    ca_f32x16_t o[DB] = {};
+    float most = -INFINITY, sum = 0.f;
+
+    auto compute = [&](int buf, uint64_t word) {
+        const uint4 *const keys = lds + buf * 2 * T::SIZE, *const values = keys + T::SIZE;
+        ca_f32x16_t s[KB] = {};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) s[kb] = F::mma(T::rows(keys, kb * 32 + r, c, half), fq[c], s[kb]);
+        constexpr uint64_t FULL = KT == 64 ? ~0ull : (1ull << KT) - 1;
+        if (word != FULL) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const uint32_t w = (uint32_t)(word >> (32 * kb)) >> (4 * half);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(w >> (8 * (e / 4) + e % 4) & 1)) s[kb][e] = -INFINITY;
+            }
+        }
+        float now = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) now = fmaxf(now, s[kb][e]);
+        now = fmaxf(now, lane_xor<32>(now));
+        if (__any((now - most) * a.c > SLACK)) {             // (the first step's is: most is -infinity; -infinity - itself is no number, and not above)
+            const float to = fmaxf(most, now), by = most == to ? 1.f : __builtin_amdgcn_exp2f(most * a.c - to * a.c);
+            sum *= by;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= by;
+            most = to;
+        }
+        const float less = (most == -INFINITY ? 0.f : most) * a.c - F::LIFT;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], a.c, -less));
+                sum += s[kb][e];
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = s[kb][8 * c + e];
+                const Op p = F::operand(t);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] = F::mma(T::columns(values, kb * 32 + c * 16, d, lane), p, o[d]);
+            }
+        }
+    };
+
+    const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
+#pragma unroll 1
+    for (int64_t first = begin; first < end; first += BLOCK) {
+        look_at_masks<KT>(words, mask, first, end, a.keys);
+        __syncthreads();
+        const uint64_t mine = words[lane];
+        uint64_t left = __ballot(mine != 0);
+        if (left) {
+            int i = __builtin_ctzll(left), buf = 0;
+            uint64_t word = uniform(words[i]);
+            left &= left - 1;
+            fetch(first + i, word);
+            place(0);
+            __syncthreads();
+#pragma unroll 1
+            for (;;) {
+                const bool more = left != 0;
+                uint64_t next = 0;
+                if (more) {
+                    i = __builtin_ctzll(left);
+                    left &= left - 1;
+                    next = uniform(words[i]);
+                    fetch(first + i, next);
+                }
+                compute(buf, word);
+                if (!more) break;
+                place(buf ^ 1);
+                __syncthreads();
+                buf ^= 1;
+                word = next;
+            }
+        }
+        __syncthreads();                  // the words and the buffers are free again
+    }
+
+    sum += lane_xor<32>(sum);
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query without keys: zeros
+    if (row >= a.rows) return;
+    const float level = sum == 0.f ? INFINITY : (most == -INFINITY ? 0.f : most) * a.c - F::LIFT + __builtin_amdgcn_logf(sum);
+    const int64_t at = bh * a.rows + row;
+    if (a.splits > 1) {
+        const int64_t of = int64_t(split) * (a.units / a.splits / a.row_tiles) * a.rows + at;
+        if (half == 0) a.part_lse[of] = level;
+        float *const p = a.part + of * a.columns;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = 32 * d + 8 * g + 4 * half;
+                if (col < a.columns)
+                    *reinterpret_cast<float4 *>(p + col) =
+                        make_float4(o[d][4 * g] * inverse, o[d][4 * g + 1] * inverse, o[d][4 * g + 2] * inverse, o[d][4 * g + 3] * inverse);
+            }
+        return;
+    }
+    if (a.lse && half == 0) a.lse[at] = level;
+    char *const p = a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = 32 * d + 8 * g + 4 * half;
+            if (col < a.columns)
+                F::store4(p + col * F::BYTES, o[d][4 * g] * inverse, o[d][4 * g + 1] * inverse, o[d][4 * g + 2] * inverse, o[d][4 * g + 3] * inverse);
+        }
+}
+
+// The splits' results of a row as one: weights 2^(level - largest level).  Four columns a lane.
+template <typename F>
+__global__ __launch_bounds__(WG) void join_kernel(FwdArgs a, int64_t all_rows) {
+    const int quads = a.columns / 4;
+    const int64_t i = int64_t(blockIdx.x) * WG + threadIdx.x, at = i / quads;
+    const int col = int(i - at * quads) * 4;
+    if (at >= all_rows) return;
+    float most = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) {
+        const float l = a.part_lse[s * all_rows + at];
+        if (l != INFINITY) most = fmaxf(most, l);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float l = a.part_lse[s * all_rows + at];
+        if (l == INFINITY) continue;                     // (no key that takes part)
+        const float w = __builtin_amdgcn_exp2f(l - (most == -INFINITY ? 0.f : most));
+        const float4 v = *reinterpret_cast<const float4 *>(a.part + (s * all_rows + at) * a.columns + col);
+        sum += w;
+        acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
+    }
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t bh = at / a.rows, b = bh / a.key_heads, kh = bh - b * a.key_heads;
+    const int row = int(at - bh * a.rows);
+    if (a.lse && col == 0) a.lse[at] = sum == 0.f ? INFINITY : most + __builtin_amdgcn_logf(sum);
+    char *const p = a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
+    F::store4(p + col * F::BYTES, acc.x * by, acc.y * by, acc.z * by, acc.w * by);
+}
+
+}  // namespace
+
+__attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(const lffn_cross_attention *a) {
+    LFFN_REQUIRE(a, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->B >= 0 && a->q_len >= 0 && a->k_len >= 0 && a->heads >= 0 && a->key_heads >= 1 && a->columns >= 1, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->heads % a->key_heads == 0 && a->format >= 0 && a->format <= 2, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->scale > 0.f && a->scale <= 3.4e38f, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->columns % 8 == 0 && a->columns <= 128, LFFN_ERR_UNSUPPORTED);
+    const int64_t size = a->format == LFFN_ROWS_F32 ? 4 : 2;
+    for (int d = 0; d < 3; ++d)
+        for (const int64_t s : {a->q_strides[d], a->k_strides[d], a->v_strides[d]})
+            LFFN_REQUIRE(s >= 0 && s * size % 16 == 0, LFFN_ERR_BAD_ARG);
+    const bool no_rows = a->B == 0 || a->q_len == 0 || a->heads == 0, no_keys = a->B == 0 || a->k_len == 0;
+    LFFN_REQUIRE((a->q || no_rows) && ((a->k && a->v) || no_keys) && a->mask_stride >= 0, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(lffn_aligned16(a->q) && lffn_aligned16(a->k) && lffn_aligned16(a->v), LFFN_ERR_BAD_ARG);
+    const int64_t most = int64_t(1) << 30;
+    LFFN_REQUIRE(a->heads <= 65536 && a->q_len < most && a->k_len < most && a->B < most, LFFN_ERR_UNSUPPORTED);
+    LFFN_REQUIRE(no_rows || (a->q_len * (a->heads / a->key_heads) < most &&
+                             a->B * a->key_heads <= (int64_t(1) << 40) / (a->q_len * (a->heads / a->key_heads))), LFFN_ERR_UNSUPPORTED);
+    return LFFN_OK;
+}
+
+namespace {
+
+constexpr int64_t WANTED = 512;           // workgroups, where there are keys enough to share out
+constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
+
+// Fills sizes in; the workspace's bytes.
+int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
+    const int64_t size = c.format == LFFN_ROWS_F32 ? 4 : 2;
+    const int kt = c.format == LFFN_ROWS_F32 && c.columns > 64 ? 32 : 64;
+    a.q = static_cast<const char *>(c.q), a.k = static_cast<const char *>(c.k), a.v = static_cast<const char *>(c.v);
+    a.mask = c.key_mask, a.mask_stride = c.mask_stride;
+    a.qb = c.q_strides[0] * size, a.qt = c.q_strides[1] * size, a.qh = c.q_strides[2] * size;
+    a.kb = c.k_strides[0] * size, a.kt = c.k_strides[1] * size, a.kh = c.k_strides[2] * size;
+    a.vb = c.v_strides[0] * size, a.vt = c.v_strides[1] * size, a.vh = c.v_strides[2] * size;
+    a.keys = c.k_len, a.q_len = c.q_len;
+    a.key_heads = (int)c.key_heads, a.group = int(c.heads / c.key_heads), a.columns = (int)c.columns;
+    a.rows = int(c.q_len * a.group);
+    a.row_tiles = (a.rows + TILE - 1) / TILE;
+    a.steps = (c.k_len + kt - 1) / kt;
+    a.c = c.scale * LOG2E;
+    const int64_t tiles = c.B * c.key_heads * a.row_tiles;
+    int64_t splits = tiles > 0 && tiles < WANTED ? (WANTED + tiles - 1) / tiles : 1;
+    if (splits > a.steps / LEAST_STEPS) splits = a.steps / LEAST_STEPS;
+    if (splits < 1) splits = 1;
+    a.split_steps = (a.steps + splits - 1) / splits;
+    a.splits = a.split_steps ? int((a.steps + a.split_steps - 1) / a.split_steps) : 1;
+    a.units = tiles * a.splits;
+    return a.splits > 1 ? a.splits * c.B * c.key_heads * a.rows * (a.columns + 1) * 4 : 0;
+}
+
+template <typename F, int DP, int KT>
+int launch(const FwdArgs &a, hipStream_t stream) {
+    static LdsGrant granted;
+    const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + BLOCK * 8;
+    if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&cross_attention_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
+    cross_attention_kernel<F, DP, KT><<<dim3((unsigned)a.units), dim3(WG), bytes, stream>>>(a);
+    if (a.splits > 1) {
+        const int64_t rows = a.units / a.splits / a.row_tiles * a.rows;
+        join_kernel<F><<<dim3((unsigned)((rows * (a.columns / 4) + WG - 1) / WG)), dim3(WG), 0, stream>>>(a, rows);
+    }
+    return lffn_launch_status();
+}
+
+template <typename F>
+int launch(const FwdArgs &a, hipStream_t stream) {
+    if (a.columns <= 32) return launch<F, 32, 64>(a, stream);
+    if (a.columns <= 64) return launch<F, 64, 64>(a, stream);
+    return launch<F, 128, F::PLANES == 1 ? 64 : 32>(a, stream);
+}
+
+}  // namespace
+
+extern "C" int lffn_cross_attention_workspace_bytes(const lffn_cross_attention *c, int64_t *bytes) {
+    LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
+    if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
+    FwdArgs a{};
+    *bytes = plan(*c, a);
+    return LFFN_OK;
+}
+
+extern "C" int lffn_cross_attention_fwd(const lffn_cross_attention *c, void *out, float *lse, void *workspace, int64_t workspace_bytes,
+                                        void *stream) {
+    if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
+    FwdArgs a{};
+    const int64_t bytes = plan(*c, a);
+    if (a.units == 0) return LFFN_OK;
+    LFFN_REQUIRE(out && lffn_aligned16(out), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(bytes == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= bytes), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a.units <= INT32_MAX, LFFN_ERR_UNSUPPORTED);
+    a.out = static_cast<char *>(out), a.lse = lse;
+    a.part = static_cast<float *>(workspace);
+    a.part_lse = a.part ? a.part + int64_t(a.splits) * c->B * c->key_heads * a.rows * a.columns : nullptr;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (c->format == LFFN_ROWS_F32) return launch<F32>(a, s);
+    return c->format == LFFN_ROWS_BF16 ? launch<BF16>(a, s) : launch<F16>(a, s);
+}

@@ -1324,6 +1324,185 @@ def _(q, k, v, mask):
     return torch.empty_like(q)
 
 
+# ----------------------------------------------------------------------------- attention to an encoder's states
+
+def _head_strides(t):
+    """Strides (batch, token, head) of t [B, L, heads, columns]; of a dimension of one they say nothing."""
+    return (ctypes.c_int64 * 3)(*(0 if n <= 1 else s for n, s in zip(t.shape, t.stride()[:3])))
+
+
+def _head_rows(t):
+    """t [B, L, heads, columns] as the kernels read it, a copy where it has to be: the columns together, addresses and strides of 16 bytes."""
+    if t is None:
+        return None
+    size = t.element_size()
+    if (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and all(n <= 1 or s * size % 16 == 0
+                                                                              for n, s in zip(t.shape, t.stride()[:3])):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _aligned(t):
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _neighbours_together(p):
+    return p if p is None or p.shape[-1] <= 1 or p.stride(-1) == 1 else p.contiguous()
+
+
+def _qk_norm_rotary_args(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved):
+    a = _lib.QkNormRotary()
+    a.q, a.k, a.q_weight, a.k_weight, a.table = (_lib.ptr(t) for t in (q, k, q_weight, k_weight, table))
+    a.B, a.q_len, a.q_heads, a.columns = q.shape
+    a.q_strides, a.eps, a.format, a.interleaved = _head_strides(q), eps, row_format(q.dtype), interleaved
+    if k is not None:
+        a.k_len, a.k_heads, a.k_strides = k.shape[1], k.shape[2], _head_strides(k)
+    if table is not None:
+        a.table_rows, a.rotary = table.shape
+        for name, p in (("q_positions", q_positions), ("k_positions", k_positions)):
+            if p is not None:
+                setattr(a, name, p.data_ptr())
+                setattr(a, name + "_stride", p.stride(0) if p.dim() == 2 and p.shape[0] > 1 else 0)
+                a.positions_64 = p.dtype == torch.int64
+    return a
+
+
+_L.define("qk_norm_rotary(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? table, Tensor? q_positions, Tensor? k_positions, "
+          "float eps, bool interleaved) -> Tensor[]")
+
+
+def _qk_norm_rotary_impl(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved):
+    """q, k [B, L, heads, columns] (k None: one result); weights [columns], table [positions, rotary] fp32; positions [B, L] or [L], int32 or
+    int64, both alike."""
+    _lib.require_gpu(q, k, q_weight, k_weight, table, q_positions, k_positions)
+    q, k, q_weight, k_weight, table = _head_rows(q), _head_rows(k), _aligned(q_weight), _aligned(k_weight), _aligned(table)
+    q_positions, k_positions = _neighbours_together(q_positions), _neighbours_together(k_positions)
+    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k) if t is not None]
+    a = _qk_norm_rotary_args(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)
+    with _dev_guard(q):
+        rc = _lib.load().lffn_qk_norm_rotary_fwd(ctypes.byref(a), out[0].data_ptr(), out[-1].data_ptr(), _lib.stream_of(q))
+    _lib.check(rc, f"lffn_qk_norm_rotary_fwd(q={tuple(q.shape)}, k={None if k is None else tuple(k.shape)})")
+    return out
+
+
+_L.impl("qk_norm_rotary", _qk_norm_rotary_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::qk_norm_rotary")
+def _(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved):
+    return [t.new_empty(t.shape) for t in (q, k) if t is not None]
+
+
+_L.define("qk_norm_rotary_bwd(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? table, Tensor? q_positions, Tensor? k_positions, "
+          "float eps, bool interleaved, Tensor g_q, Tensor? g_k, bool want_q_weight, bool want_k_weight) -> Tensor[]")
+
+
+def _qk_norm_rotary_bwd_impl(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved, g_q, g_k, want_q_weight,
+                             want_k_weight):
+    """-> gradients of q, of k where there is one, and of the weights that are wanted."""
+    _lib.require_gpu(q, k, q_weight, k_weight, table, q_positions, k_positions, g_q, g_k)
+    q, k, q_weight, k_weight, table = _head_rows(q), _head_rows(k), _aligned(q_weight), _aligned(k_weight), _aligned(table)
+    q_positions, k_positions, g_q, g_k = _neighbours_together(q_positions), _neighbours_together(k_positions), _aligned(g_q), _aligned(g_k)
+    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k) if t is not None]
+    a = _qk_norm_rotary_args(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)
+    weights = [None, None]
+    for i, (wanted, t) in enumerate(((want_q_weight, q), (want_k_weight, k))):
+        if wanted:           # (a sum over no rows is nothing that a kernel writes)
+            weights[i] = (torch.empty if t.numel() else torch.zeros)(t.shape[3], dtype=torch.float32, device=q.device)
+    given = [None if w is None or t.numel() == 0 else w.data_ptr() for w, t in zip(weights, (q, k))]
+    with _dev_guard(q):
+        lib, n = _lib.load(), ctypes.c_int64(0)
+        _lib.check(lib.lffn_qk_norm_rotary_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_qk_norm_rotary_bwd_workspace_bytes")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        rc = lib.lffn_qk_norm_rotary_bwd(ctypes.byref(a), _lib.ptr(g_q), _lib.ptr(g_k), out[0].data_ptr(), out[-1].data_ptr(), *given,
+                                         ws.data_ptr(), ws.nbytes, _lib.stream_of(q))
+    _lib.check(rc, f"lffn_qk_norm_rotary_bwd(q={tuple(q.shape)}, k={None if k is None else tuple(k.shape)})")
+    return out + [w for w in weights if w is not None]
+
+
+_L.impl("qk_norm_rotary_bwd", _qk_norm_rotary_bwd_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::qk_norm_rotary_bwd")
+def _(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved, g_q, g_k, want_q_weight, want_k_weight):
+    return ([t.new_empty(t.shape) for t in (q, k) if t is not None]
+            + [q.new_empty(q.shape[3], dtype=torch.float32) for wanted in (want_q_weight, want_k_weight) if wanted])
+
+
+CROSS_ATTENTION_MAX_COLUMNS = 128
+QK_NORM_MAX_COLUMNS = 256
+
+
+def _cross_attention_args(q, k, v, key_mask, scale):
+    a = _lib.CrossAttention()
+    a.q, a.k, a.v, a.key_mask = (_lib.ptr(t) for t in (q, k, v, key_mask))
+    a.B, a.q_len, a.heads, a.columns = q.shape
+    a.k_len, a.key_heads = k.shape[1:3]
+    a.q_strides, a.k_strides, a.v_strides = _head_strides(q), _head_strides(k), _head_strides(v)
+    a.mask_stride = 0 if key_mask is None or key_mask.shape[0] <= 1 else key_mask.stride(0)
+    a.scale, a.format = scale, row_format(q.dtype)
+    return a
+
+
+_L.define("cross_attention(Tensor q, Tensor k, Tensor v, Tensor? key_mask, float scale, bool keep) -> (Tensor, Tensor)")
+
+
+def _cross_attention_impl(q, k, v, key_mask, scale, keep):
+    """q [B, L, heads, columns], k, v [B, keys, key heads, columns], key_mask [B, keys] bool or None -> (out [B, L, heads, columns], with
+    `keep` what the backward needs of every row, fp32)."""
+    _lib.require_gpu(q, k, v, key_mask)
+    q, k, v, key_mask = _head_rows(q), _head_rows(k), _head_rows(v), _neighbours_together(key_mask)
+    a = _cross_attention_args(q, k, v, key_mask, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2] if keep else 0, dtype=torch.float32, device=q.device)
+    with _dev_guard(q):
+        lib, n = _lib.load(), ctypes.c_int64(0)
+        _lib.check(lib.lffn_cross_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_cross_attention_workspace_bytes")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
+        rc = lib.lffn_cross_attention_fwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr() if keep else None, _lib.ptr(ws), n.value,
+                                          _lib.stream_of(q))
+    _lib.check(rc, f"lffn_cross_attention_fwd(q={tuple(q.shape)}, k={tuple(k.shape)})")
+    return out, lse
+
+
+_L.impl("cross_attention", _cross_attention_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::cross_attention")
+def _(q, k, v, key_mask, scale, keep):
+    return q.new_empty(q.shape), q.new_empty(q.shape[0] * q.shape[1] * q.shape[2] if keep else 0, dtype=torch.float32)
+
+
+_L.define("cross_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor? key_mask, float scale, Tensor out, Tensor lse, Tensor g) "
+          "-> (Tensor, Tensor, Tensor)")
+
+
+def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, lse, g):
+    _lib.require_gpu(q, k, v, key_mask, out, lse, g)
+    q, k, v, key_mask, g = _head_rows(q), _head_rows(k), _head_rows(v), _neighbours_together(key_mask), _aligned(g)
+    a = _cross_attention_args(q, k, v, key_mask, scale)
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+    with _dev_guard(q):
+        lib, n = _lib.load(), ctypes.c_int64(0)
+        _lib.check(lib.lffn_cross_attention_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_cross_attention_bwd_workspace_bytes")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        rc = lib.lffn_cross_attention_bwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), g.data_ptr(), *(t.data_ptr() for t in grads),
+                                          ws.data_ptr(), n.value, _lib.stream_of(q))
+    _lib.check(rc, f"lffn_cross_attention_bwd(q={tuple(q.shape)}, k={tuple(k.shape)})")
+    return tuple(grads)
+
+
+_L.impl("cross_attention_bwd", _cross_attention_bwd_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::cross_attention_bwd")
+def _(q, k, v, key_mask, scale, out, lse, g):
+    return tuple(t.new_empty(t.shape) for t in (q, k, v))
+
+
 fht = torch.ops.lookupffn.fht
 bh4_diag = torch.ops.lookupffn.bh4_diag
 bh4_fold = torch.ops.lookupffn.bh4_fold
@@ -1358,3 +1537,7 @@ lookup_inner = torch.ops.lookupffn.lookup_inner
 linear = torch.ops.lookupffn.linear
 linear_norm = torch.ops.lookupffn.linear_norm
 attention = torch.ops.lookupffn.attention
+qk_norm_rotary = torch.ops.lookupffn.qk_norm_rotary
+qk_norm_rotary_bwd = torch.ops.lookupffn.qk_norm_rotary_bwd
+cross_attention = torch.ops.lookupffn.cross_attention
+cross_attention_bwd = torch.ops.lookupffn.cross_attention_bwd
