@@ -949,7 +949,8 @@ int lffn_cross_attention_fwd(const lffn_cross_attention *a, void *out, float *ls
 
 /*
  * Its backward: from out and lse of the forward and the gradient of out, the gradients of q, k and v, all contiguous as out (k's and v's
- * [B, k_len, key_heads, columns]); zeros for keys that take no part.  No atomics: the same bits on every call.
+ * [B, k_len, key_heads, columns]); zeros for keys that take no part.  grad_q NULL, or grad_k and grad_v NULL: not wanted.  No atomics:
+ * the same bits on every call.
  */
 int lffn_cross_attention_bwd_workspace_bytes(const lffn_cross_attention *a, int64_t *bytes);
 int lffn_cross_attention_bwd(const lffn_cross_attention *a, const void *out, const float *lse, const void *g_out, void *grad_q, void *grad_k,

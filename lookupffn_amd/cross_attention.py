@@ -9,6 +9,7 @@ import math
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
+from torch.compiler import is_compiling
 
 from . import _lib, ops
 
@@ -26,6 +27,14 @@ def _check_heads(name, t, like=None):
     if like is not None:
         _require(t.dtype == like.dtype, f"{name}: {t.dtype}, queries are {like.dtype}")
         _require(t.shape[0] == like.shape[0] and t.shape[3] == like.shape[3], f"{name}: {tuple(t.shape)}, queries are {tuple(like.shape)}")
+
+
+def _host():
+    """The host path (csrc/host_attention.h), which answers None where it is not for a call; False where there is none."""
+    if is_compiling():
+        return False
+    host = _lib.loaded_host
+    return _lib.host() if host is None else host
 
 
 def rotary_table(positions, columns, base=10000.0, device=None):
@@ -91,6 +100,11 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, *, table=None, q_pos
     (i, i + rotated / 2), with ``interleaved`` (2 i, 2 i + 1).  Norms and rotation in float32, one rounding.
 
     -> (q, k) in new contiguous arrays, k None where it was.  Gradients: q, k and both weights; sums in a fixed order."""
+    host = _host()
+    if host:
+        out = host.qk_norm_rotary(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)
+        if out is not None:
+            return out
     _lib.require_gpu(q, k, q_weight, k_weight, table, q_positions, k_positions)
     _check_heads("q", q)
     columns = q.shape[3]
@@ -128,7 +142,9 @@ class CrossAttentionFunction(Function):
     @once_differentiable
     def backward(ctx, g):
         q, k, v, key_mask, out, lse = ctx.saved_tensors
-        return (*ops.cross_attention_bwd(q, k, v, key_mask, ctx.scale, out, lse, g), None, None)
+        of_queries, of_keys = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        grads = list(ops.cross_attention_bwd(q, k, v, key_mask, ctx.scale, out, lse, g, of_queries, of_keys))
+        return ((grads.pop(0) if of_queries else None), *(grads if of_keys else (None, None)), None, None)
 
 
 def cross_attention(q, k, v, key_mask=None, *, scale=None):
@@ -142,6 +158,11 @@ def cross_attention(q, k, v, key_mask=None, *, scale=None):
     float32: products of three bfloat16 terms a number, sums in float32, as exact as a float32 product; 16 bits: softmax weights rounded to the
     type, sums in float32, one rounding of the result.  Infinities and NaN of keys that take part may make any result of their head NaN.
     -> [B, L, heads, columns].  Gradients: q, k and v, the same bits on every call."""
+    host = _host()
+    if host:
+        out = host.cross_attention(q, k, v, key_mask, scale)
+        if out is not None:
+            return out
     _lib.require_gpu(q, k, v, key_mask)
     _check_heads("q", q)
     _check_heads("k", k, q)

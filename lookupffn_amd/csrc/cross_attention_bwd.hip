@@ -494,8 +494,11 @@ extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const voi
     if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
     Plan p = plan(*c);
     if (p.q.units == 0 && p.k.units == 0) return LFFN_OK;
-    LFFN_REQUIRE(p.q.units == 0 || (out && lse && g_out && grad_q), LFFN_ERR_BAD_ARG);
-    LFFN_REQUIRE(p.k.units == 0 || (grad_k && grad_v), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(p.q.units == 0 || (out && lse && g_out), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(p.k.units == 0 || (grad_k != nullptr) == (grad_v != nullptr), LFFN_ERR_BAD_ARG);
+    if (!grad_q) p.q.units = 0;                            // not wanted
+    if (!grad_k) p.k.units = 0;
+    if (p.q.units == 0 && p.k.units == 0) return LFFN_OK;
     for (const void *t : {out, g_out, (const void *)grad_q, (const void *)grad_k, (const void *)grad_v}) LFFN_REQUIRE(lffn_aligned16(t), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.floats == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= p.floats * 4), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.q.units <= INT32_MAX && p.k.units <= INT32_MAX &&

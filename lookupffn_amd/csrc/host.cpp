@@ -28,6 +28,8 @@
 #include <dlfcn.h>
 
 #include <array>
+#include <cmath>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -71,7 +73,14 @@ using torch::autograd::variable_list;
     X(lffn_ln_bh4_block_wgrad_f32)          \
     X(lffn_layer_norm_bwd_f32)              \
     X(lffn_sum_partials_f32)                \
-    X(lffn_sum_many_f32)
+    X(lffn_sum_many_f32)                    \
+    X(lffn_qk_norm_rotary_fwd)              \
+    X(lffn_qk_norm_rotary_bwd)              \
+    X(lffn_qk_norm_rotary_bwd_workspace_bytes) \
+    X(lffn_cross_attention_fwd)             \
+    X(lffn_cross_attention_workspace_bytes) \
+    X(lffn_cross_attention_bwd)             \
+    X(lffn_cross_attention_bwd_workspace_bytes)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -673,9 +682,13 @@ PyObject *forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+#include "host_attention.h"
+
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
+    {"qk_norm_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk_norm_rotary)), METH_FASTCALL, nullptr},
+    {"cross_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cross_attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -1476,31 +1476,32 @@ def _(q, k, v, key_mask, scale, keep):
     return q.new_empty(q.shape), q.new_empty(q.shape[0] * q.shape[1] * q.shape[2] if keep else 0, dtype=torch.float32)
 
 
-_L.define("cross_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor? key_mask, float scale, Tensor out, Tensor lse, Tensor g) "
-          "-> (Tensor, Tensor, Tensor)")
+_L.define("cross_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor? key_mask, float scale, Tensor out, Tensor lse, Tensor g, bool of_queries, "
+          "bool of_keys) -> Tensor[]")
 
 
-def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, lse, g):
+def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, lse, g, of_queries, of_keys):
+    """-> the gradient of q if it is wanted, then those of k and v if they are."""
     _lib.require_gpu(q, k, v, key_mask, out, lse, g)
     q, k, v, key_mask, g = _head_rows(q), _head_rows(k), _head_rows(v), _neighbours_together(key_mask), _aligned(g)
     a = _cross_attention_args(q, k, v, key_mask, scale)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys))]
     with _dev_guard(q):
         lib, n = _lib.load(), ctypes.c_int64(0)
         _lib.check(lib.lffn_cross_attention_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_cross_attention_bwd_workspace_bytes")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        rc = lib.lffn_cross_attention_bwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), g.data_ptr(), *(t.data_ptr() for t in grads),
+        rc = lib.lffn_cross_attention_bwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), g.data_ptr(), *(_lib.ptr(t) for t in grads),
                                           ws.data_ptr(), n.value, _lib.stream_of(q))
     _lib.check(rc, f"lffn_cross_attention_bwd(q={tuple(q.shape)}, k={tuple(k.shape)})")
-    return tuple(grads)
+    return [t for t in grads if t is not None]
 
 
 _L.impl("cross_attention_bwd", _cross_attention_bwd_impl, "CUDA")
 
 
 @torch.library.register_fake("lookupffn::cross_attention_bwd")
-def _(q, k, v, key_mask, scale, out, lse, g):
-    return tuple(t.new_empty(t.shape) for t in (q, k, v))
+def _(q, k, v, key_mask, scale, out, lse, g, of_queries, of_keys):
+    return [t.new_empty(t.shape) for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys)) if wanted]
 
 
 fht = torch.ops.lookupffn.fht

@@ -7,6 +7,16 @@ from lookupffn_amd import qk_norm_rotary, rotary_table
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+@pytest.fixture(autouse=True, params=["host", "python"])
+def either_path(request, monkeypatch):
+    """The calls with the host path in C++ and without."""
+    if request.param == "python":
+        monkeypatch.setattr(lookupffn_amd._lib, "loaded_host", False)
+    else:
+        assert lookupffn_amd._lib.host()
+    return request.param
+
+
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
