@@ -132,7 +132,10 @@ template <typename F, int DP, int KT>
 struct Tile {
     static constexpr int PIECES = DP / 8, PLANE = KT * PIECES, SIZE = F::PLANES * PLANE;     // in 16-byte words
     static constexpr int SHARE = PLANE / WG;                                                 // pieces a thread brings
-    static __device__ __forceinline__ int turned(int row) {
+    typedef __attribute__((address_space(3))) const char *lds_bytes;
+    typedef uint32_t word_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) const word_t *lds_words;
+    static __host__ __device__ __forceinline__ constexpr int turned(int row) {
         if constexpr (DP == 32) return (row >> 2) & 3;
         else if constexpr (DP == 64) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
         else return (row & 3) << 2 | ((row >> 2) & 3);
@@ -143,32 +146,48 @@ struct Tile {
 #pragma unroll
         for (int p = 0; p < F::PLANES; ++p) lds[p * PLANE + at(row, piece)] = f.p[p];
     }
-    // operand of 32 of the tile's rows (the lane's is `row`), 16 columns `chunk`
-    static __device__ __forceinline__ Frag<F::PLANES> rows(const uint4 *lds, int row, int chunk, int half) {
-        Frag<F::PLANES> f;
-#pragma unroll
-        for (int p = 0; p < F::PLANES; ++p) f.p[p] = lds[p * PLANE + at(row, 2 * chunk + half)];
-        return f;
-    }
-    // operand of 32 of the tile's columns (32 db + lane % 32) with the sum over its rows base + 4 half + {0 .. 3, 8 .. 11}: the order in which a lane
-    // has the elements 8 c .. 8 c + 7 of a result, base = 32 x (its block of rows) + 16 c
-    static __device__ __forceinline__ Frag<F::PLANES> columns(const uint4 *lds, int base, int db, int lane) {
-        const int row = base + 4 * (lane >> 5) + ((lane & 15) >> 2), piece = 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), byte = 8 * (lane & 1);
-        Frag<F::PLANES> f;
-#pragma unroll
-        for (int p = 0; p < F::PLANES; ++p) {
-            const auto lo = transposed(lds + p * PLANE + at(row, piece), byte), hi = transposed(lds + p * PLANE + at(row + 8, piece), byte);
-            f.p[p] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        }
-        return f;
-    }
 
-private:
+    // Where a lane reads, as byte addresses in LDS: of a tile at 0, block of 32 rows (16 where the sum is over rows) 0, term 0; what
+    // else there is to a place is a constant of the instruction.
+    struct Reader {
+        uint32_t row[DP / 16], lo[DP / 32], hi[DP / 32];
+        __device__ __forceinline__ explicit Reader(const uint4 *lds, int lane) {
+            const uint32_t base = (uint32_t)(uintptr_t)(lds_bytes)lds;
+            const int r = lane & 31, half = lane >> 5;
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) row[c] = base + at(r, 2 * c + half) * 16;
+            const int first = 4 * half + ((lane & 15) >> 2), piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), byte = 8 * (lane & 1);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) {
+                lo[d] = base + at(first, 4 * d + piece) * 16 + byte;
+                hi[d] = base + at(first + 8, 4 * d + piece) * 16 + byte;
+            }
+        }
+        // operand of the 32 rows from 32 b, 16 columns `chunk`, of the tile at `tile` (in 16-byte words)
+        __device__ __forceinline__ Frag<F::PLANES> rows(int tile, int b, int chunk) const {
+            Frag<F::PLANES> f;
+#pragma unroll
+            for (int p = 0; p < F::PLANES; ++p) f.p[p] = __builtin_bit_cast(uint4, *(lds_words)(uintptr_t)(row[chunk] + (tile + p * PLANE + b * 32 * PIECES) * 16));
+            return f;
+        }
+        // operand of the tile's columns 32 d + lane % 32 with the sum over its rows 16 c + 4 half + {0 .. 3, 8 .. 11}: the order in which
+        // a lane has the elements 8 (c % 2) .. + 7 of a result of the rows from 32 (c / 2)
+        __device__ __forceinline__ Frag<F::PLANES> columns(int tile, int c, int d) const {
+            Frag<F::PLANES> f;
+#pragma unroll
+            for (int p = 0; p < F::PLANES; ++p) {
+                const uint32_t off = (tile + p * PLANE + c * 16 * PIECES) * 16;
+                const uint2 a = transposed(lo[d] + off), b = transposed(hi[d] + off);
+                f.p[p] = make_uint4(a.x, a.y, b.x, b.y);
+            }
+            return f;
+        }
+    };
+
     // Of 16 lanes' 8 bytes, lanes 4 i .. 4 i + 3 having 16 numbers of row i: lane j gets the four rows' number j.
-    static __device__ __forceinline__ uint2 transposed(const uint4 *word, int byte) {
+    static __device__ __forceinline__ uint2 transposed(uint32_t at) {
         typedef __attribute__((address_space(3))) ca_i16x4_t lds_t;
-        lds_t *const p = (lds_t *)(__attribute__((address_space(3))) char *)(reinterpret_cast<const char *>(word) + byte);
-        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t *)(uintptr_t)at));
     }
 };
 
@@ -179,14 +198,25 @@ __device__ __forceinline__ Frag<F::PLANES> own_rows(const char *row, bool live, 
     return F::operand(live && piece < pieces ? F::load(row + piece * 8 * F::BYTES) : F::zero());
 }
 
+// Division of numbers below 2^31 by one that the host knows: the compiler's division takes thirty instructions, this one three.
+struct Divisor {
+    uint32_t by, multiplier, shift;
+    Divisor() = default;
+    explicit Divisor(uint32_t d) : by(d), multiplier(0), shift(0) {
+        while ((1u << shift) < d) ++shift;
+        multiplier = uint32_t((((uint64_t(1) << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (__umulhi(n, multiplier) + n) >> shift; }
+};
+
 // Queries of the heads that share a key head are rows of one matrix: row r is token r / group, head h' * group + r % group.
 struct Rows {
     const char *base;                     // of the batch and the key head's first query head
     int64_t token, head;                  // strides in bytes
-    int group;
+    Divisor group;
     __device__ __forceinline__ const char *at(int r) const {
-        const int t = group == 1 ? r : r / group;
-        return base + t * token + (r - t * group) * head;
+        const int t = group.quotient(r);
+        return base + t * token + (r - t * group.by) * head;
     }
 };
 
@@ -210,16 +240,152 @@ __device__ __forceinline__ uint64_t uniform(uint64_t v) {
     return (uint64_t)hi << 32 | lo;
 }
 
+// 16 bytes a lane from memory straight to LDS, the wavefront's 1 KB together at lds_byte_addr.  Inline assembly, so that the compiler does not wait for the
+// copy before LDS reads of the other buffer; whoever reads waits (arrived) and has a barrier.  M0 is put back: the compiler
+// reserves it and does not honour a clobber declaration of it.
+__device__ __forceinline__ void copy_to_lds(const char *base, uint32_t lane_offset, uint32_t lds_byte_addr) {
+    uint32_t saved_m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved_m0)
+                 : "v"(lane_offset), "s"(base), "s"(lds_byte_addr)
+                 : "memory");
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Brings the rows of two arrays, tile by tile, into a buffer of two tiles: numbers of 16 bits as they are, by copies that pass no register; fp32 numbers
+// through registers, where they are split.  begin(): asked for; end(): there, after the barrier that follows.
+template <typename F, int DP, int KT>
+struct Feed {
+    typedef Tile<F, DP, KT> T;
+    static constexpr int ROWS_APART = WG / T::PIECES;         // of a thread's pieces
+    static_assert(T::turned(ROWS_APART) == 0 || T::SHARE == 1, "a thread's pieces are turned alike");
+    uint4 *lds;
+    uint32_t lds_byte;
+    int row, piece;                       // of the thread's first piece; the piece is that of memory
+    typename F::Raw raw[F::PLANES == 1 ? 1 : 2 * T::SHARE];
+
+    __device__ __forceinline__ Feed(uint4 *at, int pieces) : lds(at) {
+        const int tid = threadIdx.x;
+        row = tid / T::PIECES;
+        piece = tid % T::PIECES;
+        if constexpr (F::PLANES == 1) {
+            lds_byte = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)at + (tid >> 6) * 1024;
+            piece ^= T::turned(row);
+        }
+        column = (piece < pieces ? piece : 0) * 8 * F::BYTES;         // (what is beyond the columns meets zeros or is not stored)
+    }
+    // Piece i of a thread is at a + offset_a(row), b + offset_b(row) of tile row `row`.
+    template <typename A, typename B>
+    __device__ __forceinline__ void begin(int buf, const char *a, const char *b, A &&offset_a, B &&offset_b) {
+#pragma unroll
+        for (int i = 0; i < T::SHARE; ++i) {
+            const int r = row + i * ROWS_APART;
+            const uint32_t from_a = offset_a(r, i) + column, from_b = offset_b(r, i) + column;
+            if constexpr (F::PLANES == 1) {
+                const uint32_t to = lds_byte + (buf * 2 * T::SIZE + i * WG) * 16;
+                copy_to_lds(a, from_a, __builtin_amdgcn_readfirstlane(to));
+                copy_to_lds(b, from_b, __builtin_amdgcn_readfirstlane(to + T::SIZE * 16));
+            } else {
+                raw[2 * i] = F::load(a + from_a);
+                raw[2 * i + 1] = F::load(b + from_b);
+            }
+        }
+    }
+    __device__ __forceinline__ void end(int buf) {
+        if constexpr (F::PLANES == 1) {
+            arrived();
+        } else {
+            uint4 *const to = lds + buf * 2 * T::SIZE;
+#pragma unroll
+            for (int i = 0; i < T::SHARE; ++i) {
+                T::put(to, row + i * ROWS_APART, piece, raw[2 * i]);
+                T::put(to + T::SIZE, row + i * ROWS_APART, piece, raw[2 * i + 1]);
+            }
+        }
+    }
+
+private:
+    uint32_t column;
+};
+
+// The keys and values of a step: those that take no part are the step's first that does once more (their weights are zero, and what they hold is
+// not looked at).  Every step that is asked for has one.
+template <typename F, int DP, int KT>
+struct KeyFeed : Feed<F, DP, KT> {
+    const char *k, *v;
+    int64_t k_stride, v_stride;           // bytes; 64 of either fit in 32 bits
+    __device__ __forceinline__ KeyFeed(uint4 *at, int pieces, const char *k, const char *v, int64_t ks, int64_t vs)
+        : Feed<F, DP, KT>(at, pieces), k(k), v(v), k_stride(ks), v_stride(vs) {}
+    __device__ __forceinline__ void begin(int buf, int64_t step, uint64_t word) {
+        constexpr uint64_t FULL = ~0ull >> (64 - KT);
+        const char *const kp = k + step * KT * k_stride, *const vp = v + step * KT * v_stride;
+        const uint32_t ks = (uint32_t)k_stride, vs = (uint32_t)v_stride;
+        if (word == FULL) {
+            Feed<F, DP, KT>::begin(buf, kp, vp, [&](int r, int) { return r * ks; }, [&](int r, int) { return r * vs; });
+        } else {
+            const int first = __builtin_ctzll(word);
+            auto of = [&](int r) { return (uint32_t)(word >> r & 1 ? r : first); };
+            Feed<F, DP, KT>::begin(buf, kp, vp, [&](int r, int) { return of(r) * ks; }, [&](int r, int) { return of(r) * vs; });
+        }
+    }
+};
+
+// Walks the steps of [begin, end) that have a key that takes part: compute(buffer, word) with the buffer as a constant, once behind each begin and end of the feed.
+template <int KT, typename KF, typename C>
+__device__ __forceinline__ void walk_keys(KF &feed, uint64_t *words, const uint8_t *mask, int64_t begin, int64_t end, int64_t keys, C &&compute) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int64_t first = begin; first < end; first += BLOCK) {
+        look_at_masks<KT>(words, mask, first, end, keys);
+        __syncthreads();
+        uint64_t left = __ballot(words[lane] != 0);
+        if (left) {
+            uint64_t word, next = 0;
+            auto ask = [&](int buf) {                    // for the next step, if there is one
+                if (!left) return false;
+                const int i = __builtin_ctzll(left);
+                left &= left - 1;
+                next = uniform(words[i]);
+                feed.begin(buf, first + i, next);
+                return true;
+            };
+            ask(0);
+            feed.end(0);
+            __syncthreads();
+#pragma unroll 1
+            for (;;) {
+                word = next;
+                bool more = ask(1);
+                compute(std::integral_constant<int, 0>{}, word);
+                if (!more) break;
+                feed.end(1);
+                __syncthreads();
+                word = next;
+                more = ask(0);
+                compute(std::integral_constant<int, 1>{}, word);
+                if (!more) break;
+                feed.end(0);
+                __syncthreads();
+            }
+        }
+        __syncthreads();                  // the words and the buffers are free again
+    }
+}
+
 // Where row `row` (of the queries that share key head kh, or with group 1 of the keys) of a batch is in [B, len, heads, columns]: its number of heads' rows.
-__device__ __forceinline__ int64_t heads_row(int64_t b, int64_t kh, int row, int64_t len, int key_heads, int group) {
-    const int token = group == 1 ? row : row / group;
-    return ((b * len + token) * key_heads + kh) * group + (row - token * group);
+__device__ __forceinline__ int64_t heads_row(int b, int kh, int row, int64_t len, int key_heads, const Divisor &group) {
+    const int token = group.quotient(row);
+    return ((b * len + token) * key_heads + kh) * group.by + (row - token * group.by);
 }
 
 // Which unit of work a workgroup has: neighbours (tiles that read the same keys) on one XCD.
-__device__ __forceinline__ int64_t unit_of(int64_t block, int64_t blocks) {
-    const int64_t xcd = block & 7, per = blocks >> 3, rem = blocks & 7;
-    return xcd * per + (xcd < rem ? xcd : rem) + (block >> 3);
+struct Unit {
+    int tile, split, bh, b, kh;
+};
+__device__ __forceinline__ Unit unit_of(uint32_t block, uint32_t blocks, const Divisor &tiles, const Divisor &splits, const Divisor &key_heads) {
+    const uint32_t xcd = block & 7, per = blocks >> 3, rem = blocks & 7, unit = xcd * per + (xcd < rem ? xcd : rem) + (block >> 3);
+    const uint32_t pair = tiles.quotient(unit), bh = splits.quotient(pair), b = key_heads.quotient(bh);
+    return {int(unit - pair * tiles.by), int(pair - bh * splits.by), int(bh), int(b), int(bh - b * key_heads.by)};
 }
 
 }  // namespace cross_attention

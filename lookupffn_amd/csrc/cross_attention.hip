@@ -17,9 +17,9 @@ struct FwdArgs {
     char *out;
     float *lse, *part, *part_lse;         // parts: [splits, B, key heads, rows(, columns)]
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, mask_stride;         // strides in bytes
-    int64_t keys, steps, split_steps;
-    int key_heads, group, rows, row_tiles, splits, columns;
-    int64_t q_len, units;
+    int64_t keys, steps, split_steps, q_len;
+    Divisor group, tiles, split_by, heads;               // query heads of a key head, tiles of rows, shares of the keys, key heads
+    int key_heads, rows, row_tiles, splits, columns, units;
     float c;                              // scale log2 e
 };
 
@@ -33,36 +33,16 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     extern __shared__ __attribute__((aligned(16))) uint4 lds[];           // [2][keys, values], words
     uint64_t *const words = reinterpret_cast<uint64_t *>(lds + 4 * T::SIZE);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, half = lane >> 5;
-    const int64_t unit = unit_of(blockIdx.x, a.units);
-    const int tile = unit % a.row_tiles, split = unit / a.row_tiles % a.splits;
-    const int64_t bh = unit / a.row_tiles / a.splits, b = bh / a.key_heads, kh = bh - b * a.key_heads;
+    const Unit unit = unit_of(blockIdx.x, a.units, a.tiles, a.split_by, a.heads);
+    const int tile = unit.tile, split = unit.split, bh = unit.bh, b = unit.b, kh = unit.kh;
     const int pieces = a.columns / 8;
-    const Rows rows{a.q + b * a.qb + kh * a.group * a.qh, a.qt, a.qh, a.group};
+    const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
     const char *const kp = a.k + b * a.kb + kh * a.kh, *const vp = a.v + b * a.vb + kh * a.vh;
     const uint8_t *const mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
     const int row = tile * TILE + wave * ROWS + r;
 
-    typename F::Raw rk[T::SHARE], rv[T::SHARE];
-    auto fetch = [&](int64_t step, uint64_t word) {
-#pragma unroll
-        for (int i = 0; i < T::SHARE; ++i) {
-            const int p = tid + WG * i, key = p / T::PIECES, piece = p % T::PIECES;
-            const bool live = (word >> key & 1) && piece < pieces;
-            const int64_t at = step * KT + key;
-            rk[i] = live ? F::load(kp + at * a.kt + piece * 8 * F::BYTES) : F::zero();
-            rv[i] = live ? F::load(vp + at * a.vt + piece * 8 * F::BYTES) : F::zero();
-        }
-    };
-    auto place = [&](int buf) {
-        uint4 *const to = lds + buf * 2 * T::SIZE;
-#pragma unroll
-        for (int i = 0; i < T::SHARE; ++i) {
-            const int p = tid + WG * i, key = p / T::PIECES, piece = p % T::PIECES;
-            T::put(to, key, piece, rk[i]);
-            T::put(to + T::SIZE, key, piece, rv[i]);
-        }
-    };
-
+    KeyFeed<F, DP, KT> feed(lds, pieces, kp, vp, a.kt, a.vt);
+    const typename T::Reader read(lds, lane);
     Op fq[CHUNKS];
     {
         const bool live = row < a.rows;
@@ -73,14 +53,14 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     ca_f32x16_t o[DB] = {};
     float most = -INFINITY, sum = 0.f;
 
-    auto compute = [&](int buf, uint64_t word) {
-        const uint4 *const keys = lds + buf * 2 * T::SIZE, *const values = keys + T::SIZE;
+    auto compute = [&](auto buf, uint64_t word) {
+        constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
         ca_f32x16_t s[KB] = {};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) s[kb] = F::mma(T::rows(keys, kb * 32 + r, c, half), fq[c], s[kb]);
-        constexpr uint64_t FULL = KT == 64 ? ~0ull : (1ull << KT) - 1;
+            for (int c = 0; c < CHUNKS; ++c) s[kb] = F::mma(read.rows(KEYS, kb, c), fq[c], s[kb]);
+        constexpr uint64_t FULL = ~0ull >> (64 - KT);
         if (word != FULL) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -120,53 +100,21 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
                 for (int e = 0; e < 8; ++e) t[e] = s[kb][8 * c + e];
                 const Op p = F::operand(t);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = F::mma(T::columns(values, kb * 32 + c * 16, d, lane), p, o[d]);
+                for (int d = 0; d < DB; ++d) o[d] = F::mma(read.columns(VALUES, 2 * kb + c, d), p, o[d]);
             }
         }
     };
 
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
-#pragma unroll 1
-    for (int64_t first = begin; first < end; first += BLOCK) {
-        look_at_masks<KT>(words, mask, first, end, a.keys);
-        __syncthreads();
-        const uint64_t mine = words[lane];
-        uint64_t left = __ballot(mine != 0);
-        if (left) {
-            int i = __builtin_ctzll(left), buf = 0;
-            uint64_t word = uniform(words[i]);
-            left &= left - 1;
-            fetch(first + i, word);
-            place(0);
-            __syncthreads();
-#pragma unroll 1
-            for (;;) {
-                const bool more = left != 0;
-                uint64_t next = 0;
-                if (more) {
-                    i = __builtin_ctzll(left);
-                    left &= left - 1;
-                    next = uniform(words[i]);
-                    fetch(first + i, next);
-                }
-                compute(buf, word);
-                if (!more) break;
-                place(buf ^ 1);
-                __syncthreads();
-                buf ^= 1;
-                word = next;
-            }
-        }
-        __syncthreads();                  // the words and the buffers are free again
-    }
+    walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
 
     sum += lane_xor<32>(sum);
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query without keys: zeros
     if (row >= a.rows) return;
     const float level = sum == 0.f ? INFINITY : (most == -INFINITY ? 0.f : most) * a.c - F::LIFT + __builtin_amdgcn_logf(sum);
-    const int64_t at = bh * a.rows + row;
+    const int64_t at = int64_t(bh) * a.rows + row;
     if (a.splits > 1) {
-        const int64_t of = int64_t(split) * (a.units / a.splits / a.row_tiles) * a.rows + at;
+        const int64_t of = int64_t(split) * (a.units / (a.splits * a.row_tiles)) * a.rows + at;
         if (half == 0) a.part_lse[of] = level;
         float *const p = a.part + of * a.columns;
 #pragma unroll
@@ -215,8 +163,7 @@ __global__ __launch_bounds__(WG) void join_kernel(FwdArgs a, int64_t all_rows) {
         acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
     }
     const float by = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t bh = at / a.rows, b = bh / a.key_heads, kh = bh - b * a.key_heads;
-    const int row = int(at - bh * a.rows);
+    const int bh = int(at / a.rows), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, row = int(at - int64_t(bh) * a.rows);
     if (a.lse && col == 0) a.lse[at] = sum == 0.f ? INFINITY : most + __builtin_amdgcn_logf(sum);
     char *const p = a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
     F::store4(p + col * F::BYTES, acc.x * by, acc.y * by, acc.z * by, acc.w * by);
@@ -234,6 +181,10 @@ __attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(co
     for (int d = 0; d < 3; ++d)
         for (const int64_t s : {a->q_strides[d], a->k_strides[d], a->v_strides[d]})
             LFFN_REQUIRE(s >= 0 && s * size % 16 == 0, LFFN_ERR_BAD_ARG);
+    // (the kernels address a tile's rows by 32 bits)
+    const int64_t far = int64_t(1) << 32;
+    LFFN_REQUIRE(a->k_strides[1] * size < far / 64 && a->v_strides[1] * size < far / 64 && a->q_strides[1] * size < far / 128 &&
+                     a->q_strides[2] * size < far / 4 / (a->heads / a->key_heads > 0 ? a->heads / a->key_heads : 1), LFFN_ERR_UNSUPPORTED);
     const bool no_rows = a->B == 0 || a->q_len == 0 || a->heads == 0, no_keys = a->B == 0 || a->k_len == 0;
     LFFN_REQUIRE((a->q || no_rows) && ((a->k && a->v) || no_keys) && a->mask_stride >= 0, LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(lffn_aligned16(a->q) && lffn_aligned16(a->k) && lffn_aligned16(a->v), LFFN_ERR_BAD_ARG);
@@ -249,7 +200,7 @@ namespace {
 constexpr int64_t WANTED = 512;           // workgroups, where there are keys enough to share out
 constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
 
-// Fills sizes in; the workspace's bytes.
+// Fills sizes in; the workspace's bytes, or -1: too many tiles.
 int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     const int64_t size = c.format == LFFN_ROWS_F32 ? 4 : 2;
     const int kt = c.format == LFFN_ROWS_F32 && c.columns > 64 ? 32 : 64;
@@ -259,8 +210,9 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     a.kb = c.k_strides[0] * size, a.kt = c.k_strides[1] * size, a.kh = c.k_strides[2] * size;
     a.vb = c.v_strides[0] * size, a.vt = c.v_strides[1] * size, a.vh = c.v_strides[2] * size;
     a.keys = c.k_len, a.q_len = c.q_len;
-    a.key_heads = (int)c.key_heads, a.group = int(c.heads / c.key_heads), a.columns = (int)c.columns;
-    a.rows = int(c.q_len * a.group);
+    const int64_t group = c.heads / c.key_heads;
+    a.key_heads = (int)c.key_heads, a.columns = (int)c.columns;
+    a.rows = int(c.q_len * group);
     a.row_tiles = (a.rows + TILE - 1) / TILE;
     a.steps = (c.k_len + kt - 1) / kt;
     a.c = c.scale * LOG2E;
@@ -270,8 +222,11 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     if (splits < 1) splits = 1;
     a.split_steps = (a.steps + splits - 1) / splits;
     a.splits = a.split_steps ? int((a.steps + a.split_steps - 1) / a.split_steps) : 1;
-    a.units = tiles * a.splits;
-    return a.splits > 1 ? a.splits * c.B * c.key_heads * a.rows * (a.columns + 1) * 4 : 0;
+    a.group = Divisor(group > 0 ? (uint32_t)group : 1), a.heads = Divisor((uint32_t)a.key_heads);
+    a.tiles = Divisor(a.row_tiles > 0 ? (uint32_t)a.row_tiles : 1), a.split_by = Divisor((uint32_t)a.splits);
+    if (tiles > INT32_MAX / a.splits) return -1;
+    a.units = int(tiles * a.splits);
+    return a.splits > 1 ? int64_t(a.splits) * c.B * c.key_heads * a.rows * (a.columns + 1) * 4 : 0;
 }
 
 template <typename F, int DP, int KT>
@@ -281,7 +236,7 @@ int launch(const FwdArgs &a, hipStream_t stream) {
     if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&cross_attention_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
     cross_attention_kernel<F, DP, KT><<<dim3((unsigned)a.units), dim3(WG), bytes, stream>>>(a);
     if (a.splits > 1) {
-        const int64_t rows = a.units / a.splits / a.row_tiles * a.rows;
+        const int64_t rows = int64_t(a.units / (a.splits * a.row_tiles)) * a.rows;
         join_kernel<F><<<dim3((unsigned)((rows * (a.columns / 4) + WG - 1) / WG)), dim3(WG), 0, stream>>>(a, rows);
     }
     return lffn_launch_status();
@@ -301,6 +256,7 @@ extern "C" int lffn_cross_attention_workspace_bytes(const lffn_cross_attention *
     if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
     FwdArgs a{};
     *bytes = plan(*c, a);
+    LFFN_REQUIRE(*bytes >= 0, LFFN_ERR_UNSUPPORTED);
     return LFFN_OK;
 }
 
@@ -309,10 +265,10 @@ extern "C" int lffn_cross_attention_fwd(const lffn_cross_attention *c, void *out
     if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
     FwdArgs a{};
     const int64_t bytes = plan(*c, a);
+    LFFN_REQUIRE(bytes >= 0, LFFN_ERR_UNSUPPORTED);
     if (a.units == 0) return LFFN_OK;
     LFFN_REQUIRE(out && lffn_aligned16(out), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(bytes == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= bytes), LFFN_ERR_BAD_ARG);
-    LFFN_REQUIRE(a.units <= INT32_MAX, LFFN_ERR_UNSUPPORTED);
     a.out = static_cast<char *>(out), a.lse = lse;
     a.part = static_cast<float *>(workspace);
     a.part_lse = a.part ? a.part + int64_t(a.splits) * c->B * c->key_heads * a.rows * a.columns : nullptr;

@@ -17,7 +17,7 @@ __attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(co
 
 namespace {
 
-constexpr int NORM_ROWS = 1024;           // rows whose longest is looked for by one workgroup
+constexpr int NORM_ROWS = 128;            // rows of a workgroup of delta_kernel, 8 to a group of 16 lanes, asked for together
 constexpr float P_LIFT = 14.f;            // half precision
 
 struct BwdArgs {
@@ -28,8 +28,10 @@ struct BwdArgs {
     float *delta, *g_norms, *v_norms;     // [B, key heads, rows]; squares of the longest rows: [B, key heads, tiles]
     float *part;                          // [splits, B, key heads, rows or keys, columns] (keys: of k, then of v)
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, mask_stride;         // strides in bytes
-    int64_t keys, steps, split_steps, q_len, units;
-    int batch_heads, key_heads, group, rows, tiles, splits, columns, g_tiles, v_tiles;
+    int64_t keys, steps, split_steps, q_len;
+    Divisor group, tile_by, split_by, heads, norm_tiles; // query heads of a key head, standing tiles, shares of what passes, key heads, delta_kernel's tiles
+    int64_t units;
+    int batch_heads, key_heads, rows, tiles, splits, columns, g_tiles, v_tiles;
     float c, scale;
 };
 
@@ -43,40 +45,56 @@ __device__ __forceinline__ float wave_most(float v) {
     return fmaxf(v, lane_xor<32>(v));
 }
 
-// delta of every row; half precision: the longest rows of g and v as well.  16 lanes a row, 8 columns a lane.
+// delta of every row; half precision: the longest rows of g and v as well.  16 lanes a row, 8 columns a lane.  Bound by memory: out and g (and v) once.
+// (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16 65 us.)
 template <typename F, bool NORMS>
 __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
-    const int lane = threadIdx.x & 15, col = lane * 8, tiles = a.g_tiles + a.v_tiles;
-    const int64_t bh = blockIdx.x / tiles, b = bh / a.key_heads, kh = bh - b * a.key_heads;
-    const int tile = int(blockIdx.x - bh * tiles);
+    constexpr int EACH = NORM_ROWS / (WG / 16);
+    const int lane = threadIdx.x & 15, tiles = a.g_tiles + a.v_tiles;
+    const bool on = lane * 8 < a.columns;
+    const int col = on ? lane * 8 : 0;
+    const int bh = a.norm_tiles.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * tiles;
     float most = 0.f;
     if (tile < a.g_tiles) {
-        for (int row = tile * NORM_ROWS + threadIdx.x / 16; row < min(a.rows, (tile + 1) * NORM_ROWS); row += WG / 16) {
-            float dot = 0.f, squares = 0.f;
-            if (col < a.columns) {
-                const int64_t at = (heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES;
-                float o[8], g[8];
-                F::unpack(F::load(a.out + at), o);
-                F::unpack(F::load(a.g + at), g);
+        typename F::Raw o[EACH], g[EACH];
+        const int first = tile * NORM_ROWS + threadIdx.x / 16;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dot = fmaf(o[i], g[i], dot), squares = fmaf(g[i], g[i], squares);
-            }
-            dot = lane_group_sum<16>(dot);
-            if (NORMS) most = fmaxf(most, lane_group_sum<16>(squares));
-            if (lane == 0) a.delta[bh * a.rows + row] = dot;
+        for (int i = 0; i < EACH; ++i) {
+            const int row = min(first + i * (WG / 16), a.rows - 1);
+            const int64_t at = (heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES;
+            o[i] = F::load(a.out + at);
+            g[i] = F::load(a.g + at);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            float dot = 0.f, squares = 0.f, u[8], v[8];
+            F::unpack(o[i], u);
+            F::unpack(g[i], v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot), squares = fmaf(v[e], v[e], squares);
+            dot = lane_group_sum<16>(on ? dot : 0.f);
+            if (NORMS) most = fmaxf(most, lane_group_sum<16>(on ? squares : 0.f));
+            const int row = first + i * (WG / 16);
+            if (lane == 0 && row < a.rows) a.delta[int64_t(bh) * a.rows + row] = dot;
         }
     } else if (NORMS) {
-        const int64_t begin = int64_t(tile - a.g_tiles) * NORM_ROWS, end = begin + NORM_ROWS < a.keys ? begin + NORM_ROWS : a.keys;
-        for (int64_t key = begin + threadIdx.x / 16; key < end; key += WG / 16) {
-            if (a.mask && a.mask[b * a.mask_stride + key] == 0) continue;        // (the 16 lanes alike)
-            float squares = 0.f;
-            if (col < a.columns) {
-                float v[8];
-                F::unpack(F::load(a.v + b * a.vb + kh * a.vh + key * a.vt + col * F::BYTES), v);
+        typename F::Raw x[EACH];
+        bool live[EACH];
+        const int64_t first = int64_t(tile - a.g_tiles) * NORM_ROWS + threadIdx.x / 16;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) squares = fmaf(v[i], v[i], squares);
-            }
-            most = fmaxf(most, lane_group_sum<16>(squares));
+        for (int i = 0; i < EACH; ++i) {
+            const int64_t key = first + i * (WG / 16), at = key < a.keys ? key : a.keys - 1;
+            live[i] = !a.mask || a.mask[b * a.mask_stride + at] != 0;
+            x[i] = F::load(a.v + b * a.vb + kh * a.vh + at * a.vt + col * F::BYTES);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            float squares = 0.f, v[8];
+            F::unpack(x[i], v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) squares = fmaf(v[e], v[e], squares);
+            squares = lane_group_sum<16>(on ? squares : 0.f);
+            if (live[i]) most = fmaxf(most, squares);
         }
     }
     if (NORMS) {
@@ -86,8 +104,8 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
         __syncthreads();
         if (threadIdx.x == 0) {
             most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-            if (tile < a.g_tiles) a.g_norms[bh * a.g_tiles + tile] = most;
-            else a.v_norms[bh * a.v_tiles + tile - a.g_tiles] = most;
+            if (tile < a.g_tiles) a.g_norms[int64_t(bh) * a.g_tiles + tile] = most;
+            else a.v_norms[int64_t(bh) * a.v_tiles + tile - a.g_tiles] = most;
         }
     }
 }
@@ -120,47 +138,27 @@ __device__ __forceinline__ void store_sums(const ca_f32x16_t (&o)[DB], float by,
 }
 
 template <typename F, int DP, int KT>
-__global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void query_gradient_kernel(BwdArgs a) {
+__global__ __launch_bounds__(WG, F::PLANES == 1 ? 2 : 1) void query_gradient_kernel(BwdArgs a) {
     typedef Tile<F, DP, KT> T;
     typedef Frag<F::PLANES> Op;
     constexpr int CHUNKS = DP / 16, KB = KT / 32, DB = DP / 32;
     extern __shared__ __attribute__((aligned(16))) uint4 lds[];           // [2][keys, values], words
     uint64_t *const words = reinterpret_cast<uint64_t *>(lds + 4 * T::SIZE);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, half = lane >> 5;
-    const int64_t unit = unit_of(blockIdx.x, a.units);
-    const int tile = unit % a.tiles, split = unit / a.tiles % a.splits;
-    const int64_t bh = unit / a.tiles / a.splits, b = bh / a.key_heads, kh = bh - b * a.key_heads;
+    const Unit unit = unit_of(blockIdx.x, a.units, a.tile_by, a.split_by, a.heads);
+    const int tile = unit.tile, split = unit.split, bh = unit.bh, b = unit.b, kh = unit.kh;
     const int pieces = a.columns / 8;
     const char *const kp = a.k + b * a.kb + kh * a.kh, *const vp = a.v + b * a.vb + kh * a.vh;
     const uint8_t *const mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
     const int row = tile * TILE + wave * ROWS + r;
     const bool live = row < a.rows;
 
-    typename F::Raw rk[T::SHARE], rv[T::SHARE];
-    auto fetch = [&](int64_t step, uint64_t word) {
-#pragma unroll
-        for (int i = 0; i < T::SHARE; ++i) {
-            const int p = tid + WG * i, key = p / T::PIECES, piece = p % T::PIECES;
-            const bool in = (word >> key & 1) && piece < pieces;
-            const int64_t at = step * KT + key;
-            rk[i] = in ? F::load(kp + at * a.kt + piece * 8 * F::BYTES) : F::zero();
-            rv[i] = in ? F::load(vp + at * a.vt + piece * 8 * F::BYTES) : F::zero();
-        }
-    };
-    auto place = [&](int buf) {
-        uint4 *const to = lds + buf * 2 * T::SIZE;
-#pragma unroll
-        for (int i = 0; i < T::SHARE; ++i) {
-            const int p = tid + WG * i, key = p / T::PIECES, piece = p % T::PIECES;
-            T::put(to, key, piece, rk[i]);
-            T::put(to + T::SIZE, key, piece, rv[i]);
-        }
-    };
-
+    KeyFeed<F, DP, KT> feed(lds, pieces, kp, vp, a.kt, a.vt);
+    const typename T::Reader read(lds, lane);
     const int64_t out_row = heads_row(b, kh, live ? row : 0, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
     Op fq[CHUNKS], fg[CHUNKS];
     {
-        const char *const p = Rows{a.q + b * a.qb + kh * a.group * a.qh, a.qt, a.qh, a.group}.at(live ? row : 0);
+        const char *const p = Rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group}.at(live ? row : 0);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             fq[c] = own_rows<F>(p, live, c, half, pieces);
@@ -169,18 +167,18 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void query_
     }
     const int lift = ds_exponent<F>(a, bh);
     const float f = __builtin_amdgcn_ldexpf(1.f, lift);
-    const float level = live ? a.lse[bh * a.rows + row] : INFINITY, delta = live ? a.delta[bh * a.rows + row] * f : 0.f;
+    const float level = live ? a.lse[int64_t(bh) * a.rows + row] : INFINITY, delta = live ? a.delta[int64_t(bh) * a.rows + row] * f : 0.f;
     ca_f32x16_t dq[DB] = {};
 
-    auto compute = [&](int buf, uint64_t word) {
-        const uint4 *const keys = lds + buf * 2 * T::SIZE, *const values = keys + T::SIZE;
+    auto compute = [&](auto buf, uint64_t word) {
+        constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             ca_f32x16_t s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
-                s = F::mma(T::rows(keys, kb * 32 + r, c, half), fq[c], s);
-                dp = F::mma(T::rows(values, kb * 32 + r, c, half), fg[c], dp);
+                s = F::mma(read.rows(KEYS, kb, c), fq[c], s);
+                dp = F::mma(read.rows(VALUES, kb, c), fg[c], dp);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -level)) * fmaf(dp[e], f, -delta);
@@ -198,46 +196,15 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void query_
                 for (int e = 0; e < 8; ++e) t[e] = s[8 * c + e];
                 const Op ds = F::operand(t);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) dq[d] = F::mma(T::columns(keys, kb * 32 + c * 16, d, lane), ds, dq[d]);
+                for (int d = 0; d < DB; ++d) dq[d] = F::mma(read.columns(KEYS, 2 * kb + c, d), ds, dq[d]);
             }
         }
     };
 
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
-#pragma unroll 1
-    for (int64_t first = begin; first < end; first += BLOCK) {
-        look_at_masks<KT>(words, mask, first, end, a.keys);
-        __syncthreads();
-        uint64_t left = __ballot(words[lane] != 0);
-        if (left) {
-            int i = __builtin_ctzll(left), buf = 0;
-            uint64_t word = uniform(words[i]);
-            left &= left - 1;
-            fetch(first + i, word);
-            place(0);
-            __syncthreads();
-#pragma unroll 1
-            for (;;) {
-                const bool more = left != 0;
-                uint64_t next = 0;
-                if (more) {
-                    i = __builtin_ctzll(left);
-                    left &= left - 1;
-                    next = uniform(words[i]);
-                    fetch(first + i, next);
-                }
-                compute(buf, word);
-                if (!more) break;
-                place(buf ^ 1);
-                __syncthreads();
-                buf ^= 1;
-                word = next;
-            }
-        }
-        __syncthreads();                  // the words and the buffers are free again
-    }
+    walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
     if (!live) return;
-    float *const part = a.splits > 1 ? a.part + (int64_t(split) * a.batch_heads * a.rows + bh * a.rows + row) * a.columns : nullptr;
+    float *const part = a.splits > 1 ? a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns : nullptr;
     store_sums<F, DB>(dq, __builtin_amdgcn_ldexpf(a.scale, -lift), a.gq + out_row, part, a.columns, half);
 }
 
@@ -249,71 +216,77 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void key_gr
     extern __shared__ __attribute__((aligned(16))) uint4 lds[];           // [2][rows, their gradients], [2][levels, deltas]
     float *const levels = reinterpret_cast<float *>(lds + 4 * T::SIZE);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, half = lane >> 5;
-    const int64_t unit = unit_of(blockIdx.x, a.units);
-    const int tile = unit % a.tiles, split = unit / a.tiles % a.splits;
-    const int64_t bh = unit / a.tiles / a.splits, b = bh / a.key_heads, kh = bh - b * a.key_heads;
+    const Unit unit = unit_of(blockIdx.x, a.units, a.tile_by, a.split_by, a.heads);
+    const int tile = unit.tile, split = unit.split, bh = unit.bh, b = unit.b, kh = unit.kh;
     const int pieces = a.columns / 8;
     const int64_t key = int64_t(tile) * TILE + wave * ROWS + r;
-    const bool in = key < a.keys, live = in && (!a.mask || a.mask[b * a.mask_stride + key] != 0);
-    const Rows rows{a.q + b * a.qb + kh * a.group * a.qh, a.qt, a.qh, a.group};
+    const bool in = key < a.keys;
+    const int64_t at_key = in ? key : a.keys - 1;
+    const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
+    const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
 
-    Op fk[CHUNKS], fv[CHUNKS];
-    {
-        const int64_t at = live ? key : 0;
-        const char *const kp = a.k + b * a.kb + kh * a.kh + at * a.kt, *const vp = a.v + b * a.vb + kh * a.vh + at * a.vt;
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            fk[c] = own_rows<F>(kp, live, c, half, pieces);
-            fv[c] = own_rows<F>(vp, live, c, half, pieces);
-        }
-    }
-    const bool wave_works = __any(live), works = __syncthreads_or(live);
+    // (a masked key is read as any other: what it holds stays in its own column, which is not stored)
+    const uint8_t flag = a.mask ? a.mask[b * a.mask_stride + at_key] : 1;
     constexpr bool HALF = F::LIFT != 0.f;
     const int lift = ds_exponent<F>(a, bh);
     const float f = __builtin_amdgcn_ldexpf(1.f, HALF ? lift - int(P_LIFT) : 0);
+    Op fk[CHUNKS], fv[CHUNKS];
+    {
+        const char *const kp = a.k + b * a.kb + kh * a.kh + at_key * a.kt, *const vp = a.v + b * a.vb + kh * a.vh + at_key * a.vt;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            fk[c] = own_rows<F>(kp, true, c, half, pieces);
+            fv[c] = own_rows<F>(vp, true, c, half, pieces);
+        }
+    }
 
-    typename F::Raw rq[T::SHARE], rg[T::SHARE];
+    // Rows beyond the last are the last once more: their levels are infinite and so their weights zero.  A step's addresses go by its first token; where
+    // the heads that share a key divide KT they are the same for every step.
+    Feed<F, DP, KT> feed(lds, pieces);
+    const typename T::Reader read(lds, lane);
+    const bool even = KT % a.group.by == 0;
+    const int64_t g_token = int64_t(a.key_heads) * a.group.by * a.columns * F::BYTES;
+    const char *const gp = a.g + (b * a.q_len * g_token + kh * a.group.by * a.columns * F::BYTES);
+    uint32_t q_offset[T::SHARE], g_offset[T::SHARE];
     float level = 0.f, delta = 0.f;
-    auto fetch = [&](int64_t step) {
+    auto ask = [&](int buf, int64_t step) {
+        const int first = int(step) * KT, token = a.group.quotient(first);
+        if (step == begin || !even || first + KT > a.rows) {
 #pragma unroll
-        for (int i = 0; i < T::SHARE; ++i) {
-            const int p = tid + WG * i, piece = p % T::PIECES, row = int(step) * KT + p / T::PIECES;
-            const bool on = row < a.rows && piece < pieces;
-            rq[i] = on ? F::load(rows.at(row) + piece * 8 * F::BYTES) : F::zero();
-            rg[i] = on ? F::load(a.g + (heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns + piece * 8) * F::BYTES) : F::zero();
+            for (int i = 0; i < T::SHARE; ++i) {
+                const int row = min(first + feed.row + i * feed.ROWS_APART, a.rows - 1), t = a.group.quotient(row), h = row - t * a.group.by;
+                q_offset[i] = (t - token) * (uint32_t)a.qt + h * (uint32_t)a.qh;
+                g_offset[i] = (t - token) * (uint32_t)g_token + h * (uint32_t)(a.columns * F::BYTES);
+            }
         }
-        if (tid < KT) {
-            const int row = int(step) * KT + tid;
-            level = row < a.rows ? a.lse[bh * a.rows + row] - (HALF ? P_LIFT : 0.f) : INFINITY;
-            delta = row < a.rows ? a.delta[bh * a.rows + row] * f : 0.f;
-        }
+        feed.begin(buf, rows.base + token * a.qt, gp + token * g_token, [&](int, int i) { return q_offset[i]; }, [&](int, int i) { return g_offset[i]; });
+        // (nothing is made of the numbers here: that would wait for them, and for the copies)
+        const int64_t of_row = int64_t(bh) * a.rows + min(first + tid % KT, a.rows - 1);
+        level = a.lse[of_row];
+        delta = a.delta[of_row];
     };
-    auto place = [&](int buf) {
-        uint4 *const to = lds + buf * 2 * T::SIZE;
-#pragma unroll
-        for (int i = 0; i < T::SHARE; ++i) {
-            const int p = tid + WG * i, row = p / T::PIECES, piece = p % T::PIECES;
-            T::put(to, row, piece, rq[i]);
-            T::put(to + T::SIZE, row, piece, rg[i]);
-        }
+    auto placed = [&](int buf, int64_t step) {
         if (tid < KT) {
-            levels[buf * 2 * KT + tid] = level;
-            levels[buf * 2 * KT + KT + tid] = delta;
+            const bool on = int(step) * KT + tid < a.rows;
+            levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
+            levels[buf * 2 * KT + KT + tid] = on ? delta * f : 0.f;
         }
+        feed.end(buf);
     };
 
     ca_f32x16_t dk[DB] = {}, dv[DB] = {};
-    auto compute = [&](int buf) {
-        const uint4 *const queries = lds + buf * 2 * T::SIZE, *const gradients = queries + T::SIZE;
-        const float *const level = levels + buf * 2 * KT + 4 * half, *const delta = level + KT;
+    auto compute = [&](auto buf) {
+        constexpr int QUERIES = decltype(buf)::value * 2 * T::SIZE, GRADIENTS = QUERIES + T::SIZE;
+        const float *const level = levels + decltype(buf)::value * 2 * KT + 4 * half, *const delta = level + KT;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             ca_f32x16_t s = {}, dp = {};
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                s = F::mma(T::rows(queries, rb * 32 + r, c, half), fk[c], s);
-                dp = F::mma(T::rows(gradients, rb * 32 + r, c, half), fv[c], dp);
-            }
+            for (int c = 0; c < CHUNKS; ++c) s = F::mma(read.rows(QUERIES, rb, c), fk[c], s);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) dp = F::mma(read.rows(GRADIENTS, rb, c), fv[c], dp);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const float4 l = *reinterpret_cast<const float4 *>(level + rb * 32 + 8 * g), d = *reinterpret_cast<const float4 *>(delta + rb * 32 + 8 * g);
@@ -325,36 +298,47 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void key_gr
                     dp[4 * g + e] = p * fmaf(dp[4 * g + e], f, -ds[e]);
                 }
             }
+            Op p[2], ds[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float t[8], u[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = s[8 * c + e], u[e] = dp[8 * c + e];
-                const Op p = F::operand(t), ds = F::operand(u);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    dv[d] = F::mma(T::columns(gradients, rb * 32 + c * 16, d, lane), p, dv[d]);
-                    dk[d] = F::mma(T::columns(queries, rb * 32 + c * 16, d, lane), ds, dk[d]);
-                }
+                p[c] = F::operand(t), ds[c] = F::operand(u);
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) dv[d] = F::mma(read.columns(GRADIENTS, 2 * rb + c, d), p[c], dv[d]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) dk[d] = F::mma(read.columns(QUERIES, 2 * rb + c, d), ds[c], dk[d]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
+    if (begin < end) ask(0, begin);
+    const bool live = in && flag != 0, wave_works = __any(live), works = __syncthreads_or(live);
+    if (begin < end) placed(0, begin);
     if (works && begin < end) {
-        int buf = 0;
-        fetch(begin);
-        place(0);
         __syncthreads();
 #pragma unroll 1
         for (int64_t step = begin;;) {
-            const bool more = ++step < end;
-            if (more) fetch(step);
-            if (wave_works) compute(buf);
+            bool more = ++step < end;
+            if (more) ask(1, step);
+            if (wave_works) compute(std::integral_constant<int, 0>{});
             if (!more) break;
-            place(buf ^ 1);
+            placed(1, step);
             __syncthreads();
-            buf ^= 1;
+            more = ++step < end;
+            if (more) ask(0, step);
+            if (wave_works) compute(std::integral_constant<int, 1>{});
+            if (!more) break;
+            placed(0, step);
+            __syncthreads();
         }
     }
     if (!in) return;
@@ -362,7 +346,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void key_gr
 #pragma unroll
         for (int d = 0; d < DB; ++d) dk[d] = ca_f32x16_t{}, dv[d] = ca_f32x16_t{};
     }
-    const int64_t at = heads_row(b, kh, int(key), a.keys, a.key_heads, 1) * a.columns * F::BYTES, all = int64_t(a.batch_heads) * a.keys;
+    const int64_t at = ((b * a.keys + key) * a.key_heads + kh) * a.columns * F::BYTES, all = int64_t(a.batch_heads) * a.keys;
     float *const part = a.splits > 1 ? a.part + (int64_t(split) * all + bh * a.keys + key) * a.columns : nullptr;
     store_sums<F, DB>(dk, __builtin_amdgcn_ldexpf(a.scale, -lift), a.gk + at, part, a.columns, half);
     store_sums<F, DB>(dv, HALF ? 1.f / 16384.f : 1.f, a.gv + at, part ? part + a.splits * all * a.columns : nullptr, a.columns, half);
@@ -370,8 +354,8 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void key_gr
 
 // The splits' sums of a row as one, in their order.  Four columns a lane.
 template <typename F>
-__global__ __launch_bounds__(WG) void add_splits_kernel(const float *part, char *out, int64_t all, int rows, int64_t len, int key_heads, int group,
-                                                        int splits, int columns) {
+__global__ __launch_bounds__(WG) void add_splits_kernel(const float *part, char *out, int64_t all, int rows, int64_t len, Divisor key_heads,
+                                                        Divisor group, int splits, int columns) {
     const int quads = columns / 4;
     const int64_t i = int64_t(blockIdx.x) * WG + threadIdx.x, at = i / quads;
     const int col = int(i - at * quads) * 4;
@@ -381,8 +365,8 @@ __global__ __launch_bounds__(WG) void add_splits_kernel(const float *part, char 
         const float4 v = *reinterpret_cast<const float4 *>(part + (s * all + at) * columns + col);
         acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
     }
-    const int64_t bh = at / rows, b = bh / key_heads, kh = bh - b * key_heads;
-    F::store4(out + (heads_row(b, kh, int(at - bh * rows), len, key_heads, group) * columns + col) * F::BYTES, acc.x, acc.y, acc.z, acc.w);
+    const int bh = int(at / rows), b = key_heads.quotient(bh), kh = bh - b * key_heads.by;
+    F::store4(out + (heads_row(b, kh, int(at - int64_t(bh) * rows), len, key_heads.by, group) * columns + col) * F::BYTES, acc.x, acc.y, acc.z, acc.w);
 }
 
 constexpr int64_t WANTED = 512;           // workgroups, where there is enough to share out
@@ -404,6 +388,7 @@ void share_out(BwdArgs &a, int64_t standing, int64_t passing, int kt, int64_t ba
     a.split_steps = (a.steps + splits - 1) / splits;
     a.splits = a.split_steps ? int((a.steps + a.split_steps - 1) / a.split_steps) : 1;
     a.units = tiles * a.splits;
+    a.tile_by = Divisor(a.tiles > 0 ? (uint32_t)a.tiles : 1), a.split_by = Divisor((uint32_t)a.splits);
 }
 
 Plan plan(const lffn_cross_attention &c) {
@@ -417,12 +402,15 @@ Plan plan(const lffn_cross_attention &c) {
     a.kb = c.k_strides[0] * size, a.kt = c.k_strides[1] * size, a.kh = c.k_strides[2] * size;
     a.vb = c.v_strides[0] * size, a.vt = c.v_strides[1] * size, a.vh = c.v_strides[2] * size;
     a.keys = c.k_len, a.q_len = c.q_len, a.batch_heads = (int)batch_heads;
-    a.key_heads = (int)c.key_heads, a.group = int(c.heads / c.key_heads), a.columns = (int)c.columns;
-    a.rows = int(c.q_len * a.group);
+    const int64_t group = c.heads / c.key_heads;
+    a.key_heads = (int)c.key_heads, a.columns = (int)c.columns;
+    a.rows = int(c.q_len * group);
+    a.group = Divisor(group > 0 ? (uint32_t)group : 1), a.heads = Divisor((uint32_t)a.key_heads);
     a.c = c.scale * LOG2E, a.scale = c.scale;
     const bool norms = c.format == LFFN_ROWS_F16;
     a.g_tiles = (a.rows + NORM_ROWS - 1) / NORM_ROWS;
     a.v_tiles = norms ? int((a.keys + NORM_ROWS - 1) / NORM_ROWS) : 0;
+    a.norm_tiles = Divisor(a.g_tiles + a.v_tiles > 0 ? uint32_t(a.g_tiles + a.v_tiles) : 1);
     p.q = p.k = a;
     share_out(p.q, a.rows, a.keys, kt, batch_heads);
     share_out(p.k, a.keys, a.rows, kt, batch_heads);
@@ -441,9 +429,9 @@ Plan plan(const lffn_cross_attention &c) {
 }
 
 template <typename F>
-void add_splits(const float *part, char *out, const BwdArgs &a, int rows, int64_t len, int group, hipStream_t stream) {
+void add_splits(const float *part, char *out, const BwdArgs &a, int rows, int64_t len, Divisor group, hipStream_t stream) {
     const int64_t all = int64_t(a.batch_heads) * rows;
-    add_splits_kernel<F><<<dim3((unsigned)((all * (a.columns / 4) + WG - 1) / WG)), dim3(WG), 0, stream>>>(part, out, all, rows, len, a.key_heads,
+    add_splits_kernel<F><<<dim3((unsigned)((all * (a.columns / 4) + WG - 1) / WG)), dim3(WG), 0, stream>>>(part, out, all, rows, len, a.heads,
                                                                                                      group, a.splits, a.columns);
 }
 
@@ -466,8 +454,8 @@ int launch(const Plan &p, hipStream_t stream) {
         key_gradient_kernel<F, DP, KT><<<dim3((unsigned)p.k.units), dim3(WG), bytes, stream>>>(p.k);
         if (p.k.splits > 1) {
             const int64_t one = int64_t(p.k.splits) * p.k.batch_heads * p.k.keys * p.k.columns;
-            add_splits<F>(p.k.part, p.k.gk, p.k, (int)p.k.keys, p.k.keys, 1, stream);
-            add_splits<F>(p.k.part + one, p.k.gv, p.k, (int)p.k.keys, p.k.keys, 1, stream);
+            add_splits<F>(p.k.part, p.k.gk, p.k, (int)p.k.keys, p.k.keys, Divisor(1), stream);
+            add_splits<F>(p.k.part + one, p.k.gv, p.k, (int)p.k.keys, p.k.keys, Divisor(1), stream);
         }
     }
     return lffn_launch_status();
