@@ -67,6 +67,7 @@ struct BF16 {
     static __device__ __forceinline__ Raw zero() { return {make_uint4(0, 0, 0, 0)}; }
     static __device__ __forceinline__ Frag<1> operand(const Raw &r) { return {{r.u}}; }
     static __device__ __forceinline__ void unpack(const Raw &r, float (&v)[8]) { BF16Row::unpack(r.u, v); }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return BF16Row::pack2(a, b); }
     static __device__ __forceinline__ void store4(char *p, float a, float b, float c, float d) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(BF16Row::pack2(a, b), BF16Row::pack2(c, d));
     }
@@ -86,6 +87,7 @@ struct F16 {
     static __device__ __forceinline__ Raw zero() { return BF16::zero(); }
     static __device__ __forceinline__ Frag<1> operand(const Raw &r) { return {{r.u}}; }
     static __device__ __forceinline__ void unpack(const Raw &r, float (&v)[8]) { F16Row::unpack(r.u, v); }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return F16Row::pack2(a, b); }
     static __device__ __forceinline__ void store4(char *p, float a, float b, float c, float d) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(F16Row::pack2(a, b), F16Row::pack2(c, d));
     }
@@ -125,6 +127,38 @@ struct F32 {
         *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
     }
 };
+
+// The columns 32 d + 8 g + 4 half .. + 3 of a lane's row (half = lane / 32) to memory, by d and g; `row` where the lane's row begins, all lanes together.  Of 16-bit
+// results the lanes of a row exchange four columns of two groups, so that each has eight that lie together and stores 16 bytes.
+template <typename F, int DB>
+__device__ __forceinline__ void store_row(const ca_f32x16_t (&o)[DB], float by, char *row, bool live, int columns, int half) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+        if constexpr (F::BYTES == 4) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = 32 * d + 8 * g + 4 * half;
+                if (live && col < columns)
+                    F::store4(row + col * F::BYTES, o[d][4 * g] * by, o[d][4 * g + 1] * by, o[d][4 * g + 2] * by, o[d][4 * g + 3] * by);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; g += 2) {
+                uint32_t a[2], b[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    a[e] = F::pack2(o[d][4 * g + 2 * e] * by, o[d][4 * g + 2 * e + 1] * by);
+                    b[e] = F::pack2(o[d][4 * g + 4 + 2 * e] * by, o[d][4 * g + 4 + 2 * e + 1] * by);
+                    // the upper lanes' a and the lower lanes' b change places
+                    const auto swapped = __builtin_amdgcn_permlane32_swap(a[e], b[e], false, false);
+                    a[e] = swapped[0], b[e] = swapped[1];
+                }
+                const int col = 32 * d + 8 * (g + half);
+                if (live && col < columns) *reinterpret_cast<uint4 *>(row + col * 2) = make_uint4(a[0], a[1], b[0], b[1]);
+            }
+        }
+    }
+}
 
 // A tile of KT rows of DP numbers in LDS, PLANES terms of 16 bits, DP / 8 pieces of 16 bytes a row.  The pieces of a row are turned by its number, so
 // that the 16 rows that an operand's read takes of one piece, and the 4 rows x 64 bytes that half a transposing read takes, are on different banks.

@@ -53,7 +53,9 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     ca_f32x16_t o[DB] = {};
     float most = -INFINITY, sum = 0.f;
 
+    const bool wave_works = tile * TILE + wave * ROWS < a.rows;
     auto compute = [&](auto buf, uint64_t word) {
+        if (!wave_works) return;
         constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
         ca_f32x16_t s[KB] = {};
 #pragma unroll
@@ -110,61 +112,77 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
 
     sum += lane_xor<32>(sum);
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query without keys: zeros
-    if (row >= a.rows) return;
     const float level = sum == 0.f ? INFINITY : (most == -INFINITY ? 0.f : most) * a.c - F::LIFT + __builtin_amdgcn_logf(sum);
+    const bool live = row < a.rows;
     const int64_t at = int64_t(bh) * a.rows + row;
     if (a.splits > 1) {
         const int64_t of = int64_t(split) * (a.units / (a.splits * a.row_tiles)) * a.rows + at;
-        if (half == 0) a.part_lse[of] = level;
-        float *const p = a.part + of * a.columns;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int col = 32 * d + 8 * g + 4 * half;
-                if (col < a.columns)
-                    *reinterpret_cast<float4 *>(p + col) =
-                        make_float4(o[d][4 * g] * inverse, o[d][4 * g + 1] * inverse, o[d][4 * g + 2] * inverse, o[d][4 * g + 3] * inverse);
-            }
+        if (live && half == 0) a.part_lse[of] = level;
+        store_row<F32, DB>(o, inverse, reinterpret_cast<char *>(a.part + of * a.columns), live, a.columns, half);
         return;
     }
-    if (a.lse && half == 0) a.lse[at] = level;
-    char *const p = a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int col = 32 * d + 8 * g + 4 * half;
-            if (col < a.columns)
-                F::store4(p + col * F::BYTES, o[d][4 * g] * inverse, o[d][4 * g + 1] * inverse, o[d][4 * g + 2] * inverse, o[d][4 * g + 3] * inverse);
-        }
+    if (a.lse && live && half == 0) a.lse[at] = level;
+    store_row<F, DB>(o, inverse, a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES, live, a.columns, half);
 }
 
-// The splits' results of a row as one: weights 2^(level - largest level).  Four columns a lane.
+// The splits' results of a row as one: weights 2^(level - largest level).  Four columns a lane, a fourth of the splits a wavefront, four of them asked for
+// together.  (One thread for all splits of four columns: 16 splits of 128 rows x 128 columns 14.6 us.)
 template <typename F>
 __global__ __launch_bounds__(WG) void join_kernel(FwdArgs a, int64_t all_rows) {
-    const int quads = a.columns / 4;
-    const int64_t i = int64_t(blockIdx.x) * WG + threadIdx.x, at = i / quads;
-    const int col = int(i - at * quads) * 4;
-    if (at >= all_rows) return;
-    float most = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) {
-        const float l = a.part_lse[s * all_rows + at];
-        if (l != INFINITY) most = fmaxf(most, l);
-    }
+    constexpr int TOGETHER = 4;
+    __shared__ float4 sums[WAVES][64];
+    __shared__ float2 weights[WAVES][64];                // largest level, sum of weights
+    const int quads = a.columns / 4, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = int64_t(blockIdx.x) * 64 + lane, last = all_rows * quads - 1, at = (i < last ? i : last) / quads;
+    const int col = int((i < last ? i : last) - at * quads) * 4;
+    float most = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float l = a.part_lse[s * all_rows + at];
-        if (l == INFINITY) continue;                     // (no key that takes part)
-        const float w = __builtin_amdgcn_exp2f(l - (most == -INFINITY ? 0.f : most));
-        const float4 v = *reinterpret_cast<const float4 *>(a.part + (s * all_rows + at) * a.columns + col);
-        sum += w;
-        acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
+    for (int first = wave; first < a.splits; first += WAVES * TOGETHER) {
+        float l[TOGETHER], now = most;
+        float4 v[TOGETHER];
+#pragma unroll
+        for (int n = 0; n < TOGETHER; ++n) {
+            const int64_t s = min(first + n * WAVES, a.splits - 1);
+            l[n] = a.part_lse[s * all_rows + at];
+            v[n] = *reinterpret_cast<const float4 *>(a.part + (s * all_rows + at) * a.columns + col);
+        }
+#pragma unroll
+        for (int n = 0; n < TOGETHER; ++n) {
+            if (first + n * WAVES >= a.splits || l[n] == INFINITY) l[n] = -INFINITY, v[n] = make_float4(0.f, 0.f, 0.f, 0.f);      // (no key that takes part)
+            now = fmaxf(now, l[n]);
+        }
+        const float less = now == -INFINITY ? 0.f : now, by = __builtin_amdgcn_exp2f(most - less);
+        sum *= by;
+        acc.x *= by, acc.y *= by, acc.z *= by, acc.w *= by;
+#pragma unroll
+        for (int n = 0; n < TOGETHER; ++n) {
+            const float w = __builtin_amdgcn_exp2f(l[n] - less);
+            sum += w;
+            acc.x = fmaf(w, v[n].x, acc.x), acc.y = fmaf(w, v[n].y, acc.y), acc.z = fmaf(w, v[n].z, acc.z), acc.w = fmaf(w, v[n].w, acc.w);
+        }
+        most = now;
+    }
+    sums[wave][lane] = acc;
+    weights[wave][lane] = make_float2(most, sum);
+    __syncthreads();
+    if (wave != 0 || i > last) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all = fmaxf(all, weights[w][lane].x);
+    const float less = all == -INFINITY ? 0.f : all;
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float2 m = weights[w][lane];
+        const float4 v = sums[w][lane];
+        const float by = __builtin_amdgcn_exp2f(m.x - less);
+        sum = fmaf(by, m.y, sum);
+        acc.x = fmaf(by, v.x, acc.x), acc.y = fmaf(by, v.y, acc.y), acc.z = fmaf(by, v.z, acc.z), acc.w = fmaf(by, v.w, acc.w);
     }
     const float by = sum == 0.f ? 0.f : 1.f / sum;
     const int bh = int(at / a.rows), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, row = int(at - int64_t(bh) * a.rows);
-    if (a.lse && col == 0) a.lse[at] = sum == 0.f ? INFINITY : most + __builtin_amdgcn_logf(sum);
+    if (a.lse && col == 0) a.lse[at] = sum == 0.f ? INFINITY : less + __builtin_amdgcn_logf(sum);
     char *const p = a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
     F::store4(p + col * F::BYTES, acc.x * by, acc.y * by, acc.z * by, acc.w * by);
 }
@@ -203,7 +221,7 @@ constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
 // Fills sizes in; the workspace's bytes, or -1: too many tiles.
 int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     const int64_t size = c.format == LFFN_ROWS_F32 ? 4 : 2;
-    const int kt = c.format == LFFN_ROWS_F32 && c.columns > 64 ? 32 : 64;
+    const int kt = c.format == LFFN_ROWS_F32 && c.columns > 32 ? 32 : 64;
     a.q = static_cast<const char *>(c.q), a.k = static_cast<const char *>(c.k), a.v = static_cast<const char *>(c.v);
     a.mask = c.key_mask, a.mask_stride = c.mask_stride;
     a.qb = c.q_strides[0] * size, a.qt = c.q_strides[1] * size, a.qh = c.q_strides[2] * size;
@@ -237,7 +255,7 @@ int launch(const FwdArgs &a, hipStream_t stream) {
     cross_attention_kernel<F, DP, KT><<<dim3((unsigned)a.units), dim3(WG), bytes, stream>>>(a);
     if (a.splits > 1) {
         const int64_t rows = int64_t(a.units / (a.splits * a.row_tiles)) * a.rows;
-        join_kernel<F><<<dim3((unsigned)((rows * (a.columns / 4) + WG - 1) / WG)), dim3(WG), 0, stream>>>(a, rows);
+        join_kernel<F><<<dim3((unsigned)((rows * (a.columns / 4) + 63) / 64)), dim3(WG), 0, stream>>>(a, rows);
     }
     return lffn_launch_status();
 }
@@ -245,7 +263,7 @@ int launch(const FwdArgs &a, hipStream_t stream) {
 template <typename F>
 int launch(const FwdArgs &a, hipStream_t stream) {
     if (a.columns <= 32) return launch<F, 32, 64>(a, stream);
-    if (a.columns <= 64) return launch<F, 64, 64>(a, stream);
+    if (a.columns <= 64) return launch<F, 64, F::PLANES == 1 ? 64 : 32>(a, stream);
     return launch<F, 128, F::PLANES == 1 ? 64 : 32>(a, stream);
 }
 

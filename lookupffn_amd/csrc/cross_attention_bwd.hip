@@ -114,31 +114,19 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
 template <typename F>
 __device__ __forceinline__ int ds_exponent(const BwdArgs &a, int64_t bh) {
     if constexpr (F::LIFT == 0.f) return 0;
-    float g = 0.f, v = 0.f;
-    for (int i = threadIdx.x & 63; i < a.g_tiles; i += 64) g = fmaxf(g, a.g_norms[bh * a.g_tiles + i]);
-    for (int i = threadIdx.x & 63; i < a.v_tiles; i += 64) v = fmaxf(v, a.v_norms[bh * a.v_tiles + i]);
+    if (a.g_tiles == 0 || a.v_tiles == 0) return 0;
+    const float *const gs = a.g_norms + bh * a.g_tiles, *const vs = a.v_norms + bh * a.v_tiles;
+    const int lane = threadIdx.x & 63;
+    float g = gs[min(lane, a.g_tiles - 1)], v = vs[min(lane, a.v_tiles - 1)];
+    for (int i = lane + 64; i < a.g_tiles; i += 64) g = fmaxf(g, gs[i]);
+    for (int i = lane + 64; i < a.v_tiles; i += 64) v = fmaxf(v, vs[i]);
     const float most = 2.f * sqrtf(wave_most(g)) * sqrtf(wave_most(v));
     const int e = int(__float_as_uint(most) >> 23) - 127;    // most < 2^(e + 1)
     return most > 0.f && e < 128 ? __builtin_amdgcn_readfirstlane(min(max(14 - e, -60), 60)) : 0;
 }
 
-// The sums of a standing row, or a split's part of them, to where they belong.
-template <typename F, int DB>
-__device__ __forceinline__ void store_sums(const ca_f32x16_t (&o)[DB], float by, char *out, float *part, int columns, int half) {
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int col = 32 * d + 8 * g + 4 * half;
-            if (col >= columns) continue;
-            const float t[4] = {o[d][4 * g] * by, o[d][4 * g + 1] * by, o[d][4 * g + 2] * by, o[d][4 * g + 3] * by};
-            if (part) *reinterpret_cast<float4 *>(part + col) = make_float4(t[0], t[1], t[2], t[3]);
-            else F::store4(out + col * F::BYTES, t[0], t[1], t[2], t[3]);
-        }
-}
-
 template <typename F, int DP, int KT>
-__global__ __launch_bounds__(WG, F::PLANES == 1 ? 2 : 1) void query_gradient_kernel(BwdArgs a) {
+__global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1 || DP <= 64 ? 2 : 1) void query_gradient_kernel(BwdArgs a) {
     typedef Tile<F, DP, KT> T;
     typedef Frag<F::PLANES> Op;
     constexpr int CHUNKS = DP / 16, KB = KT / 32, DB = DP / 32;
@@ -170,7 +158,9 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 ? 2 : 1) void query_gradient_ker
     const float level = live ? a.lse[int64_t(bh) * a.rows + row] : INFINITY, delta = live ? a.delta[int64_t(bh) * a.rows + row] * f : 0.f;
     ca_f32x16_t dq[DB] = {};
 
+    const bool wave_works = tile * TILE + wave * ROWS < a.rows;
     auto compute = [&](auto buf, uint64_t word) {
+        if (!wave_works) return;
         constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -203,13 +193,13 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 ? 2 : 1) void query_gradient_ker
 
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
-    if (!live) return;
-    float *const part = a.splits > 1 ? a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns : nullptr;
-    store_sums<F, DB>(dq, __builtin_amdgcn_ldexpf(a.scale, -lift), a.gq + out_row, part, a.columns, half);
+    const float by = __builtin_amdgcn_ldexpf(a.scale, -lift);
+    if (a.splits > 1) store_row<F32, DB>(dq, by, reinterpret_cast<char *>(a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns), live, a.columns, half);
+    else store_row<F, DB>(dq, by, a.gq + out_row, live, a.columns, half);
 }
 
 template <typename F, int DP, int KT>
-__global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdArgs a) {
+__global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdArgs a) {
     typedef Tile<F, DP, KT> T;
     typedef Frag<F::PLANES> Op;
     constexpr int CHUNKS = DP / 16, RB = KT / 32, DB = DP / 32;
@@ -341,32 +331,50 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 2 : 1) void key_gr
             __syncthreads();
         }
     }
-    if (!in) return;
     if (!live) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) dk[d] = ca_f32x16_t{}, dv[d] = ca_f32x16_t{};
     }
-    const int64_t at = ((b * a.keys + key) * a.key_heads + kh) * a.columns * F::BYTES, all = int64_t(a.batch_heads) * a.keys;
-    float *const part = a.splits > 1 ? a.part + (int64_t(split) * all + bh * a.keys + key) * a.columns : nullptr;
-    store_sums<F, DB>(dk, __builtin_amdgcn_ldexpf(a.scale, -lift), a.gk + at, part, a.columns, half);
-    store_sums<F, DB>(dv, HALF ? 1.f / 16384.f : 1.f, a.gv + at, part ? part + a.splits * all * a.columns : nullptr, a.columns, half);
+    const float by_k = __builtin_amdgcn_ldexpf(a.scale, -lift), by_v = HALF ? 1.f / 16384.f : 1.f;
+    if (a.splits > 1) {
+        const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key) * a.columns;
+        store_row<F32, DB>(dk, by_k, reinterpret_cast<char *>(a.part + of), in, a.columns, half);
+        store_row<F32, DB>(dv, by_v, reinterpret_cast<char *>(a.part + a.splits * all * a.columns + of), in, a.columns, half);
+    } else {
+        const int64_t at = ((b * a.keys + key) * a.key_heads + kh) * a.columns * F::BYTES;
+        store_row<F, DB>(dk, by_k, a.gk + at, in, a.columns, half);
+        store_row<F, DB>(dv, by_v, a.gv + at, in, a.columns, half);
+    }
 }
 
-// The splits' sums of a row as one, in their order.  Four columns a lane.
+// The splits' sums of a row as one, in their order, four of them asked for together; `second` beside `part` where there are two arrays.  Four columns a lane.
+struct AddArgs {
+    const float *part[2];
+    char *out[2];
+    int64_t all, len;                     // rows: [batch, heads of keys] x rows
+    Divisor heads, group;
+    int rows, splits, columns;
+};
 template <typename F>
-__global__ __launch_bounds__(WG) void add_splits_kernel(const float *part, char *out, int64_t all, int rows, int64_t len, Divisor key_heads,
-                                                        Divisor group, int splits, int columns) {
-    const int quads = columns / 4;
+__global__ __launch_bounds__(WG) void add_splits_kernel(AddArgs a) {
+    constexpr int TOGETHER = 4;
+    const int quads = a.columns / 4;
     const int64_t i = int64_t(blockIdx.x) * WG + threadIdx.x, at = i / quads;
     const int col = int(i - at * quads) * 4;
-    if (at >= all) return;
+    if (at >= a.all) return;
+    const float *const part = a.part[blockIdx.y] + at * a.columns + col;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < splits; ++s) {
-        const float4 v = *reinterpret_cast<const float4 *>(part + (s * all + at) * columns + col);
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    for (int first = 0; first < a.splits; first += TOGETHER) {
+        float4 v[TOGETHER];
+#pragma unroll
+        for (int n = 0; n < TOGETHER; ++n) v[n] = *reinterpret_cast<const float4 *>(part + min(first + n, a.splits - 1) * a.all * a.columns);
+#pragma unroll
+        for (int n = 0; n < TOGETHER; ++n)
+            if (first + n < a.splits) acc.x += v[n].x, acc.y += v[n].y, acc.z += v[n].z, acc.w += v[n].w;
     }
-    const int bh = int(at / rows), b = key_heads.quotient(bh), kh = bh - b * key_heads.by;
-    F::store4(out + (heads_row(b, kh, int(at - int64_t(bh) * rows), len, key_heads.by, group) * columns + col) * F::BYTES, acc.x, acc.y, acc.z, acc.w);
+    const int bh = int(at / a.rows), b = a.heads.quotient(bh), kh = bh - b * a.heads.by;
+    F::store4(a.out[blockIdx.y] + (heads_row(b, kh, int(at - int64_t(bh) * a.rows), a.len, a.heads.by, a.group) * a.columns + col) * F::BYTES, acc.x, acc.y, acc.z,
+              acc.w);
 }
 
 constexpr int64_t WANTED = 512;           // workgroups, where there is enough to share out
@@ -395,7 +403,7 @@ Plan plan(const lffn_cross_attention &c) {
     Plan p;
     BwdArgs a{};
     const int64_t size = c.format == LFFN_ROWS_F32 ? 4 : 2, batch_heads = c.B * c.key_heads;
-    const int kt = c.format == LFFN_ROWS_F32 && c.columns > 64 ? 32 : 64;
+    const int kt = c.format == LFFN_ROWS_F32 && c.columns > 32 ? 32 : 64;
     a.q = static_cast<const char *>(c.q), a.k = static_cast<const char *>(c.k), a.v = static_cast<const char *>(c.v);
     a.mask = c.key_mask, a.mask_stride = c.mask_stride;
     a.qb = c.q_strides[0] * size, a.qt = c.q_strides[1] * size, a.qh = c.q_strides[2] * size;
@@ -429,10 +437,8 @@ Plan plan(const lffn_cross_attention &c) {
 }
 
 template <typename F>
-void add_splits(const float *part, char *out, const BwdArgs &a, int rows, int64_t len, Divisor group, hipStream_t stream) {
-    const int64_t all = int64_t(a.batch_heads) * rows;
-    add_splits_kernel<F><<<dim3((unsigned)((all * (a.columns / 4) + WG - 1) / WG)), dim3(WG), 0, stream>>>(part, out, all, rows, len, a.heads,
-                                                                                                     group, a.splits, a.columns);
+void add_splits(const AddArgs &a, int arrays, hipStream_t stream) {
+    add_splits_kernel<F><<<dim3((unsigned)((a.all * (a.columns / 4) + WG - 1) / WG), arrays), dim3(WG), 0, stream>>>(a);
 }
 
 template <typename F, int DP, int KT>
@@ -445,18 +451,20 @@ int launch(const Plan &p, hipStream_t stream) {
         const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + BLOCK * 8;
         if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&query_gradient_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
         query_gradient_kernel<F, DP, KT><<<dim3((unsigned)p.q.units), dim3(WG), bytes, stream>>>(p.q);
-        if (p.q.splits > 1) add_splits<F>(p.q.part, p.q.gq, p.q, p.q.rows, p.q.q_len, p.q.group, stream);
+        const BwdArgs &q = p.q;
+        if (q.splits > 1)
+            add_splits<F>({{q.part, nullptr}, {q.gq, nullptr}, int64_t(q.batch_heads) * q.rows, q.q_len, q.heads, q.group, q.rows, q.splits, q.columns}, 1, stream);
     }
     if (p.k.units > 0) {
         static LdsGrant granted;
         const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + 4 * KT * 4;
         if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&key_gradient_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
         key_gradient_kernel<F, DP, KT><<<dim3((unsigned)p.k.units), dim3(WG), bytes, stream>>>(p.k);
-        if (p.k.splits > 1) {
-            const int64_t one = int64_t(p.k.splits) * p.k.batch_heads * p.k.keys * p.k.columns;
-            add_splits<F>(p.k.part, p.k.gk, p.k, (int)p.k.keys, p.k.keys, Divisor(1), stream);
-            add_splits<F>(p.k.part + one, p.k.gv, p.k, (int)p.k.keys, p.k.keys, Divisor(1), stream);
-        }
+        const BwdArgs &k = p.k;
+        const int64_t all = int64_t(k.batch_heads) * k.keys;
+        if (k.splits > 1)
+            add_splits<F>({{k.part, k.part + k.splits * all * k.columns}, {k.gk, k.gv}, all, k.keys, k.heads, Divisor(1), (int)k.keys, k.splits, k.columns}, 2,
+                          stream);
     }
     return lffn_launch_status();
 }
@@ -464,7 +472,7 @@ int launch(const Plan &p, hipStream_t stream) {
 template <typename F>
 int launch(const Plan &p, hipStream_t stream) {
     if (p.q.columns <= 32) return launch<F, 32, 64>(p, stream);
-    if (p.q.columns <= 64) return launch<F, 64, 64>(p, stream);
+    if (p.q.columns <= 64) return launch<F, 64, F::PLANES == 1 ? 64 : 32>(p, stream);
     return launch<F, 128, F::PLANES == 1 ? 64 : 32>(p, stream);
 }
 
