@@ -20,13 +20,20 @@ struct FwdArgs {
     int64_t keys, steps, split_steps, q_len;
     Divisor group, tiles, split_by, heads;               // query heads of a key head, tiles of rows, shares of the keys, key heads
     int key_heads, rows, row_tiles, splits, columns, units;
+    int few_waves;                        // few_rows_kernel's wavefronts, 0: not the one
     float c;                              // scale log2 e
 };
 
+// few_rows_kernel: rows at most.  us, few_rows_kernel and cross_attention_kernel: 16 x 512 keys x 12 heads x 64 half, 1 row 8.1, 13.5; 4 x 16384 x 8 x 128 bfloat16,
+// 1 row 59, 56, 2 rows 61, 60, 4 rows 69, 61; 64 x 512 x 16 x 64 bfloat16, 1 row 31, 36, 4 rows 49, 36; fp32 32 x 2048 x 16 x 64, 1 row 100, 123, 8 x 1024 x 8 x 128, 4 rows
+// 20, 40, 32 x 1024 x 12 x 64, 3 rows 53, 64.
+constexpr int few_rows(bool f32) { return f32 ? 4 : 2; }
+constexpr int FEW_WAVES = 16;             // wavefronts of a workgroup at most,
+constexpr int FEW_TOGETHER = 2;           // keys of a group of lanes asked for together
 constexpr float SLACK = 6.f;              // how far (powers of two) a row's largest score may outgrow the one that its sums go by
 
 template <typename F, int DP, int KT>
-__global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1 || DP <= 64 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
+__global__ __launch_bounds__(WG, DP <= 64 ? 3 : F::PLANES == 1 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
     typedef Tile<F, DP, KT> T;
     typedef Frag<F::PLANES> Op;
     constexpr int CHUNKS = DP / 16, KB = KT / 32, DB = DP / 32;
@@ -125,30 +132,164 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     store_row<F, DB>(o, inverse, a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES, live, a.columns, half);
 }
 
+// A row or two for a key head (fp32: up to four): single tokens, with the heads that share it.  On the vector ALU, which keeps up with the memory here (a number of a key or value
+// is one multiply-add a row) and needs neither tiles nor barriers: G lanes have a key and its value, 16 bytes a lane, 64 / G keys a wavefront and FEW_TOGETHER of them
+// asked for at a time, so that a short call waits for memory once and its code is short (a launch fetches it anew).  Every group of lanes has a softmax of
+// its own keys; groups and wavefronts are joined at the end.  Up to sixteen wavefronts a workgroup, so that 512 keys need no second kernel to join shares.
+template <typename R, typename F, int G, int RN>
+__global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(FwdArgs a) {
+    constexpr int N = R::N, KEYS = 64 / G;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, group = lane / G, j = lane % G;
+    const Unit unit = unit_of(blockIdx.x, a.units, a.tiles, a.split_by, a.heads);
+    const int split = unit.split, bh = unit.bh, b = unit.b, kh = unit.kh;
+    const bool on = j * N < a.columns;
+    const int64_t column = on ? j * 16 : 0;
+    const char *const kp = a.k + b * a.kb + kh * a.kh + column, *const vp = a.v + b * a.vb + kh * a.vh + column;
+    const uint8_t *const mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+    const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.keys ? begin + a.split_steps : a.keys;      // (steps of one key)
+    const int64_t first = begin + wave * (KEYS * FEW_TOGETHER) + group;
+
+    uint4 k[FEW_TOGETHER], v[FEW_TOGETHER];
+    bool live[FEW_TOGETHER];
+    auto fetch = [&](int64_t from) {
+#pragma unroll
+        for (int u = 0; u < FEW_TOGETHER; ++u) {
+            const int64_t key = from + u * KEYS, at = key < end ? key : end - 1;
+            live[u] = key < end && (!mask || mask[at] != 0);
+            k[u] = *reinterpret_cast<const uint4 *>(kp + at * a.kt);
+            v[u] = *reinterpret_cast<const uint4 *>(vp + at * a.vt);
+        }
+    };
+    if (begin < end) fetch(first);
+    float q[RN][N], acc[RN][N] = {}, most[RN], sum[RN] = {};
+    const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh + column, a.qt, a.qh, a.group};
+#pragma unroll
+    for (int r = 0; r < RN; ++r) {
+        most[r] = -INFINITY;
+        R::unpack(*reinterpret_cast<const uint4 *>(rows.at(r < a.rows ? r : 0)), q[r]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) q[r][e] = on ? q[r][e] * a.c : 0.f;
+    }
+#pragma unroll 1
+    for (int64_t at = first; at - group < end;) {
+        float s[RN][FEW_TOGETHER];
+#pragma unroll
+        for (int u = 0; u < FEW_TOGETHER; ++u) {
+            float x[N];
+            R::unpack(k[u], x);
+#pragma unroll
+            for (int r = 0; r < RN; ++r) {
+                float dot = 0.f;
+#pragma unroll
+                for (int e = 0; e < N; ++e) dot = fmaf(q[r][e], on ? x[e] : 0.f, dot);
+                s[r][u] = live[u] ? lane_group_sum<G>(dot) : -INFINITY;
+            }
+        }
+        float w[RN][FEW_TOGETHER];
+#pragma unroll
+        for (int r = 0; r < RN; ++r) {
+            float now = most[r];
+#pragma unroll
+            for (int u = 0; u < FEW_TOGETHER; ++u) now = fmaxf(now, s[r][u]);
+            const float less = now == -INFINITY ? 0.f : now, by = most[r] == now ? 1.f : __builtin_amdgcn_exp2f(most[r] - less);
+            sum[r] *= by;
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[r][e] *= by;
+#pragma unroll
+            for (int u = 0; u < FEW_TOGETHER; ++u) {
+                w[r][u] = __builtin_amdgcn_exp2f(s[r][u] - less);
+                sum[r] += w[r][u];
+            }
+            most[r] = now;
+        }
+#pragma unroll
+        for (int u = 0; u < FEW_TOGETHER; ++u) {
+            float x[N];
+            R::unpack(v[u], x);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float value = live[u] ? x[e] : 0.f;                // (whatever is there)
+#pragma unroll
+                for (int r = 0; r < RN; ++r) acc[r][e] = fmaf(w[r][u], value, acc[r][e]);
+            }
+        }
+        at += waves * (KEYS * FEW_TOGETHER);
+        if (at - group < end) fetch(at);
+    }
+
+    __shared__ float2 of_wave[FEW_WAVES][RN];            // largest score, sum of weights
+    __shared__ float4 sums[FEW_WAVES][RN][G * N / 4];
+    auto over_groups = [](float x, auto &&f) {
+        if constexpr (G <= 4) x = f(x, lane_xor<4>(x));
+        if constexpr (G <= 8) x = f(x, lane_xor<8>(x));
+        if constexpr (G <= 16) x = f(x, lane_xor<16>(x));
+        return f(x, lane_xor<32>(x));
+    };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
+    auto plus = [](float x, float y) { return x + y; };
+#pragma unroll
+    for (int r = 0; r < RN; ++r) {
+        const float all = over_groups(most[r], larger), by = most[r] == all ? 1.f : __builtin_amdgcn_exp2f(most[r] - all);
+        const float total = over_groups(sum[r] * by, plus);
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[r][e] = over_groups(acc[r][e] * by, plus);
+        if (lane == 0) of_wave[wave][r] = make_float2(all, total);
+        if (group == 0) {
+#pragma unroll
+            for (int e = 0; e < N; e += 4) sums[wave][r][(j * N + e) / 4] = make_float4(acc[r][e], acc[r][e + 1], acc[r][e + 2], acc[r][e + 3]);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < RN * (G * N / 4); i += blockDim.x) {
+        const int r = i / (G * N / 4), quad = i % (G * N / 4), col = quad * 4;
+        if (r >= a.rows || col >= a.columns) continue;
+        float all = -INFINITY, total = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int n = 0; n < waves; ++n) all = fmaxf(all, of_wave[n][r].x);
+        for (int n = 0; n < waves; ++n) {
+            const float2 m = of_wave[n][r];
+            const float4 x = sums[n][r][quad];
+            const float by = m.x == all ? 1.f : __builtin_amdgcn_exp2f(m.x - all);
+            total = fmaf(by, m.y, total);
+            o.x = fmaf(by, x.x, o.x), o.y = fmaf(by, x.y, o.y), o.z = fmaf(by, x.z, o.z), o.w = fmaf(by, x.w, o.w);
+        }
+        const float inverse = total == 0.f ? 0.f : 1.f / total, level = total == 0.f ? INFINITY : all + __builtin_amdgcn_logf(total);
+        const int64_t at = int64_t(bh) * a.rows + r;
+        if (a.splits > 1) {
+            const int64_t of = int64_t(split) * (a.units / a.splits) * a.rows + at;
+            if (quad == 0) a.part_lse[of] = level;
+            *reinterpret_cast<float4 *>(a.part + of * a.columns + col) = make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse);
+        } else {
+            if (quad == 0 && a.lse) a.lse[at] = level;
+            F::store4(a.out + (heads_row(b, kh, r, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES, o.x * inverse, o.y * inverse, o.z * inverse,
+                      o.w * inverse);
+        }
+    }
+}
+
 // The splits' results of a row as one: weights 2^(level - largest level).  Four columns a lane, a fourth of the splits a wavefront, four of them asked for
-// together.  (One thread for all splits of four columns: 16 splits of 128 rows x 128 columns 14.6 us.)
-template <typename F>
+// together; of few splits all by one thread.  (One thread for all, one split after the other: 16 splits of 128 rows x 128 columns 14.6 us, so 4.8; 2 splits of
+// 32000 rows x 64 columns, a wavefront each 11.2, one thread 6.)
+template <typename F, int SHARES>
 __global__ __launch_bounds__(WG) void join_kernel(FwdArgs a, int64_t all_rows) {
     constexpr int TOGETHER = 4;
-    __shared__ float4 sums[WAVES][64];
-    __shared__ float2 weights[WAVES][64];                // largest level, sum of weights
     const int quads = a.columns / 4, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t i = int64_t(blockIdx.x) * 64 + lane, last = all_rows * quads - 1, at = (i < last ? i : last) / quads;
+    const int64_t i = SHARES == 1 ? int64_t(blockIdx.x) * WG + threadIdx.x : int64_t(blockIdx.x) * 64 + lane, last = all_rows * quads - 1, at = (i < last ? i : last) / quads;
     const int col = int((i < last ? i : last) - at * quads) * 4;
     float most = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int first = wave; first < a.splits; first += WAVES * TOGETHER) {
+    for (int first = SHARES == 1 ? 0 : wave; first < a.splits; first += SHARES * TOGETHER) {
         float l[TOGETHER], now = most;
         float4 v[TOGETHER];
 #pragma unroll
         for (int n = 0; n < TOGETHER; ++n) {
-            const int64_t s = min(first + n * WAVES, a.splits - 1);
+            const int64_t s = min(first + n * SHARES, a.splits - 1);
             l[n] = a.part_lse[s * all_rows + at];
             v[n] = *reinterpret_cast<const float4 *>(a.part + (s * all_rows + at) * a.columns + col);
         }
 #pragma unroll
         for (int n = 0; n < TOGETHER; ++n) {
-            if (first + n * WAVES >= a.splits || l[n] == INFINITY) l[n] = -INFINITY, v[n] = make_float4(0.f, 0.f, 0.f, 0.f);      // (no key that takes part)
+            if (first + n * SHARES >= a.splits || l[n] == INFINITY) l[n] = -INFINITY, v[n] = make_float4(0.f, 0.f, 0.f, 0.f);      // (no key that takes part)
             now = fmaxf(now, l[n]);
         }
         const float less = now == -INFINITY ? 0.f : now, by = __builtin_amdgcn_exp2f(most - less);
@@ -162,24 +303,29 @@ __global__ __launch_bounds__(WG) void join_kernel(FwdArgs a, int64_t all_rows) {
         }
         most = now;
     }
-    sums[wave][lane] = acc;
-    weights[wave][lane] = make_float2(most, sum);
-    __syncthreads();
-    if (wave != 0 || i > last) return;
-    float all = -INFINITY;
+    float less = most == -INFINITY ? 0.f : most;
+    if constexpr (SHARES > 1) {
+        __shared__ float4 sums[SHARES][64];
+        __shared__ float2 weights[SHARES][64];           // largest level, sum of weights
+        sums[wave][lane] = acc;
+        weights[wave][lane] = make_float2(most, sum);
+        __syncthreads();
+        if (wave != 0) return;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) all = fmaxf(all, weights[w][lane].x);
-    const float less = all == -INFINITY ? 0.f : all;
-    sum = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 1; w < SHARES; ++w) most = fmaxf(most, weights[w][lane].x);
+        less = most == -INFINITY ? 0.f : most;
+        sum = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const float2 m = weights[w][lane];
-        const float4 v = sums[w][lane];
-        const float by = __builtin_amdgcn_exp2f(m.x - less);
-        sum = fmaf(by, m.y, sum);
-        acc.x = fmaf(by, v.x, acc.x), acc.y = fmaf(by, v.y, acc.y), acc.z = fmaf(by, v.z, acc.z), acc.w = fmaf(by, v.w, acc.w);
+        for (int w = 0; w < SHARES; ++w) {
+            const float2 m = weights[w][lane];
+            const float4 v = sums[w][lane];
+            const float by = __builtin_amdgcn_exp2f(m.x - less);
+            sum = fmaf(by, m.y, sum);
+            acc.x = fmaf(by, v.x, acc.x), acc.y = fmaf(by, v.y, acc.y), acc.z = fmaf(by, v.z, acc.z), acc.w = fmaf(by, v.w, acc.w);
+        }
     }
+    if (i > last) return;
     const float by = sum == 0.f ? 0.f : 1.f / sum;
     const int bh = int(at / a.rows), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, row = int(at - int64_t(bh) * a.rows);
     if (a.lse && col == 0) a.lse[at] = sum == 0.f ? INFINITY : less + __builtin_amdgcn_logf(sum);
@@ -215,8 +361,17 @@ __attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(co
 
 namespace {
 
+constexpr int64_t COMPUTE_UNITS = 256;    // a tile each and more: the keys are not shared out
 constexpr int64_t WANTED = 512;           // workgroups, where there are keys enough to share out
 constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
+
+constexpr int64_t FEW_WANTED = 4096;      // few_rows_kernel: wavefronts
+
+// Lanes that have a key in few_rows_kernel.
+int lanes_of_a_key(const lffn_cross_attention &c) {
+    const int lanes = int(c.columns) * (c.format == LFFN_ROWS_F32 ? 4 : 2) / 16;
+    return lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
+}
 
 // Fills sizes in; the workspace's bytes, or -1: too many tiles.
 int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
@@ -235,8 +390,15 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     a.steps = (c.k_len + kt - 1) / kt;
     a.c = c.scale * LOG2E;
     const int64_t tiles = c.B * c.key_heads * a.row_tiles;
-    int64_t splits = tiles > 0 && tiles < WANTED ? (WANTED + tiles - 1) / tiles : 1;
+    int64_t splits = tiles > 0 && tiles < COMPUTE_UNITS ? (WANTED + tiles - 1) / tiles : 1;
     if (splits > a.steps / LEAST_STEPS) splits = a.steps / LEAST_STEPS;
+    if (a.rows <= few_rows(c.format == LFFN_ROWS_F32)) {
+        const int64_t at_once = 64 / lanes_of_a_key(c) * FEW_TOGETHER, rounds = (c.k_len + at_once - 1) / at_once;
+        a.few_waves = int(rounds < 1 ? 1 : rounds < FEW_WAVES ? rounds : FEW_WAVES);
+        a.steps = c.k_len;
+        splits = tiles > 0 ? FEW_WANTED / (tiles * a.few_waves) : 1;
+        if (splits > rounds / a.few_waves) splits = rounds / a.few_waves;
+    }
     if (splits < 1) splits = 1;
     a.split_steps = (a.steps + splits - 1) / splits;
     a.splits = a.split_steps ? int((a.steps + a.split_steps - 1) / a.split_steps) : 1;
@@ -247,16 +409,41 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     return a.splits > 1 ? int64_t(a.splits) * c.B * c.key_heads * a.rows * (a.columns + 1) * 4 : 0;
 }
 
+template <typename F>
+void join(const FwdArgs &a, hipStream_t stream) {
+    const int64_t rows = int64_t(a.units / (a.splits * a.row_tiles)) * a.rows, quads = rows * (a.columns / 4);
+    if (a.splits > 4) join_kernel<F, WAVES><<<dim3((unsigned)((quads + 63) / 64)), dim3(WG), 0, stream>>>(a, rows);
+    else join_kernel<F, 1><<<dim3((unsigned)((quads + WG - 1) / WG)), dim3(WG), 0, stream>>>(a, rows);
+}
+
+template <typename F, typename R, int G>
+int launch_few(const FwdArgs &a, hipStream_t stream) {
+    const dim3 grid((unsigned)a.units), block(64 * a.few_waves);
+    if (a.rows == 1) few_rows_kernel<R, F, G, 1><<<grid, block, 0, stream>>>(a);
+    else if (a.rows == 2) few_rows_kernel<R, F, G, 2><<<grid, block, 0, stream>>>(a);
+    else few_rows_kernel<R, F, G, 4><<<grid, block, 0, stream>>>(a);
+    if (a.splits > 1) join<F>(a, stream);
+    return lffn_launch_status();
+}
+
+template <typename F, typename R>
+int launch_few(const FwdArgs &a, int lanes, hipStream_t stream) {
+    switch (lanes) {
+        case 4: return launch_few<F, R, 4>(a, stream);
+        case 8: return launch_few<F, R, 8>(a, stream);
+        case 16: return launch_few<F, R, 16>(a, stream);
+        default: if constexpr (R::N == 4) return launch_few<F, R, 32>(a, stream);
+    }
+    return LFFN_ERR_UNSUPPORTED;          // (16-bit heads have at most 128 columns)
+}
+
 template <typename F, int DP, int KT>
 int launch(const FwdArgs &a, hipStream_t stream) {
     static LdsGrant granted;
     const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + BLOCK * 8;
     if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&cross_attention_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
     cross_attention_kernel<F, DP, KT><<<dim3((unsigned)a.units), dim3(WG), bytes, stream>>>(a);
-    if (a.splits > 1) {
-        const int64_t rows = int64_t(a.units / (a.splits * a.row_tiles)) * a.rows;
-        join_kernel<F><<<dim3((unsigned)((rows * (a.columns / 4) + 63) / 64)), dim3(WG), 0, stream>>>(a, rows);
-    }
+    if (a.splits > 1) join<F>(a, stream);
     return lffn_launch_status();
 }
 
@@ -291,6 +478,11 @@ extern "C" int lffn_cross_attention_fwd(const lffn_cross_attention *c, void *out
     a.part = static_cast<float *>(workspace);
     a.part_lse = a.part ? a.part + int64_t(a.splits) * c->B * c->key_heads * a.rows * a.columns : nullptr;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a.few_waves) {
+        const int lanes = lanes_of_a_key(*c);
+        if (c->format == LFFN_ROWS_F32) return launch_few<F32, F32Row>(a, lanes, s);
+        return c->format == LFFN_ROWS_BF16 ? launch_few<BF16, BF16Row>(a, lanes, s) : launch_few<F16, F16Row>(a, lanes, s);
+    }
     if (c->format == LFFN_ROWS_F32) return launch<F32>(a, s);
     return c->format == LFFN_ROWS_BF16 ? launch<BF16>(a, s) : launch<F16>(a, s);
 }

@@ -377,6 +377,7 @@ __global__ __launch_bounds__(WG) void add_splits_kernel(AddArgs a) {
               acc.w);
 }
 
+constexpr int64_t COMPUTE_UNITS = 256;    // standing tiles, and more: what passes is not shared out
 constexpr int64_t WANTED = 512;           // workgroups, where there is enough to share out
 constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
 
@@ -390,7 +391,7 @@ void share_out(BwdArgs &a, int64_t standing, int64_t passing, int kt, int64_t ba
     a.tiles = int((standing + TILE - 1) / TILE);
     a.steps = (passing + kt - 1) / kt;
     const int64_t tiles = batch_heads * a.tiles;
-    int64_t splits = tiles > 0 && tiles < WANTED ? (WANTED + tiles - 1) / tiles : 1;
+    int64_t splits = tiles > 0 && tiles < COMPUTE_UNITS ? (WANTED + tiles - 1) / tiles : 1;
     if (splits > a.steps / LEAST_STEPS) splits = a.steps / LEAST_STEPS;
     if (splits < 1) splits = 1;
     a.split_steps = (a.steps + splits - 1) / splits;
