@@ -225,6 +225,28 @@ struct Tile {
     }
 };
 
+// N products, product i with the operand that load(i) reads from LDS, AHEAD operands asked for ahead of the one that is used: left to itself the compiler asks for
+// one, waits for it, and asks for the next (keys' gradients of 4 x 2048 to 4096 x 16 x 128 bfloat16, in pairs: see there).
+template <typename F, int N, bool ORDERED = true, typename L, typename M>
+__device__ __forceinline__ void products(L &&load, M &&multiply) {
+    if constexpr (!ORDERED) {
+        static_for<N>([&](auto i) { multiply(i, load(i)); });
+        return;
+    }
+    constexpr int MOST = F::PLANES == 1 ? 4 : 2, AHEAD = N < MOST ? N : MOST, ORDER = 0x406;        // (what may pass: the vector and scalar ALU)
+    Frag<F::PLANES> f[AHEAD];
+    static_for<AHEAD>([&](auto i) { f[i] = load(i); });
+    __builtin_amdgcn_sched_barrier(ORDER);
+    static_for<N>([&](auto i) {
+        multiply(i, f[i % AHEAD]);
+        __builtin_amdgcn_sched_barrier(ORDER);
+        if constexpr (i + AHEAD < N) {
+            f[i % AHEAD] = load(std::integral_constant<int, i + AHEAD>{});
+            __builtin_amdgcn_sched_barrier(ORDER);
+        }
+    });
+}
+
 // Operand layout of a wavefront's own 32 rows straight from memory: 16 columns `chunk` of the lane's row (8 of them, by half), zeros beyond the row.
 template <typename F>
 __device__ __forceinline__ Frag<F::PLANES> own_rows(const char *row, bool live, int chunk, int half, int pieces) {

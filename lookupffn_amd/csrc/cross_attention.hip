@@ -33,7 +33,7 @@ constexpr int FEW_TOGETHER = 2;           // keys of a group of lanes asked for 
 constexpr float SLACK = 6.f;              // how far (powers of two) a row's largest score may outgrow the one that its sums go by
 
 template <typename F, int DP, int KT>
-__global__ __launch_bounds__(WG, DP <= 64 ? 3 : F::PLANES == 1 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
+__global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F::PLANES == 1 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
     typedef Tile<F, DP, KT> T;
     typedef Frag<F::PLANES> Op;
     constexpr int CHUNKS = DP / 16, KB = KT / 32, DB = DP / 32;
@@ -65,10 +65,8 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 3 : F::PLANES == 1 ? 2 : 1) void cro
         if (!wave_works) return;
         constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
         ca_f32x16_t s[KB] = {};
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) s[kb] = F::mma(read.rows(KEYS, kb, c), fq[c], s[kb]);
+        products<F, KB * CHUNKS, F::PLANES == 1>([&](auto i) { return read.rows(KEYS, i % KB, i / KB); },
+                                 [&](auto i, const Op &k) { s[i % KB] = F::mma(k, fq[i / KB], s[i % KB]); });
         constexpr uint64_t FULL = ~0ull >> (64 - KT);
         if (word != FULL) {
 #pragma unroll
@@ -95,6 +93,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 3 : F::PLANES == 1 ? 2 : 1) void cro
             most = to;
         }
         const float less = (most == -INFINITY ? 0.f : most) * a.c - F::LIFT;
+        Op p[2 * KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -107,11 +106,11 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 3 : F::PLANES == 1 ? 2 : 1) void cro
                 float t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = s[kb][8 * c + e];
-                const Op p = F::operand(t);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = F::mma(read.columns(VALUES, 2 * kb + c, d), p, o[d]);
+                p[2 * kb + c] = F::operand(t);
             }
         }
+        products<F, 2 * KB * DB, F::PLANES == 1>([&](auto i) { return read.columns(VALUES, i / DB, i % DB); },
+                                 [&](auto i, const Op &v) { o[i % DB] = F::mma(v, p[i / DB], o[i % DB]); });
     };
 
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;

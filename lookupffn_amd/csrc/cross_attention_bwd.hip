@@ -165,11 +165,10 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             ca_f32x16_t s = {}, dp = {};
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                s = F::mma(read.rows(KEYS, kb, c), fq[c], s);
-                dp = F::mma(read.rows(VALUES, kb, c), fg[c], dp);
-            }
+            products<F, 2 * CHUNKS>([&](auto i) { return read.rows(i % 2 ? VALUES : KEYS, kb, i / 2); }, [&](auto i, const Op &x) {
+                if constexpr (i % 2) dp = F::mma(x, fg[i / 2], dp);
+                else s = F::mma(x, fq[i / 2], s);
+            });
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -level)) * fmaf(dp[e], f, -delta);
             const uint32_t part = (uint32_t)(word >> (32 * kb));
@@ -179,15 +178,16 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
                 for (int e = 0; e < 16; ++e)
                     if (!(w >> (8 * (e / 4) + e % 4) & 1)) s[e] = 0.f;
             }
+            Op ds[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = s[8 * c + e];
-                const Op ds = F::operand(t);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) dq[d] = F::mma(read.columns(KEYS, 2 * kb + c, d), ds, dq[d]);
+                ds[c] = F::operand(t);
             }
+            products<F, 2 * DB>([&](auto i) { return read.columns(KEYS, 2 * kb + i / DB, i % DB); },
+                                [&](auto i, const Op &x) { dq[i % DB] = F::mma(x, ds[i / DB], dq[i % DB]); });
         }
     };
 
@@ -271,12 +271,10 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             ca_f32x16_t s = {}, dp = {};
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) s = F::mma(read.rows(QUERIES, rb, c), fk[c], s);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) dp = F::mma(read.rows(GRADIENTS, rb, c), fv[c], dp);
-            __builtin_amdgcn_sched_barrier(0);
+            products<F, 2 * CHUNKS>([&](auto i) { return read.rows(i % 2 ? GRADIENTS : QUERIES, rb, i / 2); }, [&](auto i, const Op &x) {
+                if constexpr (i % 2) dp = F::mma(x, fv[i / 2], dp);
+                else s = F::mma(x, fk[i / 2], s);
+            });
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const float4 l = *reinterpret_cast<const float4 *>(level + rb * 32 + 8 * g), d = *reinterpret_cast<const float4 *>(delta + rb * 32 + 8 * g);
@@ -296,17 +294,10 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
                 for (int e = 0; e < 8; ++e) t[e] = s[8 * c + e], u[e] = dp[8 * c + e];
                 p[c] = F::operand(t), ds[c] = F::operand(u);
             }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) dv[d] = F::mma(read.columns(GRADIENTS, 2 * rb + c, d), p[c], dv[d]);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) dk[d] = F::mma(read.columns(QUERIES, 2 * rb + c, d), ds[c], dk[d]);
-            __builtin_amdgcn_sched_barrier(0);
+            products<F, 4 * DB>([&](auto i) { return read.columns(i % 2 ? QUERIES : GRADIENTS, 2 * rb + i / 2 / DB, i / 2 % DB); }, [&](auto i, const Op &x) {
+                if constexpr (i % 2) dk[i / 2 % DB] = F::mma(x, ds[i / 2 / DB], dk[i / 2 % DB]);
+                else dv[i / 2 % DB] = F::mma(x, p[i / 2 / DB], dv[i / 2 % DB]);
+            });
         }
     };
 
@@ -347,6 +338,201 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
     }
 }
 
+// The same with two wavefronts a block of 32 keys: one forms the weights and the values' gradient, the other ds and the keys' gradient, and the weights go from one
+// to the other through LDS, in fp32.  Each has half of the operands and sums (128 columns: 96 registers for 192), so that two fit on a SIMD, the one's
+// exponentials beside the other's products; with all in one wavefront a SIMD has one, which waits for itself (4 x 2048 to 4096 x 16 x 128 bfloat16: 758 us).
+// Between two barriers: the weights' products with a step of 32 rows and the scores of the next one, whose rows are there, while those of the one after
+// are on their way (three buffers).
+template <typename F, int DP, int ROLE>
+__device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *const lds) {
+    constexpr bool OF_V = ROLE == 0;
+    constexpr int KT = 32, THREADS = 2 * WG, BUFFERS = 3, CHUNKS = DP / 16, DB = DP / 32;
+    typedef Tile<F, DP, KT> T;
+    typedef Frag<F::PLANES> Op;
+    constexpr int SHARE = 2 * T::PLANE / THREADS;        // of the pieces of a step's rows and their gradients
+    static_assert(SHARE >= 1 && T::PLANE % 64 == 0, "a wavefront's pieces are of one tile");
+    float4 *const handed = reinterpret_cast<float4 *>(lds + BUFFERS * 2 * T::SIZE);
+    float *const levels = reinterpret_cast<float *>(handed + BUFFERS * WAVES * 256);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave & 3;
+    const int r = lane & 31, half = lane >> 5;
+    const Unit unit = unit_of(blockIdx.x, a.units, a.tile_by, a.split_by, a.heads);
+    const int tile = unit.tile, split = unit.split, bh = unit.bh, b = unit.b, kh = unit.kh;
+    const int pieces = a.columns / 8;
+    const int64_t key = int64_t(tile) * TILE + pair * ROWS + r;
+    const bool in = key < a.keys;
+    const int64_t at_key = in ? key : a.keys - 1;
+    const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
+    // whether the tile's keys take part: every wavefront looks at all 128
+    uint64_t flags[2] = {~0ull, ~0ull};
+    if (a.mask) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t k = int64_t(tile) * TILE + 64 * i + lane;
+            flags[i] = __ballot(a.mask[b * a.mask_stride + (k < a.keys ? k : a.keys - 1)] != 0 && k < a.keys);
+        }
+    }
+    constexpr bool HALF = F::LIFT != 0.f;
+    const int lift = ds_exponent<F>(a, bh);
+    const float f = __builtin_amdgcn_ldexpf(1.f, HALF ? lift - int(P_LIFT) : 0);
+    Op own[CHUNKS];                       // the weights' wavefront: keys; the other: values
+    {
+        const char *const p = OF_V ? a.k + b * a.kb + kh * a.kh + at_key * a.kt : a.v + b * a.vb + kh * a.vh + at_key * a.vt;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) own[c] = own_rows<F>(p, true, c, half, pieces);
+    }
+
+    const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
+    const int64_t g_token = int64_t(a.key_heads) * a.group.by * a.columns * F::BYTES;
+    const char *const gp = a.g + (b * a.q_len * g_token + kh * a.group.by * a.columns * F::BYTES);
+    typename F::Raw raw[F::PLANES == 1 ? 1 : SHARE];
+    float level = 0.f, delta = 0.f;
+    // piece i of the thread: of tile (0: rows, 1: gradients), row and place in memory
+    auto piece_of = [&](int i, int &of, int &row, int &place) {
+        const int p = tid + THREADS * i, q = p % T::PLANE;
+        of = p / T::PLANE, row = q / T::PIECES, place = q % T::PIECES;
+        if constexpr (F::PLANES == 1) place ^= T::turned(row);
+    };
+    auto ask = [&](int buf, int64_t step) {
+        const int first = int(step) * KT, token = a.group.quotient(first);
+        const char *const q_base = rows.base + token * a.qt, *const g_base = gp + token * g_token;
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+            int of, at, place;
+            piece_of(i, of, at, place);
+            const int row = min(first + at, a.rows - 1), t = a.group.quotient(row), h = row - t * a.group.by;
+            const uint32_t column = (place < pieces ? place : 0) * 8 * F::BYTES;
+            const uint32_t offset = (t - token) * (of ? (uint32_t)g_token : (uint32_t)a.qt) + h * (of ? (uint32_t)(a.columns * F::BYTES) : (uint32_t)a.qh) + column;
+            const bool of_g = __builtin_amdgcn_readfirstlane(of);
+            const char *const base = of_g ? g_base : q_base;
+            if constexpr (F::PLANES == 1) {
+                const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (buf * 2 * T::SIZE + i * THREADS + wave * 64) * 16;
+                copy_to_lds(base, offset, __builtin_amdgcn_readfirstlane(to));
+            } else {
+                raw[i] = F::load(base + offset);
+            }
+        }
+        const int64_t of_row = int64_t(bh) * a.rows + min(first + tid % KT, a.rows - 1);
+        level = a.lse[of_row];
+        delta = a.delta[of_row];
+    };
+    auto placed = [&](int buf, int64_t step) {
+        if (tid < KT) {
+            const bool on = int(step) * KT + tid < a.rows;
+            levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
+            levels[buf * 2 * KT + KT + tid] = on ? delta * f : 0.f;
+        }
+        if constexpr (F::PLANES == 1) {
+            arrived();
+        } else {
+#pragma unroll
+            for (int i = 0; i < SHARE; ++i) {
+                int of, at, place;
+                piece_of(i, of, at, place);
+                T::put(lds + (buf * 2 + of) * T::SIZE, at, place, raw[i]);
+            }
+        }
+    };
+
+    const typename T::Reader read(lds, lane);
+    ca_f32x16_t sums[DB] = {}, s;
+    Op p[2];
+    // scores and weights, or g . v, of a step
+    auto first_half = [&](auto buf) {
+        constexpr int QUERIES = decltype(buf)::value * 2 * T::SIZE, GRADIENTS = QUERIES + T::SIZE;
+        s = ca_f32x16_t{};
+        if constexpr (OF_V) {
+            products<F, CHUNKS>([&](auto i) { return read.rows(QUERIES, 0, i); }, [&](auto i, const Op &x) { s = F::mma(x, own[i], s); });
+            float4 *const to = handed + (decltype(buf)::value * WAVES + pair) * 256 + lane;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 l = *reinterpret_cast<const float4 *>(levels + decltype(buf)::value * 2 * KT + 8 * g + 4 * half);
+                const float ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.c, -ls[e]));
+                to[g * 64] = make_float4(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
+            }
+        } else {
+            products<F, CHUNKS>([&](auto i) { return read.rows(GRADIENTS, 0, i); }, [&](auto i, const Op &x) { s = F::mma(x, own[i], s); });
+        }
+    };
+    // the products with them
+    auto second_half = [&](auto buf) {
+        constexpr int QUERIES = decltype(buf)::value * 2 * T::SIZE, GRADIENTS = QUERIES + T::SIZE;
+        if constexpr (!OF_V) {
+            const float4 *const from = handed + (decltype(buf)::value * WAVES + pair) * 256 + lane;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 w = from[g * 64], d = *reinterpret_cast<const float4 *>(levels + decltype(buf)::value * 2 * KT + KT + 8 * g + 4 * half);
+                const float ws[4] = {w.x, w.y, w.z, w.w}, ds[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * g + e] = ws[e] * fmaf(s[4 * g + e], f, -ds[e]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float t[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = s[8 * c + e];
+            p[c] = F::operand(t);
+        }
+        if constexpr (OF_V) {
+            products<F, 2 * DB>([&](auto i) { return read.columns(GRADIENTS, i / DB, i % DB); },
+                                [&](auto i, const Op &x) { sums[i % DB] = F::mma(x, p[i / DB], sums[i % DB]); });
+        } else {
+            products<F, 2 * DB>([&](auto i) { return read.columns(QUERIES, i / DB, i % DB); },
+                                [&](auto i, const Op &x) { sums[i % DB] = F::mma(x, p[i / DB], sums[i % DB]); });
+        }
+    };
+
+    if (begin < end) ask(0, begin);
+    const bool live = in && (flags[pair >> 1] >> (32 * (pair & 1) + r) & 1), wave_works = __any(live), works = (flags[0] | flags[1]) != 0;
+    if (begin < end) placed(0, begin);
+    if (works && begin < end) {
+        __syncthreads();
+        if (begin + 1 < end) ask(1, begin + 1);
+        if (wave_works) first_half(std::integral_constant<int, 0>{});
+        int64_t step = begin;
+        // a step whose scores are there: in buffer `now`, the next step's rows on their way to `next`
+        auto body = [&](auto now, auto next, auto behind) {
+            const bool more = step + 1 < end;
+            if (more) placed(decltype(next)::value, step + 1);
+            __syncthreads();
+            if (step + 2 < end) ask(decltype(behind)::value, step + 2);
+            if (wave_works) {
+                second_half(now);
+                if (more) first_half(next);
+            }
+            ++step;
+            return more;
+        };
+        const std::integral_constant<int, 0> zero;
+        const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 2> two;
+#pragma unroll 1
+        while (body(zero, one, two) && body(one, two, zero) && body(two, zero, one)) {
+        }
+    }
+    if (!live) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) sums[d] = ca_f32x16_t{};
+    }
+    const float by = OF_V ? (HALF ? 1.f / 16384.f : 1.f) : __builtin_amdgcn_ldexpf(a.scale, -lift);
+    if (a.splits > 1) {
+        const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key + (OF_V ? a.splits * all : 0)) * a.columns;
+        store_row<F32, DB>(sums, by, reinterpret_cast<char *>(a.part + of), in, a.columns, half);
+    } else {
+        store_row<F, DB>(sums, by, (OF_V ? a.gv : a.gk) + ((b * a.keys + key) * a.key_heads + kh) * a.columns * F::BYTES, in, a.columns, half);
+    }
+}
+
+template <typename F, int DP>
+__global__ __launch_bounds__(2 * WG, 2) void key_gradient_pairs_kernel(BwdArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint4 lds[];           // [3][rows, their gradients], [3][4] weights, [3][levels, deltas]
+    // (whole wavefronts go either way, and either way has the same barriers in the same order)
+    if (__builtin_amdgcn_readfirstlane(threadIdx.x) < WG) key_gradient_pairs<F, DP, 0>(a, lds);
+    else key_gradient_pairs<F, DP, 1>(a, lds);
+}
+
 // The splits' sums of a row as one, in their order, four of them asked for together; `second` beside `part` where there are two arrays.  Four columns a lane.
 struct AddArgs {
     const float *part[2];
@@ -376,6 +562,9 @@ __global__ __launch_bounds__(WG) void add_splits_kernel(AddArgs a) {
     F::store4(a.out[blockIdx.y] + (heads_row(b, kh, int(at - int64_t(bh) * a.rows), a.len, a.heads.by, a.group) * a.columns + col) * F::BYTES, acc.x, acc.y, acc.z,
               acc.w);
 }
+
+// Which form of the keys' gradients heads of so many columns get.
+constexpr bool in_pairs(int planes, int columns) { return planes == 1 ? columns > 64 : columns > 32 && columns <= 64; }
 
 constexpr int64_t COMPUTE_UNITS = 256;    // standing tiles, and more: what passes is not shared out
 constexpr int64_t WANTED = 512;           // workgroups, where there is enough to share out
@@ -422,7 +611,7 @@ Plan plan(const lffn_cross_attention &c) {
     a.norm_tiles = Divisor(a.g_tiles + a.v_tiles > 0 ? uint32_t(a.g_tiles + a.v_tiles) : 1);
     p.q = p.k = a;
     share_out(p.q, a.rows, a.keys, kt, batch_heads);
-    share_out(p.k, a.keys, a.rows, kt, batch_heads);
+    share_out(p.k, a.keys, a.rows, in_pairs(c.format == LFFN_ROWS_F32 ? 3 : 1, int(c.columns)) ? 32 : kt, batch_heads);
     auto take = [&](int64_t floats) {
         const int64_t at = p.floats;
         p.floats += (floats + 3) / 4 * 4;
@@ -458,9 +647,15 @@ int launch(const Plan &p, hipStream_t stream) {
     }
     if (p.k.units > 0) {
         static LdsGrant granted;
-        const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + 4 * KT * 4;
-        if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&key_gradient_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
-        key_gradient_kernel<F, DP, KT><<<dim3((unsigned)p.k.units), dim3(WG), bytes, stream>>>(p.k);
+        if constexpr (in_pairs(F::PLANES, DP)) {
+            const size_t bytes = 3 * (2 * Tile<F, DP, 32>::SIZE * 16 + WAVES * 4096 + 2 * 32 * 4);
+            if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&key_gradient_pairs_kernel<F, DP>), bytes, granted)) return LFFN_ERR_LAUNCH;
+            key_gradient_pairs_kernel<F, DP><<<dim3((unsigned)p.k.units), dim3(2 * WG), bytes, stream>>>(p.k);
+        } else {
+            const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + 4 * KT * 4;
+            if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&key_gradient_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
+            key_gradient_kernel<F, DP, KT><<<dim3((unsigned)p.k.units), dim3(WG), bytes, stream>>>(p.k);
+        }
         const BwdArgs &k = p.k;
         const int64_t all = int64_t(k.batch_heads) * k.keys;
         if (k.splits > 1)
