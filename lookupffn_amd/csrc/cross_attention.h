@@ -52,6 +52,13 @@ __device__ __forceinline__ void split3(const float (&v)[8], uint4 (&t)[3]) {
     for (int k = 0; k < 3; ++k) t[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
 }
 
+// f of a lane's number and of that of the lane 32 away, on the vector ALU (an LDS permute is waited for).
+template <typename T>
+__device__ __forceinline__ float of_both_halves(float v, T &&f) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 struct BF16 {
     static constexpr int PLANES = 1, BYTES = 2;
     static constexpr float LIFT = 0.f;                 // added to the exponents of the softmax's weights

@@ -82,7 +82,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F:
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) now = fmaxf(now, s[kb][e]);
-        now = fmaxf(now, lane_xor<32>(now));
+        now = of_both_halves(now, [](float x, float y) { return fmaxf(x, y); });
         if (__any((now - most) * a.c > SLACK)) {             // (the first step's is: most is -infinity; -infinity - itself is no number, and not above)
             const float to = fmaxf(most, now), by = most == to ? 1.f : __builtin_amdgcn_exp2f(most * a.c - to * a.c);
             sum *= by;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F:
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
 
-    sum += lane_xor<32>(sum);
+    sum = of_both_halves(sum, [](float x, float y) { return x + y; });
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query without keys: zeros
     const float level = sum == 0.f ? INFINITY : (most == -INFINITY ? 0.f : most) * a.c - F::LIFT + __builtin_amdgcn_logf(sum);
     const bool live = row < a.rows;
