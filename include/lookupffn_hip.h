@@ -929,8 +929,9 @@ int lffn_qk_norm_rotary_bwd(const lffn_qk_norm_rotary *a, const void *g_q, const
  * Attention of queries to keys and values of another length, key_heads <= heads (heads / key_heads neighbouring query heads share a key head):
  *   out[b, i, h] = sum_j p_j v[b, j, h'],  p = softmax_j(scale q[b, i, h] . k[b, j, h'])  over the keys that take part.
  * q: [B, q_len, heads, columns], k, v: [B, k_len, key_heads, columns], by strides (elements) of batch, token and head, multiples of 16 bytes,
- * as are the addresses; columns lie together, a multiple of 8, at most 128.  key_mask: [B, k_len] bytes, not 0 where a key takes part, with a
- * batch stride, or NULL.  Keys and values that take no part are not read.  A query without keys gets zeros.  scale: positive, finite.
+ * as are the addresses; 128 tokens and the heads of a key head lie within 32 bits (token strides below 2^25 bytes, q's head stride times the heads that share a
+ * key head below 2^30); columns lie together, a multiple of 8, at most 128.  key_mask: [B, k_len] bytes, not 0 where a key takes part, with a
+ * batch stride, or NULL.  What keys and values that take no part hold does not matter.  A query without keys gets zeros.  scale: positive, finite.
  * format 0: fp32 accuracy, 1 and 2: products of 16 bits, sums in fp32, softmax weights rounded to the format.
  * out: [B, q_len, heads, columns], in the format.  lse: [B, key_heads, q_len * heads / key_heads] or NULL, what the backward needs of a row
  * (private to it).  workspace: 16-byte aligned, of lffn_cross_attention_workspace_bytes (0: may be NULL).

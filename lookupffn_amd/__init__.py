@@ -12,11 +12,11 @@ from .gather import (LookupGather, WeightedVectorGatherAdd, gather, indexed_inne
                      weighted_gather_add, weighted_vector_gather_add, weighted_vector_scatter_add)
 from .cross_attention import CrossAttentionFunction, QkNormRotary, cross_attention, qk_norm_rotary, rotary_table
 from .lookup import BH4, Hashing, LookupFFN
-from .encoder import Attention, Encoder, EncoderLayer, Lookup, RobertaEmbeddings
+from .encoder import Attention, CrossAttention, Encoder, EncoderLayer, Lookup, RobertaEmbeddings
 
 __all__ = [
     "BH4", "Hashing", "LookupFFN",
-    "Attention", "EncoderLayer", "Encoder", "Lookup", "RobertaEmbeddings",
+    "Attention", "CrossAttention", "EncoderLayer", "Encoder", "Lookup", "RobertaEmbeddings",
     "bh4", "bh4_cuda", "hadamard", "hadamard_transform", "fast_hadamard_transform",
     "FastHadamardTransform", "FastHadamardTransformDim512", "FastHadamardTransformDim1024",
     "compute_code_score", "compute_code_score_torch", "bin2dec", "ComputeCodeScore",

@@ -152,7 +152,7 @@ def cross_attention(q, k, v, key_mask=None, *, scale=None):
 
     q: [B, L, heads, columns], k, v: [B, keys, key heads, columns], of one type, with any strides (as for ``qk_norm_rotary``); heads a multiple of
     key heads, neighbouring query heads share one.  columns: a multiple of 8, at most 128.  key_mask: [B, keys] bool, True where a key takes part, or
-    None; keys and values that take no part are not read, whatever they hold.  A query without keys gets zeros (and gives none a gradient).
+    None; whatever keys and values that take no part hold.  A query without keys gets zeros (and gives none a gradient).
     scale: positive, 1 / sqrt(columns) if None.  One query a sequence is the step of a decoder over kept keys and values.
 
     float32: products of three bfloat16 terms a number, sums in float32, as exact as a float32 product; 16 bits: softmax weights rounded to the

@@ -3,7 +3,7 @@
 // A workgroup has 128 rows (queries of the heads that share a key head), 32 a wavefront, and walks the keys 64 at a time with the running maximum and
 // sum of a softmax taken in one pass.  Keys and values are fetched a step ahead and lie in LDS as in memory, in two buffers; scores are
 // formed as keys x queries, weights times values as (values turned round) x weights.  Steps without a key that takes part are left out, masked
-// keys and values are zeros that nobody fetched.  Where there are too few rows to fill the chip the keys are shared out over several workgroups,
+// keys and values are the step's first that takes part once more.  Where there are too few rows to fill the chip the keys are shared out over several workgroups,
 // whose results a second kernel joins.
 #include "cross_attention.h"
 

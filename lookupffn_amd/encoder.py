@@ -4,6 +4,7 @@ of src/roberta/models/postnorm.py:6-28), with the same module and parameter
 names so that a reference state_dict loads unchanged.  ``LookupFFN`` and, without
 gradients, the attention's products and softmax run on the gfx950 kernels of this
 package; embeddings, LayerNorms and the attention in training are plain PyTorch-ROCm.
+``CrossAttention`` reads the encoder's states from another sequence, with and without gradients.
 
 ``config`` carries the attributes the reference reads: hidden_size,
 num_attention_heads, attention_head_size, attention_probs_dropout_prob,
@@ -20,6 +21,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 from . import ops
+from .cross_attention import cross_attention, qk_norm_rotary, rotary_table
 from .lookup import LookupFFN
 
 _GLOBAL_HOOKS = torch.nn.modules.module
@@ -171,6 +173,67 @@ class Attention(nn.Module):
 # What the kernels stand in for: a class or a module with another one has it called.
 _FORWARDS[Attention] = Attention.forward
 _OWN_METHODS = tuple((name, getattr(Attention, name)) for name in ("attention", "transpose_for_scores", "_attend"))
+
+
+class CrossAttention(nn.Module):
+    """Pre-norm attention of a sequence to the states of an encoder, of another length (nothing in the reference, whose encoder has no reader): LayerNorm of
+    the hidden states, queries from them, keys and values from the states, norms of queries and keys for each head, with ``rotary_columns`` the rotation to
+    their positions, softmax over the states that take part, output projection.  Forward and backward on this package's kernels
+    (``qk_norm_rotary``, ``cross_attention``) in float32 and, under autocast, 16 bits.
+
+    ``config`` as for ``Attention``, optionally num_key_value_heads (fewer than query heads), encoder_hidden_size (of the states) and rotary_columns
+    (0: no rotation; positions up to max_position_embeddings).  The weights of the softmax have no dropout: attention_probs_dropout_prob is not read."""
+
+    def __init__(self, config):
+        super().__init__()
+        self.num_attention_heads = config.num_attention_heads
+        self.num_key_value_heads = getattr(config, "num_key_value_heads", None) or config.num_attention_heads
+        self.attention_head_size = config.attention_head_size
+        self.qk_norm_eps = config.layer_norm_eps
+        all_heads, key_heads = self.num_attention_heads * self.attention_head_size, self.num_key_value_heads * self.attention_head_size
+        states = getattr(config, "encoder_hidden_size", None) or config.hidden_size
+
+        self.LayerNorm = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_eps)
+        self.query = nn.Linear(config.hidden_size, all_heads)
+        self.key = nn.Linear(states, key_heads)
+        self.value = nn.Linear(states, key_heads)
+        self.dense = nn.Linear(all_heads, config.hidden_size)
+        self.query_norm = nn.Parameter(torch.ones(self.attention_head_size))
+        self.key_norm = nn.Parameter(torch.ones(self.attention_head_size))
+        columns = getattr(config, "rotary_columns", 0)
+        self.register_buffer("rotary", rotary_table(config.max_position_embeddings, columns) if columns else None, persistent=False)
+
+    def _heads(self, x, heads):
+        return x.view(*x.shape[:-1], heads, self.attention_head_size)
+
+    def _states(self, encoder_hidden_states):
+        return (self._heads(self.key(encoder_hidden_states), self.num_key_value_heads),
+                self._heads(self.value(encoder_hidden_states), self.num_key_value_heads))
+
+    def states(self, encoder_hidden_states, positions=None):
+        """Keys (normed and rotated) and values [B, states, key heads, head size] of an encoder's states [B, states, hidden], for calls that read
+        the same states again, such as a decoder's next tokens."""
+        keys, values = self._states(encoder_hidden_states)
+        return qk_norm_rotary(keys, None, self.key_norm, table=self.rotary, q_positions=positions, eps=self.qk_norm_eps)[0], values
+
+    def forward(self, hidden_states, encoder_hidden_states=None, encoder_attention_mask=None, *, states=None, positions=None,
+                encoder_positions=None):
+        """hidden_states [B, L, hidden]; either encoder_hidden_states [B, states, hidden] or what ``states`` returned for them; the mask [B, states], True or
+        above 0 where a state takes part; positions of the tokens and the states (with rotary_columns), 0, 1, 2 ... if None."""
+        if (states is None) == (encoder_hidden_states is None):
+            raise ValueError("either encoder_hidden_states or states")
+        queries = self._heads(self.query(self.LayerNorm(hidden_states)), self.num_attention_heads)
+        norm = dict(table=self.rotary, q_positions=positions, eps=self.qk_norm_eps)
+        if states is None:
+            keys, values = self._states(encoder_hidden_states)
+            queries, keys = qk_norm_rotary(queries, keys, self.query_norm, self.key_norm, k_positions=encoder_positions, **norm)
+        else:
+            keys, values = states
+            queries, _ = qk_norm_rotary(queries, None, self.query_norm, **norm)
+        mask = encoder_attention_mask
+        if mask is not None and mask.dtype != torch.bool:
+            mask = mask > 0
+        return self.dense(cross_attention(queries, keys, values, mask).flatten(2))
 
 
 class EncoderLayer(nn.Module):

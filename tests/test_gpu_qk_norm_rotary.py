@@ -100,3 +100,96 @@ def test_against_64_bits(B, Lq, Lk, H, Hk, D, R, interleaved, dtype):
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in zip(outs, run()))
     assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad([t for t in run() if t is not None], leaves, gs)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layouts_and_types(dtype):
+    """Any strides give the bits of contiguous arrays; weights of q's type and positions of either width; zeros and large numbers."""
+    B, L, H, Hk, D = 2, 9, 4, 2, 64
+    q, k = _randn(B, L, H, D, dtype=dtype), _randn(B, L, Hk, D, dtype=dtype, seed=1)
+    table, qw = rotary_table(50, 32, device=DEV), 1 + 0.2 * _randn(D, seed=4)
+    at = torch.randint(0, 50, (B, L), device=DEV)
+    want = qk_norm_rotary(q, k, qw, qw, table=table, q_positions=at, k_positions=at)
+
+    def same(q, k, at=at, kat=at):
+        assert all(torch.equal(a, b) for a, b in zip(qk_norm_rotary(q, k, qw, qw, table=table, q_positions=at, k_positions=kat), want))
+
+    qkv = torch.cat((q, k, k), 2)
+    same(qkv[:, :, :H], qkv[:, :, H:H + Hk])
+    first = lambda t: t.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)  # noqa: E731
+    same(first(q), first(k))
+    odd = lambda t: torch.cat((t.flatten()[:1], t.flatten()))[1:].view(t.shape)  # noqa: E731
+    same(odd(q), odd(k))
+    same(q, k, at.int(), at)
+    same(q, k, at.int(), at.int())
+    same(q, k, torch.stack((at, at), 2)[:, :, 0])
+    row = qk_norm_rotary(q, k, qw, qw, table=table, q_positions=at[0], k_positions=at[0])
+    all_rows = qk_norm_rotary(q, k, qw, qw, table=table, q_positions=at[:1].expand(B, -1), k_positions=at[0])
+    assert all(torch.equal(a, b) for a, b in zip(row, all_rows))
+    own = qw.to(dtype)
+    assert torch.equal(qk_norm_rotary(q, None, own)[0], qk_norm_rotary(q, None, own.float())[0])
+    x = torch.zeros(1, 2, 1, D, device=DEV, dtype=dtype)
+    assert not qk_norm_rotary(x)[0].any()
+    x[0, 1] = 100.0
+    y = qk_norm_rotary(x, eps=0.0)[0]
+    assert y[0, 0].isnan().all() and (y[0, 1].float() - 1).abs().max() <= torch.finfo(dtype).eps       # 0 / 0, as the formula has it
+
+
+def test_nothing_to_do():
+    for B, Lq, Lk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        q, k = _randn(B, Lq, 4, 64).requires_grad_(), _randn(B, Lk, 2, 64).requires_grad_()
+        w = torch.ones(64, device=DEV, requires_grad=True)
+        a, b = qk_norm_rotary(q, k, w, w)
+        assert a.shape == q.shape and b.shape == k.shape
+        grads = torch.autograd.grad((a, b), (q, k, w), (torch.ones_like(a), torch.ones_like(b)))
+        assert [t.shape for t in grads] == [q.shape, k.shape, w.shape] and grads[2].isfinite().all()
+
+
+def test_one_of_two_gradients():
+    q, k, w = _randn(2, 3, 4, 64).requires_grad_(), _randn(2, 5, 2, 64, seed=1).requires_grad_(), torch.ones(64, device=DEV, requires_grad=True)
+    g = _randn(2, 3, 4, 64, seed=2)
+    a, b = qk_norm_rotary(q, k, w, w)
+    gq, gk, gw = torch.autograd.grad(a, (q, k, w), g)
+    alone = torch.autograd.grad(qk_norm_rotary(q, None, w)[0], (q, w), g)
+    assert torch.equal(gq, alone[0]) and torch.equal(gw, alone[1]) and not gk.any()
+    a, b = qk_norm_rotary(q, k, w, w)
+    got = torch.autograd.grad((a, b), (q, k), (g, torch.ones_like(b)), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(got[0].sum(), q)
+
+
+def test_captured_and_replayed():
+    q, k = (_randn(3, n, 4, 64, dtype=torch.float16, seed=n).requires_grad_() for n in (70, 90))
+    w, table = torch.ones(64, device=DEV, requires_grad=True), rotary_table(100, 64, device=DEV)
+    at = torch.randint(0, 100, (3, 70), device=DEV)
+    gs = [torch.ones(3, n, 4, 64, device=DEV, dtype=torch.float16) for n in (70, 90)]
+
+    def step(q, k, w):
+        out = qk_norm_rotary(q, k, w, w, table=table, q_positions=at)
+        return (*(t.detach() for t in out), *torch.autograd.grad(out, (q, k, w), gs))
+
+    step(q, k, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step(q, k, w)
+    for i in range(4):
+        with torch.no_grad():
+            for t in (q, k, *gs):
+                t.copy_(_randn(*t.shape, seed=i).half())
+            w.copy_(1 + 0.1 * _randn(64, seed=i))
+            at.copy_(torch.randint(0, 100, at.shape, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = [t.detach().clone().requires_grad_() for t in (q, k, w)]
+        assert all(torch.equal(a, b) for a, b in zip(got, step(*fresh)))
+
+
+def test_rows_beyond_32_bits():
+    base = torch.empty(300, 1 << 24, dtype=torch.bfloat16, device=DEV)
+    x = _randn(1, 300, 1, 64, dtype=torch.bfloat16)
+    base[:, 64:128] = x[0, :, 0]
+    far = base[:, 64:128][None, :, None]
+    table = rotary_table(300, 64, device=DEV)
+    assert torch.equal(qk_norm_rotary(far, far, table=table)[1], qk_norm_rotary(x, x, table=table)[0])
