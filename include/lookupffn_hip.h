@@ -933,8 +933,8 @@ int lffn_qk_norm_rotary_bwd(const lffn_qk_norm_rotary *a, const void *g_q, const
  * key head below 2^30); columns lie together, a multiple of 8, at most 128.  key_mask: [B, k_len] bytes, not 0 where a key takes part, with a
  * batch stride, or NULL.  What keys and values that take no part hold does not matter.  A query without keys gets zeros.  scale: positive, finite.
  * format 0: fp32 accuracy, 1 and 2: products of 16 bits, sums in fp32, softmax weights rounded to the format.
- * out: [B, q_len, heads, columns], in the format.  lse: [B, key_heads, q_len * heads / key_heads] or NULL, what the backward needs of a row
- * (private to it).  workspace: 16-byte aligned, of lffn_cross_attention_workspace_bytes (0: may be NULL).
+ * out: [B, q_len, heads, columns], in the format.  kept: what the backward needs beside out (private to it), of lffn_cross_attention_kept_bytes, 16-byte aligned,
+ * or NULL.  workspace: 16-byte aligned, of lffn_cross_attention_workspace_bytes (0: may be NULL).
  */
 typedef struct lffn_cross_attention {
     const void *q, *k, *v;
@@ -946,15 +946,16 @@ typedef struct lffn_cross_attention {
     int32_t format;
 } lffn_cross_attention;
 int lffn_cross_attention_workspace_bytes(const lffn_cross_attention *a, int64_t *bytes);
-int lffn_cross_attention_fwd(const lffn_cross_attention *a, void *out, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+int lffn_cross_attention_kept_bytes(const lffn_cross_attention *a, int64_t *bytes);
+int lffn_cross_attention_fwd(const lffn_cross_attention *a, void *out, void *kept, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
- * Its backward: from out and lse of the forward and the gradient of out, the gradients of q, k and v, all contiguous as out (k's and v's
+ * Its backward: from out and kept of the forward and the gradient of out, the gradients of q, k and v, all contiguous as out (k's and v's
  * [B, k_len, key_heads, columns]); zeros for keys that take no part.  grad_q NULL, or grad_k and grad_v NULL: not wanted.  No atomics:
  * the same bits on every call.
  */
 int lffn_cross_attention_bwd_workspace_bytes(const lffn_cross_attention *a, int64_t *bytes);
-int lffn_cross_attention_bwd(const lffn_cross_attention *a, const void *out, const float *lse, const void *g_out, void *grad_q, void *grad_k,
+int lffn_cross_attention_bwd(const lffn_cross_attention *a, const void *out, const void *kept, const void *g_out, void *grad_q, void *grad_k,
                              void *grad_v, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus

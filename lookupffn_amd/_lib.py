@@ -164,6 +164,7 @@ SIGNATURES["lffn_qk_norm_rotary_fwd"] = [ctypes.POINTER(QkNormRotary), _vp, _vp,
 SIGNATURES["lffn_qk_norm_rotary_bwd_workspace_bytes"] = [ctypes.POINTER(QkNormRotary), ctypes.POINTER(_i64)]
 SIGNATURES["lffn_qk_norm_rotary_bwd"] = [ctypes.POINTER(QkNormRotary), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
 SIGNATURES["lffn_cross_attention_workspace_bytes"] = [ctypes.POINTER(CrossAttention), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_cross_attention_kept_bytes"] = [ctypes.POINTER(CrossAttention), ctypes.POINTER(_i64)]
 SIGNATURES["lffn_cross_attention_fwd"] = [ctypes.POINTER(CrossAttention), _vp, _vp, _vp, _i64, _vp]
 SIGNATURES["lffn_cross_attention_bwd_workspace_bytes"] = [ctypes.POINTER(CrossAttention), ctypes.POINTER(_i64)]
 SIGNATURES["lffn_cross_attention_bwd"] = [ctypes.POINTER(CrossAttention), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]

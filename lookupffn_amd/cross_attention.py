@@ -129,21 +129,21 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, *, table=None, q_pos
 
 
 class CrossAttentionFunction(Function):
-    """``cross_attention`` behind its checks: keeps the result and one number a row for the backward."""
+    """``cross_attention`` behind its checks: keeps the result for the backward, with a number a row and what the result's rounding took."""
 
     @staticmethod
     def forward(ctx, q, k, v, key_mask, scale):
-        out, lse = ops.cross_attention(q, k, v, key_mask, scale, True)
-        ctx.save_for_backward(q, k, v, key_mask, out, lse)
+        out, kept = ops.cross_attention(q, k, v, key_mask, scale, True)
+        ctx.save_for_backward(q, k, v, key_mask, out, kept)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, key_mask, out, lse = ctx.saved_tensors
+        q, k, v, key_mask, out, kept = ctx.saved_tensors
         of_queries, of_keys = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        grads = list(ops.cross_attention_bwd(q, k, v, key_mask, ctx.scale, out, lse, g, of_queries, of_keys))
+        grads = list(ops.cross_attention_bwd(q, k, v, key_mask, ctx.scale, out, kept, g, of_queries, of_keys))
         return ((grads.pop(0) if of_queries else None), *(grads if of_keys else (None, None)), None, None)
 
 

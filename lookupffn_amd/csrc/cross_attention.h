@@ -75,6 +75,7 @@ struct BF16 {
     static __device__ __forceinline__ Frag<1> operand(const Raw &r) { return {{r.u}}; }
     static __device__ __forceinline__ void unpack(const Raw &r, float (&v)[8]) { BF16Row::unpack(r.u, v); }
     static __device__ __forceinline__ uint32_t pack2(float a, float b) { return BF16Row::pack2(a, b); }
+    static __device__ __forceinline__ float rounded(float a) { return (float)(__bf16)a; }
     static __device__ __forceinline__ void store4(char *p, float a, float b, float c, float d) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(BF16Row::pack2(a, b), BF16Row::pack2(c, d));
     }
@@ -95,6 +96,7 @@ struct F16 {
     static __device__ __forceinline__ Frag<1> operand(const Raw &r) { return {{r.u}}; }
     static __device__ __forceinline__ void unpack(const Raw &r, float (&v)[8]) { F16Row::unpack(r.u, v); }
     static __device__ __forceinline__ uint32_t pack2(float a, float b) { return F16Row::pack2(a, b); }
+    static __device__ __forceinline__ float rounded(float a) { return (float)(_Float16)a; }
     static __device__ __forceinline__ void store4(char *p, float a, float b, float c, float d) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(F16Row::pack2(a, b), F16Row::pack2(c, d));
     }
@@ -133,12 +135,14 @@ struct F32 {
     static __device__ __forceinline__ void store4(char *p, float a, float b, float c, float d) {
         *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
     }
+    static __device__ __forceinline__ float rounded(float a) { return a; }
 };
 
 // The columns 32 d + 8 g + 4 half .. + 3 of a lane's row (half = lane / 32) to memory, by d and g; `row` where the lane's row begins, all lanes together.  Of 16-bit
 // results the lanes of a row exchange four columns of two groups, so that each has eight that lie together and stores 16 bytes.
+// rest: where what the rounding takes goes, or null.
 template <typename F, int DB>
-__device__ __forceinline__ void store_row(const ca_f32x16_t (&o)[DB], float by, char *row, bool live, int columns, int half) {
+__device__ __forceinline__ void store_row(const ca_f32x16_t (&o)[DB], float by, char *row, bool live, int columns, int half, char *rest = nullptr) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
         if constexpr (F::BYTES == 4) {
@@ -151,17 +155,26 @@ __device__ __forceinline__ void store_row(const ca_f32x16_t (&o)[DB], float by, 
         } else {
 #pragma unroll
             for (int g = 0; g < 4; g += 2) {
-                uint32_t a[2], b[2];
+                float t[8];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    a[e] = F::pack2(o[d][4 * g + 2 * e] * by, o[d][4 * g + 2 * e + 1] * by);
-                    b[e] = F::pack2(o[d][4 * g + 4 + 2 * e] * by, o[d][4 * g + 4 + 2 * e + 1] * by);
-                    // the upper lanes' a and the lower lanes' b change places
-                    const auto swapped = __builtin_amdgcn_permlane32_swap(a[e], b[e], false, false);
-                    a[e] = swapped[0], b[e] = swapped[1];
+                for (int e = 0; e < 8; ++e) t[e] = o[d][4 * g + e] * by;
+                auto put = [&](char *to) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        // the upper lanes' first four columns and the lower lanes' last four change places
+                        const auto swapped = __builtin_amdgcn_permlane32_swap(F::pack2(t[2 * e], t[2 * e + 1]), F::pack2(t[4 + 2 * e], t[4 + 2 * e + 1]), false, false);
+                        w[e] = swapped[0], w[2 + e] = swapped[1];
+                    }
+                    const int col = 32 * d + 8 * (g + half);
+                    if (live && col < columns) *reinterpret_cast<uint4 *>(to + col * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                };
+                put(row);
+                if (rest) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) t[e] -= F::rounded(t[e]);
+                    put(rest);
                 }
-                const int col = 32 * d + 8 * (g + half);
-                if (live && col < columns) *reinterpret_cast<uint4 *>(row + col * 2) = make_uint4(a[0], a[1], b[0], b[1]);
             }
         }
     }
@@ -439,6 +452,19 @@ __device__ __forceinline__ void walk_keys(KF &feed, uint64_t *words, const uint8
 __device__ __forceinline__ int64_t heads_row(int b, int kh, int row, int64_t len, int key_heads, const Divisor &group) {
     const int token = group.quotient(row);
     return ((b * len + token) * key_heads + kh) * group.by + (row - token * group.by);
+}
+
+// What a forward keeps for its backward beside the result: every row's level, and of 16-bit results what their rounding took, in the same format: delta, a sum
+// of the result times its gradient, is what is left of ds where a query has few keys, and with the rounded result alone ds would be off by as much as by
+// its own rounding and more (5 keys: 3.7e-3 of the queries' gradients in bfloat16 where a rounding is 1.7e-3).
+struct Kept {
+    float *levels;
+    char *rest;
+};
+inline int64_t kept_bytes(int64_t rows, int64_t columns, int bytes) { return (rows * 4 + 15) / 16 * 16 + (bytes == 2 ? rows * columns * 2 : 0); }
+inline Kept kept_at(void *p, int64_t rows, int bytes) {
+    char *const at = static_cast<char *>(p);
+    return {static_cast<float *>(p), at && bytes == 2 ? at + (rows * 4 + 15) / 16 * 16 : nullptr};
 }
 
 // Which unit of work a workgroup has: neighbours (tiles that read the same keys) on one XCD.

@@ -14,7 +14,7 @@ namespace {
 struct FwdArgs {
     const char *q, *k, *v;
     const uint8_t *mask;
-    char *out;
+    char *out, *rest;                     // rest: null, or where what the rounding takes goes
     float *lse, *part, *part_lse;         // parts: [splits, B, key heads, rows(, columns)]
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, mask_stride;         // strides in bytes
     int64_t keys, steps, split_steps, q_len;
@@ -31,6 +31,13 @@ constexpr int few_rows(bool f32) { return f32 ? 4 : 2; }
 constexpr int FEW_WAVES = 16;             // wavefronts of a workgroup at most,
 constexpr int FEW_TOGETHER = 2;           // keys of a group of lanes asked for together
 constexpr float SLACK = 6.f;              // how far (powers of two) a row's largest score may outgrow the one that its sums go by
+
+// Four columns of a result, and what their rounding takes.
+template <typename F>
+__device__ __forceinline__ void store_result(const FwdArgs &a, int64_t at, const float4 &v) {
+    F::store4(a.out + at, v.x, v.y, v.z, v.w);
+    if (a.rest) F::store4(a.rest + at, v.x - F::rounded(v.x), v.y - F::rounded(v.y), v.z - F::rounded(v.z), v.w - F::rounded(v.w));
+}
 
 template <typename F, int DP, int KT>
 __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F::PLANES == 1 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
@@ -128,7 +135,8 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F:
         return;
     }
     if (a.lse && live && half == 0) a.lse[at] = level;
-    store_row<F, DB>(o, inverse, a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES, live, a.columns, half);
+    const int64_t of = heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
+    store_row<F, DB>(o, inverse, a.out + of, live, a.columns, half, a.rest ? a.rest + of : nullptr);
 }
 
 // A row or two for a key head (fp32: up to four): single tokens, with the heads that share it.  On the vector ALU, which keeps up with the memory here (a number of a key or value
@@ -260,8 +268,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(FwdArgs a) {
             *reinterpret_cast<float4 *>(a.part + of * a.columns + col) = make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse);
         } else {
             if (quad == 0 && a.lse) a.lse[at] = level;
-            F::store4(a.out + (heads_row(b, kh, r, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES, o.x * inverse, o.y * inverse, o.z * inverse,
-                      o.w * inverse);
+            store_result<F>(a, (heads_row(b, kh, r, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES,
+                            make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse));
         }
     }
 }
@@ -328,8 +336,8 @@ __global__ __launch_bounds__(WG) void join_kernel(FwdArgs a, int64_t all_rows) {
     const float by = sum == 0.f ? 0.f : 1.f / sum;
     const int bh = int(at / a.rows), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, row = int(at - int64_t(bh) * a.rows);
     if (a.lse && col == 0) a.lse[at] = sum == 0.f ? INFINITY : less + __builtin_amdgcn_logf(sum);
-    char *const p = a.out + heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
-    F::store4(p + col * F::BYTES, acc.x * by, acc.y * by, acc.z * by, acc.w * by);
+    store_result<F>(a, (heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES,
+                    make_float4(acc.x * by, acc.y * by, acc.z * by, acc.w * by));
 }
 
 }  // namespace
@@ -464,16 +472,24 @@ extern "C" int lffn_cross_attention_workspace_bytes(const lffn_cross_attention *
     return LFFN_OK;
 }
 
-extern "C" int lffn_cross_attention_fwd(const lffn_cross_attention *c, void *out, float *lse, void *workspace, int64_t workspace_bytes,
+extern "C" int lffn_cross_attention_kept_bytes(const lffn_cross_attention *c, int64_t *bytes) {
+    LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
+    if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
+    *bytes = kept_bytes(c->B * c->q_len * c->heads, c->columns, c->format == LFFN_ROWS_F32 ? 4 : 2);
+    return LFFN_OK;
+}
+
+extern "C" int lffn_cross_attention_fwd(const lffn_cross_attention *c, void *out, void *kept, void *workspace, int64_t workspace_bytes,
                                         void *stream) {
     if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
     FwdArgs a{};
     const int64_t bytes = plan(*c, a);
     LFFN_REQUIRE(bytes >= 0, LFFN_ERR_UNSUPPORTED);
     if (a.units == 0) return LFFN_OK;
-    LFFN_REQUIRE(out && lffn_aligned16(out), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(out && lffn_aligned16(out) && lffn_aligned16(kept), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(bytes == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= bytes), LFFN_ERR_BAD_ARG);
-    a.out = static_cast<char *>(out), a.lse = lse;
+    const Kept k = kept_at(kept, c->B * c->q_len * c->heads, c->format == LFFN_ROWS_F32 ? 4 : 2);
+    a.out = static_cast<char *>(out), a.lse = k.levels, a.rest = k.rest;
     a.part = static_cast<float *>(workspace);
     a.part_lse = a.part ? a.part + int64_t(a.splits) * c->B * c->key_heads * a.rows * a.columns : nullptr;
     hipStream_t s = static_cast<hipStream_t>(stream);

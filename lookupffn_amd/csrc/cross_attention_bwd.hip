@@ -21,7 +21,7 @@ constexpr int NORM_ROWS = 128;            // rows of a workgroup of delta_kernel
 constexpr float P_LIFT = 14.f;            // half precision
 
 struct BwdArgs {
-    const char *q, *k, *v, *out, *g;
+    const char *q, *k, *v, *out, *rest, *g;
     const uint8_t *mask;
     const float *lse;
     char *gq, *gk, *gv;
@@ -45,7 +45,7 @@ __device__ __forceinline__ float wave_most(float v) {
     return fmaxf(v, lane_xor<32>(v));
 }
 
-// delta of every row; half precision: the longest rows of g and v as well.  16 lanes a row, 8 columns a lane.  Bound by memory: out and g (and v) once.
+// delta of every row; half precision: the longest rows of g and v as well.  16 lanes a row, 8 columns a lane.  Bound by memory: out, its rest and g (and v) once.
 // (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16 65 us.)
 template <typename F, bool NORMS>
 __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
     const int bh = a.norm_tiles.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * tiles;
     float most = 0.f;
     if (tile < a.g_tiles) {
-        typename F::Raw o[EACH], g[EACH];
+        typename F::Raw o[EACH], g[EACH], rest[F::PLANES == 1 ? EACH : 1];
         const int first = tile * NORM_ROWS + threadIdx.x / 16;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
@@ -64,12 +64,19 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
             const int64_t at = (heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES;
             o[i] = F::load(a.out + at);
             g[i] = F::load(a.g + at);
+            if constexpr (F::PLANES == 1) rest[i] = F::load(a.rest + at);
         }
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             float dot = 0.f, squares = 0.f, u[8], v[8];
             F::unpack(o[i], u);
             F::unpack(g[i], v);
+            if constexpr (F::PLANES == 1) {
+                float w[8];
+                F::unpack(rest[i], w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[e] += w[e];
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot), squares = fmaf(v[e], v[e], squares);
             dot = lane_group_sum<16>(on ? dot : 0.f);
@@ -681,23 +688,24 @@ extern "C" int lffn_cross_attention_bwd_workspace_bytes(const lffn_cross_attenti
     return LFFN_OK;
 }
 
-extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const void *out, const float *lse, const void *g_out, void *grad_q,
+extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const void *out, const void *kept, const void *g_out, void *grad_q,
                                         void *grad_k, void *grad_v, void *workspace, int64_t workspace_bytes, void *stream) {
     if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
     Plan p = plan(*c);
     if (p.q.units == 0 && p.k.units == 0) return LFFN_OK;
-    LFFN_REQUIRE(p.q.units == 0 || (out && lse && g_out), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(p.q.units == 0 || (out && kept && g_out), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.k.units == 0 || (grad_k != nullptr) == (grad_v != nullptr), LFFN_ERR_BAD_ARG);
     if (!grad_q) p.q.units = 0;                            // not wanted
     if (!grad_k) p.k.units = 0;
     if (p.q.units == 0 && p.k.units == 0) return LFFN_OK;
-    for (const void *t : {out, g_out, (const void *)grad_q, (const void *)grad_k, (const void *)grad_v}) LFFN_REQUIRE(lffn_aligned16(t), LFFN_ERR_BAD_ARG);
+    for (const void *t : {out, kept, g_out, (const void *)grad_q, (const void *)grad_k, (const void *)grad_v}) LFFN_REQUIRE(lffn_aligned16(t), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.floats == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= p.floats * 4), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.q.units <= INT32_MAX && p.k.units <= INT32_MAX &&
                      int64_t(p.q.batch_heads) * (p.q.g_tiles + p.q.v_tiles) <= INT32_MAX, LFFN_ERR_UNSUPPORTED);
     float *const w = static_cast<float *>(workspace);
+    const Kept k = kept_at(const_cast<void *>(kept), c->B * c->q_len * c->heads, c->format == LFFN_ROWS_F32 ? 4 : 2);
     for (BwdArgs *a : {&p.q, &p.k}) {
-        a->out = static_cast<const char *>(out), a->g = static_cast<const char *>(g_out), a->lse = lse;
+        a->out = static_cast<const char *>(out), a->g = static_cast<const char *>(g_out), a->lse = k.levels, a->rest = k.rest;
         a->gq = static_cast<char *>(grad_q), a->gk = static_cast<char *>(grad_k), a->gv = static_cast<char *>(grad_v);
         a->delta = w + p.delta, a->g_norms = w + p.g_norms, a->v_norms = w + p.v_norms, a->part = w + p.part;
     }

@@ -79,6 +79,7 @@ using torch::autograd::variable_list;
     X(lffn_qk_norm_rotary_bwd_workspace_bytes) \
     X(lffn_cross_attention_fwd)             \
     X(lffn_cross_attention_workspace_bytes) \
+    X(lffn_cross_attention_kept_bytes)      \
     X(lffn_cross_attention_bwd)             \
     X(lffn_cross_attention_bwd_workspace_bytes)
 

@@ -304,13 +304,13 @@ struct AttentionInputs {
 };
 
 struct CrossAttentionBackward : public torch::autograd::Node {
-    SavedVariable q, k, v, mask, result, lse;
+    SavedVariable q, k, v, mask, result, kept;
     double scale = 0;
 
     std::string name() const override { return "CrossAttentionBackward"; }
 
     void release_variables() override {
-        for (SavedVariable *s : {&q, &k, &v, &mask, &result, &lse}) s->reset_data();
+        for (SavedVariable *s : {&q, &k, &v, &mask, &result, &kept}) s->reset_data();
     }
 
     variable_list apply(variable_list &&grads) override {
@@ -326,7 +326,7 @@ struct CrossAttentionBackward : public torch::autograd::Node {
         at::AutoGradMode no_grad(false);
         const auto self = shared_from_this();
         AttentionInputs in{q.unpack(self), k.unpack(self), v.unpack(self), mask.unpack(self), scale};
-        const Tensor result_ = result.unpack(self), lse_ = lse.unpack(self), g = aligned_contiguous(grads[0]);
+        const Tensor result_ = result.unpack(self), kept_ = kept.unpack(self), g = aligned_contiguous(grads[0]);
         const at::Device dev = in.q.device();
         const c10::DeviceGuard guard(dev);
         void *st = stream_on(dev);
@@ -341,7 +341,7 @@ struct CrossAttentionBackward : public torch::autograd::Node {
         int64_t bytes = 0;
         CALL(lffn_cross_attention_bwd_workspace_bytes, &a, &bytes);
         const Tensor ws = empty_bytes(bytes, dev);
-        CALL(lffn_cross_attention_bwd, &a, result_.data_ptr(), f32(lse_), g.data_ptr(), out[0].defined() ? out[0].data_ptr() : nullptr,
+        CALL(lffn_cross_attention_bwd, &a, result_.data_ptr(), kept_.data_ptr(), g.data_ptr(), out[0].defined() ? out[0].data_ptr() : nullptr,
              of_keys ? out[1].data_ptr() : nullptr, of_keys ? out[2].data_ptr() : nullptr, ws.data_ptr(), bytes, st);
         return out;
     }
@@ -377,12 +377,15 @@ PyObject *cross_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
         laid.lay_out();
         const lffn_cross_attention a = laid.arguments();
         out = at::empty(in.q.sizes(), in.q.options());
-        Tensor lse, ws;
-        if (grads) lse = empty_f32({a.B * a.q_len * a.heads}, dev);
+        Tensor kept, ws;
         int64_t bytes = 0;
+        if (grads) {
+            CALL(lffn_cross_attention_kept_bytes, &a, &bytes);
+            kept = empty_bytes(bytes, dev);
+        }
         CALL(lffn_cross_attention_workspace_bytes, &a, &bytes);
         if (bytes > 0) ws = empty_bytes(bytes, dev);
-        CALL(lffn_cross_attention_fwd, &a, out.data_ptr(), f32(lse), bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_on(dev));
+        CALL(lffn_cross_attention_fwd, &a, out.data_ptr(), grads ? kept.data_ptr() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_on(dev));
         if (grads) {
             auto node = std::shared_ptr<CrossAttentionBackward>(new CrossAttentionBackward(), torch::autograd::deleteNode);
             node->set_next_edges(torch::autograd::collect_next_edges(in.q, in.k, in.v));
@@ -391,7 +394,7 @@ PyObject *cross_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
             node->k = SavedVariable(in.k, false);
             node->v = SavedVariable(in.v, false);
             node->mask = SavedVariable(in.mask, false);
-            node->lse = SavedVariable(lse, false);
+            node->kept = SavedVariable(kept, false);
             torch::autograd::set_history(out, node);
             node->result = SavedVariable(out, true);
         }

@@ -1450,25 +1450,31 @@ def _cross_attention_args(q, k, v, key_mask, scale):
     return a
 
 
+def _kept_bytes(q):
+    """lffn_cross_attention_kept_bytes: every row's level, and of 16-bit results what their rounding took."""
+    rows = q.shape[0] * q.shape[1] * q.shape[2]
+    return (rows * 4 + 15) // 16 * 16 + (rows * q.shape[3] * 2 if q.element_size() == 2 else 0)
+
+
 _L.define("cross_attention(Tensor q, Tensor k, Tensor v, Tensor? key_mask, float scale, bool keep) -> (Tensor, Tensor)")
 
 
 def _cross_attention_impl(q, k, v, key_mask, scale, keep):
     """q [B, L, heads, columns], k, v [B, keys, key heads, columns], key_mask [B, keys] bool or None -> (out [B, L, heads, columns], with
-    `keep` what the backward needs of every row, fp32)."""
+    `keep` what the backward needs beside it, bytes)."""
     _lib.require_gpu(q, k, v, key_mask)
     q, k, v, key_mask = _head_rows(q, True), _head_rows(k, True), _head_rows(v, True), _neighbours_together(key_mask)
     a = _cross_attention_args(q, k, v, key_mask, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2] if keep else 0, dtype=torch.float32, device=q.device)
+    kept = torch.empty(_kept_bytes(q) if keep else 0, dtype=torch.uint8, device=q.device)
     with _dev_guard(q):
         lib, n = _lib.load(), ctypes.c_int64(0)
         _lib.check(lib.lffn_cross_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_cross_attention_workspace_bytes")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
-        rc = lib.lffn_cross_attention_fwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr() if keep else None, _lib.ptr(ws), n.value,
+        rc = lib.lffn_cross_attention_fwd(ctypes.byref(a), out.data_ptr(), kept.data_ptr() if keep else None, _lib.ptr(ws), n.value,
                                           _lib.stream_of(q))
     _lib.check(rc, f"lffn_cross_attention_fwd(q={tuple(q.shape)}, k={tuple(k.shape)})")
-    return out, lse
+    return out, kept
 
 
 _L.impl("cross_attention", _cross_attention_impl, "CUDA")
@@ -1476,16 +1482,16 @@ _L.impl("cross_attention", _cross_attention_impl, "CUDA")
 
 @torch.library.register_fake("lookupffn::cross_attention")
 def _(q, k, v, key_mask, scale, keep):
-    return q.new_empty(q.shape), q.new_empty(q.shape[0] * q.shape[1] * q.shape[2] if keep else 0, dtype=torch.float32)
+    return q.new_empty(q.shape), q.new_empty(_kept_bytes(q) if keep else 0, dtype=torch.uint8)
 
 
-_L.define("cross_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor? key_mask, float scale, Tensor out, Tensor lse, Tensor g, bool of_queries, "
+_L.define("cross_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor? key_mask, float scale, Tensor out, Tensor kept, Tensor g, bool of_queries, "
           "bool of_keys) -> Tensor[]")
 
 
-def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, lse, g, of_queries, of_keys):
+def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, kept, g, of_queries, of_keys):
     """-> the gradient of q if it is wanted, then those of k and v if they are."""
-    _lib.require_gpu(q, k, v, key_mask, out, lse, g)
+    _lib.require_gpu(q, k, v, key_mask, out, kept, g)
     q, k, v, key_mask, g = _head_rows(q, True), _head_rows(k, True), _head_rows(v, True), _neighbours_together(key_mask), _aligned(g)
     a = _cross_attention_args(q, k, v, key_mask, scale)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys))]
@@ -1493,7 +1499,7 @@ def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, lse, g, of_queries,
         lib, n = _lib.load(), ctypes.c_int64(0)
         _lib.check(lib.lffn_cross_attention_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_cross_attention_bwd_workspace_bytes")
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        rc = lib.lffn_cross_attention_bwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), g.data_ptr(), *(_lib.ptr(t) for t in grads),
+        rc = lib.lffn_cross_attention_bwd(ctypes.byref(a), out.data_ptr(), kept.data_ptr(), g.data_ptr(), *(_lib.ptr(t) for t in grads),
                                           ws.data_ptr(), n.value, _lib.stream_of(q))
     _lib.check(rc, f"lffn_cross_attention_bwd(q={tuple(q.shape)}, k={tuple(k.shape)})")
     return [t for t in grads if t is not None]
@@ -1503,7 +1509,7 @@ _L.impl("cross_attention_bwd", _cross_attention_bwd_impl, "CUDA")
 
 
 @torch.library.register_fake("lookupffn::cross_attention_bwd")
-def _(q, k, v, key_mask, scale, out, lse, g, of_queries, of_keys):
+def _(q, k, v, key_mask, scale, out, kept, g, of_queries, of_keys):
     return [t.new_empty(t.shape) for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys)) if wanted]
 
 
