@@ -16,10 +16,12 @@ struct FwdArgs {
     const uint8_t *mask;
     char *out, *rest;                     // rest: null, or where what the rounding takes goes
     float *lse, *part, *part_lse;         // parts: [splits, B, key heads, rows(, columns)]
+    float *k_levels, *v_levels;           // fp32 numbers in two terms: log2 of the longest rows, [B, key heads, level_tiles]
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, mask_stride;         // strides in bytes
     int64_t keys, steps, split_steps, q_len;
-    Divisor group, tiles, split_by, heads;               // query heads of a key head, tiles of rows, shares of the keys, key heads
+    Divisor group, tiles, split_by, heads, level_by;     // query heads of a key head, tiles of rows, shares of the keys, key heads, level_tiles
     int key_heads, rows, row_tiles, splits, columns, units;
+    int level_tiles;
     int few_waves;                        // few_rows_kernel's wavefronts, 0: not the one
     float c;                              // scale log2 e
 };
@@ -39,8 +41,50 @@ __device__ __forceinline__ void store_result(const FwdArgs &a, int64_t at, const
     if (a.rest) F::store4(a.rest + at, v.x - F::rounded(v.x), v.y - F::rounded(v.y), v.z - F::rounded(v.z), v.w - F::rounded(v.w));
 }
 
+__device__ __forceinline__ float level_of(const F32::Raw &r, bool on) {
+    float v[8];
+    F32::unpack(on ? r : F32::zero(), v);
+    return row_level(v);
+}
+
+// log2 of the longest of 128 keys that take part, and of their values.  Bound by memory: both once.
+__global__ __launch_bounds__(WG) void levels_kernel(FwdArgs a) {
+    constexpr int EACH = LEVEL_ROWS / (WG / 16);
+    __shared__ float red[2][WAVES];
+    const int lane = threadIdx.x & 15, col = lane * 8 < a.columns ? lane * 8 : 0;
+    const bool on = lane * 8 < a.columns;
+    const int bh = a.level_by.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * a.level_tiles;
+    F32::Raw k[EACH], v[EACH];
+    bool live[EACH];
+    const int64_t first = int64_t(tile) * LEVEL_ROWS + threadIdx.x / 16;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int64_t key = first + i * (WG / 16), at = key < a.keys ? key : a.keys - 1;
+        live[i] = !a.mask || a.mask[b * a.mask_stride + at] != 0;
+        k[i] = F32::load(a.k + b * a.kb + kh * a.kh + at * a.kt + col * 4);
+        v[i] = F32::load(a.v + b * a.vb + kh * a.vh + at * a.vt + col * 4);
+    }
+    float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const float lk = level_of(k[i], on), lv = level_of(v[i], on);
+        if (live[i]) most[0] = fmaxf(most[0], lk), most[1] = fmaxf(most[1], lv);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        most[n] = fmaxf(most[n], lane_xor<16>(most[n]));
+        most[n] = fmaxf(most[n], lane_xor<32>(most[n]));
+        if ((threadIdx.x & 63) == 0) red[n][threadIdx.x >> 6] = most[n];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const float *const r = red[threadIdx.x];
+        (threadIdx.x ? a.v_levels : a.k_levels)[blockIdx.x] = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+    }
+}
+
 template <typename F, int DP, int KT>
-__global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F::PLANES == 1 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
+__global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F::PLANES <= 2 ? 2 : 1) void cross_attention_kernel(FwdArgs a) {
     typedef Tile<F, DP, KT> T;
     typedef Frag<F::PLANES> Op;
     constexpr int CHUNKS = DP / 16, KB = KT / 32, DB = DP / 32;
@@ -58,11 +102,19 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F:
     KeyFeed<F, DP, KT> feed(lds, pieces, kp, vp, a.kt, a.vt);
     const typename T::Reader read(lds, lane);
     Op fq[CHUNKS];
+    float by_c = a.c, by_v = 1.f;         // what takes scores to powers of two, results to what they are
     {
         const bool live = row < a.rows;
         const char *const p = rows.at(live ? row : 0);
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) fq[c] = own_rows<F>(p, live, c, half, pieces);
+        const int eq = own_rows<F>(p, live, half, pieces, fq);
+        if constexpr (F::SCALED) {
+            // keys and values by the longest of theirs
+            const int ek = exponent_for(longest(a.k_levels, bh, a.level_tiles)), ev = exponent_for(longest(a.v_levels, bh, a.level_tiles));
+            feed.scale_a = __builtin_amdgcn_ldexpf(1.f, ek);
+            feed.scale_b = __builtin_amdgcn_ldexpf(1.f, ev);
+            by_c = fmaxf(__builtin_amdgcn_ldexpf(a.c, -(eq + ek)), 0x1p-126f);       // (not zero, by which -infinity is no number: scores of nothing either way)
+            by_v = __builtin_amdgcn_ldexpf(1.f, -ev);
+        }
     }
     ca_f32x16_t o[DB] = {};
     float most = -INFINITY, sum = 0.f;
@@ -90,8 +142,8 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F:
 #pragma unroll
             for (int e = 0; e < 16; ++e) now = fmaxf(now, s[kb][e]);
         now = of_both_halves(now, [](float x, float y) { return fmaxf(x, y); });
-        if (__any((now - most) * a.c > SLACK)) {             // (the first step's is: most is -infinity; -infinity - itself is no number, and not above)
-            const float to = fmaxf(most, now), by = most == to ? 1.f : __builtin_amdgcn_exp2f(most * a.c - to * a.c);
+        if (__any((now - most) * by_c > SLACK)) {             // (the first step's is: most is -infinity; -infinity - itself is no number, and not above)
+            const float to = fmaxf(most, now), by = most == to ? 1.f : __builtin_amdgcn_exp2f(most * by_c - to * by_c);
             sum *= by;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
@@ -99,13 +151,13 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F:
                 for (int e = 0; e < 16; ++e) o[d][e] *= by;
             most = to;
         }
-        const float less = (most == -INFINITY ? 0.f : most) * a.c - F::LIFT;
+        const float less = (most == -INFINITY ? 0.f : most) * by_c - F::LIFT;
         Op p[2 * KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], a.c, -less));
+                s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], by_c, -less));
                 sum += s[kb][e];
             }
 #pragma unroll
@@ -124,8 +176,8 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : DP <= 64 || F:
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
 
     sum = of_both_halves(sum, [](float x, float y) { return x + y; });
-    const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query without keys: zeros
-    const float level = sum == 0.f ? INFINITY : (most == -INFINITY ? 0.f : most) * a.c - F::LIFT + __builtin_amdgcn_logf(sum);
+    const float inverse = sum == 0.f ? 0.f : by_v / sum;     // a query without keys: zeros
+    const float level = sum == 0.f ? INFINITY : (most == -INFINITY ? 0.f : most) * by_c - F::LIFT + __builtin_amdgcn_logf(sum);
     const bool live = row < a.rows;
     const int64_t at = int64_t(bh) * a.rows + row;
     if (a.splits > 1) {
@@ -372,6 +424,11 @@ constexpr int64_t COMPUTE_UNITS = 256;    // a tile each and more: the keys are 
 constexpr int64_t WANTED = 512;           // workgroups, where there are keys enough to share out
 constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
 
+// fp32: from where two terms of half precision are faster, with the look at keys and values that they take.  us, three terms and two, batch x rows x keys x heads x
+// columns: 1 x 512 x 512 x 12 x 64 22, 27; 8 x 512 x 512 x 8 x 32 22, 23; 8 x 256 x 256 x 8 x 128 42, 35; 4 x 512 x 512 x 12 x 64 39, 37; 1 x 1024 x 1024 x 8 x 128 54, 42;
+// 16 x 4096 x 77 x 8 x 64 109, 100; fewer rows: 16 x 128 x 512 x 12 x 64 37, 42; 64 x 128 x 512 x 12 x 64 94, 98; 32 x 64 x 1024 x 8 x 64 59, 67.
+constexpr int64_t TWO_LEAST_ROWS = 256;   // of a key head
+constexpr double TWO_LEAST_PRODUCTS = 5e8;        // multiply-adds of scores
 constexpr int64_t FEW_WANTED = 4096;      // few_rows_kernel: wavefronts
 
 // Lanes that have a key in few_rows_kernel.
@@ -407,13 +464,20 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
         if (splits > rounds / a.few_waves) splits = rounds / a.few_waves;
     }
     if (splits < 1) splits = 1;
+    // fp32 numbers in two terms: where the products that this saves cost more than the look at keys and values
+    const bool two = c.format == LFFN_ROWS_F32 && !a.few_waves && a.rows >= TWO_LEAST_ROWS &&
+                     (double)tiles * TILE * (double)c.k_len * (double)c.columns >= TWO_LEAST_PRODUCTS;
+    a.level_tiles = two ? int((c.k_len + LEVEL_ROWS - 1) / LEVEL_ROWS) : 0;
+    a.level_by = Divisor(a.level_tiles > 0 ? (uint32_t)a.level_tiles : 1);
     a.split_steps = (a.steps + splits - 1) / splits;
     a.splits = a.split_steps ? int((a.steps + a.split_steps - 1) / a.split_steps) : 1;
     a.group = Divisor(group > 0 ? (uint32_t)group : 1), a.heads = Divisor((uint32_t)a.key_heads);
     a.tiles = Divisor(a.row_tiles > 0 ? (uint32_t)a.row_tiles : 1), a.split_by = Divisor((uint32_t)a.splits);
     if (tiles > INT32_MAX / a.splits) return -1;
     a.units = int(tiles * a.splits);
-    return a.splits > 1 ? int64_t(a.splits) * c.B * c.key_heads * a.rows * (a.columns + 1) * 4 : 0;
+    const int64_t batch_heads = c.B * c.key_heads;
+    if (batch_heads * a.level_tiles > INT32_MAX) return -1;
+    return (2 * batch_heads * a.level_tiles + (a.splits > 1 ? a.splits * batch_heads * a.rows * (a.columns + 1) : 0)) * 4;
 }
 
 template <typename F>
@@ -490,13 +554,24 @@ extern "C" int lffn_cross_attention_fwd(const lffn_cross_attention *c, void *out
     LFFN_REQUIRE(bytes == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= bytes), LFFN_ERR_BAD_ARG);
     const Kept k = kept_at(kept, c->B * c->q_len * c->heads, c->format == LFFN_ROWS_F32 ? 4 : 2);
     a.out = static_cast<char *>(out), a.lse = k.levels, a.rest = k.rest;
-    a.part = static_cast<float *>(workspace);
-    a.part_lse = a.part ? a.part + int64_t(a.splits) * c->B * c->key_heads * a.rows * a.columns : nullptr;
+    // (parts first: they are read 16 bytes at a time)
+    float *at = static_cast<float *>(workspace);
+    const int64_t batch_heads = c->B * c->key_heads;
+    if (a.splits > 1) {
+        a.part = at;
+        a.part_lse = at + a.splits * batch_heads * a.rows * a.columns;
+        at = a.part_lse + a.splits * batch_heads * a.rows;
+    }
+    if (a.level_tiles) a.k_levels = at, a.v_levels = at + batch_heads * a.level_tiles;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a.few_waves) {
         const int lanes = lanes_of_a_key(*c);
         if (c->format == LFFN_ROWS_F32) return launch_few<F32, F32Row>(a, lanes, s);
         return c->format == LFFN_ROWS_BF16 ? launch_few<BF16, BF16Row>(a, lanes, s) : launch_few<F16, F16Row>(a, lanes, s);
+    }
+    if (a.level_tiles) {
+        levels_kernel<<<dim3((unsigned)(batch_heads * a.level_tiles)), dim3(WG), 0, s>>>(a);
+        return launch<F32Two>(a, s);
     }
     if (c->format == LFFN_ROWS_F32) return launch<F32>(a, s);
     return c->format == LFFN_ROWS_BF16 ? launch<BF16>(a, s) : launch<F16>(a, s);

@@ -7,8 +7,10 @@
 // has one owner and a fixed order: no atomics, the same bits on every call.  Where there are too few standing rows or keys to fill
 // the chip what passes is shared out over several workgroups, and a last kernel adds their sums.
 //
-// Half precision: p is held 2^14 times larger (at most 2^14), ds times a power of two that takes 2 |g| |v|, of the longest
-// rows of the batch and key head, which no ds exceeds, below 2^15: gradients of any size, and weights of many keys, stay among half's normal numbers.
+// Half precision, and fp32 numbers in two terms of it: p is held 2^14 times larger (at most 2^14), ds times a power of two that takes 2 |g| |v|, of the
+// longest rows of the batch and key head, which no ds exceeds, below 2^15: gradients of any size, and weights of many keys, stay among half's normal numbers.
+// fp32 numbers are scaled by the longest rows of q, k, v and g in the same way, and p and ds once more by what a key's, or a query's, largest so far leaves
+// of half's range (fit).
 #include "cross_attention.h"
 
 using namespace cross_attention;
@@ -17,120 +19,126 @@ __attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(co
 
 namespace {
 
-constexpr int NORM_ROWS = 128;            // rows of a workgroup of delta_kernel, 8 to a group of 16 lanes, asked for together
-constexpr float P_LIFT = 14.f;            // half precision
+constexpr float P_LIFT = 14.f;            // half precision, one term or two
 
 struct BwdArgs {
     const char *q, *k, *v, *out, *rest, *g;
     const uint8_t *mask;
     const float *lse;
     char *gq, *gk, *gv;
-    float *delta, *g_norms, *v_norms;     // [B, key heads, rows]; squares of the longest rows: [B, key heads, tiles]
+    float *delta;                         // [B, key heads, rows]
+    float *g_levels, *q_levels, *v_levels, *k_levels;                // log2 of the longest rows, [B, key heads, g_tiles or v_tiles]
     float *part;                          // [splits, B, key heads, rows or keys, columns] (keys: of k, then of v)
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, mask_stride;         // strides in bytes
     int64_t keys, steps, split_steps, q_len;
-    Divisor group, tile_by, split_by, heads, norm_tiles; // query heads of a key head, standing tiles, shares of what passes, key heads, delta_kernel's tiles
+    Divisor group, tile_by, split_by, heads, level_tiles; // query heads of a key head, standing tiles, shares of what passes, key heads, delta_kernel's tiles
     int64_t units;
     int batch_heads, key_heads, rows, tiles, splits, columns, g_tiles, v_tiles;
     float c, scale;
 };
 
-// Largest of v over the wavefront
-__device__ __forceinline__ float wave_most(float v) {
-    v = fmaxf(v, lane_xor<1>(v));
-    v = fmaxf(v, lane_xor<2>(v));
-    v = fmaxf(v, lane_xor<4>(v));
-    v = fmaxf(v, lane_xor<8>(v));
-    v = fmaxf(v, lane_xor<16>(v));
-    return fmaxf(v, lane_xor<32>(v));
-}
-
-// delta of every row; half precision: the longest rows of g and v as well.  16 lanes a row, 8 columns a lane.  Bound by memory: out, its rest and g (and v) once.
-// (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16 65 us.)
-template <typename F, bool NORMS>
+// delta of every row; half precision: the longest rows of g and v as well; fp32 numbers in two terms: of q and k, too.  16 lanes a row, 8 columns a lane, 8 rows to a group of
+// lanes, asked for together.  Bound by memory: out, its rest and g (and v, q, k) once.  (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16
+// 65 us, so 13.)
+template <typename F, bool LEVELS>
 __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
-    constexpr int EACH = NORM_ROWS / (WG / 16);
+    constexpr int EACH = LEVEL_ROWS / (WG / 16);
     const int lane = threadIdx.x & 15, tiles = a.g_tiles + a.v_tiles;
     const bool on = lane * 8 < a.columns;
     const int col = on ? lane * 8 : 0;
-    const int bh = a.norm_tiles.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * tiles;
-    float most = 0.f;
+    const int bh = a.level_tiles.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * tiles;
+    float most[2] = {-INFINITY, -INFINITY};             // of g and q, or v and k
+    auto look = [&](int n, const typename F::Raw &r, bool live) {
+        float v[8];
+        F::unpack(on ? r : F::zero(), v);
+        const float l = row_level(v);
+        if (live) most[n] = fmaxf(most[n], l);
+    };
     if (tile < a.g_tiles) {
-        typename F::Raw o[EACH], g[EACH], rest[F::PLANES == 1 ? EACH : 1];
-        const int first = tile * NORM_ROWS + threadIdx.x / 16;
+        typename F::Raw o[EACH], g[EACH], rest[F::BYTES == 2 ? EACH : 1], q[F::SCALED ? EACH : 1];
+        const int first = tile * LEVEL_ROWS + threadIdx.x / 16;
+        const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int row = min(first + i * (WG / 16), a.rows - 1);
             const int64_t at = (heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES;
             o[i] = F::load(a.out + at);
             g[i] = F::load(a.g + at);
-            if constexpr (F::PLANES == 1) rest[i] = F::load(a.rest + at);
+            if constexpr (F::BYTES == 2) rest[i] = F::load(a.rest + at);
+            if constexpr (F::SCALED) q[i] = F::load(rows.at(row) + col * F::BYTES);
         }
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            float dot = 0.f, squares = 0.f, u[8], v[8];
+            float dot = 0.f, u[8], v[8];
             F::unpack(o[i], u);
             F::unpack(g[i], v);
-            if constexpr (F::PLANES == 1) {
+            if constexpr (F::BYTES == 2) {
                 float w[8];
                 F::unpack(rest[i], w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) u[e] += w[e];
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot), squares = fmaf(v[e], v[e], squares);
+            for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
             dot = lane_group_sum<16>(on ? dot : 0.f);
-            if (NORMS) most = fmaxf(most, lane_group_sum<16>(on ? squares : 0.f));
             const int row = first + i * (WG / 16);
             if (lane == 0 && row < a.rows) a.delta[int64_t(bh) * a.rows + row] = dot;
+            if (LEVELS) look(0, g[i], true);            // (a row once more changes nothing)
+            if constexpr (F::SCALED) look(1, q[i], true);
         }
-    } else if (NORMS) {
-        typename F::Raw x[EACH];
+    } else if (LEVELS) {
+        typename F::Raw v[EACH], k[F::SCALED ? EACH : 1];
         bool live[EACH];
-        const int64_t first = int64_t(tile - a.g_tiles) * NORM_ROWS + threadIdx.x / 16;
+        const int64_t first = int64_t(tile - a.g_tiles) * LEVEL_ROWS + threadIdx.x / 16;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int64_t key = first + i * (WG / 16), at = key < a.keys ? key : a.keys - 1;
             live[i] = !a.mask || a.mask[b * a.mask_stride + at] != 0;
-            x[i] = F::load(a.v + b * a.vb + kh * a.vh + at * a.vt + col * F::BYTES);
+            v[i] = F::load(a.v + b * a.vb + kh * a.vh + at * a.vt + col * F::BYTES);
+            if constexpr (F::SCALED) k[i] = F::load(a.k + b * a.kb + kh * a.kh + at * a.kt + col * F::BYTES);
         }
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            float squares = 0.f, v[8];
-            F::unpack(x[i], v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) squares = fmaf(v[e], v[e], squares);
-            squares = lane_group_sum<16>(on ? squares : 0.f);
-            if (live[i]) most = fmaxf(most, squares);
+            look(0, v[i], live[i]);
+            if constexpr (F::SCALED) look(1, k[i], live[i]);
         }
     }
-    if (NORMS) {
-        __shared__ float red[WAVES];
-        most = wave_most(most);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+    if (LEVELS) {
+        __shared__ float red[2][WAVES];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            most[n] = fmaxf(most[n], lane_xor<16>(most[n]));
+            most[n] = fmaxf(most[n], lane_xor<32>(most[n]));
+            if ((threadIdx.x & 63) == 0) red[n][threadIdx.x >> 6] = most[n];
+        }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-            if (tile < a.g_tiles) a.g_norms[int64_t(bh) * a.g_tiles + tile] = most;
-            else a.v_norms[int64_t(bh) * a.v_tiles + tile - a.g_tiles] = most;
+        if (threadIdx.x < (F::SCALED ? 2 : 1)) {
+            const float *const r = red[threadIdx.x];
+            const float all = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+            if (tile < a.g_tiles) (threadIdx.x ? a.q_levels : a.g_levels)[int64_t(bh) * a.g_tiles + tile] = all;
+            else (threadIdx.x ? a.k_levels : a.v_levels)[int64_t(bh) * a.v_tiles + tile - a.g_tiles] = all;
         }
     }
 }
 
-// What ds is multiplied with, as an exponent; half precision alone.
+// The powers of two that everything is multiplied with, as exponents: ds, and of fp32 numbers in two terms q, k, v and g.
+struct Exponents {
+    int ds, q, k, v, g;
+};
 template <typename F>
-__device__ __forceinline__ int ds_exponent(const BwdArgs &a, int64_t bh) {
-    if constexpr (F::LIFT == 0.f) return 0;
-    if (a.g_tiles == 0 || a.v_tiles == 0) return 0;
-    const float *const gs = a.g_norms + bh * a.g_tiles, *const vs = a.v_norms + bh * a.v_tiles;
-    const int lane = threadIdx.x & 63;
-    float g = gs[min(lane, a.g_tiles - 1)], v = vs[min(lane, a.v_tiles - 1)];
-    for (int i = lane + 64; i < a.g_tiles; i += 64) g = fmaxf(g, gs[i]);
-    for (int i = lane + 64; i < a.v_tiles; i += 64) v = fmaxf(v, vs[i]);
-    const float most = 2.f * sqrtf(wave_most(g)) * sqrtf(wave_most(v));
-    const int e = int(__float_as_uint(most) >> 23) - 127;    // most < 2^(e + 1)
-    return most > 0.f && e < 128 ? __builtin_amdgcn_readfirstlane(min(max(14 - e, -60), 60)) : 0;
+__device__ __forceinline__ Exponents exponents(const BwdArgs &a, int64_t bh) {
+    Exponents e{};
+    if constexpr (F::LIFT != 0.f) {
+        const float g = longest(a.g_levels, bh, a.g_tiles), v = longest(a.v_levels, bh, a.v_tiles);
+        if (g != -INFINITY && v != -INFINITY) e.ds = 14 - (int)ceilf(1.f + g + v);
+        if constexpr (F::SCALED) {
+            e.q = exponent_for(longest(a.q_levels, bh, a.g_tiles)), e.k = exponent_for(longest(a.k_levels, bh, a.v_tiles));
+            e.v = exponent_for(v), e.g = exponent_for(g);
+        }
+    }
+    return e;
 }
+__device__ __forceinline__ float power(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
 template <typename F, int DP, int KT>
 __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1 || DP <= 64 ? 2 : 1) void query_gradient_kernel(BwdArgs a) {
@@ -151,19 +159,16 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     KeyFeed<F, DP, KT> feed(lds, pieces, kp, vp, a.kt, a.vt);
     const typename T::Reader read(lds, lane);
     const int64_t out_row = heads_row(b, kh, live ? row : 0, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES;
+    const Exponents e2 = exponents<F>(a, bh);
+    if constexpr (F::SCALED) feed.scale_a = power(e2.k), feed.scale_b = power(e2.v);
     Op fq[CHUNKS], fg[CHUNKS];
-    {
-        const char *const p = Rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group}.at(live ? row : 0);
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            fq[c] = own_rows<F>(p, live, c, half, pieces);
-            fg[c] = own_rows<F>(a.g + out_row, live, c, half, pieces);
-        }
-    }
-    const int lift = ds_exponent<F>(a, bh);
-    const float f = __builtin_amdgcn_ldexpf(1.f, lift);
-    const float level = live ? a.lse[int64_t(bh) * a.rows + row] : INFINITY, delta = live ? a.delta[int64_t(bh) * a.rows + row] * f : 0.f;
+    const int eq = own_rows<F>(Rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group}.at(live ? row : 0), live, half, pieces, fq);
+    const int eg = own_rows<F>(a.g + out_row, live, half, pieces, fg);
+    const float f = power(e2.ds - eg - e2.v), by_c = __builtin_amdgcn_ldexpf(a.c, -(eq + e2.k));
+    const float level = live ? a.lse[int64_t(bh) * a.rows + row] : INFINITY;
+    const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], e2.ds) : 0.f;
     ca_f32x16_t dq[DB] = {};
+    int fitted = F::SCALED ? FIT_FIRST : 0;
 
     const bool wave_works = tile * TILE + wave * ROWS < a.rows;
     auto compute = [&](auto buf, uint64_t word) {
@@ -177,7 +182,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
                 else s = F::mma(x, fq[i / 2], s);
             });
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -level)) * fmaf(dp[e], f, -delta);
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], by_c, -level)) * fmaf(dp[e], f, -delta);
             const uint32_t part = (uint32_t)(word >> (32 * kb));
             if (part != ~0u) {
                 const uint32_t w = part >> (4 * half);
@@ -185,6 +190,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
                 for (int e = 0; e < 16; ++e)
                     if (!(w >> (8 * (e / 4) + e % 4) & 1)) s[e] = 0.f;
             }
+            if constexpr (F::SCALED) fit(s, fitted, dq);
             Op ds[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
 
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
-    const float by = __builtin_amdgcn_ldexpf(a.scale, -lift);
+    const float by = __builtin_amdgcn_ldexpf(a.scale, -(e2.ds + e2.k + fitted));
     if (a.splits > 1) store_row<F32, DB>(dq, by, reinterpret_cast<char *>(a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns), live, a.columns, half);
     else store_row<F, DB>(dq, by, a.gq + out_row, live, a.columns, half);
 }
@@ -225,21 +231,17 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
     // (a masked key is read as any other: what it holds stays in its own column, which is not stored)
     const uint8_t flag = a.mask ? a.mask[b * a.mask_stride + at_key] : 1;
     constexpr bool HALF = F::LIFT != 0.f;
-    const int lift = ds_exponent<F>(a, bh);
-    const float f = __builtin_amdgcn_ldexpf(1.f, HALF ? lift - int(P_LIFT) : 0);
+    const Exponents e2 = exponents<F>(a, bh);
+    const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
     Op fk[CHUNKS], fv[CHUNKS];
-    {
-        const char *const kp = a.k + b * a.kb + kh * a.kh + at_key * a.kt, *const vp = a.v + b * a.vb + kh * a.vh + at_key * a.vt;
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            fk[c] = own_rows<F>(kp, true, c, half, pieces);
-            fv[c] = own_rows<F>(vp, true, c, half, pieces);
-        }
-    }
+    const int ek = own_rows<F>(a.k + b * a.kb + kh * a.kh + at_key * a.kt, true, half, pieces, fk);
+    const int ev = own_rows<F>(a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, fv);
+    const float f = power(of_delta - e2.g - ev), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + ek));
 
     // Rows beyond the last are the last once more: their levels are infinite and so their weights zero.  A step's addresses go by its first token; where
     // the heads that share a key divide KT they are the same for every step.
     Feed<F, DP, KT> feed(lds, pieces);
+    if constexpr (F::SCALED) feed.scale_a = power(e2.q), feed.scale_b = power(e2.g);
     const typename T::Reader read(lds, lane);
     const bool even = KT % a.group.by == 0;
     const int64_t g_token = int64_t(a.key_heads) * a.group.by * a.columns * F::BYTES;
@@ -266,12 +268,13 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
         if (tid < KT) {
             const bool on = int(step) * KT + tid < a.rows;
             levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
-            levels[buf * 2 * KT + KT + tid] = on ? delta * f : 0.f;
+            levels[buf * 2 * KT + KT + tid] = on ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
         }
         feed.end(buf);
     };
 
     ca_f32x16_t dk[DB] = {}, dv[DB] = {};
+    int fitted_p = F::SCALED ? FIT_FIRST : 0, fitted_ds = fitted_p;
     auto compute = [&](auto buf) {
         constexpr int QUERIES = decltype(buf)::value * 2 * T::SIZE, GRADIENTS = QUERIES + T::SIZE;
         const float *const level = levels + decltype(buf)::value * 2 * KT + 4 * half, *const delta = level + KT;
@@ -288,11 +291,12 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
                 const float ls[4] = {l.x, l.y, l.z, l.w}, ds[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.c, -ls[e]));
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], by_c, -ls[e]));
                     s[4 * g + e] = p;
                     dp[4 * g + e] = p * fmaf(dp[4 * g + e], f, -ds[e]);
                 }
             }
+            if constexpr (F::SCALED) fit(s, fitted_p, dv), fit(dp, fitted_ds, dk);
             Op p[2], ds[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -333,7 +337,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
 #pragma unroll
         for (int d = 0; d < DB; ++d) dk[d] = ca_f32x16_t{}, dv[d] = ca_f32x16_t{};
     }
-    const float by_k = __builtin_amdgcn_ldexpf(a.scale, -lift), by_v = HALF ? 1.f / 16384.f : 1.f;
+    const float by_k = __builtin_amdgcn_ldexpf(a.scale, -(e2.ds + e2.q + fitted_ds)), by_v = power((HALF ? -int(P_LIFT) : 0) - e2.g - fitted_p);
     if (a.splits > 1) {
         const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key) * a.columns;
         store_row<F32, DB>(dk, by_k, reinterpret_cast<char *>(a.part + of), in, a.columns, half);
@@ -379,14 +383,11 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
         }
     }
     constexpr bool HALF = F::LIFT != 0.f;
-    const int lift = ds_exponent<F>(a, bh);
-    const float f = __builtin_amdgcn_ldexpf(1.f, HALF ? lift - int(P_LIFT) : 0);
+    const Exponents e2 = exponents<F>(a, bh);
+    const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
     Op own[CHUNKS];                       // the weights' wavefront: keys; the other: values
-    {
-        const char *const p = OF_V ? a.k + b * a.kb + kh * a.kh + at_key * a.kt : a.v + b * a.vb + kh * a.vh + at_key * a.vt;
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) own[c] = own_rows<F>(p, true, c, half, pieces);
-    }
+    const int of_own = own_rows<F>(OF_V ? a.k + b * a.kb + kh * a.kh + at_key * a.kt : a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, own);
+    const float f = power(of_delta - e2.g - of_own), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + of_own));
 
     const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
     const int64_t g_token = int64_t(a.key_heads) * a.group.by * a.columns * F::BYTES;
@@ -426,7 +427,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
         if (tid < KT) {
             const bool on = int(step) * KT + tid < a.rows;
             levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
-            levels[buf * 2 * KT + KT + tid] = on ? delta * f : 0.f;
+            levels[buf * 2 * KT + KT + tid] = on ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
         }
         if constexpr (F::PLANES == 1) {
             arrived();
@@ -435,13 +436,14 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
             for (int i = 0; i < SHARE; ++i) {
                 int of, at, place;
                 piece_of(i, of, at, place);
-                T::put(lds + (buf * 2 + of) * T::SIZE, at, place, raw[i]);
+                T::put(lds + (buf * 2 + of) * T::SIZE, at, place, raw[i], power(of ? e2.g : e2.q));
             }
         }
     };
 
     const typename T::Reader read(lds, lane);
     ca_f32x16_t sums[DB] = {}, s;
+    int fitted = F::SCALED ? FIT_FIRST : 0;
     Op p[2];
     // scores and weights, or g . v, of a step
     auto first_half = [&](auto buf) {
@@ -455,7 +457,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
                 const float4 l = *reinterpret_cast<const float4 *>(levels + decltype(buf)::value * 2 * KT + 8 * g + 4 * half);
                 const float ls[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.c, -ls[e]));
+                for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], by_c, -ls[e]));
                 to[g * 64] = make_float4(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
             }
         } else {
@@ -475,6 +477,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
                 for (int e = 0; e < 4; ++e) s[4 * g + e] = ws[e] * fmaf(s[4 * g + e], f, -ds[e]);
             }
         }
+        if constexpr (F::SCALED) fit(s, fitted, sums);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             float t[8];
@@ -523,7 +526,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
 #pragma unroll
         for (int d = 0; d < DB; ++d) sums[d] = ca_f32x16_t{};
     }
-    const float by = OF_V ? (HALF ? 1.f / 16384.f : 1.f) : __builtin_amdgcn_ldexpf(a.scale, -lift);
+    const float by = OF_V ? power((HALF ? -int(P_LIFT) : 0) - e2.g - fitted) : __builtin_amdgcn_ldexpf(a.scale, -(e2.ds + e2.q + fitted));
     if (a.splits > 1) {
         const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key + (OF_V ? a.splits * all : 0)) * a.columns;
         store_row<F32, DB>(sums, by, reinterpret_cast<char *>(a.part + of), in, a.columns, half);
@@ -571,7 +574,7 @@ __global__ __launch_bounds__(WG) void add_splits_kernel(AddArgs a) {
 }
 
 // Which form of the keys' gradients heads of so many columns get.
-constexpr bool in_pairs(int planes, int columns) { return planes == 1 ? columns > 64 : columns > 32 && columns <= 64; }
+constexpr bool in_pairs(int planes, int columns) { return columns > (planes == 1 ? 64 : 32); }
 
 constexpr int64_t COMPUTE_UNITS = 256;    // standing tiles, and more: what passes is not shared out
 constexpr int64_t WANTED = 512;           // workgroups, where there is enough to share out
@@ -580,7 +583,7 @@ constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
 // The two large launches and where the workspace's parts begin (in floats).
 struct Plan {
     BwdArgs q{}, k{};
-    int64_t delta = 0, g_norms = 0, v_norms = 0, part = 0, floats = 0;
+    int64_t delta = 0, g_levels = 0, q_levels = 0, v_levels = 0, k_levels = 0, part = 0, floats = 0;
 };
 
 void share_out(BwdArgs &a, int64_t standing, int64_t passing, int kt, int64_t batch_heads) {
@@ -612,21 +615,23 @@ Plan plan(const lffn_cross_attention &c) {
     a.rows = int(c.q_len * group);
     a.group = Divisor(group > 0 ? (uint32_t)group : 1), a.heads = Divisor((uint32_t)a.key_heads);
     a.c = c.scale * LOG2E, a.scale = c.scale;
-    const bool norms = c.format == LFFN_ROWS_F16;
-    a.g_tiles = (a.rows + NORM_ROWS - 1) / NORM_ROWS;
-    a.v_tiles = norms ? int((a.keys + NORM_ROWS - 1) / NORM_ROWS) : 0;
-    a.norm_tiles = Divisor(a.g_tiles + a.v_tiles > 0 ? uint32_t(a.g_tiles + a.v_tiles) : 1);
+    const bool levels = c.format != LFFN_ROWS_BF16, scaled = c.format == LFFN_ROWS_F32;
+    a.g_tiles = (a.rows + LEVEL_ROWS - 1) / LEVEL_ROWS;
+    a.v_tiles = levels ? int((a.keys + LEVEL_ROWS - 1) / LEVEL_ROWS) : 0;
+    a.level_tiles = Divisor(a.g_tiles + a.v_tiles > 0 ? uint32_t(a.g_tiles + a.v_tiles) : 1);
     p.q = p.k = a;
     share_out(p.q, a.rows, a.keys, kt, batch_heads);
-    share_out(p.k, a.keys, a.rows, in_pairs(c.format == LFFN_ROWS_F32 ? 3 : 1, int(c.columns)) ? 32 : kt, batch_heads);
+    share_out(p.k, a.keys, a.rows, in_pairs(c.format == LFFN_ROWS_F32 ? 2 : 1, int(c.columns)) ? 32 : kt, batch_heads);
     auto take = [&](int64_t floats) {
         const int64_t at = p.floats;
         p.floats += (floats + 3) / 4 * 4;
         return at;
     };
     p.delta = take(batch_heads * a.rows);
-    p.g_norms = take(norms ? batch_heads * a.g_tiles : 0);
-    p.v_norms = take(batch_heads * a.v_tiles);
+    p.g_levels = take(levels ? batch_heads * a.g_tiles : 0);
+    p.q_levels = take(scaled ? batch_heads * a.g_tiles : 0);
+    p.v_levels = take(batch_heads * a.v_tiles);
+    p.k_levels = take(scaled ? batch_heads * a.v_tiles : 0);
     const int64_t of_q = p.q.splits > 1 ? p.q.splits * batch_heads * a.rows * a.columns : 0;
     const int64_t of_k = p.k.splits > 1 ? 2 * p.k.splits * batch_heads * a.keys * a.columns : 0;
     p.part = take(of_q > of_k ? of_q : of_k);             // (one launch's are added up before the next begins)
@@ -640,9 +645,9 @@ void add_splits(const AddArgs &a, int arrays, hipStream_t stream) {
 
 template <typename F, int DP, int KT>
 int launch(const Plan &p, hipStream_t stream) {
-    constexpr bool NORMS = F::LIFT != 0.f;
+    constexpr bool LEVELS = F::LIFT != 0.f;
     const int64_t tiles = int64_t(p.q.batch_heads) * (p.q.g_tiles + p.q.v_tiles);
-    if (tiles > 0) delta_kernel<F, NORMS><<<dim3((unsigned)tiles), dim3(WG), 0, stream>>>(p.q);
+    if (tiles > 0) delta_kernel<F, LEVELS><<<dim3((unsigned)tiles), dim3(WG), 0, stream>>>(p.q);
     if (p.q.units > 0) {
         static LdsGrant granted;
         const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + BLOCK * 8;
@@ -707,9 +712,9 @@ extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const voi
     for (BwdArgs *a : {&p.q, &p.k}) {
         a->out = static_cast<const char *>(out), a->g = static_cast<const char *>(g_out), a->lse = k.levels, a->rest = k.rest;
         a->gq = static_cast<char *>(grad_q), a->gk = static_cast<char *>(grad_k), a->gv = static_cast<char *>(grad_v);
-        a->delta = w + p.delta, a->g_norms = w + p.g_norms, a->v_norms = w + p.v_norms, a->part = w + p.part;
+        a->delta = w + p.delta, a->g_levels = w + p.g_levels, a->q_levels = w + p.q_levels, a->v_levels = w + p.v_levels, a->k_levels = w + p.k_levels, a->part = w + p.part;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (c->format == LFFN_ROWS_F32) return launch<F32>(p, s);
+    if (c->format == LFFN_ROWS_F32) return launch<F32Two>(p, s);
     return c->format == LFFN_ROWS_BF16 ? launch<BF16>(p, s) : launch<F16>(p, s);
 }
