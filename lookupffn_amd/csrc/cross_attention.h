@@ -545,12 +545,14 @@ __device__ __forceinline__ void walk_keys(KF &feed, uint64_t *words, const uint8
         uint64_t left = __ballot(words[lane] != 0);
         if (left) {
             uint64_t word, next = 0;
+            int64_t step, coming = 0;
             auto ask = [&](int buf) {                    // for the next step, if there is one
                 if (!left) return false;
                 const int i = __builtin_ctzll(left);
                 left &= left - 1;
                 next = uniform(words[i]);
-                feed.begin(buf, first + i, next);
+                coming = first + i;
+                feed.begin(buf, coming, next);
                 return true;
             };
             ask(0);
@@ -558,15 +560,15 @@ __device__ __forceinline__ void walk_keys(KF &feed, uint64_t *words, const uint8
             __syncthreads();
 #pragma unroll 1
             for (;;) {
-                word = next;
+                word = next, step = coming;
                 bool more = ask(1);
-                compute(std::integral_constant<int, 0>{}, word);
+                compute(std::integral_constant<int, 0>{}, word, step);
                 if (!more) break;
                 feed.end(1);
                 __syncthreads();
-                word = next;
+                word = next, step = coming;
                 more = ask(0);
-                compute(std::integral_constant<int, 1>{}, word);
+                compute(std::integral_constant<int, 1>{}, word, step);
                 if (!more) break;
                 feed.end(0);
                 __syncthreads();

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F:
     float most = -INFINITY, sum = 0.f;
 
     const bool wave_works = tile * TILE + wave * ROWS < a.rows;
-    auto compute = [&](auto buf, uint64_t word) {
+    auto compute = [&](auto buf, uint64_t word, int64_t) {
         if (!wave_works) return;
         constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
         ca_f32x16_t s[KB] = {};

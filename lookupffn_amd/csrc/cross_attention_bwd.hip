@@ -3,14 +3,16 @@
 //   delta_i = g_i . o_i;  p_ij = 2^(c s_ij - lse_i);  ds_ij = p_ij (g_i . v_j - delta_i)
 //   grad v_j = sum_i p_ij g_i;  grad k_j = scale sum_i ds_ij q_i;  grad q_i = scale sum_j ds_ij k_j
 // Three kernels: delta; the queries' gradients, a workgroup's 128 rows standing and the keys and values passing; the keys' and values', 128 keys
-// standing and the rows with their gradients passing.  Scores and g . v are formed twice (seven products for five), for that every sum
-// has one owner and a fixed order: no atomics, the same bits on every call.  Where there are too few standing rows or keys to fill
+// standing and the rows with their gradients passing.  Scores and g . v are formed twice (seven products for five; once where a key head has 128 rows at most, in one
+// kernel for both), for that every sum has one owner and a fixed order: no atomics, the same bits on every call.  Where there are too few standing rows or keys to fill
 // the chip what passes is shared out over several workgroups, and a last kernel adds their sums.
 //
 // Half precision, and fp32 numbers in two terms of it: p is held 2^14 times larger (at most 2^14), ds times a power of two that takes 2 |g| |v|, of the
 // longest rows of the batch and key head, which no ds exceeds, below 2^15: gradients of any size, and weights of many keys, stay among half's normal numbers.
 // fp32 numbers are scaled by the longest rows of q, k, v and g in the same way, and p and ds once more by what a key's, or a query's, largest so far leaves
 // of half's range (fit).
+#include <algorithm>
+
 #include "cross_attention.h"
 
 using namespace cross_attention;
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     int fitted = F::SCALED ? FIT_FIRST : 0;
 
     const bool wave_works = tile * TILE + wave * ROWS < a.rows;
-    auto compute = [&](auto buf, uint64_t word) {
+    auto compute = [&](auto buf, uint64_t word, int64_t) {
         if (!wave_works) return;
         constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
 #pragma unroll
@@ -209,6 +211,154 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     const float by = __builtin_amdgcn_ldexpf(a.scale, -(e2.ds + e2.k + fitted));
     if (a.splits > 1) store_row<F32, DB>(dq, by, reinterpret_cast<char *>(a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns), live, a.columns, half);
     else store_row<F, DB>(dq, by, a.gq + out_row, live, a.columns, half);
+}
+
+// All three gradients where the rows of a key head are 128 at most: they and their gradients stay in LDS, the keys pass 32 at a time, and of a step's keys
+// every sum over the rows is there at once, so that scores and g . v are formed once (five products for seven) and keys and values read once.  A wavefront has 32
+// rows: it forms their weights and ds with the step's keys, adds to their queries' gradients, and leaves both in LDS, turned round; then of the four tiles
+// of 32 columns x 32 keys, two of values' and two of keys' gradients, each wavefront forms one.  What it formed is stored in the next step, so that no step waits for a store.
+template <typename F>
+__global__ __launch_bounds__(WG, 2) void gradients_kernel(BwdArgs a) {
+    constexpr int DP = 64, KT = 32, CHUNKS = DP / 16, DB = DP / 32, OWN = TILE / 16;
+    typedef Tile<F, DP, TILE> Own;
+    typedef Tile<F, DP, KT> T;
+    typedef Tile<F, KT, TILE> Turned;
+    typedef Frag<1> Op;
+    static_assert(F::PLANES == 1 && DB * 2 == WAVES, "a tile of the results a wavefront");
+    extern __shared__ __attribute__((aligned(16))) uint4 lds[];           // rows, their gradients, [2][keys, values], weights, ds, words
+    constexpr int GRADIENTS_AT = Own::SIZE, PASSING = 2 * Own::SIZE, WEIGHTS = PASSING + 4 * T::SIZE, WORDS = WEIGHTS + 2 * Turned::SIZE;
+    uint64_t *const words = reinterpret_cast<uint64_t *>(lds + WORDS);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, half = lane >> 5;
+    const Unit unit = unit_of(blockIdx.x, a.units, a.tile_by, a.split_by, a.heads);
+    const int split = unit.split, bh = unit.bh, b = unit.b, kh = unit.kh;
+    const int pieces = a.columns / 8;
+    const char *const kp = a.k + b * a.kb + kh * a.kh, *const vp = a.v + b * a.vb + kh * a.vh;
+    const uint8_t *const mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+    const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
+    const int row = wave * ROWS + r;
+    const bool live = row < a.rows, wave_works = wave * ROWS < a.rows;
+
+    {
+        const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
+        const char *const gp = a.g + (b * a.q_len * a.key_heads + kh) * int64_t(a.group.by) * a.columns * F::BYTES;
+        Feed<F, DP, TILE> own(lds, pieces);
+        // (rows beyond the last are the last once more: their levels are infinite and so their weights zero)
+        own.begin(0, rows.base, gp, [&](int at, int) { const int i = min(at, a.rows - 1), t = a.group.quotient(i); return t * (uint32_t)a.qt + (i - t * a.group.by) * (uint32_t)a.qh; },
+                  [&](int at, int) {
+                      const int i = min(at, a.rows - 1), t = a.group.quotient(i);
+                      return (t * a.key_heads * a.group.by + (i - t * a.group.by)) * (uint32_t)(a.columns * F::BYTES);
+                  });
+        own.end(0);
+    }
+    // zeros for keys that take no part, and for the weights and ds of wavefronts without rows
+    auto result = [&](int64_t key) { return ((b * a.keys + key) * a.key_heads + kh) * int64_t(a.columns * F::BYTES); };
+    const uint4 zeros = make_uint4(0, 0, 0, 0);
+    if (mask) {
+        constexpr int EACH = 8, APART = WG / 8;
+        const int64_t last = end * KT < a.keys ? end * KT : a.keys;
+        const int piece = tid & 7;
+        for (int64_t first = begin * KT + tid / 8; first < last; first += EACH * APART) {
+            uint8_t flag[EACH];
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) flag[i] = mask[first + i * APART < last ? first + i * APART : last - 1];
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int64_t key = first + i * APART;
+                if (key < last && !flag[i] && piece < pieces) {
+                    *reinterpret_cast<uint4 *>(a.gk + result(key) + piece * 16) = zeros;
+                    *reinterpret_cast<uint4 *>(a.gv + result(key) + piece * 16) = zeros;
+                }
+            }
+        }
+    }
+    if (!wave_works) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) lds[WEIGHTS + wave * 128 + i * 64 + lane] = zeros, lds[WEIGHTS + Turned::SIZE + wave * 128 + i * 64 + lane] = zeros;
+    }
+    __syncthreads();
+
+    constexpr bool HALF = F::LIFT != 0.f;
+    const Exponents e2 = exponents<F>(a, bh);
+    const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
+    const float f = power(of_delta);
+    const float level = live ? a.lse[int64_t(bh) * a.rows + row] - (HALF ? P_LIFT : 0.f) : INFINITY;
+    const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], of_delta) : 0.f;
+    KeyFeed<F, DP, KT> feed(lds + PASSING, pieces, kp, vp, a.kt, a.vt);
+    const typename T::Reader read(lds + PASSING, lane);
+    const typename Own::Reader read_own(lds, lane);
+    Op fq[CHUNKS], fg[CHUNKS];
+    static_for<CHUNKS>([&](auto c) {      // (zeros beyond the columns, for what keys and values have there)
+        const bool on = 2 * c + half < pieces;
+        const Op q = read_own.rows(0, wave, c), g = read_own.rows(GRADIENTS_AT, wave, c);
+        fq[c] = {{on ? q.p[0] : zeros}}, fg[c] = {{on ? g.p[0] : zeros}};
+    });
+    ca_f32x16_t dq[DB] = {}, sum[1] = {};
+
+    // the wavefront's tile of the results
+    const int d = wave & 1;
+    const bool of_v = wave < 2;
+    const typename Turned::Reader read_turned(lds + WEIGHTS + (of_v ? 0 : Turned::SIZE), lane);
+    typename Own::Reader read_mine(lds + (of_v ? GRADIENTS_AT : 0), lane);
+    read_mine.lo[0] = d ? read_mine.lo[1] : read_mine.lo[0], read_mine.hi[0] = d ? read_mine.hi[1] : read_mine.hi[0];
+    const float by = of_v ? (HALF ? power(-int(P_LIFT)) : 1.f) : __builtin_amdgcn_ldexpf(a.scale, -e2.ds);
+    char *const to = (of_v ? a.gv : a.gk) + d * 32 * F::BYTES;
+    int64_t formed = -1;                  // the step that `sum` is of
+    uint32_t formed_word = 0;
+    auto store = [&]() {
+        if (formed < 0) return;
+        const bool in = formed_word >> r & 1;
+        store_row<F, 1>(sum, by, to + result(formed * KT + (in ? r : 0)), in, a.columns - 32 * d, half);
+    };
+    auto compute = [&](auto buf, uint64_t word, int64_t step) {
+        constexpr int KEYS = decltype(buf)::value * 2 * T::SIZE, VALUES = KEYS + T::SIZE;
+        store();
+        if (wave_works) {
+            ca_f32x16_t s = {}, dp = {};
+            products<F, 2 * CHUNKS>([&](auto i) { return read.rows(i % 2 ? VALUES : KEYS, 0, i / 2); }, [&](auto i, const Op &x) {
+                if constexpr (i % 2) dp = F::mma(x, fg[i / 2], dp);
+                else s = F::mma(x, fq[i / 2], s);
+            });
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -level));
+                dp[e] = s[e] * fmaf(dp[e], f, -delta);
+            }
+            if ((uint32_t)word != ~0u) {
+                const uint32_t w = (uint32_t)word >> (4 * half);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(w >> (8 * (e / 4) + e % 4) & 1)) s[e] = 0.f, dp[e] = 0.f;
+            }
+            Op p[2], ds[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float t[8], u[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = s[8 * c + e], u[e] = dp[8 * c + e];
+                p[c] = F::operand(t), ds[c] = F::operand(u);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint2 *const at = reinterpret_cast<uint2 *>(lds + WEIGHTS + Turned::at(row, 2 * c + i)) + half;
+                    at[0] = i ? make_uint2(p[c].p[0].z, p[c].p[0].w) : make_uint2(p[c].p[0].x, p[c].p[0].y);
+                    at[2 * Turned::SIZE] = i ? make_uint2(ds[c].p[0].z, ds[c].p[0].w) : make_uint2(ds[c].p[0].x, ds[c].p[0].y);
+                }
+            }
+            products<F, 2 * DB>([&](auto i) { return read.columns(KEYS, i / DB, i % DB); },
+                                [&](auto i, const Op &x) { dq[i % DB] = F::mma(x, ds[i / DB], dq[i % DB]); });
+        }
+        lds_barrier();                    // (copies on their way stay so)
+        sum[0] = ca_f32x16_t{};
+        Op x[OWN], y[OWN];
+        static_for<OWN>([&](auto c) { x[c] = read_mine.columns(0, c, 0), y[c] = read_turned.columns(0, c, 0); });
+        static_for<OWN>([&](auto c) { sum[0] = F::mma(x[c], y[c], sum[0]); });
+        formed = step, formed_word = (uint32_t)word;
+    };
+
+    walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
+    store();
+    const float by_q = __builtin_amdgcn_ldexpf(a.scale, -e2.ds);
+    if (a.splits > 1) store_row<F32, DB>(dq, by_q, reinterpret_cast<char *>(a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns), live, a.columns, half);
+    else store_row<F, DB>(dq, by_q, a.gq + heads_row(b, kh, live ? row : 0, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES, live, a.columns, half);
 }
 
 template <typename F, int DP, int KT>
@@ -543,7 +693,9 @@ __global__ __launch_bounds__(2 * WG, 2) void key_gradient_pairs_kernel(BwdArgs a
     else key_gradient_pairs<F, DP, 1>(a, lds);
 }
 
-// The splits' sums of a row as one, in their order, four of them asked for together; `second` beside `part` where there are two arrays.  Four columns a lane.
+// The splits' sums of a row as one, in a fixed order, four of them asked for together; `second` beside `part` where there are two arrays.  Four columns a lane; of
+// more splits than four each wavefront of a workgroup adds a share (1 x 128 rows, 128 splits of 4096 keys x 4 x 64 bfloat16: 12.7 us in one share,
+// 4.8 in four).
 struct AddArgs {
     const float *part[2];
     char *out[2];
@@ -551,23 +703,34 @@ struct AddArgs {
     Divisor heads, group;
     int rows, splits, columns;
 };
-template <typename F>
+template <typename F, int SHARES>
 __global__ __launch_bounds__(WG) void add_splits_kernel(AddArgs a) {
     constexpr int TOGETHER = 4;
-    const int quads = a.columns / 4;
-    const int64_t i = int64_t(blockIdx.x) * WG + threadIdx.x, at = i / quads;
-    const int col = int(i - at * quads) * 4;
-    if (at >= a.all) return;
+    const int quads = a.columns / 4, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = SHARES == 1 ? int64_t(blockIdx.x) * WG + threadIdx.x : int64_t(blockIdx.x) * 64 + lane, last = a.all * quads - 1, at = (i < last ? i : last) / quads;
+    const int col = int((i < last ? i : last) - at * quads) * 4;
     const float *const part = a.part[blockIdx.y] + at * a.columns + col;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int first = 0; first < a.splits; first += TOGETHER) {
+    for (int first = SHARES == 1 ? 0 : wave; first < a.splits; first += SHARES * TOGETHER) {
         float4 v[TOGETHER];
 #pragma unroll
-        for (int n = 0; n < TOGETHER; ++n) v[n] = *reinterpret_cast<const float4 *>(part + min(first + n, a.splits - 1) * a.all * a.columns);
+        for (int n = 0; n < TOGETHER; ++n) v[n] = *reinterpret_cast<const float4 *>(part + min(first + n * SHARES, a.splits - 1) * a.all * a.columns);
 #pragma unroll
         for (int n = 0; n < TOGETHER; ++n)
-            if (first + n < a.splits) acc.x += v[n].x, acc.y += v[n].y, acc.z += v[n].z, acc.w += v[n].w;
+            if (first + n * SHARES < a.splits) acc.x += v[n].x, acc.y += v[n].y, acc.z += v[n].z, acc.w += v[n].w;
     }
+    if constexpr (SHARES > 1) {
+        __shared__ float4 sums[SHARES][64];
+        sums[wave][lane] = acc;
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int n = 1; n < SHARES; ++n) {
+            const float4 v = sums[n][lane];
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        }
+    }
+    if (i > last) return;
     const int bh = int(at / a.rows), b = a.heads.quotient(bh), kh = bh - b * a.heads.by;
     F::store4(a.out[blockIdx.y] + (heads_row(b, kh, int(at - int64_t(bh) * a.rows), a.len, a.heads.by, a.group) * a.columns + col) * F::BYTES, acc.x, acc.y, acc.z,
               acc.w);
@@ -580,9 +743,14 @@ constexpr int64_t COMPUTE_UNITS = 256;    // standing tiles, and more: what pass
 constexpr int64_t WANTED = 512;           // workgroups, where there is enough to share out
 constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
 
-// The two large launches and where the workspace's parts begin (in floats).
+// All gradients in one kernel: where a key head's rows fit in LDS beside what passes.  us of a forward and backward, the gradients in two kernels and in one, batch x
+// rows x keys x key heads x columns: 64 x 128 x 512 x 8 x 64 half 116, 92 (the kernels alone 46 + 27, 45; at least 31 for its bytes); 64 x 32 91, 72; 64 x 1 71, 54;
+// 16 x 128 x 512 x 12 x 64 bfloat16 67, 59; 256 x 128 x 128 x 8 x 64 163, 143; 4 x 128 x 4096 x 8 x 64 67, 53; 1 x 128 x 4096 x 4 x 64 38, 34.
+constexpr bool in_one(int format, int64_t columns, int64_t rows) { return format != LFFN_ROWS_F32 && columns > 32 && columns <= 64 && rows <= TILE; }
+
+// The large launches, two or one, and where the workspace's parts begin (in floats).
 struct Plan {
-    BwdArgs q{}, k{};
+    BwdArgs q{}, k{}, both{};
     int64_t delta = 0, g_levels = 0, q_levels = 0, v_levels = 0, k_levels = 0, part = 0, floats = 0;
 };
 
@@ -619,7 +787,8 @@ Plan plan(const lffn_cross_attention &c) {
     a.g_tiles = (a.rows + LEVEL_ROWS - 1) / LEVEL_ROWS;
     a.v_tiles = levels ? int((a.keys + LEVEL_ROWS - 1) / LEVEL_ROWS) : 0;
     a.level_tiles = Divisor(a.g_tiles + a.v_tiles > 0 ? uint32_t(a.g_tiles + a.v_tiles) : 1);
-    p.q = p.k = a;
+    p.q = p.k = p.both = a;
+    if (in_one(c.format, c.columns, a.rows)) share_out(p.both, a.rows, a.keys, 32, batch_heads);
     share_out(p.q, a.rows, a.keys, kt, batch_heads);
     share_out(p.k, a.keys, a.rows, in_pairs(c.format == LFFN_ROWS_F32 ? 2 : 1, int(c.columns)) ? 32 : kt, batch_heads);
     auto take = [&](int64_t floats) {
@@ -634,13 +803,16 @@ Plan plan(const lffn_cross_attention &c) {
     p.k_levels = take(scaled ? batch_heads * a.v_tiles : 0);
     const int64_t of_q = p.q.splits > 1 ? p.q.splits * batch_heads * a.rows * a.columns : 0;
     const int64_t of_k = p.k.splits > 1 ? 2 * p.k.splits * batch_heads * a.keys * a.columns : 0;
-    p.part = take(of_q > of_k ? of_q : of_k);             // (one launch's are added up before the next begins)
+    const int64_t of_both = p.both.splits > 1 ? p.both.splits * batch_heads * a.rows * a.columns : 0;
+    p.part = take(std::max({of_q, of_k, of_both}));       // (one launch's are added up before the next begins)
     return p;
 }
 
 template <typename F>
 void add_splits(const AddArgs &a, int arrays, hipStream_t stream) {
-    add_splits_kernel<F><<<dim3((unsigned)((a.all * (a.columns / 4) + WG - 1) / WG), arrays), dim3(WG), 0, stream>>>(a);
+    const int64_t quads = a.all * (a.columns / 4);
+    if (a.splits > 4) add_splits_kernel<F, WAVES><<<dim3((unsigned)((quads + 63) / 64), arrays), dim3(WG), 0, stream>>>(a);
+    else add_splits_kernel<F, 1><<<dim3((unsigned)((quads + WG - 1) / WG), arrays), dim3(WG), 0, stream>>>(a);
 }
 
 template <typename F, int DP, int KT>
@@ -648,14 +820,26 @@ int launch(const Plan &p, hipStream_t stream) {
     constexpr bool LEVELS = F::LIFT != 0.f;
     const int64_t tiles = int64_t(p.q.batch_heads) * (p.q.g_tiles + p.q.v_tiles);
     if (tiles > 0) delta_kernel<F, LEVELS><<<dim3((unsigned)tiles), dim3(WG), 0, stream>>>(p.q);
+    auto add_queries = [&](const BwdArgs &q) {
+        if (q.splits > 1)
+            add_splits<F>({{q.part, nullptr}, {q.gq, nullptr}, int64_t(q.batch_heads) * q.rows, q.q_len, q.heads, q.group, q.rows, q.splits, q.columns}, 1, stream);
+    };
+    if constexpr (F::PLANES == 1 && DP == 64) {
+        if (p.both.units > 0 && p.q.units > 0 && p.k.units > 0) {
+            static LdsGrant granted;
+            const size_t bytes = (2 * Tile<F, DP, TILE>::SIZE + 4 * Tile<F, DP, 32>::SIZE + 2 * Tile<F, 32, TILE>::SIZE) * 16 + BLOCK * 8;
+            if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&gradients_kernel<F>), bytes, granted)) return LFFN_ERR_LAUNCH;
+            gradients_kernel<F><<<dim3((unsigned)p.both.units), dim3(WG), bytes, stream>>>(p.both);
+            add_queries(p.both);
+            return lffn_launch_status();
+        }
+    }
     if (p.q.units > 0) {
         static LdsGrant granted;
         const size_t bytes = 4 * Tile<F, DP, KT>::SIZE * 16 + BLOCK * 8;
         if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&query_gradient_kernel<F, DP, KT>), bytes, granted)) return LFFN_ERR_LAUNCH;
         query_gradient_kernel<F, DP, KT><<<dim3((unsigned)p.q.units), dim3(WG), bytes, stream>>>(p.q);
-        const BwdArgs &q = p.q;
-        if (q.splits > 1)
-            add_splits<F>({{q.part, nullptr}, {q.gq, nullptr}, int64_t(q.batch_heads) * q.rows, q.q_len, q.heads, q.group, q.rows, q.splits, q.columns}, 1, stream);
+        add_queries(p.q);
     }
     if (p.k.units > 0) {
         static LdsGrant granted;
@@ -705,11 +889,11 @@ extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const voi
     if (p.q.units == 0 && p.k.units == 0) return LFFN_OK;
     for (const void *t : {out, kept, g_out, (const void *)grad_q, (const void *)grad_k, (const void *)grad_v}) LFFN_REQUIRE(lffn_aligned16(t), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.floats == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= p.floats * 4), LFFN_ERR_BAD_ARG);
-    LFFN_REQUIRE(p.q.units <= INT32_MAX && p.k.units <= INT32_MAX &&
+    LFFN_REQUIRE(p.q.units <= INT32_MAX && p.k.units <= INT32_MAX && p.both.units <= INT32_MAX &&
                      int64_t(p.q.batch_heads) * (p.q.g_tiles + p.q.v_tiles) <= INT32_MAX, LFFN_ERR_UNSUPPORTED);
     float *const w = static_cast<float *>(workspace);
     const Kept k = kept_at(const_cast<void *>(kept), c->B * c->q_len * c->heads, c->format == LFFN_ROWS_F32 ? 4 : 2);
-    for (BwdArgs *a : {&p.q, &p.k}) {
+    for (BwdArgs *a : {&p.q, &p.k, &p.both}) {
         a->out = static_cast<const char *>(out), a->g = static_cast<const char *>(g_out), a->lse = k.levels, a->rest = k.rest;
         a->gq = static_cast<char *>(grad_q), a->gk = static_cast<char *>(grad_k), a->gv = static_cast<char *>(grad_v);
         a->delta = w + p.delta, a->g_levels = w + p.g_levels, a->q_levels = w + p.q_levels, a->v_levels = w + p.v_levels, a->k_levels = w + p.k_levels, a->part = w + p.part;
