@@ -92,9 +92,9 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, *, table=None, q_pos
 
         y = x / sqrt(mean(x^2) + eps) * weight;  (a, b) -> (a cos - b sin, b cos + a sin)
 
-    q: [B, L, heads, columns], k: [B, keys, key heads, columns] of the same type or None (single tokens against keys that are kept; their weight and positions are
-    then left alone), with any
-    strides (a copy is made where the columns do not lie together or not at multiples of 16 bytes).  columns: a multiple of 8, at most 256.
+    q: [B, L, heads, columns], k: [B, keys, key heads, columns] of the same type or None (single tokens against keys that are kept; their weight
+    and positions are then left alone), with any strides (a copy is made where the columns do not lie together or not at multiples of 16 bytes).
+    columns: a multiple of 8, at most 256.
     weights: [columns], float32 or of q's type, or None.  table: ``rotary_table`` or any [positions, rotated columns] float32 of cosines and then sines, or
     None for no rotation.  positions: int32 or int64, [L] or [B, L], or None for 0, 1, 2 ...; one outside the table takes its nearest row.  Pairs are columns
     (i, i + rotated / 2), with ``interleaved`` (2 i, 2 i + 1).  Norms and rotation in float32, one rounding.
@@ -155,8 +155,10 @@ def cross_attention(q, k, v, key_mask=None, *, scale=None):
     None; whatever keys and values that take no part hold.  A query without keys gets zeros (and gives none a gradient).
     scale: positive, 1 / sqrt(columns) if None.  One query a sequence is the step of a decoder over kept keys and values.
 
-    float32: products of three bfloat16 terms a number, sums in float32, as exact as a float32 product; 16 bits: softmax weights rounded to the
-    type, sums in float32, one rounding of the result.  Infinities and NaN of keys that take part may make any result of their head NaN.
+    float32: products of two half-precision or three bfloat16 terms a number, sums in float32, errors as those of a float32 product; with two terms (large
+    calls, and the backward) a number of k or v (backward: also q and the gradient) 2^14 times smaller than the longest row of its batch and head begins to lose
+    bits.  16 bits: softmax weights rounded to the type, sums in float32, one rounding of the result.  Infinities and NaN of keys that take part may
+    make any result of their head NaN.
     -> [B, L, heads, columns].  Gradients: q, k and v, the same bits on every call."""
     host = _host()
     if host:

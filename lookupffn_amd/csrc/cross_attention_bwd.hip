@@ -11,6 +11,8 @@
 // longest rows of the batch and key head, which no ds exceeds, below 2^15: gradients of any size, and weights of many keys, stay among half's normal numbers.
 // fp32 numbers are scaled by the longest rows of q, k, v and g in the same way, and p and ds once more by what a key's, or a query's, largest so far leaves
 // of half's range (fit).
+//
+// Bound by the products where there are many rows and keys: 4 x 2048 x 4096 x 16 x 128 bfloat16 keys' gradients 645 us (0.85 PFLOP/s), queries' 375 (1.1), delta 13.
 #include <algorithm>
 
 #include "cross_attention.h"

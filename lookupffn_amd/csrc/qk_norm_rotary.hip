@@ -8,6 +8,8 @@
 // vectors whose columns are each other's partners, so that the rotation stays in the lane; sine and cosine of a lane's columns (fp32: two
 // to four times a 16-bit row's bytes) are read once for several heads of a token.  Queries and keys are one launch: the workgroups
 // of one follow those of the other.
+// 16384 tokens of 12 + 12 heads of 64, fp32: 35.5 us for 201 MB; 2 x 32768 tokens of 8 heads of 64, half: forward 32 us for 134 MB, backward 44 for 201 and
+// 4 for the weights' partial sums (a copy moves 5.1 TB/s).
 #include "rows16.h"
 
 namespace {
