@@ -934,6 +934,7 @@ int lffn_qk_norm_rotary_bwd(const lffn_qk_norm_rotary *a, const void *g_q, const
  * batch stride, or NULL.  What keys and values that take no part hold does not matter.  A query without keys gets zeros.  scale: positive, finite.
  * format 0: fp32 accuracy (2e-7 of the result's norm against 64 bits), but keys and values, in the backward queries and
  * gradients too, may be held to 2^-36 of the longest such row of the batch and key head; 1 and 2: products of 16 bits, sums in fp32, softmax weights rounded to the format.
+ * A launch has fewer than 2^32 threads (B * key_heads below some 4 million with single tokens and many keys, 8 million in the backward), else LFFN_ERR_UNSUPPORTED.
  * out: [B, q_len, heads, columns], in the format.  kept: what the backward needs beside out (private to it), of lffn_cross_attention_kept_bytes, 16-byte aligned,
  * or NULL.  workspace: 16-byte aligned, of lffn_cross_attention_workspace_bytes (0: may be NULL).
  */

@@ -159,7 +159,8 @@ def cross_attention(q, k, v, key_mask=None, *, scale=None):
     calls, and the backward) a number of k or v (backward: also q and the gradient) 2^14 times smaller than the longest row of its batch and head begins to lose
     bits.  16 bits: softmax weights rounded to the type, sums in float32, one rounding of the result.  Infinities and NaN of keys that take part may
     make any result of their head NaN.
-    -> [B, L, heads, columns].  Gradients: q, k and v, the same bits on every call."""
+    -> [B, L, heads, columns].  Gradients: q, k and v, the same bits on every call.  A step with its backward can be captured in a graph, but not while
+    an earlier graph holds its leaves (RuntimeError)."""
     host = _host()
     if host:
         out = host.cross_attention(q, k, v, key_mask, scale)

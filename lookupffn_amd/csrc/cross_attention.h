@@ -598,6 +598,9 @@ inline Kept kept_at(void *p, int64_t rows, int bytes) {
 }
 
 // Which unit of work a workgroup has: neighbours (tiles that read the same keys) on one XCD.
+// Threads of a launch at most.
+constexpr int64_t MOST_THREADS = UINT32_MAX;
+
 struct Unit {
     int tile, split, bh, b, kh;
 };

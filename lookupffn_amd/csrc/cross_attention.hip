@@ -477,10 +477,10 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     a.splits = a.split_steps ? int((a.steps + a.split_steps - 1) / a.split_steps) : 1;
     a.group = Divisor(group > 0 ? (uint32_t)group : 1), a.heads = Divisor((uint32_t)a.key_heads);
     a.tiles = Divisor(a.row_tiles > 0 ? (uint32_t)a.row_tiles : 1), a.split_by = Divisor((uint32_t)a.splits);
-    if (tiles > INT32_MAX / a.splits) return -1;
+    if (tiles > MOST_THREADS / (a.few_waves ? 64 * a.few_waves : WG) / a.splits) return -1;
     a.units = int(tiles * a.splits);
     const int64_t batch_heads = c.B * c.key_heads;
-    if (batch_heads * a.level_tiles > INT32_MAX) return -1;
+    if (batch_heads * a.level_tiles > MOST_THREADS / WG) return -1;
     return (2 * batch_heads * a.level_tiles + (a.splits > 1 ? a.splits * batch_heads * a.rows * (a.columns + 1) : 0)) * 4;
 }
 

@@ -753,6 +753,7 @@ constexpr bool in_one(int format, int64_t columns, int64_t rows) { return format
 // The large launches, two or one, and where the workspace's parts begin (in floats).
 struct Plan {
     BwdArgs q{}, k{}, both{};
+    bool fits = true;                     // every launch
     int64_t delta = 0, g_levels = 0, q_levels = 0, v_levels = 0, k_levels = 0, part = 0, floats = 0;
 };
 
@@ -793,6 +794,7 @@ Plan plan(const lffn_cross_attention &c) {
     if (in_one(c.format, c.columns, a.rows)) share_out(p.both, a.rows, a.keys, 32, batch_heads);
     share_out(p.q, a.rows, a.keys, kt, batch_heads);
     share_out(p.k, a.keys, a.rows, in_pairs(c.format == LFFN_ROWS_F32 ? 2 : 1, int(c.columns)) ? 32 : kt, batch_heads);
+    p.fits = std::max({p.q.units, 2 * p.k.units, p.both.units, batch_heads * (a.g_tiles + a.v_tiles)}) <= MOST_THREADS / WG;
     auto take = [&](int64_t floats) {
         const int64_t at = p.floats;
         p.floats += (floats + 3) / 4 * 4;
@@ -875,7 +877,9 @@ int launch(const Plan &p, hipStream_t stream) {
 extern "C" int lffn_cross_attention_bwd_workspace_bytes(const lffn_cross_attention *c, int64_t *bytes) {
     LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
     if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
-    *bytes = plan(*c).floats * 4;
+    const Plan p = plan(*c);
+    LFFN_REQUIRE(p.fits, LFFN_ERR_UNSUPPORTED);
+    *bytes = p.floats * 4;
     return LFFN_OK;
 }
 
@@ -883,6 +887,7 @@ extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const voi
                                         void *grad_k, void *grad_v, void *workspace, int64_t workspace_bytes, void *stream) {
     if (const int rc = lffn_internal_cross_attention_check(c)) return rc;
     Plan p = plan(*c);
+    LFFN_REQUIRE(p.fits, LFFN_ERR_UNSUPPORTED);
     if (p.q.units == 0 && p.k.units == 0) return LFFN_OK;
     LFFN_REQUIRE(p.q.units == 0 || (out && kept && g_out), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.k.units == 0 || (grad_k != nullptr) == (grad_v != nullptr), LFFN_ERR_BAD_ARG);
@@ -891,8 +896,6 @@ extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const voi
     if (p.q.units == 0 && p.k.units == 0) return LFFN_OK;
     for (const void *t : {out, kept, g_out, (const void *)grad_q, (const void *)grad_k, (const void *)grad_v}) LFFN_REQUIRE(lffn_aligned16(t), LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(p.floats == 0 || (workspace && lffn_aligned16(workspace) && workspace_bytes >= p.floats * 4), LFFN_ERR_BAD_ARG);
-    LFFN_REQUIRE(p.q.units <= INT32_MAX && p.k.units <= INT32_MAX && p.both.units <= INT32_MAX &&
-                     int64_t(p.q.batch_heads) * (p.q.g_tiles + p.q.v_tiles) <= INT32_MAX, LFFN_ERR_UNSUPPORTED);
     float *const w = static_cast<float *>(workspace);
     const Kept k = kept_at(const_cast<void *>(kept), c->B * c->q_len * c->heads, c->format == LFFN_ROWS_F32 ? 4 : 2);
     for (BwdArgs *a : {&p.q, &p.k, &p.both}) {

@@ -80,6 +80,20 @@ bool any_gradient(std::initializer_list<const Tensor *> tensors) {
     return false;
 }
 
+// A backward that is captured must not meet a leaf whose gradient accumulates on another stream, as it does while a graph from before the capture holds it: the
+// engine then has the captured stream wait for that one, and the process ends in its thread.  Refused here, where it can be raised.
+void refuse_foreign_leaves(std::initializer_list<const Tensor *> tensors, const at::Device &dev) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(stream_on(dev)), &capture) != hipSuccess || capture == hipStreamCaptureStatusNone) return;
+    const c10::Stream now = c10::impl::VirtualGuardImpl(dev.type()).getStream(dev);
+    for (const Tensor *t : tensors) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        TORCH_CHECK(!node || !node->stream() || *node->stream() == now,
+                    "lookupffn_amd: this forward is captured, but a graph from before the capture still holds one of its leaves: drop that graph's results first");
+    }
+}
+
 // Queries or keys: four dimensions, a format, not empty.
 bool heads_tensor(PyObject *o, Tensor &t) {
     if (!plain(o)) return false;
@@ -224,6 +238,7 @@ PyObject *qk_norm_rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Py_RETURN_NONE;
     if (any_tangent({&in.q, &in.k, &in.q_weight, &in.k_weight, &in.table})) Py_RETURN_NONE;
     const bool grads = any_gradient({&in.q, &in.k, &in.q_weight, &in.k_weight});
+    if (grads) refuse_foreign_leaves({&in.q, &in.k, &in.q_weight, &in.k_weight}, dev);
     Tensor q_out, k_out;
     {
         const WithoutInterpreter unlocked;
@@ -369,6 +384,7 @@ PyObject *cross_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Py_RETURN_NONE;
     if (any_tangent({&in.q, &in.k, &in.v})) Py_RETURN_NONE;
     const bool grads = any_gradient({&in.q, &in.k, &in.v});
+    if (grads) refuse_foreign_leaves({&in.q, &in.k, &in.v}, dev);
     Tensor out;
     {
         const WithoutInterpreter unlocked;

@@ -283,7 +283,7 @@ int64_t plan(const lffn_qk_norm_rotary &c, Args &a, int lpr, int hc, bool backwa
         t.sb = s[0], t.st = s[1], t.sh = s[2];
         t.chunks = (t.heads + hc - 1) / hc;
         const int64_t groups = WG / lpr, want = (t.tokens * t.chunks + groups - 1) / groups;
-        if (!backward && total + want > INT32_MAX) return -1;
+        if (!backward && total + want > UINT32_MAX / WG) return -1;           // (threads of a launch)
         t.workgroups = int(backward && want > BWD_WORKGROUPS ? BWD_WORKGROUPS : want);
         total += t.workgroups;
     }

@@ -197,3 +197,15 @@ def test_module_surface():
     assert module.rotary.shape == (50, 16)
     with pytest.raises(ValueError):
         module(torch.zeros(1, 2, 96))
+
+
+def test_more_threads_than_a_launch_has():
+    """2^26 batches of one token: refused with the plan, before anything is launched."""
+    lib, n = _lib.load(), ctypes.c_int64(0)
+    a = _attention(B=1 << 26, q_len=1, heads=2)
+    assert lib.lffn_cross_attention_workspace_bytes(a, ctypes.byref(n)) == UNSUPPORTED
+    assert lib.lffn_cross_attention_fwd(a, P, None, None, 0, None) == UNSUPPORTED
+    assert lib.lffn_cross_attention_bwd_workspace_bytes(a, ctypes.byref(n)) == UNSUPPORTED
+    assert lib.lffn_cross_attention_bwd(a, P, P, P, P, P, P, P, 1 << 60, None) == UNSUPPORTED
+    a = _norm(B=1 << 28, q_len=8)
+    assert lib.lffn_qk_norm_rotary_fwd(a, P, P, None) == UNSUPPORTED
