@@ -30,7 +30,7 @@ struct FwdArgs {
     float c;                              // scale log2 e
 };
 
-// few_rows_kernel: rows at most.  us, few_rows_kernel and cross_attention_kernel: 16 x 512 keys x 12 heads x 64 half, 1 row 8.1, 13.5; 4 x 16384 x 8 x 128 bfloat16,
+// few_rows_kernel: rows at most.  us, few_rows_kernel and cross_attention_kernel: 16 x 512 keys x 12 heads x 64 half, 1 row 7.8, 13.5; 4 x 16384 x 8 x 128 bfloat16,
 // 1 row 59, 56, 2 rows 61, 60, 4 rows 69, 61; 64 x 512 x 16 x 64 bfloat16, 1 row 31, 36, 4 rows 49, 36; fp32 32 x 2048 x 16 x 64, 1 row 100, 123, 8 x 1024 x 8 x 128, 4 rows
 // 20, 40, 32 x 1024 x 12 x 64, 3 rows 53, 64.
 constexpr int few_rows(bool f32) { return f32 ? 4 : 2; }
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F:
 // asked for at a time, so that a short call waits for memory once and its code is short (a launch fetches it anew).  Every group of lanes has a softmax of
 // its own keys; groups and wavefronts are joined at the end.  Up to sixteen wavefronts a workgroup, so that 512 keys need no second kernel to join shares.
 template <typename R, typename F, int G, int RN>
-__global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * FEW_WAVES, RN == 1 ? 8 : 4) void few_rows_kernel(FwdArgs a) {
     constexpr int N = R::N, KEYS = 64 / G;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, group = lane / G, j = lane % G;
     const Unit unit = unit_of(blockIdx.x, a.units, a.tiles, a.split_by, a.heads);
@@ -212,18 +212,31 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(FwdArgs a) {
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.keys ? begin + a.split_steps : a.keys;      // (steps of one key)
     const int64_t first = begin + wave * (KEYS * FEW_TOGETHER) + group;
 
+    // Whether a step's keys take part is asked for a step ahead of them: a wavefront does not ask for keys of which none does, but for its first, which wait for
+    // nothing: 8 x 1 to 16384 of 16384 x 8 x 128 bfloat16 104 us, so 88.  (Keys and values a step ahead, too: 70 registers, so that a compute unit has one workgroup of 16 wavefronts for two, 256 x 512 x 16 x 64 half 94 us, so 107.)
     uint4 k[FEW_TOGETHER], v[FEW_TOGETHER];
-    bool live[FEW_TOGETHER];
+    bool live[FEW_TOGETHER], next[FEW_TOGETHER];
+    const int64_t apart = waves * (KEYS * FEW_TOGETHER);
+    auto look = [&](int64_t from, bool (&live)[FEW_TOGETHER]) {
+#pragma unroll
+        for (int u = 0; u < FEW_TOGETHER; ++u) {
+            const int64_t key = from + u * KEYS;
+            live[u] = key < end && (!mask || mask[key] != 0);
+        }
+    };
     auto fetch = [&](int64_t from) {
 #pragma unroll
         for (int u = 0; u < FEW_TOGETHER; ++u) {
             const int64_t key = from + u * KEYS, at = key < end ? key : end - 1;
-            live[u] = key < end && (!mask || mask[at] != 0);
             k[u] = *reinterpret_cast<const uint4 *>(kp + at * a.kt);
             v[u] = *reinterpret_cast<const uint4 *>(vp + at * a.vt);
         }
     };
-    if (begin < end) fetch(first);
+    if (begin < end) {
+        fetch(first);
+        look(first, live);
+        look(first + apart, next);
+    }
     float q[RN][N], acc[RN][N] = {}, most[RN], sum[RN] = {};
     const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh + column, a.qt, a.qh, a.group};
 #pragma unroll
@@ -234,7 +247,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(FwdArgs a) {
         for (int e = 0; e < N; ++e) q[r][e] = on ? q[r][e] * a.c : 0.f;
     }
 #pragma unroll 1
-    for (int64_t at = first; at - group < end;) {
+    for (int64_t at = first; at - group < end; at += apart) {
         float s[RN][FEW_TOGETHER];
 #pragma unroll
         for (int u = 0; u < FEW_TOGETHER; ++u) {
@@ -276,8 +289,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(FwdArgs a) {
                 for (int r = 0; r < RN; ++r) acc[r][e] = fmaf(w[r][u], value, acc[r][e]);
             }
         }
-        at += waves * (KEYS * FEW_TOGETHER);
-        if (at - group < end) fetch(at);
+        bool one = false;
+#pragma unroll
+        for (int u = 0; u < FEW_TOGETHER; ++u) live[u] = next[u], one |= next[u];
+        if (__any(one)) fetch(at + apart);
+        look(at + 2 * apart, next);
     }
 
     __shared__ float2 of_wave[FEW_WAVES][RN];            // largest score, sum of weights
@@ -303,19 +319,21 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(FwdArgs a) {
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < RN * (G * N / 4); i += blockDim.x) {
-        const int r = i / (G * N / 4), quad = i % (G * N / 4), col = quad * 4;
+    // The wavefronts' sums as one, a group of 16 lanes four columns, a lane a wavefront (a lane all of them: 16 x 512 x 12 x 64 half 8.2 us for 7.8, 77 keys 4.4 for 4.2)
+    for (int i = threadIdx.x / FEW_WAVES; i < RN * (G * N / 4); i += blockDim.x / FEW_WAVES) {
+        const int r = i / (G * N / 4), quad = i % (G * N / 4), col = quad * 4, n = threadIdx.x % FEW_WAVES;
         if (r >= a.rows || col >= a.columns) continue;
-        float all = -INFINITY, total = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int n = 0; n < waves; ++n) all = fmaxf(all, of_wave[n][r].x);
-        for (int n = 0; n < waves; ++n) {
-            const float2 m = of_wave[n][r];
-            const float4 x = sums[n][r][quad];
-            const float by = m.x == all ? 1.f : __builtin_amdgcn_exp2f(m.x - all);
-            total = fmaf(by, m.y, total);
-            o.x = fmaf(by, x.x, o.x), o.y = fmaf(by, x.y, o.y), o.z = fmaf(by, x.z, o.z), o.w = fmaf(by, x.w, o.w);
-        }
+        const float2 m = n < waves ? of_wave[n][r] : make_float2(-INFINITY, 0.f);
+        const float4 x = n < waves ? sums[n][r][quad] : make_float4(0.f, 0.f, 0.f, 0.f);
+        float all = m.x;
+        all = larger(all, lane_xor<1>(all));
+        all = larger(all, lane_xor<2>(all));
+        all = larger(all, lane_xor<4>(all));
+        all = larger(all, lane_xor<8>(all));
+        const float by = m.x == all ? 1.f : __builtin_amdgcn_exp2f(m.x - all), total = lane_group_sum<FEW_WAVES>(by * m.y);
+        const float4 o = make_float4(lane_group_sum<FEW_WAVES>(by * x.x), lane_group_sum<FEW_WAVES>(by * x.y), lane_group_sum<FEW_WAVES>(by * x.z),
+                                     lane_group_sum<FEW_WAVES>(by * x.w));
+        if (n != 0) continue;
         const float inverse = total == 0.f ? 0.f : 1.f / total, level = total == 0.f ? INFINITY : all + __builtin_amdgcn_logf(total);
         const int64_t at = int64_t(bh) * a.rows + r;
         if (a.splits > 1) {
