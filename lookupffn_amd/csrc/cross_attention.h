@@ -145,11 +145,24 @@ struct F32 {
     static __device__ __forceinline__ float rounded(float a) { return a; }
 };
 
+// What sums are multiplied with on their way out: a number, or, where sums are scaled to half's range, a number and a power of two that a float may not have.
+struct Factor {
+    float by;
+    int exponent;
+};
+__device__ __forceinline__ float times(float v, float by) { return v * by; }
+__device__ __forceinline__ float times(float v, const Factor &f) { return __builtin_amdgcn_ldexpf(v * f.by, f.exponent); }
+template <typename F>
+__device__ __forceinline__ auto factor(float by, int exponent) {
+    if constexpr (F::SCALED) return Factor{by, exponent};
+    else return __builtin_amdgcn_ldexpf(by, exponent);
+}
+
 // The columns 32 d + 8 g + 4 half .. + 3 of a lane's row (half = lane / 32) to memory, by d and g; `row` where the lane's row begins, all lanes together.  Of 16-bit
 // results the lanes of a row exchange four columns of two groups, so that each has eight that lie together and stores 16 bytes.
 // rest: where what the rounding takes goes, or null.
-template <typename F, int DB>
-__device__ __forceinline__ void store_row(const ca_f32x16_t (&o)[DB], float by, char *row, bool live, int columns, int half, char *rest = nullptr) {
+template <typename F, int DB, typename S>
+__device__ __forceinline__ void store_row(const ca_f32x16_t (&o)[DB], const S &by, char *row, bool live, int columns, int half, char *rest = nullptr) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
         if constexpr (F::BYTES == 4) {
@@ -157,14 +170,14 @@ __device__ __forceinline__ void store_row(const ca_f32x16_t (&o)[DB], float by, 
             for (int g = 0; g < 4; ++g) {
                 const int col = 32 * d + 8 * g + 4 * half;
                 if (live && col < columns)
-                    F::store4(row + col * F::BYTES, o[d][4 * g] * by, o[d][4 * g + 1] * by, o[d][4 * g + 2] * by, o[d][4 * g + 3] * by);
+                    F::store4(row + col * F::BYTES, times(o[d][4 * g], by), times(o[d][4 * g + 1], by), times(o[d][4 * g + 2], by), times(o[d][4 * g + 3], by));
             }
         } else {
 #pragma unroll
             for (int g = 0; g < 4; g += 2) {
                 float t[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = o[d][4 * g + e] * by;
+                for (int e = 0; e < 8; ++e) t[e] = times(o[d][4 * g + e], by);
                 auto put = [&](char *to) {
                     uint32_t w[4];
 #pragma unroll

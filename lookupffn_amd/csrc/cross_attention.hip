@@ -106,7 +106,8 @@ __global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F:
     KeyFeed<F, DP, KT> feed(lds, pieces, kp, vp, a.kt, a.vt);
     const typename T::Reader read(lds, lane);
     Op fq[CHUNKS];
-    float by_c = a.c, by_v = 1.f;         // what takes scores to powers of two, results to what they are
+    float by_c = a.c;                     // what takes scores to powers of two
+    int of_v = 0;                         // and values to what they are, as an exponent
     {
         const bool live = row < a.rows;
         const char *const p = rows.at(live ? row : 0);
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F:
             feed.scale_a = __builtin_amdgcn_ldexpf(1.f, ek);
             feed.scale_b = __builtin_amdgcn_ldexpf(1.f, ev);
             by_c = fmaxf(__builtin_amdgcn_ldexpf(a.c, -(eq + ek)), 0x1p-126f);       // (not zero, by which -infinity is no number: scores of nothing either way)
-            by_v = __builtin_amdgcn_ldexpf(1.f, -ev);
+            of_v = -ev;
         }
     }
     ca_f32x16_t o[DB] = {};
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F:
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
 
     sum = of_both_halves(sum, [](float x, float y) { return x + y; });
-    const float inverse = sum == 0.f ? 0.f : by_v / sum;     // a query without keys: zeros
+    const auto inverse = factor<F>(sum == 0.f ? 0.f : 1.f / sum, of_v);     // a query without keys: zeros
     const float level = sum == 0.f ? INFINITY : (most == -INFINITY ? 0.f : most) * by_c - F::LIFT + __builtin_amdgcn_logf(sum);
     const bool live = row < a.rows;
     const int64_t at = int64_t(bh) * a.rows + row;

@@ -210,7 +210,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
 
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
-    const float by = __builtin_amdgcn_ldexpf(a.scale, -(e2.ds + e2.k + fitted));
+    const auto by = factor<F>(a.scale, -(e2.ds + e2.k + fitted));
     if (a.splits > 1) store_row<F32, DB>(dq, by, reinterpret_cast<char *>(a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns), live, a.columns, half);
     else store_row<F, DB>(dq, by, a.gq + out_row, live, a.columns, half);
 }
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
 #pragma unroll
         for (int d = 0; d < DB; ++d) dk[d] = ca_f32x16_t{}, dv[d] = ca_f32x16_t{};
     }
-    const float by_k = __builtin_amdgcn_ldexpf(a.scale, -(e2.ds + e2.q + fitted_ds)), by_v = power((HALF ? -int(P_LIFT) : 0) - e2.g - fitted_p);
+    const auto by_k = factor<F>(a.scale, -(e2.ds + e2.q + fitted_ds)), by_v = factor<F>(1.f, (HALF ? -int(P_LIFT) : 0) - e2.g - fitted_p);
     if (a.splits > 1) {
         const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key) * a.columns;
         store_row<F32, DB>(dk, by_k, reinterpret_cast<char *>(a.part + of), in, a.columns, half);
@@ -678,7 +678,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
 #pragma unroll
         for (int d = 0; d < DB; ++d) sums[d] = ca_f32x16_t{};
     }
-    const float by = OF_V ? power((HALF ? -int(P_LIFT) : 0) - e2.g - fitted) : __builtin_amdgcn_ldexpf(a.scale, -(e2.ds + e2.q + fitted));
+    const auto by = OF_V ? factor<F>(1.f, (HALF ? -int(P_LIFT) : 0) - e2.g - fitted) : factor<F>(a.scale, -(e2.ds + e2.q + fitted));
     if (a.splits > 1) {
         const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key + (OF_V ? a.splits * all : 0)) * a.columns;
         store_row<F32, DB>(sums, by, reinterpret_cast<char *>(a.part + of), in, a.columns, half);

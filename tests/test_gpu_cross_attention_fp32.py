@@ -88,6 +88,8 @@ def test_numbers_of_many_sizes(B, Lq, Lk, H, Hk, D):
     _held(q * 1e-20, k * 1e20, v * 1e-25, g * 1e25)
     _held(q * 1e18, k * 1e-18, v * 1e18, g * 1e-12)
     _held(q * 1e-30, k * 1e-10, v, g)   # (scores of nothing)
+    _held(q, k, v * 1e-34, g)           # (results near the end of the range, whose scaling back is no fp32 number)
+    _held(q * 1e-16, k * 1e16, v * 1e-16, g * 1e-17)
     _held(q * powers(B, 1, H, 1, low=-20), k * powers(B, 1, Hk, 1, low=-20), v * powers(B, 1, Hk, 1, low=-20), g * powers(B, 1, H, 1, low=-20))
 
 
