@@ -110,3 +110,17 @@ def test_captured_and_replayed(dtype):
 @pytest.mark.parametrize("Lq,Lk,D", [(37, 45, 40), (128, 31, 64), (5, 2100, 64)])
 def test_nothing_is_written_beside_the_results(Lq, Lk, D, dtype):
     attention.test_nothing_is_written_beside_the_results(Lq, Lk, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("mask", [None, "holes"])
+def test_shared_out_with_a_tile_for_every_compute_unit(mask, dtype):
+    """Rows that fill the chip once and many keys, which are shared out over three workgroups each: against the same queries a few at a time, whose results are
+    off by no more than the bounds against 64 bits."""
+    B, L, keys, H, D = 4, 1000, 2900, 8, 64
+    q, k, v = (_randn(B, n, H, D, dtype=dtype, seed=s) for s, n in enumerate((L, keys, keys)))
+    mask = _mask(mask, B, keys)
+    out = cross_attention(q, k, v, mask)
+    some = torch.arange(0, L, 97, device=DEV)
+    want, _, (bound,) = _reference(q[:, some], k, v, mask, D ** -0.5)
+    _close(out[:, some], want, bound)
