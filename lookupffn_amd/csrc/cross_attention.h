@@ -299,16 +299,31 @@ struct F32Two {
     static __device__ __forceinline__ float rounded(float a) { return a; }
 };
 
-// log2 of a row's length, 16 lanes a row, 8 columns a lane; -infinity where there is nothing but zeros, or no length.  (By way of the largest number's
+// Largest over an aligned group of lanes, as lane_group_sum; from groups to the wavefront.
+template <int LANES>
+__device__ __forceinline__ float lane_group_max(float v) {
+    if constexpr (LANES > 1) v = fmaxf(v, lane_xor<1>(v));
+    if constexpr (LANES > 2) v = fmaxf(v, lane_xor<2>(v));
+    if constexpr (LANES > 4) v = fmaxf(v, lane_xor<4>(v));
+    if constexpr (LANES > 8) v = fmaxf(v, lane_xor<8>(v));
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float over_groups_max(float v) {
+    if constexpr (LANES <= 4) v = fmaxf(v, lane_xor<4>(v));
+    if constexpr (LANES <= 8) v = fmaxf(v, lane_xor<8>(v));
+    v = fmaxf(v, lane_xor<16>(v));
+    return fmaxf(v, lane_xor<32>(v));
+}
+
+// log2 of a row's length, LANES lanes a row, 8 columns a lane; -infinity where there is nothing but zeros, or no length.  (By way of the largest number's
 // power of two: squares would leave fp32's range.)
+template <int LANES>
 __device__ __forceinline__ float row_level(const float (&v)[8]) {
     float most = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
-    most = fmaxf(most, lane_xor<1>(most));
-    most = fmaxf(most, lane_xor<2>(most));
-    most = fmaxf(most, lane_xor<4>(most));
-    most = fmaxf(most, lane_xor<8>(most));
+    most = lane_group_max<LANES>(most);
     const int e = int(__float_as_uint(most) >> 23) - 127;
     float squares = 0.f;
 #pragma unroll
@@ -316,10 +331,11 @@ __device__ __forceinline__ float row_level(const float (&v)[8]) {
         const float x = __builtin_amdgcn_ldexpf(v[i], -e);
         squares = fmaf(x, x, squares);
     }
-    squares = lane_group_sum<16>(squares);
+    squares = lane_group_sum<LANES>(squares);
     return most > 0.f && is_finite(squares) ? (float)e + 0.5f * __builtin_amdgcn_logf(squares) : -INFINITY;
 }
-constexpr int LEVEL_ROWS = 128;           // rows of a workgroup that looks for the longest: 8 to a group of 16 lanes, asked for together
+constexpr int LEVEL_ROWS = 128;           // rows of a workgroup that looks for the longest: those of a group of lanes are asked for together
+constexpr int level_lanes(int columns) { return columns <= 32 ? 4 : columns <= 64 ? 8 : 16; }
 
 // Largest of the `tiles` levels of a batch and key head (every lane's); -infinity of none.
 __device__ __forceinline__ float longest(const float *levels, int64_t bh, int tiles) {

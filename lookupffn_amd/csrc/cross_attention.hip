@@ -45,25 +45,27 @@ __device__ __forceinline__ void store_result(const FwdArgs &a, int64_t at, const
     if (a.rest) F::store4(a.rest + at, v.x - F::rounded(v.x), v.y - F::rounded(v.y), v.z - F::rounded(v.z), v.w - F::rounded(v.w));
 }
 
+template <int LANES>
 __device__ __forceinline__ float level_of(const F32::Raw &r, bool on) {
     float v[8];
     F32::unpack(on ? r : F32::zero(), v);
-    return row_level(v);
+    return row_level<LANES>(v);
 }
 
 // log2 of the longest of 128 keys that take part, and of their values.  Bound by memory: both once.
+template <int LANES>
 __global__ __launch_bounds__(WG) void levels_kernel(FwdArgs a) {
-    constexpr int EACH = LEVEL_ROWS / (WG / 16);
+    constexpr int APART = WG / LANES, EACH = LEVEL_ROWS / APART;
     __shared__ float red[2][WAVES];
-    const int lane = threadIdx.x & 15, col = lane * 8 < a.columns ? lane * 8 : 0;
+    const int lane = threadIdx.x % LANES, col = lane * 8 < a.columns ? lane * 8 : 0;
     const bool on = lane * 8 < a.columns;
     const int bh = a.level_by.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * a.level_tiles;
     F32::Raw k[EACH], v[EACH];
     bool live[EACH];
-    const int64_t first = int64_t(tile) * LEVEL_ROWS + threadIdx.x / 16;
+    const int64_t first = int64_t(tile) * LEVEL_ROWS + threadIdx.x / LANES;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        const int64_t key = first + i * (WG / 16), at = key < a.keys ? key : a.keys - 1;
+        const int64_t key = first + i * APART, at = key < a.keys ? key : a.keys - 1;
         live[i] = !a.mask || a.mask[b * a.mask_stride + at] != 0;
         k[i] = F32::load(a.k + b * a.kb + kh * a.kh + at * a.kt + col * 4);
         v[i] = F32::load(a.v + b * a.vb + kh * a.vh + at * a.vt + col * 4);
@@ -71,13 +73,12 @@ __global__ __launch_bounds__(WG) void levels_kernel(FwdArgs a) {
     float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        const float lk = level_of(k[i], on), lv = level_of(v[i], on);
+        const float lk = level_of<LANES>(k[i], on), lv = level_of<LANES>(v[i], on);
         if (live[i]) most[0] = fmaxf(most[0], lk), most[1] = fmaxf(most[1], lv);
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-        most[n] = fmaxf(most[n], lane_xor<16>(most[n]));
-        most[n] = fmaxf(most[n], lane_xor<32>(most[n]));
+        most[n] = over_groups_max<LANES>(most[n]);
         if ((threadIdx.x & 63) == 0) red[n][threadIdx.x >> 6] = most[n];
     }
     __syncthreads();
@@ -599,7 +600,11 @@ extern "C" int lffn_cross_attention_fwd(const lffn_cross_attention *c, void *out
         return c->format == LFFN_ROWS_BF16 ? launch_few<BF16, BF16Row>(a, lanes, s) : launch_few<F16, F16Row>(a, lanes, s);
     }
     if (a.level_tiles) {
-        levels_kernel<<<dim3((unsigned)(batch_heads * a.level_tiles)), dim3(WG), 0, s>>>(a);
+        const dim3 grid((unsigned)(batch_heads * a.level_tiles)), block(WG);
+        const int lanes = level_lanes(a.columns);
+        if (lanes == 4) levels_kernel<4><<<grid, block, 0, s>>>(a);
+        else if (lanes == 8) levels_kernel<8><<<grid, block, 0, s>>>(a);
+        else levels_kernel<16><<<grid, block, 0, s>>>(a);
         return launch<F32Two>(a, s);
     }
     if (c->format == LFFN_ROWS_F32) return launch<F32>(a, s);

@@ -41,13 +41,13 @@ struct BwdArgs {
     float c, scale;
 };
 
-// delta of every row; half precision: the longest rows of g and v as well; fp32 numbers in two terms: of q and k, too.  16 lanes a row, 8 columns a lane, 8 rows to a group of
-// lanes, asked for together.  Bound by memory: out, its rest and g (and v, q, k) once.  (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16
+// delta of every row; half precision: the longest rows of g and v as well; fp32 numbers in two terms: of q and k, too.  A lane has 8 columns, the rows of a group of lanes are
+// asked for together.  Bound by memory: out, its rest and g (and v, q, k) once.  (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16
 // 65 us, so 13.)
-template <typename F, bool LEVELS>
+template <typename F, int LANES, bool LEVELS>
 __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
-    constexpr int EACH = LEVEL_ROWS / (WG / 16);
-    const int lane = threadIdx.x & 15, tiles = a.g_tiles + a.v_tiles;
+    constexpr int APART = WG / LANES, EACH = LEVEL_ROWS / APART;
+    const int lane = threadIdx.x % LANES, tiles = a.g_tiles + a.v_tiles;
     const bool on = lane * 8 < a.columns;
     const int col = on ? lane * 8 : 0;
     const int bh = a.level_tiles.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * tiles;
@@ -55,16 +55,16 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
     auto look = [&](int n, const typename F::Raw &r, bool live) {
         float v[8];
         F::unpack(on ? r : F::zero(), v);
-        const float l = row_level(v);
+        const float l = row_level<LANES>(v);
         if (live) most[n] = fmaxf(most[n], l);
     };
     if (tile < a.g_tiles) {
         typename F::Raw o[EACH], g[EACH], rest[F::BYTES == 2 ? EACH : 1], q[F::SCALED ? EACH : 1];
-        const int first = tile * LEVEL_ROWS + threadIdx.x / 16;
+        const int first = tile * LEVEL_ROWS + threadIdx.x / LANES;
         const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int row = min(first + i * (WG / 16), a.rows - 1);
+            const int row = min(first + i * APART, a.rows - 1);
             const int64_t at = (heads_row(b, kh, row, a.q_len, a.key_heads, a.group) * a.columns + col) * F::BYTES;
             o[i] = F::load(a.out + at);
             g[i] = F::load(a.g + at);
@@ -84,8 +84,8 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
-            dot = lane_group_sum<16>(on ? dot : 0.f);
-            const int row = first + i * (WG / 16);
+            dot = lane_group_sum<LANES>(on ? dot : 0.f);
+            const int row = first + i * APART;
             if (lane == 0 && row < a.rows) a.delta[int64_t(bh) * a.rows + row] = dot;
             if (LEVELS) look(0, g[i], true);            // (a row once more changes nothing)
             if constexpr (F::SCALED) look(1, q[i], true);
@@ -93,10 +93,10 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
     } else if (LEVELS) {
         typename F::Raw v[EACH], k[F::SCALED ? EACH : 1];
         bool live[EACH];
-        const int64_t first = int64_t(tile - a.g_tiles) * LEVEL_ROWS + threadIdx.x / 16;
+        const int64_t first = int64_t(tile - a.g_tiles) * LEVEL_ROWS + threadIdx.x / LANES;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int64_t key = first + i * (WG / 16), at = key < a.keys ? key : a.keys - 1;
+            const int64_t key = first + i * APART, at = key < a.keys ? key : a.keys - 1;
             live[i] = !a.mask || a.mask[b * a.mask_stride + at] != 0;
             v[i] = F::load(a.v + b * a.vb + kh * a.vh + at * a.vt + col * F::BYTES);
             if constexpr (F::SCALED) k[i] = F::load(a.k + b * a.kb + kh * a.kh + at * a.kt + col * F::BYTES);
@@ -111,8 +111,7 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
         __shared__ float red[2][WAVES];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            most[n] = fmaxf(most[n], lane_xor<16>(most[n]));
-            most[n] = fmaxf(most[n], lane_xor<32>(most[n]));
+            most[n] = over_groups_max<LANES>(most[n]);
             if ((threadIdx.x & 63) == 0) red[n][threadIdx.x >> 6] = most[n];
         }
         __syncthreads();
@@ -823,7 +822,7 @@ template <typename F, int DP, int KT>
 int launch(const Plan &p, hipStream_t stream) {
     constexpr bool LEVELS = F::LIFT != 0.f;
     const int64_t tiles = int64_t(p.q.batch_heads) * (p.q.g_tiles + p.q.v_tiles);
-    if (tiles > 0) delta_kernel<F, LEVELS><<<dim3((unsigned)tiles), dim3(WG), 0, stream>>>(p.q);
+    if (tiles > 0) delta_kernel<F, level_lanes(DP), LEVELS><<<dim3((unsigned)tiles), dim3(WG), 0, stream>>>(p.q);
     auto add_queries = [&](const BwdArgs &q) {
         if (q.splits > 1)
             add_splits<F>({{q.part, nullptr}, {q.gq, nullptr}, int64_t(q.batch_heads) * q.rows, q.q_len, q.heads, q.group, q.rows, q.splits, q.columns}, 1, stream);
