@@ -445,7 +445,8 @@ __attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(co
 namespace {
 
 constexpr int64_t COMPUTE_UNITS = 256;    // a tile each and more: the keys are not shared out,
-constexpr int64_t WANTED = 512;           // workgroups, where there are keys enough to share out
+constexpr int64_t WANTED = 512;           // workgroups at most, where there are keys enough to share out (two a compute unit: up to a tile's shares more, 3 x 500 rows x 1500
+                                          // keys x 10 x 128 bfloat16 32 us, so 43)
 // but where a compute unit has little more than one tile (it has room for two or three) and the keys are so many that the join is little beside them.  us, whole and in
 // shares, rows x keys x heads x columns: half 4000 x 4000 x 8 x 64 75, 64; x 6000 109, 79; x 12 heads 84, 78; x 15 heads 93, 108; 2 x 2000 x 2000 x 8 x 64 41, 43, x 3000
 // 57, 50; 4000 x 4000 x 8 x 32 63, 45; bfloat16 4000 x 8000 x 8 x 128 195, 163; fp32 4000 x 4000 x 8 x 64 144, 128, x 128 241, 251.
@@ -483,9 +484,9 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     a.steps = (c.k_len + kt - 1) / kt;
     a.c = c.scale * LOG2E;
     const int64_t tiles = c.B * c.key_heads * a.row_tiles;
-    int64_t splits = tiles > 0 && tiles < COMPUTE_UNITS ? (WANTED + tiles - 1) / tiles : 1;
+    int64_t splits = tiles > 0 && tiles < COMPUTE_UNITS ? WANTED / tiles : 1;
     if (splits > a.steps / LEAST_STEPS) splits = a.steps / LEAST_STEPS;
-    if (tiles >= COMPUTE_UNITS && tiles < MOST_TILES && c.k_len >= MANY_KEYS && (c.format != LFFN_ROWS_F32 || c.columns <= 64)) splits = (MANY_WANTED + tiles - 1) / tiles;
+    if (tiles >= COMPUTE_UNITS && tiles < MOST_TILES && c.k_len >= MANY_KEYS && (c.format != LFFN_ROWS_F32 || c.columns <= 64)) splits = MANY_WANTED / tiles;
     if (a.rows <= few_rows(c.format == LFFN_ROWS_F32)) {
         const int64_t at_once = 64 / lanes_of_a_key(c) * FEW_TOGETHER, rounds = (c.k_len + at_once - 1) / at_once;
         a.few_waves = int(rounds < 1 ? 1 : rounds < FEW_WAVES ? rounds : FEW_WAVES);
