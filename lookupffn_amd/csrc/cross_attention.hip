@@ -452,6 +452,11 @@ constexpr int64_t WANTED = 512;           // workgroups at most, where there are
 // 57, 50; 4000 x 4000 x 8 x 32 63, 45; bfloat16 4000 x 8000 x 8 x 128 195, 163; fp32 4000 x 4000 x 8 x 64 144, 128, x 128 241, 251.
 constexpr int64_t MANY_KEYS = 2816;
 constexpr int64_t MOST_TILES = 400, MANY_WANTED = 768;
+// Where one wavefront of a tile's four has rows more tiles stand beside each other: 20 x 24 x 6571 x 12 x 16 half 70, 44; 32 x 8 x 2000 x 12 x 64 bfloat16 56, 45; 16 x 20 x
+// 3000 x 8 x 128 half 49, 51; 4 x 16 x 8000 x 8 x 64 bfloat16 (16 shares, 32) 19, 23; 24 x 4 x 2877 x 12 x 64 half 49 with two shares, with three, more than stand beside each
+// other, 62.
+constexpr int64_t ONE_WAVE_KEYS = 1536, ONE_WAVE_LEAST = 192, ONE_WAVE_MOST = 512;
+constexpr int64_t one_wave_wanted(int64_t columns) { return columns <= 32 ? 1024 : 768; }
 constexpr int64_t LEAST_STEPS = 2;        // of a workgroup
 
 // fp32: from where two terms of half precision are faster, with the look at keys and values that they take.  us, three terms and two, batch x rows x keys x heads x
@@ -487,6 +492,7 @@ int64_t plan(const lffn_cross_attention &c, FwdArgs &a) {
     int64_t splits = tiles > 0 && tiles < COMPUTE_UNITS ? WANTED / tiles : 1;
     if (splits > a.steps / LEAST_STEPS) splits = a.steps / LEAST_STEPS;
     if (tiles >= COMPUTE_UNITS && tiles < MOST_TILES && c.k_len >= MANY_KEYS && (c.format != LFFN_ROWS_F32 || c.columns <= 64)) splits = MANY_WANTED / tiles;
+    if (a.rows <= ROWS && c.columns <= 64 && tiles >= ONE_WAVE_LEAST && tiles < ONE_WAVE_MOST && c.k_len >= ONE_WAVE_KEYS) splits = one_wave_wanted(c.columns) / tiles;
     if (a.rows <= few_rows(c.format == LFFN_ROWS_F32)) {
         const int64_t at_once = 64 / lanes_of_a_key(c) * FEW_TOGETHER, rounds = (c.k_len + at_once - 1) / at_once;
         a.few_waves = int(rounds < 1 ? 1 : rounds < FEW_WAVES ? rounds : FEW_WAVES);

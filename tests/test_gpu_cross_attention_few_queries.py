@@ -114,13 +114,13 @@ def test_nothing_is_written_beside_the_results(Lq, Lk, D, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("mask", [None, "holes"])
-def test_shared_out_with_a_tile_for_every_compute_unit(mask, dtype):
-    """Rows that fill the chip once and many keys, which are shared out over three workgroups each: against the same queries a few at a time, whose results are
+@pytest.mark.parametrize("B,L,keys,H,D", [(4, 1000, 2900, 8, 64), (24, 20, 1600, 8, 32), (25, 32, 1537, 8, 64)])
+def test_shared_out_with_a_tile_for_every_compute_unit(B, L, keys, H, D, mask, dtype):
+    """Rows that fill the chip once and many keys, which are shared out over two to five workgroups each: against the same queries a few at a time, whose results are
     off by no more than the bounds against 64 bits."""
-    B, L, keys, H, D = 4, 1000, 2900, 8, 64
     q, k, v = (_randn(B, n, H, D, dtype=dtype, seed=s) for s, n in enumerate((L, keys, keys)))
     mask = _mask(mask, B, keys)
     out = cross_attention(q, k, v, mask)
-    some = torch.arange(0, L, 97, device=DEV)
+    some = torch.arange(0, L, 97 if L > 100 else 1, device=DEV)
     want, _, (bound,) = _reference(q[:, some], k, v, mask, D ** -0.5)
     _close(out[:, some], want, bound)
