@@ -11,7 +11,7 @@
 // to half's range, those that stand each row by its own.  A number that passes is held to 2^-22 of itself, or to 2^-36 of the longest row of its head where that
 // is more, any other to 2^-22.  Elsewhere a float is three bfloat16 terms of 8 bits each, which together are it (the exponent range is the same, so nothing has to be
 // scaled), and of the nine products six are formed, those of at least 2^-16: what is left out is below 2^-22 of the product.  (Two terms for three, 16 x 512 x 512
-// x 12 x 64: forward 77 us to 54 and 12 for the look, queries' gradients 111 to 78, keys' 159 to 113.)
+// x 12 x 64: forward 77 us to 54 and 10 for the look, queries' gradients 111 to 78, keys' 159 to 113.)
 #pragma once
 
 #include "rows16.h"
