@@ -529,7 +529,7 @@ int launch_few(const FwdArgs &a, hipStream_t stream) {
     const dim3 grid((unsigned)a.units), block(64 * a.few_waves);
     if (a.rows == 1) few_rows_kernel<R, F, G, 1><<<grid, block, 0, stream>>>(a);
     else if (a.rows == 2) few_rows_kernel<R, F, G, 2><<<grid, block, 0, stream>>>(a);
-    else few_rows_kernel<R, F, G, 4><<<grid, block, 0, stream>>>(a);
+    else if constexpr (few_rows(F::BYTES == 4) > 2) few_rows_kernel<R, F, G, 4><<<grid, block, 0, stream>>>(a);
     if (a.splits > 1) join<F>(a, stream);
     return lffn_launch_status();
 }

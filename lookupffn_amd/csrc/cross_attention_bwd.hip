@@ -86,7 +86,7 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
             for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
             dot = lane_group_sum<LANES>(on ? dot : 0.f);
             const int row = first + i * APART;
-            if (lane == 0 && row < a.rows) a.delta[int64_t(bh) * a.rows + row] = dot;
+            if (lane == 0 && row < a.rows) a.delta[int64_t(bh) * a.rows + row] = a.keys == 1 ? 0.f : dot;         // (of_products)
             if (LEVELS) look(0, g[i], true);            // (a row once more changes nothing)
             if constexpr (F::SCALED) look(1, q[i], true);
         }
@@ -142,6 +142,8 @@ __device__ __forceinline__ Exponents exponents(const BwdArgs &a, int64_t bh) {
     return e;
 }
 __device__ __forceinline__ float power(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
+// What g . v is multiplied with.  A single key has all the weight, and ds is nothing; g . v and delta, summed in different orders, would leave their roundings.
+__device__ __forceinline__ float of_products(const BwdArgs &a, int e) { return a.keys == 1 ? 0.f : power(e); }
 
 template <typename F, int DP, int KT>
 __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1 || DP <= 64 ? 2 : 1) void query_gradient_kernel(BwdArgs a) {
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     Op fq[CHUNKS], fg[CHUNKS];
     const int eq = own_rows<F>(Rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group}.at(live ? row : 0), live, half, pieces, fq);
     const int eg = own_rows<F>(a.g + out_row, live, half, pieces, fg);
-    const float f = power(e2.ds - eg - e2.v), by_c = __builtin_amdgcn_ldexpf(a.c, -(eq + e2.k));
+    const float f = of_products(a, e2.ds - eg - e2.v), by_c = __builtin_amdgcn_ldexpf(a.c, -(eq + e2.k));
     const float level = live ? a.lse[int64_t(bh) * a.rows + row] : INFINITY;
     const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], e2.ds) : 0.f;
     ca_f32x16_t dq[DB] = {};
@@ -281,7 +283,7 @@ __global__ __launch_bounds__(WG, 2) void gradients_kernel(BwdArgs a) {
     constexpr bool HALF = F::LIFT != 0.f;
     const Exponents e2 = exponents<F>(a, bh);
     const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
-    const float f = power(of_delta);
+    const float f = of_products(a, of_delta);
     const float level = live ? a.lse[int64_t(bh) * a.rows + row] - (HALF ? P_LIFT : 0.f) : INFINITY;
     const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], of_delta) : 0.f;
     KeyFeed<F, DP, KT> feed(lds + PASSING, pieces, kp, vp, a.kt, a.vt);
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
     Op fk[CHUNKS], fv[CHUNKS];
     const int ek = own_rows<F>(a.k + b * a.kb + kh * a.kh + at_key * a.kt, true, half, pieces, fk);
     const int ev = own_rows<F>(a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, fv);
-    const float f = power(of_delta - e2.g - ev), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + ek));
+    const float f = of_products(a, of_delta - e2.g - ev), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + ek));
 
     // Rows beyond the last are the last once more: their levels are infinite and so their weights zero.  A step's addresses go by its first token; where
     // the heads that share a key divide KT they are the same for every step.
@@ -538,7 +540,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
     const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
     Op own[CHUNKS];                       // the weights' wavefront: keys; the other: values
     const int of_own = own_rows<F>(OF_V ? a.k + b * a.kb + kh * a.kh + at_key * a.kt : a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, own);
-    const float f = power(of_delta - e2.g - of_own), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + of_own));
+    const float f = of_products(a, of_delta - e2.g - of_own), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + of_own));
 
     const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
     const int64_t g_token = int64_t(a.key_heads) * a.group.by * a.columns * F::BYTES;

@@ -124,3 +124,16 @@ def test_shared_out_with_a_tile_for_every_compute_unit(B, L, keys, H, D, mask, d
     some = torch.arange(0, L, 97 if L > 100 else 1, device=DEV)
     want, _, (bound,) = _reference(q[:, some], k, v, mask, D ** -0.5)
     _close(out[:, some], want, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("L,D", [(1, 64), (5, 16), (70, 64), (200, 64), (150, 128)])
+def test_a_single_key(L, D, dtype):
+    """It has all the weight: its values are the result, and the gradients of queries and keys are zeros, not what two sums of the same terms differ by."""
+    q, k, v, g = (_randn(3, n, 4, D, dtype=dtype, seed=s) for s, n in enumerate((L, 1, 1, L)))
+    for mask in (None, torch.tensor([[True], [False], [True]], device=DEV)):
+        out, (gq, gk, gv) = _run(q, k, v, mask, None, g)
+        want, gradients, bounds = _reference(q, k, v, mask, D ** -0.5, g)
+        _close(out, want, bounds[0])
+        _close(gv, gradients[2], bounds[3])
+        assert not gq.any() and not gk.any()
