@@ -7,7 +7,7 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 from torch.compiler import is_compiling
 
@@ -35,6 +35,15 @@ def _host():
         return False
     host = _lib.loaded_host
     return _lib.host() if host is None else host
+
+
+def _recorded(*tensors):
+    """Whether a call is the autograd function's: a gradient is recorded, or an input has a tangent of forward mode, which the function refuses and the operator
+    behind it would drop."""
+    tensors = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return not is_compiling() and forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def rotary_table(positions, columns, base=10000.0, device=None):
@@ -122,7 +131,7 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, *, table=None, q_pos
         q_positions, k_positions = q_positions.long(), k_positions.long()
     args = (q, k, q_weight, k_weight, table, q_positions, k_positions, float(eps),
             bool(interleaved))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    if _recorded(*args[:4]):
         return QkNormRotary.apply(*args)
     out = ops.qk_norm_rotary(*args)
     return out[0], (out[1] if k is not None else None)
@@ -179,6 +188,6 @@ def cross_attention(q, k, v, key_mask=None, *, scale=None):
                  f"key_mask: {tuple(k.shape[:2])} bool, got {tuple(key_mask.shape)} {key_mask.dtype}")
     scale = columns ** -0.5 if scale is None else float(scale)
     _require(0 < scale < math.inf, f"scale: {scale}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _recorded(q, k, v):
         return CrossAttentionFunction.apply(q, k, v, key_mask, scale)
     return ops.cross_attention(q, k, v, key_mask, scale, False)[0]
