@@ -203,6 +203,14 @@ class CrossAttention(nn.Module):
         columns = getattr(config, "rotary_columns", 0)
         self.register_buffer("rotary", rotary_table(config.max_position_embeddings, columns) if columns else None, persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        # the rotation goes where the module goes, in float32: 16 bits would turn far positions by other angles
+        table = self.rotary
+        super()._apply(fn, recurse)
+        if table is not None and self.rotary.dtype != table.dtype:
+            self.rotary = table.to(self.rotary.device)
+        return self
+
     def _heads(self, x, heads):
         return x.view(*x.shape[:-1], heads, self.attention_head_size)
 
