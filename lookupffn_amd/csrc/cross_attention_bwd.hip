@@ -32,6 +32,7 @@ struct BwdArgs {
     char *gq, *gk, *gv;
     float *delta;                         // [B, key heads, rows]
     float *g_levels, *q_levels, *v_levels, *k_levels;                // log2 of the longest rows, [B, key heads, g_tiles or v_tiles]
+    int32_t *single;                      // [B], with a mask: whether one key alone takes part
     float *part;                          // [splits, B, key heads, rows or keys, columns] (keys: of k, then of v)
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, mask_stride;         // strides in bytes
     int64_t keys, steps, split_steps, q_len;
@@ -40,6 +41,26 @@ struct BwdArgs {
     int batch_heads, key_heads, rows, tiles, splits, columns, g_tiles, v_tiles;
     float c, scale;
 };
+
+// How many keys of a sequence take part, as far as two: a workgroup looks at 4096 flags at a time and seldom at more.
+__device__ __forceinline__ void look_for_a_single_key(const BwdArgs &a, int b) {
+    constexpr int EACH = 16;
+    const uint8_t *const mask = a.mask + b * a.mask_stride;
+    int found = 0;
+    for (int64_t first = threadIdx.x; first - threadIdx.x < a.keys && found < 2; first += EACH * WG) {
+        uint8_t flag[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) flag[i] = mask[first + i * WG < a.keys ? first + i * WG : a.keys - 1];
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) mine += first + i * WG < a.keys && flag[i] != 0;
+        found += __syncthreads_count(mine > 0);
+        found += __syncthreads_or(mine > 1);
+    }
+    if (threadIdx.x == 0) a.single[b] = found == 1;
+}
+// A key that takes part alone has all the weight, and ds is nothing; g . v and delta, summed in different orders, would leave their roundings.  So both are held to zero.
+__device__ __forceinline__ bool single_key(const BwdArgs &a, int b) { return a.mask ? a.single[b] != 0 : a.keys == 1; }
 
 // delta of every row; half precision: the longest rows of g and v as well; fp32 numbers in two terms: of q and k, too.  A lane has 8 columns, the rows of a group of lanes are
 // asked for together.  Bound by memory: out, its rest and g (and v, q, k) once.  (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16
@@ -50,6 +71,7 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
     const int lane = threadIdx.x % LANES, tiles = a.g_tiles + a.v_tiles;
     const bool on = lane * 8 < a.columns;
     const int col = on ? lane * 8 : 0;
+    if (blockIdx.x >= (uint32_t)a.batch_heads * tiles) return look_for_a_single_key(a, blockIdx.x - (uint32_t)a.batch_heads * tiles);
     const int bh = a.level_tiles.quotient(blockIdx.x), b = a.heads.quotient(bh), kh = bh - b * a.key_heads, tile = blockIdx.x - bh * tiles;
     float most[2] = {-INFINITY, -INFINITY};             // of g and q, or v and k
     auto look = [&](int n, const typename F::Raw &r, bool live) {
@@ -86,7 +108,7 @@ __global__ __launch_bounds__(WG) void delta_kernel(BwdArgs a) {
             for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
             dot = lane_group_sum<LANES>(on ? dot : 0.f);
             const int row = first + i * APART;
-            if (lane == 0 && row < a.rows) a.delta[int64_t(bh) * a.rows + row] = a.keys == 1 ? 0.f : dot;         // (of_products)
+            if (lane == 0 && row < a.rows) a.delta[int64_t(bh) * a.rows + row] = dot;
             if (LEVELS) look(0, g[i], true);            // (a row once more changes nothing)
             if constexpr (F::SCALED) look(1, q[i], true);
         }
@@ -142,8 +164,6 @@ __device__ __forceinline__ Exponents exponents(const BwdArgs &a, int64_t bh) {
     return e;
 }
 __device__ __forceinline__ float power(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
-// What g . v is multiplied with.  A single key has all the weight, and ds is nothing; g . v and delta, summed in different orders, would leave their roundings.
-__device__ __forceinline__ float of_products(const BwdArgs &a, int e) { return a.keys == 1 ? 0.f : power(e); }
 
 template <typename F, int DP, int KT>
 __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1 || DP <= 64 ? 2 : 1) void query_gradient_kernel(BwdArgs a) {
@@ -169,9 +189,10 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     Op fq[CHUNKS], fg[CHUNKS];
     const int eq = own_rows<F>(Rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group}.at(live ? row : 0), live, half, pieces, fq);
     const int eg = own_rows<F>(a.g + out_row, live, half, pieces, fg);
-    const float f = of_products(a, e2.ds - eg - e2.v), by_c = __builtin_amdgcn_ldexpf(a.c, -(eq + e2.k));
+    const bool single = single_key(a, b);
+    const float f = single ? 0.f : power(e2.ds - eg - e2.v), by_c = __builtin_amdgcn_ldexpf(a.c, -(eq + e2.k));
     const float level = live ? a.lse[int64_t(bh) * a.rows + row] : INFINITY;
-    const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], e2.ds) : 0.f;
+    const float delta = live && !single ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], e2.ds) : 0.f;
     ca_f32x16_t dq[DB] = {};
     int fitted = F::SCALED ? FIT_FIRST : 0;
 
@@ -283,9 +304,10 @@ __global__ __launch_bounds__(WG, 2) void gradients_kernel(BwdArgs a) {
     constexpr bool HALF = F::LIFT != 0.f;
     const Exponents e2 = exponents<F>(a, bh);
     const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
-    const float f = of_products(a, of_delta);
+    const bool single = single_key(a, b);
+    const float f = single ? 0.f : power(of_delta);
     const float level = live ? a.lse[int64_t(bh) * a.rows + row] - (HALF ? P_LIFT : 0.f) : INFINITY;
-    const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], of_delta) : 0.f;
+    const float delta = live && !single ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], of_delta) : 0.f;
     KeyFeed<F, DP, KT> feed(lds + PASSING, pieces, kp, vp, a.kt, a.vt);
     const typename T::Reader read(lds + PASSING, lane);
     const typename Own::Reader read_own(lds, lane);
@@ -389,7 +411,8 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
     Op fk[CHUNKS], fv[CHUNKS];
     const int ek = own_rows<F>(a.k + b * a.kb + kh * a.kh + at_key * a.kt, true, half, pieces, fk);
     const int ev = own_rows<F>(a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, fv);
-    const float f = of_products(a, of_delta - e2.g - ev), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + ek));
+    const bool single = single_key(a, b);
+    const float f = single ? 0.f : power(of_delta - e2.g - ev), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + ek));
 
     // Rows beyond the last are the last once more: their levels are infinite and so their weights zero.  A step's addresses go by its first token; where
     // the heads that share a key divide KT they are the same for every step.
@@ -421,7 +444,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
         if (tid < KT) {
             const bool on = int(step) * KT + tid < a.rows;
             levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
-            levels[buf * 2 * KT + KT + tid] = on ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
+            levels[buf * 2 * KT + KT + tid] = on && !single ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
         }
         feed.end(buf);
     };
@@ -540,7 +563,8 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
     const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
     Op own[CHUNKS];                       // the weights' wavefront: keys; the other: values
     const int of_own = own_rows<F>(OF_V ? a.k + b * a.kb + kh * a.kh + at_key * a.kt : a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, own);
-    const float f = of_products(a, of_delta - e2.g - of_own), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + of_own));
+    const bool single = single_key(a, b);
+    const float f = single ? 0.f : power(of_delta - e2.g - of_own), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + of_own));
 
     const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
     const int64_t g_token = int64_t(a.key_heads) * a.group.by * a.columns * F::BYTES;
@@ -580,7 +604,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
         if (tid < KT) {
             const bool on = int(step) * KT + tid < a.rows;
             levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
-            levels[buf * 2 * KT + KT + tid] = on ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
+            levels[buf * 2 * KT + KT + tid] = on && !single ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
         }
         if constexpr (F::PLANES == 1) {
             arrived();
@@ -756,7 +780,7 @@ constexpr bool in_one(int format, int64_t columns, int64_t rows) { return format
 struct Plan {
     BwdArgs q{}, k{}, both{};
     bool fits = true;                     // every launch
-    int64_t delta = 0, g_levels = 0, q_levels = 0, v_levels = 0, k_levels = 0, part = 0, floats = 0;
+    int64_t delta = 0, g_levels = 0, q_levels = 0, v_levels = 0, k_levels = 0, single = 0, part = 0, floats = 0;
 };
 
 void share_out(BwdArgs &a, int64_t standing, int64_t passing, int kt, int64_t batch_heads) {
@@ -796,7 +820,7 @@ Plan plan(const lffn_cross_attention &c) {
     if (in_one(c.format, c.columns, a.rows)) share_out(p.both, a.rows, a.keys, 32, batch_heads);
     share_out(p.q, a.rows, a.keys, kt, batch_heads);
     share_out(p.k, a.keys, a.rows, in_pairs(c.format == LFFN_ROWS_F32 ? 2 : 1, int(c.columns)) ? 32 : kt, batch_heads);
-    p.fits = std::max({p.q.units, 2 * p.k.units, p.both.units, batch_heads * (a.g_tiles + a.v_tiles)}) <= MOST_THREADS / WG;
+    p.fits = std::max({p.q.units, 2 * p.k.units, p.both.units, batch_heads * (a.g_tiles + a.v_tiles) + c.B}) <= MOST_THREADS / WG;
     auto take = [&](int64_t floats) {
         const int64_t at = p.floats;
         p.floats += (floats + 3) / 4 * 4;
@@ -807,6 +831,7 @@ Plan plan(const lffn_cross_attention &c) {
     p.q_levels = take(scaled ? batch_heads * a.g_tiles : 0);
     p.v_levels = take(batch_heads * a.v_tiles);
     p.k_levels = take(scaled ? batch_heads * a.v_tiles : 0);
+    p.single = take(c.B);
     const int64_t of_q = p.q.splits > 1 ? p.q.splits * batch_heads * a.rows * a.columns : 0;
     const int64_t of_k = p.k.splits > 1 ? 2 * p.k.splits * batch_heads * a.keys * a.columns : 0;
     const int64_t of_both = p.both.splits > 1 ? p.both.splits * batch_heads * a.rows * a.columns : 0;
@@ -825,7 +850,8 @@ template <typename F, int DP, int KT>
 int launch(const Plan &p, hipStream_t stream) {
     constexpr bool LEVELS = F::LIFT != 0.f;
     const int64_t tiles = int64_t(p.q.batch_heads) * (p.q.g_tiles + p.q.v_tiles);
-    if (tiles > 0) delta_kernel<F, level_lanes(DP), LEVELS><<<dim3((unsigned)tiles), dim3(WG), 0, stream>>>(p.q);
+    const int64_t looks = p.q.mask ? p.q.batch_heads / p.q.key_heads : 0;               // for a single key, a workgroup a sequence
+    if (tiles + looks > 0) delta_kernel<F, level_lanes(DP), LEVELS><<<dim3((unsigned)(tiles + looks)), dim3(WG), 0, stream>>>(p.q);
     auto add_queries = [&](const BwdArgs &q) {
         if (q.splits > 1)
             add_splits<F>({{q.part, nullptr}, {q.gq, nullptr}, int64_t(q.batch_heads) * q.rows, q.q_len, q.heads, q.group, q.rows, q.splits, q.columns}, 1, stream);
@@ -904,6 +930,7 @@ extern "C" int lffn_cross_attention_bwd(const lffn_cross_attention *c, const voi
         a->out = static_cast<const char *>(out), a->g = static_cast<const char *>(g_out), a->lse = k.levels, a->rest = k.rest;
         a->gq = static_cast<char *>(grad_q), a->gk = static_cast<char *>(grad_k), a->gv = static_cast<char *>(grad_v);
         a->delta = w + p.delta, a->g_levels = w + p.g_levels, a->q_levels = w + p.q_levels, a->v_levels = w + p.v_levels, a->k_levels = w + p.k_levels, a->part = w + p.part;
+        a->single = reinterpret_cast<int32_t *>(w + p.single);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (c->format == LFFN_ROWS_F32) return launch<F32Two>(p, s);
