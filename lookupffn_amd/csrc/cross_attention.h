@@ -10,7 +10,7 @@
 // calls with work enough to pay for a launch that looks for the longest rows of every batch and key head: by them the numbers that pass are scaled (powers of two)
 // to half's range, those that stand each row by its own.  A number that passes is held to 2^-22 of itself, or to 2^-36 of the longest row of its head where that
 // is more, any other to 2^-22.  Elsewhere a float is three bfloat16 terms of 8 bits each, which together are it (the exponent range is the same, so nothing has to be
-// scaled), and of the nine products six are formed, those of at least 2^-16: what is left out is below 2^-22 of the product.  (Two terms for three, 16 x 512 x 512
+// scaled), and of the nine products six are formed, those of at least 2^-16: what is left out, second times third terms, is at most 2^-22 of the product.  (Two terms for three, 16 x 512 x 512
 // x 12 x 64: forward 77 us to 54 and 10 for the look, queries' gradients 111 to 78, keys' 159 to 113.)
 #pragma once
 
@@ -36,7 +36,8 @@ struct Frag {
     uint4 p[PLANES];
 };
 
-// Eight fp32 numbers as three bfloat16 terms by cutting off: exact.
+// Eight fp32 numbers as three bfloat16 terms: exact.  The first is cut off (rounded, the largest numbers would pass the range), the second, below 2^-7 of the first's
+// power of two, rounded to the nearest, so that the third is at most 2^-16 of it, of either sign (cut off as well: 2^-15, always towards zero, for which twice as much would be left out; within 1 % of the time).
 __device__ __forceinline__ void split3(const float (&v)[8], uint4 (&t)[3]) {
     uint32_t w[3][4];
 #pragma unroll
@@ -44,11 +45,11 @@ __device__ __forceinline__ void split3(const float (&v)[8], uint4 (&t)[3]) {
         float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-            const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-            w[k][i] = __builtin_amdgcn_perm(y, x, 0x07060302);       // the upper halves of both
+            // (the upper halves of both; of the third term nothing is left below them)
+            w[k][i] = k == 1 ? BF16Row::pack2(a, b) : __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
             if (k < 2) {
-                a -= __uint_as_float(x & 0xFFFF0000u);
-                b -= __uint_as_float(y & 0xFFFF0000u);
+                a -= __uint_as_float(w[k][i] << 16);
+                b -= __uint_as_float(w[k][i] & 0xFFFF0000u);
             }
         }
     }
