@@ -930,7 +930,7 @@ int lffn_qk_norm_rotary_bwd(const lffn_qk_norm_rotary *a, const void *g_q, const
  *   out[b, i, h] = sum_j p_j v[b, j, h'],  p = softmax_j(scale q[b, i, h] . k[b, j, h'])  over the keys that take part.
  * q: [B, q_len, heads, columns], k, v: [B, k_len, key_heads, columns], by strides (elements) of batch, token and head, multiples of 16 bytes,
  * as are the addresses; 128 tokens and the heads of a key head lie within 32 bits (token strides below 2^25 bytes, q's head stride times the heads that share a
- * key head below 2^30); columns lie together, a multiple of 8, at most 128.  key_mask: [B, k_len] bytes, not 0 where a key takes part, with a
+ * key head, where more than one does, below 2^30); columns lie together, a multiple of 8, at most 128.  key_mask: [B, k_len] bytes, not 0 where a key takes part, with a
  * batch stride, or NULL.  What keys and values that take no part hold does not matter.  A query without keys gets zeros.  scale: positive, finite.
  * format 0: fp32 accuracy (2e-7 of the result's norm against 64 bits), but keys and values, in the backward queries and
  * gradients too, may be held to 2^-36 of the longest such row of the batch and key head; 1 and 2: products of 16 bits, sums in fp32, softmax weights rounded to the format.

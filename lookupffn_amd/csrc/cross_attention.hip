@@ -433,10 +433,10 @@ __attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(co
     for (int d = 0; d < 3; ++d)
         for (const int64_t s : {a->q_strides[d], a->k_strides[d], a->v_strides[d]})
             LFFN_REQUIRE(s >= 0 && s * size % 16 == 0, LFFN_ERR_BAD_ARG);
-    // (the kernels address a tile's rows by 32 bits)
-    const int64_t far = int64_t(1) << 32;
+    // (the kernels address a tile's rows, of the heads that share a key head, by 32 bits)
+    const int64_t far = int64_t(1) << 32, group = a->heads / a->key_heads;
     LFFN_REQUIRE(a->k_strides[1] * size < far / 64 && a->v_strides[1] * size < far / 64 && a->q_strides[1] * size < far / 128 &&
-                     a->q_strides[2] * size < far / 4 / (a->heads / a->key_heads > 0 ? a->heads / a->key_heads : 1), LFFN_ERR_UNSUPPORTED);
+                     (group <= 1 || a->q_strides[2] * size <= (far / 4 - 1) / group), LFFN_ERR_UNSUPPORTED);
     const bool no_rows = a->B == 0 || a->q_len == 0 || a->heads == 0, no_keys = a->B == 0 || a->k_len == 0;
     LFFN_REQUIRE((a->q || no_rows) && ((a->k && a->v) || no_keys) && a->mask_stride >= 0, LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(lffn_aligned16(a->q) && lffn_aligned16(a->k) && lffn_aligned16(a->v), LFFN_ERR_BAD_ARG);

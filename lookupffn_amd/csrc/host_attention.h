@@ -40,10 +40,10 @@ Tensor aligned_contiguous(const Tensor &t) {
     return aligned(c) ? c : c.clone();
 }
 
-// [B, L, heads, columns] as the kernels read it, a copy where it has to be; near: 128 tokens and all heads within 32 bits.
-Tensor head_rows(const Tensor &t, bool near = false) {
+// [B, L, heads, columns] as the kernels read it, a copy where it has to be; near, if not 0: 128 tokens of so many neighbouring heads within 32 bits.
+Tensor head_rows(const Tensor &t, int64_t near = 0) {
     if (near && ((t.size(1) > 1 && t.stride(1) * t.element_size() >= int64_t(1) << 25) ||
-                 (t.size(2) > 1 && t.stride(2) * t.size(2) * t.element_size() >= int64_t(1) << 30)))
+                 (near > 1 && t.stride(2) * near * t.element_size() >= int64_t(1) << 30)))
         return aligned_contiguous(t);
     bool as_it_is = (t.stride(3) == 1 || t.size(3) == 1) && aligned(t);
     for (int d = 0; d < 3; ++d) as_it_is = as_it_is && (t.size(d) <= 1 || t.stride(d) * t.element_size() % 16 == 0);
@@ -294,9 +294,9 @@ struct AttentionInputs {
     double scale = 0;
 
     void lay_out() {
-        q = head_rows(q, true);
-        k = head_rows(k, true);
-        v = head_rows(v, true);
+        q = head_rows(q, q.size(2) / k.size(2));          // (the heads that share a key head)
+        k = head_rows(k, 1);
+        v = head_rows(v, 1);
         mask = neighbours_together(mask);
     }
 

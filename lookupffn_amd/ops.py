@@ -1331,18 +1331,23 @@ def _head_strides(t):
     return (ctypes.c_int64 * 3)(*(0 if n <= 1 else s for n, s in zip(t.shape, t.stride()[:3])))
 
 
-def _head_rows(t, near=False):
-    """t [B, L, heads, columns] as the kernels read it, a copy where it has to be: the columns together, addresses and strides of 16 bytes; near:
-    128 tokens and all heads within 32 bits."""
+def _head_rows(t, near=0):
+    """t [B, L, heads, columns] as the kernels read it, a copy where it has to be: the columns together, addresses and strides of 16 bytes; near, if not 0:
+    128 tokens of so many neighbouring heads within 32 bits."""
     if t is None:
         return None
     size = t.element_size()
-    if near and (t.shape[1] > 1 and t.stride(1) * size >= 1 << 25 or t.shape[2] > 1 and t.stride(2) * t.shape[2] * size >= 1 << 30):
+    if near and (t.shape[1] > 1 and t.stride(1) * size >= 1 << 25 or near > 1 and t.stride(2) * near * size >= 1 << 30):
         return t.contiguous()
     if (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and all(n <= 1 or s * size % 16 == 0
                                                                               for n, s in zip(t.shape, t.stride()[:3])):
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _sharing(q, k):
+    """Query heads that share a key head."""
+    return max(1, q.shape[2] // max(1, k.shape[2]))
 
 
 def _aligned(t):
@@ -1463,7 +1468,7 @@ def _cross_attention_impl(q, k, v, key_mask, scale, keep):
     """q [B, L, heads, columns], k, v [B, keys, key heads, columns], key_mask [B, keys] bool or None -> (out [B, L, heads, columns], with
     `keep` what the backward needs beside it, bytes)."""
     _lib.require_gpu(q, k, v, key_mask)
-    q, k, v, key_mask = _head_rows(q, True), _head_rows(k, True), _head_rows(v, True), _neighbours_together(key_mask)
+    q, k, v, key_mask = _head_rows(q, _sharing(q, k)), _head_rows(k, 1), _head_rows(v, 1), _neighbours_together(key_mask)
     a = _cross_attention_args(q, k, v, key_mask, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     kept = torch.empty(_kept_bytes(q) if keep else 0, dtype=torch.uint8, device=q.device)
@@ -1492,7 +1497,7 @@ _L.define("cross_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor? key_mask, f
 def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, kept, g, of_queries, of_keys):
     """-> the gradient of q if it is wanted, then those of k and v if they are."""
     _lib.require_gpu(q, k, v, key_mask, out, kept, g)
-    q, k, v, key_mask, g = _head_rows(q, True), _head_rows(k, True), _head_rows(v, True), _neighbours_together(key_mask), _aligned(g)
+    q, k, v, key_mask, g = _head_rows(q, _sharing(q, k)), _head_rows(k, 1), _head_rows(v, 1), _neighbours_together(key_mask), _aligned(g)
     a = _cross_attention_args(q, k, v, key_mask, scale)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys))]
     with _dev_guard(q):
