@@ -219,12 +219,25 @@ HOST_PATH = os.path.join(_PKG_DIR, "_host.so")
 loaded_host = None                    # False: not to be had
 
 
-def _load_host():
+def _import_host():
     if not os.path.exists(HOST_PATH):
         raise ImportError(f"{HOST_PATH} is missing")
     from . import _host as module
     if module.torch_version != str(torch.__version__):
         raise ImportError(f"{HOST_PATH} was built against torch {module.torch_version}, this is {torch.__version__}")
+    return module
+
+
+def host_module():
+    """The host library's module for what only C++ can look at, whichever path a call takes; None where it is missing or another torch's."""
+    try:
+        return _import_host()
+    except ImportError:
+        return None
+
+
+def _load_host():
+    module = _import_host()
     from . import ops
     from .lookup import BH4
     module.bind(LIB_PATH, torch.nn.LayerNorm, BH4, (ops.LN_BWD_PARTIALS, ops.PROJECT_BWD_PARTIALS, ops.COLUMN_SUM_CHUNK_ROWS))

@@ -46,6 +46,23 @@ def _recorded(*tensors):
     return not is_compiling() and forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def _refuse_foreign_leaves(*tensors):
+    """As the host path (csrc/host_attention.h) in front of its nodes: no forward is captured while a graph from before the capture holds one of its leaves, for
+    the captured backward would end the process.  Without the host library nothing tells whether one does, and no forward with gradients is captured."""
+    if is_compiling() or not torch.is_grad_enabled():
+        return
+    module = _lib.host_module()
+    if module is not None:
+        module.refuse_foreign_leaves(*tensors)
+        return
+    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf and t.is_cuda]
+    if leaves:
+        with torch.cuda.device(leaves[0].device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("lookupffn_amd: a forward with gradients is captured only with the host library (_host.so), which looks whether a graph from "
+                                   "before the capture still holds its leaves")
+
+
 def rotary_table(positions, columns, base=10000.0, device=None):
     """Cosines and sines for ``qk_norm_rotary``: [positions, columns] float32, of angles p * base^(-2 i / columns) taken in 64 bits, the cosines of
     columns / 2 angles and then the sines.  columns: a multiple of 16, how many of a head are rotated."""
@@ -115,6 +132,7 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, *, table=None, q_pos
         if out is not None:
             return out
     _lib.require_gpu(q, k, q_weight, k_weight, table, q_positions, k_positions)
+    _refuse_foreign_leaves(q, k, q_weight, k_weight if k is not None else None)
     _check_heads("q", q)
     columns = q.shape[3]
     _require(columns % 8 == 0 and 8 <= columns <= ops.QK_NORM_MAX_COLUMNS, f"q: heads of {columns} columns")
@@ -176,6 +194,7 @@ def cross_attention(q, k, v, key_mask=None, *, scale=None):
         if out is not None:
             return out
     _lib.require_gpu(q, k, v, key_mask)
+    _refuse_foreign_leaves(q, k, v)
     _check_heads("q", q)
     _check_heads("k", k, q)
     _check_heads("v", v, q)

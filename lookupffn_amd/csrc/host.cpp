@@ -689,6 +689,8 @@ PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
     {"qk_norm_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk_norm_rotary)), METH_FASTCALL, nullptr},
+    {"refuse_foreign_leaves", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(static_cast<PyObject *(*)(PyObject *, PyObject *const *, Py_ssize_t)>(refuse_foreign_leaves))),
+     METH_FASTCALL, nullptr},
     {"cross_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cross_attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

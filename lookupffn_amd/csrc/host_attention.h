@@ -94,6 +94,18 @@ void refuse_foreign_leaves(std::initializer_list<const Tensor *> tensors, const 
     }
 }
 
+// refuse_foreign_leaves(tensors or None ...): the same in front of Python's autograd functions
+PyObject *refuse_foreign_leaves(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (!THPVariable_Check(args[i])) continue;
+        const Tensor &t = THPVariable_Unpack(args[i]);
+        if (ordinary(t)) refuse_foreign_leaves({&t}, t.device());
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 // Queries or keys: four dimensions, a format, not empty.
 bool heads_tensor(PyObject *o, Tensor &t) {
     if (!plain(o)) return false;
