@@ -441,9 +441,10 @@ __attribute__((visibility("hidden"))) int lffn_internal_cross_attention_check(co
     LFFN_REQUIRE((a->q || no_rows) && ((a->k && a->v) || no_keys) && a->mask_stride >= 0, LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(lffn_aligned16(a->q) && lffn_aligned16(a->k) && lffn_aligned16(a->v), LFFN_ERR_BAD_ARG);
     const int64_t most = int64_t(1) << 30;
-    LFFN_REQUIRE(a->heads <= 65536 && a->q_len < most && a->k_len < most && a->B < most, LFFN_ERR_UNSUPPORTED);
-    LFFN_REQUIRE(no_rows || (a->q_len * (a->heads / a->key_heads) < most &&
-                             a->B * a->key_heads <= (int64_t(1) << 40) / (a->q_len * (a->heads / a->key_heads))), LFFN_ERR_UNSUPPORTED);
+    LFFN_REQUIRE(a->heads <= 65536 && a->key_heads <= 65536 && a->q_len < most && a->k_len < most && a->B < most, LFFN_ERR_UNSUPPORTED);
+    // (with no query head there may be key heads all the same; 2^32 of batches and heads times 2^23 tiles of keys is a number yet)
+    const int64_t rows = a->q_len * group;
+    LFFN_REQUIRE(rows < most && a->B * a->key_heads <= (int64_t(1) << 40) / (rows > 256 ? rows : 256), LFFN_ERR_UNSUPPORTED);
     return LFFN_OK;
 }
 
