@@ -1361,6 +1361,28 @@ def _neighbours_together(p):
     return p if p is None or p.shape[-1] <= 1 or p.stride(-1) == 1 else p.contiguous()
 
 
+def _fit_heads(q, *others):
+    assert q.dim() == 4 and row_format(q.dtype) is not None
+    for t in others:
+        assert t is None or t.dim() == 4 and t.dtype == q.dtype and t.shape[0] == q.shape[0] and t.shape[3] == q.shape[3]
+
+
+def _fit_norm(q, k, q_weight, k_weight, table, q_positions, k_positions):
+    """Arrays that do not fit each other would be read beyond their ends."""
+    _fit_heads(q, k)
+    assert all(w is None or w.dtype == torch.float32 and w.shape == q.shape[3:] for w in (q_weight, k_weight))
+    assert table is None or table.dtype == torch.float32 and table.dim() == 2
+    for p, t in ((q_positions, q), (k_positions, k)):
+        assert p is None or t is not None and p.dtype in (torch.int32, torch.int64) and p.shape in (t.shape[:2], t.shape[1:2])
+    assert q_positions is None or k_positions is None or q_positions.dtype == k_positions.dtype
+
+
+def _fit_attention(q, k, v, key_mask):
+    _fit_heads(q, k, v)
+    assert v.shape == k.shape and k.shape[2] >= 1 and q.shape[2] % k.shape[2] == 0
+    assert key_mask is None or key_mask.dtype == torch.bool and key_mask.shape == k.shape[:2]
+
+
 def _qk_norm_rotary_args(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved):
     a = _lib.QkNormRotary()
     a.q, a.k, a.q_weight, a.k_weight, a.table = (_lib.ptr(t) for t in (q, k, q_weight, k_weight, table))
@@ -1386,6 +1408,7 @@ def _qk_norm_rotary_impl(q, k, q_weight, k_weight, table, q_positions, k_positio
     """q, k [B, L, heads, columns] (k None: one result); weights [columns], table [positions, rotary] fp32; positions [B, L] or [L], int32 or
     int64, both alike."""
     _lib.require_gpu(q, k, q_weight, k_weight, table, q_positions, k_positions)
+    _fit_norm(q, k, q_weight, k_weight, table, q_positions, k_positions)
     q, k, q_weight, k_weight, table = _head_rows(q), _head_rows(k), _aligned(q_weight), _aligned(k_weight), _aligned(table)
     q_positions, k_positions = _neighbours_together(q_positions), _neighbours_together(k_positions)
     out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k) if t is not None]
@@ -1412,6 +1435,9 @@ def _qk_norm_rotary_bwd_impl(q, k, q_weight, k_weight, table, q_positions, k_pos
                              want_k_weight):
     """-> gradients of q, of k where there is one, and of the weights that are wanted."""
     _lib.require_gpu(q, k, q_weight, k_weight, table, q_positions, k_positions, g_q, g_k)
+    _fit_norm(q, k, q_weight, k_weight, table, q_positions, k_positions)
+    for g, t in ((g_q, q), (g_k, k)):
+        assert (g is None) == (t is None) and (g is None or g.shape == t.shape and g.dtype == t.dtype)
     q, k, q_weight, k_weight, table = _head_rows(q), _head_rows(k), _aligned(q_weight), _aligned(k_weight), _aligned(table)
     q_positions, k_positions, g_q, g_k = _neighbours_together(q_positions), _neighbours_together(k_positions), _aligned(g_q), _aligned(g_k)
     out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k) if t is not None]
@@ -1468,6 +1494,7 @@ def _cross_attention_impl(q, k, v, key_mask, scale, keep):
     """q [B, L, heads, columns], k, v [B, keys, key heads, columns], key_mask [B, keys] bool or None -> (out [B, L, heads, columns], with
     `keep` what the backward needs beside it, bytes)."""
     _lib.require_gpu(q, k, v, key_mask)
+    _fit_attention(q, k, v, key_mask)
     q, k, v, key_mask = _head_rows(q, _sharing(q, k)), _head_rows(k, 1), _head_rows(v, 1), _neighbours_together(key_mask)
     a = _cross_attention_args(q, k, v, key_mask, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -1497,6 +1524,8 @@ _L.define("cross_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor? key_mask, f
 def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, kept, g, of_queries, of_keys):
     """-> the gradient of q if it is wanted, then those of k and v if they are."""
     _lib.require_gpu(q, k, v, key_mask, out, kept, g)
+    _fit_attention(q, k, v, key_mask)
+    assert all(t.shape == q.shape and t.dtype == q.dtype for t in (out, g)) and kept.dtype == torch.uint8 and kept.shape == (_kept_bytes(q),)
     q, k, v, key_mask, g = _head_rows(q, _sharing(q, k)), _head_rows(k, 1), _head_rows(v, 1), _neighbours_together(key_mask), _aligned(g)
     a = _cross_attention_args(q, k, v, key_mask, scale)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys))]
