@@ -353,7 +353,8 @@ struct CrossAttentionBackward : public torch::autograd::Node {
         at::AutoGradMode no_grad(false);
         const auto self = shared_from_this();
         AttentionInputs in{q.unpack(self), k.unpack(self), v.unpack(self), mask.unpack(self), scale};
-        const Tensor result_ = result.unpack(self), kept_ = kept.unpack(self), g = aligned_contiguous(grads[0]);
+        // (hooks on saved tensors may have laid out anew what the forward left contiguous)
+        const Tensor result_ = aligned_contiguous(result.unpack(self)), kept_ = aligned_contiguous(kept.unpack(self)), g = aligned_contiguous(grads[0]);
         const at::Device dev = in.q.device();
         const c10::DeviceGuard guard(dev);
         void *st = stream_on(dev);

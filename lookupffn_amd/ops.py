@@ -1526,6 +1526,7 @@ def _cross_attention_bwd_impl(q, k, v, key_mask, scale, out, kept, g, of_queries
     _lib.require_gpu(q, k, v, key_mask, out, kept, g)
     _fit_attention(q, k, v, key_mask)
     assert all(t.shape == q.shape and t.dtype == q.dtype for t in (out, g)) and kept.dtype == torch.uint8 and kept.shape == (_kept_bytes(q),)
+    out, kept = _aligned(out), _aligned(kept)
     q, k, v, key_mask, g = _head_rows(q, _sharing(q, k)), _head_rows(k, 1), _head_rows(v, 1), _neighbours_together(key_mask), _aligned(g)
     a = _cross_attention_args(q, k, v, key_mask, scale)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys))]
