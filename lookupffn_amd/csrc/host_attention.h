@@ -50,6 +50,13 @@ Tensor head_rows(const Tensor &t, int64_t near = 0) {
     return as_it_is ? t : aligned_contiguous(t);
 }
 
+// What hooks on saved tensors gave back has the type and shape of what was saved: the kernels' reads go by one array's.
+constexpr const char *OTHER = "lookupffn_amd: a hook on saved tensors gave back one of another type or shape";
+bool alike(const Tensor &a, const Tensor &b) { return a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes() && a.device() == b.device(); }
+bool heads_of(const Tensor &t, const Tensor &q) {
+    return t.dim() == 4 && t.scalar_type() == q.scalar_type() && t.size(0) == q.size(0) && t.size(3) == q.size(3) && t.numel() > 0 && t.device() == q.device();
+}
+
 Tensor neighbours_together(const Tensor &t) {
     return !t.defined() || t.size(t.dim() - 1) <= 1 || t.stride(t.dim() - 1) == 1 ? t : t.contiguous();
 }
@@ -161,6 +168,16 @@ struct NormInputs {
     }
 };
 
+bool norm_weight(const Tensor &w, const Tensor &t) {
+    return !w.defined() || (w.dim() == 1 && w.size(0) == t.size(3) && w.scalar_type() == at::kFloat);
+}
+
+bool norm_positions(const Tensor &p, const Tensor &t) {
+    if (!p.defined()) return true;
+    if (p.scalar_type() != at::kLong && p.scalar_type() != at::kInt) return false;
+    return p.dim() == 1 ? p.size(0) == t.size(1) : p.dim() == 2 && p.size(0) == t.size(0) && p.size(1) == t.size(1);
+}
+
 struct QkNormRotaryBackward : public torch::autograd::Node {
     SavedVariable q, k, q_weight, k_weight, table, q_positions, k_positions;
     double eps = 0;
@@ -179,6 +196,14 @@ struct QkNormRotaryBackward : public torch::autograd::Node {
         return out;
     }
 
+    static void fit(const NormInputs &in, const variable_list &grads) {
+        TORCH_CHECK(heads_of(in.q, in.q) && (!in.k.defined() || heads_of(in.k, in.q)) && (!grads[0].defined() || alike(in.q, grads[0])) &&
+                        (!grads[1].defined() || (in.k.defined() && alike(in.k, grads[1]))) && norm_weight(in.q_weight, in.q) && norm_weight(in.k_weight, in.q) &&
+                        (!in.table.defined() || (in.table.dim() == 2 && in.table.scalar_type() == at::kFloat)) && norm_positions(in.q_positions, in.q) &&
+                        (!in.k_positions.defined() || (in.k.defined() && norm_positions(in.k_positions, in.k))) &&
+                        (!in.q_positions.defined() || !in.k_positions.defined() || in.q_positions.scalar_type() == in.k_positions.scalar_type()), OTHER);
+    }
+
     variable_list gradients(const variable_list &grads) {
         variable_list out(4);
         if (!grads[0].defined() && !grads[1].defined()) return out;
@@ -189,6 +214,7 @@ struct QkNormRotaryBackward : public torch::autograd::Node {
         const at::Device dev = in.q.device();
         const c10::DeviceGuard guard(dev);
         void *st = stream_on(dev);
+        fit(in, grads);
         in.lay_out();
         const lffn_qk_norm_rotary a = in.arguments();
         const Tensor g_q = grads[0].defined() ? aligned_contiguous(grads[0]) : at::zeros(in.q.sizes(), in.q.options());
@@ -208,16 +234,6 @@ struct QkNormRotaryBackward : public torch::autograd::Node {
         return out;
     }
 };
-
-bool norm_weight(const Tensor &w, const Tensor &t) {
-    return !w.defined() || (w.dim() == 1 && w.size(0) == t.size(3) && w.scalar_type() == at::kFloat);
-}
-
-bool norm_positions(const Tensor &p, const Tensor &t) {
-    if (!p.defined()) return true;
-    if (p.scalar_type() != at::kLong && p.scalar_type() != at::kInt) return false;
-    return p.dim() == 1 ? p.size(0) == t.size(1) : p.dim() == 2 && p.size(0) == t.size(0) && p.size(1) == t.size(1);
-}
 
 // qk_norm_rotary(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved) -> (q, k or None), or None: not for this path
 PyObject *qk_norm_rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -358,6 +374,9 @@ struct CrossAttentionBackward : public torch::autograd::Node {
         const at::Device dev = in.q.device();
         const c10::DeviceGuard guard(dev);
         void *st = stream_on(dev);
+        TORCH_CHECK(alike(in.q, g) && heads_of(in.q, in.q) && heads_of(in.k, in.q) && alike(in.v, in.k) && in.q.size(2) % in.k.size(2) == 0 && alike(result_, in.q) &&
+                        kept_.scalar_type() == at::kByte && kept_.dim() == 1 && kept_.device() == dev &&
+                        (!in.mask.defined() || (in.mask.scalar_type() == at::kBool && in.mask.sizes() == in.k.sizes().slice(0, 2))), OTHER);
         in.lay_out();
         const lffn_cross_attention a = in.arguments();
         const bool of_keys = task_should_compute_output(1) || task_should_compute_output(2);
@@ -367,6 +386,8 @@ struct CrossAttentionBackward : public torch::autograd::Node {
             out[2] = at::empty(in.v.sizes(), in.v.options());
         }
         int64_t bytes = 0;
+        CALL(lffn_cross_attention_kept_bytes, &a, &bytes);
+        TORCH_CHECK(kept_.numel() == bytes, OTHER);
         CALL(lffn_cross_attention_bwd_workspace_bytes, &a, &bytes);
         const Tensor ws = empty_bytes(bytes, dev);
         CALL(lffn_cross_attention_bwd, &a, result_.data_ptr(), kept_.data_ptr(), g.data_ptr(), out[0].defined() ? out[0].data_ptr() : nullptr,
