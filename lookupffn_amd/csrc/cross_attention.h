@@ -37,7 +37,8 @@ struct Frag {
 };
 
 // Eight fp32 numbers as three bfloat16 terms: exact.  The first is cut off (rounded, the largest numbers would pass the range), the second, below 2^-7 of the first's
-// power of two, rounded to the nearest, so that the third is at most 2^-16 of it, of either sign (cut off as well: 2^-15, always towards zero, for which twice as much would be left out; within 1 % of the time).
+// power of two, rounded to the nearest, so that the third is at most 2^-16 of it, of either sign (cut off as well, 2^-15, always towards zero: within 1 % of the time,
+// and twice as much left out).
 __device__ __forceinline__ void split3(const float (&v)[8], uint4 (&t)[3]) {
     uint32_t w[3][4];
 #pragma unroll
@@ -431,7 +432,8 @@ __device__ __forceinline__ int own_rows(const char *row, bool live, int half, in
     return exponent;
 }
 
-// Division of numbers below 2^31 by one that the host knows: the compiler's division takes thirty instructions, this one three.
+// Division of numbers below 2^31 by one that the host knows (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994): the compiler's takes
+// thirty instructions, this one three.
 struct Divisor {
     uint32_t by, multiplier, shift;
     Divisor() = default;
@@ -627,10 +629,10 @@ inline Kept kept_at(void *p, int64_t rows, int bytes) {
     return {static_cast<float *>(p), at && bytes == 2 ? at + (rows * 4 + 15) / 16 * 16 : nullptr};
 }
 
-// Which unit of work a workgroup has: neighbours (tiles that read the same keys) on one XCD.
 // Threads of a launch at most.
 constexpr int64_t MOST_THREADS = UINT32_MAX;
 
+// Which unit of work a workgroup has: neighbours (tiles that read the same keys) on one XCD.
 struct Unit {
     int tile, split, bh, b, kh;
 };

@@ -39,7 +39,7 @@ struct Args {
 // What a lane holds of a row: vectors a and b (in units of 16 bytes), partners where the row is rotated by halves.
 struct Slot {
     int a, b;
-    bool has_a, has_b, turned_a, turned_b;
+    bool has_a, has_b, turned;
 };
 template <typename R>
 __device__ __forceinline__ Slot slot_of(int s, int columns, int rotary) {
@@ -49,7 +49,7 @@ __device__ __forceinline__ Slot slot_of(int s, int columns, int rotary) {
     o.b = s < half ? s + half : turned + rest + 1;
     o.has_a = o.a < vectors;
     o.has_b = o.b < vectors;
-    o.turned_a = o.turned_b = s < half;
+    o.turned = s < half;
     return o;
 }
 
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(WG) void norm_rotary_kernel(Args a) {
     const Tensor &t = a.t[second];
     const int wg = blockIdx.x - (second ? a.t[0].workgroups : 0), lane = threadIdx.x % LPR;
     const Slot s = slot_of<R>(lane, a.columns, a.rotary);
-    const bool turned = s.turned_a && a.rotary > 0;
+    const bool turned = s.turned;
     float wa[N], wb[N], ga[N] = {}, gb[N] = {};
     load_weight<N>(t.w, s.a, s.has_a, wa);
     load_weight<N>(t.w, s.b, s.has_b, wb);
