@@ -7,7 +7,7 @@
 // whose results a second kernel joins.
 //
 // Bound by the products where there are many rows, else by memory.  4 x 2048 rows x 4096 keys x 16 heads x 128 columns bfloat16 300 us, 0.92 PFLOP/s of the 1.26 that a
-// large product reaches; 32 x 512 x 512 x 12 x 64 fp32 100 and 21 for the look at keys and values; one row of 32 heads on 4 x 16384 keys x 8 x 128 bfloat16, an eighth of
+// large product reaches; 32 x 512 x 512 x 12 x 64 fp32 95 and 21 for the look at keys and values; one row of 32 heads on 4 x 16384 keys x 8 x 128 bfloat16, an eighth of
 // them masked, 52 us, 4.5 TB/s, and 5 for the join.
 #include "cross_attention.h"
 
@@ -169,6 +169,7 @@ __global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F:
                 s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], by_c, -less));
                 of_step[e % (F::PLANES == 1 ? 2 : 4)] += s[kb][e];
             }
+            // (16 bits: weights of one term, a rounding each of either sign beside the result's one: 1.4 times its error; two terms would be three products for two)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float t[8];

@@ -9,6 +9,7 @@
 //
 // Half precision, and fp32 numbers in two terms of it: p is held 2^14 times larger (at most 2^14), ds times a power of two that takes 2 |g| |v|, of the
 // longest rows of the batch and key head, which no ds exceeds, below 2^15: gradients of any size, and weights of many keys, stay among half's normal numbers.
+// 16 bits: weights and ds are operands of one term, a rounding each beside the gradients' own (1.4 to 1.5 times that alone; two terms each would be ten products for seven).
 // fp32 numbers are scaled by the longest rows of q, k, v and g in the same way, and p and ds once more by what a key's, or a query's, largest so far leaves
 // of half's range (fit).
 //
