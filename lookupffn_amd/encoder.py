@@ -204,10 +204,12 @@ class CrossAttention(nn.Module):
         self.register_buffer("rotary", rotary_table(config.max_position_embeddings, columns) if columns else None, persistent=False)
 
     def _apply(self, fn, recurse=True):
-        # the rotation goes where the module goes, in float32: 16 bits would turn far positions by other angles
+        # the rotation goes where the module goes, in float32: 16 bits would turn far positions by other angles; a module that gets its memory only now has none to bring
         table = self.rotary
         super()._apply(fn, recurse)
-        if table is not None and self.rotary.dtype != table.dtype:
+        if table is not None and table.is_meta and not self.rotary.is_meta:
+            self.rotary = rotary_table(*table.shape, device=self.rotary.device)
+        elif table is not None and self.rotary.dtype != table.dtype:
             self.rotary = table.to(self.rotary.device)
         return self
 
