@@ -158,8 +158,8 @@ __global__ __launch_bounds__(WG, F::PLANES <= 2 && DP <= 64 ? 3 : DP <= 64 || F:
             most = to;
         }
         const float less = (most == -INFINITY ? 0.f : most) * by_c - F::LIFT;
-        // A step's weights are added up by themselves: one after the other onto the sum of all keys so far, each rounded as that is, 16384 of them left a row 1e-6
-        // off, so 2.5e-7.  (In as many sums as cost no time: two for four 4096 x 16384 x 8 x 72 fp32 942 us, 953; 4 x 2048 x 4096 x 16 x 128 bfloat16 313, 310.)
+        // A step's weights are added up by themselves: one after the other onto the sum of all keys so far, each rounded as that is, 16384 of them left a row 9.8e-7
+        // off, so 3.6e-7.  (In as many sums as cost no time: two for four 4096 x 16384 x 8 x 72 fp32 942 us, 953; 4 x 2048 x 4096 x 16 x 128 bfloat16 313, 310.)
         float of_step[F::PLANES == 1 ? 2 : 4] = {};
         Op p[2 * KB];
 #pragma unroll

@@ -116,3 +116,21 @@ def test_compiled(backend):
     want = _step(_block, parts)
     for _ in range(2):
         assert all(torch.equal(a, b) for a, b in zip(_step(compiled, parts), want))
+
+
+def test_batched_gradients_are_refused_and_a_jacobian_is_not():
+    """Gradients of many vectors in one pass, which the backward does not take; one after the other they are those of the formula."""
+    q, k, v = (t[:1, :3, :2, :16].float().clone() for t in _inputs())
+    leaf = q.clone().requires_grad_()
+    out = cross_attention(leaf, k, v)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaf, torch.eye(out.numel(), device=DEV).view(-1, *out.shape), is_grads_batched=True)
+    got = torch.autograd.functional.jacobian(lambda t: cross_attention(t, k, v), q)
+    q64, k64, v64 = (t.double().cpu() for t in (q, k, v))
+    want = torch.autograd.functional.jacobian(lambda t: torch.einsum("bhij,bjhd->bihd", (torch.einsum("bihd,bjhd->bhij", t, k64) / 4).softmax(-1), v64), q64)
+    # sums of three keys and sixteen columns, of terms of size 1 to 4: some ten roundings of 2^-24
+    assert (got.double().cpu() - want).abs().max() <= 2.0 ** -19
+    leaf = q.clone().requires_grad_()
+    y, _ = qk_norm_rotary(leaf)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaf, torch.eye(y.numel(), device=DEV).view(-1, *y.shape), is_grads_batched=True)
