@@ -933,7 +933,8 @@ int lffn_qk_norm_rotary_bwd(const lffn_qk_norm_rotary *a, const void *g_q, const
  * key head, where more than one does, below 2^30); columns lie together, a multiple of 8, at most 128.  key_mask: [B, k_len] bytes, not 0 where a key takes part, with a
  * batch stride, or NULL.  What keys and values that take no part hold does not matter.  A query without keys gets zeros.  scale: positive, finite.
  * format 0: fp32 accuracy (against 64 bits, numbers of N(0, 1): results 2e-7 to 4e-7 of their norm off with up to 700 keys, 1.1e-6 with 8192 and
- * 2.3e-6 with 32768; gradients 3e-7 to 6.3e-7 with up to 700 rows and keys, 1.6e-6 with 12800 rows and 9000 keys, 2.5e-6 with 32768 keys), but keys and values, in the backward queries and
+ * 2.3e-6 with 32768; gradients 3e-7 to 6.3e-7 with up to 700 rows and keys, 1.6e-6 with 12800 rows and 9000 keys, 2.5e-6 with 32768 keys; with scores up to
+ * 40 2e-6 to 3.5e-6), but keys and values, in the backward queries and
  * gradients too, may be held to 2^-36 of the longest such row of the batch and key head; 1 and 2: products of 16 bits, sums in fp32, softmax weights, and in the backward the scores' gradients,
  * rounded to the format (2: those to 2^-39 of twice the longest gradient row times the longest value row of the batch and key head).
  * A launch has fewer than 2^32 threads (B * key_heads below some 4 million with single tokens and many keys, 8 million in the backward), else LFFN_ERR_UNSUPPORTED.

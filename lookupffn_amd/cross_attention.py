@@ -183,7 +183,8 @@ def cross_attention(q, k, v, key_mask=None, *, scale=None):
     scale: positive, 1 / sqrt(columns) if None.  One query a sequence is the step of a decoder over kept keys and values.
 
     float32: products of two half-precision or three bfloat16 terms a number, sums in float32, errors of the size of float32 products' (results 2e-7 to 4e-7 of their norm with up
-    to 700 keys, 1.1e-6 with 8192, 2.3e-6 with 32768; gradients 3e-7 to 6.3e-7 with up to 700 rows and keys, 2.5e-6 with 32768 keys); with two terms (large
+    to 700 keys, 1.1e-6 with 8192, 2.3e-6 with 32768; gradients 3e-7 to 6.3e-7 with up to 700 rows and keys, 2.5e-6 with 32768 keys,
+    3.5e-6 with scores up to 40); with two terms (large
     calls, and the backward) a number of k or v (backward: also q and the gradient) 2^14 times smaller than the longest row of its batch and head begins to lose
     bits.  16 bits: softmax weights (backward: the scores' gradients, too) rounded to the type, sums in float32, one rounding of the result; a half-precision gradient row 2^16 times smaller than
     the longest of its batch and head begins to lose bits.  Infinities and NaN of keys that take part may make any result of their head NaN.
