@@ -60,8 +60,9 @@ __device__ __forceinline__ void look_for_a_single_key(const BwdArgs &a, int b) {
     }
     if (threadIdx.x == 0) a.single[b] = found == 1;
 }
-// A key that takes part alone has all the weight, and ds is nothing; g . v and delta, summed in different orders, would leave their roundings.  So both are held to zero.
-__device__ __forceinline__ bool single_key(const BwdArgs &a, int b) { return a.mask ? a.single[b] != 0 : a.keys == 1; }
+// What the queries' and keys' gradients are multiplied with.  A key that takes part alone has all the weight, and ds is nothing; g . v and delta, summed in different orders,
+// would leave their roundings.
+__device__ __forceinline__ float gradient_scale(const BwdArgs &a, int b) { return (a.mask ? a.single[b] != 0 : a.keys == 1) ? 0.f : a.scale; }
 
 // delta of every row; half precision: the longest rows of g and v as well; fp32 numbers in two terms: of q and k, too.  A lane has 8 columns, the rows of a group of lanes are
 // asked for together.  Bound by memory: out, its rest and g (and v, q, k) once.  (Rows one after the other, 1024 a workgroup: 4 x 2048 rows of 16 x 128 bfloat16
@@ -190,10 +191,9 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
     Op fq[CHUNKS], fg[CHUNKS];
     const int eq = own_rows<F>(Rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group}.at(live ? row : 0), live, half, pieces, fq);
     const int eg = own_rows<F>(a.g + out_row, live, half, pieces, fg);
-    const bool single = single_key(a, b);
-    const float f = single ? 0.f : power(e2.ds - eg - e2.v), by_c = __builtin_amdgcn_ldexpf(a.c, -(eq + e2.k));
+    const float f = power(e2.ds - eg - e2.v), by_c = __builtin_amdgcn_ldexpf(a.c, -(eq + e2.k));
     const float level = live ? a.lse[int64_t(bh) * a.rows + row] : INFINITY;
-    const float delta = live && !single ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], e2.ds) : 0.f;
+    const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], e2.ds) : 0.f;
     ca_f32x16_t dq[DB] = {};
     int fitted = F::SCALED ? FIT_FIRST : 0;
 
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(WG, F::PLANES == 1 && DP <= 64 ? 3 : F::PLANES == 1
 
     const int64_t begin = split * a.split_steps, end = begin + a.split_steps < a.steps ? begin + a.split_steps : a.steps;
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
-    const auto by = factor<F>(a.scale, -(e2.ds + e2.k + fitted));
+    const auto by = factor<F>(gradient_scale(a, b), -(e2.ds + e2.k + fitted));
     if (a.splits > 1) store_row<F32, DB>(dq, by, reinterpret_cast<char *>(a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns), live, a.columns, half);
     else store_row<F, DB>(dq, by, a.gq + out_row, live, a.columns, half);
 }
@@ -305,10 +305,9 @@ __global__ __launch_bounds__(WG, 2) void gradients_kernel(BwdArgs a) {
     constexpr bool HALF = F::LIFT != 0.f;
     const Exponents e2 = exponents<F>(a, bh);
     const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
-    const bool single = single_key(a, b);
-    const float f = single ? 0.f : power(of_delta);
+    const float f = power(of_delta);
     const float level = live ? a.lse[int64_t(bh) * a.rows + row] - (HALF ? P_LIFT : 0.f) : INFINITY;
-    const float delta = live && !single ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], of_delta) : 0.f;
+    const float delta = live ? __builtin_amdgcn_ldexpf(a.delta[int64_t(bh) * a.rows + row], of_delta) : 0.f;
     KeyFeed<F, DP, KT> feed(lds + PASSING, pieces, kp, vp, a.kt, a.vt);
     const typename T::Reader read(lds + PASSING, lane);
     const typename Own::Reader read_own(lds, lane);
@@ -326,7 +325,7 @@ __global__ __launch_bounds__(WG, 2) void gradients_kernel(BwdArgs a) {
     const typename Turned::Reader read_turned(lds + WEIGHTS + (of_v ? 0 : Turned::SIZE), lane);
     typename Own::Reader read_mine(lds + (of_v ? GRADIENTS_AT : 0), lane);
     read_mine.lo[0] = d ? read_mine.lo[1] : read_mine.lo[0], read_mine.hi[0] = d ? read_mine.hi[1] : read_mine.hi[0];
-    const float by = of_v ? (HALF ? power(-int(P_LIFT)) : 1.f) : __builtin_amdgcn_ldexpf(a.scale, -e2.ds);
+    const float by_q = __builtin_amdgcn_ldexpf(gradient_scale(a, b), -e2.ds), by = of_v ? (HALF ? power(-int(P_LIFT)) : 1.f) : by_q;
     char *const to = (of_v ? a.gv : a.gk) + d * 32 * F::BYTES;
     int64_t formed = -1;                  // the step that `sum` is of
     uint32_t formed_word = 0;
@@ -382,7 +381,6 @@ __global__ __launch_bounds__(WG, 2) void gradients_kernel(BwdArgs a) {
 
     walk_keys<KT>(feed, words, mask, begin, end, a.keys, compute);
     store();
-    const float by_q = __builtin_amdgcn_ldexpf(a.scale, -e2.ds);
     if (a.splits > 1) store_row<F32, DB>(dq, by_q, reinterpret_cast<char *>(a.part + ((int64_t(split) * a.batch_heads + bh) * a.rows + row) * a.columns), live, a.columns, half);
     else store_row<F, DB>(dq, by_q, a.gq + heads_row(b, kh, live ? row : 0, a.q_len, a.key_heads, a.group) * a.columns * F::BYTES, live, a.columns, half);
 }
@@ -412,8 +410,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
     Op fk[CHUNKS], fv[CHUNKS];
     const int ek = own_rows<F>(a.k + b * a.kb + kh * a.kh + at_key * a.kt, true, half, pieces, fk);
     const int ev = own_rows<F>(a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, fv);
-    const bool single = single_key(a, b);
-    const float f = single ? 0.f : power(of_delta - e2.g - ev), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + ek));
+    const float f = power(of_delta - e2.g - ev), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + ek));
 
     // Rows beyond the last are the last once more: their levels are infinite and so their weights zero.  A step's addresses go by its first token; where
     // the heads that share a key divide KT they are the same for every step.
@@ -445,7 +442,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
         if (tid < KT) {
             const bool on = int(step) * KT + tid < a.rows;
             levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
-            levels[buf * 2 * KT + KT + tid] = on && !single ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
+            levels[buf * 2 * KT + KT + tid] = on ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
         }
         feed.end(buf);
     };
@@ -514,7 +511,7 @@ __global__ __launch_bounds__(WG, DP <= 64 ? 2 : 1) void key_gradient_kernel(BwdA
 #pragma unroll
         for (int d = 0; d < DB; ++d) dk[d] = ca_f32x16_t{}, dv[d] = ca_f32x16_t{};
     }
-    const auto by_k = factor<F>(a.scale, -(e2.ds + e2.q + fitted_ds)), by_v = factor<F>(1.f, (HALF ? -int(P_LIFT) : 0) - e2.g - fitted_p);
+    const auto by_k = factor<F>(gradient_scale(a, b), -(e2.ds + e2.q + fitted_ds)), by_v = factor<F>(1.f, (HALF ? -int(P_LIFT) : 0) - e2.g - fitted_p);
     if (a.splits > 1) {
         const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key) * a.columns;
         store_row<F32, DB>(dk, by_k, reinterpret_cast<char *>(a.part + of), in, a.columns, half);
@@ -564,8 +561,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
     const int of_delta = HALF ? e2.ds - int(P_LIFT) : 0;
     Op own[CHUNKS];                       // the weights' wavefront: keys; the other: values
     const int of_own = own_rows<F>(OF_V ? a.k + b * a.kb + kh * a.kh + at_key * a.kt : a.v + b * a.vb + kh * a.vh + at_key * a.vt, true, half, pieces, own);
-    const bool single = single_key(a, b);
-    const float f = single ? 0.f : power(of_delta - e2.g - of_own), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + of_own));
+    const float f = power(of_delta - e2.g - of_own), by_c = __builtin_amdgcn_ldexpf(a.c, -(e2.q + of_own));
 
     const Rows rows{a.q + b * a.qb + kh * a.group.by * a.qh, a.qt, a.qh, a.group};
     const int64_t g_token = int64_t(a.key_heads) * a.group.by * a.columns * F::BYTES;
@@ -605,7 +601,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
         if (tid < KT) {
             const bool on = int(step) * KT + tid < a.rows;
             levels[buf * 2 * KT + tid] = on ? level - (HALF ? P_LIFT : 0.f) : INFINITY;
-            levels[buf * 2 * KT + KT + tid] = on && !single ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
+            levels[buf * 2 * KT + KT + tid] = on ? __builtin_amdgcn_ldexpf(delta, of_delta) : 0.f;
         }
         if constexpr (F::PLANES == 1) {
             arrived();
@@ -704,7 +700,7 @@ __device__ __forceinline__ void key_gradient_pairs(const BwdArgs &a, uint4 *cons
 #pragma unroll
         for (int d = 0; d < DB; ++d) sums[d] = ca_f32x16_t{};
     }
-    const auto by = OF_V ? factor<F>(1.f, (HALF ? -int(P_LIFT) : 0) - e2.g - fitted) : factor<F>(a.scale, -(e2.ds + e2.q + fitted));
+    const auto by = OF_V ? factor<F>(1.f, (HALF ? -int(P_LIFT) : 0) - e2.g - fitted) : factor<F>(gradient_scale(a, b), -(e2.ds + e2.q + fitted));
     if (a.splits > 1) {
         const int64_t all = int64_t(a.batch_heads) * a.keys, of = (split * all + bh * a.keys + key + (OF_V ? a.splits * all : 0)) * a.columns;
         store_row<F32, DB>(sums, by, reinterpret_cast<char *>(a.part + of), in, a.columns, half);
@@ -822,9 +818,10 @@ Plan plan(const lffn_cross_attention &c) {
     share_out(p.q, a.rows, a.keys, kt, batch_heads);
     share_out(p.k, a.keys, a.rows, in_pairs(c.format == LFFN_ROWS_F32 ? 2 : 1, int(c.columns)) ? 32 : kt, batch_heads);
     p.fits = std::max({p.q.units, 2 * p.k.units, p.both.units, batch_heads * (a.g_tiles + a.v_tiles) + c.B}) <= MOST_THREADS / WG;
+    // (whole lines: parts that began 16 bytes into one were written in 47 us for 43, keys' gradients of 4 x 333 x 509 x 8 x 128 fp32)
     auto take = [&](int64_t floats) {
         const int64_t at = p.floats;
-        p.floats += (floats + 3) / 4 * 4;
+        p.floats += (floats + 63) / 64 * 64;
         return at;
     };
     p.delta = take(batch_heads * a.rows);
