@@ -41,7 +41,7 @@ extern "C" {
 #define LFFN_ERR_LAUNCH      -3   /* hipGetLastError() after the launch was not hipSuccess */
 #define LFFN_ERR_SCRATCH     -4   /* an entry point that allocates nothing: the shape exceeds its static scratch */
 
-#define LFFN_ABI_VERSION 16
+#define LFFN_ABI_VERSION 17
 
 /* ABI version of the loaded library (LFFN_ABI_VERSION at build time). */
 int lffn_version(void);
@@ -962,6 +962,81 @@ int lffn_cross_attention_fwd(const lffn_cross_attention *a, void *out, void *kep
 int lffn_cross_attention_bwd_workspace_bytes(const lffn_cross_attention *a, int64_t *bytes);
 int lffn_cross_attention_bwd(const lffn_cross_attention *a, const void *out, const void *kept, const void *g_out, void *grad_q, void *grad_k,
                              void *grad_v, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------- both ends of a vocabulary, and the norm beside them */
+
+/* Formats: those of the gather's rows, 0 float, 1 bfloat16, 2 half. */
+
+/*
+ * Rows of an embedding table by token number: out[n] = scale * weight[ids[n]], zeros where ids[n] is no row; fp32 products, one rounding.
+ * ids: [tokens], int64 where ids_64 is not 0, else int32.  weight: [rows, columns], `stride` elements from row to row; out: [tokens, columns], contiguous.  Any widths and
+ * alignments of whole numbers (those of 16 bytes are faster).  tokens < 2^31, rows < 2^31 - 1, columns <= 2^20; a launch has fewer than 2^32 threads, else LFFN_ERR_UNSUPPORTED.
+ */
+typedef struct lffn_embedding {
+    const void *ids, *weight;
+    int64_t tokens, rows, columns, stride, padding;
+    float scale;
+    int32_t format, ids_64;
+} lffn_embedding;
+int lffn_embedding_fwd(const lffn_embedding *a, void *out, void *stream);
+
+/*
+ * Its backward: grad_weight [rows, columns], contiguous, from g [tokens, columns], contiguous: row r is scale times the sum of the tokens with that number, zeros where there are
+ * none and for row `padding` (-1: none).  weight may be NULL.  Tokens are sorted by their numbers, sums are in fp32 in the sorted tokens' order, one rounding: the same bits on every call.
+ * workspace: 16-byte aligned.
+ */
+int lffn_embedding_bwd_workspace_bytes(const lffn_embedding *a, int64_t *bytes);
+int lffn_embedding_bwd(const lffn_embedding *a, const void *g, void *grad_weight, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Layer norm of rows: out = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) * weight + bias, sums in fp32, one rounding.
+ * x: [rows, columns], `stride` elements from row to row; weight, bias: [columns], fp32 where weight_f32 is not 0, else of the format, each or NULL; out: [rows, columns], contiguous.
+ * Any widths and alignments of whole numbers (those of 16 bytes are faster); rows < 2^24, columns <= 2^24.  stats: [rows, 2], every row's mean and 1 / sigma, for the backward, or NULL.
+ */
+typedef struct lffn_layer_norm_rows {
+    const void *x, *weight, *bias;
+    int64_t rows, columns, stride;
+    float eps;
+    int32_t format, weight_f32;
+} lffn_layer_norm_rows;
+int lffn_layer_norm_rows_fwd(const lffn_layer_norm_rows *a, void *out, float *stats, void *stream);
+
+/*
+ * Its backward, from stats of the forward and g [rows, columns], contiguous: grad_x [rows, columns], contiguous, grad_weight and grad_bias [columns] as weight and bias, each NULL
+ * where it is not wanted.  Sums over the rows in a fixed order: the same bits on every call.  workspace: 16-byte aligned, may be NULL without grad_weight and grad_bias.
+ */
+int lffn_layer_norm_rows_bwd_workspace_bytes(const lffn_layer_norm_rows *a, int64_t *bytes);
+int lffn_layer_norm_rows_bwd(const lffn_layer_norm_rows *a, const float *stats, const void *g, void *grad_x, void *grad_weight, void *grad_bias,
+                             void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Softmax cross entropy of a projection to a vocabulary, without the logits in memory:
+ *   l_nv = hidden[n] . weight[v] + bias[v],  loss_n = log sum_v exp l_nv - l_n,label(n)
+ * for the tokens that have a label: those whose number is not ignore_index and one of the vocabulary's.  The others take no part, whatever their rows hold.
+ * hidden: [tokens, columns], weight: [vocabulary, columns], rows of `columns` numbers that lie together (hidden_stride, weight_stride elements apart, multiples of 16 bytes,
+ * as are the addresses); columns a multiple of 8, at most 65536; vocabulary at most 2^22, tokens at most 2^24.  bias: [vocabulary] of bias_format, or NULL.
+ * labels: [tokens], int64 where labels_64 is not 0, else int32.
+ * reduction 0: loss is [tokens], zeros for the others; 1: their mean (0 of none), 2: their sum; [1].
+ * format 0: products of two half-precision terms a number, fp32 accuracy; in the backward a number of hidden or weight is held to 2^-38 of the largest of its array.
+ * 1 and 2: sums in fp32; in the backward the logits' gradients are rounded to the format.
+ * kept: what the backward needs, of lffn_linear_cross_entropy_kept_bytes, 16-byte aligned, or NULL.  workspace: 16-byte aligned.
+ */
+typedef struct lffn_linear_cross_entropy {
+    const void *hidden, *weight, *bias, *labels;
+    int64_t tokens, vocabulary, columns, hidden_stride, weight_stride, ignore_index;
+    int32_t format, bias_format, labels_64, reduction;
+} lffn_linear_cross_entropy;
+int lffn_linear_cross_entropy_kept_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes);
+int lffn_linear_cross_entropy_workspace_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes);
+int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a, float *loss, void *kept, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Its backward, tokens >= 1: from kept of the forward and the loss's gradient, [tokens] or [1], those of hidden [tokens, columns] and weight [vocabulary, columns], contiguous,
+ * 16-byte aligned, in the format, and of bias [vocabulary] in bias_format; each NULL where it is not wanted, grad_bias only beside grad_weight.  The same bits on every call.
+ */
+int lffn_linear_cross_entropy_bwd_workspace_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes);
+int lffn_linear_cross_entropy_bwd(const lffn_linear_cross_entropy *a, const void *kept, const float *g_loss, void *grad_hidden, void *grad_weight, void *grad_bias,
+                                  void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

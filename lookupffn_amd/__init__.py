@@ -11,6 +11,8 @@ from .compute_code_score import ComputeCodeScore, bin2dec, compute_code_score, c
 from .gather import (LookupGather, WeightedVectorGatherAdd, gather, indexed_inner_product, lookup_gather,
                      weighted_gather_add, weighted_vector_gather_add, weighted_vector_scatter_add)
 from .cross_attention import CrossAttentionFunction, QkNormRotary, cross_attention, qk_norm_rotary, rotary_table
+from .norm import LayerNorm, layer_norm
+from .vocabulary import Embedding, LinearCrossEntropy, embedding, linear_cross_entropy
 from .lookup import BH4, Hashing, LookupFFN
 from .encoder import Attention, CrossAttention, Encoder, EncoderLayer, Lookup, RobertaEmbeddings
 
@@ -23,4 +25,5 @@ __all__ = [
     "gather", "weighted_gather_add", "weighted_vector_gather_add", "indexed_inner_product",
     "weighted_vector_scatter_add", "WeightedVectorGatherAdd", "LookupGather", "lookup_gather",
     "cross_attention", "qk_norm_rotary", "rotary_table", "CrossAttentionFunction", "QkNormRotary",
+    "embedding", "layer_norm", "linear_cross_entropy", "Embedding", "LayerNorm", "LinearCrossEntropy",
 ]

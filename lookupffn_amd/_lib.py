@@ -16,7 +16,7 @@ _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 # LOOKUPFFN_HIP_LIB points at another build of the same ABI (e.g. a tuning build)
 LIB_PATH = os.environ.get("LOOKUPFFN_HIP_LIB") or os.path.join(_PKG_DIR, "liblookupffn_hip.so")
 
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 LFFN_OK = 0
 LFFN_ERR_BAD_ARG = -1
@@ -160,6 +160,36 @@ class CrossAttention(ctypes.Structure):
                 ("mask_stride", _i64), ("scale", _f32), ("format", _i32)]
 
 
+class LinearCrossEntropy(ctypes.Structure):
+    """struct lffn_linear_cross_entropy of include/lookupffn_hip.h."""
+    _fields_ = [("hidden", _vp), ("weight", _vp), ("bias", _vp), ("labels", _vp), ("tokens", _i64), ("vocabulary", _i64), ("columns", _i64),
+                ("hidden_stride", _i64), ("weight_stride", _i64), ("ignore_index", _i64), ("format", _i32), ("bias_format", _i32), ("labels_64", _i32),
+                ("reduction", _i32)]
+
+
+class Embedding(ctypes.Structure):
+    """struct lffn_embedding of include/lookupffn_hip.h."""
+    _fields_ = [("ids", _vp), ("weight", _vp), ("tokens", _i64), ("rows", _i64), ("columns", _i64), ("stride", _i64), ("padding", _i64), ("scale", _f32),
+                ("format", _i32), ("ids_64", _i32)]
+
+
+class LayerNormRows(ctypes.Structure):
+    """struct lffn_layer_norm_rows of include/lookupffn_hip.h."""
+    _fields_ = [("x", _vp), ("weight", _vp), ("bias", _vp), ("rows", _i64), ("columns", _i64), ("stride", _i64), ("eps", _f32), ("format", _i32),
+                ("weight_f32", _i32)]
+
+
+SIGNATURES["lffn_embedding_fwd"] = [ctypes.POINTER(Embedding), _vp, _vp]
+SIGNATURES["lffn_embedding_bwd_workspace_bytes"] = [ctypes.POINTER(Embedding), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_embedding_bwd"] = [ctypes.POINTER(Embedding), _vp, _vp, _vp, _i64, _vp]
+SIGNATURES["lffn_layer_norm_rows_fwd"] = [ctypes.POINTER(LayerNormRows), _vp, _vp, _vp]
+SIGNATURES["lffn_layer_norm_rows_bwd_workspace_bytes"] = [ctypes.POINTER(LayerNormRows), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_layer_norm_rows_bwd"] = [ctypes.POINTER(LayerNormRows), _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
+SIGNATURES["lffn_linear_cross_entropy_kept_bytes"] = [ctypes.POINTER(LinearCrossEntropy), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_linear_cross_entropy_workspace_bytes"] = [ctypes.POINTER(LinearCrossEntropy), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_linear_cross_entropy_fwd"] = [ctypes.POINTER(LinearCrossEntropy), _vp, _vp, _vp, _i64, _vp]
+SIGNATURES["lffn_linear_cross_entropy_bwd_workspace_bytes"] = [ctypes.POINTER(LinearCrossEntropy), ctypes.POINTER(_i64)]
+SIGNATURES["lffn_linear_cross_entropy_bwd"] = [ctypes.POINTER(LinearCrossEntropy), _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
 SIGNATURES["lffn_qk_norm_rotary_fwd"] = [ctypes.POINTER(QkNormRotary), _vp, _vp, _vp]
 SIGNATURES["lffn_qk_norm_rotary_bwd_workspace_bytes"] = [ctypes.POINTER(QkNormRotary), ctypes.POINTER(_i64)]
 SIGNATURES["lffn_qk_norm_rotary_bwd"] = [ctypes.POINTER(QkNormRotary), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]

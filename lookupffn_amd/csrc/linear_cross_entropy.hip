@@ -1,0 +1,880 @@
+// Softmax cross entropy of a projection to a large vocabulary, and its gradients, without the logits in memory:
+//
+//   l_nv = h_n . W_v + b_v,   lse_n = log sum_v exp l_nv,   loss_n = lse_n - l_n,label(n)
+//   d_nv = (exp(l_nv - lse_n) - [v = label(n)]) g_n,   dh_n = sum_v d_nv W_v,   dW_v = sum_n d_nv h_n,   db_v = sum_n d_nv
+//
+// Tokens without a label take no part and cost nothing: the labelled ones' rows are first laid together (`rows`), and how many there are stays on the device, so that
+// every launch behind is of a fixed size and its workgroups, one a compute unit, share out what there is.
+//
+// Forward: tiles of 256 vocabulary entries x 256 tokens (product_tiles.h); a tile's logits become, in its registers, each token's largest and sum of exponentials, 8
+// bytes for 256 logits, and a second launch joins those of a token.
+// Backward: the logits of a piece of the vocabulary are formed once more, d is written in 16 bits (a float's in two terms), and one launch forms from it both gradients' products:
+// dW whole, its sum over the tokens, and dh in shares of the vocabulary, added up in fp32 in memory.  What a share adds to is its own: no atomics on results, the same bits
+// on every call.
+#include "product_tiles.h"
+
+namespace {
+
+using namespace product_tiles;
+
+constexpr int TILE = 256;                       // tokens and vocabulary entries of a tile
+constexpr int THREADS = 512, WAVES_M = 2, WAVES_N = 4, MB = TILE / WAVES_M / 32, NB = TILE / WAVES_N / 32;
+constexpr int COMPUTE_UNITS = 256, XCDS = 8;
+constexpr int CHUNK = 64;                       // tokens a workgroup lays together
+constexpr int COUNTED_FROM = 4096;              // tokens from which on a launch of its own counts the labelled ones of every chunk
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LIFT = 16384.f;                 // d times 2^14: half's normal numbers then reach down to 2^-28 of a row's largest
+constexpr int64_t D_BYTES = int64_t(512) << 20; // of a piece's d, at most (few, large pieces: with many tokens 2048 entries at least)
+constexpr int64_t PARTS_BYTES = int64_t(256) << 20;
+constexpr int SHARES = 64;                      // of the vocabulary, for dh, at most
+
+__host__ __device__ constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// What the backward needs beside the inputs, and what the forward's launches share.
+struct Kept {
+    int32_t *head;      // [4]: labelled tokens; the exponents of the largest of their rows and of the weights (two-term numbers)
+    int32_t *pos;       // [N]: where a token's row is among the labelled ones, or -1
+    int32_t *label;     // [labelled]
+    float2 *level;      // [labelled]: a token's largest logit, and one over the sum of the exponentials of what they are below it
+};
+int64_t kept_bytes(int64_t N) { return 16 + up(N * 4, 16) * 4; }
+Kept kept_at(void *at, int64_t N) {
+    char *p = static_cast<char *>(at);
+    const int64_t n = up(N * 4, 16);
+    return {reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + 16), reinterpret_cast<int32_t *>(p + 16 + n), reinterpret_cast<float2 *>(p + 16 + 2 * n)};
+}
+
+struct Sizes {
+    int N, V, K;               // tokens, vocabulary, columns
+    int64_t Kp, Vp;            // columns of laid-together rows, entries of padded arrays
+};
+
+struct Operands {
+    Sizes s;
+    Kept kept;
+    Source weight;             // as the products read it
+    char *rows;                // [Np, Kp] the labelled tokens' rows
+    int64_t rows_plane;
+    float *bias;               // [Vp] fp32, -infinity behind the vocabulary
+    float *weight_scale;       // two-term numbers: [Vp], [Np], by which sums are multiplied
+    float *row_scale;
+};
+
+__device__ __forceinline__ Source rows_of(const Operands &o, int labelled) {
+    return {o.rows, o.s.Kp * 2, o.rows_plane, (int)up(labelled, TILE), (int)o.s.Kp};
+}
+
+// ---------------------------------------------------------------- the labelled tokens
+
+struct RowsArgs {
+    Operands o;
+    const void *hidden, *labels, *bias;
+    int64_t hidden_stride, ignore;
+    int32_t labels_64, bias_format;            // of the gather's row formats; -1: none
+    const int32_t *counts;                     // labelled tokens of every chunk, or null
+    int32_t *token;                            // [labelled]
+    float *loss;                               // [N]: zeros for the others, or null
+    int32_t *queues;                           // counters to clear, or null
+    int num_queues;
+};
+
+__device__ __forceinline__ int label_of(const void *labels, int wide, int64_t i, int64_t ignore, int V) {
+    const int64_t y = wide ? static_cast<const int64_t *>(labels)[i] : static_cast<const int32_t *>(labels)[i];
+    return y == ignore || y < 0 || y >= V ? -1 : (int)y;
+}
+
+__global__ __launch_bounds__(256) void count_kernel(const void *labels, int wide, int64_t ignore, int V, int N, int32_t *counts) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const uint64_t live = __ballot(i < N && label_of(labels, wide, i, ignore, V) >= 0);
+    if (threadIdx.x % 64 == 0 && i < N) counts[i / CHUNK] = __popcll(live);
+}
+
+__device__ __forceinline__ float wave_most(float v) {
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) v = fmaxf(v, __shfl_xor(v, m));
+    return v;
+}
+
+// A row of `columns` numbers as the products read it, zeros up to `padded`, by one wavefront.  Two-term numbers: scaled by the row's largest, or to `exponent` where that is
+// given; -> the exponent of the way back.
+template <typename R, int PLANES>
+__device__ __forceinline__ int lay_row(const char *from, char *to, int64_t plane, int columns, int64_t padded, const int *exponent) {
+    const int lane = threadIdx.x % 64;
+    if constexpr (PLANES == 1) {
+        for (int c = lane * 8; c < padded; c += 512)
+            *reinterpret_cast<uint4 *>(to + c * 2) = c < columns ? *reinterpret_cast<const uint4 *>(from + c * 2) : make_uint4(0, 0, 0, 0);
+        return 0;
+    } else {
+        int e;
+        float scale;
+        if (exponent) {
+            e = *exponent;
+            scale = __builtin_amdgcn_ldexpf(1.f, -e);
+        } else {
+            float most = 0.f;
+            for (int c = lane * 4; c < columns; c += 256) {
+                const float4 v = *reinterpret_cast<const float4 *>(from + c * 4);
+                most = fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+            }
+            scale = scale_to(wave_most(most), 13, e);
+        }
+        for (int c = lane * 8; c < padded; c += 512) {
+            uint32_t h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
+            if (c < columns) {
+                const float4 a = *reinterpret_cast<const float4 *>(from + c * 4), b = *reinterpret_cast<const float4 *>(from + c * 4 + 16);
+                const float v[8] = {a.x * scale, a.y * scale, a.z * scale, a.w * scale, b.x * scale, b.y * scale, b.z * scale, b.w * scale};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    h[i] = split_hi(v[2 * i], v[2 * i + 1], 1.f);
+                    l[i] = split_rest(v[2 * i], v[2 * i + 1], h[i]);
+                }
+            }
+            *reinterpret_cast<uint4 *>(to + c * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(to + plane + c * 2) = make_uint4(l[0], l[1], l[2], l[3]);
+        }
+        return e;
+    }
+}
+
+__device__ __forceinline__ float bias_of(const void *bias, int format, int v) {
+    if (format == LFFN_ROWS_F32) return static_cast<const float *>(bias)[v];
+    if (format == LFFN_ROWS_BF16) return (float)static_cast<const __bf16 *>(bias)[v];
+    return (float)static_cast<const _Float16 *>(bias)[v];
+}
+
+// Workgroups 0 .. tokens / CHUNK - 1: the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
+// one fills the last tile's rows up with zeros.  The workgroups behind: the bias in fp32.
+template <typename R, int PLANES, bool BACKWARD>
+__global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
+    const Sizes &s = a.o.s;
+    const Kept &k = a.o.kept;
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, chunks = (s.N + CHUNK - 1) / CHUNK;
+    if ((int)blockIdx.x >= chunks) {
+        const int v = ((int)blockIdx.x - chunks) * 256 + tid;
+        if (v < s.Vp) a.o.bias[v] = v >= s.V ? -INFINITY : a.bias_format < 0 ? 0.f : bias_of(a.bias, a.bias_format, v);
+        if (BACKWARD && v < a.num_queues) a.queues[v] = 0;
+        return;
+    }
+    __shared__ int place[CHUNK], before[4];
+    const int t0 = blockIdx.x * CHUNK;
+    int labelled = 0;              // up to and with this chunk
+    if constexpr (!BACKWARD) {
+        int n = 0;
+        if (a.counts)
+            for (int i = tid; i < (int)blockIdx.x; i += 256) n += a.counts[i];
+        else
+            for (int i = tid; i < t0; i += 256) n += label_of(a.labels, a.labels_64, i, a.ignore, s.V) >= 0;
+#pragma unroll
+        for (int m = 32; m > 0; m /= 2) n += __shfl_xor(n, m);
+        if (lane == 0) before[wave] = n;
+        __syncthreads();
+        const int first = before[0] + before[1] + before[2] + before[3], t = t0 + lane;
+        const int y = t < s.N ? label_of(a.labels, a.labels_64, t, a.ignore, s.V) : -1;
+        const uint64_t live = __ballot(y >= 0);
+        labelled = first + __popcll(live);
+        if (wave == 0) {
+            const int at = y >= 0 ? first + __popcll(live & ((uint64_t(1) << lane) - 1)) : -1;
+            place[lane] = at;
+            if (t < s.N) {
+                k.pos[t] = at;
+                if (y >= 0) k.label[at] = y, a.token[at] = t;
+                else if (a.loss) a.loss[t] = 0.f;
+            }
+            if ((int)blockIdx.x == chunks - 1 && lane == 0) k.head[0] = labelled;
+        }
+    } else {
+        labelled = k.head[0];
+        if (wave == 0) place[lane] = t0 + lane < s.N ? k.pos[t0 + lane] : -1;
+    }
+    __syncthreads();
+    const int64_t row_bytes = s.Kp * 2;
+    for (int i = wave; i < CHUNK; i += 4) {
+        const int at = place[i];
+        if (at < 0) continue;
+        const char *from = static_cast<const char *>(a.hidden) + (int64_t(t0) + i) * a.hidden_stride * R::BYTES;
+        const int e = lay_row<R, PLANES>(from, a.o.rows + at * row_bytes, a.o.rows_plane, s.K, s.Kp, BACKWARD ? k.head + 1 : nullptr);
+        if (PLANES == 2 && !BACKWARD && lane == 0) {
+            a.o.row_scale[at] = __builtin_amdgcn_ldexpf(1.f, e);
+            atomicMax(k.head + 1, e);
+        }
+    }
+    if ((int)blockIdx.x == chunks - 1) {
+        const int64_t from = labelled * row_bytes / 16, to = up(labelled, TILE) * row_bytes / 16;
+        for (int64_t i = from + tid; i < to; i += 256)
+            for (int p = 0; p < PLANES; ++p) *reinterpret_cast<uint4 *>(a.o.rows + p * a.o.rows_plane + i * 16) = make_uint4(0, 0, 0, 0);
+        if (PLANES == 2 && !BACKWARD)
+            for (int i = labelled + tid; i < up(labelled, TILE); i += 256) a.o.row_scale[i] = 1.f;
+    }
+}
+
+__global__ void head_kernel(int32_t *head) {
+    if (threadIdx.x < 4) head[threadIdx.x] = threadIdx.x == 0 ? 0 : -1000;
+}
+
+// fp32 weights in two half-precision terms: each row by its largest, or, in the backward, all by the array's.
+template <bool BACKWARD>
+__global__ __launch_bounds__(256) void weight_kernel(Operands o, const float *w, int64_t stride) {
+    const int v = blockIdx.x * 4 + threadIdx.x / 64;
+    if (v >= o.s.Vp) return;
+    int e = 0;
+    if (v < o.s.V)
+        e = lay_row<F32Row, 2>(reinterpret_cast<const char *>(w + v * stride), const_cast<char *>(o.weight.at) + v * o.weight.stride, o.weight.plane, o.s.K, o.s.K,
+                               BACKWARD ? o.kept.head + 2 : nullptr);
+    if (threadIdx.x % 64 == 0) {
+        o.weight_scale[v] = __builtin_amdgcn_ldexpf(1.f, e);
+        if (!BACKWARD && v < o.s.V) atomicMax(o.kept.head + 2, e);
+    }
+}
+
+// ---------------------------------------------------------------- logits
+
+// A workgroup's tiles of vt x nt: those of an XCD follow each other, eight tiles of the vocabulary at a time against one tile of tokens after the other, so that the compute
+// units of an XCD read the same ones.
+template <typename Each>
+__device__ __forceinline__ void for_tiles(int vt, int nt, Each &&each) {
+    const int xcd = blockIdx.x % XCDS, slots = gridDim.x / XCDS, total = vt * nt, share = (total + XCDS - 1) / XCDS;
+    for (int i = blockIdx.x / XCDS; i < share; i += slots) {
+        const int id = xcd * share + i;
+        if (id >= total) return;
+        const int group = id / (8 * nt), in = id - group * 8 * nt, height = min(8, vt - group * 8);
+        each(group * 8 + in % height, in / height);
+    }
+}
+
+struct Tiled {
+    static constexpr uint32_t LDS = 2 * (TILE + TILE) * 128;
+};
+
+// A tile's products: entries from v0, tokens from n0.
+template <typename F>
+__device__ __forceinline__ void logits(Sums<MB, NB> &sums, const Operands &o, int labelled, int v0, int n0, uint32_t lds) {
+    typedef Along<TILE, THREADS, F::PLANES> Side;
+    const int wave = threadIdx.x / 64;
+    const Side a(o.weight, v0), b(rows_of(o, labelled), n0);
+    const typename Side::Reader ra(wave / WAVES_N * MB * 32), rb(wave % WAVES_N * NB * 32);
+    sums.clear();
+    multiply<F>(sums, a, b, ra, rb, lds, 0, (o.s.K + Side::K - 1) / Side::K, [](int, const uint4 &) {});
+}
+
+// The logits of the tile's 16 entries of block i for the token of block j: l[e] of entry mfma_row(e, half)
+template <typename F>
+__device__ __forceinline__ void with_bias(float (&l)[16], const f32x16_t &sum, const Operands &o, int v, float row_scale) {
+    const int half = threadIdx.x % 64 / 32;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const float4 b = *reinterpret_cast<const float4 *>(o.bias + v + 8 * g + 4 * half);
+        if constexpr (F::PLANES == 1) {
+            l[4 * g] = sum[4 * g] + b.x, l[4 * g + 1] = sum[4 * g + 1] + b.y, l[4 * g + 2] = sum[4 * g + 2] + b.z, l[4 * g + 3] = sum[4 * g + 3] + b.w;
+        } else {
+            const float4 w = *reinterpret_cast<const float4 *>(o.weight_scale + v + 8 * g + 4 * half);
+            l[4 * g] = fmaf(sum[4 * g] * w.x, row_scale, b.x), l[4 * g + 1] = fmaf(sum[4 * g + 1] * w.y, row_scale, b.y);
+            l[4 * g + 2] = fmaf(sum[4 * g + 2] * w.z, row_scale, b.z), l[4 * g + 3] = fmaf(sum[4 * g + 3] * w.w, row_scale, b.w);
+        }
+    }
+}
+
+struct ForwardArgs {
+    Operands o;
+    float2 *parts;         // [tiles of the vocabulary, Np]: largest, sum of exponentials of what they are below it
+    float *at_label;       // [labelled]
+    int64_t Np;
+};
+
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.f : m;
+    return make_float2(m, a.y * __builtin_amdgcn_exp2f((a.x - from) * LOG2E) + b.y * __builtin_amdgcn_exp2f((b.x - from) * LOG2E));
+}
+
+template <typename F>
+__global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
+    const uint32_t lds = lds_byte_of(lds_words);
+    float2 *const halves = reinterpret_cast<float2 *>(reinterpret_cast<char *>(lds_words) + Tiled::LDS);     // [WAVES_M][TILE]
+    const Operands &o = a.o;
+    const int labelled = o.kept.head[0], tid = threadIdx.x, wave = tid / 64, lane = tid % 64, half = lane / 32;
+    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+    for_tiles((o.s.V + TILE - 1) / TILE, (labelled + TILE - 1) / TILE, [&](int vt, int nt) {
+        Sums<MB, NB> sums;
+        logits<F>(sums, o, labelled, vt * TILE, nt * TILE, lds);
+        const int v0 = vt * TILE + wm * MB * 32;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int column = wn * NB * 32 + j * 32 + lane % 32, n = nt * TILE + column;
+            const float row_scale = F::PLANES == 2 ? o.row_scale[n] : 1.f;
+            const int at = n < labelled ? o.kept.label[n] - v0 : -1;
+            float2 of = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                float l[16];
+                with_bias<F>(l, sums.v[i][j], o, v0 + 32 * i, row_scale);
+                float most = of.x;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) most = fmaxf(most, l[e]);
+                const float from = most == -INFINITY ? 0.f : most;
+                float sum = of.y * __builtin_amdgcn_exp2f((of.x - from) * LOG2E);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f((l[e] - from) * LOG2E);
+                of = make_float2(most, sum);
+                const int r = at - 32 * i;
+                if (r >= 0 && r < 32 && r / 4 % 2 == half) {
+                    float found = l[0];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) found = mfma_row(e, half) == r ? l[e] : found;
+                    a.at_label[n] = found;
+                }
+            }
+            const float2 other = make_float2(__shfl_xor(of.x, 32), __shfl_xor(of.y, 32));
+            if (half == 0) halves[wm * TILE + column] = joined(of, other);
+        }
+        __syncthreads();
+        if (tid < TILE) a.parts[vt * a.Np + nt * TILE + tid] = joined(halves[tid], halves[TILE + tid]);
+        // (the next tile's products have barriers before halves is written again)
+    });
+}
+
+struct JoinArgs {
+    Kept kept;
+    const float2 *parts;
+    const float *at_label;
+    const int32_t *token;
+    int64_t Np;
+    int tiles;
+    float *loss;           // by token
+    float *losses;         // by place
+};
+
+// A token's parts: 16 threads.
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
+    __shared__ float2 shares[16][17];
+    const int labelled = a.kept.head[0], in = threadIdx.x % 16, slice = threadIdx.x / 16, n = blockIdx.x * 16 + in;
+    if ((int)blockIdx.x * 16 >= labelled) return;
+    float2 of = make_float2(-INFINITY, 0.f);
+#pragma unroll 4
+    for (int t = slice; t < a.tiles; t += 16) of = joined(of, a.parts[t * a.Np + n]);
+    shares[slice][in] = of;
+    __syncthreads();
+    if (slice == 0 && n < labelled) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) of = joined(of, shares[i][in]);
+        const float loss = (of.x - a.at_label[n]) + __logf(of.y);
+        a.kept.level[n] = make_float2(of.x, 1.f / of.y);
+        if (a.loss) a.loss[a.token[n]] = loss;
+        else a.losses[n] = loss;
+    }
+}
+
+// The tokens' sum, or mean (0 of none), in 64 bits.
+__global__ __launch_bounds__(1024) void sum_kernel(const int32_t *head, const float *losses, float *loss, int mean) {
+    __shared__ double sums[16];
+    const int labelled = head[0];
+    double sum = 0;
+    for (int i = threadIdx.x; i < labelled; i += 1024) sum += losses[i];
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) sum += __shfl_xor(sum, m);
+    if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) sum += sums[i];
+        *loss = (float)(mean ? sum / (labelled > 0 ? labelled : 1) : sum);
+    }
+}
+
+// ---------------------------------------------------------------- gradients
+
+struct BackwardArgs {
+    Operands o;
+    char *d;                   // [Np, ld] (two planes): a piece's
+    int64_t d_bytes, d_plane;  // how large it may be; the second plane's distance
+    float *parts;              // [shares, labelled, K]
+    int64_t parts_bytes;
+    const float *g_loss;       // [1] or [N]
+    float *coefficient;        // [labelled] or null: what d is multiplied with beside `factor`
+    float *power;              // [1]: of both gradients, where there are coefficients
+    int32_t *queues;
+    void *grad_hidden, *grad_weight, *grad_bias;
+    int32_t bias_format, reduction, pieces;
+};
+
+// How a piece is laid out, from the number of labelled tokens, alike in every launch.
+struct Piece {
+    int v0, width, ld, nt;     // entries, numbers of d's rows, tiles of tokens
+    int shares, share;         // of the piece's entries, for dh: steps each
+};
+template <typename F>
+__device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, int piece) {
+    constexpr int K = STEP / F::PLANES;
+    Piece p;
+    p.nt = (labelled + TILE - 1) / TILE;
+    const int64_t rows = max(p.nt, 1) * int64_t(TILE);
+    p.ld = (int)min(a.o.s.Vp, max(int64_t(TILE), a.d_bytes / (rows * 2 * F::PLANES) / TILE * TILE));
+    const int64_t first = int64_t(piece) * p.ld;
+    p.v0 = (int)min(first, int64_t(a.o.s.V));
+    p.width = min(p.ld, a.o.s.V - p.v0);
+    // a share's sum is about as long as one over the tokens, so that tasks are alike; all pieces have as many
+    const int steps = p.ld / K, most = (int)min(int64_t(SHARES), a.parts_bytes / (max(labelled, 1) * int64_t(a.o.s.K) * 4));
+    p.shares = max(1, min(most, steps / max(16, (labelled + K - 1) / K)));
+    p.share = (steps + p.shares - 1) / p.shares;
+    return p;
+}
+
+// What both gradients' sums are multiplied with: of a sum or mean what all tokens' d are, else the power of two that their coefficients were divided by.
+__device__ __forceinline__ float factor_of(const BackwardArgs &a, int labelled) {
+    if (a.reduction == 0) return *a.power;
+    return *a.g_loss / (a.reduction == 1 ? (float)max(labelled, 1) : 1.f) * (1.f / LIFT);
+}
+
+// Tokens' own gradients by the power of two of their largest.
+__global__ __launch_bounds__(1024) void coefficient_kernel(BackwardArgs a) {
+    __shared__ float most[16];
+    const int tid = threadIdx.x;
+    float v = 0.f;
+    for (int i = tid; i < a.o.s.N; i += 1024)
+        if (a.o.kept.pos[i] >= 0) v = fmaxf(v, fabsf(a.g_loss[i]));
+    v = wave_most(v);
+    if (tid % 64 == 0) most[tid / 64] = v;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) v = fmaxf(v, most[i]);
+    int e;
+    const float scale = scale_to(v, 0, e);
+    for (int i = tid; i < a.o.s.N; i += 1024)
+        if (a.o.kept.pos[i] >= 0) a.coefficient[a.o.kept.pos[i]] = a.g_loss[i] * scale;
+    if (tid == 0) *a.power = __builtin_amdgcn_ldexpf(1.f / LIFT, e);
+}
+
+template <typename F>
+__global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece) {
+    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
+    const uint32_t lds = lds_byte_of(lds_words);
+    const Operands &o = a.o;
+    const int labelled = o.kept.head[0], wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N;
+    const Piece p = piece_of<F>(a, labelled, piece);
+    const float scale = F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : 1.f;
+    for_tiles((p.width + TILE - 1) / TILE, p.nt, [&](int vt, int nt) {
+        Sums<MB, NB> sums;
+        logits<F>(sums, o, labelled, p.v0 + vt * TILE, nt * TILE, lds);
+        const int in = vt * TILE + wm * MB * 32, v0 = p.v0 + in;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int n = nt * TILE + wn * NB * 32 + j * 32 + lane % 32;
+            const bool live = n < labelled;
+            const float2 level = live ? o.kept.level[n] : make_float2(0.f, 0.f);
+            const float by = live ? LIFT * (a.coefficient ? a.coefficient[n] : 1.f) : 0.f;
+            const int at = live ? o.kept.label[n] - v0 : -1;
+            char *const row = a.d + (int64_t(n) * p.ld + in) * 2;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                float l[16];
+                with_bias<F>(l, sums.v[i][j], o, v0 + 32 * i, scale);
+                const int r = at - 32 * i;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float q = __builtin_amdgcn_exp2f((l[e] - level.x) * LOG2E);
+                    l[e] = live ? fmaf(q, level.y, mfma_row(e, half) == r ? -1.f : 0.f) * by : 0.f;
+                }
+                auto put = [&](char *to) {
+#pragma unroll
+                    for (int g = 0; g < 4; g += 2) {
+                        // the lanes of a row exchange four numbers of two groups, so that each has eight that lie together
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const auto s = __builtin_amdgcn_permlane32_swap(F::pack2(l[4 * g + 2 * e], l[4 * g + 2 * e + 1]),
+                                                                            F::pack2(l[4 * g + 4 + 2 * e], l[4 * g + 5 + 2 * e]), false, false);
+                            w[e] = s[0], w[2 + e] = s[1];
+                        }
+                        *reinterpret_cast<uint4 *>(to + (32 * i + 8 * (g + half)) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                };
+                put(row);
+                if constexpr (F::PLANES == 2) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) l[e] -= (float)(_Float16)l[e];
+                    put(row + a.d_plane);
+                }
+            }
+        }
+    });
+}
+
+__device__ __forceinline__ float dot_ones(BF16, uint4 u, float sum) {
+    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+    const pair_t one = {(__bf16)1.f, (__bf16)1.f};
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, w[i]), one, sum, false);
+    return sum;
+}
+__device__ __forceinline__ float dot_ones(F16, uint4 u, float sum) {
+    typedef _Float16 pair_t __attribute__((ext_vector_type(2)));
+    const pair_t one = {(_Float16)1.f, (_Float16)1.f};
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(pair_t, w[i]), one, sum, false);
+    return sum;
+}
+
+// Eight numbers in the results' format.
+template <typename R>
+__device__ __forceinline__ void store8(char *to, const float (&v)[8]) {
+    if constexpr (R::BYTES == 4) {
+        *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4 *>(to + 16) = make_float4(v[4], v[5], v[6], v[7]);
+    } else
+        *reinterpret_cast<uint4 *>(to) = R::pack(v);
+}
+
+// A share of dh: tokens from n0 x columns from h0, the sum over steps first .. end - 1 of the piece's entries.
+template <typename F>
+__device__ __forceinline__ void hidden_task(const BackwardArgs &a, const Piece &p, int labelled, int piece, int share, int n0, int h0, uint32_t lds) {
+    typedef Along<TILE, THREADS, F::PLANES> Left;
+    typedef Across<TILE, THREADS, F::PLANES> Right;
+    const Operands &o = a.o;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32;
+    const Left left({a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld}, n0);
+    Source w = o.weight;
+    w.at += p.v0 * w.stride;
+    w.rows = p.width;
+    const Right right(w, h0);
+    const typename Left::Reader ra(wave / WAVES_N * MB * 32);
+    const typename Right::Reader rb(wave % WAVES_N * NB * 32);
+    Sums<MB, NB> sums;
+    sums.clear();
+    const int first = share * p.share, steps = (p.width + Left::K - 1) / Left::K;
+    multiply<F>(sums, left, right, ra, rb, lds, first, min(steps, first + p.share), [](int, const uint4 &) {});
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int h = h0 + (wave % WAVES_N * NB + j) * 32 + lane % 32;
+        if (h >= o.s.K) continue;
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int n = n0 + (wave / WAVES_N * MB + i) * 32;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int row = n + mfma_row(e, half);
+                float *const at = a.parts + (int64_t(share) * labelled + row) * o.s.K + h;
+                if (row < labelled) *at = piece ? *at + sums.v[i][j][e] : sums.v[i][j][e];
+            }
+        }
+    }
+}
+
+// dW's entries from v0 (of the piece) x columns from h0, and, with the first columns, db's.
+template <typename F, typename R>
+__device__ __forceinline__ void weight_task(const BackwardArgs &a, const Piece &p, int labelled, int v0, int h0, uint32_t lds) {
+    typedef Across<TILE, THREADS, F::PLANES> Side;
+    const Operands &o = a.o;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N;
+    Source rows = rows_of(o, labelled);
+    const Side left(rows, h0), right({a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld}, v0);
+    const typename Side::Reader ra(wm * MB * 32), rb(wn * NB * 32);
+    Sums<MB, NB> sums;
+    sums.clear();
+    float bias[NB] = {};
+    const bool of_bias = h0 == 0 && wm == 0 && a.grad_bias;
+    multiply<F>(sums, left, right, ra, rb, lds, 0, (labelled + Side::K - 1) / Side::K, [&](int j, const uint4 &u) {
+        if (of_bias) bias[j] = dot_ones(F(), u, bias[j]);
+    });
+    const float factor = factor_of(a, labelled), by = F::PLANES == 2 ? factor * __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : factor;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int in = v0 + (wn * NB + j) * 32 + lane % 32, v = p.v0 + in;
+        const bool live = in < p.width;
+        if (of_bias) {
+            const float sum = (bias[j] + __shfl_xor(bias[j], 32)) * factor;
+            if (half == 0 && live) {
+                if (a.bias_format == LFFN_ROWS_F32) static_cast<float *>(a.grad_bias)[v] = sum;
+                else if (a.bias_format == LFFN_ROWS_BF16) static_cast<__bf16 *>(a.grad_bias)[v] = (__bf16)sum;
+                else static_cast<_Float16 *>(a.grad_bias)[v] = (_Float16)sum;
+            }
+        }
+        char *const row = static_cast<char *>(a.grad_weight) + int64_t(v) * o.s.K * R::BYTES;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; g += 2) {
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(sums.v[i][j][4 * g + e] * by), __float_as_uint(sums.v[i][j][4 * g + 4 + e] * by),
+                                                                    false, false);
+                    t[e] = __uint_as_float(s[0]), t[4 + e] = __uint_as_float(s[1]);
+                }
+                const int h = h0 + (wm * MB + i) * 32 + 8 * (g + half);
+                if (live && h < o.s.K) store8<R>(row + h * R::BYTES, t);
+            }
+    }
+}
+
+// Both gradients of a piece: a queue of tasks, the shares of dh first.
+template <typename F, typename R>
+__global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, int piece) {
+    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
+    __shared__ int next;
+    const uint32_t lds = lds_byte_of(lds_words);
+    const int labelled = a.o.kept.head[0];
+    const Piece p = piece_of<F>(a, labelled, piece);
+    if (p.width <= 0) return;
+    const int ht = (a.o.s.K + TILE - 1) / TILE, vt = (p.width + TILE - 1) / TILE;
+    const int hidden = a.grad_hidden ? p.shares * p.nt * ht : 0, total = hidden + (a.grad_weight ? vt * ht : 0);
+    for (;;) {
+        if (threadIdx.x == 0) next = atomicAdd(a.queues + piece, 1);
+        __syncthreads();
+        const int task = __builtin_amdgcn_readfirstlane(next);
+        __syncthreads();
+        if (task >= total) return;
+        if (task < hidden) {
+            const int h = task % ht, n = task / ht % p.nt, share = task / ht / p.nt;
+            hidden_task<F>(a, p, labelled, piece, share, n * TILE, h * TILE, lds);
+        } else {
+            const int t = task - hidden;
+            weight_task<F, R>(a, p, labelled, t / ht * TILE, t % ht * TILE, lds);
+        }
+    }
+}
+
+// dh: a labelled token's shares added up, zeros for the others.
+template <typename F, typename R>
+__global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
+    const Sizes &s = a.o.s;
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, pieces = s.K / 8, t = i / pieces, c = i % pieces * 8;
+    if (t >= s.N) return;
+    const int at = a.o.kept.pos[t], labelled = a.o.kept.head[0];
+    float v[8] = {};
+    if (at >= 0) {
+        const int shares = piece_of<F>(a, labelled, 0).shares;
+        for (int p = 0; p < shares; ++p) {
+            const float *from = a.parts + (int64_t(p) * labelled + at) * s.K + c;
+            const float4 x = *reinterpret_cast<const float4 *>(from), y = *reinterpret_cast<const float4 *>(from + 4);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+        }
+        const float by = factor_of(a, labelled) * (F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, a.o.kept.head[2]) : 1.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= by;
+    }
+    store8<R>(static_cast<char *>(a.grad_hidden) + (t * s.K + c) * R::BYTES, v);
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- C entries
+
+namespace {
+
+int planes_of(const lffn_linear_cross_entropy &a) { return a.format == LFFN_ROWS_F32 ? 2 : 1; }
+
+int check(const lffn_linear_cross_entropy *a) {
+    LFFN_REQUIRE(a, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->format >= 0 && a->format <= 2 && a->bias_format >= 0 && a->bias_format <= 2 && a->reduction >= 0 && a->reduction <= 2, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->tokens >= 0 && a->vocabulary >= 1 && a->columns >= 8, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->columns % 8 == 0 && a->columns <= 65536 && a->tokens <= (1 << 24) && a->vocabulary <= (1 << 22), LFFN_ERR_UNSUPPORTED);
+    const int64_t size = a->format == LFFN_ROWS_F32 ? 4 : 2, most = int64_t(1) << 22;
+    LFFN_REQUIRE(a->weight && lffn_aligned16(a->weight) && a->weight_stride >= a->columns && a->weight_stride * size % 16 == 0, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->tokens == 0 || (a->hidden && a->labels), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(lffn_aligned16(a->hidden) && a->hidden_stride >= 0 && a->hidden_stride * size % 16 == 0, LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(a->weight_stride <= most, LFFN_ERR_UNSUPPORTED);
+    return LFFN_OK;
+}
+
+// Takes pieces of a workspace one after the other; with base null it only counts.
+struct Carver {
+    char *base;
+    int64_t used = 0;
+    template <typename T>
+    T *take(int64_t n) {
+        T *const p = base ? reinterpret_cast<T *>(base + used) : nullptr;
+        used += up(n * (int64_t)sizeof(T), 256);
+        return p;
+    }
+};
+
+Operands operands(const lffn_linear_cross_entropy &a, Carver &c) {
+    Operands o{};
+    const int64_t Np = up(a.tokens, TILE);
+    o.s = {(int)a.tokens, (int)a.vocabulary, (int)a.columns, up(a.columns, STEP), up(a.vocabulary, TILE)};
+    const int planes = planes_of(a);
+    o.rows_plane = Np * o.s.Kp * 2;
+    o.rows = c.take<char>(o.rows_plane * planes);
+    o.bias = c.take<float>(o.s.Vp);
+    o.weight = {static_cast<const char *>(a.weight), a.weight_stride * 2, 0, o.s.V, o.s.K};
+    if (planes == 2) {
+        o.weight_scale = c.take<float>(o.s.Vp);
+        o.row_scale = c.take<float>(Np);
+        const int64_t plane = a.vocabulary * a.columns * 2;
+        o.weight = {c.take<char>(plane * 2), a.columns * 2, plane, o.s.V, o.s.K};
+    }
+    return o;
+}
+
+struct Forward {
+    ForwardArgs f;
+    RowsArgs r;
+    JoinArgs j;
+    void *kept;
+    int32_t *counts;
+};
+int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Forward &f) {
+    Carver c{base};
+    const int64_t Np = up(a.tokens, TILE);
+    f = {};
+    f.f.o = operands(a, c);
+    f.f.Np = f.j.Np = Np;
+    f.j.tiles = int((a.vocabulary + TILE - 1) / TILE);
+    f.j.parts = f.f.parts = c.take<float2>(f.j.tiles * Np);
+    f.j.at_label = f.f.at_label = c.take<float>(Np);
+    f.j.losses = c.take<float>(Np);
+    f.j.token = f.r.token = c.take<int32_t>(Np);
+    f.counts = c.take<int32_t>(a.tokens / CHUNK + 1);
+    f.kept = with_kept ? c.take<char>(kept_bytes(a.tokens)) : nullptr;
+    return c.used;
+}
+
+struct Backward {
+    BackwardArgs b;
+    RowsArgs r;
+};
+int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
+    Carver c{base};
+    w = {};
+    const int64_t Np = up(a.tokens, TILE), planes = planes_of(a), K = a.columns;
+    BackwardArgs &b = w.b;
+    b.o = operands(a, c);
+    const int64_t Vp = b.o.s.Vp, least = Np * (Vp < 2048 ? Vp : 2048) * 2 * planes, whole = Np * Vp * 2 * planes;
+    b.d_bytes = least > D_BYTES ? least : whole < D_BYTES ? whole : D_BYTES;
+    b.d_plane = b.d_bytes / 2;
+    b.d = c.take<char>(b.d_bytes);
+    const int64_t one = a.tokens * K * 4;
+    b.parts_bytes = one > PARTS_BYTES ? one : one * SHARES < PARTS_BYTES ? one * SHARES : PARTS_BYTES;
+    b.parts = c.take<float>(b.parts_bytes / 4);
+    b.coefficient = c.take<float>(a.reduction == 0 ? Np : 0);
+    b.power = c.take<float>(1);
+    if (a.reduction != 0) b.coefficient = nullptr;
+    // as many launches as pieces if all tokens are labelled; with fewer the last ones find nothing
+    const int64_t ld = b.d_bytes / (Np > 0 ? Np * 2 * planes : 1) / TILE * TILE;
+    b.pieces = a.tokens == 0 ? 0 : int((a.vocabulary + ld - 1) / ld);
+    b.queues = c.take<int32_t>(b.pieces);
+    return c.used;
+}
+
+void fill(RowsArgs &r, const lffn_linear_cross_entropy &a, const Operands &o) {
+    r.o = o;
+    r.hidden = a.hidden, r.labels = a.labels, r.bias = a.bias;
+    r.hidden_stride = a.hidden_stride, r.ignore = a.ignore_index;
+    r.labels_64 = a.labels_64, r.bias_format = a.bias ? a.bias_format : -1;
+}
+
+template <bool BACKWARD>
+void launch_rows(const lffn_linear_cross_entropy &a, const RowsArgs &r, hipStream_t st) {
+    const int64_t flat = r.num_queues > r.o.s.Vp ? r.num_queues : r.o.s.Vp;
+    const dim3 grid(unsigned((a.tokens + CHUNK - 1) / CHUNK + (flat + 255) / 256));
+    if (a.format == LFFN_ROWS_F32) {
+        weight_kernel<BACKWARD><<<dim3(unsigned(r.o.s.Vp / 4)), dim3(256), 0, st>>>(r.o, static_cast<const float *>(a.weight), a.weight_stride);
+        rows_kernel<F32Row, 2, BACKWARD><<<grid, dim3(256), 0, st>>>(r);
+    } else
+        rows_kernel<F16Row, 1, BACKWARD><<<grid, dim3(256), 0, st>>>(r);
+}
+
+unsigned workgroups(int64_t tiles) { return unsigned(tiles >= COMPUTE_UNITS ? COMPUTE_UNITS : up(tiles, XCDS)); }
+
+constexpr size_t LDS_BYTES = Tiled::LDS + WAVES_M * TILE * sizeof(float2);
+
+template <typename F>
+int forward(const Forward &f, hipStream_t st) {
+    static LdsGrant granted;
+    if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&forward_kernel<F>), LDS_BYTES, granted)) return LFFN_ERR_LAUNCH;
+    forward_kernel<F><<<dim3(workgroups(f.j.tiles * (f.f.Np / TILE))), dim3(THREADS), LDS_BYTES, st>>>(f.f);
+    return LFFN_OK;
+}
+
+template <typename F, typename R>
+int backward(const BackwardArgs &b, hipStream_t st) {
+    static LdsGrant granted_d, granted_g;
+    if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&d_kernel<F>), LDS_BYTES, granted_d) ||
+        !lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&gradients_kernel<F, R>), Tiled::LDS, granted_g))
+        return LFFN_ERR_LAUNCH;
+    for (int p = 0; p < b.pieces; ++p) {
+        d_kernel<F><<<dim3(COMPUTE_UNITS), dim3(THREADS), LDS_BYTES, st>>>(b, p);
+        gradients_kernel<F, R><<<dim3(COMPUTE_UNITS), dim3(THREADS), Tiled::LDS, st>>>(b, p);
+    }
+    if (b.grad_hidden) {
+        const int64_t n = int64_t(b.o.s.N) * (b.o.s.K / 8);
+        hidden_kernel<F, R><<<dim3(unsigned((n + 255) / 256)), dim3(256), 0, st>>>(b);
+    }
+    return LFFN_OK;
+}
+
+}  // namespace
+
+extern "C" int lffn_linear_cross_entropy_kept_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes) {
+    LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
+    const int rc = check(a);
+    if (rc == LFFN_OK) *bytes = kept_bytes(a->tokens);
+    return rc;
+}
+
+extern "C" int lffn_linear_cross_entropy_workspace_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes) {
+    LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
+    const int rc = check(a);
+    Forward f;
+    if (rc == LFFN_OK) *bytes = carve(*a, nullptr, true, f);
+    return rc;
+}
+
+extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a, float *loss, void *kept, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int rc = check(a);
+    if (rc != LFFN_OK) return rc;
+    LFFN_REQUIRE(loss || (a->reduction == 0 && a->tokens == 0), LFFN_ERR_BAD_ARG);
+    Forward f;
+    LFFN_REQUIRE(workspace && lffn_aligned16(workspace) && workspace_bytes >= carve(*a, static_cast<char *>(workspace), true, f), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(lffn_aligned16(kept), LFFN_ERR_BAD_ARG);
+    if (a->reduction == 0 && a->tokens == 0) return LFFN_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    f.f.o.kept = f.j.kept = kept_at(kept ? kept : f.kept, a->tokens);
+    fill(f.r, *a, f.f.o);
+    if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.losses = nullptr;
+    if (a->format == LFFN_ROWS_F32 || a->tokens == 0) head_kernel<<<dim3(1), dim3(64), 0, st>>>(f.f.o.kept.head);
+    if (a->tokens > 0) {
+        if (a->tokens > COUNTED_FROM) {
+            count_kernel<<<dim3(unsigned((a->tokens + 255) / 256)), dim3(256), 0, st>>>(a->labels, a->labels_64, a->ignore_index, f.f.o.s.V, f.f.o.s.N, f.counts);
+            f.r.counts = f.counts;
+        }
+        launch_rows<false>(*a, f.r, st);
+        const int done = a->format == LFFN_ROWS_F32 ? forward<F32Two>(f, st) : a->format == LFFN_ROWS_BF16 ? forward<BF16>(f, st) : forward<F16>(f, st);
+        if (done != LFFN_OK) return done;
+        join_kernel<<<dim3(unsigned(f.f.Np / 16)), dim3(256), 0, st>>>(f.j);
+    }
+    if (a->reduction != 0) sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(f.f.o.kept.head, f.j.losses, loss, a->reduction == 1);
+    return lffn_launch_status();
+}
+
+extern "C" int lffn_linear_cross_entropy_bwd_workspace_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes) {
+    LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
+    const int rc = check(a);
+    Backward w;
+    if (rc == LFFN_OK) *bytes = carve(*a, nullptr, w);
+    return rc;
+}
+
+extern "C" int lffn_linear_cross_entropy_bwd(const lffn_linear_cross_entropy *a, const void *kept, const float *g_loss, void *grad_hidden, void *grad_weight,
+                                             void *grad_bias, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int rc = check(a);
+    if (rc != LFFN_OK) return rc;
+    LFFN_REQUIRE(a->tokens >= 1, LFFN_ERR_UNSUPPORTED);
+    LFFN_REQUIRE(kept && g_loss && lffn_aligned16(kept) && lffn_aligned16(grad_hidden) && lffn_aligned16(grad_weight), LFFN_ERR_BAD_ARG);
+    LFFN_REQUIRE(grad_weight || !grad_bias, LFFN_ERR_BAD_ARG);
+    Backward w;
+    LFFN_REQUIRE(workspace && lffn_aligned16(workspace) && workspace_bytes >= carve(*a, static_cast<char *>(workspace), w), LFFN_ERR_BAD_ARG);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    BackwardArgs &b = w.b;
+    b.o.kept = kept_at(const_cast<void *>(kept), a->tokens);
+    b.g_loss = g_loss;
+    b.grad_hidden = grad_hidden, b.grad_weight = grad_weight, b.grad_bias = grad_bias;
+    b.bias_format = a->bias_format, b.reduction = a->reduction;
+    fill(w.r, *a, b.o);
+    w.r.queues = b.queues, w.r.num_queues = b.pieces;
+    launch_rows<true>(*a, w.r, st);
+    if (a->reduction == 0) coefficient_kernel<<<dim3(1), dim3(1024), 0, st>>>(b);
+    const int done = a->format == LFFN_ROWS_F32    ? backward<F32Two, F32Row>(b, st)
+                     : a->format == LFFN_ROWS_BF16 ? backward<BF16, BF16Row>(b, st)
+                                                   : backward<F16, F16Row>(b, st);
+    return done != LFFN_OK ? done : lffn_launch_status();
+}

@@ -1548,6 +1548,269 @@ def _(q, k, v, key_mask, scale, out, kept, g, of_queries, of_keys):
     return [t.new_empty(t.shape) for t, wanted in ((q, of_queries), (k, of_keys), (v, of_keys)) if wanted]
 
 
+# ----------------------------------------------------------------------------- both ends of a vocabulary
+
+def _fit_rows(t):
+    """Rows whose columns lie together, one stride from row to row; a copy where they do not."""
+    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+EMBEDDING_MAX_ROWS, EMBEDDING_MAX_COLUMNS = (1 << 31) - 2, 1 << 20
+
+
+def _fit_embedding(ids, weight, padding):
+    assert ids.dim() == 1 and ids.dtype in (torch.int32, torch.int64) and -1 <= padding < max(1, weight.shape[0])
+    assert weight.dim() == 2 and row_format(weight.dtype) is not None
+
+
+def _embedding_args(ids, weight, rows, columns, dtype, scale, padding):
+    a = _lib.Embedding()
+    a.ids, a.weight = _lib.ptr(ids), _lib.ptr(weight)
+    a.tokens, a.rows, a.columns, a.stride, a.padding = ids.shape[0], rows, columns, 0 if weight is None else _row_stride(weight), padding
+    a.scale, a.format, a.ids_64 = scale, row_format(dtype), ids.dtype == torch.int64
+    return a
+
+
+_L.define("embedding(Tensor ids, Tensor weight, float scale, int padding) -> Tensor")
+
+
+def _embedding_impl(ids, weight, scale, padding):
+    """ids [tokens], weight [rows, columns] -> [tokens, columns]."""
+    _lib.require_gpu(ids, weight)
+    _fit_embedding(ids, weight, padding)
+    ids, weight = ids.contiguous(), _fit_rows(weight)
+    out = torch.empty(ids.shape[0], weight.shape[1], dtype=weight.dtype, device=weight.device)
+    if out.numel():
+        a = _embedding_args(ids, weight, *weight.shape, weight.dtype, scale, padding)
+        with _dev_guard(weight):
+            rc = _lib.load().lffn_embedding_fwd(ctypes.byref(a), out.data_ptr(), _lib.stream_of(weight))
+        _lib.check(rc, f"lffn_embedding_fwd(ids={tuple(ids.shape)}, weight={tuple(weight.shape)})")
+    return out
+
+
+_L.impl("embedding", _embedding_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::embedding")
+def _(ids, weight, scale, padding):
+    return weight.new_empty(ids.shape[0], weight.shape[1])
+
+
+_L.define("embedding_bwd(Tensor ids, Tensor g, int rows, float scale, int padding) -> Tensor")
+
+
+def _embedding_bwd_impl(ids, g, rows, scale, padding):
+    """ids [tokens], g [tokens, columns] -> the table's gradient [rows, columns]."""
+    _lib.require_gpu(ids, g)
+    assert ids.dim() == 1 and ids.dtype in (torch.int32, torch.int64) and -1 <= padding < max(1, rows)
+    assert g.dim() == 2 and g.shape[0] == ids.shape[0] and row_format(g.dtype) is not None
+    ids, g = ids.contiguous(), g.contiguous()
+    grad = torch.empty(rows, g.shape[1], dtype=g.dtype, device=g.device)
+    if grad.numel():
+        a = _embedding_args(ids, None, *grad.shape, g.dtype, scale, padding)
+        with _dev_guard(g):
+            lib, n = _lib.load(), ctypes.c_int64(0)
+            _lib.check(lib.lffn_embedding_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_embedding_bwd_workspace_bytes")
+            ws = torch.empty(n.value, dtype=torch.uint8, device=g.device)
+            rc = lib.lffn_embedding_bwd(ctypes.byref(a), g.data_ptr(), grad.data_ptr(), _lib.ptr(ws), n.value, _lib.stream_of(g))
+        _lib.check(rc, f"lffn_embedding_bwd(ids={tuple(ids.shape)}, weight={tuple(grad.shape)})")
+    return grad
+
+
+_L.impl("embedding_bwd", _embedding_bwd_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::embedding_bwd")
+def _(ids, g, rows, scale, padding):
+    return g.new_empty(rows, g.shape[1])
+
+
+# ----------------------------------------------------------------------------- layer norm of rows
+
+LAYER_NORM_MAX_ROWS, LAYER_NORM_MAX_COLUMNS = (1 << 24) - 1, 1 << 24
+
+
+def _fit_layer_norm(x, weight, bias):
+    """Arrays that do not fit each other would be read beyond their ends."""
+    assert x.dim() == 2 and x.shape[1] >= 1 and row_format(x.dtype) is not None
+    given = [t for t in (weight, bias) if t is not None]
+    assert all(t.shape == x.shape[1:] and t.dtype in (torch.float32, x.dtype) and t.dtype == given[0].dtype for t in given)
+
+
+def _layer_norm_args(x, weight, bias, eps):
+    a = _lib.LayerNormRows()
+    a.x, a.weight, a.bias = (_lib.ptr(t) for t in (x, weight, bias))
+    a.rows, a.columns = x.shape
+    a.stride, a.eps, a.format = _row_stride(x), eps, row_format(x.dtype)
+    a.weight_f32 = (x if weight is None and bias is None else bias if weight is None else weight).dtype == torch.float32
+    return a
+
+
+_L.define("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool keep) -> (Tensor, Tensor)")
+
+
+def _layer_norm_impl(x, weight, bias, eps, keep):
+    """x [rows, columns], weight and bias [columns] or None -> (out [rows, columns], with `keep` every row's mean and 1 / sigma [rows, 2])."""
+    _lib.require_gpu(x, weight, bias)
+    _fit_layer_norm(x, weight, bias)
+    x, weight, bias = _fit_rows(x), None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(x.shape[0] if keep else 0, 2, dtype=torch.float32, device=x.device)
+    a = _layer_norm_args(x, weight, bias, eps)
+    with _dev_guard(x):
+        rc = _lib.load().lffn_layer_norm_rows_fwd(ctypes.byref(a), out.data_ptr(), stats.data_ptr() if keep else None, _lib.stream_of(x))
+    _lib.check(rc, f"lffn_layer_norm_rows_fwd(x={tuple(x.shape)})")
+    return out, stats
+
+
+_L.impl("layer_norm", _layer_norm_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::layer_norm")
+def _(x, weight, bias, eps, keep):
+    return x.new_empty(x.shape), x.new_empty(x.shape[0] if keep else 0, 2, dtype=torch.float32)
+
+
+_L.define("layer_norm_rows_bwd(Tensor x, Tensor? weight, Tensor? bias, Tensor stats, Tensor g, bool of_x, bool of_weight, bool of_bias) -> Tensor[]")
+
+
+def _layer_norm_rows_bwd_impl(x, weight, bias, stats, g, of_x, of_weight, of_bias):
+    """-> the gradients of x, weight and bias that are wanted."""
+    _lib.require_gpu(x, weight, bias, stats, g)
+    _fit_layer_norm(x, weight, bias)
+    assert stats.shape == (x.shape[0], 2) and stats.dtype == torch.float32 and g.shape == x.shape and g.dtype == x.dtype
+    assert not (of_weight and weight is None) and not (of_bias and bias is None)
+    x, weight, g, stats = _fit_rows(x), None if weight is None else weight.contiguous(), g.contiguous(), _aligned(stats)
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None for t, wanted in ((x, of_x), (weight, of_weight), (bias, of_bias))]
+    a = _layer_norm_args(x, weight, bias, 0.0)
+    with _dev_guard(x):
+        lib, n = _lib.load(), ctypes.c_int64(0)
+        _lib.check(lib.lffn_layer_norm_rows_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_layer_norm_rows_bwd_workspace_bytes")
+        ws = torch.empty(n.value if of_weight or of_bias else 0, dtype=torch.uint8, device=x.device)
+        rc = lib.lffn_layer_norm_rows_bwd(ctypes.byref(a), stats.data_ptr(), g.data_ptr(), *(_lib.ptr(t) for t in grads), _lib.ptr(ws), n.value,
+                                          _lib.stream_of(x))
+    _lib.check(rc, f"lffn_layer_norm_rows_bwd(x={tuple(x.shape)})")
+    return [t for t in grads if t is not None]
+
+
+_L.impl("layer_norm_rows_bwd", _layer_norm_rows_bwd_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::layer_norm_rows_bwd")
+def _(x, weight, bias, stats, g, of_x, of_weight, of_bias):
+    return [t.new_empty(t.shape) for t, wanted in ((x, of_x), (weight, of_weight), (bias, of_bias)) if wanted]
+
+
+# ----------------------------------------------------------------------------- softmax cross entropy of a projection
+
+REDUCTIONS = ("none", "mean", "sum")
+LOSS_MAX_COLUMNS, LOSS_MAX_VOCABULARY, LOSS_MAX_TOKENS = 65536, 1 << 22, 1 << 24
+
+
+def _fit_loss(hidden, weight, bias, labels, reduction):
+    """Arrays that do not fit each other would be read beyond their ends."""
+    assert hidden.dim() == 2 and weight.dim() == 2 and labels.dim() == 1 and 0 <= reduction < len(REDUCTIONS)
+    assert row_format(hidden.dtype) is not None and weight.dtype == hidden.dtype and weight.shape[1] == hidden.shape[1]
+    assert labels.shape[0] == hidden.shape[0] and labels.dtype in (torch.int32, torch.int64)
+    assert bias is None or bias.dtype in (torch.float32, hidden.dtype) and bias.shape == weight.shape[:1]
+
+
+def _rows_together(t):
+    """t [rows, columns] as the kernels read it, a copy where it has to be: the columns together, address and stride of 16 bytes."""
+    size = t.element_size()
+    if (t.shape[1] <= 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0 and (
+            t.shape[0] <= 1 or t.stride(0) >= t.shape[1] and t.stride(0) * size % 16 == 0 and t.stride(0) < 1 << 22):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _linear_cross_entropy_args(hidden, weight, bias, labels, ignore_index, reduction):
+    a = _lib.LinearCrossEntropy()
+    a.hidden, a.weight, a.bias, a.labels = (_lib.ptr(t) for t in (hidden, weight, bias, labels))
+    a.tokens, a.columns = hidden.shape
+    a.vocabulary, a.hidden_stride, a.weight_stride = weight.shape[0], _row_stride(hidden), _row_stride(weight)
+    a.ignore_index, a.format, a.labels_64, a.reduction = ignore_index, row_format(hidden.dtype), labels.dtype == torch.int64, reduction
+    a.bias_format = 0 if bias is None else row_format(bias.dtype)
+    return a
+
+
+def _loss_kept_bytes(tokens):
+    """lffn_linear_cross_entropy_kept_bytes: how many tokens have a label, where a token is among them, and of those the label and two levels."""
+    return 16 + (tokens * 4 + 15) // 16 * 16 * 4
+
+
+_L.define("linear_cross_entropy(Tensor hidden, Tensor weight, Tensor? bias, Tensor labels, int ignore_index, int reduction, bool keep) -> (Tensor, Tensor)")
+
+
+def _linear_cross_entropy_impl(hidden, weight, bias, labels, ignore_index, reduction, keep):
+    """hidden [tokens, columns], weight [vocabulary, columns], bias [vocabulary] or None, labels [tokens] -> (loss, [tokens] or [] by REDUCTIONS[reduction], with
+    `keep` what the backward needs, bytes)."""
+    _lib.require_gpu(hidden, weight, bias, labels)
+    _fit_loss(hidden, weight, bias, labels, reduction)
+    hidden, weight, labels = _rows_together(hidden), _rows_together(weight), labels.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    a = _linear_cross_entropy_args(hidden, weight, bias, labels, ignore_index, reduction)
+    loss = torch.empty(hidden.shape[:1] if reduction == 0 else (), dtype=torch.float32, device=hidden.device)
+    kept = torch.empty(_loss_kept_bytes(hidden.shape[0]) if keep else 0, dtype=torch.uint8, device=hidden.device)
+    with _dev_guard(hidden):
+        lib, n = _lib.load(), ctypes.c_int64(0)
+        _lib.check(lib.lffn_linear_cross_entropy_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_linear_cross_entropy_workspace_bytes")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=hidden.device)
+        rc = lib.lffn_linear_cross_entropy_fwd(ctypes.byref(a), loss.data_ptr(), kept.data_ptr() if keep else None, ws.data_ptr(), n.value,
+                                               _lib.stream_of(hidden))
+    _lib.check(rc, f"lffn_linear_cross_entropy_fwd(hidden={tuple(hidden.shape)}, weight={tuple(weight.shape)})")
+    return loss, kept
+
+
+_L.impl("linear_cross_entropy", _linear_cross_entropy_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::linear_cross_entropy")
+def _(hidden, weight, bias, labels, ignore_index, reduction, keep):
+    return (hidden.new_empty(hidden.shape[:1] if reduction == 0 else (), dtype=torch.float32),
+            hidden.new_empty(_loss_kept_bytes(hidden.shape[0]) if keep else 0, dtype=torch.uint8))
+
+
+_L.define("linear_cross_entropy_bwd(Tensor hidden, Tensor weight, Tensor? bias, Tensor labels, int ignore_index, int reduction, Tensor kept, Tensor g, "
+          "bool of_hidden, bool of_weight, bool of_bias) -> Tensor[]")
+
+
+def _linear_cross_entropy_bwd_impl(hidden, weight, bias, labels, ignore_index, reduction, kept, g, of_hidden, of_weight, of_bias):
+    """-> the gradients of hidden, weight and bias that are wanted."""
+    _lib.require_gpu(hidden, weight, bias, labels, kept, g)
+    _fit_loss(hidden, weight, bias, labels, reduction)
+    assert kept.dtype == torch.uint8 and kept.shape == (_loss_kept_bytes(hidden.shape[0]),)
+    assert g.dtype == torch.float32 and g.shape == (hidden.shape[:1] if reduction == 0 else ()) and not (of_bias and bias is None)
+    hidden, weight, labels, kept = _rows_together(hidden), _rows_together(weight), labels.contiguous(), _aligned(kept)
+    bias, g = None if bias is None else bias.contiguous(), g.contiguous()
+    new = torch.zeros if hidden.shape[0] == 0 else torch.empty
+    # (the bias's gradient is formed beside the weight's)
+    grads = [new(t.shape, dtype=t.dtype, device=t.device) if wanted else None
+             for t, wanted in ((hidden, of_hidden), (weight, of_weight or of_bias), (bias, of_bias))]
+    if hidden.shape[0] > 0:
+        a = _linear_cross_entropy_args(hidden, weight, bias, labels, ignore_index, reduction)
+        with _dev_guard(hidden):
+            lib, n = _lib.load(), ctypes.c_int64(0)
+            _lib.check(lib.lffn_linear_cross_entropy_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_linear_cross_entropy_bwd_workspace_bytes")
+            ws = torch.empty(n.value, dtype=torch.uint8, device=hidden.device)
+            rc = lib.lffn_linear_cross_entropy_bwd(ctypes.byref(a), kept.data_ptr(), g.data_ptr(), *(_lib.ptr(t) for t in grads), ws.data_ptr(), n.value,
+                                                   _lib.stream_of(hidden))
+        _lib.check(rc, f"lffn_linear_cross_entropy_bwd(hidden={tuple(hidden.shape)}, weight={tuple(weight.shape)})")
+    return [t for t, wanted in zip(grads, (of_hidden, of_weight, of_bias)) if wanted]
+
+
+_L.impl("linear_cross_entropy_bwd", _linear_cross_entropy_bwd_impl, "CUDA")
+
+
+@torch.library.register_fake("lookupffn::linear_cross_entropy_bwd")
+def _(hidden, weight, bias, labels, ignore_index, reduction, kept, g, of_hidden, of_weight, of_bias):
+    return [t.new_empty(t.shape) for t, wanted in ((hidden, of_hidden), (weight, of_weight), (bias, of_bias)) if wanted]
+
+
 fht = torch.ops.lookupffn.fht
 bh4_diag = torch.ops.lookupffn.bh4_diag
 bh4_fold = torch.ops.lookupffn.bh4_fold
@@ -1586,3 +1849,9 @@ qk_norm_rotary = torch.ops.lookupffn.qk_norm_rotary
 qk_norm_rotary_bwd = torch.ops.lookupffn.qk_norm_rotary_bwd
 cross_attention = torch.ops.lookupffn.cross_attention
 cross_attention_bwd = torch.ops.lookupffn.cross_attention_bwd
+embedding = torch.ops.lookupffn.embedding
+embedding_bwd = torch.ops.lookupffn.embedding_bwd
+layer_norm = torch.ops.lookupffn.layer_norm
+layer_norm_rows_bwd = torch.ops.lookupffn.layer_norm_rows_bwd
+linear_cross_entropy = torch.ops.lookupffn.linear_cross_entropy
+linear_cross_entropy_bwd = torch.ops.lookupffn.linear_cross_entropy_bwd
