@@ -81,7 +81,18 @@ using torch::autograd::variable_list;
     X(lffn_cross_attention_workspace_bytes) \
     X(lffn_cross_attention_kept_bytes)      \
     X(lffn_cross_attention_bwd)             \
-    X(lffn_cross_attention_bwd_workspace_bytes)
+    X(lffn_cross_attention_bwd_workspace_bytes) \
+    X(lffn_embedding_fwd)                   \
+    X(lffn_embedding_bwd)                   \
+    X(lffn_embedding_bwd_workspace_bytes)   \
+    X(lffn_layer_norm_rows_fwd)             \
+    X(lffn_layer_norm_rows_bwd)             \
+    X(lffn_layer_norm_rows_bwd_workspace_bytes) \
+    X(lffn_linear_cross_entropy_fwd)        \
+    X(lffn_linear_cross_entropy_workspace_bytes) \
+    X(lffn_linear_cross_entropy_kept_bytes) \
+    X(lffn_linear_cross_entropy_bwd)        \
+    X(lffn_linear_cross_entropy_bwd_workspace_bytes)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -684,6 +695,7 @@ PyObject *forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 #include "host_attention.h"
+#include "host_vocabulary.h"
 
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
@@ -692,6 +704,9 @@ PyMethodDef methods[] = {
     {"refuse_foreign_leaves", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(static_cast<PyObject *(*)(PyObject *, PyObject *const *, Py_ssize_t)>(refuse_foreign_leaves))),
      METH_FASTCALL, nullptr},
     {"cross_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cross_attention)), METH_FASTCALL, nullptr},
+    {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding)), METH_FASTCALL, nullptr},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm)), METH_FASTCALL, nullptr},
+    {"linear_cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_cross_entropy)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -7,8 +7,8 @@
 struct NoSecondGradient : public torch::autograd::Node {
     std::string name() const override { return "NoSecondGradient"; }
     variable_list apply(variable_list &&) override {
-        TORCH_CHECK(false, "lookupffn_amd: the gradients of qk_norm_rotary and cross_attention cannot be differentiated (a graph through them was "
-                           "asked for with create_graph)");
+        TORCH_CHECK(false, "lookupffn_amd: the gradients of this package's operators cannot be differentiated (a graph through them was asked for "
+                           "with create_graph)");
     }
 };
 

@@ -7,7 +7,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .cross_attention import _DTYPES, _recorded, _refuse_foreign_leaves, _require
+from .cross_attention import _DTYPES, _host, _recorded, _refuse_foreign_leaves, _require
 
 
 class LayerNorm(Function):
@@ -38,6 +38,11 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
 
     -> [..., columns] of x's type.  Gradients: x, weight and bias, sums over the rows in a fixed order, the same bits on every call; none of theirs, and none in forward mode (an error);
     captured in graphs as ``cross_attention`` is."""
+    host = _host()
+    if host:
+        out = host.layer_norm(x, weight, bias, eps)
+        if out is not None:
+            return out
     _lib.require_gpu(x, weight, bias)
     _refuse_foreign_leaves(x, weight, bias)
     _require(x.dim() >= 1 and x.dtype in _DTYPES, f"x: [..., columns] float32, float16 or bfloat16, got {tuple(x.shape)} {x.dtype}")

@@ -10,7 +10,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .cross_attention import _DTYPES, _recorded, _refuse_foreign_leaves, _require
+from .cross_attention import _DTYPES, _host, _recorded, _refuse_foreign_leaves, _require
 
 
 class Embedding(Function):
@@ -38,6 +38,11 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None):
 
     -> [..., columns] of weight's type.  Gradient: weight, the whole table, from the tokens sorted by their numbers: sums in float32 in a fixed order, one rounding, the same bits on
     every call; none of its own, and none in forward mode (an error); captured in graphs as ``cross_attention`` is."""
+    host = _host()
+    if host:
+        out = host.embedding(ids, weight, scale, padding_idx)
+        if out is not None:
+            return out
     _lib.require_gpu(ids, weight)
     _refuse_foreign_leaves(weight)
     _require(ids.dtype in (torch.int32, torch.int64), f"ids: int32 or int64, got {ids.dtype}")
@@ -85,6 +90,11 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
     float32: products of two half-precision terms a number, sums in float32, errors of the size of float32 products'; in the backward a number of hidden or
     weight is held to 2^-38 of the largest of its array.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half: held to 2^-38 of the largest token's).
     -> float32.  Gradients: hidden, weight and bias, the same bits on every call; none of theirs, and none in forward mode (an error); captured in graphs as ``cross_attention`` is."""
+    host = _host()
+    if host:
+        out = host.linear_cross_entropy(hidden, weight, bias, labels, ignore_index, reduction)
+        if out is not None:
+            return out
     _lib.require_gpu(hidden, weight, bias, labels)
     _refuse_foreign_leaves(hidden, weight, bias)
     _require(hidden.dim() >= 1 and hidden.dtype in _DTYPES, f"hidden: [..., columns] float32, float16 or bfloat16, got {tuple(hidden.shape)} {hidden.dtype}")
