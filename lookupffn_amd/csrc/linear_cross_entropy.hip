@@ -20,7 +20,7 @@ using namespace product_tiles;
 constexpr int TILE = 256;                       // tokens and vocabulary entries of a tile
 constexpr int THREADS = 512, WAVES_M = 2, WAVES_N = 4, MB = TILE / WAVES_M / 32, NB = TILE / WAVES_N / 32;
 constexpr int COMPUTE_UNITS = 256, XCDS = 8;
-constexpr int CHUNK = 64;                       // tokens a workgroup lays together
+constexpr int CHUNK = 64, PARTS = 4;            // tokens whose places a workgroup finds, and workgroups that lay their rows
 constexpr int COUNTED_FROM = 4096;              // tokens from which on a launch of its own counts the labelled ones of every chunk
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LIFT = 16384.f;                 // d times 2^14: half's normal numbers then reach down to 2^-28 of a row's largest
@@ -74,8 +74,6 @@ struct RowsArgs {
     const int32_t *counts;                     // labelled tokens of every chunk, or null
     int32_t *token;                            // [labelled]
     float *loss;                               // [N]: zeros for the others, or null
-    int32_t *queues;                           // counters to clear, or null
-    int num_queues;
 };
 
 __device__ __forceinline__ int label_of(const void *labels, int wide, int64_t i, int64_t ignore, int V) {
@@ -142,26 +140,30 @@ __device__ __forceinline__ float bias_of(const void *bias, int format, int v) {
     return (float)static_cast<const _Float16 *>(bias)[v];
 }
 
-// Workgroups 0 .. tokens / CHUNK - 1: the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
+// Of many that raise one number only those that would are atomic (32003 rows: 370 us otherwise, 25 like this).
+__device__ __forceinline__ void raise(int32_t *most, int v) {
+    if (__hip_atomic_load(most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < v) atomicMax(most, v);
+}
+
+// Workgroups PARTS (tokens / CHUNK): the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
 // one fills the last tile's rows up with zeros.  The workgroups behind: the bias in fp32.
 template <typename R, int PLANES, bool BACKWARD>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     const Sizes &s = a.o.s;
     const Kept &k = a.o.kept;
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, chunks = (s.N + CHUNK - 1) / CHUNK;
-    if ((int)blockIdx.x >= chunks) {
-        const int v = ((int)blockIdx.x - chunks) * 256 + tid;
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, chunks = (s.N + CHUNK - 1) / CHUNK, chunk = blockIdx.x / PARTS, part = blockIdx.x % PARTS;
+    if (chunk >= chunks) {
+        const int v = ((int)blockIdx.x - chunks * PARTS) * 256 + tid;
         if (v < s.Vp) a.o.bias[v] = v >= s.V ? -INFINITY : a.bias_format < 0 ? 0.f : bias_of(a.bias, a.bias_format, v);
-        if (BACKWARD && v < a.num_queues) a.queues[v] = 0;
         return;
     }
     __shared__ int place[CHUNK], before[4];
-    const int t0 = blockIdx.x * CHUNK;
+    const int t0 = chunk * CHUNK;
     int labelled = 0;              // up to and with this chunk
     if constexpr (!BACKWARD) {
         int n = 0;
         if (a.counts)
-            for (int i = tid; i < (int)blockIdx.x; i += 256) n += a.counts[i];
+            for (int i = tid; i < chunk; i += 256) n += a.counts[i];
         else
             for (int i = tid; i < t0; i += 256) n += label_of(a.labels, a.labels_64, i, a.ignore, s.V) >= 0;
 #pragma unroll
@@ -175,12 +177,12 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
         if (wave == 0) {
             const int at = y >= 0 ? first + __popcll(live & ((uint64_t(1) << lane) - 1)) : -1;
             place[lane] = at;
-            if (t < s.N) {
+            if (t < s.N && part == 0) {
                 k.pos[t] = at;
                 if (y >= 0) k.label[at] = y, a.token[at] = t;
                 else if (a.loss) a.loss[t] = 0.f;
             }
-            if ((int)blockIdx.x == chunks - 1 && lane == 0) k.head[0] = labelled;
+            if (chunk == chunks - 1 && part == 0 && lane == 0) k.head[0] = labelled;
         }
     } else {
         labelled = k.head[0];
@@ -188,19 +190,19 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     }
     __syncthreads();
     const int64_t row_bytes = s.Kp * 2;
-    for (int i = wave; i < CHUNK; i += 4) {
+    for (int i = part * 4 + wave; i < CHUNK; i += 4 * PARTS) {
         const int at = place[i];
         if (at < 0) continue;
         const char *from = static_cast<const char *>(a.hidden) + (int64_t(t0) + i) * a.hidden_stride * R::BYTES;
         const int e = lay_row<R, PLANES>(from, a.o.rows + at * row_bytes, a.o.rows_plane, s.K, s.Kp, BACKWARD ? k.head + 1 : nullptr);
         if (PLANES == 2 && !BACKWARD && lane == 0) {
             a.o.row_scale[at] = __builtin_amdgcn_ldexpf(1.f, e);
-            atomicMax(k.head + 1, e);
+            raise(k.head + 1, e);
         }
     }
-    if ((int)blockIdx.x == chunks - 1) {
+    if (chunk == chunks - 1) {
         const int64_t from = labelled * row_bytes / 16, to = up(labelled, TILE) * row_bytes / 16;
-        for (int64_t i = from + tid; i < to; i += 256)
+        for (int64_t i = from + part * 256 + tid; i < to; i += 256 * PARTS)
             for (int p = 0; p < PLANES; ++p) *reinterpret_cast<uint4 *>(a.o.rows + p * a.o.rows_plane + i * 16) = make_uint4(0, 0, 0, 0);
         if (PLANES == 2 && !BACKWARD)
             for (int i = labelled + tid; i < up(labelled, TILE); i += 256) a.o.row_scale[i] = 1.f;
@@ -222,38 +224,62 @@ __global__ __launch_bounds__(256) void weight_kernel(Operands o, const float *w,
                                BACKWARD ? o.kept.head + 2 : nullptr);
     if (threadIdx.x % 64 == 0) {
         o.weight_scale[v] = __builtin_amdgcn_ldexpf(1.f, e);
-        if (!BACKWARD && v < o.s.V) atomicMax(o.kept.head + 2, e);
+        if (!BACKWARD && v < o.s.V) raise(o.kept.head + 2, e);
     }
 }
 
 // ---------------------------------------------------------------- logits
 
-// A workgroup's tiles of vt x nt: those of an XCD follow each other, eight tiles of the vocabulary at a time against one tile of tokens after the other, so that the compute
-// units of an XCD read the same ones.
-template <typename Each>
-__device__ __forceinline__ void for_tiles(int vt, int nt, Each &&each) {
-    const int xcd = blockIdx.x % XCDS, slots = gridDim.x / XCDS, total = vt * nt, share = (total + XCDS - 1) / XCDS;
-    for (int i = blockIdx.x / XCDS; i < share; i += slots) {
-        const int id = xcd * share + i;
-        if (id >= total) return;
-        const int group = id / (8 * nt), in = id - group * 8 * nt, height = min(8, vt - group * 8);
-        each(group * 8 + in % height, in / height);
+// A workgroup's tasks of `total`, in turn: those of an XCD follow each other, so that its compute units read the same ones.
+struct Turns {
+    int at, end, step;
+    __device__ __forceinline__ explicit Turns(int total) {
+        const int xcd = blockIdx.x % XCDS, share = (total + XCDS - 1) / XCDS;
+        step = gridDim.x / XCDS;
+        at = xcd * share + blockIdx.x / XCDS;
+        end = min(total, (xcd + 1) * share);
     }
-}
-
-struct Tiled {
-    static constexpr uint32_t LDS = 2 * (TILE + TILE) * 128;
+    __device__ __forceinline__ bool any() const { return at < end; }
 };
 
-// A tile's products: entries from v0, tokens from n0.
-template <typename F>
-__device__ __forceinline__ void logits(Sums<MB, NB> &sums, const Operands &o, int labelled, int v0, int n0, uint32_t lds) {
+// A tile of vt x nt: eight tiles of the vocabulary at a time against one tile of tokens after the other.
+struct Place {
+    int v, n;
+    __device__ __forceinline__ Place(int id, int vt, int nt) {
+        const int group = id / (8 * nt), in = id - group * 8 * nt, height = min(8, vt - group * 8);
+        v = (group * 8 + in % height) * TILE;
+        n = in / height * TILE;
+    }
+};
+
+typedef Along<TILE, THREADS, 1> AlongOne;
+constexpr uint32_t STREAM_LDS = Stream<F16, MB, NB, AlongOne, AlongOne>::LDS;      // (of any operands)
+
+// The logits of one tile after the other: entries from v0 on, in all `width`, and the labelled tokens; each(sums, place) has the sums of a tile's products.
+template <typename F, typename Each>
+__device__ __forceinline__ void for_logits(const Operands &o, int labelled, int v0, int width, uint32_t lds, Each &&each) {
     typedef Along<TILE, THREADS, F::PLANES> Side;
-    const int wave = threadIdx.x / 64;
-    const Side a(o.weight, v0), b(rows_of(o, labelled), n0);
-    const typename Side::Reader ra(wave / WAVES_N * MB * 32), rb(wave % WAVES_N * NB * 32);
-    sums.clear();
-    multiply<F>(sums, a, b, ra, rb, lds, 0, (o.s.K + Side::K - 1) / Side::K, [](int, const uint4 &) {});
+    const int wave = threadIdx.x / 64, vt = (width + TILE - 1) / TILE, nt = (labelled + TILE - 1) / TILE, steps = max(2, (o.s.K + Side::K - 1) / Side::K);
+    Turns turns(vt * nt);
+    if (!turns.any()) return;
+    const Source rows = rows_of(o, labelled);
+    Place place(turns.at, vt, nt);
+    Side a(o.weight, v0 + place.v), b(rows, place.n);
+    Stream<F, MB, NB, Side, Side> stream(lds, wave / WAVES_N * MB * 32, wave % WAVES_N * NB * 32);
+    stream.prime(a, b, 0);
+    for (;;) {
+        const int next = turns.at + turns.step;
+        const bool more = next < turns.end;
+        const Place then(more ? next : turns.at, vt, nt);
+        const Side next_a(o.weight, v0 + then.v), next_b(rows, then.n);
+        Sums<MB, NB> sums;
+        sums.clear();
+        stream.multiply(sums, a, b, 0, steps, next_a, next_b, 0, [](int, const uint4 &) {});
+        each(sums, place);
+        if (!more) break;
+        turns.at = next, place = then;
+    }
+    stream.done();
 }
 
 // The logits of the tile's 16 entries of block i for the token of block j: l[e] of entry mfma_row(e, half)
@@ -289,17 +315,15 @@ template <typename F>
 __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
     const uint32_t lds = lds_byte_of(lds_words);
-    float2 *const halves = reinterpret_cast<float2 *>(reinterpret_cast<char *>(lds_words) + Tiled::LDS);     // [WAVES_M][TILE]
+    float2 *const halves = reinterpret_cast<float2 *>(reinterpret_cast<char *>(lds_words) + STREAM_LDS);     // [WAVES_M][TILE]
     const Operands &o = a.o;
     const int labelled = o.kept.head[0], tid = threadIdx.x, wave = tid / 64, lane = tid % 64, half = lane / 32;
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-    for_tiles((o.s.V + TILE - 1) / TILE, (labelled + TILE - 1) / TILE, [&](int vt, int nt) {
-        Sums<MB, NB> sums;
-        logits<F>(sums, o, labelled, vt * TILE, nt * TILE, lds);
-        const int v0 = vt * TILE + wm * MB * 32;
+    for_logits<F>(o, labelled, 0, o.s.V, lds, [&](const Sums<MB, NB> &sums, const Place &p) {
+        const int v0 = p.v + wm * MB * 32;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const int column = wn * NB * 32 + j * 32 + lane % 32, n = nt * TILE + column;
+            const int column = wn * NB * 32 + j * 32 + lane % 32, n = p.n + column;
             const float row_scale = F::PLANES == 2 ? o.row_scale[n] : 1.f;
             const int at = n < labelled ? o.kept.label[n] - v0 : -1;
             float2 of = make_float2(-INFINITY, 0.f);
@@ -327,7 +351,7 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
             if (half == 0) halves[wm * TILE + column] = joined(of, other);
         }
         __syncthreads();
-        if (tid < TILE) a.parts[vt * a.Np + nt * TILE + tid] = joined(halves[tid], halves[TILE + tid]);
+        if (tid < TILE) a.parts[p.v / TILE * a.Np + p.n + tid] = joined(halves[tid], halves[TILE + tid]);
         // (the next tile's products have barriers before halves is written again)
     });
 }
@@ -390,7 +414,6 @@ struct BackwardArgs {
     const float *g_loss;       // [1] or [N]
     float *coefficient;        // [labelled] or null: what d is multiplied with beside `factor`
     float *power;              // [1]: of both gradients, where there are coefficients
-    int32_t *queues;
     void *grad_hidden, *grad_weight, *grad_bias;
     int32_t bias_format, reduction, pieces;
 };
@@ -398,7 +421,7 @@ struct BackwardArgs {
 // How a piece is laid out, from the number of labelled tokens, alike in every launch.
 struct Piece {
     int v0, width, ld, nt;     // entries, numbers of d's rows, tiles of tokens
-    int shares, share;         // of the piece's entries, for dh: steps each
+    int shares, share;         // of dh's sum over the piece's entries; of steps, an even number, each: the piece's own
 };
 template <typename F>
 __device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, int piece) {
@@ -410,10 +433,11 @@ __device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, i
     const int64_t first = int64_t(piece) * p.ld;
     p.v0 = (int)min(first, int64_t(a.o.s.V));
     p.width = min(p.ld, a.o.s.V - p.v0);
-    // a share's sum is about as long as one over the tokens, so that tasks are alike; all pieces have as many
-    const int steps = p.ld / K, most = (int)min(int64_t(SHARES), a.parts_bytes / (max(labelled, 1) * int64_t(a.o.s.K) * 4));
-    p.shares = max(1, min(most, steps / max(16, (labelled + K - 1) / K)));
-    p.share = (steps + p.shares - 1) / p.shares;
+    // a share's sum is about as long as one over the tokens, so that tasks are alike; no piece has more than the first
+    const int steps = (min(p.ld, a.o.s.V) + K - 1) / K, most = (int)min(int64_t(SHARES), a.parts_bytes / (max(labelled, 1) * int64_t(a.o.s.K) * 4));
+    const int shares = max(1, min(most, steps / max(16, (labelled + K - 1) / K)));
+    p.share = (steps + 2 * shares - 1) / (2 * shares) * 2;
+    p.shares = ((p.width + K - 1) / K + p.share - 1) / p.share;
     return p;
 }
 
@@ -449,13 +473,11 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
     const int labelled = o.kept.head[0], wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N;
     const Piece p = piece_of<F>(a, labelled, piece);
     const float scale = F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : 1.f;
-    for_tiles((p.width + TILE - 1) / TILE, p.nt, [&](int vt, int nt) {
-        Sums<MB, NB> sums;
-        logits<F>(sums, o, labelled, p.v0 + vt * TILE, nt * TILE, lds);
-        const int in = vt * TILE + wm * MB * 32, v0 = p.v0 + in;
+    for_logits<F>(o, labelled, p.v0, p.width, lds, [&](const Sums<MB, NB> &sums, const Place &tile) {
+        const int in = tile.v + wm * MB * 32, v0 = p.v0 + in;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const int n = nt * TILE + wn * NB * 32 + j * 32 + lane % 32;
+            const int n = tile.n + wn * NB * 32 + j * 32 + lane % 32;
             const bool live = n < labelled;
             const float2 level = live ? o.kept.level[n] : make_float2(0.f, 0.f);
             const float by = live ? LIFT * (a.coefficient ? a.coefficient[n] : 1.f) : 0.f;
@@ -523,113 +545,134 @@ __device__ __forceinline__ void store8(char *to, const float (&v)[8]) {
         *reinterpret_cast<uint4 *>(to) = R::pack(v);
 }
 
-// A share of dh: tokens from n0 x columns from h0, the sum over steps first .. end - 1 of the piece's entries.
+// dh: shares of the piece's entries x tiles of tokens x tiles of columns, one after the other; each adds to its own part.
 template <typename F>
-__device__ __forceinline__ void hidden_task(const BackwardArgs &a, const Piece &p, int labelled, int piece, int share, int n0, int h0, uint32_t lds) {
+__device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece &p, int labelled, bool first_piece, uint32_t lds) {
     typedef Along<TILE, THREADS, F::PLANES> Left;
     typedef Across<TILE, THREADS, F::PLANES> Right;
     const Operands &o = a.o;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32;
-    const Left left({a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld}, n0);
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, ht = (o.s.K + TILE - 1) / TILE;
+    const Source d{a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld};
     Source w = o.weight;
     w.at += p.v0 * w.stride;
     w.rows = p.width;
-    const Right right(w, h0);
-    const typename Left::Reader ra(wave / WAVES_N * MB * 32);
-    const typename Right::Reader rb(wave % WAVES_N * NB * 32);
-    Sums<MB, NB> sums;
-    sums.clear();
-    const int first = share * p.share, steps = (p.width + Left::K - 1) / Left::K;
-    multiply<F>(sums, left, right, ra, rb, lds, first, min(steps, first + p.share), [](int, const uint4 &) {});
+    struct Task {
+        int share, n, h, first, end;
+        // (d has zeros behind the piece's last entry, up to a whole tile: an odd number of steps is followed by one of them)
+        __device__ __forceinline__ Task(int id, const Piece &p, int ht, int steps)
+            : share(id / ht / p.nt), n(id / ht % p.nt * TILE), h(id % ht * TILE), first(share * p.share), end(min((steps + 1) / 2 * 2, first + p.share)) {}
+    };
+    const int steps = (p.width + Left::K - 1) / Left::K;
+    Turns turns(p.shares * p.nt * ht);
+    if (!turns.any()) return;
+    Task task(turns.at, p, ht, steps);
+    Left left(d, task.n);
+    Right right(w, task.h);
+    Stream<F, MB, NB, Left, Right> stream(lds, wave / WAVES_N * MB * 32, wave % WAVES_N * NB * 32);
+    stream.prime(left, right, task.first);
+    for (;;) {
+        const int next = turns.at + turns.step;
+        const bool more = next < turns.end;
+        const Task then(more ? next : turns.at, p, ht, steps);
+        const Left next_left(d, then.n);
+        const Right next_right(w, then.h);
+        Sums<MB, NB> sums;
+        sums.clear();
+        stream.multiply(sums, left, right, task.first, task.end, next_left, next_right, then.first, [](int, const uint4 &) {});
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        const int h = h0 + (wave % WAVES_N * NB + j) * 32 + lane % 32;
-        if (h >= o.s.K) continue;
+        for (int j = 0; j < NB; ++j) {
+            const int h = task.h + (wave % WAVES_N * NB + j) * 32 + lane % 32;
+            if (h >= o.s.K) continue;
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-            const int n = n0 + (wave / WAVES_N * MB + i) * 32;
+            for (int i = 0; i < MB; ++i) {
+                const int n = task.n + (wave / WAVES_N * MB + i) * 32;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int row = n + mfma_row(e, half);
-                float *const at = a.parts + (int64_t(share) * labelled + row) * o.s.K + h;
-                if (row < labelled) *at = piece ? *at + sums.v[i][j][e] : sums.v[i][j][e];
+                for (int e = 0; e < 16; ++e) {
+                    const int row = n + mfma_row(e, half);
+                    float *const at = a.parts + (int64_t(task.share) * labelled + row) * o.s.K + h;
+                    if (row < labelled) *at = first_piece ? sums.v[i][j][e] : *at + sums.v[i][j][e];
+                }
             }
         }
+        if (!more) break;
+        turns.at = next, task = then;
     }
+    stream.done();
 }
 
-// dW's entries from v0 (of the piece) x columns from h0, and, with the first columns, db's.
+// dW: tiles of the piece's entries x tiles of columns, and, with the first columns, db.
 template <typename F, typename R>
-__device__ __forceinline__ void weight_task(const BackwardArgs &a, const Piece &p, int labelled, int v0, int h0, uint32_t lds) {
+__device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece &p, int labelled, uint32_t lds) {
     typedef Across<TILE, THREADS, F::PLANES> Side;
     const Operands &o = a.o;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N;
-    Source rows = rows_of(o, labelled);
-    const Side left(rows, h0), right({a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld}, v0);
-    const typename Side::Reader ra(wm * MB * 32), rb(wn * NB * 32);
-    Sums<MB, NB> sums;
-    sums.clear();
-    float bias[NB] = {};
-    const bool of_bias = h0 == 0 && wm == 0 && a.grad_bias;
-    multiply<F>(sums, left, right, ra, rb, lds, 0, (labelled + Side::K - 1) / Side::K, [&](int j, const uint4 &u) {
-        if (of_bias) bias[j] = dot_ones(F(), u, bias[j]);
-    });
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N, ht = (o.s.K + TILE - 1) / TILE;
+    const Source rows = rows_of(o, labelled), d{a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld};
+    // (rows and d have zeros behind the last token, up to a whole tile)
+    const int steps = labelled ? max(2, (labelled + Side::K - 1) / Side::K) : 0;
     const float factor = factor_of(a, labelled), by = F::PLANES == 2 ? factor * __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : factor;
+    Turns turns((p.width + TILE - 1) / TILE * ht);
+    if (!turns.any()) return;
+    int v0 = turns.at / ht * TILE, h0 = turns.at % ht * TILE;
+    Side left(rows, h0), right(d, v0);
+    Stream<F, MB, NB, Side, Side> stream(lds, wm * MB * 32, wn * NB * 32);
+    if (steps) stream.prime(left, right, 0);
+    for (;;) {
+        const int next = turns.at + turns.step;
+        const bool more = next < turns.end;
+        const int next_v = (more ? next : turns.at) / ht * TILE, next_h = (more ? next : turns.at) % ht * TILE;
+        const Side next_left(rows, next_h), next_right(d, next_v);
+        Sums<MB, NB> sums;
+        sums.clear();
+        float bias[NB] = {};
+        const bool of_bias = h0 == 0 && wm == 0 && a.grad_bias;
+        if (steps)
+            stream.multiply(sums, left, right, 0, steps, next_left, next_right, 0, [&](int j, const uint4 &u) {
+                if (of_bias) bias[j] = dot_ones(F(), u, bias[j]);
+            });
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        const int in = v0 + (wn * NB + j) * 32 + lane % 32, v = p.v0 + in;
-        const bool live = in < p.width;
-        if (of_bias) {
-            const float sum = (bias[j] + __shfl_xor(bias[j], 32)) * factor;
-            if (half == 0 && live) {
-                if (a.bias_format == LFFN_ROWS_F32) static_cast<float *>(a.grad_bias)[v] = sum;
-                else if (a.bias_format == LFFN_ROWS_BF16) static_cast<__bf16 *>(a.grad_bias)[v] = (__bf16)sum;
-                else static_cast<_Float16 *>(a.grad_bias)[v] = (_Float16)sum;
-            }
-        }
-        char *const row = static_cast<char *>(a.grad_weight) + int64_t(v) * o.s.K * R::BYTES;
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int g = 0; g < 4; g += 2) {
-                float t[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(sums.v[i][j][4 * g + e] * by), __float_as_uint(sums.v[i][j][4 * g + 4 + e] * by),
-                                                                    false, false);
-                    t[e] = __uint_as_float(s[0]), t[4 + e] = __uint_as_float(s[1]);
+        for (int j = 0; j < NB; ++j) {
+            const int in = v0 + (wn * NB + j) * 32 + lane % 32, v = p.v0 + in;
+            const bool live = in < p.width;
+            if (of_bias) {
+                const float sum = (bias[j] + __shfl_xor(bias[j], 32)) * factor;
+                if (half == 0 && live) {
+                    if (a.bias_format == LFFN_ROWS_F32) static_cast<float *>(a.grad_bias)[v] = sum;
+                    else if (a.bias_format == LFFN_ROWS_BF16) static_cast<__bf16 *>(a.grad_bias)[v] = (__bf16)sum;
+                    else static_cast<_Float16 *>(a.grad_bias)[v] = (_Float16)sum;
                 }
-                const int h = h0 + (wm * MB + i) * 32 + 8 * (g + half);
-                if (live && h < o.s.K) store8<R>(row + h * R::BYTES, t);
             }
+            char *const row = static_cast<char *>(a.grad_weight) + int64_t(v) * o.s.K * R::BYTES;
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; g += 2) {
+                    float t[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(sums.v[i][j][4 * g + e] * by), __float_as_uint(sums.v[i][j][4 * g + 4 + e] * by),
+                                                                        false, false);
+                        t[e] = __uint_as_float(s[0]), t[4 + e] = __uint_as_float(s[1]);
+                    }
+                    const int h = h0 + (wm * MB + i) * 32 + 8 * (g + half);
+                    if (live && h < o.s.K) store8<R>(row + h * R::BYTES, t);
+                }
+        }
+        if (!more) break;
+        turns.at = next, v0 = next_v, h0 = next_h;
     }
+    stream.done();
 }
 
-// Both gradients of a piece: a queue of tasks, the shares of dh first.
+// Both gradients of a piece.
 template <typename F, typename R>
 __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, int piece) {
     extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
-    __shared__ int next;
     const uint32_t lds = lds_byte_of(lds_words);
     const int labelled = a.o.kept.head[0];
     const Piece p = piece_of<F>(a, labelled, piece);
     if (p.width <= 0) return;
-    const int ht = (a.o.s.K + TILE - 1) / TILE, vt = (p.width + TILE - 1) / TILE;
-    const int hidden = a.grad_hidden ? p.shares * p.nt * ht : 0, total = hidden + (a.grad_weight ? vt * ht : 0);
-    for (;;) {
-        if (threadIdx.x == 0) next = atomicAdd(a.queues + piece, 1);
-        __syncthreads();
-        const int task = __builtin_amdgcn_readfirstlane(next);
-        __syncthreads();
-        if (task >= total) return;
-        if (task < hidden) {
-            const int h = task % ht, n = task / ht % p.nt, share = task / ht / p.nt;
-            hidden_task<F>(a, p, labelled, piece, share, n * TILE, h * TILE, lds);
-        } else {
-            const int t = task - hidden;
-            weight_task<F, R>(a, p, labelled, t / ht * TILE, t % ht * TILE, lds);
-        }
-    }
+    if (a.grad_hidden && labelled) hidden_tasks<F>(a, p, labelled, piece == 0, lds);
+    if (a.grad_weight) weight_tasks<F, R>(a, p, labelled, lds);
 }
 
 // dh: a labelled token's shares added up, zeros for the others.
@@ -642,6 +685,7 @@ __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
     float v[8] = {};
     if (at >= 0) {
         const int shares = piece_of<F>(a, labelled, 0).shares;
+#pragma unroll 8
         for (int p = 0; p < shares; ++p) {
             const float *from = a.parts + (int64_t(p) * labelled + at) * s.K + c;
             const float4 x = *reinterpret_cast<const float4 *>(from), y = *reinterpret_cast<const float4 *>(from + 4);
@@ -690,7 +734,7 @@ struct Carver {
 Operands operands(const lffn_linear_cross_entropy &a, Carver &c) {
     Operands o{};
     const int64_t Np = up(a.tokens, TILE);
-    o.s = {(int)a.tokens, (int)a.vocabulary, (int)a.columns, up(a.columns, STEP), up(a.vocabulary, TILE)};
+    o.s = {(int)a.tokens, (int)a.vocabulary, (int)a.columns, up(a.columns, 2 * STEP), up(a.vocabulary, TILE)};
     const int planes = planes_of(a);
     o.rows_plane = Np * o.s.Kp * 2;
     o.rows = c.take<char>(o.rows_plane * planes);
@@ -751,7 +795,6 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     // as many launches as pieces if all tokens are labelled; with fewer the last ones find nothing
     const int64_t ld = b.d_bytes / (Np > 0 ? Np * 2 * planes : 1) / TILE * TILE;
     b.pieces = a.tokens == 0 ? 0 : int((a.vocabulary + ld - 1) / ld);
-    b.queues = c.take<int32_t>(b.pieces);
     return c.used;
 }
 
@@ -764,8 +807,7 @@ void fill(RowsArgs &r, const lffn_linear_cross_entropy &a, const Operands &o) {
 
 template <bool BACKWARD>
 void launch_rows(const lffn_linear_cross_entropy &a, const RowsArgs &r, hipStream_t st) {
-    const int64_t flat = r.num_queues > r.o.s.Vp ? r.num_queues : r.o.s.Vp;
-    const dim3 grid(unsigned((a.tokens + CHUNK - 1) / CHUNK + (flat + 255) / 256));
+    const dim3 grid(unsigned((a.tokens + CHUNK - 1) / CHUNK * PARTS + (r.o.s.Vp + 255) / 256));
     if (a.format == LFFN_ROWS_F32) {
         weight_kernel<BACKWARD><<<dim3(unsigned(r.o.s.Vp / 4)), dim3(256), 0, st>>>(r.o, static_cast<const float *>(a.weight), a.weight_stride);
         rows_kernel<F32Row, 2, BACKWARD><<<grid, dim3(256), 0, st>>>(r);
@@ -775,7 +817,7 @@ void launch_rows(const lffn_linear_cross_entropy &a, const RowsArgs &r, hipStrea
 
 unsigned workgroups(int64_t tiles) { return unsigned(tiles >= COMPUTE_UNITS ? COMPUTE_UNITS : up(tiles, XCDS)); }
 
-constexpr size_t LDS_BYTES = Tiled::LDS + WAVES_M * TILE * sizeof(float2);
+constexpr size_t LDS_BYTES = STREAM_LDS + WAVES_M * TILE * sizeof(float2);
 
 template <typename F>
 int forward(const Forward &f, hipStream_t st) {
@@ -789,11 +831,11 @@ template <typename F, typename R>
 int backward(const BackwardArgs &b, hipStream_t st) {
     static LdsGrant granted_d, granted_g;
     if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&d_kernel<F>), LDS_BYTES, granted_d) ||
-        !lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&gradients_kernel<F, R>), Tiled::LDS, granted_g))
+        !lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&gradients_kernel<F, R>), STREAM_LDS, granted_g))
         return LFFN_ERR_LAUNCH;
     for (int p = 0; p < b.pieces; ++p) {
         d_kernel<F><<<dim3(COMPUTE_UNITS), dim3(THREADS), LDS_BYTES, st>>>(b, p);
-        gradients_kernel<F, R><<<dim3(COMPUTE_UNITS), dim3(THREADS), Tiled::LDS, st>>>(b, p);
+        gradients_kernel<F, R><<<dim3(COMPUTE_UNITS), dim3(THREADS), STREAM_LDS, st>>>(b, p);
     }
     if (b.grad_hidden) {
         const int64_t n = int64_t(b.o.s.N) * (b.o.s.K / 8);
@@ -870,7 +912,6 @@ extern "C" int lffn_linear_cross_entropy_bwd(const lffn_linear_cross_entropy *a,
     b.grad_hidden = grad_hidden, b.grad_weight = grad_weight, b.grad_bias = grad_bias;
     b.bias_format = a->bias_format, b.reduction = a->reduction;
     fill(w.r, *a, b.o);
-    w.r.queues = b.queues, w.r.num_queues = b.pieces;
     launch_rows<true>(*a, w.r, st);
     if (a->reduction == 0) coefficient_kernel<<<dim3(1), dim3(1024), 0, st>>>(b);
     const int done = a->format == LFFN_ROWS_F32    ? backward<F32Two, F32Row>(b, st)

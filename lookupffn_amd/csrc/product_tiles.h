@@ -82,15 +82,11 @@ struct Along {
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) offset[i] = uint32_t(min(r + i * (THREADS / 8), s.rows - 1 - row) * s.stride);
     }
-    __device__ __forceinline__ void begin(int step, uint32_t lds) const {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 1024), column = min(step * K + k, last) * 2;
-        if constexpr (PLANES == 1) {
-#pragma unroll
-            for (int i = 0; i < SHARE; ++i) copy_to_lds(base, offset[i] + column, lds + wave + i * THREADS * 16);
-        } else {
-#pragma unroll
-            for (int i = 0; i < SHARE; ++i) copy_to_lds_far(base + plane + offset[i] + column, lds + wave + i * THREADS * 16);
-        }
+    // the thread's i-th piece of a step
+    __device__ __forceinline__ void begin(int step, uint32_t lds, int i) const {
+        const uint32_t to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 1024) + i * THREADS * 16, column = min(step * K + k, last) * 2;
+        if constexpr (PLANES == 1) copy_to_lds(base, offset[i] + column, to);
+        else copy_to_lds_far(base + plane + offset[i] + column, to);
     }
     static __device__ __forceinline__ void copy_to_lds_far(const char *at, uint32_t lds_byte) {
         uint32_t saved_m0;
@@ -131,19 +127,15 @@ struct Across {
         row = tid / PIECES;
         column = min((tid % PIECES ^ 4 * (row % 4)) * 8, s.columns - 8 - column0) * 2;
     }
-    __device__ __forceinline__ void begin(int step, uint32_t lds) const {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 1024);
-        // the step's rows lie within 32 bits of its first one
-        const int first = step * K;
+    // the thread's i-th piece of a step
+    __device__ __forceinline__ void begin(int step, uint32_t lds, int i) const {
+        const uint32_t to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 1024) + i * THREADS * 16;
+        // the step's rows lie within 32 bits of its first one (a step that is behind the last row reads that)
+        const int first = min(step * K, last_row), r = row + i * (THREADS / PIECES);
         const char *from = base + first * stride;
-#pragma unroll
-        for (int i = 0; i < SHARE; ++i) {
-            const int r = row + i * (THREADS / PIECES);
-            // (a plane's rows are a multiple of the rows that a pass of all threads takes: uniform)
-            const char *const of = PLANES == 2 && i * (THREADS / PIECES) >= K ? from + plane : from;
-            const int in_plane = PLANES == 2 && i * (THREADS / PIECES) >= K ? r - K : r;
-            copy_to_lds(of, uint32_t(min(in_plane, last_row - first) * stride) + column, lds + wave + i * THREADS * 16);
-        }
+        // (a plane's rows are a multiple of the rows that a pass of all threads takes: uniform)
+        const bool second = PLANES == 2 && i * (THREADS / PIECES) >= K;
+        copy_to_lds(second ? from + plane : from, uint32_t(min(second ? r - K : r, last_row - first) * (int)stride) + column, to);
     }
     struct Reader {
         uint32_t at[4];           // by d % 4
@@ -180,71 +172,106 @@ struct Sums {
     }
 };
 
-// Adds the products of steps first .. end - 1.  lds: two buffers of (A's + B's words) each.  of_b(operand) is shown B's operands.
-template <typename F, int MB, int NB, typename A, typename B, typename OfB>
-__device__ __forceinline__ void multiply(Sums<MB, NB> &sums, const A &a, const B &b, const typename A::Reader &ra, const typename B::Reader &rb, uint32_t lds, int first,
-                                         int end, OfB &&of_b) {
-    constexpr uint32_t BUFFER = (A::WORDS + B::WORDS) * 16;
-    if (first >= end) return;
-    a.begin(first, lds);
-    b.begin(first, lds + A::WORDS * 16);
-    uint32_t now = lds;
-    for (int s = first; s < end; ++s) {
-        arrived();
-        __syncthreads();                  // everyone's copies are there, and nobody reads the other buffer any more
-        const uint32_t next = lds + (now == lds ? BUFFER : 0);
-        if (s + 1 < end) {
-            a.begin(s + 1, next);
-            b.begin(s + 1, next + A::WORDS * 16);
-        }
-        if constexpr (F::PLANES == 1) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint4 fa[MB], fb[NB];
-#pragma unroll
-                for (int i = 0; i < MB; ++i) fa[i] = ra.operand(now, i, c);
-#pragma unroll
-                for (int j = 0; j < NB; ++j) fb[j] = rb.operand(now + A::WORDS * 16, j, c);
-#pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    of_b(j, fb[j]);
-#pragma unroll
-                    for (int i = 0; i < MB; ++i) sums.v[i][j] = F::mma(fa[i], fb[j], sums.v[i][j]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint4 fa[2][MB], fb[2][NB];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-#pragma unroll
-                    for (int i = 0; i < MB; ++i) fa[p][i] = ra.operand(now, i, 2 * p + c);
-#pragma unroll
-                    for (int j = 0; j < NB; ++j) fb[p][j] = rb.operand(now + A::WORDS * 16, j, 2 * p + c);
-                }
-#pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    of_b(j, fb[1][j]);
-                    of_b(j, fb[0][j]);
-                }
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-#pragma unroll
-                    for (int i = 0; i < MB; ++i) sums.v[i][j] = F::mma(fa[1][i], fb[0][j], sums.v[i][j]);
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-#pragma unroll
-                    for (int i = 0; i < MB; ++i) sums.v[i][j] = F::mma(fa[0][i], fb[1][j], sums.v[i][j]);
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-#pragma unroll
-                    for (int i = 0; i < MB; ++i) sums.v[i][j] = F::mma(fa[0][i], fb[0][j], sums.v[i][j]);
-            }
-        }
-        now = next;
+// The products of one tile after the other.  The steps of all tiles are one stream: while a step's products are formed the next one is there, and the one behind it is on its way, also where
+// it is the next tile's, so that neither a tile's first copies nor what becomes of its results leave the matrix cores without operands.  In a step four chunks of operands are read from
+// LDS, each while the products of the chunk before are formed; with the last one in registers the buffer is free: the one barrier of a step stands there, before the last chunk's products.
+// Every tile has at least two steps.
+template <typename F, int MB, int NB, typename A, typename B>
+struct Stream {
+    static constexpr uint32_t OF_B = A::WORDS * 16, BUFFER = (A::WORDS + B::WORDS) * 16, LDS = 2 * BUFFER;
+    const typename A::Reader ra;
+    const typename B::Reader rb;
+    uint32_t now, other;                 // buffers: of the step that is next to be multiplied, and of the one behind it
+
+    __device__ __forceinline__ Stream(uint32_t lds, int row_a, int row_b) : ra(row_a), rb(row_b), now(lds), other(lds + BUFFER) {}
+
+    static constexpr int COPIES = A::SHARE + B::SHARE, READS = MB + NB, PRODUCTS = MB * NB;
+    static __device__ __forceinline__ void copy(const A &a, const B &b, int step, uint32_t buffer, int n) {
+        if (n < A::SHARE) a.begin(step, buffer, n);
+        else b.begin(step, buffer + OF_B, n - A::SHARE);
     }
-    __syncthreads();                      // the buffers are free
-}
+    static __device__ __forceinline__ void copy(const A &a, const B &b, int step, uint32_t buffer) {
+#pragma unroll
+        for (int n = 0; n < COPIES; ++n) copy(a, b, step, buffer, n);
+    }
+    // the first tile's first two steps
+    __device__ __forceinline__ void prime(const A &a, const B &b, int first) const {
+        copy(a, b, first, now);
+        copy(a, b, first + 1, other);
+        arrived();
+        __syncthreads();
+    }
+    // Nothing is on its way any more, and nobody reads the buffers.
+    static __device__ __forceinline__ void done() {
+        arrived();
+        __syncthreads();
+    }
+    // Adds the products of steps first .. end - 1 of (of_a, of_b); behind them those from next_first of (next_a, next_b) are brought, which become of_a and of_b (behind the last tile
+    // any steps that can be read, and done()).  seen(j, operand) is shown B's operands.
+    template <typename Seen>
+    __device__ __forceinline__ void multiply(Sums<MB, NB> &sums, A &of_a, B &of_b, int first, int end, const A &next_a, const B &next_b, int next_first, Seen &&seen) {
+        // chunk c: of one plane, numbers 16 c .. of both; of two, numbers 16 (c / 2) .., of A the second terms and then the first, of B the first and then the second
+        constexpr bool TWO = F::PLANES == 2;
+        uint4 fa[2][MB], fb[2][NB];
+        // the n-th read of a chunk's operands, in the order in which the products want them
+        auto read = [&](uint32_t buffer, int c, int n) {
+            const int part_a = TWO ? (c % 2 == 0 ? 2 : 0) + c / 2 : c, part_b = TWO ? (c % 2 == 0 ? 0 : 2) + c / 2 : c;
+            if (n == 0) fb[c % 2][0] = rb.operand(buffer + OF_B, 0, part_b);
+            else if (n <= MB) fa[c % 2][n - 1] = ra.operand(buffer, n - 1, part_a);
+            else fb[c % 2][n - MB] = rb.operand(buffer + OF_B, n - MB, part_b);
+        };
+        auto read_all = [&](uint32_t buffer, int c) {
+#pragma unroll
+            for (int n = 0; n < READS; ++n) read(buffer, c, n);
+        };
+        // a chunk's products, between(n) behind the n-th; nothing is moved across
+        auto form = [&](int c, auto &&between) {
+#pragma unroll
+            for (int n = 0; n < PRODUCTS; ++n) {
+                const int i = n % MB, j = n / MB;
+                if (i == 0) seen(j, fb[c % 2][j]);
+                sums.v[i][j] = F::mma(fa[c % 2][i], fb[c % 2][j], sums.v[i][j]);
+                between(n);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // of two planes, the product of both first terms: B's are those of the chunk before, whose place the next chunk's take
+        auto form_first = [&](int c) {
+            if (TWO && c % 2 == 1) {
+#pragma unroll
+                for (int n = 0; n < PRODUCTS; ++n) sums.v[n % MB][n / MB] = F::mma(fa[1][n % MB], fb[0][n / MB], sums.v[n % MB][n / MB]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        read_all(now, 0);
+        int ahead = 2;
+        for (int s = first; s < end; ++s) {
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                form_first(c);
+                form(c, [&](int n) {
+#pragma unroll
+                    for (int r = n * READS / PRODUCTS; r < (n + 1) * READS / PRODUCTS; ++r) read(now, c + 1, r);
+                });
+            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");       // the next step is there, and nobody reads this one any more
+            form_first(3);
+            if (s + 2 == end) {
+                of_a = next_a;
+                of_b = next_b;
+                ahead = next_first - end + 2;
+            }
+            form(3, [&](int n) {
+#pragma unroll
+                for (int r = n * READS / PRODUCTS; r < (n + 1) * READS / PRODUCTS; ++r) read(other, 0, r);            // (behind the last step: read again later)
+#pragma unroll
+                for (int r = n * COPIES / PRODUCTS; r < (n + 1) * COPIES / PRODUCTS; ++r) copy(of_a, of_b, s + ahead, now, r);
+            });
+            const uint32_t swap = now;
+            now = other;
+            other = swap;
+        }
+    }
+};
 
 }  // namespace product_tiles
