@@ -36,12 +36,12 @@ struct Kept {
     int32_t *pos;       // [N]: where a token's row is among the labelled ones, or -1
     int32_t *label;     // [labelled]
     float2 *level;      // [labelled]: a token's largest logit, and one over the sum of the exponentials of what they are below it
-};
-int64_t kept_bytes(int64_t N) { return 16 + up(N * 4, 16) * 4; }
+};                      // (the last two up to a whole tile: tiles are read whole)
+int64_t kept_bytes(int64_t N) { return 16 + up(N * 4, 16) + up(N, TILE) * 12; }
 Kept kept_at(void *at, int64_t N) {
     char *p = static_cast<char *>(at);
-    const int64_t n = up(N * 4, 16);
-    return {reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + 16), reinterpret_cast<int32_t *>(p + 16 + n), reinterpret_cast<float2 *>(p + 16 + 2 * n)};
+    const int64_t n = up(N * 4, 16), tiles = up(N, TILE);
+    return {reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + 16), reinterpret_cast<int32_t *>(p + 16 + n), reinterpret_cast<float2 *>(p + 16 + n + tiles * 4)};
 }
 
 struct Sizes {
@@ -255,17 +255,45 @@ struct Place {
 typedef Along<TILE, THREADS, 1> AlongOne;
 constexpr uint32_t STREAM_LDS = Stream<F16, MB, NB, AlongOne, AlongOne>::LDS;      // (of any operands)
 
-// The logits of one tile after the other: entries from v0 on, in all `width`, and the labelled tokens; each(sums, place) has the sums of a tile's products.
-template <typename F, typename Each>
-__device__ __forceinline__ void for_logits(const Operands &o, int labelled, int v0, int width, uint32_t lds, Each &&each) {
+// What a tile's logits become takes numbers of its entries and its tokens: 1 KB of each, brought to LDS with the tile's first step, a wavefront a kilobyte, two tiles' places in turn.  Loads
+// from memory would return behind the next tile's copies and be waited for as long.
+enum Beside { BIAS, LABEL, WEIGHT_SCALE, ROW_SCALE, LEVEL, LEVEL_END = LEVEL + 2, COEFFICIENT = LEVEL_END, BESIDES };
+constexpr uint32_t BESIDE_BYTES = BESIDES * 1024;
+static_assert(TILE == 256 && BESIDES <= THREADS / 64, "a wavefront's copy is one array's share of a tile");
+
+template <bool BACKWARD>
+__device__ __forceinline__ void bring_beside(const Operands &o, const float *coefficient, int v0, int n0, uint32_t lds) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const void *from = nullptr;
+    if (wave == BIAS) from = o.bias + v0;
+    else if (wave == LABEL) from = o.kept.label + n0;
+    else if (wave == WEIGHT_SCALE && o.weight_scale) from = o.weight_scale + v0;
+    else if (wave == ROW_SCALE && !BACKWARD && o.row_scale) from = o.row_scale + n0;
+    else if (BACKWARD && wave >= LEVEL && wave < LEVEL_END) from = o.kept.level + n0 + (wave - LEVEL) * 128;
+    else if (BACKWARD && wave == COEFFICIENT && coefficient) from = coefficient + n0;
+    if (from) copy_to_lds((const char *)uniform((uint64_t)from), threadIdx.x % 64 * 16, lds + wave * 1024);
+}
+template <typename T>
+__device__ __forceinline__ T beside(uint32_t lds, Beside of, int at) {
+    typedef uint32_t words_t __attribute__((ext_vector_type(sizeof(T) / 4)));
+    return __builtin_bit_cast(T, *(const __attribute__((address_space(3))) words_t *)(uintptr_t)(lds + of * 1024 + at * sizeof(T)));
+}
+
+// The logits of one tile after the other: entries from v0 on, in all `width`, and the labelled tokens; each(sums, place, lds) has the sums of a tile's products, of one plane with the bias, and
+// what came beside it, and calls landed() before it stores anything.
+template <typename F, bool BACKWARD, typename Each>
+__device__ __forceinline__ void for_logits(const Operands &o, const float *coefficient, int labelled, int v0, int width, uint32_t lds, Each &&each) {
     typedef Along<TILE, THREADS, F::PLANES> Side;
-    const int wave = threadIdx.x / 64, vt = (width + TILE - 1) / TILE, nt = (labelled + TILE - 1) / TILE, steps = max(2, (o.s.K + Side::K - 1) / Side::K);
+    const int wave = threadIdx.x / 64, half = threadIdx.x % 64 / 32, vt = (width + TILE - 1) / TILE, nt = (labelled + TILE - 1) / TILE;
+    const int steps = max(2, (o.s.K + Side::K - 1) / Side::K);
     Turns turns(vt * nt);
     if (!turns.any()) return;
     const Source rows = rows_of(o, labelled);
     Place place(turns.at, vt, nt);
     Side a(o.weight, v0 + place.v), b(rows, place.n);
     Stream<F, MB, NB, Side, Side> stream(lds, wave / WAVES_N * MB * 32, wave % WAVES_N * NB * 32);
+    uint32_t by = lds + STREAM_LDS, next_by = by + BESIDE_BYTES;
+    bring_beside<BACKWARD>(o, coefficient, v0 + place.v, place.n, by);
     stream.prime(a, b, 0);
     for (;;) {
         const int next = turns.at + turns.step;
@@ -273,26 +301,41 @@ __device__ __forceinline__ void for_logits(const Operands &o, int labelled, int 
         const Place then(more ? next : turns.at, vt, nt);
         const Side next_a(o.weight, v0 + then.v), next_b(rows, then.n);
         Sums<MB, NB> sums;
-        sums.clear();
-        stream.multiply(sums, a, b, 0, steps, next_a, next_b, 0, [](int, const uint4 &) {});
-        each(sums, place);
+        if constexpr (F::PLANES == 1) {
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float4 bias = beside<float4>(by, BIAS, (wave / WAVES_N * MB + i) * 8 + 2 * g + half);
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+                        sums.v[i][j][4 * g] = bias.x, sums.v[i][j][4 * g + 1] = bias.y, sums.v[i][j][4 * g + 2] = bias.z, sums.v[i][j][4 * g + 3] = bias.w;
+                }
+        } else
+            sums.clear();
+        stream.multiply(sums, a, b, 0, steps, next_a, next_b, 0, [](int, const uint4 &) {},
+                        [&] { bring_beside<BACKWARD>(o, coefficient, v0 + then.v, then.n, next_by); });
+        each(sums, place, by);
         if (!more) break;
         turns.at = next, place = then;
+        const uint32_t swap = by;
+        by = next_by;
+        next_by = swap;
     }
     stream.done();
 }
 
-// The logits of the tile's 16 entries of block i for the token of block j: l[e] of entry mfma_row(e, half)
+// The logits of block i's 16 entries, `row` of the tile's first of them, for a token: l[e] of entry mfma_row(e, half).
 template <typename F>
-__device__ __forceinline__ void with_bias(float (&l)[16], const f32x16_t &sum, const Operands &o, int v, float row_scale) {
+__device__ __forceinline__ void logits_of(float (&l)[16], const f32x16_t &sum, uint32_t lds, int row, float row_scale) {
     const int half = threadIdx.x % 64 / 32;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const float4 b = *reinterpret_cast<const float4 *>(o.bias + v + 8 * g + 4 * half);
         if constexpr (F::PLANES == 1) {
-            l[4 * g] = sum[4 * g] + b.x, l[4 * g + 1] = sum[4 * g + 1] + b.y, l[4 * g + 2] = sum[4 * g + 2] + b.z, l[4 * g + 3] = sum[4 * g + 3] + b.w;
+#pragma unroll
+            for (int e = 4 * g; e < 4 * g + 4; ++e) l[e] = sum[e];
         } else {
-            const float4 w = *reinterpret_cast<const float4 *>(o.weight_scale + v + 8 * g + 4 * half);
+            const float4 b = beside<float4>(lds, BIAS, row / 4 + 2 * g + half), w = beside<float4>(lds, WEIGHT_SCALE, row / 4 + 2 * g + half);
             l[4 * g] = fmaf(sum[4 * g] * w.x, row_scale, b.x), l[4 * g + 1] = fmaf(sum[4 * g + 1] * w.y, row_scale, b.y);
             l[4 * g + 2] = fmaf(sum[4 * g + 2] * w.z, row_scale, b.z), l[4 * g + 3] = fmaf(sum[4 * g + 3] * w.w, row_scale, b.w);
         }
@@ -315,22 +358,21 @@ template <typename F>
 __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
     const uint32_t lds = lds_byte_of(lds_words);
-    float2 *const halves = reinterpret_cast<float2 *>(reinterpret_cast<char *>(lds_words) + STREAM_LDS);     // [WAVES_M][TILE]
+    float2 *const halves = reinterpret_cast<float2 *>(reinterpret_cast<char *>(lds_words) + STREAM_LDS + 2 * BESIDE_BYTES);     // [WAVES_M][TILE]
     const Operands &o = a.o;
     const int labelled = o.kept.head[0], tid = threadIdx.x, wave = tid / 64, lane = tid % 64, half = lane / 32;
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-    for_logits<F>(o, labelled, 0, o.s.V, lds, [&](const Sums<MB, NB> &sums, const Place &p) {
-        const int v0 = p.v + wm * MB * 32;
+    for_logits<F, false>(o, nullptr, labelled, 0, o.s.V, lds, [&](const Sums<MB, NB> &sums, const Place &p, uint32_t by) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int column = wn * NB * 32 + j * 32 + lane % 32, n = p.n + column;
-            const float row_scale = F::PLANES == 2 ? o.row_scale[n] : 1.f;
-            const int at = n < labelled ? o.kept.label[n] - v0 : -1;
+            const float row_scale = F::PLANES == 2 ? beside<float>(by, ROW_SCALE, column) : 1.f;
+            const int at = n < labelled ? beside<int>(by, LABEL, column) - p.v - wm * MB * 32 : -1;
             float2 of = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 float l[16];
-                with_bias<F>(l, sums.v[i][j], o, v0 + 32 * i, row_scale);
+                logits_of<F>(l, sums.v[i][j], by, (wm * MB + i) * 32, row_scale);
                 float most = of.x;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) most = fmaxf(most, l[e]);
@@ -344,12 +386,14 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
                     float found = l[0];
 #pragma unroll
                     for (int e = 1; e < 16; ++e) found = mfma_row(e, half) == r ? l[e] : found;
+                    arrived();
                     a.at_label[n] = found;
                 }
             }
             const float2 other = make_float2(__shfl_xor(of.x, 32), __shfl_xor(of.y, 32));
             if (half == 0) halves[wm * TILE + column] = joined(of, other);
         }
+        arrived();
         __syncthreads();
         if (tid < TILE) a.parts[p.v / TILE * a.Np + p.n + tid] = joined(halves[tid], halves[TILE + tid]);
         // (the next tile's products have barriers before halves is written again)
@@ -473,25 +517,32 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
     const int labelled = o.kept.head[0], wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N;
     const Piece p = piece_of<F>(a, labelled, piece);
     const float scale = F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : 1.f;
-    for_logits<F>(o, labelled, p.v0, p.width, lds, [&](const Sums<MB, NB> &sums, const Place &tile) {
-        const int in = tile.v + wm * MB * 32, v0 = p.v0 + in;
+    for_logits<F, true>(o, a.coefficient, labelled, p.v0, p.width, lds, [&](const Sums<MB, NB> &sums, const Place &tile, uint32_t beside_) {
+        const int in = tile.v + wm * MB * 32;
+        bool stored = false;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const int n = tile.n + wn * NB * 32 + j * 32 + lane % 32;
+            const int column = wn * NB * 32 + j * 32 + lane % 32, n = tile.n + column;
             const bool live = n < labelled;
-            const float2 level = live ? o.kept.level[n] : make_float2(0.f, 0.f);
-            const float by = live ? LIFT * (a.coefficient ? a.coefficient[n] : 1.f) : 0.f;
-            const int at = live ? o.kept.label[n] - v0 : -1;
+            // (a token behind the last: exponentials of minus infinity, times zero)
+            const float2 level = live ? beside<float2>(beside_, LEVEL, column) : make_float2(INFINITY, 0.f);
+            const float by = LIFT * (a.coefficient ? beside<float>(beside_, COEFFICIENT, column) : 1.f), p_by = live ? level.y * by : 0.f;
+            const int at = live ? beside<int>(beside_, LABEL, column) - p.v0 - in : -1;
             char *const row = a.d + (int64_t(n) * p.ld + in) * 2;
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 float l[16];
-                with_bias<F>(l, sums.v[i][j], o, v0 + 32 * i, scale);
-                const int r = at - 32 * i;
+                logits_of<F>(l, sums.v[i][j], beside_, (wm * MB + i) * 32, scale);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float q = __builtin_amdgcn_exp2f((l[e] - level.x) * LOG2E);
-                    l[e] = live ? fmaf(q, level.y, mfma_row(e, half) == r ? -1.f : 0.f) * by : 0.f;
+                for (int e = 0; e < 16; ++e) l[e] = __builtin_amdgcn_exp2f((l[e] - level.x) * LOG2E) * p_by;
+                const int r = at - 32 * i;
+                if (r >= 0 && r < 32 && r / 4 % 2 == half) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) l[e] -= mfma_row(e, half) == r ? by : 0.f;
+                }
+                if (!stored) {
+                    arrived();
+                    stored = true;
                 }
                 auto put = [&](char *to) {
 #pragma unroll
@@ -578,7 +629,8 @@ __device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece 
         const Right next_right(w, then.h);
         Sums<MB, NB> sums;
         sums.clear();
-        stream.multiply(sums, left, right, task.first, task.end, next_left, next_right, then.first, [](int, const uint4 &) {});
+        stream.multiply(sums, left, right, task.first, task.end, next_left, next_right, then.first, [](int, const uint4 &) {}, [] {});
+        stream.landed();
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int h = task.h + (wave % WAVES_N * NB + j) * 32 + lane % 32;
@@ -628,7 +680,8 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
         if (steps)
             stream.multiply(sums, left, right, 0, steps, next_left, next_right, 0, [&](int j, const uint4 &u) {
                 if (of_bias) bias[j] = dot_ones(F(), u, bias[j]);
-            });
+            }, [] {});
+        stream.landed();
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int in = v0 + (wn * NB + j) * 32 + lane % 32, v = p.v0 + in;
@@ -817,7 +870,7 @@ void launch_rows(const lffn_linear_cross_entropy &a, const RowsArgs &r, hipStrea
 
 unsigned workgroups(int64_t tiles) { return unsigned(tiles >= COMPUTE_UNITS ? COMPUTE_UNITS : up(tiles, XCDS)); }
 
-constexpr size_t LDS_BYTES = STREAM_LDS + WAVES_M * TILE * sizeof(float2);
+constexpr size_t LDS_BYTES = STREAM_LDS + 2 * BESIDE_BYTES + WAVES_M * TILE * sizeof(float2);
 
 template <typename F>
 int forward(const Forward &f, hipStream_t st) {

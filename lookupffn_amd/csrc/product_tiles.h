@@ -201,15 +201,18 @@ struct Stream {
         arrived();
         __syncthreads();
     }
+    static __device__ __forceinline__ void landed() { arrived(); }
     // Nothing is on its way any more, and nobody reads the buffers.
     static __device__ __forceinline__ void done() {
         arrived();
         __syncthreads();
     }
     // Adds the products of steps first .. end - 1 of (of_a, of_b); behind them those from next_first of (next_a, next_b) are brought, which become of_a and of_b (behind the last tile
-    // any steps that can be read, and done()).  seen(j, operand) is shown B's operands.
-    template <typename Seen>
-    __device__ __forceinline__ void multiply(Sums<MB, NB> &sums, A &of_a, B &of_b, int first, int end, const A &next_a, const B &next_b, int next_first, Seen &&seen) {
+    // any steps that can be read, and done()).  seen(j, operand) is shown B's operands; beside() is called once, for copies that come with the next tile's first step.  Between two tiles the
+    // caller waits (landed) for what is on its way, before it stores anything: the second tile's first step does not wait, so that the stores have that long.
+    template <typename Seen, typename Beside>
+    __device__ __forceinline__ void multiply(Sums<MB, NB> &sums, A &of_a, B &of_b, int first, int end, const A &next_a, const B &next_b, int next_first, Seen &&seen,
+                                             Beside &&beside) {
         // chunk c: of one plane, numbers 16 c .. of both; of two, numbers 16 (c / 2) .., of A the second terms and then the first, of B the first and then the second
         constexpr bool TWO = F::PLANES == 2;
         uint4 fa[2][MB], fb[2][NB];
@@ -254,12 +257,14 @@ struct Stream {
                     for (int r = n * READS / PRODUCTS; r < (n + 1) * READS / PRODUCTS; ++r) read(now, c + 1, r);
                 });
             }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");       // the next step is there, and nobody reads this one any more
+            if (s > first) arrived();
+            lds_barrier();                       // the next step is there, and nobody reads this one any more
             form_first(3);
             if (s + 2 == end) {
                 of_a = next_a;
                 of_b = next_b;
                 ahead = next_first - end + 2;
+                beside();
             }
             form(3, [&](int n) {
 #pragma unroll

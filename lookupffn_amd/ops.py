@@ -1740,7 +1740,7 @@ def _linear_cross_entropy_args(hidden, weight, bias, labels, ignore_index, reduc
 
 def _loss_kept_bytes(tokens):
     """lffn_linear_cross_entropy_kept_bytes: how many tokens have a label, where a token is among them, and of those the label and two levels."""
-    return 16 + (tokens * 4 + 15) // 16 * 16 * 4
+    return 16 + (tokens * 4 + 15) // 16 * 16 + (tokens + 255) // 256 * 256 * 12
 
 
 _L.define("linear_cross_entropy(Tensor hidden, Tensor weight, Tensor? bias, Tensor labels, int ignore_index, int reduction, bool keep) -> (Tensor, Tensor)")
