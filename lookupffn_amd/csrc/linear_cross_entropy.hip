@@ -24,7 +24,7 @@ constexpr int CHUNK = 64, PARTS = 4;            // tokens whose places a workgro
 constexpr int COUNTED_FROM = 4096;              // tokens from which on a launch of its own counts the labelled ones of every chunk
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LIFT = 16384.f;                 // d times 2^14: half's normal numbers then reach down to 2^-28 of a row's largest
-constexpr int64_t D_BYTES = int64_t(512) << 20; // of a piece's d, at most (few, large pieces: with many tokens 2048 entries at least)
+constexpr int64_t D_BYTES = int64_t(1) << 30;   // of a piece's d, at most (with many tokens 2048 entries at least)
 constexpr int64_t PARTS_BYTES = int64_t(256) << 20;
 constexpr int SHARES = 64;                      // of the vocabulary, for dh, at most
 
@@ -458,14 +458,19 @@ struct BackwardArgs {
     const float *g_loss;       // [1] or [N]
     float *coefficient;        // [labelled] or null: what d is multiplied with beside `factor`
     float *power;              // [1]: of both gradients, where there are coefficients
+    int32_t *shares;           // [1]
     void *grad_hidden, *grad_weight, *grad_bias;
     int32_t bias_format, reduction, pieces;
 };
 
+// Entries of a piece, whole tiles, that fit so many bytes.  d's rows are some more apart: rows at a distance of a power of two would share few of the cache's channels.
+constexpr int APART = 64;
+__host__ __device__ constexpr int64_t widest(int64_t bytes, int64_t rows, int planes) { return (bytes / (rows * 2 * planes) - APART) / TILE * TILE; }
+
 // How a piece is laid out, from the number of labelled tokens, alike in every launch.
 struct Piece {
-    int v0, width, ld, nt;     // entries, numbers of d's rows, tiles of tokens
-    int shares, share;         // of dh's sum over the piece's entries; of steps, an even number, each: the piece's own
+    int v0, width, ld, nt;     // entries; numbers from row to row of d; tiles of tokens
+    int steps;                 // of dh's sum over the entries of a whole piece
 };
 template <typename F>
 __device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, int piece) {
@@ -473,16 +478,45 @@ __device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, i
     Piece p;
     p.nt = (labelled + TILE - 1) / TILE;
     const int64_t rows = max(p.nt, 1) * int64_t(TILE);
-    p.ld = (int)min(a.o.s.Vp, max(int64_t(TILE), a.d_bytes / (rows * 2 * F::PLANES) / TILE * TILE));
-    const int64_t first = int64_t(piece) * p.ld;
-    p.v0 = (int)min(first, int64_t(a.o.s.V));
-    p.width = min(p.ld, a.o.s.V - p.v0);
-    // a share's sum is about as long as one over the tokens, so that tasks are alike; no piece has more than the first
-    const int steps = (min(p.ld, a.o.s.V) + K - 1) / K, most = (int)min(int64_t(SHARES), a.parts_bytes / (max(labelled, 1) * int64_t(a.o.s.K) * 4));
-    const int shares = max(1, min(most, steps / max(16, (labelled + K - 1) / K)));
-    p.share = (steps + 2 * shares - 1) / (2 * shares) * 2;
-    p.shares = ((p.width + K - 1) / K + p.share - 1) / p.share;
+    const int tiles = int(a.o.s.Vp / TILE), most = (int)min(int64_t(tiles), widest(a.d_bytes, rows, F::PLANES) / TILE);
+    const int pieces = (tiles + most - 1) / most, whole = (tiles + pieces - 1) / pieces * TILE;            // as few as fit, and all alike
+    p.ld = whole + APART;
+    p.v0 = (int)min(int64_t(piece) * whole, int64_t(a.o.s.V));
+    p.width = min(whole, a.o.s.V - p.v0);
+    p.steps = (min(whole, a.o.s.V) + K - 1) / K;
     return p;
+}
+
+// A piece's tasks on the compute units: tiles of dW, steps_w steps each, go round, and the `more` first compute units have one more than the others; dh's tiles, whose sums over the
+// entries can be cut anywhere, fill up: all compute units take `all` of its tasks, steps_h steps each, and those with a tile less of dW go on to `some`.
+struct Balance {
+    int more, all, some, length;
+    __device__ __forceinline__ Balance(int weight_tasks, int steps_w, int hidden_tasks, int steps_h) {
+        more = weight_tasks % COMPUTE_UNITS;
+        length = INT32_MAX;
+        for (int less = steps_w / steps_h, last = less + 1; less <= last; ++less) {       // tasks that a tile of dW is worth
+            int s = (hidden_tasks + more * less + COMPUTE_UNITS - 1) / COMPUTE_UNITS, a = s - less;
+            if (a < 0) a = 0, s = (hidden_tasks + COMPUTE_UNITS - more - 1) / (COMPUTE_UNITS - more);
+            const int l = max(s * steps_h, a * steps_h + (more ? steps_w : 0));
+            if (l < length) length = l, all = a, some = s;
+        }
+    }
+};
+
+// Into how many shares of the vocabulary dh's sums are cut, by how long a piece's launch takes and what the shares cost in memory; lane i looks at i + 1.  A step of all compute units takes
+// 2.1 us, memory moves 5.1 TB/s.  (4915 labelled tokens, 50265 x 512: 9 shares are 253 steps, 10 in whole rounds were 314.)
+template <typename F>
+__device__ __forceinline__ int shares_of(const BackwardArgs &a, int labelled) {
+    constexpr int K = STEP / F::PLANES;
+    const Piece p = piece_of<F>(a, labelled, 0);
+    const int ht = (a.o.s.K + TILE - 1) / TILE, fit = (int)min(int64_t(SHARES), a.parts_bytes / (max(labelled, 1) * int64_t(a.o.s.K) * 4));
+    const int n = threadIdx.x % 64 + 1, share = (p.steps + 2 * n - 1) / (2 * n) * 2, shares = (p.steps + share - 1) / share;
+    const Balance b((p.width + TILE - 1) / TILE * ht, (labelled + K - 1) / K, shares * p.nt * ht, share);      // (whether or not dW is wanted: the same bits)
+    const float cost = n > max(1, fit) ? INFINITY : b.length + shares * (float)labelled * a.o.s.K * 7.5e-7f;
+    float least = cost;
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) least = fminf(least, __shfl_xor(least, m));
+    return __ffsll((unsigned long long)__ballot(cost == least));
 }
 
 // What both gradients' sums are multiplied with: of a sum or mean what all tokens' d are, else the power of two that their coefficients were divided by.
@@ -567,6 +601,11 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
             }
         }
     });
+    // (one of the workgroups that have the fewest tiles)
+    if (piece == 0 && blockIdx.x == gridDim.x - 1 && wave == 0) {
+        const int shares = shares_of<F>(a, labelled);
+        if (lane == 0) *a.shares = shares;
+    }
 }
 
 __device__ __forceinline__ float dot_ones(BF16, uint4 u, float sum) {
@@ -598,7 +637,7 @@ __device__ __forceinline__ void store8(char *to, const float (&v)[8]) {
 
 // dh: shares of the piece's entries x tiles of tokens x tiles of columns, one after the other; each adds to its own part.
 template <typename F>
-__device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece &p, int labelled, bool first_piece, uint32_t lds) {
+__device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece &p, int labelled, int piece, int unit, uint32_t lds) {
     typedef Along<TILE, THREADS, F::PLANES> Left;
     typedef Across<TILE, THREADS, F::PLANES> Right;
     const Operands &o = a.o;
@@ -610,21 +649,30 @@ __device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece 
     struct Task {
         int share, n, h, first, end;
         // (d has zeros behind the piece's last entry, up to a whole tile: an odd number of steps is followed by one of them)
-        __device__ __forceinline__ Task(int id, const Piece &p, int ht, int steps)
-            : share(id / ht / p.nt), n(id / ht % p.nt * TILE), h(id % ht * TILE), first(share * p.share), end(min((steps + 1) / 2 * 2, first + p.share)) {}
+        __device__ __forceinline__ Task(int id, const Piece &p, int ht, int length, int steps)
+            : share(id / ht / p.nt), n(id / ht % p.nt * TILE), h(id % ht * TILE), first(share * length), end(min((steps + 1) / 2 * 2, first + length)) {}
     };
-    const int steps = (p.width + Left::K - 1) / Left::K;
-    Turns turns(p.shares * p.nt * ht);
-    if (!turns.any()) return;
-    Task task(turns.at, p, ht, steps);
+    // shares of an even number of steps, alike in all pieces; the last piece may have fewer
+    const int wanted = *a.shares, length = (p.steps + 2 * wanted - 1) / (2 * wanted) * 2, steps = (p.width + Left::K - 1) / Left::K;
+    const int tasks = (steps + length - 1) / length * p.nt * ht;
+    const Balance balance(a.grad_weight ? (p.width + TILE - 1) / TILE * ht : 0, (labelled + Left::K - 1) / Left::K, tasks, length);
+    const int rounds = unit < balance.more ? balance.all : balance.some;
+    // a compute unit's round-th task: neighbours take neighbouring ones
+    auto id_of = [&](int round) {
+        return round < balance.all ? round * COMPUTE_UNITS + unit
+                                   : balance.all * COMPUTE_UNITS + (round - balance.all) * (COMPUTE_UNITS - balance.more) + unit - balance.more;
+    };
+    if (rounds == 0 || id_of(0) >= tasks) return;
+    int round = 0;
+    Task task(id_of(0), p, ht, length, steps);
     Left left(d, task.n);
     Right right(w, task.h);
     Stream<F, MB, NB, Left, Right> stream(lds, wave / WAVES_N * MB * 32, wave % WAVES_N * NB * 32);
     stream.prime(left, right, task.first);
     for (;;) {
-        const int next = turns.at + turns.step;
-        const bool more = next < turns.end;
-        const Task then(more ? next : turns.at, p, ht, steps);
+        const int next = id_of(round + 1);
+        const bool more = round + 1 < rounds && next < tasks;
+        const Task then(more ? next : id_of(round), p, ht, length, steps);
         const Left next_left(d, then.n);
         const Right next_right(w, then.h);
         Sums<MB, NB> sums;
@@ -642,19 +690,19 @@ __device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece 
                 for (int e = 0; e < 16; ++e) {
                     const int row = n + mfma_row(e, half);
                     float *const at = a.parts + (int64_t(task.share) * labelled + row) * o.s.K + h;
-                    if (row < labelled) *at = first_piece ? sums.v[i][j][e] : *at + sums.v[i][j][e];
+                    if (row < labelled) *at = piece == 0 ? sums.v[i][j][e] : *at + sums.v[i][j][e];
                 }
             }
         }
         if (!more) break;
-        turns.at = next, task = then;
+        ++round, task = then;
     }
     stream.done();
 }
 
 // dW: tiles of the piece's entries x tiles of columns, and, with the first columns, db.
 template <typename F, typename R>
-__device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece &p, int labelled, uint32_t lds) {
+__device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece &p, int labelled, int unit, uint32_t lds) {
     typedef Across<TILE, THREADS, F::PLANES> Side;
     const Operands &o = a.o;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N, ht = (o.s.K + TILE - 1) / TILE;
@@ -662,16 +710,16 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
     // (rows and d have zeros behind the last token, up to a whole tile)
     const int steps = labelled ? max(2, (labelled + Side::K - 1) / Side::K) : 0;
     const float factor = factor_of(a, labelled), by = F::PLANES == 2 ? factor * __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : factor;
-    Turns turns((p.width + TILE - 1) / TILE * ht);
-    if (!turns.any()) return;
-    int v0 = turns.at / ht * TILE, h0 = turns.at % ht * TILE;
+    const int tasks = (p.width + TILE - 1) / TILE * ht;
+    int task = unit;
+    if (task >= tasks) return;
+    int v0 = task / ht * TILE, h0 = task % ht * TILE;
     Side left(rows, h0), right(d, v0);
     Stream<F, MB, NB, Side, Side> stream(lds, wm * MB * 32, wn * NB * 32);
     if (steps) stream.prime(left, right, 0);
     for (;;) {
-        const int next = turns.at + turns.step;
-        const bool more = next < turns.end;
-        const int next_v = (more ? next : turns.at) / ht * TILE, next_h = (more ? next : turns.at) % ht * TILE;
+        const bool more = task + COMPUTE_UNITS < tasks;
+        const int next = more ? task + COMPUTE_UNITS : task, next_v = next / ht * TILE, next_h = next % ht * TILE;
         const Side next_left(rows, next_h), next_right(d, next_v);
         Sums<MB, NB> sums;
         sums.clear();
@@ -711,7 +759,7 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
                 }
         }
         if (!more) break;
-        turns.at = next, v0 = next_v, h0 = next_h;
+        task = next, v0 = next_v, h0 = next_h;
     }
     stream.done();
 }
@@ -724,8 +772,10 @@ __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, i
     const int labelled = a.o.kept.head[0];
     const Piece p = piece_of<F>(a, labelled, piece);
     if (p.width <= 0) return;
-    if (a.grad_hidden && labelled) hidden_tasks<F>(a, p, labelled, piece == 0, lds);
-    if (a.grad_weight) weight_tasks<F, R>(a, p, labelled, lds);
+    // (COMPUTE_UNITS workgroups; the units of an XCD have neighbouring numbers)
+    const int unit = blockIdx.x % XCDS * (COMPUTE_UNITS / XCDS) + blockIdx.x / XCDS;
+    if (a.grad_hidden && labelled) hidden_tasks<F>(a, p, labelled, piece, unit, lds);
+    if (a.grad_weight) weight_tasks<F, R>(a, p, labelled, unit, lds);
 }
 
 // dh: a labelled token's shares added up, zeros for the others.
@@ -737,7 +787,7 @@ __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
     const int at = a.o.kept.pos[t], labelled = a.o.kept.head[0];
     float v[8] = {};
     if (at >= 0) {
-        const int shares = piece_of<F>(a, labelled, 0).shares;
+        const int steps = piece_of<F>(a, labelled, 0).steps, wanted = *a.shares, length = (steps + 2 * wanted - 1) / (2 * wanted) * 2, shares = (steps + length - 1) / length;
 #pragma unroll 8
         for (int p = 0; p < shares; ++p) {
             const float *from = a.parts + (int64_t(p) * labelled + at) * s.K + c;
@@ -835,7 +885,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     const int64_t Np = up(a.tokens, TILE), planes = planes_of(a), K = a.columns;
     BackwardArgs &b = w.b;
     b.o = operands(a, c);
-    const int64_t Vp = b.o.s.Vp, least = Np * (Vp < 2048 ? Vp : 2048) * 2 * planes, whole = Np * Vp * 2 * planes;
+    const int64_t Vp = b.o.s.Vp, least = Np * ((Vp < 2048 ? Vp : 2048) + APART) * 2 * planes, whole = Np * (Vp + APART) * 2 * planes;
     b.d_bytes = least > D_BYTES ? least : whole < D_BYTES ? whole : D_BYTES;
     b.d_plane = b.d_bytes / 2;
     b.d = c.take<char>(b.d_bytes);
@@ -844,10 +894,11 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     b.parts = c.take<float>(b.parts_bytes / 4);
     b.coefficient = c.take<float>(a.reduction == 0 ? Np : 0);
     b.power = c.take<float>(1);
+    b.shares = c.take<int32_t>(1);
     if (a.reduction != 0) b.coefficient = nullptr;
     // as many launches as pieces if all tokens are labelled; with fewer the last ones find nothing
-    const int64_t ld = b.d_bytes / (Np > 0 ? Np * 2 * planes : 1) / TILE * TILE;
-    b.pieces = a.tokens == 0 ? 0 : int((a.vocabulary + ld - 1) / ld);
+    const int64_t entries = a.tokens == 0 ? 0 : widest(b.d_bytes, Np, (int)planes);
+    b.pieces = a.tokens == 0 ? 0 : int((a.vocabulary + entries - 1) / entries);
     return c.used;
 }
 
