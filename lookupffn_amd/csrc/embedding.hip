@@ -2,7 +2,7 @@
 //
 //   out[n] = s W[id_n],   dW[r] = s sum of g[n] over the tokens n with id_n = r
 //
-// Both are bound by memory.  Backward: the tokens are sorted by their numbers (stable, 9 bits a pass, a launch a pass behind one that counts), their list is cut into pieces of equal
+// Both are bound by memory.  Backward: the tokens are sorted by their numbers (stable, 9 bits a pass: a launch that counts and one that sorts; up to 2048 tokens one launch for all), their list is cut into pieces of equal
 // length, whatever the numbers' frequencies, and a wavefront adds up a piece's runs of equal numbers, 16 bytes of a row a lane.  A run inside a piece is a row of the result; of one that
 // passes a piece's end each piece leaves its part, and a last launch adds those.  While the tokens are sorted, on a few compute units, the others clear the table's gradient.
 #include "rows16.h"
@@ -11,7 +11,7 @@ namespace {
 
 constexpr int WG = 256;
 constexpr int BITS = 9, DIGITS = 1 << BITS;
-constexpr int CHUNK = 2048, PER_WAVE = CHUNK / (WG / 64), ROUNDS = PER_WAVE / 64;    // tokens that a workgroup sorts
+constexpr int SORT_WG = 1024, CHUNK = 2048, EACH = CHUNK / SORT_WG, PER_WAVE = EACH * 64;        // tokens that a workgroup sorts
 constexpr int FILL_BYTES = 64 * 1024;        // of a workgroup that clears
 constexpr int JOIN_WG = 512;
 
@@ -43,10 +43,10 @@ __device__ __forceinline__ uint32_t row_of(const void *ids, int wide, int64_t n,
     return id >= 0 && id < int64_t(rows) ? (uint32_t)id : rows;
 }
 
-// LANES threads take a row, EACH of their 16 bytes (or numbers) at a time.
+// LANES threads take a row, AHEAD of their 16 bytes (or numbers) at a time.
 template <typename R, int LANES>
 __global__ __launch_bounds__(WG) void forward_kernel(Args a) {
-    constexpr int EACH = 4;
+    constexpr int AHEAD = 4;
     const uint32_t n = blockIdx.x * (WG / LANES) + threadIdx.x / LANES, in = threadIdx.x % LANES;
     if (n >= a.tokens) return;
     const uint32_t row = row_of(a.ids, a.ids_64, n, a.rows);
@@ -54,13 +54,13 @@ __global__ __launch_bounds__(WG) void forward_kernel(Args a) {
     const char *from = static_cast<const char *>(a.weight) + (there ? row * a.stride : 0) * R::BYTES;
     char *to = static_cast<char *>(a.out) + int64_t(n) * a.columns * R::BYTES;
     constexpr int SIZE = R::N * R::BYTES;
-    for (uint32_t p0 = in; p0 < a.pieces; p0 += EACH * LANES) {
-        typename R::raw_t raw[EACH];
+    for (uint32_t p0 = in; p0 < a.pieces; p0 += AHEAD * LANES) {
+        typename R::raw_t raw[AHEAD];
 #pragma unroll
-        for (int k = 0; k < EACH; ++k)
+        for (int k = 0; k < AHEAD; ++k)
             if (p0 + k * LANES < a.pieces && there) raw[k] = *reinterpret_cast<const typename R::raw_t *>(from + int64_t(p0 + k * LANES) * SIZE);
 #pragma unroll
-        for (int k = 0; k < EACH; ++k) {
+        for (int k = 0; k < AHEAD; ++k) {
             if (p0 + k * LANES >= a.pieces) continue;
             float v[R::N] = {};
             if (there) {
@@ -86,7 +86,6 @@ struct SortArgs {
     const uint2 *from;         // (row, token), or null: the tokens themselves
     uint2 *to;
     int32_t *counts;           // [chunks][DIGITS]: this pass's
-    int32_t *next;             // the next pass's, or null
     uint32_t tokens, rows;
     int chunks, shift, ids_64;
     Fill fill;
@@ -101,90 +100,146 @@ __device__ __forceinline__ uint2 entry(const SortArgs &a, uint32_t i) {
 // A workgroup behind the sorting ones: 64 KB of zeros.
 __device__ __forceinline__ void clear(const Fill &f, int64_t workgroup) {
     const int64_t first = workgroup * FILL_BYTES, end = min(first + FILL_BYTES, f.bytes);
-    for (int64_t i = first + threadIdx.x * 16; i + 16 <= end; i += WG * 16) *reinterpret_cast<uint4 *>(f.at + i) = make_uint4(0, 0, 0, 0);
+    for (int64_t i = first + threadIdx.x * 16; i + 16 <= end; i += SORT_WG * 16) *reinterpret_cast<uint4 *>(f.at + i) = make_uint4(0, 0, 0, 0);
     if (end == f.bytes && threadIdx.x < f.bytes % 16 / 2) reinterpret_cast<uint16_t *>(f.at + f.bytes / 16 * 16)[threadIdx.x] = 0;
 }
 
-// How often a chunk has each digit of the first pass, and zeros for the counts of the others.
-__global__ __launch_bounds__(WG) void count_kernel(SortArgs a, int passes) {
+// How often a chunk has each of a pass's digits.
+__global__ __launch_bounds__(SORT_WG) void count_kernel(SortArgs a) {
     if ((int)blockIdx.x >= a.chunks) return clear(a.fill, blockIdx.x - a.chunks);
     __shared__ int32_t count[DIGITS];
-    for (int d = threadIdx.x; d < DIGITS; d += WG) count[d] = 0;
+    if (threadIdx.x < DIGITS) count[threadIdx.x] = 0;
     __syncthreads();
-    const uint32_t first = blockIdx.x * uint32_t(CHUNK);
 #pragma unroll
-    for (int k = 0; k < CHUNK / WG; ++k) {
-        const uint32_t i = first + k * WG + threadIdx.x;
-        if (i < a.tokens) atomicAdd(&count[entry(a, i).x & (DIGITS - 1)], 1);
+    for (int k = 0; k < EACH; ++k) {
+        const uint32_t i = blockIdx.x * uint32_t(CHUNK) + k * SORT_WG + threadIdx.x;
+        if (i < a.tokens) atomicAdd(&count[entry(a, i).x >> a.shift & (DIGITS - 1)], 1);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < DIGITS; d += WG) {
-        a.counts[int64_t(blockIdx.x) * DIGITS + d] = count[d];
-        for (int p = 1; p < passes; ++p) a.counts[(int64_t(p) * a.chunks + blockIdx.x) * DIGITS + d] = 0;
-    }
+    if (threadIdx.x < DIGITS) a.counts[int64_t(blockIdx.x) * DIGITS + threadIdx.x] = count[threadIdx.x];
 }
 
-// One pass: a chunk's entries go to their places, those of a digit in the order they had.
-__global__ __launch_bounds__(WG) void sort_kernel(SortArgs a) {
-    if ((int)blockIdx.x >= a.chunks) return clear(a.fill, blockIdx.x - a.chunks);
-    __shared__ int32_t place[DIGITS];                  // where a digit's entries of this chunk begin
-    __shared__ int32_t waves[WG / 64][DIGITS];         // how many of a digit a wavefront has had so far
-    __shared__ int32_t total[WG / 64];
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    // a digit's entries in the chunks before this one and in all; two neighbouring digits a thread
-    int before[2] = {0, 0}, all[2] = {0, 0};
-    for (int c = 0; c < a.chunks; ++c) {
-        const int2 n = *reinterpret_cast<const int2 *>(a.counts + int64_t(c) * DIGITS + 2 * tid);
-        if (c < (int)blockIdx.x) before[0] += n.x, before[1] += n.y;
-        all[0] += n.x, all[1] += n.y;
-    }
-    int sum = all[0] + all[1], upto = sum;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const int v = __shfl_up(upto, m);
-        if (lane >= m) upto += v;
-    }
-    if (lane == 63) total[wave] = upto;
-    for (int d = tid; d < WG / 64 * DIGITS; d += WG) waves[0][d] = 0;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += total[w];
-    place[2 * tid] = upto - sum + before[0];
-    place[2 * tid + 1] = upto - sum + all[0] + before[1];
+// What a workgroup needs to put a chunk's entries in the order of a digit.
+struct Sorter {
+    int32_t place[DIGITS];                     // where a digit's entries of this chunk begin
+    int32_t had[SORT_WG / 64][DIGITS];         // how many of a digit a wavefront has had
+    int32_t total[DIGITS / 64];
+};
 
-    uint2 e[ROUNDS];
-    int rank[ROUNDS];
-    const uint32_t first = blockIdx.x * uint32_t(CHUNK) + wave * PER_WAVE + lane;
+// A thread's entries are numbers wave * PER_WAVE + k * 64 + lane of the chunk: -> which of its digit's an entry is within its wavefront.
+__device__ __forceinline__ void rank_entries(Sorter &s, const uint2 (&e)[EACH], const bool (&live)[EACH], int shift, int (&rank)[EACH]) {
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    for (int d = lane; d < DIGITS; d += 64) s.had[wave][d] = 0;
+    __builtin_amdgcn_wave_barrier();           // (a wavefront's LDS accesses keep their order)
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k) {
-        const uint32_t i = first + k * 64;
-        e[k] = i < a.tokens ? entry(a, i) : make_uint2(0, 0);
-    }
-#pragma unroll
-    for (int k = 0; k < ROUNDS; ++k) {
-        const bool live = first + k * 64 < a.tokens;
-        const uint32_t digit = e[k].x >> a.shift & (DIGITS - 1);
+    for (int k = 0; k < EACH; ++k) {
+        const uint32_t digit = e[k].x >> shift & (DIGITS - 1);
         // the lanes of the same digit
-        uint64_t same = __ballot(live);
+        uint64_t same = __ballot(live[k]);
 #pragma unroll
         for (int b = 0; b < BITS; ++b) {
             const uint64_t set = __ballot(digit >> b & 1);
             same &= digit >> b & 1 ? set : ~set;
         }
         const int earlier = __popcll(same & ((uint64_t(1) << lane) - 1));
-        rank[k] = live ? waves[wave][digit] + earlier : 0;
-        __builtin_amdgcn_wave_barrier();               // (a wavefront's LDS accesses keep their order)
-        if (live && earlier == 0) waves[wave][digit] = rank[k] + __popcll(same);
+        rank[k] = live[k] ? s.had[wave][digit] + earlier : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (live[k] && earlier == 0) s.had[wave][digit] = rank[k] + __popcll(same);
         __builtin_amdgcn_wave_barrier();
     }
+}
+
+// A digit's entries in all chunks (thread d's) -> where they begin.  Barriers inside.
+__device__ __forceinline__ int begin_of_digit(Sorter &s, int all) {
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    int upto = all;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        const int v = __shfl_up(upto, m);
+        if (lane >= m) upto += v;
+    }
+    if (threadIdx.x < DIGITS && lane == 63) s.total[wave] = upto;
+    __syncthreads();
+    if (threadIdx.x < DIGITS)
+        for (int w = 0; w < wave; ++w) upto += s.total[w];
+    return upto - all;
+}
+
+__device__ __forceinline__ int place_of(const Sorter &s, uint32_t digit, int rank) {
+    int at = s.place[digit] + rank;
+    for (int w = 0; w < (int)threadIdx.x / 64; ++w) at += s.had[w][digit];
+    return at;
+}
+
+// One pass: a chunk's entries go to their places, those of a digit in the order they had.
+__global__ __launch_bounds__(SORT_WG) void sort_kernel(SortArgs a) {
+    if ((int)blockIdx.x >= a.chunks) return clear(a.fill, blockIdx.x - a.chunks);
+    __shared__ Sorter s;
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    uint2 e[EACH];
+    bool live[EACH];
+    int rank[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const uint32_t i = blockIdx.x * uint32_t(CHUNK) + wave * PER_WAVE + k * 64 + lane;
+        live[k] = i < a.tokens;
+        e[k] = live[k] ? entry(a, i) : make_uint2(0, 0);
+    }
+    // a digit's entries in the chunks before this one and in all
+    int before = 0, all = 0;
+    if (tid < DIGITS) {
+#pragma unroll 8
+        for (int c = 0; c < a.chunks; ++c) {
+            const int n = a.counts[int64_t(c) * DIGITS + tid];
+            if (c < (int)blockIdx.x) before += n;
+            all += n;
+        }
+    }
+    const int begin = begin_of_digit(s, all);
+    if (tid < DIGITS) s.place[tid] = begin + before;
+    rank_entries(s, e, live, a.shift, rank);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k) {
-        if (first + k * 64 >= a.tokens) continue;
-        const uint32_t digit = e[k].x >> a.shift & (DIGITS - 1);
-        int at = place[digit] + rank[k];
-        for (int w = 0; w < wave; ++w) at += waves[w][digit];
-        a.to[at] = e[k];
-        if (a.next) atomicAdd(a.next + int64_t(at / CHUNK) * DIGITS + (e[k].x >> (a.shift + BITS) & (DIGITS - 1)), 1);
+    for (int k = 0; k < EACH; ++k)
+        if (live[k]) a.to[place_of(s, e[k].x >> a.shift & (DIGITS - 1), rank[k])] = e[k];
+}
+
+// All passes of one chunk, by one workgroup in LDS.
+__global__ __launch_bounds__(SORT_WG) void sort_one_kernel(SortArgs a, int passes) {
+    if (blockIdx.x >= 1) return clear(a.fill, blockIdx.x - 1);
+    __shared__ Sorter s;
+    __shared__ uint2 list[CHUNK];
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    uint2 e[EACH];
+    bool live[EACH];
+    int rank[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const uint32_t i = wave * PER_WAVE + k * 64 + lane;
+        live[k] = i < a.tokens;
+        e[k] = live[k] ? entry(a, i) : make_uint2(0, 0);
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * BITS;
+        rank_entries(s, e, live, shift, rank);
+        __syncthreads();
+        int all = 0;
+        if (tid < DIGITS)
+#pragma unroll
+            for (int w = 0; w < SORT_WG / 64; ++w) all += s.had[w][tid];
+        const int begin = begin_of_digit(s, all);
+        if (tid < DIGITS) s.place[tid] = begin;
+        __syncthreads();
+        uint2 *const to = p + 1 < passes ? list : a.to;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+            if (live[k]) to[place_of(s, e[k].x >> shift & (DIGITS - 1), rank[k])] = e[k];
+        __syncthreads();
+        if (p + 1 < passes) {
+#pragma unroll
+            for (int k = 0; k < EACH; ++k)
+                if (live[k]) e[k] = list[wave * PER_WAVE + k * 64 + lane];
+        }
     }
 }
 
@@ -334,7 +389,7 @@ Space space_of(const lffn_embedding &a) {
     s.passes = passes_of(a.rows);
     s.length = length_of(a.tokens);
     s.pieces = (a.tokens + s.length - 1) / s.length;
-    s.counts = up(s.passes * s.chunks * DIGITS * 4);
+    s.counts = up(s.chunks * DIGITS * 4);
     s.lists = up(a.tokens * 8);
     s.parts = s.pieces * 2 * a.columns * 4;
     s.bytes = s.counts + 2 * s.lists + s.parts;
@@ -402,31 +457,28 @@ extern "C" int lffn_embedding_bwd(const lffn_embedding *c, const void *g, void *
     int32_t *const counts = reinterpret_cast<int32_t *>(ws);
     uint2 *const lists[2] = {reinterpret_cast<uint2 *>(ws + s.counts), reinterpret_cast<uint2 *>(ws + s.counts + s.lists)};
     const int64_t size = c->format == LFFN_ROWS_F32 ? 4 : 2, bytes = c->rows * c->columns * size;
-    // every launch clears an equal share
-    const int launches = c->tokens == 0 ? 1 : 1 + s.passes;
+    // every launch that sorts clears an equal share
+    const bool one = s.chunks == 1;
+    const int launches = c->tokens == 0 || one ? 1 : 2 * s.passes;
     const int64_t share = (bytes / launches + 1023) / 1024 * 1024;
     const bool vectors = c->columns * size % 16 == 0 && lffn_aligned16(g);
     const int64_t width = vectors ? c->columns * size / 16 : c->columns;
-    LFFN_REQUIRE(share / FILL_BYTES + 1 + s.chunks < (int64_t(1) << 32) / WG && s.pieces * ((width + 63) / 64) < (int64_t(1) << 32) / JOIN_WG, LFFN_ERR_UNSUPPORTED);
+    LFFN_REQUIRE(share / FILL_BYTES + 1 + s.chunks < (int64_t(1) << 32) / SORT_WG && s.pieces * ((width + 63) / 64) < (int64_t(1) << 32) / JOIN_WG, LFFN_ERR_UNSUPPORTED);
     SortArgs a{};
     a.ids = c->ids, a.padding = c->padding, a.ids_64 = c->ids_64;
     a.tokens = (uint32_t)c->tokens, a.rows = (uint32_t)c->rows, a.chunks = (int)s.chunks;
+    a.counts = counts, a.to = lists[0];
     for (int i = 0; i < launches; ++i) {
         const int64_t first = i * share < bytes ? i * share : bytes, end = i + 1 == launches || (i + 1) * share > bytes ? bytes : (i + 1) * share;
         a.fill = {static_cast<char *>(grad) + first, end - first};
-        const dim3 grid(unsigned(s.chunks + (a.fill.bytes + FILL_BYTES - 1) / FILL_BYTES));
-        if (grid.x == 0) continue;
-        if (i == 0) {
-            a.counts = counts;
-            count_kernel<<<grid, dim3(WG), 0, st>>>(a, s.passes);
-        } else {
-            a.counts = counts + (i - 1) * s.chunks * DIGITS;
-            a.next = i < s.passes ? counts + i * s.chunks * DIGITS : nullptr;
-            a.from = i == 1 ? nullptr : lists[i % 2];
-            a.to = lists[1 - i % 2];
-            a.shift = (i - 1) * BITS;
-            sort_kernel<<<grid, dim3(WG), 0, st>>>(a);
-        }
+        const dim3 grid(unsigned(s.chunks + (a.fill.bytes + FILL_BYTES - 1) / FILL_BYTES)), block(SORT_WG);
+        if (one) sort_one_kernel<<<grid, block, 0, st>>>(a, s.passes);
+        else if (i % 2 == 0) {
+            if (i > 0) a.from = a.to, a.to = lists[i / 2 % 2];
+            a.shift = i / 2 * BITS;
+            count_kernel<<<grid, block, 0, st>>>(a);
+        } else
+            sort_kernel<<<grid, block, 0, st>>>(a);
     }
     if (c->tokens > 0) {
         const SumArgs m{a.to,     g, grad, reinterpret_cast<float *>(ws + s.counts + 2 * s.lists), a.tokens, a.rows, (uint32_t)c->columns, (uint32_t)width,

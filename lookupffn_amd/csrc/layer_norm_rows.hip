@@ -11,7 +11,7 @@
 namespace {
 
 constexpr int WG = 256;
-constexpr int PARTS = 512;               // workgroups of a backward, at most: each leaves two rows of sums
+constexpr int PARTS = 1024;              // workgroups of a backward, at most: each leaves two rows of sums
 constexpr int WIDE_COLUMNS = 1024;       // columns of a workgroup that adds up a wide backward's columns
 
 // A number of a format by itself.

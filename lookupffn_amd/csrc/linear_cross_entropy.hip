@@ -400,6 +400,144 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
     });
 }
 
+// ---------------------------------------------------------------- few tokens
+
+// Up to 64 tokens of 16 bits: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a time, whose
+// rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, four such in flight.  Nothing is laid together before: a launch less.
+constexpr int FEW = 64, FEW_AHEAD = 4;
+constexpr int few_stride(int columns) { return int(up(columns, STEP)) / 8 | 1; }                // 16-byte pieces of a row in LDS: odd, so that 16 rows meet every bank once
+constexpr int64_t few_lds(int64_t tokens, int64_t columns) {
+    return (tokens <= 32 ? 32 : 64) * int64_t(few_stride((int)columns)) * 16 + 8 * FEW * 8 + FEW * 4;
+}
+bool few_tokens(const lffn_linear_cross_entropy &a) { return a.format != LFFN_ROWS_F32 && a.tokens <= FEW && few_lds(a.tokens, a.columns) <= 160 * 1024; }
+
+struct FewArgs {
+    RowsArgs r;
+    float2 *parts;
+    float *at_label;
+    int64_t Np;
+};
+
+template <typename F, int TOKENS>
+__global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
+    constexpr int JB = TOKENS / 32, WAVES = THREADS / 64;
+    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
+    const Operands &o = a.r.o;
+    const int V = o.s.V, K = o.s.K, tid = threadIdx.x, wave = tid / 64, lane = tid % 64, half = lane / 32;
+    const int stride = few_stride(K), pieces = int(up(K, STEP)) / 8, steps = pieces / 8;
+    float2 *const waves = reinterpret_cast<float2 *>(lds_words + TOKENS * stride);       // [WAVES][TOKENS]
+    int *const tokens = reinterpret_cast<int *>(waves + WAVES * TOKENS);                 // [TOKENS]
+    // the labelled tokens: every wavefront sees them all
+    const int y = lane < o.s.N ? label_of(a.r.labels, a.r.labels_64, lane, a.r.ignore, V) : -1;
+    const uint64_t live = __ballot(y >= 0);
+    const int labelled = __popcll(live), place = __popcll(live & ((uint64_t(1) << lane) - 1));
+    if (wave == 0 && y >= 0) tokens[place] = lane;
+    if (blockIdx.x == 0 && wave == 0) {
+        if (lane == 0) o.kept.head[0] = labelled;
+        if (lane < o.s.N) {
+            o.kept.pos[lane] = y >= 0 ? place : -1;
+            if (y >= 0) o.kept.label[place] = y, a.r.token[place] = lane;
+            else if (a.r.loss) a.r.loss[lane] = 0.f;
+        }
+    }
+    if (labelled == 0) return;
+    const int blocks = (V + 31) / 32, all = gridDim.x * WAVES;
+    int block = blockIdx.x * WAVES + wave;
+    uint4 w[FEW_AHEAD][4];
+    const char *row = nullptr;
+    auto begin_block = [&] { row = o.weight.at + int64_t(min(block * 32 + lane % 32, V - 1)) * o.weight.stride; };
+    auto load = [&](int s, uint4 (&to)[4]) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) to[c] = *reinterpret_cast<const uint4 *>(row + min(s * 64 + half * 32 + c * 8, K - 8) * 2);
+    };
+    if (block < blocks) {
+        begin_block();
+#pragma unroll
+        for (int s = 0; s < FEW_AHEAD; ++s) load(s, w[s]);
+    }
+    __syncthreads();
+    for (int i = tid; i < TOKENS * pieces; i += THREADS) {
+        const int r = i / pieces, p = i - r * pieces;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < labelled && p * 8 < K) v = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.r.hidden) + (tokens[r] * a.r.hidden_stride + p * 8) * 2);
+        lds_words[r * stride + p] = v;
+    }
+    __syncthreads();
+    const uint32_t lds = lds_byte_of(lds_words) + (lane % 32 * stride + half * 4) * 16;
+    int label[JB];
+    float2 of[JB];
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+        const int n = 32 * j + lane % 32;
+        label[j] = n < labelled ? label_of(a.r.labels, a.r.labels_64, tokens[n], a.r.ignore, V) : -1;
+        of[j] = make_float2(-INFINITY, 0.f);
+    }
+    for (; block < blocks; block += all) {
+        f32x16_t sums[JB];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int v = block * 32 + mfma_row(e, half);
+            const float b = v >= V ? -INFINITY : a.r.bias_format < 0 ? 0.f : bias_of(a.r.bias, a.r.bias_format, v);
+#pragma unroll
+            for (int j = 0; j < JB; ++j) sums[j][e] = b;
+        }
+        for (int s0 = 0; s0 < steps; s0 += FEW_AHEAD) {
+#pragma unroll
+            for (int k = 0; k < FEW_AHEAD; ++k) {
+                const int s = s0 + k;
+                if (s < steps) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int j = 0; j < JB; ++j) {
+                            const uint4 x = __builtin_bit_cast(uint4, *(const lds_word_t *)(uintptr_t)(lds + (j * 32 * stride + s * 8 + c) * 16));
+                            sums[j] = F::mma(w[k][c], x, sums[j]);
+                        }
+                    if (s + FEW_AHEAD < steps) load(s + FEW_AHEAD, w[k]);
+                }
+            }
+        }
+        const int v0 = block * 32;
+        if (block + all < blocks) {                 // the next block's first steps
+            block += all;
+            begin_block();
+            block -= all;
+#pragma unroll
+            for (int s = 0; s < FEW_AHEAD; ++s) load(s, w[s]);
+        }
+#pragma unroll
+        for (int j = 0; j < JB; ++j) {
+            float most = of[j].x;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) most = fmaxf(most, sums[j][e]);
+            const float from = most == -INFINITY ? 0.f : most;
+            float sum = of[j].y * __builtin_amdgcn_exp2f((of[j].x - from) * LOG2E);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f((sums[j][e] - from) * LOG2E);
+            of[j] = make_float2(most, sum);
+            const int r = label[j] - v0;
+            if (label[j] >= 0 && r >= 0 && r < 32 && r / 4 % 2 == half) {
+                float found = sums[j][0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) found = mfma_row(e, half) == r ? sums[j][e] : found;
+                a.at_label[32 * j + lane % 32] = found;
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+        const float2 other = make_float2(__shfl_xor(of[j].x, 32), __shfl_xor(of[j].y, 32));
+        if (half == 0) waves[wave * TOKENS + 32 * j + lane] = joined(of[j], other);
+    }
+    __syncthreads();
+    if (tid < TOKENS) {
+        float2 sum = waves[tid];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) sum = joined(sum, waves[i * TOKENS + tid]);
+        a.parts[blockIdx.x * a.Np + tid] = sum;
+    }
+}
+
 struct JoinArgs {
     Kept kept;
     const float2 *parts;
@@ -866,7 +1004,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Fo
     f.f.o = operands(a, c);
     f.f.Np = f.j.Np = Np;
     f.j.tiles = int((a.vocabulary + TILE - 1) / TILE);
-    f.j.parts = f.f.parts = c.take<float2>(f.j.tiles * Np);
+    f.j.parts = f.f.parts = c.take<float2>(f.j.tiles * Np);          // (a tile each, or, of few tokens, a workgroup: no more)
     f.j.at_label = f.f.at_label = c.take<float>(Np);
     f.j.losses = c.take<float>(Np);
     f.j.token = f.r.token = c.take<int32_t>(Np);
@@ -923,6 +1061,16 @@ unsigned workgroups(int64_t tiles) { return unsigned(tiles >= COMPUTE_UNITS ? CO
 
 constexpr size_t LDS_BYTES = STREAM_LDS + 2 * BESIDE_BYTES + WAVES_M * TILE * sizeof(float2);
 
+template <typename F, int TOKENS>
+int few(const lffn_linear_cross_entropy &a, Forward &f, hipStream_t st) {
+    static LdsGrant granted;
+    const int64_t lds = few_lds(a.tokens, a.columns);
+    if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&few_kernel<F, TOKENS>), lds, granted)) return LFFN_ERR_LAUNCH;
+    if (f.j.tiles > COMPUTE_UNITS) f.j.tiles = COMPUTE_UNITS;              // (a workgroup's eight wavefronts have a tile's entries, and then another's)
+    few_kernel<F, TOKENS><<<dim3(f.j.tiles), dim3(THREADS), lds, st>>>({f.r, f.f.parts, f.f.at_label, f.f.Np});
+    return LFFN_OK;
+}
+
 template <typename F>
 int forward(const Forward &f, hipStream_t st) {
     static LdsGrant granted;
@@ -978,7 +1126,12 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
     fill(f.r, *a, f.f.o);
     if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.losses = nullptr;
     if (a->format == LFFN_ROWS_F32 || a->tokens == 0) head_kernel<<<dim3(1), dim3(64), 0, st>>>(f.f.o.kept.head);
-    if (a->tokens > 0) {
+    if (a->tokens > 0 && few_tokens(*a)) {
+        const bool bf16 = a->format == LFFN_ROWS_BF16;
+        const int done = a->tokens <= 32 ? (bf16 ? few<BF16, 32>(*a, f, st) : few<F16, 32>(*a, f, st)) : bf16 ? few<BF16, 64>(*a, f, st) : few<F16, 64>(*a, f, st);
+        if (done != LFFN_OK) return done;
+        join_kernel<<<dim3(unsigned((a->tokens + 15) / 16)), dim3(256), 0, st>>>(f.j);
+    } else if (a->tokens > 0) {
         if (a->tokens > COUNTED_FROM) {
             count_kernel<<<dim3(unsigned((a->tokens + 255) / 256)), dim3(256), 0, st>>>(a->labels, a->labels_64, a->ignore_index, f.f.o.s.V, f.f.o.s.N, f.counts);
             f.r.counts = f.counts;
