@@ -1014,7 +1014,7 @@ int lffn_layer_norm_rows_bwd(const lffn_layer_norm_rows *a, const float *stats, 
  *   l_nv = hidden[n] . weight[v] + bias[v],  loss_n = log sum_v exp l_nv - l_n,label(n)
  * for the tokens that have a label: those whose number is not ignore_index and one of the vocabulary's.  The others take no part, whatever their rows hold.
  * hidden: [tokens, columns], weight: [vocabulary, columns], rows of `columns` numbers that lie together (hidden_stride, weight_stride elements apart, multiples of 16 bytes,
- * as are the addresses); columns a multiple of 8, at most 65536; vocabulary at most 2^22, tokens at most 2^24.  bias: [vocabulary] of bias_format, or NULL.
+ * as are the addresses); columns a multiple of 8, at most 65536; vocabulary at most 2^22, tokens at most 2^24, tokens * columns at most 2^32.  bias: [vocabulary] of bias_format, or NULL.
  * labels: [tokens], int64 where labels_64 is not 0, else int32.
  * reduction 0: loss is [tokens], zeros for the others; 1: their mean (0 of none), 2: their sum; [1].
  * format 0: products of two half-precision terms a number, fp32 accuracy; in the backward a number of hidden or weight is held to 2^-38 of the largest of its array.

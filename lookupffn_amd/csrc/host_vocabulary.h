@@ -263,7 +263,7 @@ struct LossInputs {
         if (hidden.dim() < 1 || hidden.numel() == 0 || format_of(hidden) < 0 || weight.dim() != 2 || weight.numel() == 0 || weight.scalar_type() != hidden.scalar_type()) return false;
         const int64_t columns = hidden.size(hidden.dim() - 1);
         return columns % 8 == 0 && columns <= 65536 && weight.size(1) == columns && weight.size(0) <= 1 << 22 && token_numbers(labels) &&
-               labels.sizes() == hidden.sizes().slice(0, hidden.dim() - 1) && labels.numel() <= 1 << 24 &&
+               labels.sizes() == hidden.sizes().slice(0, hidden.dim() - 1) && labels.numel() <= 1 << 24 && hidden.numel() <= int64_t(1) << 32 &&
                (!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0) && (bias.scalar_type() == at::kFloat || bias.scalar_type() == hidden.scalar_type())));
     }
     // rows, table, b and y are what hidden, weight, bias and labels are laid out as

@@ -140,9 +140,17 @@ __device__ __forceinline__ float bias_of(const void *bias, int format, int v) {
     return (float)static_cast<const _Float16 *>(bias)[v];
 }
 
-// Of many that raise one number only those that would are atomic (32003 rows: 370 us otherwise, 25 like this).
-__device__ __forceinline__ void raise(int32_t *most, int v) {
-    if (__hip_atomic_load(most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < v) atomicMax(most, v);
+// The exponent of the largest of n powers of two, to *most, by a workgroup that others may be beside: one atomic for it.
+__device__ __forceinline__ void raise(int32_t *most, const float *scales, int first, int n, int step, float *red) {
+    float v = 0.f;
+    for (int i = first; i < n; i += step) v = fmaxf(v, scales[i]);
+    v = wave_most(v);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (unsigned i = 1; i < blockDim.x / 64; ++i) v = fmaxf(v, red[i]);
+        if (v > 0.f) atomicMax(most, ilogbf(v));
+    }
 }
 
 // Workgroups PARTS (tokens / CHUNK): the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
@@ -195,10 +203,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
         if (at < 0) continue;
         const char *from = static_cast<const char *>(a.hidden) + (int64_t(t0) + i) * a.hidden_stride * R::BYTES;
         const int e = lay_row<R, PLANES>(from, a.o.rows + at * row_bytes, a.o.rows_plane, s.K, s.Kp, BACKWARD ? k.head + 1 : nullptr);
-        if (PLANES == 2 && !BACKWARD && lane == 0) {
-            a.o.row_scale[at] = __builtin_amdgcn_ldexpf(1.f, e);
-            raise(k.head + 1, e);
-        }
+        if (PLANES == 2 && !BACKWARD && lane == 0) a.o.row_scale[at] = __builtin_amdgcn_ldexpf(1.f, e);
     }
     if (chunk == chunks - 1) {
         const int64_t from = labelled * row_bytes / 16, to = up(labelled, TILE) * row_bytes / 16;
@@ -223,8 +228,8 @@ __global__ __launch_bounds__(256) void weight_kernel(Operands o, const float *w,
         e = lay_row<F32Row, 2>(reinterpret_cast<const char *>(w + v * stride), const_cast<char *>(o.weight.at) + v * o.weight.stride, o.weight.plane, o.s.K, o.s.K,
                                BACKWARD ? o.kept.head + 2 : nullptr);
     if (threadIdx.x % 64 == 0) {
-        o.weight_scale[v] = __builtin_amdgcn_ldexpf(1.f, e);
-        if (!BACKWARD && v < o.s.V) raise(o.kept.head + 2, e);
+        // (entries behind the vocabulary: no larger than any)
+        o.weight_scale[v] = v < o.s.V ? __builtin_amdgcn_ldexpf(1.f, e) : BACKWARD ? 1.f : 0.f;
     }
 }
 
@@ -403,13 +408,15 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
 // ---------------------------------------------------------------- few tokens
 
 // Up to 64 tokens of 16 bits: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a time, whose
-// rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, four such in flight.  Nothing is laid together before: a launch less.
-constexpr int FEW = 64, FEW_AHEAD = 4;
+// rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, six such in flight.  Nothing is laid together before: a launch less.
+constexpr int FEW = 64, FEW_AHEAD = 6;
 constexpr int few_stride(int columns) { return int(up(columns, STEP)) / 8 | 1; }                // 16-byte pieces of a row in LDS: odd, so that 16 rows meet every bank once
 constexpr int64_t few_lds(int64_t tokens, int64_t columns) {
     return (tokens <= 32 ? 32 : 64) * int64_t(few_stride((int)columns)) * 16 + 8 * FEW * 8 + FEW * 4;
 }
 bool few_tokens(const lffn_linear_cross_entropy &a) { return a.format != LFFN_ROWS_F32 && a.tokens <= FEW && few_lds(a.tokens, a.columns) <= 160 * 1024; }
+
+int few_workgroups(const lffn_linear_cross_entropy &a) { return (int)min((a.vocabulary + 31) / 32, int64_t(COMPUTE_UNITS)); }
 
 struct FewArgs {
     RowsArgs r;
@@ -442,7 +449,7 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
     }
     if (labelled == 0) return;
     const int blocks = (V + 31) / 32, all = gridDim.x * WAVES;
-    int block = blockIdx.x * WAVES + wave;
+    int block = wave * gridDim.x + blockIdx.x;
     uint4 w[FEW_AHEAD][4];
     const char *row = nullptr;
     auto begin_block = [&] { row = o.weight.at + int64_t(min(block * 32 + lane % 32, V - 1)) * o.weight.stride; };
@@ -547,12 +554,22 @@ struct JoinArgs {
     int tiles;
     float *loss;           // by token
     float *losses;         // by place
+    const float *weight_scale, *row_scale;       // two-term numbers
+    int entries, joining;                        // workgroups that join; those behind look for the largest of the scales
 };
+
+constexpr int LOOKING = 16;
 
 // A token's parts: 16 threads.
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     __shared__ float2 shares[16][17];
     const int labelled = a.kept.head[0], in = threadIdx.x % 16, slice = threadIdx.x / 16, n = blockIdx.x * 16 + in;
+    if ((int)blockIdx.x >= a.joining) {
+        const int i = blockIdx.x - a.joining;
+        if (i < LOOKING) raise(a.kept.head + 2, a.weight_scale, i * 256 + threadIdx.x, a.entries, LOOKING * 256, &shares[0][0].x);
+        else raise(a.kept.head + 1, a.row_scale, (i - LOOKING) * 256 + threadIdx.x, labelled, LOOKING * 256, &shares[0][0].x);
+        return;
+    }
     if ((int)blockIdx.x * 16 >= labelled) return;
     float2 of = make_float2(-INFINITY, 0.f);
 #pragma unroll 4
@@ -916,23 +933,34 @@ __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, i
     if (a.grad_weight) weight_tasks<F, R>(a, p, labelled, unit, lds);
 }
 
-// dh: a labelled token's shares added up, zeros for the others.
+// dh: a labelled token's shares added up, zeros for the others; four threads for eight columns.
 template <typename F, typename R>
 __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
+    __shared__ float4 sums[3][64][2];
     const Sizes &s = a.o.s;
-    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, pieces = s.K / 8, t = i / pieces, c = i % pieces * 8;
-    if (t >= s.N) return;
-    const int at = a.o.kept.pos[t], labelled = a.o.kept.head[0];
+    const int in = threadIdx.x % 64, part = threadIdx.x / 64, pieces = s.K / 8;
+    const int64_t i = int64_t(blockIdx.x) * 64 + in, t = i / pieces, c = i % pieces * 8;
+    const int at = t < s.N ? a.o.kept.pos[t] : -1, labelled = a.o.kept.head[0];
     float v[8] = {};
     if (at >= 0) {
         const int steps = piece_of<F>(a, labelled, 0).steps, wanted = *a.shares, length = (steps + 2 * wanted - 1) / (2 * wanted) * 2, shares = (steps + length - 1) / length;
-#pragma unroll 8
-        for (int p = 0; p < shares; ++p) {
+#pragma unroll 4
+        for (int p = part; p < shares; p += 4) {
             const float *from = a.parts + (int64_t(p) * labelled + at) * s.K + c;
             const float4 x = *reinterpret_cast<const float4 *>(from), y = *reinterpret_cast<const float4 *>(from + 4);
             v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
         }
+        if (part > 0) sums[part - 1][in][0] = make_float4(v[0], v[1], v[2], v[3]), sums[part - 1][in][1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    __syncthreads();
+    if (part > 0 || t >= s.N) return;
+    if (at >= 0) {
         const float by = factor_of(a, labelled) * (F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, a.o.kept.head[2]) : 1.f);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const float4 x = sums[p][in][0], y = sums[p][in][1];
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= by;
     }
@@ -951,7 +979,8 @@ int check(const lffn_linear_cross_entropy *a) {
     LFFN_REQUIRE(a, LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(a->format >= 0 && a->format <= 2 && a->bias_format >= 0 && a->bias_format <= 2 && a->reduction >= 0 && a->reduction <= 2, LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(a->tokens >= 0 && a->vocabulary >= 1 && a->columns >= 8, LFFN_ERR_BAD_ARG);
-    LFFN_REQUIRE(a->columns % 8 == 0 && a->columns <= 65536 && a->tokens <= (1 << 24) && a->vocabulary <= (1 << 22), LFFN_ERR_UNSUPPORTED);
+    LFFN_REQUIRE(a->columns % 8 == 0 && a->columns <= 65536 && a->tokens <= (1 << 24) && a->vocabulary <= (1 << 22) && a->tokens * a->columns <= int64_t(1) << 32,
+                 LFFN_ERR_UNSUPPORTED);
     const int64_t size = a->format == LFFN_ROWS_F32 ? 4 : 2, most = int64_t(1) << 22;
     LFFN_REQUIRE(a->weight && lffn_aligned16(a->weight) && a->weight_stride >= a->columns && a->weight_stride * size % 16 == 0, LFFN_ERR_BAD_ARG);
     LFFN_REQUIRE(a->tokens == 0 || (a->hidden && a->labels), LFFN_ERR_BAD_ARG);
@@ -1004,7 +1033,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Fo
     f.f.o = operands(a, c);
     f.f.Np = f.j.Np = Np;
     f.j.tiles = int((a.vocabulary + TILE - 1) / TILE);
-    f.j.parts = f.f.parts = c.take<float2>(f.j.tiles * Np);          // (a tile each, or, of few tokens, a workgroup: no more)
+    f.j.parts = f.f.parts = c.take<float2>((few_tokens(a) ? few_workgroups(a) : f.j.tiles) * Np);
     f.j.at_label = f.f.at_label = c.take<float>(Np);
     f.j.losses = c.take<float>(Np);
     f.j.token = f.r.token = c.take<int32_t>(Np);
@@ -1066,7 +1095,7 @@ int few(const lffn_linear_cross_entropy &a, Forward &f, hipStream_t st) {
     static LdsGrant granted;
     const int64_t lds = few_lds(a.tokens, a.columns);
     if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&few_kernel<F, TOKENS>), lds, granted)) return LFFN_ERR_LAUNCH;
-    if (f.j.tiles > COMPUTE_UNITS) f.j.tiles = COMPUTE_UNITS;              // (a workgroup's eight wavefronts have a tile's entries, and then another's)
+    f.j.tiles = few_workgroups(a);
     few_kernel<F, TOKENS><<<dim3(f.j.tiles), dim3(THREADS), lds, st>>>({f.r, f.f.parts, f.f.at_label, f.f.Np});
     return LFFN_OK;
 }
@@ -1091,7 +1120,7 @@ int backward(const BackwardArgs &b, hipStream_t st) {
     }
     if (b.grad_hidden) {
         const int64_t n = int64_t(b.o.s.N) * (b.o.s.K / 8);
-        hidden_kernel<F, R><<<dim3(unsigned((n + 255) / 256)), dim3(256), 0, st>>>(b);
+        hidden_kernel<F, R><<<dim3(unsigned((n + 63) / 64)), dim3(256), 0, st>>>(b);
     }
     return LFFN_OK;
 }
@@ -1130,7 +1159,8 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
         const bool bf16 = a->format == LFFN_ROWS_BF16;
         const int done = a->tokens <= 32 ? (bf16 ? few<BF16, 32>(*a, f, st) : few<F16, 32>(*a, f, st)) : bf16 ? few<BF16, 64>(*a, f, st) : few<F16, 64>(*a, f, st);
         if (done != LFFN_OK) return done;
-        join_kernel<<<dim3(unsigned((a->tokens + 15) / 16)), dim3(256), 0, st>>>(f.j);
+        f.j.joining = int((a->tokens + 15) / 16);
+        join_kernel<<<dim3(f.j.joining), dim3(256), 0, st>>>(f.j);
     } else if (a->tokens > 0) {
         if (a->tokens > COUNTED_FROM) {
             count_kernel<<<dim3(unsigned((a->tokens + 255) / 256)), dim3(256), 0, st>>>(a->labels, a->labels_64, a->ignore_index, f.f.o.s.V, f.f.o.s.N, f.counts);
@@ -1139,7 +1169,9 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
         launch_rows<false>(*a, f.r, st);
         const int done = a->format == LFFN_ROWS_F32 ? forward<F32Two>(f, st) : a->format == LFFN_ROWS_BF16 ? forward<BF16>(f, st) : forward<F16>(f, st);
         if (done != LFFN_OK) return done;
-        join_kernel<<<dim3(unsigned(f.f.Np / 16)), dim3(256), 0, st>>>(f.j);
+        f.j.joining = int(f.f.Np / 16);
+        f.j.weight_scale = f.f.o.weight_scale, f.j.row_scale = f.f.o.row_scale, f.j.entries = (int)a->vocabulary;
+        join_kernel<<<dim3(f.j.joining + (a->format == LFFN_ROWS_F32 ? 2 * LOOKING : 0)), dim3(256), 0, st>>>(f.j);
     }
     if (a->reduction != 0) sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(f.f.o.kept.head, f.j.losses, loss, a->reduction == 1);
     return lffn_launch_status();

@@ -1708,7 +1708,7 @@ def _(x, weight, bias, stats, g, of_x, of_weight, of_bias):
 # ----------------------------------------------------------------------------- softmax cross entropy of a projection
 
 REDUCTIONS = ("none", "mean", "sum")
-LOSS_MAX_COLUMNS, LOSS_MAX_VOCABULARY, LOSS_MAX_TOKENS = 65536, 1 << 22, 1 << 24
+LOSS_MAX_COLUMNS, LOSS_MAX_VOCABULARY, LOSS_MAX_TOKENS, LOSS_MAX_NUMBERS = 65536, 1 << 22, 1 << 24, 1 << 32
 
 
 def _fit_loss(hidden, weight, bias, labels, reduction):

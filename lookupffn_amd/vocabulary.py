@@ -82,7 +82,7 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
 
         loss_n = log sum_v exp l_nv - l_n,label(n),  l_nv = hidden[n] . weight[v] + bias[v]
 
-    hidden: [..., columns], weight: [vocabulary, columns] of its type, columns a multiple of 8 (at most 65536; vocabulary at most 2^22, tokens at most 2^24), with any strides (a copy is
+    hidden: [..., columns], weight: [vocabulary, columns] of its type, columns a multiple of 8 (at most 65536; vocabulary at most 2^22, tokens at most 2^24, 2^32 numbers of hidden), with any strides (a copy is
     made where columns do not lie together or rows not at multiples of 16 bytes); bias: [vocabulary], float32 or of that type, or None; labels: [...] int32 or
     int64.  A token whose label is ignore_index, or no number of the vocabulary, has no part in anything, whatever its row holds, and costs nothing:
     its loss and gradient are zeros.  reduction: "mean" over the tokens that have a label (0 of none), "sum", or "none" (the shape of labels).
@@ -106,7 +106,7 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
              f"bias: [{weight.shape[0]}] float32 or {hidden.dtype}, got {None if bias is None else (tuple(bias.shape), bias.dtype)}")
     _require(labels.shape == hidden.shape[:-1] and labels.dtype in (torch.int32, torch.int64),
              f"labels: {tuple(hidden.shape[:-1])} int32 or int64, got {tuple(labels.shape)} {labels.dtype}")
-    _require(labels.numel() <= ops.LOSS_MAX_TOKENS, f"labels: {labels.numel()} tokens")
+    _require(labels.numel() <= ops.LOSS_MAX_TOKENS and hidden.numel() <= ops.LOSS_MAX_NUMBERS, f"hidden: {tuple(hidden.shape)}")
     _require(reduction in ops.REDUCTIONS, f"reduction: {reduction!r}")
     _require(isinstance(ignore_index, int) and -1 << 63 <= ignore_index < 1 << 63, f"ignore_index: {ignore_index!r}")
     args = hidden.reshape(-1, columns), weight, bias, labels.reshape(-1), ignore_index, ops.REDUCTIONS.index(reduction)
