@@ -14,11 +14,13 @@ from .cross_attention import CrossAttentionFunction, QkNormRotary, cross_attenti
 from .norm import LayerNorm, layer_norm
 from .vocabulary import Embedding, LinearCrossEntropy, embedding, linear_cross_entropy
 from .lookup import BH4, Hashing, LookupFFN
-from .encoder import Attention, CrossAttention, Encoder, EncoderLayer, Lookup, RobertaEmbeddings
+from .encoder import (Attention, CrossAttention, Encoder, EncoderLayer, Lookup, LookupForMaskedLM, MaskedLMHead,
+                      RobertaEmbeddings)
 
 __all__ = [
     "BH4", "Hashing", "LookupFFN",
     "Attention", "CrossAttention", "EncoderLayer", "Encoder", "Lookup", "RobertaEmbeddings",
+    "LookupForMaskedLM", "MaskedLMHead",
     "bh4", "bh4_cuda", "hadamard", "hadamard_transform", "fast_hadamard_transform",
     "FastHadamardTransform", "FastHadamardTransformDim512", "FastHadamardTransformDim1024",
     "compute_code_score", "compute_code_score_torch", "bin2dec", "ComputeCodeScore",

@@ -4,7 +4,9 @@ of src/roberta/models/postnorm.py:6-28), with the same module and parameter
 names so that a reference state_dict loads unchanged.  ``LookupFFN`` and, without
 gradients, the attention's products and softmax run on the gfx950 kernels of this
 package; embeddings, LayerNorms and the attention in training are plain PyTorch-ROCm.
-``CrossAttention`` reads the encoder's states from another sequence, with and without gradients.
+``CrossAttention`` reads the encoder's states from another sequence, with and without gradients.  ``LookupForMaskedLM`` is
+the model with what it is pre-trained by: the embeddings' gradient, the head's layer norm and the loss over the vocabulary
+run on this package's kernels too.
 
 ``config`` carries the attributes the reference reads: hidden_size,
 num_attention_heads, attention_head_size, attention_probs_dropout_prob,
@@ -23,9 +25,11 @@ from torch.utils.checkpoint import checkpoint
 from . import ops
 from .cross_attention import cross_attention, qk_norm_rotary, rotary_table
 from .lookup import LookupFFN
+from .norm import layer_norm
+from .vocabulary import embedding, linear_cross_entropy
 
 _GLOBAL_HOOKS = torch.nn.modules.module
-_FORWARDS = {kind: kind.forward for kind in (nn.Linear, nn.LayerNorm, nn.Dropout)}       # (and Attention, below)
+_FORWARDS = {kind: kind.forward for kind in (nn.Linear, nn.LayerNorm, nn.Dropout, nn.Embedding)}       # (and Attention, below)
 
 
 def _plain(module, kind):
@@ -51,10 +55,14 @@ def _kernel_operand(t, shape, device):
 
 class RobertaEmbeddings(nn.Module):
     """word + token-type + position embeddings, LayerNorm, dropout
-    (src/roberta/models/postnorm.py:6-28); positions are offset by pad_token_id + 1."""
+    (src/roberta/models/postnorm.py:6-28); positions are offset by pad_token_id + 1.
 
-    def __init__(self, config):
+    kernels: the tables are read, and their gradients summed, by this package's ``embedding`` (the same numbers forward; gradients that cannot be
+    differentiated again) wherever a table is the nn.Embedding it was built with."""
+
+    def __init__(self, config, kernels=False):
         super().__init__()
+        self.kernels = kernels
         self.pad_token_id = config.pad_token_id
         self.word_embeddings = nn.Embedding(config.vocab_size, config.hidden_size)
         self.position_embeddings = nn.Embedding(config.max_position_embeddings + 2, config.hidden_size)
@@ -62,10 +70,16 @@ class RobertaEmbeddings(nn.Module):
         self.LayerNorm = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_eps)
         self.dropout = nn.Dropout(config.hidden_dropout_prob)
 
+    def _rows(self, table, ids):
+        if (self.kernels and _plain(table, nn.Embedding) and table.weight.is_cuda and table.max_norm is None and not table.sparse
+                and not table.scale_grad_by_freq):
+            return embedding(ids, table.weight, padding_idx=table.padding_idx)
+        return table(ids)
+
     def forward(self, input_ids, token_type_ids, position_ids):
-        x = (self.word_embeddings(input_ids)
-             + self.token_type_embeddings(token_type_ids)
-             + self.position_embeddings(position_ids + (self.pad_token_id + 1)))
+        x = (self._rows(self.word_embeddings, input_ids)
+             + self._rows(self.token_type_embeddings, token_type_ids)
+             + self._rows(self.position_embeddings, position_ids + (self.pad_token_id + 1)))
         return self.dropout(self.LayerNorm(x))
 
 
@@ -304,3 +318,42 @@ class Lookup(nn.Module):
 
     def set_input_embeddings(self, value):
         self.embeddings.word_embeddings = value
+
+
+class MaskedLMHead(nn.Module):
+    """What the reference pre-trains its encoder by (src/roberta/tasks/mlm.py:33-112), behind the encoder: a projection, gelu and layer norm of the states, and the projection
+    to the vocabulary by the word embeddings with a bias of its own.  With labels the loss, whose logits are never in memory as a whole and whose cost is that of the
+    labelled tokens (``linear_cross_entropy``); without, the logits.
+
+    ``config``: hidden_size, vocab_size, layer_norm_eps."""
+
+    def __init__(self, config):
+        super().__init__()
+        self.dense = nn.Linear(config.hidden_size, config.hidden_size)
+        self.LayerNorm = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_eps)
+        self.bias = nn.Parameter(torch.zeros(config.vocab_size))
+
+    def forward(self, hidden_states, word_embeddings, labels=None, *, ignore_index=-100, reduction="mean"):
+        """hidden_states [..., hidden], word_embeddings [vocabulary, hidden], labels [...] (ignore_index: not asked for) -> the loss, by ``reduction``; without labels
+        the logits [..., vocabulary]."""
+        norm = self.LayerNorm
+        hidden = layer_norm(F.gelu(self.dense(hidden_states)), norm.weight, norm.bias, eps=norm.eps)
+        if labels is None:
+            return F.linear(hidden, word_embeddings, self.bias)
+        # (under autocast the states are 16 bits wide, and the projection is as any other's)
+        return linear_cross_entropy(hidden, word_embeddings.to(hidden.dtype), self.bias, labels, ignore_index=ignore_index, reduction=reduction)
+
+
+class LookupForMaskedLM(nn.Module):
+    """``Lookup`` and ``MaskedLMHead``, which projects by the encoder's word embeddings: what the reference trains (src/roberta/tasks/mlm.py:33-112).  GPU only, as the
+    embeddings' kernels are; forward(..., labels) -> the mean loss of the labelled tokens, without labels the logits."""
+
+    def __init__(self, config):
+        super().__init__()
+        self.encoder = Lookup(config)
+        self.encoder.embeddings.kernels = True
+        self.head = MaskedLMHead(config)
+
+    def forward(self, input_ids, token_type_ids, position_ids, attention_mask, labels=None, **kwargs):
+        states, _ = self.encoder(input_ids, token_type_ids, position_ids, attention_mask, **kwargs)
+        return self.head(states, self.encoder.get_input_embeddings().weight, labels)
