@@ -35,7 +35,7 @@ struct Kept {
     int32_t *head;      // [4]: labelled tokens; the exponents of the largest of their rows and of the weights (two-term numbers)
     int32_t *pos;       // [N]: where a token's row is among the labelled ones, or -1
     int32_t *label;     // [labelled]
-    float2 *level;      // [labelled]: a token's largest logit, and one over the sum of the exponentials of what they are below it
+    float2 *level;      // [labelled]: a token's largest logit times log2(e), and one over the sum of the exponentials of what they are below it
 };                      // (the last two up to a whole tile: tiles are read whole)
 int64_t kept_bytes(int64_t N) { return 16 + up(N * 4, 16) + up(N, TILE) * 12; }
 Kept kept_at(void *at, int64_t N) {
@@ -356,7 +356,20 @@ struct ForwardArgs {
 
 __device__ __forceinline__ float2 joined(float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.f : m;
-    return make_float2(m, a.y * __builtin_amdgcn_exp2f((a.x - from) * LOG2E) + b.y * __builtin_amdgcn_exp2f((b.x - from) * LOG2E));
+    return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - from) + b.y * __builtin_amdgcn_exp2f(b.x - from));
+}
+
+// Adds 16 logits of a token to its largest and sum so far.  Levels are logits times log2(e): an exponential is one product with a sum, rounded once, and the power of two of that.
+__device__ __forceinline__ float2 with_logits(float2 of, const float (&l)[16]) {
+    float most = l[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) most = fmaxf(most, l[e]);
+    most = fmaxf(of.x, most * LOG2E);
+    const float from = most == -INFINITY ? 0.f : most;
+    float sum = of.y * __builtin_amdgcn_exp2f(of.x - from);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(l[e], LOG2E, -from));
+    return make_float2(most, sum);
 }
 
 template <typename F>
@@ -378,14 +391,7 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
             for (int i = 0; i < MB; ++i) {
                 float l[16];
                 logits_of<F>(l, sums.v[i][j], by, (wm * MB + i) * 32, row_scale);
-                float most = of.x;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) most = fmaxf(most, l[e]);
-                const float from = most == -INFINITY ? 0.f : most;
-                float sum = of.y * __builtin_amdgcn_exp2f((of.x - from) * LOG2E);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f((l[e] - from) * LOG2E);
-                of = make_float2(most, sum);
+                of = with_logits(of, l);
                 const int r = at - 32 * i;
                 if (r >= 0 && r < 32 && r / 4 % 2 == half) {
                     float found = l[0];
@@ -514,14 +520,10 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < JB; ++j) {
-            float most = of[j].x;
+            float l[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) most = fmaxf(most, sums[j][e]);
-            const float from = most == -INFINITY ? 0.f : most;
-            float sum = of[j].y * __builtin_amdgcn_exp2f((of[j].x - from) * LOG2E);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f((sums[j][e] - from) * LOG2E);
-            of[j] = make_float2(most, sum);
+            for (int e = 0; e < 16; ++e) l[e] = sums[j][e];
+            of[j] = with_logits(of[j], l);
             const int r = label[j] - v0;
             if (label[j] >= 0 && r >= 0 && r < 32 && r / 4 % 2 == half) {
                 float found = sums[j][0];
@@ -579,7 +581,8 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     if (slice == 0 && n < labelled) {
 #pragma unroll
         for (int i = 1; i < 16; ++i) of = joined(of, shares[i][in]);
-        const float loss = (of.x - a.at_label[n]) + __logf(of.y);
+        // (log2(e), rounded alike in both, falls out)
+        const float loss = (fmaf(-a.at_label[n], LOG2E, of.x) + __builtin_amdgcn_logf(of.y)) * (1.f / LOG2E);
         a.kept.level[n] = make_float2(of.x, 1.f / of.y);
         if (a.loss) a.loss[a.token[n]] = loss;
         else a.losses[n] = loss;
@@ -723,7 +726,7 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
                 float l[16];
                 logits_of<F>(l, sums.v[i][j], beside_, (wm * MB + i) * 32, scale);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) l[e] = __builtin_amdgcn_exp2f((l[e] - level.x) * LOG2E) * p_by;
+                for (int e = 0; e < 16; ++e) l[e] = __builtin_amdgcn_exp2f(fmaf(l[e], LOG2E, -level.x)) * p_by;
                 const int r = at - 32 * i;
                 if (r >= 0 && r < 32 && r / 4 % 2 == half) {
 #pragma unroll
