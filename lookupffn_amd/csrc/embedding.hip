@@ -11,22 +11,10 @@ namespace {
 
 constexpr int WG = 256;
 constexpr int BITS = 9, DIGITS = 1 << BITS;
-constexpr int SORT_WG = 1024, CHUNK = 2048, EACH = CHUNK / SORT_WG, PER_WAVE = EACH * 64;        // tokens that a workgroup sorts
+constexpr int SORT_WG = 1024, CHUNK = SORT_WG;      // tokens that a workgroup sorts, a thread each (two: 14.3 us for two passes over 32768 tokens instead of 13.1)
+constexpr int ONE_MOST = 2;                  // tokens a thread has, at most, where one workgroup sorts all (2048 tokens 17.7 us with their sums; 4096 tokens would be 23.2 instead of 22.1)
 constexpr int FILL_BYTES = 64 * 1024;        // of a workgroup that clears
 constexpr int JOIN_WG = 512;
-
-// A number of a format by itself.
-template <typename E, int B>
-struct Single {
-    static constexpr int N = 1, BYTES = B;
-    typedef E raw_t;
-    static __device__ __forceinline__ void unpack(const E &u, float (&v)[1]) { v[0] = (float)u; }
-    static __device__ __forceinline__ E pack(const float (&v)[1]) { return (E)v[0]; }
-};
-template <typename R>
-struct Vectors : R {
-    typedef uint4 raw_t;
-};
 
 struct Args {
     const void *ids, *weight;
@@ -110,11 +98,8 @@ __global__ __launch_bounds__(SORT_WG) void count_kernel(SortArgs a) {
     __shared__ int32_t count[DIGITS];
     if (threadIdx.x < DIGITS) count[threadIdx.x] = 0;
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-        const uint32_t i = blockIdx.x * uint32_t(CHUNK) + k * SORT_WG + threadIdx.x;
-        if (i < a.tokens) atomicAdd(&count[entry(a, i).x >> a.shift & (DIGITS - 1)], 1);
-    }
+    const uint32_t i = blockIdx.x * uint32_t(CHUNK) + threadIdx.x;
+    if (i < a.tokens) atomicAdd(&count[entry(a, i).x >> a.shift & (DIGITS - 1)], 1);
     __syncthreads();
     if (threadIdx.x < DIGITS) a.counts[int64_t(blockIdx.x) * DIGITS + threadIdx.x] = count[threadIdx.x];
 }
@@ -126,7 +111,8 @@ struct Sorter {
     int32_t total[DIGITS / 64];
 };
 
-// A thread's entries are numbers wave * PER_WAVE + k * 64 + lane of the chunk: -> which of its digit's an entry is within its wavefront.
+// A thread's entries are numbers (wave * EACH + k) * 64 + lane of the chunk: -> which of its digit's an entry is within its wavefront.
+template <int EACH>
 __device__ __forceinline__ void rank_entries(Sorter &s, const uint2 (&e)[EACH], const bool (&live)[EACH], int shift, int (&rank)[EACH]) {
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     for (int d = lane; d < DIGITS; d += 64) s.had[wave][d] = 0;
@@ -175,16 +161,13 @@ __device__ __forceinline__ int place_of(const Sorter &s, uint32_t digit, int ran
 __global__ __launch_bounds__(SORT_WG) void sort_kernel(SortArgs a) {
     if ((int)blockIdx.x >= a.chunks) return clear(a.fill, blockIdx.x - a.chunks);
     __shared__ Sorter s;
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    uint2 e[EACH];
-    bool live[EACH];
-    int rank[EACH];
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-        const uint32_t i = blockIdx.x * uint32_t(CHUNK) + wave * PER_WAVE + k * 64 + lane;
-        live[k] = i < a.tokens;
-        e[k] = live[k] ? entry(a, i) : make_uint2(0, 0);
-    }
+    const int tid = threadIdx.x;
+    uint2 e[1];
+    bool live[1];
+    int rank[1];
+    const uint32_t i = blockIdx.x * uint32_t(CHUNK) + tid;
+    live[0] = i < a.tokens;
+    e[0] = live[0] ? entry(a, i) : make_uint2(0, 0);
     // a digit's entries in the chunks before this one and in all
     int before = 0, all = 0;
     if (tid < DIGITS) {
@@ -199,23 +182,22 @@ __global__ __launch_bounds__(SORT_WG) void sort_kernel(SortArgs a) {
     if (tid < DIGITS) s.place[tid] = begin + before;
     rank_entries(s, e, live, a.shift, rank);
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < EACH; ++k)
-        if (live[k]) a.to[place_of(s, e[k].x >> a.shift & (DIGITS - 1), rank[k])] = e[k];
+    if (live[0]) a.to[place_of(s, e[0].x >> a.shift & (DIGITS - 1), rank[0])] = e[0];
 }
 
-// All passes of one chunk, by one workgroup in LDS.
+// All passes of EACH * SORT_WG tokens, by one workgroup in LDS.
+template <int EACH>
 __global__ __launch_bounds__(SORT_WG) void sort_one_kernel(SortArgs a, int passes) {
     if (blockIdx.x >= 1) return clear(a.fill, blockIdx.x - 1);
     __shared__ Sorter s;
-    __shared__ uint2 list[CHUNK];
+    __shared__ uint2 list[EACH * SORT_WG];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     uint2 e[EACH];
     bool live[EACH];
     int rank[EACH];
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
-        const uint32_t i = wave * PER_WAVE + k * 64 + lane;
+        const uint32_t i = (wave * EACH + k) * 64 + lane;
         live[k] = i < a.tokens;
         e[k] = live[k] ? entry(a, i) : make_uint2(0, 0);
     }
@@ -238,7 +220,7 @@ __global__ __launch_bounds__(SORT_WG) void sort_one_kernel(SortArgs a, int passe
         if (p + 1 < passes) {
 #pragma unroll
             for (int k = 0; k < EACH; ++k)
-                if (live[k]) e[k] = list[wave * PER_WAVE + k * 64 + lane];
+                if (live[k]) e[k] = list[(wave * EACH + k) * 64 + lane];
         }
     }
 }
@@ -458,7 +440,7 @@ extern "C" int lffn_embedding_bwd(const lffn_embedding *c, const void *g, void *
     uint2 *const lists[2] = {reinterpret_cast<uint2 *>(ws + s.counts), reinterpret_cast<uint2 *>(ws + s.counts + s.lists)};
     const int64_t size = c->format == LFFN_ROWS_F32 ? 4 : 2, bytes = c->rows * c->columns * size;
     // every launch that sorts clears an equal share
-    const bool one = s.chunks == 1;
+    const bool one = c->tokens > 0 && c->tokens <= ONE_MOST * SORT_WG;
     const int launches = c->tokens == 0 || one ? 1 : 2 * s.passes;
     const int64_t share = (bytes / launches + 1023) / 1024 * 1024;
     const bool vectors = c->columns * size % 16 == 0 && lffn_aligned16(g);
@@ -471,8 +453,9 @@ extern "C" int lffn_embedding_bwd(const lffn_embedding *c, const void *g, void *
     for (int i = 0; i < launches; ++i) {
         const int64_t first = i * share < bytes ? i * share : bytes, end = i + 1 == launches || (i + 1) * share > bytes ? bytes : (i + 1) * share;
         a.fill = {static_cast<char *>(grad) + first, end - first};
-        const dim3 grid(unsigned(s.chunks + (a.fill.bytes + FILL_BYTES - 1) / FILL_BYTES)), block(SORT_WG);
-        if (one) sort_one_kernel<<<grid, block, 0, st>>>(a, s.passes);
+        const dim3 grid(unsigned((one ? 1 : s.chunks) + (a.fill.bytes + FILL_BYTES - 1) / FILL_BYTES)), block(SORT_WG);
+        if (one && c->tokens <= SORT_WG) sort_one_kernel<1><<<grid, block, 0, st>>>(a, s.passes);
+        else if (one) sort_one_kernel<ONE_MOST><<<grid, block, 0, st>>>(a, s.passes);
         else if (i % 2 == 0) {
             if (i > 0) a.from = a.to, a.to = lists[i / 2 % 2];
             a.shift = i / 2 * BITS;

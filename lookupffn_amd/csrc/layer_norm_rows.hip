@@ -14,19 +14,6 @@ constexpr int WG = 256;
 constexpr int PARTS = 1024;              // workgroups of a backward, at most: each leaves two rows of sums
 constexpr int WIDE_COLUMNS = 1024;       // columns of a workgroup that adds up a wide backward's columns
 
-// A number of a format by itself.
-template <typename E, int B>
-struct Single {
-    static constexpr int N = 1, BYTES = B;
-    typedef E raw_t;
-    static __device__ __forceinline__ void unpack(const E &u, float (&v)[1]) { v[0] = (float)u; }
-    static __device__ __forceinline__ E pack(const float (&v)[1]) { return (E)v[0]; }
-};
-template <typename R>
-struct Vectors : R {
-    typedef uint4 raw_t;
-};
-
 struct Args {
     const void *x, *w, *b, *g;
     void *y, *gx;

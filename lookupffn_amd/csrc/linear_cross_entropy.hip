@@ -616,7 +616,7 @@ struct BackwardArgs {
     const float *g_loss;       // [1] or [N]
     float *coefficient;        // [labelled] or null: what d is multiplied with beside `factor`
     float *power;              // [1]: of both gradients, where there are coefficients
-    int32_t *shares;           // [1]
+    int32_t *shares;           // [2]: of the vocabulary, for dh; pieces that there are (both from the first piece's launch)
     void *grad_hidden, *grad_weight, *grad_bias;
     int32_t bias_format, reduction, pieces;
 };
@@ -629,6 +629,7 @@ __host__ __device__ constexpr int64_t widest(int64_t bytes, int64_t rows, int pl
 struct Piece {
     int v0, width, ld, nt;     // entries; numbers from row to row of d; tiles of tokens
     int steps;                 // of dh's sum over the entries of a whole piece
+    int pieces;
 };
 template <typename F>
 __device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, int piece) {
@@ -637,7 +638,8 @@ __device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, i
     p.nt = (labelled + TILE - 1) / TILE;
     const int64_t rows = max(p.nt, 1) * int64_t(TILE);
     const int tiles = int(a.o.s.Vp / TILE), most = (int)min(int64_t(tiles), widest(a.d_bytes, rows, F::PLANES) / TILE);
-    const int pieces = (tiles + most - 1) / most, whole = (tiles + pieces - 1) / pieces * TILE;            // as few as fit, and all alike
+    p.pieces = (tiles + most - 1) / most;                  // as few as fit, and all alike
+    const int whole = (tiles + p.pieces - 1) / p.pieces * TILE;
     p.ld = whole + APART;
     p.v0 = (int)min(int64_t(piece) * whole, int64_t(a.o.s.V));
     p.width = min(whole, a.o.s.V - p.v0);
@@ -701,8 +703,32 @@ __global__ __launch_bounds__(1024) void coefficient_kernel(BackwardArgs a) {
     if (tid == 0) *a.power = __builtin_amdgcn_ldexpf(1.f / LIFT, e);
 }
 
+// A block's 32 numbers of each column, 16 a lane (mfma_row), packed: w[k] has 16 bytes of column 16 k + lane % 16, the piece_of_lane-th of its four.  Lanes 32 apart and then lanes 16 apart
+// exchange halves, so that what four lanes store of a row is 64 bytes together (32 bytes at a time took the cache twice as many writes).
+__device__ __forceinline__ int piece_of_lane(int lane) { return lane / 16 % 2 * 2 + lane / 32; }
+template <typename F>
+__device__ __forceinline__ void pieces_of(const float (&l)[16], uint4 (&w)[2]) {
+    uint32_t p[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const auto s = __builtin_amdgcn_permlane32_swap(F::pack2(l[8 * h + 2 * e], l[8 * h + 2 * e + 1]), F::pack2(l[8 * h + 4 + 2 * e], l[8 * h + 5 + 2 * e]), false, false);
+            p[h][e] = s[0], p[h][2 + e] = s[1];
+        }
+    uint32_t q[2][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const auto s = __builtin_amdgcn_permlane16_swap(p[0][e], p[1][e], false, false);
+        q[0][e] = s[0], q[1][e] = s[1];
+    }
+    w[0] = make_uint4(q[0][0], q[0][1], q[0][2], q[0][3]);
+    w[1] = make_uint4(q[1][0], q[1][1], q[1][2], q[1][3]);
+}
+
 template <typename F>
 __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece) {
+    if (piece > 0 && piece >= a.shares[1]) return;
     extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
     const uint32_t lds = lds_byte_of(lds_words);
     const Operands &o = a.o;
@@ -720,7 +746,7 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
             const float2 level = live ? beside<float2>(beside_, LEVEL, column) : make_float2(INFINITY, 0.f);
             const float by = LIFT * (a.coefficient ? beside<float>(beside_, COEFFICIENT, column) : 1.f), p_by = live ? level.y * by : 0.f;
             const int at = live ? beside<int>(beside_, LABEL, column) - p.v0 - in : -1;
-            char *const row = a.d + (int64_t(n) * p.ld + in) * 2;
+            char *const row = a.d + (int64_t(n - lane % 32 + lane % 16) * p.ld + in + 8 * piece_of_lane(lane)) * 2;       // (of the block's first 16 tokens)
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 float l[16];
@@ -737,18 +763,10 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
                     stored = true;
                 }
                 auto put = [&](char *to) {
-#pragma unroll
-                    for (int g = 0; g < 4; g += 2) {
-                        // the lanes of a row exchange four numbers of two groups, so that each has eight that lie together
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const auto s = __builtin_amdgcn_permlane32_swap(F::pack2(l[4 * g + 2 * e], l[4 * g + 2 * e + 1]),
-                                                                            F::pack2(l[4 * g + 4 + 2 * e], l[4 * g + 5 + 2 * e]), false, false);
-                            w[e] = s[0], w[2 + e] = s[1];
-                        }
-                        *reinterpret_cast<uint4 *>(to + (32 * i + 8 * (g + half)) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    uint4 w[2];
+                    pieces_of<F>(l, w);
+                    *reinterpret_cast<uint4 *>(to + 64 * i) = w[0];
+                    *reinterpret_cast<uint4 *>(to + 64 * i + 32 * int64_t(p.ld)) = w[1];
                 };
                 put(row);
                 if constexpr (F::PLANES == 2) {
@@ -762,7 +780,7 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
     // (one of the workgroups that have the fewest tiles)
     if (piece == 0 && blockIdx.x == gridDim.x - 1 && wave == 0) {
         const int shares = shares_of<F>(a, labelled);
-        if (lane == 0) *a.shares = shares;
+        if (lane == 0) a.shares[0] = shares, a.shares[1] = p.pieces;
     }
 }
 
@@ -901,6 +919,22 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
                 }
             }
             char *const row = static_cast<char *>(a.grad_weight) + int64_t(v) * o.s.K * R::BYTES;
+            if constexpr (R::BYTES == 2) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+                    float l[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) l[e] = sums.v[i][j][e] * by;
+                    uint4 w[2];
+                    pieces_of<F>(l, w);
+                    const int h = h0 + (wm * MB + i) * 32 + 8 * piece_of_lane(lane), first = in - lane % 32 + lane % 16;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (first + 16 * k < p.width && h < o.s.K)
+                            *reinterpret_cast<uint4 *>(static_cast<char *>(a.grad_weight) + (int64_t(p.v0 + first + 16 * k) * o.s.K + h) * 2) = w[k];
+                }
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -925,6 +959,7 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
 // Both gradients of a piece.
 template <typename F, typename R>
 __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, int piece) {
+    if (piece > 0 && piece >= a.shares[1]) return;
     extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
     const uint32_t lds = lds_byte_of(lds_words);
     const int labelled = a.o.kept.head[0];
@@ -1064,7 +1099,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     b.parts = c.take<float>(b.parts_bytes / 4);
     b.coefficient = c.take<float>(a.reduction == 0 ? Np : 0);
     b.power = c.take<float>(1);
-    b.shares = c.take<int32_t>(1);
+    b.shares = c.take<int32_t>(2);
     if (a.reduction != 0) b.coefficient = nullptr;
     // as many launches as pieces if all tokens are labelled; with fewer the last ones find nothing
     const int64_t entries = a.tokens == 0 ? 0 : widest(b.d_bytes, Np, (int)planes);

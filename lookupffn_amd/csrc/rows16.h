@@ -37,3 +37,16 @@ struct Row16 {
 };
 typedef Row16<__bf16> BF16Row;
 typedef Row16<_Float16> F16Row;
+
+// What a lane loads and stores at a time: a row's 16 bytes, or, where addresses or widths are not of 16 bytes, a number.
+template <typename R>
+struct Vectors : R {
+    typedef uint4 raw_t;
+};
+template <typename E, int B>
+struct Single {
+    static constexpr int N = 1, BYTES = B;
+    typedef E raw_t;
+    static __device__ __forceinline__ void unpack(const E &u, float (&v)[1]) { v[0] = (float)u; }
+    static __device__ __forceinline__ E pack(const float (&v)[1]) { return (E)v[0]; }
+};
