@@ -981,34 +981,35 @@ __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, i
     if (a.grad_weight) weight_tasks<F, R>(a, p, labelled, unit, lds);
 }
 
-// dh: a labelled token's shares added up, zeros for the others; four threads for eight columns.
-template <typename F, typename R>
+// dh: a labelled token's shares added up, zeros for the others; EACH threads for eight columns.
+template <typename F, typename R, int EACH>
 __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
-    __shared__ float4 sums[3][64][2];
+    constexpr int PLACES = 256 / EACH;
+    __shared__ float4 sums[EACH][EACH > 1 ? PLACES : 1][2];
     const Sizes &s = a.o.s;
-    const int in = threadIdx.x % 64, part = threadIdx.x / 64, pieces = s.K / 8;
-    const int64_t i = int64_t(blockIdx.x) * 64 + in, t = i / pieces, c = i % pieces * 8;
+    const int in = threadIdx.x % PLACES, part = threadIdx.x / PLACES, pieces = s.K / 8;
+    const int64_t i = int64_t(blockIdx.x) * PLACES + in, t = i / pieces, c = i % pieces * 8;
     const int at = t < s.N ? a.o.kept.pos[t] : -1, labelled = a.o.kept.head[0];
     float v[8] = {};
+    auto add = [&](const float4 &x, const float4 &y) { v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w; };
     if (at >= 0) {
         const int steps = piece_of<F>(a, labelled, 0).steps, wanted = *a.shares, length = (steps + 2 * wanted - 1) / (2 * wanted) * 2, shares = (steps + length - 1) / length;
 #pragma unroll 4
-        for (int p = part; p < shares; p += 4) {
+        for (int p = part; p < shares; p += EACH) {
             const float *from = a.parts + (int64_t(p) * labelled + at) * s.K + c;
-            const float4 x = *reinterpret_cast<const float4 *>(from), y = *reinterpret_cast<const float4 *>(from + 4);
-            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+            add(*reinterpret_cast<const float4 *>(from), *reinterpret_cast<const float4 *>(from + 4));
         }
-        if (part > 0) sums[part - 1][in][0] = make_float4(v[0], v[1], v[2], v[3]), sums[part - 1][in][1] = make_float4(v[4], v[5], v[6], v[7]);
     }
-    __syncthreads();
-    if (part > 0 || t >= s.N) return;
+    if constexpr (EACH > 1) {
+        sums[part][in][0] = make_float4(v[0], v[1], v[2], v[3]), sums[part][in][1] = make_float4(v[4], v[5], v[6], v[7]);
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int p = 1; p < EACH; ++p) add(sums[p][in][0], sums[p][in][1]);
+    }
+    if (t >= s.N) return;
     if (at >= 0) {
         const float by = factor_of(a, labelled) * (F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, a.o.kept.head[2]) : 1.f);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            const float4 x = sums[p][in][0], y = sums[p][in][1];
-            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= by;
     }
@@ -1168,7 +1169,9 @@ int backward(const BackwardArgs &b, hipStream_t st) {
     }
     if (b.grad_hidden) {
         const int64_t n = int64_t(b.o.s.N) * (b.o.s.K / 8);
-        hidden_kernel<F, R><<<dim3(unsigned((n + 63) / 64)), dim3(256), 0, st>>>(b);
+        // four threads where one each would leave the chip without enough in flight (385 x 520 fp32 16.4 us with one, 11.4 with four; 32768 x 512, 4915 labelled, half 27 and 36)
+        if (n < COMPUTE_UNITS * 256) hidden_kernel<F, R, 4><<<dim3(unsigned((n + 63) / 64)), dim3(256), 0, st>>>(b);
+        else hidden_kernel<F, R, 1><<<dim3(unsigned((n + 255) / 256)), dim3(256), 0, st>>>(b);
     }
     return LFFN_OK;
 }
