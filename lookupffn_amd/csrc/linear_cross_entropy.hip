@@ -413,14 +413,17 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
 
 // ---------------------------------------------------------------- few tokens
 
-// Up to 64 tokens of 16 bits: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a time, whose
-// rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, six such in flight.  Nothing is laid together before: a launch less.
-constexpr int FEW = 64, FEW_AHEAD = 6;
-constexpr int few_stride(int columns) { return int(up(columns, STEP)) / 8 | 1; }                // 16-byte pieces of a row in LDS: odd, so that 16 rows meet every bank once
-constexpr int64_t few_lds(int64_t tokens, int64_t columns) {
-    return (tokens <= 32 ? 32 : 64) * int64_t(few_stride((int)columns)) * 16 + 8 * FEW * 8 + FEW * 4;
+// Up to 64 tokens whose rows fit LDS: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a
+// time, whose rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, six such in flight.  Nothing is laid together before: a launch less.
+// fp32 is multiplied as it is (v_mfma_f32_32x32x2_f32): at 32 tokens a product takes as long as its weights' bytes (32 x 50265 x 840 64 us; splitting the weights to memory 71 and the tiles'
+// products 100).  The exponents that the backward's two-term numbers have in common are found on the way.
+constexpr int FEW = 64, LINE = 128;                                                            // bytes of a row that a step has
+constexpr int few_stride(int64_t row_bytes) { return int(up(row_bytes, LINE)) / 16 | 1; }      // 16-byte pieces of a row in LDS: odd, so that 16 rows meet every bank once
+constexpr int64_t few_lds(int64_t tokens, int64_t row_bytes) {
+    return (tokens <= 32 ? 32 : 64) * int64_t(few_stride(row_bytes)) * 16 + 8 * FEW * 8 + FEW * 4;
 }
-bool few_tokens(const lffn_linear_cross_entropy &a) { return a.format != LFFN_ROWS_F32 && a.tokens <= FEW && few_lds(a.tokens, a.columns) <= 160 * 1024; }
+int64_t row_bytes(const lffn_linear_cross_entropy &a) { return a.columns * (a.format == LFFN_ROWS_F32 ? 4 : 2); }
+bool few_tokens(const lffn_linear_cross_entropy &a) { return a.tokens <= FEW && few_lds(a.tokens, row_bytes(a)) <= 160 * 1024; }
 
 int few_workgroups(const lffn_linear_cross_entropy &a) { return (int)min((a.vocabulary + 31) / 32, int64_t(COMPUTE_UNITS)); }
 
@@ -431,13 +434,51 @@ struct FewArgs {
     int64_t Np;
 };
 
+// Adds the products of 16 bytes of both operands.
+template <typename F>
+struct Few {
+    static constexpr int BYTES = 2, SUMS = 1;
+    static __device__ __forceinline__ void add(f32x16_t (&sums)[SUMS], const uint4 &w, const uint4 &x) { sums[0] = F::mma(w, x, sums[0]); }
+};
+template <>
+struct Few<F32Row> {
+    static constexpr int BYTES = 4, SUMS = 2;                  // (two sums: half as many roundings each, of half the size)
+    static __device__ __forceinline__ void add(f32x16_t (&sums)[SUMS], const uint4 &w, const uint4 &x) {
+        const float4 a = __builtin_bit_cast(float4, w), b = __builtin_bit_cast(float4, x);
+        sums[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, sums[0], 0, 0, 0);
+        sums[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, sums[1], 0, 0, 0);
+        sums[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, sums[0], 0, 0, 0);
+        sums[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, sums[1], 0, 0, 0);
+    }
+};
+__device__ __forceinline__ float most_of(const uint4 &u, float most) {
+    const float4 v = __builtin_bit_cast(float4, u);
+    return fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+}
+// The exponent that two-term numbers of largest magnitude `most` have, to *exponent: one atomic of a workgroup.
+__device__ __forceinline__ void raise_by(int32_t *exponent, float most, float *red) {
+    most = wave_most(most);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (unsigned i = 1; i < blockDim.x / 64; ++i) most = fmaxf(most, red[i]);
+        int e;
+        scale_to(most, 13, e);
+        atomicMax(exponent, e);
+    }
+}
+
 template <typename F, int TOKENS>
 __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
-    constexpr int JB = TOKENS / 32, WAVES = THREADS / 64;
+    typedef Few<F> Of;
+    constexpr int JB = TOKENS / 32, WAVES = THREADS / 64, BYTES = Of::BYTES;
+    constexpr bool WHOLE = BYTES == 4;
+    constexpr int AHEAD = WHOLE && TOKENS == 64 ? 4 : 6;       // steps in flight (what the registers have room for)
     extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
     const Operands &o = a.r.o;
     const int V = o.s.V, K = o.s.K, tid = threadIdx.x, wave = tid / 64, lane = tid % 64, half = lane / 32;
-    const int stride = few_stride(K), pieces = int(up(K, STEP)) / 8, steps = pieces / 8;
+    const int bytes = K * BYTES, stride = few_stride(bytes), pieces = int(up(bytes, LINE)) / 16, steps = pieces / 8;
     float2 *const waves = reinterpret_cast<float2 *>(lds_words + TOKENS * stride);       // [WAVES][TOKENS]
     int *const tokens = reinterpret_cast<int *>(waves + WAVES * TOKENS);                 // [TOKENS]
     // the labelled tokens: every wavefront sees them all
@@ -453,20 +494,24 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
             else if (a.r.loss) a.r.loss[lane] = 0.f;
         }
     }
-    if (labelled == 0) return;
+    if (labelled == 0) {
+        if (WHOLE && blockIdx.x == 0 && tid == 0) o.kept.head[1] = o.kept.head[2] = 0;
+        return;
+    }
     const int blocks = (V + 31) / 32, all = gridDim.x * WAVES;
     int block = wave * gridDim.x + blockIdx.x;
-    uint4 w[FEW_AHEAD][4];
+    uint4 w[AHEAD][4];
+    float most = 0.f, most_x = 0.f;                // of the weights, of the rows
     const char *row = nullptr;
     auto begin_block = [&] { row = o.weight.at + int64_t(min(block * 32 + lane % 32, V - 1)) * o.weight.stride; };
     auto load = [&](int s, uint4 (&to)[4]) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) to[c] = *reinterpret_cast<const uint4 *>(row + min(s * 64 + half * 32 + c * 8, K - 8) * 2);
+        for (int c = 0; c < 4; ++c) to[c] = *reinterpret_cast<const uint4 *>(row + min(s * LINE + half * 64 + c * 16, bytes - 16));
     };
     if (block < blocks) {
         begin_block();
 #pragma unroll
-        for (int s = 0; s < FEW_AHEAD; ++s) load(s, w[s]);
+        for (int s = 0; s < AHEAD; ++s) load(s, w[s]);
     }
     __syncthreads();
     // (six pieces a thread in flight: 22.0 us for 64 x 50265 x 768 instead of 24.2 one after the other)
@@ -477,12 +522,13 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
         for (int k = 0; k < BATCH; ++k) {
             const int i = i0 + k * THREADS, r = i / pieces, p = i - r * pieces;
             v[k] = make_uint4(0, 0, 0, 0);
-            if (r < labelled && p * 8 < K) v[k] = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.r.hidden) + (tokens[r] * a.r.hidden_stride + p * 8) * 2);
+            if (r < labelled && p * 16 < bytes) v[k] = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.r.hidden) + tokens[r] * a.r.hidden_stride * BYTES + p * 16);
         }
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
             const int i = i0 + k * THREADS, r = i / pieces, p = i - r * pieces;
             if (r < TOKENS) lds_words[r * stride + p] = v[k];
+            if constexpr (WHOLE) most_x = most_of(v[k], most_x);
         }
     }
     __syncthreads();
@@ -496,27 +542,30 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
         of[j] = make_float2(-INFINITY, 0.f);
     }
     for (; block < blocks; block += all) {
-        f32x16_t sums[JB];
+        f32x16_t sums[JB][Of::SUMS];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int v = block * 32 + mfma_row(e, half);
             const float b = v >= V ? -INFINITY : a.r.bias_format < 0 ? 0.f : bias_of(a.r.bias, a.r.bias_format, v);
 #pragma unroll
-            for (int j = 0; j < JB; ++j) sums[j][e] = b;
+            for (int j = 0; j < JB; ++j) {
+                sums[j][0][e] = b;
+                if constexpr (WHOLE) sums[j][1][e] = 0.f;
+            }
         }
-        for (int s0 = 0; s0 < steps; s0 += FEW_AHEAD) {
+        for (int s0 = 0; s0 < steps; s0 += AHEAD) {
 #pragma unroll
-            for (int k = 0; k < FEW_AHEAD; ++k) {
+            for (int k = 0; k < AHEAD; ++k) {
                 const int s = s0 + k;
                 if (s < steps) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c) {
 #pragma unroll
-                        for (int j = 0; j < JB; ++j) {
-                            const uint4 x = __builtin_bit_cast(uint4, *(const lds_word_t *)(uintptr_t)(lds + (j * 32 * stride + s * 8 + c) * 16));
-                            sums[j] = F::mma(w[k][c], x, sums[j]);
-                        }
-                    if (s + FEW_AHEAD < steps) load(s + FEW_AHEAD, w[k]);
+                        for (int j = 0; j < JB; ++j)
+                            Of::add(sums[j], w[k][c], __builtin_bit_cast(uint4, *(const lds_word_t *)(uintptr_t)(lds + (j * 32 * stride + s * 8 + c) * 16)));
+                        if constexpr (WHOLE) most = most_of(w[k][c], most);
+                    }
+                    if (s + AHEAD < steps) load(s + AHEAD, w[k]);
                 }
             }
         }
@@ -526,19 +575,19 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
             begin_block();
             block -= all;
 #pragma unroll
-            for (int s = 0; s < FEW_AHEAD; ++s) load(s, w[s]);
+            for (int s = 0; s < AHEAD; ++s) load(s, w[s]);
         }
 #pragma unroll
         for (int j = 0; j < JB; ++j) {
             float l[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) l[e] = sums[j][e];
+            for (int e = 0; e < 16; ++e) l[e] = WHOLE ? sums[j][0][e] + sums[j][Of::SUMS - 1][e] : sums[j][0][e];
             of[j] = with_logits(of[j], l);
             const int r = label[j] - v0;
             if (label[j] >= 0 && r >= 0 && r < 32 && r / 4 % 2 == half) {
-                float found = sums[j][0];
+                float found = l[0];
 #pragma unroll
-                for (int e = 1; e < 16; ++e) found = mfma_row(e, half) == r ? sums[j][e] : found;
+                for (int e = 1; e < 16; ++e) found = mfma_row(e, half) == r ? l[e] : found;
                 a.at_label[32 * j + lane % 32] = found;
             }
         }
@@ -554,6 +603,10 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) sum = joined(sum, waves[i * TOKENS + tid]);
         a.parts[blockIdx.x * a.Np + tid] = sum;
+    }
+    if constexpr (WHOLE) {
+        raise_by(o.kept.head + 2, most, reinterpret_cast<float *>(waves));
+        if (blockIdx.x == 0) raise_by(o.kept.head + 1, most_x, reinterpret_cast<float *>(waves));
     }
 }
 
@@ -1050,7 +1103,7 @@ struct Carver {
     }
 };
 
-Operands operands(const lffn_linear_cross_entropy &a, Carver &c) {
+Operands operands(const lffn_linear_cross_entropy &a, Carver &c, bool split) {
     Operands o{};
     const int64_t Np = up(a.tokens, TILE);
     o.s = {(int)a.tokens, (int)a.vocabulary, (int)a.columns, up(a.columns, 2 * STEP), up(a.vocabulary, TILE)};
@@ -1058,8 +1111,8 @@ Operands operands(const lffn_linear_cross_entropy &a, Carver &c) {
     o.rows_plane = Np * o.s.Kp * 2;
     o.rows = c.take<char>(o.rows_plane * planes);
     o.bias = c.take<float>(o.s.Vp);
-    o.weight = {static_cast<const char *>(a.weight), a.weight_stride * 2, 0, o.s.V, o.s.K};
-    if (planes == 2) {
+    o.weight = {static_cast<const char *>(a.weight), a.weight_stride * (planes == 2 ? 4 : 2), 0, o.s.V, o.s.K};
+    if (split) {
         o.weight_scale = c.take<float>(o.s.Vp);
         o.row_scale = c.take<float>(Np);
         const int64_t plane = a.vocabulary * a.columns * 2;
@@ -1079,7 +1132,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Fo
     Carver c{base};
     const int64_t Np = up(a.tokens, TILE);
     f = {};
-    f.f.o = operands(a, c);
+    f.f.o = operands(a, c, a.format == LFFN_ROWS_F32 && !few_tokens(a));
     f.f.Np = f.j.Np = Np;
     f.j.tiles = int((a.vocabulary + TILE - 1) / TILE);
     f.j.parts = f.f.parts = c.take<float2>((few_tokens(a) ? few_workgroups(a) : f.j.tiles) * Np);
@@ -1100,7 +1153,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     w = {};
     const int64_t Np = up(a.tokens, TILE), planes = planes_of(a), K = a.columns;
     BackwardArgs &b = w.b;
-    b.o = operands(a, c);
+    b.o = operands(a, c, planes == 2);
     const int64_t Vp = b.o.s.Vp, least = Np * ((Vp < 2048 ? Vp : 2048) + APART) * 2 * planes, whole = Np * (Vp + APART) * 2 * planes;
     b.d_bytes = least > D_BYTES ? least : whole < D_BYTES ? whole : D_BYTES;
     b.d_plane = b.d_bytes / 2;
@@ -1142,11 +1195,15 @@ constexpr size_t LDS_BYTES = STREAM_LDS + 2 * BESIDE_BYTES + WAVES_M * TILE * si
 template <typename F, int TOKENS>
 int few(const lffn_linear_cross_entropy &a, Forward &f, hipStream_t st) {
     static LdsGrant granted;
-    const int64_t lds = few_lds(a.tokens, a.columns);
+    const int64_t lds = few_lds(a.tokens, row_bytes(a));
     if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&few_kernel<F, TOKENS>), lds, granted)) return LFFN_ERR_LAUNCH;
     f.j.tiles = few_workgroups(a);
     few_kernel<F, TOKENS><<<dim3(f.j.tiles), dim3(THREADS), lds, st>>>({f.r, f.f.parts, f.f.at_label, f.f.Np});
     return LFFN_OK;
+}
+template <typename F>
+int few(const lffn_linear_cross_entropy &a, Forward &f, hipStream_t st) {
+    return a.tokens <= 32 ? few<F, 32>(a, f, st) : few<F, 64>(a, f, st);
 }
 
 template <typename F>
@@ -1207,8 +1264,7 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
     if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.losses = nullptr;
     if (a->format == LFFN_ROWS_F32 || a->tokens == 0) head_kernel<<<dim3(1), dim3(64), 0, st>>>(f.f.o.kept.head);
     if (a->tokens > 0 && few_tokens(*a)) {
-        const bool bf16 = a->format == LFFN_ROWS_BF16;
-        const int done = a->tokens <= 32 ? (bf16 ? few<BF16, 32>(*a, f, st) : few<F16, 32>(*a, f, st)) : bf16 ? few<BF16, 64>(*a, f, st) : few<F16, 64>(*a, f, st);
+        const int done = a->format == LFFN_ROWS_F32 ? few<F32Row>(*a, f, st) : a->format == LFFN_ROWS_BF16 ? few<BF16>(*a, f, st) : few<F16>(*a, f, st);
         if (done != LFFN_OK) return done;
         f.j.joining = int((a->tokens + 15) / 16);
         join_kernel<<<dim3(f.j.joining), dim3(256), 0, st>>>(f.j);
