@@ -76,6 +76,7 @@ struct SortArgs {
     int32_t *counts;           // [chunks][DIGITS]: this pass's
     uint32_t tokens, rows;
     int chunks, shift, ids_64;
+    int scanned;               // counts are those of the chunks before, and behind the last chunk's all
     Fill fill;
 };
 
@@ -102,6 +103,27 @@ __global__ __launch_bounds__(SORT_WG) void count_kernel(SortArgs a) {
     if (i < a.tokens) atomicAdd(&count[entry(a, i).x >> a.shift & (DIGITS - 1)], 1);
     __syncthreads();
     if (threadIdx.x < DIGITS) a.counts[int64_t(blockIdx.x) * DIGITS + threadIdx.x] = count[threadIdx.x];
+}
+
+// Many chunks (each reading all counts would be as much as the square of them): counts become those of the chunks before, and of all behind the last one.  16 digits a workgroup, 64 threads each.
+constexpr int SCANNED_FROM = 128;            // (a backward of 131072 tokens x 64 57 us without and with, 262144 93 and 80, 1048576 293 and 127)
+__global__ __launch_bounds__(SORT_WG) void scan_kernel(int32_t *counts, int chunks) {
+    __shared__ int32_t sums[SORT_WG / 16][17];
+    const int in = threadIdx.x % 16, slice = threadIdx.x / 16, share = (chunks + SORT_WG / 16 - 1) / (SORT_WG / 16), first = min(slice * share, chunks), end = min(first + share, chunks);
+    int32_t *const at = counts + blockIdx.x * 16 + in;
+    int sum = 0;
+#pragma unroll 8
+    for (int c = first; c < end; ++c) sum += at[int64_t(c) * DIGITS];
+    sums[slice][in] = sum;
+    __syncthreads();
+    int before = 0;
+    for (int i = 0; i < slice; ++i) before += sums[i][in];
+    for (int c = first; c < end; ++c) {
+        const int n = at[int64_t(c) * DIGITS];
+        at[int64_t(c) * DIGITS] = before;
+        before += n;
+    }
+    if (slice == SORT_WG / 16 - 1) at[int64_t(chunks) * DIGITS] = before;
 }
 
 // What a workgroup needs to put a chunk's entries in the order of a digit.
@@ -170,7 +192,10 @@ __global__ __launch_bounds__(SORT_WG) void sort_kernel(SortArgs a) {
     e[0] = live[0] ? entry(a, i) : make_uint2(0, 0);
     // a digit's entries in the chunks before this one and in all
     int before = 0, all = 0;
-    if (tid < DIGITS) {
+    if (tid < DIGITS && a.scanned) {
+        before = a.counts[int64_t(blockIdx.x) * DIGITS + tid];
+        all = a.counts[int64_t(a.chunks) * DIGITS + tid];
+    } else if (tid < DIGITS) {
 #pragma unroll 8
         for (int c = 0; c < a.chunks; ++c) {
             const int n = a.counts[int64_t(c) * DIGITS + tid];
@@ -371,7 +396,7 @@ Space space_of(const lffn_embedding &a) {
     s.passes = passes_of(a.rows);
     s.length = length_of(a.tokens);
     s.pieces = (a.tokens + s.length - 1) / s.length;
-    s.counts = up(s.chunks * DIGITS * 4);
+    s.counts = up((s.chunks + 1) * DIGITS * 4);
     s.lists = up(a.tokens * 8);
     s.parts = s.pieces * 2 * a.columns * 4;
     s.bytes = s.counts + 2 * s.lists + s.parts;
@@ -450,6 +475,7 @@ extern "C" int lffn_embedding_bwd(const lffn_embedding *c, const void *g, void *
     a.ids = c->ids, a.padding = c->padding, a.ids_64 = c->ids_64;
     a.tokens = (uint32_t)c->tokens, a.rows = (uint32_t)c->rows, a.chunks = (int)s.chunks;
     a.counts = counts, a.to = lists[0];
+    a.scanned = a.chunks > SCANNED_FROM;
     for (int i = 0; i < launches; ++i) {
         const int64_t first = i * share < bytes ? i * share : bytes, end = i + 1 == launches || (i + 1) * share > bytes ? bytes : (i + 1) * share;
         a.fill = {static_cast<char *>(grad) + first, end - first};
@@ -460,6 +486,7 @@ extern "C" int lffn_embedding_bwd(const lffn_embedding *c, const void *g, void *
             if (i > 0) a.from = a.to, a.to = lists[i / 2 % 2];
             a.shift = i / 2 * BITS;
             count_kernel<<<grid, block, 0, st>>>(a);
+            if (a.scanned) scan_kernel<<<dim3(DIGITS / 16), block, 0, st>>>(counts, a.chunks);
         } else
             sort_kernel<<<grid, block, 0, st>>>(a);
     }

@@ -9,8 +9,8 @@
 // Forward: tiles of 256 vocabulary entries x 256 tokens (product_tiles.h); a tile's logits become, in its registers, each token's largest and sum of exponentials, 8
 // bytes for 256 logits, and a second launch joins those of a token.
 // Backward: the logits of a piece of the vocabulary are formed once more, d is written in 16 bits (a float's in two terms), and one launch forms from it both gradients' products:
-// dW whole, its sum over the tokens, and dh in shares of the vocabulary, added up in fp32 in memory.  What a share adds to is its own: no atomics on results, the same bits
-// on every call.
+// dW, its sum over the tokens whole or, where its tiles are few and the tokens many, in shares of them, and dh in shares of the vocabulary, added up in fp32 in memory.  What a
+// share adds to is its own: no atomics on results, the same bits on every call.
 #include "product_tiles.h"
 
 namespace {
@@ -25,8 +25,9 @@ constexpr int COUNTED_FROM = 4096;              // tokens from which on a launch
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LIFT = 16384.f;                 // d times 2^14: half's normal numbers then reach down to 2^-28 of a row's largest
 constexpr int64_t D_BYTES = int64_t(1) << 30;   // of a piece's d, at most (with many tokens 2048 entries at least)
-constexpr int64_t PARTS_BYTES = int64_t(256) << 20;
-constexpr int SHARES = 64;                      // of the vocabulary, for dh, at most
+constexpr int64_t PARTS_BYTES = int64_t(256) << 20, WEIGHT_PARTS_BYTES = int64_t(512) << 20;
+constexpr int CUT_FROM = 2048;                  // tokens (of one plane) from which on dW's sums over them may be cut
+constexpr int SHARES = 64;                      // of the vocabulary, for dh, and of the tokens, for dW, at most
 
 __host__ __device__ constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -74,6 +75,8 @@ struct RowsArgs {
     const int32_t *counts;                     // labelled tokens of every chunk, or null
     int32_t *token;                            // [labelled]
     float *loss;                               // [N]: zeros for the others, or null
+    const float *g_loss;                       // [N]
+    float *most;                               // the backward of losses by token: of a chunk's finite g_loss
 };
 
 __device__ __forceinline__ int label_of(const void *labels, int wide, int64_t i, int64_t ignore, int V) {
@@ -92,6 +95,8 @@ __device__ __forceinline__ float wave_most(float v) {
     for (int m = 32; m > 0; m /= 2) v = fmaxf(v, __shfl_xor(v, m));
     return v;
 }
+
+__device__ __forceinline__ float wave_least(float v) { return -wave_most(-v); }
 
 // A row of `columns` numbers as the products read it, zeros up to `padded`, by one wavefront.  Two-term numbers: scaled by the row's largest, or to `exponent` where that is
 // given; -> the exponent of the way back.
@@ -114,7 +119,8 @@ __device__ __forceinline__ int lay_row(const char *from, char *to, int64_t plane
                 const float4 v = *reinterpret_cast<const float4 *>(from + c * 4);
                 most = fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
             }
-            scale = scale_to(wave_most(most), 13, e);
+            most = wave_most(most);
+            scale = scale_to(most == INFINITY ? 0.f : most, 13, e);        // (an infinite row is lost; the backward's exponent is the others')
         }
         for (int c = lane * 8; c < padded; c += 512) {
             uint32_t h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
@@ -194,7 +200,14 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
         }
     } else {
         labelled = k.head[0];
-        if (wave == 0) place[lane] = t0 + lane < s.N ? k.pos[t0 + lane] : -1;
+        if (wave == 0) {
+            const int at = t0 + lane < s.N ? k.pos[t0 + lane] : -1;
+            place[lane] = at;
+            if (a.most && part == 0) {
+                const float g = at >= 0 ? fabsf(a.g_loss[t0 + lane]) : 0.f, most = wave_most(g < INFINITY ? g : 0.f);
+                if (lane == 0) a.most[chunk] = most;
+            }
+        }
     }
     __syncthreads();
     const int64_t row_bytes = s.Kp * 2;
@@ -528,7 +541,10 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
         for (int k = 0; k < BATCH; ++k) {
             const int i = i0 + k * THREADS, r = i / pieces, p = i - r * pieces;
             if (r < TOKENS) lds_words[r * stride + p] = v[k];
-            if constexpr (WHOLE) most_x = most_of(v[k], most_x);
+            if constexpr (WHOLE) {
+                const float of_piece = most_of(v[k], 0.f);
+                most_x = fmaxf(most_x, of_piece == INFINITY ? 0.f : of_piece);       // (an infinite row is lost; the backward's exponent is the others')
+            }
         }
     }
     __syncthreads();
@@ -679,9 +695,11 @@ struct BackwardArgs {
     const float *g_loss;       // [1] or [N]
     float *coefficient;        // [labelled] or null: what d is multiplied with beside `factor`
     float *power;              // [1]: of both gradients, where there are coefficients
-    int32_t *shares;           // [2]: of the vocabulary, for dh; pieces that there are (both from the first piece's launch)
+    float *weight_parts;       // [shares, vocabulary, K] and [shares, vocabulary] of the bias, where dW's sums may be cut
+    float *bias_parts;
+    int32_t *shares;           // [3]: of the vocabulary, for dh; pieces that there are; of the tokens, for dW (all from the first piece's launch)
     void *grad_hidden, *grad_weight, *grad_bias;
-    int32_t bias_format, reduction, pieces;
+    int32_t bias_format, reduction, pieces, weight_shares;         // the last: at most
 };
 
 // Entries of a piece, whole tiles, that fit so many bytes.  d's rows are some more apart: rows at a distance of a power of two would share few of the cache's channels.
@@ -713,33 +731,63 @@ __device__ __forceinline__ Piece piece_of(const BackwardArgs &a, int labelled, i
 // A piece's tasks on the compute units: tiles of dW, steps_w steps each, go round, and the `more` first compute units have one more than the others; dh's tiles, whose sums over the
 // entries can be cut anywhere, fill up: all compute units take `all` of its tasks, steps_h steps each, and those with a tile less of dW go on to `some`.
 struct Balance {
-    int more, all, some, length;
+    int more, all, some;
+    int length, shorter, longer;               // steps of the units that take longer and of the others, whole rounds of dW aside; how many take longer
     __device__ __forceinline__ Balance(int weight_tasks, int steps_w, int hidden_tasks, int steps_h) {
         more = weight_tasks % COMPUTE_UNITS;
         length = INT32_MAX;
         for (int less = steps_w / steps_h, last = less + 1; less <= last; ++less) {       // tasks that a tile of dW is worth
             int s = (hidden_tasks + more * less + COMPUTE_UNITS - 1) / COMPUTE_UNITS, a = s - less;
             if (a < 0) a = 0, s = (hidden_tasks + COMPUTE_UNITS - more - 1) / (COMPUTE_UNITS - more);
-            const int l = max(s * steps_h, a * steps_h + (more ? steps_w : 0));
-            if (l < length) length = l, all = a, some = s;
+            const int l1 = s * steps_h, l2 = a * steps_h + (more ? steps_w : 0), l = max(l1, l2);
+            if (l < length) length = l, shorter = more ? min(l1, l2) : l1, longer = l2 == l ? more : COMPUTE_UNITS - more, all = a, some = s;
         }
+    }
+    // In steps of all compute units: those take 2.1 us, of power, and steps of a few units 1.3.
+    __device__ __forceinline__ float cost() const {
+        return shorter + (length - shorter) * (0.6f + 0.4f / COMPUTE_UNITS * longer);
+    }
+};
+
+// How dW's sums over the tokens are cut: whole, or in shares of an even number of steps.
+struct TokenShares {
+    int steps, length, shares;
+    // (rows and d have zeros behind the last token, up to a whole tile)
+    template <typename F>
+    static __device__ __forceinline__ TokenShares of(int labelled, int wanted) {
+        constexpr int K = STEP / F::PLANES;
+        const int steps = labelled ? max(2, (labelled + K - 1) / K) : 0;
+        if (wanted <= 1 || steps == 0) return {steps, steps, 1};
+        const int even = (steps + 1) / 2 * 2, length = (even + 2 * wanted - 1) / (2 * wanted) * 2;
+        return {even, length, (even + length - 1) / length};
     }
 };
 
 // Into how many shares of the vocabulary dh's sums are cut, by how long a piece's launch takes and what the shares cost in memory; lane i looks at i + 1.  A step of all compute units takes
 // 2.1 us, memory moves 5.1 TB/s.  (4915 labelled tokens, 50265 x 512: 9 shares are 253 steps, 10 in whole rounds were 314.)
+// And into how many of the tokens dW's: the next power of two while that is 4 % better, the units that take longer priced as Balance's cost and memory as it was found beside products,
+// 1.75 times as much.  (BF16: 32768 tokens, 1000 x 64, forward and backward 676 us whole and 129 cut; both gradients' sums of 65536 tokens, 50265 x 512, 12450 and 7170, of 32768 tokens 3630,
+// and 4450 if cut.)
+struct Shares {
+    int vocabulary, tokens;
+};
 template <typename F>
-__device__ __forceinline__ int shares_of(const BackwardArgs &a, int labelled) {
-    constexpr int K = STEP / F::PLANES;
+__device__ __forceinline__ Shares shares_of(const BackwardArgs &a, int labelled) {
     const Piece p = piece_of<F>(a, labelled, 0);
-    const int ht = (a.o.s.K + TILE - 1) / TILE, fit = (int)min(int64_t(SHARES), a.parts_bytes / (max(labelled, 1) * int64_t(a.o.s.K) * 4));
+    const int ht = (a.o.s.K + TILE - 1) / TILE, vt = (p.width + TILE - 1) / TILE, fit = (int)min(int64_t(SHARES), a.parts_bytes / (max(labelled, 1) * int64_t(a.o.s.K) * 4));
     const int n = threadIdx.x % 64 + 1, share = (p.steps + 2 * n - 1) / (2 * n) * 2, shares = (p.steps + share - 1) / share;
-    const Balance b((p.width + TILE - 1) / TILE * ht, (labelled + K - 1) / K, shares * p.nt * ht, share);      // (whether or not dW is wanted: the same bits)
-    const float cost = n > max(1, fit) ? INFINITY : b.length + shares * (float)labelled * a.o.s.K * 7.5e-7f;
-    float least = cost;
-#pragma unroll
-    for (int m = 32; m > 0; m /= 2) least = fminf(least, __shfl_xor(least, m));
-    return __ffsll((unsigned long long)__ballot(cost == least));
+    Shares best{1, 1};
+    float least = INFINITY;
+    for (int w = 1; w <= a.weight_shares; w *= 2) {
+        const TokenShares t = TokenShares::of<F>(labelled, w);
+        const Balance b(vt * ht * t.shares, t.length, shares * p.nt * ht, share);      // (whether or not dW is wanted: the same bits)
+        const float in_memory = (shares * (float)labelled + (t.shares > 1 ? t.shares * (float)p.width : 0.f)) * a.o.s.K * 7.5e-7f;
+        const float cost = n > max(1, fit) ? INFINITY : b.length + in_memory;
+        const int of = __ffsll((unsigned long long)__ballot(cost == wave_least(cost))) - 1;
+        const float all = __shfl(vt * ht * t.shares / COMPUTE_UNITS * t.length + b.cost() + 1.75f * in_memory, of);
+        if (all < 0.96f * least) least = all, best = {of + 1, w};
+    }
+    return best;
 }
 
 // What both gradients' sums are multiplied with: of a sum or mean what all tokens' d are, else the power of two that their coefficients were divided by.
@@ -748,22 +796,22 @@ __device__ __forceinline__ float factor_of(const BackwardArgs &a, int labelled) 
     return *a.g_loss / (a.reduction == 1 ? (float)max(labelled, 1) : 1.f) * (1.f / LIFT);
 }
 
-// Tokens' own gradients by the power of two of their largest.
-__global__ __launch_bounds__(1024) void coefficient_kernel(BackwardArgs a) {
+// Tokens' own gradients by the power of two of their largest, which is that of the chunks' largest ones.
+__global__ __launch_bounds__(1024) void coefficient_kernel(BackwardArgs a, const float *chunk_most) {
     __shared__ float most[16];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, chunks = (a.o.s.N + CHUNK - 1) / CHUNK, n = blockIdx.x * 1024 + tid;
+    const int at = n < a.o.s.N ? a.o.kept.pos[n] : -1;
+    const float g = at >= 0 ? a.g_loss[n] : 0.f;
     float v = 0.f;
-    for (int i = tid; i < a.o.s.N; i += 1024)
-        if (a.o.kept.pos[i] >= 0) v = fmaxf(v, fabsf(a.g_loss[i]));
+    for (int i = tid; i < chunks; i += 1024) v = fmaxf(v, chunk_most[i]);
     v = wave_most(v);
     if (tid % 64 == 0) most[tid / 64] = v;
     __syncthreads();
     for (int i = 0; i < 16; ++i) v = fmaxf(v, most[i]);
     int e;
     const float scale = scale_to(v, 0, e);
-    for (int i = tid; i < a.o.s.N; i += 1024)
-        if (a.o.kept.pos[i] >= 0) a.coefficient[a.o.kept.pos[i]] = a.g_loss[i] * scale;
-    if (tid == 0) *a.power = __builtin_amdgcn_ldexpf(1.f / LIFT, e);
+    if (at >= 0) a.coefficient[at] = g * scale;
+    if (n == 0) *a.power = __builtin_amdgcn_ldexpf(1.f / LIFT, e);
 }
 
 // A block's 32 numbers of each column, 16 a lane (mfma_row), packed: w[k] has 16 bytes of column 16 k + lane % 16, the piece_of_lane-th of its four.  Lanes 32 apart and then lanes 16 apart
@@ -842,8 +890,8 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
     });
     // (one of the workgroups that have the fewest tiles)
     if (piece == 0 && blockIdx.x == gridDim.x - 1 && wave == 0) {
-        const int shares = shares_of<F>(a, labelled);
-        if (lane == 0) a.shares[0] = shares, a.shares[1] = p.pieces;
+        const Shares shares = shares_of<F>(a, labelled);
+        if (lane == 0) a.shares[0] = shares.vocabulary, a.shares[1] = p.pieces, a.shares[2] = shares.tokens;
     }
 }
 
@@ -894,7 +942,8 @@ __device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece 
     // shares of an even number of steps, alike in all pieces; the last piece may have fewer
     const int wanted = *a.shares, length = (p.steps + 2 * wanted - 1) / (2 * wanted) * 2, steps = (p.width + Left::K - 1) / Left::K;
     const int tasks = (steps + length - 1) / length * p.nt * ht;
-    const Balance balance(a.grad_weight ? (p.width + TILE - 1) / TILE * ht : 0, (labelled + Left::K - 1) / Left::K, tasks, length);
+    const TokenShares of_weight = TokenShares::of<F>(labelled, a.shares[2]);
+    const Balance balance(a.grad_weight ? (p.width + TILE - 1) / TILE * ht * of_weight.shares : 0, of_weight.length, tasks, length);
     const int rounds = unit < balance.more ? balance.all : balance.some;
     // a compute unit's round-th task: neighbours take neighbouring ones
     auto id_of = [&](int round) {
@@ -939,33 +988,46 @@ __device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece 
     stream.done();
 }
 
-// dW: tiles of the piece's entries x tiles of columns, and, with the first columns, db.
+__device__ __forceinline__ void put_bias(const BackwardArgs &a, int v, float sum) {
+    if (a.bias_format == LFFN_ROWS_F32) static_cast<float *>(a.grad_bias)[v] = sum;
+    else if (a.bias_format == LFFN_ROWS_BF16) static_cast<__bf16 *>(a.grad_bias)[v] = (__bf16)sum;
+    else static_cast<_Float16 *>(a.grad_bias)[v] = (_Float16)sum;
+}
+
+// dW: shares of the tokens x tiles of the piece's entries x tiles of columns, and, with the first columns, db.
 template <typename F, typename R>
 __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece &p, int labelled, int unit, uint32_t lds) {
     typedef Across<TILE, THREADS, F::PLANES> Side;
     const Operands &o = a.o;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N, ht = (o.s.K + TILE - 1) / TILE;
     const Source rows = rows_of(o, labelled), d{a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld};
-    // (rows and d have zeros behind the last token, up to a whole tile)
-    const int steps = labelled ? max(2, (labelled + Side::K - 1) / Side::K) : 0;
+    const TokenShares shares = TokenShares::of<F>(labelled, a.shares[2]);
+    const bool whole = shares.shares == 1;
     const float factor = factor_of(a, labelled), by = F::PLANES == 2 ? factor * __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : factor;
-    const int tasks = (p.width + TILE - 1) / TILE * ht;
-    int task = unit;
-    if (task >= tasks) return;
-    int v0 = task / ht * TILE, h0 = task % ht * TILE;
-    Side left(rows, h0), right(d, v0);
+    struct Task {
+        int share, v, h, first, end;
+        __device__ __forceinline__ Task(int id, int vt, int ht, const TokenShares &s)
+            : share(id / ht / vt), v(id / ht % vt * TILE), h(id % ht * TILE), first(share * s.length), end(min(s.steps, first + s.length)) {}
+    };
+    const int vt = (p.width + TILE - 1) / TILE, tasks = shares.shares * vt * ht;
+    int id = unit;
+    if (id >= tasks) return;
+    Task task(id, vt, ht, shares);
+    Side left(rows, task.h), right(d, task.v);
     Stream<F, MB, NB, Side, Side> stream(lds, wm * MB * 32, wn * NB * 32);
-    if (steps) stream.prime(left, right, 0);
+    if (shares.steps) stream.prime(left, right, task.first);
     for (;;) {
-        const bool more = task + COMPUTE_UNITS < tasks;
-        const int next = more ? task + COMPUTE_UNITS : task, next_v = next / ht * TILE, next_h = next % ht * TILE;
-        const Side next_left(rows, next_h), next_right(d, next_v);
+        const bool more = id + COMPUTE_UNITS < tasks;
+        const int v0 = task.v, h0 = task.h;
+        if (more) id += COMPUTE_UNITS;
+        const Task then(id, vt, ht, shares);
+        const Side next_left(rows, then.h), next_right(d, then.v);
         Sums<MB, NB> sums;
         sums.clear();
         float bias[NB] = {};
         const bool of_bias = h0 == 0 && wm == 0 && a.grad_bias;
-        if (steps)
-            stream.multiply(sums, left, right, 0, steps, next_left, next_right, 0, [&](int j, const uint4 &u) {
+        if (shares.steps)
+            stream.multiply(sums, left, right, task.first, task.end, next_left, next_right, then.first, [&](int j, const uint4 &u) {
                 if (of_bias) bias[j] = dot_ones(F(), u, bias[j]);
             }, [] {});
         stream.landed();
@@ -976,13 +1038,11 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
             if (of_bias) {
                 const float sum = (bias[j] + __shfl_xor(bias[j], 32)) * factor;
                 if (half == 0 && live) {
-                    if (a.bias_format == LFFN_ROWS_F32) static_cast<float *>(a.grad_bias)[v] = sum;
-                    else if (a.bias_format == LFFN_ROWS_BF16) static_cast<__bf16 *>(a.grad_bias)[v] = (__bf16)sum;
-                    else static_cast<_Float16 *>(a.grad_bias)[v] = (_Float16)sum;
+                    if (!whole) a.bias_parts[int64_t(task.share) * o.s.V + v] = sum;
+                    else put_bias(a, v, sum);
                 }
             }
-            char *const row = static_cast<char *>(a.grad_weight) + int64_t(v) * o.s.K * R::BYTES;
-            if constexpr (R::BYTES == 2) {
+            if (R::BYTES == 2 && whole) {
 #pragma unroll
                 for (int i = 0; i < MB; ++i) {
                     float l[16];
@@ -998,6 +1058,7 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
                 }
                 continue;
             }
+            float *const row = whole ? static_cast<float *>(a.grad_weight) + int64_t(v) * o.s.K : a.weight_parts + (int64_t(task.share) * o.s.V + v) * o.s.K;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -1010,11 +1071,11 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
                         t[e] = __uint_as_float(s[0]), t[4 + e] = __uint_as_float(s[1]);
                     }
                     const int h = h0 + (wm * MB + i) * 32 + 8 * (g + half);
-                    if (live && h < o.s.K) store8<R>(row + h * R::BYTES, t);
+                    if (live && h < o.s.K) store8<F32Row>(reinterpret_cast<char *>(row + h), t);
                 }
         }
         if (!more) break;
-        task = next, v0 = next_v, h0 = next_h;
+        task = then;
     }
     stream.done();
 }
@@ -1067,6 +1128,33 @@ __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
         for (int e = 0; e < 8; ++e) v[e] *= by;
     }
     store8<R>(static_cast<char *>(a.grad_hidden) + (t * s.K + c) * R::BYTES, v);
+}
+
+// dW and db: shares added up, where there are any; a thread has eight columns or, in the workgroups behind, an entry's bias.
+template <typename F, typename R>
+__global__ __launch_bounds__(256) void weight_sum_kernel(BackwardArgs a) {
+    const Sizes &s = a.o.s;
+    const int shares = TokenShares::of<F>(a.o.kept.head[0], a.shares[2]).shares;
+    if (shares == 1) return;
+    const int64_t all = int64_t(s.V) * s.K, of_weight = (all / 8 + 255) / 256;
+    if (blockIdx.x >= of_weight) {
+        const int64_t v = (blockIdx.x - of_weight) * 256 + threadIdx.x;
+        if (v >= s.V) return;
+        float sum = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < shares; ++i) sum += a.bias_parts[int64_t(i) * s.V + v];
+        put_bias(a, (int)v, sum);
+        return;
+    }
+    const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
+    if (at >= all) return;
+    float v[8] = {};
+#pragma unroll 8
+    for (int i = 0; i < shares; ++i) {
+        const float4 x = *reinterpret_cast<const float4 *>(a.weight_parts + i * all + at), y = *reinterpret_cast<const float4 *>(a.weight_parts + i * all + at + 4);
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+    }
+    store8<R>(static_cast<char *>(a.grad_weight) + at * R::BYTES, v);
 }
 
 }  // namespace
@@ -1162,12 +1250,23 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     b.parts_bytes = one > PARTS_BYTES ? one : one * SHARES < PARTS_BYTES ? one * SHARES : PARTS_BYTES;
     b.parts = c.take<float>(b.parts_bytes / 4);
     b.coefficient = c.take<float>(a.reduction == 0 ? Np : 0);
+    w.r.most = c.take<float>(a.reduction == 0 ? (a.tokens + CHUNK - 1) / CHUNK : 0);
     b.power = c.take<float>(1);
-    b.shares = c.take<int32_t>(2);
-    if (a.reduction != 0) b.coefficient = nullptr;
+    b.shares = c.take<int32_t>(3);
+    if (a.reduction != 0) b.coefficient = nullptr, w.r.most = nullptr;
     // as many launches as pieces if all tokens are labelled; with fewer the last ones find nothing
     const int64_t entries = a.tokens == 0 ? 0 : widest(b.d_bytes, Np, (int)planes);
     b.pieces = a.tokens == 0 ? 0 : int((a.vocabulary + entries - 1) / entries);
+    // dW's sums may be cut into as many shares as a piece's tiles leave compute units without one, if a sum is long enough to be worth a launch
+    const int64_t each = b.pieces == 0 ? 0 : (Vp / TILE + b.pieces - 1) / b.pieces * ((K + TILE - 1) / TILE), rows = a.vocabulary * (K + 1) * 4;
+    const bool cut = b.pieces > 0 && a.tokens * planes >= CUT_FROM && each * 2 <= COMPUTE_UNITS;
+    const int64_t most = cut ? min(min(int64_t(SHARES), COMPUTE_UNITS / each), WEIGHT_PARTS_BYTES / rows) : 1;
+    b.weight_shares = 1;
+    while (b.weight_shares * 2 <= most) b.weight_shares *= 2;
+    if (b.weight_shares > 1) {
+        b.weight_parts = c.take<float>(b.weight_shares * a.vocabulary * K);
+        b.bias_parts = c.take<float>(b.weight_shares * a.vocabulary);
+    }
     return c.used;
 }
 
@@ -1229,6 +1328,10 @@ int backward(const BackwardArgs &b, hipStream_t st) {
         // four threads where one each would leave the chip without enough in flight (385 x 520 fp32 16.4 us with one, 11.4 with four; 32768 x 512, 4915 labelled, half 27 and 36)
         if (n < COMPUTE_UNITS * 256) hidden_kernel<F, R, 4><<<dim3(unsigned((n + 63) / 64)), dim3(256), 0, st>>>(b);
         else hidden_kernel<F, R, 1><<<dim3(unsigned((n + 255) / 256)), dim3(256), 0, st>>>(b);
+    }
+    if (b.grad_weight && b.weight_shares > 1) {
+        const int64_t n = int64_t(b.o.s.V) * (b.o.s.K / 8), of_bias = b.grad_bias ? (b.o.s.V + 255) / 256 : 0;
+        weight_sum_kernel<F, R><<<dim3(unsigned((n + 255) / 256 + of_bias)), dim3(256), 0, st>>>(b);
     }
     return LFFN_OK;
 }
@@ -1308,8 +1411,9 @@ extern "C" int lffn_linear_cross_entropy_bwd(const lffn_linear_cross_entropy *a,
     b.grad_hidden = grad_hidden, b.grad_weight = grad_weight, b.grad_bias = grad_bias;
     b.bias_format = a->bias_format, b.reduction = a->reduction;
     fill(w.r, *a, b.o);
+    w.r.g_loss = g_loss;
     launch_rows<true>(*a, w.r, st);
-    if (a->reduction == 0) coefficient_kernel<<<dim3(1), dim3(1024), 0, st>>>(b);
+    if (a->reduction == 0) coefficient_kernel<<<dim3(unsigned((a->tokens + 1023) / 1024)), dim3(1024), 0, st>>>(b, w.r.most);
     const int done = a->format == LFFN_ROWS_F32    ? backward<F32Two, F32Row>(b, st)
                      : a->format == LFFN_ROWS_BF16 ? backward<BF16, BF16Row>(b, st)
                                                    : backward<F16, F16Row>(b, st);

@@ -56,9 +56,9 @@ def _check(ids, w, scale, padding, g):
     assert torch.equal(again, grad)
 
 
-# tokens, rows, columns: none and one; a run through every piece; several workgroups of a sort; one, two and three passes; rows of one lane, of many blocks; odd widths
+# tokens, rows, columns: none and one; a run through every piece; several workgroups of a sort; one, two and three passes; rows of one lane, of many blocks; odd widths; more chunks than each adds up by itself
 SIZES = [(0, 5, 8), (1, 1, 1), (1, 50265, 768), (7, 3, 16), (17, 511, 24), (33, 512, 40), (385, 8191, 389), (1024, 700, 24), (1025, 9000, 16), (2048, 100, 64), (2049, 1, 129), (4096, 50265, 32), (4097, 3000, 8), (5000, 600, 512), (9001, 50265, 96),
-         (40000, 2, 72), (3000, 300001, 9), (300, 20, 2056), (700, 31, 1030)]
+         (40000, 2, 72), (3000, 300001, 9), (300, 20, 2056), (700, 31, 1030), (600001, 700, 8)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -76,7 +76,7 @@ def _check(x, w, b, g, eps=1e-5):
 
 # rows, columns: a lane, a sixteenth of a wavefront, one, several vectors of one, a workgroup, rows that are read again; odd widths of each; more rows than a backward's workgroups
 SIZES = [(1, 1), (3, 2), (5, 7), (1, 8), (33, 16), (1, 64), (70, 65), (2100, 24), (17, 128), (19, 129), (300, 389), (4, 512), (601, 768), (5, 701), (2, 1000), (3, 1024), (530, 1026), (9, 2048),
-         (7, 2049), (2, 4096), (3, 5003), (1, 8192), (2, 8200), (600, 9000), (5, 20001)]
+         (7, 2049), (2, 4096), (3, 5003), (1, 8192), (2, 8200), (600, 9000), (5, 20001), (70, 70000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -100,10 +100,12 @@ def _check(h, w, b, y, reduction="mean", ignore=-100, g=None):
     return loss, grads
 
 
-# tokens, vocabulary, columns, share of the tokens that have a label: one of each; sizes below, at and beyond a tile's; tokens that are counted in a launch of their own; many tiles
+# tokens, vocabulary, columns, share of the tokens that have a label: one of each; sizes below, at and beyond a tile's; tokens that are counted in a launch of their own; many tiles; tokens
+# whose sums are cut
 SIZES = [(1, 1, 8, 1.0), (1, 300, 64, 1.0), (5, 7, 16, 0.8), (64, 1000, 72, 1.0), (255, 255, 40, 1.0), (256, 256, 64, 1.0), (257, 513, 136, 0.5), (300, 777, 520, 0.3), (33, 5003, 264, 1.0),
          (4200, 600, 64, 0.1), (700, 2100, 776, 0.9), (130, 4096, 1032, 1.0), (40, 70001, 24, 0.9), (64, 300, 1208, 1.0), (64, 300, 1216, 1.0), (20, 300, 2432, 1.0), (32, 40, 2424, 0.9),
-         (64, 300, 608, 1.0), (64, 300, 616, 1.0), (32, 40, 1216, 0.9), (20, 9000, 1224, 1.0)]
+         (64, 300, 608, 1.0), (64, 300, 616, 1.0), (32, 40, 1216, 0.9), (20, 9000, 1224, 1.0), (1100, 300, 40, 1.0), (5000, 300, 72, 1.0), (9001, 40, 264, 0.9),
+         (4097, 1100, 24, 0.6)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -123,7 +125,7 @@ def test_against_64_bits(N, V, K, share, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_pieces_of_the_vocabulary(dtype):
     """So many tokens that the logits' gradients are formed in several pieces: with every token labelled, and with few, which need fewer pieces than launches."""
-    N, V, K = (65536, 5000, 8) if dtype != torch.float32 else (32768, 5000, 8)
+    N, V, K = (131072, 5000, 8) if dtype != torch.float32 else (65536, 5000, 8)
     h, w = _randn(N, K, dtype=dtype), _randn(V, K, dtype=dtype, seed=1)
     b = 0.5 * _randn(V, seed=2)
     y = torch.randint(0, V, (N,), device=DEV)
@@ -189,6 +191,26 @@ def test_ignored_rows_may_hold_anything():
         wild = linear_cross_entropy(h.requires_grad_(), w.requires_grad_(), b.requires_grad_(), y)
         grads = torch.autograd.grad(wild, (h, w, b))
         assert torch.equal(wild, plain[0]) and all(torch.equal(p, q) for p, q in zip(grads, plain[1]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [40, 300])
+def test_an_infinite_token_leaves_the_others(N, dtype):
+    """A token's infinite numbers, or an infinite gradient of its loss, reach that token's loss and gradient, and no other's."""
+    V, K = 500, 64
+    h, w, b = _randn(N, K, dtype=dtype), _randn(V, K, dtype=dtype, seed=1) / 4, _randn(V, seed=2)
+    y, g = torch.randint(0, V, (N,), device=DEV), _randn(N, seed=3)
+    h[3, 5], h[N - 2, 1] = float("inf"), float("nan")
+    g[7] = float("inf")
+    leaf = h.clone().requires_grad_()
+    loss = linear_cross_entropy(leaf, w, b, y, reduction="none")
+    grad, = torch.autograd.grad(loss, leaf, g)
+    lost = [3, N - 2]
+    assert not loss[lost].isfinite().any() and not grad[lost + [7]].isfinite().all(1).any()
+    others = torch.tensor([n not in (*lost, 7) for n in range(N)], device=DEV)
+    want, bounds = _reference(h[others], w, b, y[others], -100, "none", g[others])
+    _close(loss.detach()[others], want[0], bounds[0])
+    _close(grad[others], want[1], bounds[1])
 
 
 def test_masked_vocabulary():
