@@ -21,7 +21,7 @@ constexpr int TILE = 256;                       // tokens and vocabulary entries
 constexpr int THREADS = 512, WAVES_M = 2, WAVES_N = 4, MB = TILE / WAVES_M / 32, NB = TILE / WAVES_N / 32;
 constexpr int COMPUTE_UNITS = 256, XCDS = 8;
 constexpr int CHUNK = 64, PARTS = 4;            // tokens whose places a workgroup finds, and workgroups that lay their rows
-constexpr int COUNTED_FROM = 4096;              // tokens from which on a launch of its own counts the labelled ones of every chunk
+constexpr int COUNTED = 4096;                   // tokens of a workgroup that counts the labelled ones of its chunks; with fewer every chunk looks at all before it
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LIFT = 16384.f;                 // d times 2^14: half's normal numbers then reach down to 2^-28 of a row's largest
 constexpr int64_t D_BYTES = int64_t(1) << 30;   // of a piece's d, at most (with many tokens 2048 entries at least)
@@ -72,7 +72,7 @@ struct RowsArgs {
     const void *hidden, *labels, *bias;
     int64_t hidden_stride, ignore;
     int32_t labels_64, bias_format;            // of the gather's row formats; -1: none
-    const int32_t *counts;                     // labelled tokens of every chunk, or null
+    const int32_t *counts, *groups;            // labelled tokens of every chunk and of every COUNTED, or null
     int32_t *token;                            // [labelled]
     float *loss;                               // [N]: zeros for the others, or null
     const float *g_loss;                       // [N]
@@ -84,10 +84,23 @@ __device__ __forceinline__ int label_of(const void *labels, int wide, int64_t i,
     return y == ignore || y < 0 || y >= V ? -1 : (int)y;
 }
 
-__global__ __launch_bounds__(256) void count_kernel(const void *labels, int wide, int64_t ignore, int V, int N, int32_t *counts) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    const uint64_t live = __ballot(i < N && label_of(labels, wide, i, ignore, V) >= 0);
-    if (threadIdx.x % 64 == 0 && i < N) counts[i / CHUNK] = __popcll(live);
+__global__ __launch_bounds__(1024) void count_kernel(const void *labels, int wide, int64_t ignore, int V, int N, int32_t *counts, int32_t *groups) {
+    __shared__ int sums[16];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < COUNTED / 1024; ++i) {
+        const int n = blockIdx.x * COUNTED + i * 1024 + (int)threadIdx.x;
+        const int live = __popcll(__ballot(n < N && label_of(labels, wide, n, ignore, V) >= 0));
+        if (lane == 0 && n < N) counts[n / CHUNK] = live;
+        sum += live;
+    }
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) sum += sums[i];
+        groups[blockIdx.x] = sum;
+    }
 }
 
 __device__ __forceinline__ float wave_most(float v) {
@@ -176,9 +189,11 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     int labelled = 0;              // up to and with this chunk
     if constexpr (!BACKWARD) {
         int n = 0;
-        if (a.counts)
-            for (int i = tid; i < chunk; i += 256) n += a.counts[i];
-        else
+        if (a.counts) {
+            const int group = t0 / COUNTED, first = group * (COUNTED / CHUNK);
+            for (int i = tid; i < group; i += 256) n += a.groups[i];
+            if (first + tid < chunk) n += a.counts[first + tid];
+        } else
             for (int i = tid; i < t0; i += 256) n += label_of(a.labels, a.labels_64, i, a.ignore, s.V) >= 0;
 #pragma unroll
         for (int m = 32; m > 0; m /= 2) n += __shfl_xor(n, m);
@@ -634,7 +649,7 @@ struct JoinArgs {
     int64_t Np;
     int tiles;
     float *loss;           // by token
-    float *losses;         // by place
+    double *sums;          // of a workgroup's
     const float *weight_scale, *row_scale;       // two-term numbers
     int entries, joining;                        // workgroups that join; those behind look for the largest of the scales
 };
@@ -657,23 +672,30 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     for (int t = slice; t < a.tiles; t += 16) of = joined(of, a.parts[t * a.Np + n]);
     shares[slice][in] = of;
     __syncthreads();
-    if (slice == 0 && n < labelled) {
+    if (slice != 0) return;
+    double sum = 0;
+    if (n < labelled) {
 #pragma unroll
         for (int i = 1; i < 16; ++i) of = joined(of, shares[i][in]);
         // (log2(e), rounded alike in both, falls out)
         const float loss = (fmaf(-a.at_label[n], LOG2E, of.x) + __builtin_amdgcn_logf(of.y)) * (1.f / LOG2E);
         a.kept.level[n] = make_float2(of.x, 1.f / of.y);
         if (a.loss) a.loss[a.token[n]] = loss;
-        else a.losses[n] = loss;
+        sum = loss;
     }
+    if (!a.sums) return;
+#pragma unroll
+    for (int m = 8; m > 0; m /= 2) sum += __shfl_xor(sum, m);
+    if (in == 0) a.sums[blockIdx.x] = sum;
 }
 
 // The tokens' sum, or mean (0 of none), in 64 bits.
-__global__ __launch_bounds__(1024) void sum_kernel(const int32_t *head, const float *losses, float *loss, int mean) {
+__global__ __launch_bounds__(1024) void sum_kernel(const int32_t *head, const double *parts, float *loss, int mean) {
     __shared__ double sums[16];
     const int labelled = head[0];
     double sum = 0;
-    for (int i = threadIdx.x; i < labelled; i += 1024) sum += losses[i];
+#pragma unroll 8
+    for (int i = threadIdx.x; i < (labelled + 15) / 16; i += 1024) sum += parts[i];
 #pragma unroll
     for (int m = 32; m > 0; m /= 2) sum += __shfl_xor(sum, m);
     if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
@@ -1214,7 +1236,7 @@ struct Forward {
     RowsArgs r;
     JoinArgs j;
     void *kept;
-    int32_t *counts;
+    int32_t *counts, *groups;
 };
 int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Forward &f) {
     Carver c{base};
@@ -1225,9 +1247,10 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Fo
     f.j.tiles = int((a.vocabulary + TILE - 1) / TILE);
     f.j.parts = f.f.parts = c.take<float2>((few_tokens(a) ? few_workgroups(a) : f.j.tiles) * Np);
     f.j.at_label = f.f.at_label = c.take<float>(Np);
-    f.j.losses = c.take<float>(Np);
+    f.j.sums = c.take<double>(Np / 16);
     f.j.token = f.r.token = c.take<int32_t>(Np);
     f.counts = c.take<int32_t>(a.tokens / CHUNK + 1);
+    f.groups = c.take<int32_t>(a.tokens / COUNTED + 1);
     f.kept = with_kept ? c.take<char>(kept_bytes(a.tokens)) : nullptr;
     return c.used;
 }
@@ -1364,7 +1387,7 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
     hipStream_t st = static_cast<hipStream_t>(stream);
     f.f.o.kept = f.j.kept = kept_at(kept ? kept : f.kept, a->tokens);
     fill(f.r, *a, f.f.o);
-    if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.losses = nullptr;
+    if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.sums = nullptr;
     if (a->format == LFFN_ROWS_F32 || a->tokens == 0) head_kernel<<<dim3(1), dim3(64), 0, st>>>(f.f.o.kept.head);
     if (a->tokens > 0 && few_tokens(*a)) {
         const int done = a->format == LFFN_ROWS_F32 ? few<F32Row>(*a, f, st) : a->format == LFFN_ROWS_BF16 ? few<BF16>(*a, f, st) : few<F16>(*a, f, st);
@@ -1372,9 +1395,9 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
         f.j.joining = int((a->tokens + 15) / 16);
         join_kernel<<<dim3(f.j.joining), dim3(256), 0, st>>>(f.j);
     } else if (a->tokens > 0) {
-        if (a->tokens > COUNTED_FROM) {
-            count_kernel<<<dim3(unsigned((a->tokens + 255) / 256)), dim3(256), 0, st>>>(a->labels, a->labels_64, a->ignore_index, f.f.o.s.V, f.f.o.s.N, f.counts);
-            f.r.counts = f.counts;
+        if (a->tokens > COUNTED) {
+            count_kernel<<<dim3(unsigned((a->tokens + COUNTED - 1) / COUNTED)), dim3(1024), 0, st>>>(a->labels, a->labels_64, a->ignore_index, f.f.o.s.V, f.f.o.s.N, f.counts, f.groups);
+            f.r.counts = f.counts, f.r.groups = f.groups;
         }
         launch_rows<false>(*a, f.r, st);
         const int done = a->format == LFFN_ROWS_F32 ? forward<F32Two>(f, st) : a->format == LFFN_ROWS_BF16 ? forward<BF16>(f, st) : forward<F16>(f, st);
@@ -1383,7 +1406,7 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
         f.j.weight_scale = f.f.o.weight_scale, f.j.row_scale = f.f.o.row_scale, f.j.entries = (int)a->vocabulary;
         join_kernel<<<dim3(f.j.joining + (a->format == LFFN_ROWS_F32 ? 2 * LOOKING : 0)), dim3(256), 0, st>>>(f.j);
     }
-    if (a->reduction != 0) sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(f.f.o.kept.head, f.j.losses, loss, a->reduction == 1);
+    if (a->reduction != 0) sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(f.f.o.kept.head, f.j.sums, loss, a->reduction == 1);
     return lffn_launch_status();
 }
 
