@@ -172,6 +172,9 @@ __device__ __forceinline__ void raise(int32_t *most, const float *scales, int fi
     }
 }
 
+// (exponents lower than any: the launch that joins raises them)
+__device__ __forceinline__ void begin_head(const Kept &k, int labelled) { k.head[0] = labelled, k.head[1] = k.head[2] = -1000; }
+
 // Workgroups PARTS (tokens / CHUNK): the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
 // one fills the last tile's rows up with zeros.  The workgroups behind: the bias in fp32.
 template <typename R, int PLANES, bool BACKWARD>
@@ -211,7 +214,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
                 if (y >= 0) k.label[at] = y, a.token[at] = t;
                 else if (a.loss) a.loss[t] = 0.f;
             }
-            if (chunk == chunks - 1 && part == 0 && lane == 0) k.head[0] = labelled;
+            if (chunk == chunks - 1 && part == 0 && lane == 0) begin_head(k, labelled);
         }
     } else {
         labelled = k.head[0];
@@ -240,10 +243,6 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
         if (PLANES == 2 && !BACKWARD)
             for (int i = labelled + tid; i < up(labelled, TILE); i += 256) a.o.row_scale[i] = 1.f;
     }
-}
-
-__global__ void head_kernel(int32_t *head) {
-    if (threadIdx.x < 4) head[threadIdx.x] = threadIdx.x == 0 ? 0 : -1000;
 }
 
 // fp32 weights in two half-precision terms: each row by its largest, or, in the backward, all by the array's.
@@ -483,8 +482,8 @@ __device__ __forceinline__ float most_of(const uint4 &u, float most) {
     const float4 v = __builtin_bit_cast(float4, u);
     return fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 }
-// The exponent that two-term numbers of largest magnitude `most` have, to *exponent: one atomic of a workgroup.
-__device__ __forceinline__ void raise_by(int32_t *exponent, float most, float *red) {
+// The power of two that two-term numbers of a workgroup's largest magnitude are divided by, to *scale.
+__device__ __forceinline__ void put_scale(float *scale, float most, float *red) {
     most = wave_most(most);
     __syncthreads();
     if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = most;
@@ -493,7 +492,7 @@ __device__ __forceinline__ void raise_by(int32_t *exponent, float most, float *r
         for (unsigned i = 1; i < blockDim.x / 64; ++i) most = fmaxf(most, red[i]);
         int e;
         scale_to(most, 13, e);
-        atomicMax(exponent, e);
+        *scale = __builtin_amdgcn_ldexpf(1.f, e);
     }
 }
 
@@ -515,17 +514,14 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
     const int labelled = __popcll(live), place = __popcll(live & ((uint64_t(1) << lane) - 1));
     if (wave == 0 && y >= 0) tokens[place] = lane;
     if (blockIdx.x == 0 && wave == 0) {
-        if (lane == 0) o.kept.head[0] = labelled;
+        if (lane == 0) begin_head(o.kept, labelled);
         if (lane < o.s.N) {
             o.kept.pos[lane] = y >= 0 ? place : -1;
             if (y >= 0) o.kept.label[place] = y, a.r.token[place] = lane;
             else if (a.r.loss) a.r.loss[lane] = 0.f;
         }
     }
-    if (labelled == 0) {
-        if (WHOLE && blockIdx.x == 0 && tid == 0) o.kept.head[1] = o.kept.head[2] = 0;
-        return;
-    }
+    if (labelled == 0) return;
     const int blocks = (V + 31) / 32, all = gridDim.x * WAVES;
     int block = wave * gridDim.x + blockIdx.x;
     uint4 w[AHEAD][4];
@@ -636,8 +632,8 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
         a.parts[blockIdx.x * a.Np + tid] = sum;
     }
     if constexpr (WHOLE) {
-        raise_by(o.kept.head + 2, most, reinterpret_cast<float *>(waves));
-        if (blockIdx.x == 0) raise_by(o.kept.head + 1, most_x, reinterpret_cast<float *>(waves));
+        put_scale(o.weight_scale + blockIdx.x, most, reinterpret_cast<float *>(waves));
+        if (blockIdx.x == 0) put_scale(o.row_scale, most_x, reinterpret_cast<float *>(waves));
     }
 }
 
@@ -650,8 +646,8 @@ struct JoinArgs {
     int tiles;
     float *loss;           // by token
     double *sums;          // of a workgroup's
-    const float *weight_scale, *row_scale;       // two-term numbers
-    int entries, joining;                        // workgroups that join; those behind look for the largest of the scales
+    const float *weight_scale, *row_scale;       // two-term numbers: of `entries`, and of the labelled tokens or, of few, of all
+    int entries, few, joining;                   // the last: workgroups that join; those behind look for the largest of the scales
 };
 
 constexpr int LOOKING = 16;
@@ -662,8 +658,9 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     const int labelled = a.kept.head[0], in = threadIdx.x % 16, slice = threadIdx.x / 16, n = blockIdx.x * 16 + in;
     if ((int)blockIdx.x >= a.joining) {
         const int i = blockIdx.x - a.joining;
+        if (labelled == 0) return;                   // (no numbers are multiplied)
         if (i < LOOKING) raise(a.kept.head + 2, a.weight_scale, i * 256 + threadIdx.x, a.entries, LOOKING * 256, &shares[0][0].x);
-        else raise(a.kept.head + 1, a.row_scale, (i - LOOKING) * 256 + threadIdx.x, labelled, LOOKING * 256, &shares[0][0].x);
+        else raise(a.kept.head + 1, a.row_scale, (i - LOOKING) * 256 + threadIdx.x, a.few ? 1 : labelled, LOOKING * 256, &shares[0][0].x);
         return;
     }
     if ((int)blockIdx.x * 16 >= labelled) return;
@@ -692,7 +689,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
 // The tokens' sum, or mean (0 of none), in 64 bits.
 __global__ __launch_bounds__(1024) void sum_kernel(const int32_t *head, const double *parts, float *loss, int mean) {
     __shared__ double sums[16];
-    const int labelled = head[0];
+    const int labelled = head ? head[0] : 0;
     double sum = 0;
 #pragma unroll 8
     for (int i = threadIdx.x; i < (labelled + 15) / 16; i += 1024) sum += parts[i];
@@ -1222,9 +1219,11 @@ Operands operands(const lffn_linear_cross_entropy &a, Carver &c, bool split) {
     o.rows = c.take<char>(o.rows_plane * planes);
     o.bias = c.take<float>(o.s.Vp);
     o.weight = {static_cast<const char *>(a.weight), a.weight_stride * (planes == 2 ? 4 : 2), 0, o.s.V, o.s.K};
-    if (split) {
-        o.weight_scale = c.take<float>(o.s.Vp);
+    if (planes == 2) {
+        o.weight_scale = c.take<float>(o.s.Vp);          // (of few tokens: a workgroup's, and one of the tokens)
         o.row_scale = c.take<float>(Np);
+    }
+    if (split) {
         const int64_t plane = a.vocabulary * a.columns * 2;
         o.weight = {c.take<char>(plane * 2), a.columns * 2, plane, o.s.V, o.s.K};
     }
@@ -1388,12 +1387,14 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
     f.f.o.kept = f.j.kept = kept_at(kept ? kept : f.kept, a->tokens);
     fill(f.r, *a, f.f.o);
     if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.sums = nullptr;
-    if (a->format == LFFN_ROWS_F32 || a->tokens == 0) head_kernel<<<dim3(1), dim3(64), 0, st>>>(f.f.o.kept.head);
+    // (workgroups that look for the largest scales behind those that join)
+    const int looking = a->format == LFFN_ROWS_F32 ? 2 * LOOKING : 0;
+    f.j.weight_scale = f.f.o.weight_scale, f.j.row_scale = f.f.o.row_scale;
     if (a->tokens > 0 && few_tokens(*a)) {
         const int done = a->format == LFFN_ROWS_F32 ? few<F32Row>(*a, f, st) : a->format == LFFN_ROWS_BF16 ? few<BF16>(*a, f, st) : few<F16>(*a, f, st);
         if (done != LFFN_OK) return done;
-        f.j.joining = int((a->tokens + 15) / 16);
-        join_kernel<<<dim3(f.j.joining), dim3(256), 0, st>>>(f.j);
+        f.j.joining = int((a->tokens + 15) / 16), f.j.entries = f.j.tiles, f.j.few = 1;
+        join_kernel<<<dim3(f.j.joining + looking), dim3(256), 0, st>>>(f.j);
     } else if (a->tokens > 0) {
         if (a->tokens > COUNTED) {
             count_kernel<<<dim3(unsigned((a->tokens + COUNTED - 1) / COUNTED)), dim3(1024), 0, st>>>(a->labels, a->labels_64, a->ignore_index, f.f.o.s.V, f.f.o.s.N, f.counts, f.groups);
@@ -1402,11 +1403,10 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
         launch_rows<false>(*a, f.r, st);
         const int done = a->format == LFFN_ROWS_F32 ? forward<F32Two>(f, st) : a->format == LFFN_ROWS_BF16 ? forward<BF16>(f, st) : forward<F16>(f, st);
         if (done != LFFN_OK) return done;
-        f.j.joining = int(f.f.Np / 16);
-        f.j.weight_scale = f.f.o.weight_scale, f.j.row_scale = f.f.o.row_scale, f.j.entries = (int)a->vocabulary;
-        join_kernel<<<dim3(f.j.joining + (a->format == LFFN_ROWS_F32 ? 2 * LOOKING : 0)), dim3(256), 0, st>>>(f.j);
+        f.j.joining = int(f.f.Np / 16), f.j.entries = (int)a->vocabulary;
+        join_kernel<<<dim3(f.j.joining + looking), dim3(256), 0, st>>>(f.j);
     }
-    if (a->reduction != 0) sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(f.f.o.kept.head, f.j.sums, loss, a->reduction == 1);
+    if (a->reduction != 0) sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(a->tokens > 0 ? f.f.o.kept.head : nullptr, f.j.sums, loss, a->reduction == 1);
     return lffn_launch_status();
 }
 
