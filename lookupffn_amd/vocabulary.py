@@ -89,6 +89,7 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
 
     float32: products of two half-precision terms a number, sums in float32, errors of the size of float32 products'; in the backward a number of hidden or
     weight is held to 2^-38 of the largest of its array.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half: held to 2^-38 of the largest token's).
+    Memory: the backward has a workspace of up to 1 GB for the logits' gradients (with more than some 250000 tokens 4.2 KB a token) and up to 0.75 GB for sums; float32 weights are laid out once more.
     -> float32.  Gradients: hidden, weight and bias, the same bits on every call; none of theirs, and none in forward mode (an error); captured in graphs as ``cross_attention`` is."""
     host = _host()
     if host:
