@@ -54,15 +54,15 @@ struct Operands {
     Sizes s;
     Kept kept;
     Source weight;             // as the products read it
-    char *rows;                // [Np, Kp] the labelled tokens' rows
-    int64_t rows_plane;
+    char *rows;                // [Np, Kp] the labelled tokens' rows, zeros behind the columns
     float *bias;               // [Vp] fp32, -infinity behind the vocabulary
     float *weight_scale;       // two-term numbers: [Vp], [Np], by which sums are multiplied
     float *row_scale;
 };
 
+template <int PLANES>
 __device__ __forceinline__ Source rows_of(const Operands &o, int labelled) {
-    return {o.rows, o.s.Kp * 2, o.rows_plane, (int)up(labelled, TILE), (int)o.s.Kp};
+    return {o.rows, o.s.Kp * 2 * PLANES, (int)up(labelled, TILE), (int)o.s.Kp};
 }
 
 // ---------------------------------------------------------------- the labelled tokens
@@ -114,7 +114,7 @@ __device__ __forceinline__ float wave_least(float v) { return -wave_most(-v); }
 // A row of `columns` numbers as the products read it, zeros up to `padded`, by one wavefront.  Two-term numbers: scaled by the row's largest, or to `exponent` where that is
 // given; -> the exponent of the way back.
 template <typename R, int PLANES>
-__device__ __forceinline__ int lay_row(const char *from, char *to, int64_t plane, int columns, int64_t padded, const int *exponent) {
+__device__ __forceinline__ int lay_row(const char *from, char *to, int columns, int64_t padded, const int *exponent) {
     const int lane = threadIdx.x % 64;
     if constexpr (PLANES == 1) {
         for (int c = lane * 8; c < padded; c += 512)
@@ -146,8 +146,8 @@ __device__ __forceinline__ int lay_row(const char *from, char *to, int64_t plane
                     l[i] = split_rest(v[2 * i], v[2 * i + 1], h[i]);
                 }
             }
-            *reinterpret_cast<uint4 *>(to + c * 2) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4 *>(to + plane + c * 2) = make_uint4(l[0], l[1], l[2], l[3]);
+            *reinterpret_cast<uint4 *>(to + byte_of<2>(c)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(to + byte_of<2>(c) + 64) = make_uint4(l[0], l[1], l[2], l[3]);
         }
         return e;
     }
@@ -228,18 +228,17 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
         }
     }
     __syncthreads();
-    const int64_t row_bytes = s.Kp * 2;
+    const int64_t row_bytes = s.Kp * 2 * PLANES;
     for (int i = part * 4 + wave; i < CHUNK; i += 4 * PARTS) {
         const int at = place[i];
         if (at < 0) continue;
         const char *from = static_cast<const char *>(a.hidden) + (int64_t(t0) + i) * a.hidden_stride * R::BYTES;
-        const int e = lay_row<R, PLANES>(from, a.o.rows + at * row_bytes, a.o.rows_plane, s.K, s.Kp, BACKWARD ? k.head + 1 : nullptr);
+        const int e = lay_row<R, PLANES>(from, a.o.rows + at * row_bytes, s.K, s.Kp, BACKWARD ? k.head + 1 : nullptr);
         if (PLANES == 2 && !BACKWARD && lane == 0) a.o.row_scale[at] = __builtin_amdgcn_ldexpf(1.f, e);
     }
     if (chunk == chunks - 1) {
         const int64_t from = labelled * row_bytes / 16, to = up(labelled, TILE) * row_bytes / 16;
-        for (int64_t i = from + part * 256 + tid; i < to; i += 256 * PARTS)
-            for (int p = 0; p < PLANES; ++p) *reinterpret_cast<uint4 *>(a.o.rows + p * a.o.rows_plane + i * 16) = make_uint4(0, 0, 0, 0);
+        for (int64_t i = from + part * 256 + tid; i < to; i += 256 * PARTS) *reinterpret_cast<uint4 *>(a.o.rows + i * 16) = make_uint4(0, 0, 0, 0);
         if (PLANES == 2 && !BACKWARD)
             for (int i = labelled + tid; i < up(labelled, TILE); i += 256) a.o.row_scale[i] = 1.f;
     }
@@ -252,7 +251,7 @@ __global__ __launch_bounds__(256) void weight_kernel(Operands o, const float *w,
     if (v >= o.s.Vp) return;
     int e = 0;
     if (v < o.s.V)
-        e = lay_row<F32Row, 2>(reinterpret_cast<const char *>(w + v * stride), const_cast<char *>(o.weight.at) + v * o.weight.stride, o.weight.plane, o.s.K, o.s.K,
+        e = lay_row<F32Row, 2>(reinterpret_cast<const char *>(w + v * stride), const_cast<char *>(o.weight.at) + v * o.weight.stride, o.s.K, o.weight.columns,
                                BACKWARD ? o.kept.head + 2 : nullptr);
     if (threadIdx.x % 64 == 0) {
         // (entries behind the vocabulary: no larger than any)
@@ -320,7 +319,7 @@ __device__ __forceinline__ void for_logits(const Operands &o, const float *coeff
     const int steps = max(2, (o.s.K + Side::K - 1) / Side::K);
     Turns turns(vt * nt);
     if (!turns.any()) return;
-    const Source rows = rows_of(o, labelled);
+    const Source rows = rows_of<F::PLANES>(o, labelled);
     Place place(turns.at, vt, nt);
     Side a(o.weight, v0 + place.v), b(rows, place.n);
     Stream<F, MB, NB, Side, Side> stream(lds, wave / WAVES_N * MB * 32, wave % WAVES_N * NB * 32);
@@ -443,7 +442,7 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
 // Up to 64 tokens whose rows fit LDS: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a
 // time, whose rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, six such in flight.  Nothing is laid together before: a launch less.
 // fp32 is multiplied as it is (v_mfma_f32_32x32x2_f32): at 32 tokens a product takes as long as its weights' bytes (32 x 50265 x 840 64 us; splitting the weights to memory 71 and the tiles'
-// products 100).  The exponents that the backward's two-term numbers have in common are found on the way.
+// products 71).  The exponents that the backward's two-term numbers have in common are found on the way.
 constexpr int FEW = 64, LINE = 128;                                                            // bytes of a row that a step has
 constexpr int few_stride(int64_t row_bytes) { return int(up(row_bytes, LINE)) / 16 | 1; }      // 16-byte pieces of a row in LDS: odd, so that 16 rows meet every bank once
 constexpr int64_t few_lds(int64_t tokens, int64_t row_bytes) {
@@ -707,8 +706,8 @@ __global__ __launch_bounds__(1024) void sum_kernel(const int32_t *head, const do
 
 struct BackwardArgs {
     Operands o;
-    char *d;                   // [Np, ld] (two planes): a piece's
-    int64_t d_bytes, d_plane;  // how large it may be; the second plane's distance
+    char *d;                   // [Np, ld]: a piece's
+    int64_t d_bytes;           // how large it may be
     float *parts;              // [shares, labelled, K]
     int64_t parts_bytes;
     const float *g_loss;       // [1] or [N]
@@ -876,7 +875,7 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
             const float2 level = live ? beside<float2>(beside_, LEVEL, column) : make_float2(INFINITY, 0.f);
             const float by = LIFT * (a.coefficient ? beside<float>(beside_, COEFFICIENT, column) : 1.f), p_by = live ? level.y * by : 0.f;
             const int at = live ? beside<int>(beside_, LABEL, column) - p.v0 - in : -1;
-            char *const row = a.d + (int64_t(n - lane % 32 + lane % 16) * p.ld + in + 8 * piece_of_lane(lane)) * 2;       // (of the block's first 16 tokens)
+            char *const row = a.d + (int64_t(n - lane % 32 + lane % 16) * p.ld + in) * 2 * F::PLANES + 16 * piece_of_lane(lane);       // (of the block's first 16 tokens)
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 float l[16];
@@ -895,14 +894,14 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
                 auto put = [&](char *to) {
                     uint4 w[2];
                     pieces_of<F>(l, w);
-                    *reinterpret_cast<uint4 *>(to + 64 * i) = w[0];
-                    *reinterpret_cast<uint4 *>(to + 64 * i + 32 * int64_t(p.ld)) = w[1];
+                    *reinterpret_cast<uint4 *>(to + 64 * F::PLANES * i) = w[0];
+                    *reinterpret_cast<uint4 *>(to + 64 * F::PLANES * i + 32 * F::PLANES * int64_t(p.ld)) = w[1];
                 };
                 put(row);
                 if constexpr (F::PLANES == 2) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) l[e] -= (float)(_Float16)l[e];
-                    put(row + a.d_plane);
+                    put(row + 64);
                 }
             }
         }
@@ -948,7 +947,7 @@ __device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece 
     typedef Across<TILE, THREADS, F::PLANES> Right;
     const Operands &o = a.o;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, ht = (o.s.K + TILE - 1) / TILE;
-    const Source d{a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld};
+    const Source d{a.d, int64_t(p.ld) * 2 * F::PLANES, p.nt * TILE, p.ld};
     Source w = o.weight;
     w.at += p.v0 * w.stride;
     w.rows = p.width;
@@ -1019,7 +1018,7 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
     typedef Across<TILE, THREADS, F::PLANES> Side;
     const Operands &o = a.o;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N, ht = (o.s.K + TILE - 1) / TILE;
-    const Source rows = rows_of(o, labelled), d{a.d, p.ld * 2, a.d_plane, p.nt * TILE, p.ld};
+    const Source rows = rows_of<F::PLANES>(o, labelled), d{a.d, int64_t(p.ld) * 2 * F::PLANES, p.nt * TILE, p.ld};
     const TokenShares shares = TokenShares::of<F>(labelled, a.shares[2]);
     const bool whole = shares.shares == 1;
     const float factor = factor_of(a, labelled), by = F::PLANES == 2 ? factor * __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : factor;
@@ -1215,17 +1214,16 @@ Operands operands(const lffn_linear_cross_entropy &a, Carver &c, bool split) {
     const int64_t Np = up(a.tokens, TILE);
     o.s = {(int)a.tokens, (int)a.vocabulary, (int)a.columns, up(a.columns, 2 * STEP), up(a.vocabulary, TILE)};
     const int planes = planes_of(a);
-    o.rows_plane = Np * o.s.Kp * 2;
-    o.rows = c.take<char>(o.rows_plane * planes);
+    o.rows = c.take<char>(Np * o.s.Kp * 2 * planes);
     o.bias = c.take<float>(o.s.Vp);
-    o.weight = {static_cast<const char *>(a.weight), a.weight_stride * (planes == 2 ? 4 : 2), 0, o.s.V, o.s.K};
+    o.weight = {static_cast<const char *>(a.weight), a.weight_stride * (planes == 2 ? 4 : 2), o.s.V, o.s.K};
     if (planes == 2) {
         o.weight_scale = c.take<float>(o.s.Vp);          // (of few tokens: a workgroup's, and one of the tokens)
         o.row_scale = c.take<float>(Np);
     }
     if (split) {
-        const int64_t plane = a.vocabulary * a.columns * 2;
-        o.weight = {c.take<char>(plane * 2), a.columns * 2, plane, o.s.V, o.s.K};
+        const int64_t columns = up(a.columns, STEP / 2);
+        o.weight = {c.take<char>(a.vocabulary * columns * 4), columns * 4, o.s.V, (int)columns};
     }
     return o;
 }
@@ -1266,7 +1264,6 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     b.o = operands(a, c, planes == 2);
     const int64_t Vp = b.o.s.Vp, least = Np * ((Vp < 2048 ? Vp : 2048) + APART) * 2 * planes, whole = Np * (Vp + APART) * 2 * planes;
     b.d_bytes = least > D_BYTES ? least : whole < D_BYTES ? whole : D_BYTES;
-    b.d_plane = b.d_bytes / 2;
     b.d = c.take<char>(b.d_bytes);
     const int64_t one = a.tokens * K * 4;
     b.parts_bytes = one > PARTS_BYTES ? one : one * SHARES < PARTS_BYTES ? one * SHARES : PARTS_BYTES;

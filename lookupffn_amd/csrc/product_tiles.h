@@ -5,7 +5,8 @@
 // with the summed index from row to row (Across); the latter is read from LDS by the transposing read, so that nothing is ever transposed in memory.
 // 256 x 256: a step is 64 KB and 2061 clocks of products at the peak rate, its LDS reads 1536, its copies 32 bytes a clock.
 //
-// A float is two half-precision terms in two planes (split_mfma.h): a step has 32 numbers of each plane and three products.
+// A float is two half-precision terms (split_mfma.h), "planes" of an operand: a step has 32 numbers of each plane and three products.  In memory a row's planes take turns, 32 numbers each, so
+// that a step reads whole lines (two arrays one behind the other: logits of 385 tokens, 32003 x 520, 57 us instead of 47, of 9 tokens, 50265 x 840, 100 instead of 71).
 #pragma once
 
 #include "rows16.h"
@@ -53,13 +54,19 @@ __device__ __forceinline__ void copy_to_lds(const char *base, uint32_t lane_offs
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_byte_of(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p; }
 
-// An array [rows, columns] of 16-bit numbers, `stride` bytes a row, the second plane `plane` bytes behind the first.  rows and columns (a multiple of 8) are those that may
+// An array [rows, columns] of 16-bit numbers, or of two planes' in turns, `stride` bytes a row.  rows and columns (a multiple of 8, of two planes of 32) are those that may
 // be read: what lies beyond is read as its nearest neighbour, and the other operand has zeros there, or the result is not stored.
 struct Source {
     const char *at;
-    int64_t stride, plane;
+    int64_t stride;
     int rows, columns;
 };
+
+// Where a number of the first plane is in a row, in bytes; the second's is 64 further.
+template <int PLANES>
+__host__ __device__ __forceinline__ constexpr int64_t byte_of(int64_t column) {
+    return PLANES == 1 ? column * 2 : column / 32 * 128 + column % 32 * 2;
+}
 
 // ROWS rows of a tile, the sum along them.  16-byte piece p of row r is at piece p ^ (r / 2 % 8), so that the 16 lanes of an LDS read that have the same piece
 // of 16 rows meet every bank once.
@@ -68,32 +75,22 @@ struct Along {
     static constexpr int WORDS = ROWS * 8, SHARE = WORDS / THREADS, K = STEP / PLANES;
     static_assert(WORDS % THREADS == 0 && THREADS % 64 == 0 && (THREADS / 8) % 16 == 0, "whole wavefronts, a thread's rows turned alike");
     const char *base;
-    int64_t plane;
     uint32_t offset[SHARE];       // of the thread's rows, from base
-    int k, last;                  // first number of the thread's piece in a step; the last piece that may be read
+    int k, last;                  // bytes: the thread's piece in a step; the last piece that may be read
 
     // rows from `row`, which is less than s.rows; a tile's rows lie within 32 bits
     __device__ __forceinline__ Along(const Source &s, int row) {
         base = (const char *)uniform((uint64_t)(s.at + row * s.stride));
-        const int tid = threadIdx.x, r = tid / 8, piece = (tid % 8) ^ (r / 2 % 8);
-        plane = PLANES == 2 && piece >= 4 ? s.plane : 0;
-        k = piece % (8 / PLANES) * 8;
-        last = s.columns - 8;
+        const int tid = threadIdx.x, r = tid / 8;
+        k = ((tid % 8) ^ (r / 2 % 8)) * 16;
+        last = s.columns * 2 * PLANES - 16;
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) offset[i] = uint32_t(min(r + i * (THREADS / 8), s.rows - 1 - row) * s.stride);
     }
     // the thread's i-th piece of a step
     __device__ __forceinline__ void begin(int step, uint32_t lds, int i) const {
-        const uint32_t to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 1024) + i * THREADS * 16, column = min(step * K + k, last) * 2;
-        if constexpr (PLANES == 1) copy_to_lds(base, offset[i] + column, to);
-        else copy_to_lds_far(base + plane + offset[i] + column, to);
-    }
-    static __device__ __forceinline__ void copy_to_lds_far(const char *at, uint32_t lds_byte) {
-        uint32_t saved_m0;
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                     : "=&s"(saved_m0)
-                     : "v"(at), "s"(lds_byte)
-                     : "memory");
+        const uint32_t to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 1024) + i * THREADS * 16;
+        copy_to_lds(base, offset[i] + min(step * (STEP * 2) + k, last), to);
     }
     struct Reader {
         uint32_t at[4];
@@ -116,16 +113,16 @@ struct Across {
     static constexpr int PIECES = COLUMNS / 8, WORDS = STEP * PIECES, SHARE = WORDS / THREADS, K = STEP / PLANES;
     static_assert(PIECES >= 16 && WORDS % THREADS == 0 && THREADS % PIECES == 0 && (THREADS / PIECES) % 4 == 0, "a thread's rows turned alike");
     const char *base;
-    int64_t stride, plane;
+    int64_t stride;
     int last_row, row, column;    // bytes
 
     // columns from `column0`, which is less than s.columns
     __device__ __forceinline__ Across(const Source &s, int column0) {
-        base = (const char *)uniform((uint64_t)(s.at + int64_t(column0) * 2));
-        stride = s.stride, plane = s.plane, last_row = s.rows - 1;
+        base = (const char *)uniform((uint64_t)(s.at + byte_of<PLANES>(column0)));
+        stride = s.stride, last_row = s.rows - 1;
         const int tid = threadIdx.x;
         row = tid / PIECES;
-        column = min((tid % PIECES ^ 4 * (row % 4)) * 8, s.columns - 8 - column0) * 2;
+        column = (int)byte_of<PLANES>(min((tid % PIECES ^ 4 * (row % 4)) * 8, s.columns - 8 - column0));
     }
     // the thread's i-th piece of a step
     __device__ __forceinline__ void begin(int step, uint32_t lds, int i) const {
@@ -135,7 +132,7 @@ struct Across {
         const char *from = base + first * stride;
         // (a plane's rows are a multiple of the rows that a pass of all threads takes: uniform)
         const bool second = PLANES == 2 && i * (THREADS / PIECES) >= K;
-        copy_to_lds(second ? from + plane : from, uint32_t(min(second ? r - K : r, last_row - first) * (int)stride) + column, to);
+        copy_to_lds(second ? from + 64 : from, uint32_t(min(second ? r - K : r, last_row - first) * (int)stride) + column, to);
     }
     struct Reader {
         uint32_t at[4];           // by d % 4
