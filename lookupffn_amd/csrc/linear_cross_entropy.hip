@@ -20,7 +20,7 @@ using namespace product_tiles;
 constexpr int TILE = 256;                       // tokens and vocabulary entries of a tile
 constexpr int THREADS = 512, WAVES_M = 2, WAVES_N = 4, MB = TILE / WAVES_M / 32, NB = TILE / WAVES_N / 32;
 constexpr int COMPUTE_UNITS = 256, XCDS = 8;
-constexpr int CHUNK = 64, PARTS = 4;            // tokens whose places a workgroup finds, and workgroups that lay their rows
+constexpr int CHUNK = 64;                       // tokens whose places a workgroup finds
 constexpr int COUNTED = 4096;                   // tokens of a workgroup that counts the labelled ones of its chunks; with fewer every chunk looks at all before it
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LIFT = 16384.f;                 // d times 2^14: half's normal numbers then reach down to 2^-28 of a row's largest
@@ -73,6 +73,7 @@ struct RowsArgs {
     int64_t hidden_stride, ignore;
     int32_t labels_64, bias_format;            // of the gather's row formats; -1: none
     const int32_t *counts, *groups;            // labelled tokens of every chunk and of every COUNTED, or null
+    int parts;                                 // workgroups that lay a chunk's rows
     int32_t *token;                            // [labelled]
     float *loss;                               // [N]: zeros for the others, or null
     const float *g_loss;                       // [N]
@@ -175,15 +176,15 @@ __device__ __forceinline__ void raise(int32_t *most, const float *scales, int fi
 // (exponents lower than any: the launch that joins raises them)
 __device__ __forceinline__ void begin_head(const Kept &k, int labelled) { k.head[0] = labelled, k.head[1] = k.head[2] = -1000; }
 
-// Workgroups PARTS (tokens / CHUNK): the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
+// Workgroups parts (tokens / CHUNK): the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
 // one fills the last tile's rows up with zeros.  The workgroups behind: the bias in fp32.
 template <typename R, int PLANES, bool BACKWARD>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     const Sizes &s = a.o.s;
     const Kept &k = a.o.kept;
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, chunks = (s.N + CHUNK - 1) / CHUNK, chunk = blockIdx.x / PARTS, part = blockIdx.x % PARTS;
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, chunks = (s.N + CHUNK - 1) / CHUNK, chunk = (int)blockIdx.x / a.parts, part = (int)blockIdx.x % a.parts;
     if (chunk >= chunks) {
-        const int v = ((int)blockIdx.x - chunks * PARTS) * 256 + tid;
+        const int v = ((int)blockIdx.x - chunks * a.parts) * 256 + tid;
         if (v < s.Vp) a.o.bias[v] = v >= s.V ? -INFINITY : a.bias_format < 0 ? 0.f : bias_of(a.bias, a.bias_format, v);
         return;
     }
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     }
     __syncthreads();
     const int64_t row_bytes = s.Kp * 2 * PLANES;
-    for (int i = part * 4 + wave; i < CHUNK; i += 4 * PARTS) {
+    for (int i = part * 4 + wave; i < CHUNK; i += 4 * a.parts) {
         const int at = place[i];
         if (at < 0) continue;
         const char *from = static_cast<const char *>(a.hidden) + (int64_t(t0) + i) * a.hidden_stride * R::BYTES;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     }
     if (chunk == chunks - 1) {
         const int64_t from = labelled * row_bytes / 16, to = up(labelled, TILE) * row_bytes / 16;
-        for (int64_t i = from + part * 256 + tid; i < to; i += 256 * PARTS) *reinterpret_cast<uint4 *>(a.o.rows + i * 16) = make_uint4(0, 0, 0, 0);
+        for (int64_t i = from + part * 256 + tid; i < to; i += 256 * a.parts) *reinterpret_cast<uint4 *>(a.o.rows + i * 16) = make_uint4(0, 0, 0, 0);
         if (PLANES == 2 && !BACKWARD)
             for (int i = labelled + tid; i < up(labelled, TILE); i += 256) a.o.row_scale[i] = 1.f;
     }
@@ -1294,11 +1295,12 @@ void fill(RowsArgs &r, const lffn_linear_cross_entropy &a, const Operands &o) {
     r.hidden = a.hidden, r.labels = a.labels, r.bias = a.bias;
     r.hidden_stride = a.hidden_stride, r.ignore = a.ignore_index;
     r.labels_64 = a.labels_64, r.bias_format = a.bias ? a.bias_format : -1;
+    r.parts = a.tokens > COUNTED ? 4 : 16;         // (few tokens: a row a wavefront; 385 x 520 fp32 6.5 us, by four 12.8)
 }
 
 template <bool BACKWARD>
 void launch_rows(const lffn_linear_cross_entropy &a, const RowsArgs &r, hipStream_t st) {
-    const dim3 grid(unsigned((a.tokens + CHUNK - 1) / CHUNK * PARTS + (r.o.s.Vp + 255) / 256));
+    const dim3 grid(unsigned((a.tokens + CHUNK - 1) / CHUNK * r.parts + (r.o.s.Vp + 255) / 256));
     if (a.format == LFFN_ROWS_F32) {
         weight_kernel<BACKWARD><<<dim3(unsigned(r.o.s.Vp / 4)), dim3(256), 0, st>>>(r.o, static_cast<const float *>(a.weight), a.weight_stride);
         rows_kernel<F32Row, 2, BACKWARD><<<grid, dim3(256), 0, st>>>(r);
