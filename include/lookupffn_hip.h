@@ -1019,7 +1019,7 @@ int lffn_layer_norm_rows_bwd(const lffn_layer_norm_rows *a, const float *stats, 
  * reduction 0: loss is [tokens], zeros for the others; 1: their mean (0 of none), 2: their sum; [1].
  * format 0: products of two half-precision terms a number, fp32 accuracy; in the backward a number of hidden or weight is held to 2^-38 of the largest of its array.
  * 1 and 2: sums in fp32; in the backward the logits' gradients are rounded to the format.
- * kept: what the backward needs, of lffn_linear_cross_entropy_kept_bytes, 16-byte aligned, or NULL.  workspace: 16-byte aligned.
+ * kept: what the backward needs, of lffn_linear_cross_entropy_kept_bytes, 16-byte aligned, or NULL; of up to 64 tokens it may hold the logits.  workspace: 16-byte aligned.
  */
 typedef struct lffn_linear_cross_entropy {
     const void *hidden, *weight, *bias, *labels;

@@ -1,4 +1,4 @@
-// Softmax cross entropy of a projection to a large vocabulary, and its gradients, without the logits in memory:
+// Softmax cross entropy of a projection to a large vocabulary, and its gradients, without the logits of many tokens in memory:
 //
 //   l_nv = h_n . W_v + b_v,   lse_n = log sum_v exp l_nv,   loss_n = lse_n - l_n,label(n)
 //   d_nv = (exp(l_nv - lse_n) - [v = label(n)]) g_n,   dh_n = sum_v d_nv W_v,   dW_v = sum_n d_nv h_n,   db_v = sum_n d_nv
@@ -37,13 +37,9 @@ struct Kept {
     int32_t *pos;       // [N]: where a token's row is among the labelled ones, or -1
     int32_t *label;     // [labelled]
     float2 *level;      // [labelled]: a token's largest logit times log2(e), and one over the sum of the exponentials of what they are below it
-};                      // (the last two up to a whole tile: tiles are read whole)
-int64_t kept_bytes(int64_t N) { return 16 + up(N * 4, 16) + up(N, TILE) * 12; }
-Kept kept_at(void *at, int64_t N) {
-    char *p = static_cast<char *>(at);
-    const int64_t n = up(N * 4, 16), tiles = up(N, TILE);
-    return {reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + 16), reinterpret_cast<int32_t *>(p + 16 + n), reinterpret_cast<float2 *>(p + 16 + n + tiles * 4)};
-}
+                        // (the last two up to a whole tile: tiles are read whole)
+    float *logits;      // [labelled, up(vocabulary, 32)], or null: of few tokens, where they are no more than the weights
+};
 
 struct Sizes {
     int N, V, K;               // tokens, vocabulary, columns
@@ -452,12 +448,26 @@ constexpr int64_t few_lds(int64_t tokens, int64_t row_bytes) {
 int64_t row_bytes(const lffn_linear_cross_entropy &a) { return a.columns * (a.format == LFFN_ROWS_F32 ? 4 : 2); }
 bool few_tokens(const lffn_linear_cross_entropy &a) { return a.tokens <= FEW && few_lds(a.tokens, row_bytes(a)) <= 160 * 1024; }
 
+// The backward of few tokens takes their logits from the forward where they are no more bytes than the weights, which it would read for them once more (both directions,
+// 19 tokens, 50265 x 768 fp32: 291 us with them formed again, 246 with these).
+constexpr int64_t logits_stride(int64_t vocabulary) { return up(vocabulary, 32); }
+bool keeps_logits(const lffn_linear_cross_entropy &a) { return few_tokens(a) && a.tokens * 4 <= row_bytes(a); }
+int64_t kept_bytes(const lffn_linear_cross_entropy &a, bool logits) {
+    return 16 + up(a.tokens * 4, 16) + up(a.tokens, TILE) * 12 + (logits ? a.tokens * logits_stride(a.vocabulary) * 4 : 0);
+}
+Kept kept_at(const lffn_linear_cross_entropy &a, void *at) {
+    char *p = static_cast<char *>(at);
+    const int64_t n = up(a.tokens * 4, 16), tiles = up(a.tokens, TILE);
+    return {reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + 16), reinterpret_cast<int32_t *>(p + 16 + n), reinterpret_cast<float2 *>(p + 16 + n + tiles * 4),
+            keeps_logits(a) ? reinterpret_cast<float *>(p + 16 + n + tiles * 12) : nullptr};
+}
+
 int few_workgroups(const lffn_linear_cross_entropy &a) { return (int)min((a.vocabulary + 31) / 32, int64_t(COMPUTE_UNITS)); }
 
 struct FewArgs {
     RowsArgs r;
     float2 *parts;
-    float *at_label;
+    float *at_label, *logits;      // the last: null without a backward
     int64_t Np;
 };
 
@@ -610,6 +620,11 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) l[e] = WHOLE ? sums[j][0][e] + sums[j][Of::SUMS - 1][e] : sums[j][0][e];
             of[j] = with_logits(of[j], l);
+            if (a.logits && label[j] >= 0) {
+                float *const to = a.logits + (32 * j + lane % 32) * logits_stride(V) + v0 + 4 * half;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) *reinterpret_cast<float4 *>(to + 8 * g) = make_float4(l[4 * g], l[4 * g + 1], l[4 * g + 2], l[4 * g + 3]);
+            }
             const int r = label[j] - v0;
             if (label[j] >= 0 && r >= 0 && r < 32 && r / 4 % 2 == half) {
                 float found = l[0];
@@ -809,6 +824,12 @@ __device__ __forceinline__ Shares shares_of(const BackwardArgs &a, int labelled)
     return best;
 }
 
+template <typename F>
+__device__ __forceinline__ void put_shares(const BackwardArgs &a, int labelled, const Piece &p) {
+    const Shares shares = shares_of<F>(a, labelled);
+    if (threadIdx.x % 64 == 0) a.shares[0] = shares.vocabulary, a.shares[1] = p.pieces, a.shares[2] = shares.tokens;
+}
+
 // What both gradients' sums are multiplied with: of a sum or mean what all tokens' d are, else the power of two that their coefficients were divided by.
 __device__ __forceinline__ float factor_of(const BackwardArgs &a, int labelled) {
     if (a.reduction == 0) return *a.power;
@@ -909,8 +930,47 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
     });
     // (one of the workgroups that have the fewest tiles)
     if (piece == 0 && blockIdx.x == gridDim.x - 1 && wave == 0) {
-        const Shares shares = shares_of<F>(a, labelled);
-        if (lane == 0) a.shares[0] = shares.vocabulary, a.shares[1] = p.pieces, a.shares[2] = shares.tokens;
+        put_shares<F>(a, labelled, p);
+    }
+}
+
+// d of few tokens from their logits: eight entries of a token a thread, zeros for the tokens behind (as far as dW's sums go; what dh's tile reads behind those is not stored).
+constexpr int FEW_ROWS = 2 * STEP;
+static_assert(FEW_ROWS >= FEW && FEW_ROWS <= TILE, "dW's sums over few tokens are two steps");
+template <typename F>
+__global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
+    const int labelled = a.o.kept.head[0], n = blockIdx.y, V = a.o.s.V;
+    const Piece p = piece_of<F>(a, labelled, piece);
+    if (piece == 0 && n == FEW_ROWS - 1 && blockIdx.x == 0 && threadIdx.x < 64) put_shares<F>(a, labelled, p);
+    const int in = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 8;
+    if (in >= p.ld - APART || p.width <= 0) return;
+    float l[8] = {};
+    if (n < labelled) {
+        const float2 level = a.o.kept.level[n];
+        const float by = LIFT * (a.coefficient ? a.coefficient[n] : 1.f), p_by = level.y * by;
+        const float *from = a.o.kept.logits + n * logits_stride(V) + p.v0 + in;
+        const int at = a.o.kept.label[n] - p.v0 - in;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            if (in + 4 * g >= p.width) continue;               // (the last ones may be behind the vocabulary: within the row)
+            const float4 v = *reinterpret_cast<const float4 *>(from + 4 * g);
+            const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                l[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(w[e], LOG2E, -level.x)) * p_by - (at == 4 * g + e ? by : 0.f);
+                if (in + 4 * g + e >= p.width) l[4 * g + e] = 0.f;
+            }
+        }
+    }
+    char *const to = a.d + int64_t(n) * p.ld * 2 * F::PLANES + byte_of<F::PLANES>(in);
+    auto put = [&](char *at) {
+        *reinterpret_cast<uint4 *>(at) = make_uint4(F::pack2(l[0], l[1]), F::pack2(l[2], l[3]), F::pack2(l[4], l[5]), F::pack2(l[6], l[7]));
+    };
+    put(to);
+    if constexpr (F::PLANES == 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l[e] -= (float)(_Float16)l[e];
+        put(to + 64);
     }
 }
 
@@ -1234,6 +1294,7 @@ struct Forward {
     RowsArgs r;
     JoinArgs j;
     void *kept;
+    float *logits;
     int32_t *counts, *groups;
 };
 int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Forward &f) {
@@ -1249,7 +1310,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, bool with_kept, Fo
     f.j.token = f.r.token = c.take<int32_t>(Np);
     f.counts = c.take<int32_t>(a.tokens / CHUNK + 1);
     f.groups = c.take<int32_t>(a.tokens / COUNTED + 1);
-    f.kept = with_kept ? c.take<char>(kept_bytes(a.tokens)) : nullptr;
+    f.kept = with_kept ? c.take<char>(kept_bytes(a, false)) : nullptr;
     return c.used;
 }
 
@@ -1318,7 +1379,7 @@ int few(const lffn_linear_cross_entropy &a, Forward &f, hipStream_t st) {
     const int64_t lds = few_lds(a.tokens, row_bytes(a));
     if (!lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&few_kernel<F, TOKENS>), lds, granted)) return LFFN_ERR_LAUNCH;
     f.j.tiles = few_workgroups(a);
-    few_kernel<F, TOKENS><<<dim3(f.j.tiles), dim3(THREADS), lds, st>>>({f.r, f.f.parts, f.f.at_label, f.f.Np});
+    few_kernel<F, TOKENS><<<dim3(f.j.tiles), dim3(THREADS), lds, st>>>({f.r, f.f.parts, f.f.at_label, f.logits, f.f.Np});
     return LFFN_OK;
 }
 template <typename F>
@@ -1341,7 +1402,11 @@ int backward(const BackwardArgs &b, hipStream_t st) {
         !lffn_grant_dynamic_lds(reinterpret_cast<const void *>(&gradients_kernel<F, R>), STREAM_LDS, granted_g))
         return LFFN_ERR_LAUNCH;
     for (int p = 0; p < b.pieces; ++p) {
-        d_kernel<F><<<dim3(COMPUTE_UNITS), dim3(THREADS), LDS_BYTES, st>>>(b, p);
+        if (b.o.kept.logits) {
+            const int64_t widest_piece = up((b.o.s.Vp / TILE + b.pieces - 1) / b.pieces * TILE, 2048);
+            few_d_kernel<F><<<dim3(unsigned(widest_piece / 2048), FEW_ROWS), dim3(256), 0, st>>>(b, p);
+        } else
+            d_kernel<F><<<dim3(COMPUTE_UNITS), dim3(THREADS), LDS_BYTES, st>>>(b, p);
         gradients_kernel<F, R><<<dim3(COMPUTE_UNITS), dim3(THREADS), STREAM_LDS, st>>>(b, p);
     }
     if (b.grad_hidden) {
@@ -1362,7 +1427,7 @@ int backward(const BackwardArgs &b, hipStream_t st) {
 extern "C" int lffn_linear_cross_entropy_kept_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes) {
     LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
     const int rc = check(a);
-    if (rc == LFFN_OK) *bytes = kept_bytes(a->tokens);
+    if (rc == LFFN_OK) *bytes = kept_bytes(*a, keeps_logits(*a));
     return rc;
 }
 
@@ -1383,7 +1448,8 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
     LFFN_REQUIRE(lffn_aligned16(kept), LFFN_ERR_BAD_ARG);
     if (a->reduction == 0 && a->tokens == 0) return LFFN_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    f.f.o.kept = f.j.kept = kept_at(kept ? kept : f.kept, a->tokens);
+    f.f.o.kept = f.j.kept = kept_at(*a, kept ? kept : f.kept);
+    f.logits = kept ? f.f.o.kept.logits : nullptr;
     fill(f.r, *a, f.f.o);
     if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.sums = nullptr;
     // (workgroups that look for the largest scales behind those that join)
@@ -1428,7 +1494,7 @@ extern "C" int lffn_linear_cross_entropy_bwd(const lffn_linear_cross_entropy *a,
     LFFN_REQUIRE(workspace && lffn_aligned16(workspace) && workspace_bytes >= carve(*a, static_cast<char *>(workspace), w), LFFN_ERR_BAD_ARG);
     hipStream_t st = static_cast<hipStream_t>(stream);
     BackwardArgs &b = w.b;
-    b.o.kept = kept_at(const_cast<void *>(kept), a->tokens);
+    b.o.kept = kept_at(*a, const_cast<void *>(kept));
     b.g_loss = g_loss;
     b.grad_hidden = grad_hidden, b.grad_weight = grad_weight, b.grad_bias = grad_bias;
     b.bias_format = a->bias_format, b.reduction = a->reduction;

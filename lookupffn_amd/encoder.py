@@ -322,7 +322,7 @@ class Lookup(nn.Module):
 
 class MaskedLMHead(nn.Module):
     """What the reference pre-trains its encoder by (src/roberta/tasks/mlm.py:33-112), behind the encoder: a projection, gelu and layer norm of the states, and the projection
-    to the vocabulary by the word embeddings with a bias of its own.  With labels the loss, whose logits are never in memory as a whole and whose cost is that of the
+    to the vocabulary by the word embeddings with a bias of its own.  With labels the loss, whose logits are not in memory as a whole and whose cost is that of the
     labelled tokens (``linear_cross_entropy``); without, the logits.  GPU only; hidden_size a multiple of 8.
 
     ``config``: hidden_size, vocab_size, layer_norm_eps."""

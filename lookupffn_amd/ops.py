@@ -1738,9 +1738,13 @@ def _linear_cross_entropy_args(hidden, weight, bias, labels, ignore_index, reduc
     return a
 
 
-def _loss_kept_bytes(tokens):
-    """lffn_linear_cross_entropy_kept_bytes: how many tokens have a label, where a token is among them, and of those the label and two levels."""
-    return 16 + (tokens * 4 + 15) // 16 * 16 + (tokens + 255) // 256 * 256 * 12
+def _loss_kept_bytes(hidden, weight):
+    """lffn_linear_cross_entropy_kept_bytes: how many tokens have a label, where a token is among them, and of those the label and two levels; of up to 64 tokens whose rows fit
+    160 KB the logits, where they are no more than the weights."""
+    (tokens, columns), vocabulary, size = hidden.shape, weight.shape[0], hidden.element_size()
+    kept = 16 + (tokens * 4 + 15) // 16 * 16 + (tokens + 255) // 256 * 256 * 12
+    few = tokens <= 64 and (32 if tokens <= 32 else 64) * ((columns * size + 127) // 128 * 8 | 1) * 16 + 64 * 64 + 64 * 4 <= 160 * 1024
+    return kept + (tokens * ((vocabulary + 31) // 32 * 32) * 4 if few and tokens * 4 <= columns * size else 0)
 
 
 _L.define("linear_cross_entropy(Tensor hidden, Tensor weight, Tensor? bias, Tensor labels, int ignore_index, int reduction, bool keep) -> (Tensor, Tensor)")
@@ -1755,7 +1759,7 @@ def _linear_cross_entropy_impl(hidden, weight, bias, labels, ignore_index, reduc
     bias = None if bias is None else bias.contiguous()
     a = _linear_cross_entropy_args(hidden, weight, bias, labels, ignore_index, reduction)
     loss = torch.empty(hidden.shape[:1] if reduction == 0 else (), dtype=torch.float32, device=hidden.device)
-    kept = torch.empty(_loss_kept_bytes(hidden.shape[0]) if keep else 0, dtype=torch.uint8, device=hidden.device)
+    kept = torch.empty(_loss_kept_bytes(hidden, weight) if keep else 0, dtype=torch.uint8, device=hidden.device)
     with _dev_guard(hidden):
         lib, n = _lib.load(), ctypes.c_int64(0)
         _lib.check(lib.lffn_linear_cross_entropy_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "lffn_linear_cross_entropy_workspace_bytes")
@@ -1772,7 +1776,7 @@ _L.impl("linear_cross_entropy", _linear_cross_entropy_impl, "CUDA")
 @torch.library.register_fake("lookupffn::linear_cross_entropy")
 def _(hidden, weight, bias, labels, ignore_index, reduction, keep):
     return (hidden.new_empty(hidden.shape[:1] if reduction == 0 else (), dtype=torch.float32),
-            hidden.new_empty(_loss_kept_bytes(hidden.shape[0]) if keep else 0, dtype=torch.uint8))
+            hidden.new_empty(_loss_kept_bytes(hidden, weight) if keep else 0, dtype=torch.uint8))
 
 
 _L.define("linear_cross_entropy_bwd(Tensor hidden, Tensor weight, Tensor? bias, Tensor labels, int ignore_index, int reduction, Tensor kept, Tensor g, "
@@ -1783,7 +1787,7 @@ def _linear_cross_entropy_bwd_impl(hidden, weight, bias, labels, ignore_index, r
     """-> the gradients of hidden, weight and bias that are wanted."""
     _lib.require_gpu(hidden, weight, bias, labels, kept, g)
     _fit_loss(hidden, weight, bias, labels, reduction)
-    assert kept.dtype == torch.uint8 and kept.shape == (_loss_kept_bytes(hidden.shape[0]),)
+    assert kept.dtype == torch.uint8 and kept.shape == (_loss_kept_bytes(hidden, weight),)
     assert g.dtype == torch.float32 and g.shape == (hidden.shape[:1] if reduction == 0 else ()) and not (of_bias and bias is None)
     hidden, weight, labels, kept = _rows_together(hidden), _rows_together(weight), labels.contiguous(), _aligned(kept)
     bias, g = None if bias is None else bias.contiguous(), g.contiguous()

@@ -78,7 +78,7 @@ class LinearCrossEntropy(Function):
 
 
 def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, reduction="mean"):
-    """Softmax cross entropy of the logits hidden W^T + bias, which are never in memory as a whole:
+    """Softmax cross entropy of the logits hidden W^T + bias, which are not in memory as a whole:
 
         loss_n = log sum_v exp l_nv - l_n,label(n),  l_nv = hidden[n] . weight[v] + bias[v]
 
@@ -89,7 +89,7 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
 
     float32: products of two half-precision terms a number, sums in float32, errors of the size of float32 products'; in the backward a number of hidden or
     weight is held to 2^-38 of the largest of its array.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half: held to 2^-38 of the largest token's).
-    Memory: the backward has a workspace of up to 1 GB for the logits' gradients (with more than some 250000 tokens 4.2 KB a token) and up to 0.75 GB for sums; float32 weights are laid out once more.
+    Memory: of up to 64 tokens the logits are kept for the backward where they are no more bytes than weight.  The backward has a workspace of up to 1 GB for the logits' gradients (with more than some 250000 tokens 4.2 KB a token) and up to 0.75 GB for sums; float32 weights are laid out once more.
     -> float32.  Gradients: hidden, weight and bias, the same bits on every call; none of theirs, and none in forward mode (an error); captured in graphs as ``cross_attention`` is."""
     host = _host()
     if host:

@@ -194,6 +194,16 @@ def test_ignored_rows_may_hold_anything():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,K", [(7, 64), (60, 16), (130, 64)])
+def test_no_token_has_a_label(N, K, dtype):
+    h, w, b = (_randn(N, K, dtype=dtype).requires_grad_(), _randn(200, K, dtype=dtype, seed=1).requires_grad_(), _randn(200, seed=2).requires_grad_())
+    y = torch.full((N,), -100, device=DEV)
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(h, w, b, y, reduction=reduction)
+        assert (loss == 0).all() and all((t == 0).all() for t in torch.autograd.grad(loss, (h, w, b), torch.ones_like(loss)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("N", [40, 300])
 def test_an_infinite_token_leaves_the_others(N, dtype):
     """A token's infinite numbers, or an infinite gradient of its loss, reach that token's loss and gradient, and no other's."""

@@ -126,7 +126,7 @@ OF_NORM = [("x", (5, 64, 1)), ("x", torch.float64), ("weight", (63,)), ("weight"
 
 @pytest.mark.parametrize("impl,args,name,change", [
     *(("_linear_cross_entropy_impl", lambda: dict(_loss_args(), keep=True), *c) for c in OF_LOSS),
-    *(("_linear_cross_entropy_bwd_impl", lambda: dict(_loss_args(), kept=_gpu(ops._loss_kept_bytes(6), dtype=torch.uint8), g=_gpu(dtype=torch.float32), of_hidden=True, of_weight=True,
+    *(("_linear_cross_entropy_bwd_impl", lambda: dict(_loss_args(), kept=_gpu(ops._loss_kept_bytes(_gpu(6, 64), _gpu(90, 64)), dtype=torch.uint8), g=_gpu(dtype=torch.float32), of_hidden=True, of_weight=True,
                                                       of_bias=True), *c) for c in OF_LOSS + [("kept", (64,)), ("kept", torch.int8), ("g", (6,)), ("g", torch.float16), ("bias", None)]),
     *(("_layer_norm_impl", lambda: dict(x=_gpu(5, 64), weight=_gpu(64), bias=_gpu(64), eps=1e-5, keep=True), *c) for c in OF_NORM),
     *(("_layer_norm_rows_bwd_impl", lambda: dict(x=_gpu(5, 64), weight=_gpu(64), bias=_gpu(64), stats=_gpu(5, 2, dtype=torch.float32), g=_gpu(5, 64), of_x=True, of_weight=True, of_bias=True),
@@ -192,9 +192,12 @@ def test_c_entries_check_their_arguments():
                  dict(tokens=1 << 24, columns=512, weight_stride=512)):
         assert fwd(of(**much)) == UNSUPPORTED, much
     assert fwd(of(), out=None) == BAD and fwd(of(), ws=None) == BAD and fwd(of(), ws=P + 8) == BAD and fwd(of(), size=n.value - 1) == BAD and fwd(of(), kept=P + 4) == BAD
-    assert lib.lffn_linear_cross_entropy_kept_bytes(of(), ctypes.byref(n)) == OK and n.value == ops._loss_kept_bytes(5)
-    for tokens in (0, 1, 255, 256, 257, 70000):
-        assert lib.lffn_linear_cross_entropy_kept_bytes(of(tokens=tokens), ctypes.byref(n)) == OK and n.value == ops._loss_kept_bytes(tokens)
+    for format, dtype in ((0, torch.float32), (2, torch.bfloat16)):
+        for tokens, vocabulary, columns in ((5, 90, 64), (0, 90, 64), (1, 90, 8), (32, 90, 64), (33, 90, 64), (32, 33, 1216), (32, 33, 1224), (32, 33, 2424), (32, 33, 2432), (64, 1, 608),
+                                            (64, 1, 616), (64, 1, 1208), (64, 1, 1216), (64, 1, 128), (64, 1, 120), (65, 90, 512), (255, 90, 64), (256, 90, 64), (257, 90, 64), (70000, 90, 64)):
+            a = of(tokens=tokens, vocabulary=vocabulary, columns=columns, hidden_stride=columns, weight_stride=columns, format=format)
+            want = ops._loss_kept_bytes(torch.empty(tokens, columns, dtype=dtype, device="meta"), torch.empty(vocabulary, columns, dtype=dtype, device="meta"))
+            assert lib.lffn_linear_cross_entropy_kept_bytes(a, ctypes.byref(n)) == OK and n.value == want, (tokens, vocabulary, columns, format)
     assert lib.lffn_linear_cross_entropy_bwd_workspace_bytes(of(), ctypes.byref(n)) == OK and n.value > 0
     bwd = lambda a, kept=P, g=P, gh=P, gw=P, gb=P, ws=P, size=n.value: lib.lffn_linear_cross_entropy_bwd(a, kept, g, gh, gw, gb, ws, size, None)  # noqa: E731
     assert bwd(of(), kept=None) == BAD and bwd(of(), g=None) == BAD and bwd(of(), gw=None) == BAD and bwd(of(), gh=P + 8) == BAD and bwd(of(), gw=P + 8) == BAD
