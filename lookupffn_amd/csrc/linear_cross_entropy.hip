@@ -280,6 +280,16 @@ struct Place {
     }
 };
 
+// How eight wavefronts share a tile of TILE entries, or columns, x TOKENS_ tokens: M x N of them along its entries and tokens.  Up to 64 labelled tokens take a tile of as many, here and in
+// dh: a quarter of the products (58 of 385 tokens labelled, 50265 x 768 bfloat16: logits 18.6 us for 27.2, d 21.5 for 28.4, both gradients 46 for 56; 9 labelled, 50265 x 840 fp32: 55 for 70, 61 for 84, 99 for 121).
+constexpr int NARROW = 64;
+template <int TOKENS_, int M_, int N_>
+struct OfLogits {
+    static constexpr int TOKENS = TOKENS_, M = M_, N = N_, MB = TILE / M / 32, NB = TOKENS / N / 32;
+};
+typedef OfLogits<TILE, WAVES_M, WAVES_N> WideLogits;
+typedef OfLogits<NARROW, 4, 2> NarrowLogits;
+
 typedef Along<TILE, THREADS, 1> AlongOne;
 constexpr uint32_t STREAM_LDS = Stream<F16, MB, NB, AlongOne, AlongOne>::LDS;      // (of any operands)
 
@@ -309,17 +319,19 @@ __device__ __forceinline__ T beside(uint32_t lds, Beside of, int at) {
 
 // The logits of one tile after the other: entries from v0 on, in all `width`, and the labelled tokens; each(sums, place, lds) has the sums of a tile's products, of one plane with the bias, and
 // what came beside it, and calls landed() before it stores anything.
-template <typename F, bool BACKWARD, typename Each>
+template <typename F, typename S, bool BACKWARD, typename Each>
 __device__ __forceinline__ void for_logits(const Operands &o, const float *coefficient, int labelled, int v0, int width, uint32_t lds, Each &&each) {
     typedef Along<TILE, THREADS, F::PLANES> Side;
+    typedef Along<S::TOKENS, THREADS, F::PLANES> Rows;
     const int wave = threadIdx.x / 64, half = threadIdx.x % 64 / 32, vt = (width + TILE - 1) / TILE, nt = (labelled + TILE - 1) / TILE;
     const int steps = max(2, (o.s.K + Side::K - 1) / Side::K);
     Turns turns(vt * nt);
     if (!turns.any()) return;
     const Source rows = rows_of<F::PLANES>(o, labelled);
     Place place(turns.at, vt, nt);
-    Side a(o.weight, v0 + place.v), b(rows, place.n);
-    Stream<F, MB, NB, Side, Side> stream(lds, wave / WAVES_N * MB * 32, wave % WAVES_N * NB * 32);
+    Side a(o.weight, v0 + place.v);
+    Rows b(rows, place.n);
+    Stream<F, S::MB, S::NB, Side, Rows> stream(lds, wave / S::N * S::MB * 32, wave % S::N * S::NB * 32);
     uint32_t by = lds + STREAM_LDS, next_by = by + BESIDE_BYTES;
     bring_beside<BACKWARD>(o, coefficient, v0 + place.v, place.n, by);
     stream.prime(a, b, 0);
@@ -327,16 +339,17 @@ __device__ __forceinline__ void for_logits(const Operands &o, const float *coeff
         const int next = turns.at + turns.step;
         const bool more = next < turns.end;
         const Place then(more ? next : turns.at, vt, nt);
-        const Side next_a(o.weight, v0 + then.v), next_b(rows, then.n);
-        Sums<MB, NB> sums;
+        const Side next_a(o.weight, v0 + then.v);
+        const Rows next_b(rows, then.n);
+        Sums<S::MB, S::NB> sums;
         if constexpr (F::PLANES == 1) {
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
+            for (int i = 0; i < S::MB; ++i)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const float4 bias = beside<float4>(by, BIAS, (wave / WAVES_N * MB + i) * 8 + 2 * g + half);
+                    const float4 bias = beside<float4>(by, BIAS, (wave / S::N * S::MB + i) * 8 + 2 * g + half);
 #pragma unroll
-                    for (int j = 0; j < NB; ++j)
+                    for (int j = 0; j < S::NB; ++j)
                         sums.v[i][j][4 * g] = bias.x, sums.v[i][j][4 * g + 1] = bias.y, sums.v[i][j][4 * g + 2] = bias.z, sums.v[i][j][4 * g + 3] = bias.w;
                 }
         } else
@@ -395,25 +408,22 @@ __device__ __forceinline__ float2 with_logits(float2 of, const float (&l)[16]) {
     return make_float2(most, sum);
 }
 
-template <typename F>
-__global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
-    const uint32_t lds = lds_byte_of(lds_words);
-    float2 *const halves = reinterpret_cast<float2 *>(reinterpret_cast<char *>(lds_words) + STREAM_LDS + 2 * BESIDE_BYTES);     // [WAVES_M][TILE]
+template <typename F, typename S>
+__device__ __forceinline__ void forward_tiles(const ForwardArgs &a, uint32_t lds, float2 *parts) {
     const Operands &o = a.o;
     const int labelled = o.kept.head[0], tid = threadIdx.x, wave = tid / 64, lane = tid % 64, half = lane / 32;
-    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-    for_logits<F, false>(o, nullptr, labelled, 0, o.s.V, lds, [&](const Sums<MB, NB> &sums, const Place &p, uint32_t by) {
+    const int wm = wave / S::N, wn = wave % S::N;
+    for_logits<F, S, false>(o, nullptr, labelled, 0, o.s.V, lds, [&](const Sums<S::MB, S::NB> &sums, const Place &p, uint32_t by) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int column = wn * NB * 32 + j * 32 + lane % 32, n = p.n + column;
+        for (int j = 0; j < S::NB; ++j) {
+            const int column = wn * S::NB * 32 + j * 32 + lane % 32, n = p.n + column;
             const float row_scale = F::PLANES == 2 ? beside<float>(by, ROW_SCALE, column) : 1.f;
-            const int at = n < labelled ? beside<int>(by, LABEL, column) - p.v - wm * MB * 32 : -1;
+            const int at = n < labelled ? beside<int>(by, LABEL, column) - p.v - wm * S::MB * 32 : -1;
             float2 of = make_float2(-INFINITY, 0.f);
 #pragma unroll
-            for (int i = 0; i < MB; ++i) {
+            for (int i = 0; i < S::MB; ++i) {
                 float l[16];
-                logits_of<F>(l, sums.v[i][j], by, (wm * MB + i) * 32, row_scale);
+                logits_of<F>(l, sums.v[i][j], by, (wm * S::MB + i) * 32, row_scale);
                 of = with_logits(of, l);
                 const int r = at - 32 * i;
                 if (r >= 0 && r < 32 && r / 4 % 2 == half) {
@@ -425,14 +435,30 @@ __global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
                 }
             }
             const float2 other = make_float2(__shfl_xor(of.x, 32), __shfl_xor(of.y, 32));
-            if (half == 0) halves[wm * TILE + column] = joined(of, other);
+            if (half == 0) parts[wm * S::TOKENS + column] = joined(of, other);
         }
         arrived();
         __syncthreads();
-        if (tid < TILE) a.parts[p.v / TILE * a.Np + p.n + tid] = joined(halves[tid], halves[TILE + tid]);
-        // (the next tile's products have barriers before halves is written again)
+        if (tid < S::TOKENS) {
+            float2 of = parts[tid];
+#pragma unroll
+            for (int m = 1; m < S::M; ++m) of = joined(of, parts[m * S::TOKENS + tid]);
+            a.parts[p.v / TILE * a.Np + p.n + tid] = of;
+        }
+        // (the next tile's products have barriers before the parts are written again)
     });
 }
+
+template <typename F>
+__global__ __launch_bounds__(THREADS, 2) void forward_kernel(ForwardArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
+    const uint32_t lds = lds_byte_of(lds_words);
+    float2 *const parts = reinterpret_cast<float2 *>(reinterpret_cast<char *>(lds_words) + STREAM_LDS + 2 * BESIDE_BYTES);     // of a tile's tokens, by wavefronts along the entries
+    if (a.o.kept.head[0] <= NARROW) forward_tiles<F, NarrowLogits>(a, lds, parts);
+    else forward_tiles<F, WideLogits>(a, lds, parts);
+}
+static_assert(NarrowLogits::M * NarrowLogits::TOKENS <= WAVES_M * TILE, "the parts' room");
+
 
 // ---------------------------------------------------------------- few tokens
 
@@ -877,21 +903,20 @@ __device__ __forceinline__ void pieces_of(const float (&l)[16], uint4 (&w)[2]) {
     w[1] = make_uint4(q[1][0], q[1][1], q[1][2], q[1][3]);
 }
 
-template <typename F>
-__global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece) {
-    if (piece > 0 && piece >= a.shares[1]) return;
-    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
-    const uint32_t lds = lds_byte_of(lds_words);
+constexpr int FEW_ROWS = 2 * STEP;              // tokens that dW's sums over few have, at least
+static_assert(FEW_ROWS >= FEW && FEW_ROWS <= TILE && FEW_ROWS == 2 * NARROW, "two steps; twice a narrow tile");
+
+template <typename F, typename S>
+__device__ __forceinline__ void d_tiles(const BackwardArgs &a, const Piece &p, int labelled, uint32_t lds) {
     const Operands &o = a.o;
-    const int labelled = o.kept.head[0], wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / WAVES_N, wn = wave % WAVES_N;
-    const Piece p = piece_of<F>(a, labelled, piece);
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / S::N, wn = wave % S::N;
     const float scale = F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : 1.f;
-    for_logits<F, true>(o, a.coefficient, labelled, p.v0, p.width, lds, [&](const Sums<MB, NB> &sums, const Place &tile, uint32_t beside_) {
-        const int in = tile.v + wm * MB * 32;
+    for_logits<F, S, true>(o, a.coefficient, labelled, p.v0, p.width, lds, [&](const Sums<S::MB, S::NB> &sums, const Place &tile, uint32_t beside_) {
+        const int in = tile.v + wm * S::MB * 32;
         bool stored = false;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int column = wn * NB * 32 + j * 32 + lane % 32, n = tile.n + column;
+        for (int j = 0; j < S::NB; ++j) {
+            const int column = wn * S::NB * 32 + j * 32 + lane % 32, n = tile.n + column;
             const bool live = n < labelled;
             // (a token behind the last: exponentials of minus infinity, times zero)
             const float2 level = live ? beside<float2>(beside_, LEVEL, column) : make_float2(INFINITY, 0.f);
@@ -899,9 +924,9 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
             const int at = live ? beside<int>(beside_, LABEL, column) - p.v0 - in : -1;
             char *const row = a.d + (int64_t(n - lane % 32 + lane % 16) * p.ld + in) * 2 * F::PLANES + 16 * piece_of_lane(lane);       // (of the block's first 16 tokens)
 #pragma unroll
-            for (int i = 0; i < MB; ++i) {
+            for (int i = 0; i < S::MB; ++i) {
                 float l[16];
-                logits_of<F>(l, sums.v[i][j], beside_, (wm * MB + i) * 32, scale);
+                logits_of<F>(l, sums.v[i][j], beside_, (wm * S::MB + i) * 32, scale);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) l[e] = __builtin_amdgcn_exp2f(fmaf(l[e], LOG2E, -level.x)) * p_by;
                 const int r = at - 32 * i;
@@ -920,6 +945,10 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
                     *reinterpret_cast<uint4 *>(to + 64 * F::PLANES * i + 32 * F::PLANES * int64_t(p.ld)) = w[1];
                 };
                 put(row);
+                if constexpr (S::TOKENS < FEW_ROWS && F::PLANES == 1) {              // (dW's sums are two steps at least)
+                    char *const behind = row + S::TOKENS * int64_t(p.ld) * 2 + 64 * i;
+                    *reinterpret_cast<uint4 *>(behind) = *reinterpret_cast<uint4 *>(behind + 32 * int64_t(p.ld)) = make_uint4(0, 0, 0, 0);
+                }
                 if constexpr (F::PLANES == 2) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) l[e] -= (float)(_Float16)l[e];
@@ -928,15 +957,24 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
             }
         }
     });
+}
+
+template <typename F>
+__global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece) {
+    if (piece > 0 && piece >= a.shares[1]) return;
+    extern __shared__ __attribute__((aligned(16))) uint4 lds_words[];
+    const uint32_t lds = lds_byte_of(lds_words);
+    const int labelled = a.o.kept.head[0];
+    const Piece p = piece_of<F>(a, labelled, piece);
+    if (labelled <= NARROW) d_tiles<F, NarrowLogits>(a, p, labelled, lds);
+    else d_tiles<F, WideLogits>(a, p, labelled, lds);
     // (one of the workgroups that have the fewest tiles)
-    if (piece == 0 && blockIdx.x == gridDim.x - 1 && wave == 0) {
+    if (piece == 0 && blockIdx.x == gridDim.x - 1 && threadIdx.x / 64 == 0) {
         put_shares<F>(a, labelled, p);
     }
 }
 
 // d of few tokens from their logits: eight entries of a token a thread, zeros for the tokens behind (as far as dW's sums go; what dh's tile reads behind those is not stored).
-constexpr int FEW_ROWS = 2 * STEP;
-static_assert(FEW_ROWS >= FEW && FEW_ROWS <= TILE, "dW's sums over few tokens are two steps");
 template <typename F>
 __global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
     const int labelled = a.o.kept.head[0], n = blockIdx.y, V = a.o.s.V;
@@ -1002,9 +1040,10 @@ __device__ __forceinline__ void store8(char *to, const float (&v)[8]) {
 }
 
 // dh: shares of the piece's entries x tiles of tokens x tiles of columns, one after the other; each adds to its own part.
-template <typename F>
+template <typename F, int TOKENS>
 __device__ __forceinline__ void hidden_tasks(const BackwardArgs &a, const Piece &p, int labelled, int piece, int unit, uint32_t lds) {
-    typedef Along<TILE, THREADS, F::PLANES> Left;
+    typedef Along<TOKENS, THREADS, F::PLANES> Left;
+    constexpr int MB = TOKENS / WAVES_M / 32;
     typedef Across<TILE, THREADS, F::PLANES> Right;
     const Operands &o = a.o;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, ht = (o.s.K + TILE - 1) / TILE;
@@ -1170,7 +1209,8 @@ __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, i
     if (p.width <= 0) return;
     // (COMPUTE_UNITS workgroups; the units of an XCD have neighbouring numbers)
     const int unit = blockIdx.x % XCDS * (COMPUTE_UNITS / XCDS) + blockIdx.x / XCDS;
-    if (a.grad_hidden && labelled) hidden_tasks<F>(a, p, labelled, piece, unit, lds);
+    if (a.grad_hidden && labelled > NARROW) hidden_tasks<F, TILE>(a, p, labelled, piece, unit, lds);
+    else if (a.grad_hidden && labelled) hidden_tasks<F, NARROW>(a, p, labelled, piece, unit, lds);
     if (a.grad_weight) weight_tasks<F, R>(a, p, labelled, unit, lds);
 }
 

@@ -101,11 +101,11 @@ def _check(h, w, b, y, reduction="mean", ignore=-100, g=None):
 
 
 # tokens, vocabulary, columns, share of the tokens that have a label: one of each; sizes below, at and beyond a tile's; tokens that are counted in a launch of their own; many tiles; tokens
-# whose sums are cut
+# whose sums are cut; few labelled ones
 SIZES = [(1, 1, 8, 1.0), (1, 300, 64, 1.0), (5, 7, 16, 0.8), (64, 1000, 72, 1.0), (255, 255, 40, 1.0), (256, 256, 64, 1.0), (257, 513, 136, 0.5), (300, 777, 520, 0.3), (33, 5003, 264, 1.0),
          (4200, 600, 64, 0.1), (700, 2100, 776, 0.9), (130, 4096, 1032, 1.0), (40, 70001, 24, 0.9), (64, 300, 1208, 1.0), (64, 300, 1216, 1.0), (20, 300, 2432, 1.0), (32, 40, 2424, 0.9),
          (64, 300, 608, 1.0), (64, 300, 616, 1.0), (32, 40, 1216, 0.9), (20, 9000, 1224, 1.0), (1100, 300, 40, 1.0), (5000, 300, 72, 1.0), (9001, 40, 264, 0.9),
-         (4097, 1100, 24, 0.6)]
+         (4097, 1100, 24, 0.6), (300, 777, 72, 0.1), (129, 1500, 520, 0.45), (90, 1030, 1400, 0.5)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
