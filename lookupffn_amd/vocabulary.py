@@ -82,14 +82,17 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
 
         loss_n = log sum_v exp l_nv - l_n,label(n),  l_nv = hidden[n] . weight[v] + bias[v]
 
-    hidden: [..., columns], weight: [vocabulary, columns] of its type, columns a multiple of 8 (at most 65536; vocabulary at most 2^22, tokens at most 2^24, 2^32 numbers of hidden), with any strides (a copy is
-    made where columns do not lie together or rows not at multiples of 16 bytes); bias: [vocabulary], float32 or of that type, or None; labels: [...] int32 or
-    int64.  A token whose label is ignore_index, or no number of the vocabulary, has no part in anything, whatever its row holds, and costs nothing:
-    its loss and gradient are zeros.  reduction: "mean" over the tokens that have a label (0 of none), "sum", or "none" (the shape of labels).
+    hidden: [..., columns], weight: [vocabulary, columns] of its type, columns a multiple of 8 (at most 65536; vocabulary at most 2^22, tokens at most 2^24,
+    2^32 numbers of hidden), with any strides (a copy is made where columns do not lie together or rows not at multiples of 16 bytes); bias: [vocabulary],
+    float32 or of that type, or None; labels: [...] int32 or int64. A token whose label is ignore_index, or no number of the vocabulary, has no part in
+    anything, whatever its row holds, and costs nothing: its loss and gradient are zeros. reduction: "mean" over the tokens that have a label (0 of none),
+    "sum", or "none" (the shape of labels).
 
     float32: products of two half-precision terms a number, sums in float32, errors of the size of float32 products'; in the backward a number of hidden or
-    weight is held to 2^-38 of the largest of its array.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half: held to 2^-38 of the largest token's).
-    Memory: of up to 64 tokens the logits are kept for the backward where they are no more bytes than weight.  The backward has a workspace of up to 1 GB for the logits' gradients (with more than some 250000 tokens 4.2 KB a token) and up to 0.75 GB for sums; float32 weights are laid out once more.
+    weight is held to 2^-38 of the largest of its array.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half:
+    held to 2^-38 of the largest token's).
+    Memory: of up to 64 tokens the logits are kept for the backward where they are no more bytes than weight.  The backward has a workspace of up to 1 GB for the
+    logits' gradients (with more than some 250000 tokens 4.2 KB a token) and up to 0.75 GB for sums; float32 weights are laid out once more.
     -> float32.  Gradients: hidden, weight and bias, the same bits on every call; none of theirs, and none in forward mode (an error); captured in graphs as ``cross_attention`` is."""
     host = _host()
     if host:
