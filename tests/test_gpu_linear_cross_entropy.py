@@ -101,11 +101,11 @@ def _check(h, w, b, y, reduction="mean", ignore=-100, g=None):
 
 
 # tokens, vocabulary, columns, share of the tokens that have a label: one of each; sizes below, at and beyond a tile's; tokens that are counted in a launch of their own; many tiles; tokens
-# whose sums are cut; few labelled ones
+# whose sums are cut; few labelled ones; few with kept logits, in pieces of the vocabulary
 SIZES = [(1, 1, 8, 1.0), (1, 300, 64, 1.0), (5, 7, 16, 0.8), (64, 1000, 72, 1.0), (255, 255, 40, 1.0), (256, 256, 64, 1.0), (257, 513, 136, 0.5), (300, 777, 520, 0.3), (33, 5003, 264, 1.0),
          (4200, 600, 64, 0.1), (700, 2100, 776, 0.9), (130, 4096, 1032, 1.0), (40, 70001, 24, 0.9), (64, 300, 1208, 1.0), (64, 300, 1216, 1.0), (20, 300, 2432, 1.0), (32, 40, 2424, 0.9),
          (64, 300, 608, 1.0), (64, 300, 616, 1.0), (32, 40, 1216, 0.9), (20, 9000, 1224, 1.0), (1100, 300, 40, 1.0), (5000, 300, 72, 1.0), (9001, 40, 264, 0.9),
-         (4097, 1100, 24, 0.6), (300, 777, 72, 0.1), (129, 1500, 520, 0.45), (90, 1030, 1400, 0.5)]
+         (4097, 1100, 24, 0.6), (300, 777, 72, 0.1), (129, 1500, 520, 0.45), (90, 1030, 1400, 0.5), (4, 2200000, 8, 1.0)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -304,3 +304,30 @@ def test_the_gradient_is_the_slope():
         slope = (at(1) - at(-1)) / 2
         # losses of size 5 are off by 2^-21 each, 40 of them; the third derivative of a sum of log sums over a way of length 2^-6 is below 40 * 2^-18 * 5
         assert abs(slope - (grad * way).double().sum().item() * step) <= 40 * 5 * 2.0 ** -21 + 40 * 5 * 2.0 ** -18 / 6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V,K", [(40, 300, 256), (300, 700, 64), (5000, 300, 64)])
+def test_replays_with_other_labels(N, V, K, dtype, either_path):
+    """How many tokens have a label is the replay's, not the capture's: none, few, all; each as the eager call has it, with the program's own work between."""
+    if lookupffn_amd._lib.host_module() is None:
+        pytest.skip("without the host library no forward with gradients is captured")
+    h, w, b = (_randn(N, K, dtype=dtype).requires_grad_(), (_randn(V, K, seed=1) / 8).to(dtype).requires_grad_(), _randn(V, seed=2).requires_grad_())
+    full = torch.randint(0, V, (N,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(3))
+    some = [torch.where(torch.rand(N, device=DEV, generator=torch.Generator(device=DEV).manual_seed(4)) < share, full, -100) for share in (1.0, 0.1, 0.0, 0.5, 1.0)]
+
+    def step(y):
+        loss = linear_cross_entropy(h, w, b, y)
+        return loss.detach(), *torch.autograd.grad(loss, (h, w, b))
+
+    want = [step(y) for y in some]
+    y = full.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(y)
+    for labels, expected in zip(some, want):
+        y.copy_(labels)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, expected))
+        torch.randn(1 << 20, device=DEV).sum().item()
