@@ -36,7 +36,7 @@ struct Kept {
     int32_t *head;      // [4]: labelled tokens; the exponents of the largest of their rows and of the weights (two-term numbers)
     int32_t *pos;       // [N]: where a token's row is among the labelled ones, or -1
     int32_t *label;     // [labelled]
-    float2 *level;      // [labelled]: a token's largest logit times log2(e), and one over the sum of the exponentials of what they are below it
+    float2 *level;      // [labelled]: a token's largest logit times log2(e) (level_of), and one over the sum of the exponentials of what they are below it
                         // (the last two up to a whole tile: tiles are read whole)
     float *logits;      // [labelled, up(vocabulary, 32)], or null: of few tokens, where they are no more than the weights
 };
@@ -395,16 +395,23 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b) {
     return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - from) + b.y * __builtin_amdgcn_exp2f(b.x - from));
 }
 
-// Adds 16 logits of a token to its largest and sum so far.  Levels are logits times log2(e): an exponential is one product with a sum, rounded once, and the power of two of that.
+// Levels are logits times log2(e): an exponential is one product with a sum, rounded once, and the power of two of that; what the level's own rounding is off by, all of a token's have, and
+// it falls out.  From 2^30 on it would be more than an exponential's range, and logits are 64 apart or equal: there a level is twice the logit, exactly, and the others' powers are none.
+constexpr float LARGE = 1073741824.f;
+__device__ __forceinline__ float level_of(float logit) { return fabsf(logit) >= LARGE ? logit + logit : logit * LOG2E; }
+// what logits are multiplied with to be compared with a level
+__device__ __forceinline__ float scale_of(float level) { return fabsf(level) >= 2.f * LARGE ? 2.f : LOG2E; }
+
+// Adds 16 logits of a token to its largest and sum so far.
 __device__ __forceinline__ float2 with_logits(float2 of, const float (&l)[16]) {
     float most = l[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) most = fmaxf(most, l[e]);
-    most = fmaxf(of.x, most * LOG2E);
-    const float from = most == -INFINITY ? 0.f : most;
+    most = fmaxf(of.x, level_of(most));
+    const float from = most == -INFINITY ? 0.f : most, scale = scale_of(from);
     float sum = of.y * __builtin_amdgcn_exp2f(of.x - from);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(l[e], LOG2E, -from));
+    for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(l[e], scale, -from));
     return make_float2(most, sum);
 }
 
@@ -716,7 +723,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
 #pragma unroll
         for (int i = 1; i < 16; ++i) of = joined(of, shares[i][in]);
         // (log2(e), rounded alike in both, falls out)
-        const float loss = (fmaf(-a.at_label[n], LOG2E, of.x) + __builtin_amdgcn_logf(of.y)) * (1.f / LOG2E);
+        const float scale = scale_of(of.x), loss = (fmaf(-a.at_label[n], scale, of.x) + __builtin_amdgcn_logf(of.y)) * (scale == LOG2E ? 1.f / LOG2E : 0.5f);
         a.kept.level[n] = make_float2(of.x, 1.f / of.y);
         if (a.loss) a.loss[a.token[n]] = loss;
         sum = loss;
@@ -920,7 +927,7 @@ __device__ __forceinline__ void d_tiles(const BackwardArgs &a, const Piece &p, i
             const bool live = n < labelled;
             // (a token behind the last: exponentials of minus infinity, times zero)
             const float2 level = live ? beside<float2>(beside_, LEVEL, column) : make_float2(INFINITY, 0.f);
-            const float by = LIFT * (a.coefficient ? beside<float>(beside_, COEFFICIENT, column) : 1.f), p_by = live ? level.y * by : 0.f;
+            const float by = LIFT * (a.coefficient ? beside<float>(beside_, COEFFICIENT, column) : 1.f), p_by = live ? level.y * by : 0.f, to_level = scale_of(level.x);
             const int at = live ? beside<int>(beside_, LABEL, column) - p.v0 - in : -1;
             char *const row = a.d + (int64_t(n - lane % 32 + lane % 16) * p.ld + in) * 2 * F::PLANES + 16 * piece_of_lane(lane);       // (of the block's first 16 tokens)
 #pragma unroll
@@ -928,7 +935,7 @@ __device__ __forceinline__ void d_tiles(const BackwardArgs &a, const Piece &p, i
                 float l[16];
                 logits_of<F>(l, sums.v[i][j], beside_, (wm * S::MB + i) * 32, scale);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) l[e] = __builtin_amdgcn_exp2f(fmaf(l[e], LOG2E, -level.x)) * p_by;
+                for (int e = 0; e < 16; ++e) l[e] = __builtin_amdgcn_exp2f(fmaf(l[e], to_level, -level.x)) * p_by;
                 const int r = at - 32 * i;
                 if (r >= 0 && r < 32 && r / 4 % 2 == half) {
 #pragma unroll
@@ -985,7 +992,7 @@ __global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
     float l[8] = {};
     if (n < labelled) {
         const float2 level = a.o.kept.level[n];
-        const float by = LIFT * (a.coefficient ? a.coefficient[n] : 1.f), p_by = level.y * by;
+        const float by = LIFT * (a.coefficient ? a.coefficient[n] : 1.f), p_by = level.y * by, to_level = scale_of(level.x);
         const float *from = a.o.kept.logits + n * logits_stride(V) + p.v0 + in;
         const int at = a.o.kept.label[n] - p.v0 - in;
 #pragma unroll
@@ -995,7 +1002,7 @@ __global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
             const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                l[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(w[e], LOG2E, -level.x)) * p_by - (at == 4 * g + e ? by : 0.f);
+                l[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(w[e], to_level, -level.x)) * p_by - (at == 4 * g + e ? by : 0.f);
                 if (in + 4 * g + e >= p.width) l[4 * g + e] = 0.f;
             }
         }
