@@ -469,7 +469,7 @@ static_assert(NarrowLogits::M * NarrowLogits::TOKENS <= WAVES_M * TILE, "the par
 
 // ---------------------------------------------------------------- few tokens
 
-// Up to 64 tokens whose rows fit LDS: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a
+// Up to 64 tokens whose rows fit LDS, and whose logits are no more bytes than the weights: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a
 // time, whose rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, six such in flight.  Nothing is laid together before: a launch less.
 // fp32 is multiplied as it is (v_mfma_f32_32x32x2_f32): at 32 tokens a product takes as long as its weights' bytes (32 x 50265 x 840 64 us; splitting the weights to memory 71 and the tiles'
 // products 71).  The exponents that the backward's two-term numbers have in common are found on the way.
@@ -479,12 +479,11 @@ constexpr int64_t few_lds(int64_t tokens, int64_t row_bytes) {
     return (tokens <= 32 ? 32 : 64) * int64_t(few_stride(row_bytes)) * 16 + 8 * FEW * 8 + FEW * 4;
 }
 int64_t row_bytes(const lffn_linear_cross_entropy &a) { return a.columns * (a.format == LFFN_ROWS_F32 ? 4 : 2); }
-bool few_tokens(const lffn_linear_cross_entropy &a) { return a.tokens <= FEW && few_lds(a.tokens, row_bytes(a)) <= 160 * 1024; }
-
-// The backward of few tokens takes their logits from the forward where they are no more bytes than the weights, which it would read for them once more (both directions,
-// 19 tokens, 50265 x 768 fp32: 291 us with them formed again, 246 with these).
+// The backward of few tokens takes their logits from the forward, which are no more bytes than the weights, that it would read for them once more (both directions, 19 tokens, 50265 x 768 fp32:
+// 291 us with them formed again, 246 with these).  Formed again they would be sums in another order, and a softmax has to see both directions' logits alike; so tokens that are more than a
+// row's columns in floats take the tiles, as many tokens do, in both.
 constexpr int64_t logits_stride(int64_t vocabulary) { return up(vocabulary, 32); }
-bool keeps_logits(const lffn_linear_cross_entropy &a) { return few_tokens(a) && a.tokens * 4 <= row_bytes(a); }
+bool few_tokens(const lffn_linear_cross_entropy &a) { return a.tokens <= FEW && a.tokens * 4 <= row_bytes(a) && few_lds(a.tokens, row_bytes(a)) <= 160 * 1024; }
 int64_t kept_bytes(const lffn_linear_cross_entropy &a, bool logits) {
     return 16 + up(a.tokens * 4, 16) + up(a.tokens, TILE) * 12 + (logits ? a.tokens * logits_stride(a.vocabulary) * 4 : 0);
 }
@@ -492,7 +491,7 @@ Kept kept_at(const lffn_linear_cross_entropy &a, void *at) {
     char *p = static_cast<char *>(at);
     const int64_t n = up(a.tokens * 4, 16), tiles = up(a.tokens, TILE);
     return {reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + 16), reinterpret_cast<int32_t *>(p + 16 + n), reinterpret_cast<float2 *>(p + 16 + n + tiles * 4),
-            keeps_logits(a) ? reinterpret_cast<float *>(p + 16 + n + tiles * 12) : nullptr};
+            few_tokens(a) ? reinterpret_cast<float *>(p + 16 + n + tiles * 12) : nullptr};
 }
 
 int few_workgroups(const lffn_linear_cross_entropy &a) { return (int)min((a.vocabulary + 31) / 32, int64_t(COMPUTE_UNITS)); }
@@ -1474,7 +1473,7 @@ int backward(const BackwardArgs &b, hipStream_t st) {
 extern "C" int lffn_linear_cross_entropy_kept_bytes(const lffn_linear_cross_entropy *a, int64_t *bytes) {
     LFFN_REQUIRE(bytes, LFFN_ERR_BAD_ARG);
     const int rc = check(a);
-    if (rc == LFFN_OK) *bytes = kept_bytes(*a, keeps_logits(*a));
+    if (rc == LFFN_OK) *bytes = kept_bytes(*a, few_tokens(*a));
     return rc;
 }
 

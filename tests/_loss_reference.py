@@ -48,7 +48,8 @@ def reference(h, w, b, y, c, logits_kept=False, chunk=2048):
         of_loss[at] = (worst + of.gather(1, t) + (span + (lse - logits.gather(1, t)).abs()) * 4 * E + 2.0 ** -20)[:, 0]
         moved = torch.expm1(2 * torch.where(near, of_both, 0.0).amax(1, keepdim=True) + span * 4 * E + 2.0 ** -20)
         of_p = torch.where(near.sum(1, keepdim=True) == 1, torch.full_like(moved, 2.0 ** -17), moved)
-        d, of_d = p.clone(), p * of_p
+        # (an entry's share is between 0 and 1, whatever the errors)
+        d, of_d = p.clone(), torch.where(near, (p * of_p).nan_to_num(1.0).clamp(max=1.0), 0.0)
         d.scatter_add_(1, t, torch.full_like(t, -1, dtype=torch.float64))
         of_d.scatter_add_(1, t, torch.full_like(t, 1, dtype=torch.float64) * E)
         d, of_d = d * k, of_d * k.abs()

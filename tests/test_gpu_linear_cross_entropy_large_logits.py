@@ -71,3 +71,15 @@ def test_logits_on_both_sides_of_a_level_s_units(dtype):
         y = _labels(70, V)
         want, bounds = reference(hd, wd, None, y, torch.ones(70, device=DEV))
         assert worst(linear_cross_entropy(hd, wd, None, y, reduction="none"), want[0], bounds[0]) <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("N,V,K", [*SIZES, (60, 300, 96), (64, 2000, 120)])
+def test_gradients(N, V, K, dtype):
+    """Both directions see a token's one entry at the same height, whichever kernels form their logits."""
+    h, w, y = (1e4 * _randn(N, K)).to(dtype), (1e4 * _randn(V, K, seed=1)).to(dtype), _labels(N, V)
+    g = torch.full((N,), 2.0 ** -6, device=DEV)
+    leaves = h.requires_grad_(), w.requires_grad_()
+    grads = torch.autograd.grad(linear_cross_entropy(h, w, None, y, reduction="none"), leaves, g)
+    want, bounds = reference(h, w, None, y, g)
+    assert max(worst(got, want[i], bounds[i]) for i, got in enumerate(grads, 1)) <= 1
