@@ -11,6 +11,9 @@
 // Backward: the logits of a piece of the vocabulary are formed once more, d is written in 16 bits (a float's in two terms), and one launch forms from it both gradients' products:
 // dW, its sum over the tokens whole or, where its tiles are few and the tokens many, in shares of them, and dh in shares of the vocabulary, added up in fp32 in memory.  What a
 // share adds to is its own: no atomics on results, the same bits on every call.
+//
+// fp32 in the backward: a sum's numbers have one power of two in common, so rows are laid by the largest of their array, and a row that is far below that would have few bits left.  Where rows,
+// or logits, are too far apart (far_apart) the rows are laid one by one, as in the forward, d stays a float, and both products are of the floats themselves (far_hidden, far_weight).
 #include "product_tiles.h"
 
 namespace {
@@ -33,7 +36,7 @@ __host__ __device__ constexpr int64_t up(int64_t v, int64_t to) { return (v + to
 
 // What the backward needs beside the inputs, and what the forward's launches share.
 struct Kept {
-    int32_t *head;      // [4]: labelled tokens; the exponents of the largest of their rows and of the weights (two-term numbers)
+    int32_t *head;      // [8]: labelled tokens; of two-term numbers the exponents of the largest of their rows and of the weights, and of the least ones (rows of zeros aside)
     int32_t *pos;       // [N]: where a token's row is among the labelled ones, or -1
     int32_t *label;     // [labelled]
     float2 *level;      // [labelled]: a token's largest logit times log2(e) (level_of), and one over the sum of the exponentials of what they are below it
@@ -56,6 +59,15 @@ struct Operands {
     float *row_scale;
 };
 
+// Whether two-term numbers cannot be laid by the largest of their arrays in the backward.  Rows whose largest is 2^-16 of the array's have 22 bits of it left, what a second term has at the
+// least.  And the logits that are formed of them must be those whose levels the forward left: laid either way they are off from each other by 2^-38 of the largest number of a row, of an
+// entry and the columns, which has to be no more than 2^-18.  (A row's largest is less than 2^14 times the power of two that it was divided by; kept logits are not formed again.)
+constexpr int ROWS_APART = 16, LOGITS_LARGEST = 20;
+__device__ __forceinline__ bool far_apart(const Operands &o) {
+    const int32_t *h = o.kept.head;
+    return max(h[1] - min(h[1], h[3]), h[2] - min(h[2], h[4])) > ROWS_APART || (!o.kept.logits && h[1] + h[2] + 28 + (32 - __clz(o.s.K - 1)) > LOGITS_LARGEST);
+}
+
 template <int PLANES>
 __device__ __forceinline__ Source rows_of(const Operands &o, int labelled) {
     return {o.rows, o.s.Kp * 2 * PLANES, (int)up(labelled, TILE), (int)o.s.Kp};
@@ -70,7 +82,7 @@ struct RowsArgs {
     int32_t labels_64, bias_format;            // of the gather's row formats; -1: none
     const int32_t *counts, *groups;            // labelled tokens of every chunk and of every COUNTED, or null
     int parts;                                 // workgroups that lay a chunk's rows
-    int32_t *token;                            // [labelled]
+    int32_t *token;                            // [labelled], or null
     float *loss;                               // [N]: zeros for the others, or null
     const float *g_loss;                       // [N]
     float *most;                               // the backward of losses by token: of a chunk's finite g_loss
@@ -109,20 +121,18 @@ __device__ __forceinline__ float wave_most(float v) {
 __device__ __forceinline__ float wave_least(float v) { return -wave_most(-v); }
 
 // A row of `columns` numbers as the products read it, zeros up to `padded`, by one wavefront.  Two-term numbers: scaled by the row's largest, or to `exponent` where that is
-// given; -> the exponent of the way back.
+// given; -> the power of two of the way back, 0 of a row of zeros (no sum of it is anything else) and of an infinite one (which is lost).
 template <typename R, int PLANES>
-__device__ __forceinline__ int lay_row(const char *from, char *to, int columns, int64_t padded, const int *exponent) {
+__device__ __forceinline__ float lay_row(const char *from, char *to, int columns, int64_t padded, const int *exponent) {
     const int lane = threadIdx.x % 64;
     if constexpr (PLANES == 1) {
         for (int c = lane * 8; c < padded; c += 512)
             *reinterpret_cast<uint4 *>(to + c * 2) = c < columns ? *reinterpret_cast<const uint4 *>(from + c * 2) : make_uint4(0, 0, 0, 0);
-        return 0;
+        return 1.f;
     } else {
-        int e;
-        float scale;
+        float scale, back;
         if (exponent) {
-            e = *exponent;
-            scale = __builtin_amdgcn_ldexpf(1.f, -e);
+            scale = __builtin_amdgcn_ldexpf(1.f, -*exponent), back = __builtin_amdgcn_ldexpf(1.f, *exponent);
         } else {
             float most = 0.f;
             for (int c = lane * 4; c < columns; c += 256) {
@@ -130,7 +140,9 @@ __device__ __forceinline__ int lay_row(const char *from, char *to, int columns, 
                 most = fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
             }
             most = wave_most(most);
-            scale = scale_to(most == INFINITY ? 0.f : most, 13, e);        // (an infinite row is lost; the backward's exponent is the others')
+            int e;
+            scale = scale_to(most == INFINITY ? 0.f : most, 13, e);        // (the backward's exponents are the others')
+            back = most == INFINITY || most == 0.f ? 0.f : __builtin_amdgcn_ldexpf(1.f, e);
         }
         for (int c = lane * 8; c < padded; c += 512) {
             uint32_t h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
@@ -146,7 +158,7 @@ __device__ __forceinline__ int lay_row(const char *from, char *to, int columns, 
             *reinterpret_cast<uint4 *>(to + byte_of<2>(c)) = make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4 *>(to + byte_of<2>(c) + 64) = make_uint4(l[0], l[1], l[2], l[3]);
         }
-        return e;
+        return back;
     }
 }
 
@@ -156,21 +168,24 @@ __device__ __forceinline__ float bias_of(const void *bias, int format, int v) {
     return (float)static_cast<const _Float16 *>(bias)[v];
 }
 
-// The exponent of the largest of n powers of two, to *most, by a workgroup that others may be beside: one atomic for it.
-__device__ __forceinline__ void raise(int32_t *most, const float *scales, int first, int n, int step, float *red) {
-    float v = 0.f;
-    for (int i = first; i < n; i += step) v = fmaxf(v, scales[i]);
-    v = wave_most(v);
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
+// The exponents of the largest and the least of n powers of two, zeros aside, to *most and *least, by a workgroup that others may be beside: an atomic for each.  red: 32 numbers.
+__device__ __forceinline__ void find_exponents(int32_t *most, int32_t *least, const float *scales, int first, int n, int step, float *red) {
+    float high = 0.f, low = INFINITY;
+    for (int i = first; i < n; i += step) {
+        const float v = scales[i];
+        high = fmaxf(high, v), low = v > 0.f ? fminf(low, v) : low;
+    }
+    high = wave_most(high), low = wave_least(low);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = high, red[16 + threadIdx.x / 64] = low;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (unsigned i = 1; i < blockDim.x / 64; ++i) v = fmaxf(v, red[i]);
-        if (v > 0.f) atomicMax(most, ilogbf(v));
+        for (unsigned i = 1; i < blockDim.x / 64; ++i) high = fmaxf(high, red[i]), low = fminf(low, red[16 + i]);
+        if (high > 0.f) atomicMax(most, ilogbf(high)), atomicMin(least, ilogbf(low));
     }
 }
 
-// (exponents lower than any: the launch that joins raises them)
-__device__ __forceinline__ void begin_head(const Kept &k, int labelled) { k.head[0] = labelled, k.head[1] = k.head[2] = -1000; }
+// (as low an exponent as any, and a higher one than any: the launch that joins raises and lowers them)
+__device__ __forceinline__ void begin_head(const Kept &k, int labelled) { k.head[0] = labelled, k.head[1] = k.head[2] = -116, k.head[3] = k.head[4] = 1000; }
 
 // Workgroups parts (tokens / CHUNK): the labelled tokens of a chunk take their places (in the forward; the backward reads where they are) and their rows are laid there; the last
 // one fills the last tile's rows up with zeros.  The workgroups behind: the bias in fp32.
@@ -218,6 +233,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
         if (wave == 0) {
             const int at = t0 + lane < s.N ? k.pos[t0 + lane] : -1;
             place[lane] = at;
+            if (a.token && part == 0 && at >= 0) a.token[at] = t0 + lane;
             if (a.most && part == 0) {
                 const float g = at >= 0 ? fabsf(a.g_loss[t0 + lane]) : 0.f, most = wave_most(g < INFINITY ? g : 0.f);
                 if (lane == 0) a.most[chunk] = most;
@@ -226,34 +242,32 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     }
     __syncthreads();
     const int64_t row_bytes = s.Kp * 2 * PLANES;
+    const int *const exponent = PLANES == 2 && BACKWARD && !far_apart(a.o) ? k.head + 1 : nullptr;
     for (int i = part * 4 + wave; i < CHUNK; i += 4 * a.parts) {
         const int at = place[i];
         if (at < 0) continue;
         const char *from = static_cast<const char *>(a.hidden) + (int64_t(t0) + i) * a.hidden_stride * R::BYTES;
-        const int e = lay_row<R, PLANES>(from, a.o.rows + at * row_bytes, s.K, s.Kp, BACKWARD ? k.head + 1 : nullptr);
-        if (PLANES == 2 && !BACKWARD && lane == 0) a.o.row_scale[at] = __builtin_amdgcn_ldexpf(1.f, e);
+        const float back = lay_row<R, PLANES>(from, a.o.rows + at * row_bytes, s.K, s.Kp, exponent);
+        if (PLANES == 2 && lane == 0) a.o.row_scale[at] = back;
     }
     if (chunk == chunks - 1) {
         const int64_t from = labelled * row_bytes / 16, to = up(labelled, TILE) * row_bytes / 16;
         for (int64_t i = from + part * 256 + tid; i < to; i += 256 * a.parts) *reinterpret_cast<uint4 *>(a.o.rows + i * 16) = make_uint4(0, 0, 0, 0);
-        if (PLANES == 2 && !BACKWARD)
+        if (PLANES == 2)
             for (int i = labelled + tid; i < up(labelled, TILE); i += 256) a.o.row_scale[i] = 1.f;
     }
 }
 
-// fp32 weights in two half-precision terms: each row by its largest, or, in the backward, all by the array's.
+// fp32 weights in two half-precision terms: each row by its largest, or, in the backward, all by the array's (far_apart).
 template <bool BACKWARD>
 __global__ __launch_bounds__(256) void weight_kernel(Operands o, const float *w, int64_t stride) {
     const int v = blockIdx.x * 4 + threadIdx.x / 64;
     if (v >= o.s.Vp) return;
-    int e = 0;
+    float back = 0.f;              // (of entries behind the vocabulary, and nothing to the largest and the least)
     if (v < o.s.V)
-        e = lay_row<F32Row, 2>(reinterpret_cast<const char *>(w + v * stride), const_cast<char *>(o.weight.at) + v * o.weight.stride, o.s.K, o.weight.columns,
-                               BACKWARD ? o.kept.head + 2 : nullptr);
-    if (threadIdx.x % 64 == 0) {
-        // (entries behind the vocabulary: no larger than any)
-        o.weight_scale[v] = v < o.s.V ? __builtin_amdgcn_ldexpf(1.f, e) : BACKWARD ? 1.f : 0.f;
-    }
+        back = lay_row<F32Row, 2>(reinterpret_cast<const char *>(w + v * stride), const_cast<char *>(o.weight.at) + v * o.weight.stride, o.s.K, o.weight.columns,
+                                  BACKWARD && !far_apart(o) ? o.kept.head + 2 : nullptr);
+    if (threadIdx.x % 64 == 0) o.weight_scale[v] = back;
 }
 
 // ---------------------------------------------------------------- logits
@@ -306,7 +320,7 @@ __device__ __forceinline__ void bring_beside(const Operands &o, const float *coe
     if (wave == BIAS) from = o.bias + v0;
     else if (wave == LABEL) from = o.kept.label + n0;
     else if (wave == WEIGHT_SCALE && o.weight_scale) from = o.weight_scale + v0;
-    else if (wave == ROW_SCALE && !BACKWARD && o.row_scale) from = o.row_scale + n0;
+    else if (wave == ROW_SCALE && o.row_scale) from = o.row_scale + n0;
     else if (BACKWARD && wave >= LEVEL && wave < LEVEL_END) from = o.kept.level + n0 + (wave - LEVEL) * 128;
     else if (BACKWARD && wave == COEFFICIENT && coefficient) from = coefficient + n0;
     if (from) copy_to_lds((const char *)uniform((uint64_t)from), threadIdx.x % 64 * 16, lds + wave * 1024);
@@ -484,14 +498,17 @@ int64_t row_bytes(const lffn_linear_cross_entropy &a) { return a.columns * (a.fo
 // row's columns in floats take the tiles, as many tokens do, in both.
 constexpr int64_t logits_stride(int64_t vocabulary) { return up(vocabulary, 32); }
 bool few_tokens(const lffn_linear_cross_entropy &a) { return a.tokens <= FEW && a.tokens * 4 <= row_bytes(a) && few_lds(a.tokens, row_bytes(a)) <= 160 * 1024; }
+constexpr int64_t HEAD_BYTES = 32;
 int64_t kept_bytes(const lffn_linear_cross_entropy &a, bool logits) {
-    return 16 + up(a.tokens * 4, 16) + up(a.tokens, TILE) * 12 + (logits ? a.tokens * logits_stride(a.vocabulary) * 4 : 0);
+    return HEAD_BYTES + up(a.tokens * 4, 16) + up(a.tokens, TILE) * 12 + (logits ? a.tokens * logits_stride(a.vocabulary) * 4 : 0);
 }
 Kept kept_at(const lffn_linear_cross_entropy &a, void *at) {
     char *p = static_cast<char *>(at);
     const int64_t n = up(a.tokens * 4, 16), tiles = up(a.tokens, TILE);
-    return {reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + 16), reinterpret_cast<int32_t *>(p + 16 + n), reinterpret_cast<float2 *>(p + 16 + n + tiles * 4),
-            few_tokens(a) ? reinterpret_cast<float *>(p + 16 + n + tiles * 12) : nullptr};
+    int32_t *const head = reinterpret_cast<int32_t *>(p);
+    p += HEAD_BYTES;
+    return {head, reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p + n), reinterpret_cast<float2 *>(p + n + tiles * 4),
+            few_tokens(a) ? reinterpret_cast<float *>(p + n + tiles * 12) : nullptr};
 }
 
 int few_workgroups(const lffn_linear_cross_entropy &a) { return (int)min((a.vocabulary + 31) / 32, int64_t(COMPUTE_UNITS)); }
@@ -524,17 +541,24 @@ __device__ __forceinline__ float most_of(const uint4 &u, float most) {
     const float4 v = __builtin_bit_cast(float4, u);
     return fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 }
-// The power of two that two-term numbers of a workgroup's largest magnitude are divided by, to *scale.
-__device__ __forceinline__ void put_scale(float *scale, float most, float *red) {
-    most = wave_most(most);
+// The largest and the least of rows' largest magnitudes, zeros and infinite ones aside.
+struct Range {
+    float most = 0.f, least = INFINITY;
+    __device__ __forceinline__ void add(float of_row) {
+        if (of_row > 0.f && of_row < INFINITY) most = fmaxf(most, of_row), least = fminf(least, of_row);
+    }
+};
+// The powers of two that two-term numbers of a workgroup's are divided by, to scales[0] and [1], zeros of none.
+__device__ __forceinline__ void put_scales(float *scales, Range r, float *red) {
+    r.most = wave_most(r.most), r.least = wave_least(r.least);
     __syncthreads();
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = most;
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = r.most, red[16 + threadIdx.x / 64] = r.least;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (unsigned i = 1; i < blockDim.x / 64; ++i) most = fmaxf(most, red[i]);
+    if (threadIdx.x < 2) {
+        for (unsigned i = 0; i < blockDim.x / 64; ++i) r.most = fmaxf(r.most, red[i]), r.least = fminf(r.least, red[16 + i]);
         int e;
-        scale_to(most, 13, e);
-        *scale = __builtin_amdgcn_ldexpf(1.f, e);
+        scale_to(threadIdx.x == 0 ? r.most : r.least, 13, e);
+        scales[threadIdx.x] = r.most > 0.f ? __builtin_amdgcn_ldexpf(1.f, e) : 0.f;
     }
 }
 
@@ -567,7 +591,8 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
     const int blocks = (V + 31) / 32, all = gridDim.x * WAVES;
     int block = wave * gridDim.x + blockIdx.x;
     uint4 w[AHEAD][4];
-    float most = 0.f, most_x = 0.f;                // of the weights, of the rows
+    Range of_weights, of_rows;
+    float most = 0.f;                              // of the lane's numbers of an entry
     const char *row = nullptr;
     auto begin_block = [&] { row = o.weight.at + int64_t(min(block * 32 + lane % 32, V - 1)) * o.weight.stride; };
     auto load = [&](int s, uint4 (&to)[4]) {
@@ -594,10 +619,6 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
         for (int k = 0; k < BATCH; ++k) {
             const int i = i0 + k * THREADS, r = i / pieces, p = i - r * pieces;
             if (r < TOKENS) lds_words[r * stride + p] = v[k];
-            if constexpr (WHOLE) {
-                const float of_piece = most_of(v[k], 0.f);
-                most_x = fmaxf(most_x, of_piece == INFINITY ? 0.f : of_piece);       // (an infinite row is lost; the backward's exponent is the others')
-            }
         }
     }
     __syncthreads();
@@ -639,6 +660,10 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
             }
         }
         const int v0 = block * 32;
+        if constexpr (WHOLE) {
+            of_weights.add(fmaxf(most, __shfl_xor(most, 32)));
+            most = 0.f;
+        }
         if (block + all < blocks) {                 // the next block's first steps
             block += all;
             begin_block();
@@ -679,8 +704,16 @@ __global__ __launch_bounds__(THREADS, 2) void few_kernel(FewArgs a) {
         a.parts[blockIdx.x * a.Np + tid] = sum;
     }
     if constexpr (WHOLE) {
-        put_scale(o.weight_scale + blockIdx.x, most, reinterpret_cast<float *>(waves));
-        if (blockIdx.x == 0) put_scale(o.row_scale, most_x, reinterpret_cast<float *>(waves));
+        put_scales(o.weight_scale + 2 * blockIdx.x, of_weights, reinterpret_cast<float *>(waves));
+        // (the last workgroup has no more blocks than any)
+        if (blockIdx.x == gridDim.x - 1) {
+            for (int r = wave; r < labelled; r += WAVES) {
+                float of_row = 0.f;
+                for (int p = lane; p < pieces; p += 64) of_row = most_of(lds_words[r * stride + p], of_row);
+                of_rows.add(wave_most(of_row));
+            }
+            put_scales(o.row_scale, of_rows, reinterpret_cast<float *>(waves));
+        }
     }
 }
 
@@ -693,8 +726,8 @@ struct JoinArgs {
     int tiles;
     float *loss;           // by token
     double *sums;          // of a workgroup's
-    const float *weight_scale, *row_scale;       // two-term numbers: of `entries`, and of the labelled tokens or, of few, of all
-    int entries, few, joining;                   // the last: workgroups that join; those behind look for the largest of the scales
+    const float *weight_scale, *row_scale;       // two-term numbers: of `entries`, and of the labelled tokens; of few, every workgroup's largest and least and all tokens'
+    int entries, few, joining;                   // the last: workgroups that join; those behind look for the largest and the least of the scales
 };
 
 constexpr int LOOKING = 16;
@@ -706,8 +739,9 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     if ((int)blockIdx.x >= a.joining) {
         const int i = blockIdx.x - a.joining;
         if (labelled == 0) return;                   // (no numbers are multiplied)
-        if (i < LOOKING) raise(a.kept.head + 2, a.weight_scale, i * 256 + threadIdx.x, a.entries, LOOKING * 256, &shares[0][0].x);
-        else raise(a.kept.head + 1, a.row_scale, (i - LOOKING) * 256 + threadIdx.x, a.few ? 1 : labelled, LOOKING * 256, &shares[0][0].x);
+        int32_t *const head = a.kept.head;
+        if (i < LOOKING) find_exponents(head + 2, head + 4, a.weight_scale, i * 256 + threadIdx.x, a.entries, LOOKING * 256, &shares[0][0].x);
+        else find_exponents(head + 1, head + 3, a.row_scale, (i - LOOKING) * 256 + threadIdx.x, a.few ? 2 : labelled, LOOKING * 256, &shares[0][0].x);
         return;
     }
     if ((int)blockIdx.x * 16 >= labelled) return;
@@ -764,6 +798,9 @@ struct BackwardArgs {
     float *weight_parts;       // [shares, vocabulary, K] and [shares, vocabulary] of the bias, where dW's sums may be cut
     float *bias_parts;
     int32_t *shares;           // [3]: of the vocabulary, for dh; pieces that there are; of the tokens, for dW (all from the first piece's launch)
+    const float *hidden, *whole_weight;        // numbers that are far apart: the arrays as they were given, the labelled tokens
+    int64_t hidden_stride, weight_stride;
+    const int32_t *token;
     void *grad_hidden, *grad_weight, *grad_bias;
     int32_t bias_format, reduction, pieces, weight_shares;         // the last: at most
 };
@@ -916,7 +953,7 @@ template <typename F, typename S>
 __device__ __forceinline__ void d_tiles(const BackwardArgs &a, const Piece &p, int labelled, uint32_t lds) {
     const Operands &o = a.o;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, half = lane / 32, wm = wave / S::N, wn = wave % S::N;
-    const float scale = F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, o.kept.head[1]) : 1.f;
+    const bool far = F::PLANES == 2 && far_apart(o);
     for_logits<F, S, true>(o, a.coefficient, labelled, p.v0, p.width, lds, [&](const Sums<S::MB, S::NB> &sums, const Place &tile, uint32_t beside_) {
         const int in = tile.v + wm * S::MB * 32;
         bool stored = false;
@@ -928,11 +965,12 @@ __device__ __forceinline__ void d_tiles(const BackwardArgs &a, const Piece &p, i
             const float2 level = live ? beside<float2>(beside_, LEVEL, column) : make_float2(INFINITY, 0.f);
             const float by = LIFT * (a.coefficient ? beside<float>(beside_, COEFFICIENT, column) : 1.f), p_by = live ? level.y * by : 0.f, to_level = scale_of(level.x);
             const int at = live ? beside<int>(beside_, LABEL, column) - p.v0 - in : -1;
+            const float row_scale = F::PLANES == 2 ? beside<float>(beside_, ROW_SCALE, column) : 1.f;
             char *const row = a.d + (int64_t(n - lane % 32 + lane % 16) * p.ld + in) * 2 * F::PLANES + 16 * piece_of_lane(lane);       // (of the block's first 16 tokens)
 #pragma unroll
             for (int i = 0; i < S::MB; ++i) {
                 float l[16];
-                logits_of<F>(l, sums.v[i][j], beside_, (wm * S::MB + i) * 32, scale);
+                logits_of<F>(l, sums.v[i][j], beside_, (wm * S::MB + i) * 32, row_scale);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) l[e] = __builtin_amdgcn_exp2f(fmaf(l[e], to_level, -level.x)) * p_by;
                 const int r = at - 32 * i;
@@ -943,6 +981,12 @@ __device__ __forceinline__ void d_tiles(const BackwardArgs &a, const Piece &p, i
                 if (!stored) {
                     arrived();
                     stored = true;
+                }
+                if (far) {
+                    float *const to = reinterpret_cast<float *>(a.d) + int64_t(n) * p.ld + in + 32 * i + 4 * half;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) *reinterpret_cast<float4 *>(to + 8 * g) = make_float4(l[4 * g], l[4 * g + 1], l[4 * g + 2], l[4 * g + 3]);
+                    continue;
                 }
                 auto put = [&](char *to) {
                     uint4 w[2];
@@ -980,6 +1024,16 @@ __global__ __launch_bounds__(THREADS, 2) void d_kernel(BackwardArgs a, int piece
     }
 }
 
+// Eight numbers in the results' format.
+template <typename R>
+__device__ __forceinline__ void store8(char *to, const float (&v)[8]) {
+    if constexpr (R::BYTES == 4) {
+        *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4 *>(to + 16) = make_float4(v[4], v[5], v[6], v[7]);
+    } else
+        *reinterpret_cast<uint4 *>(to) = R::pack(v);
+}
+
 // d of few tokens from their logits: eight entries of a token a thread, zeros for the tokens behind (as far as dW's sums go; what dh's tile reads behind those is not stored).
 template <typename F>
 __global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
@@ -1005,6 +1059,10 @@ __global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
                 if (in + 4 * g + e >= p.width) l[4 * g + e] = 0.f;
             }
         }
+    }
+    if (F::PLANES == 2 && far_apart(a.o)) {
+        store8<F32Row>(a.d + (int64_t(n) * p.ld + in) * 4, l);
+        return;
     }
     char *const to = a.d + int64_t(n) * p.ld * 2 * F::PLANES + byte_of<F::PLANES>(in);
     auto put = [&](char *at) {
@@ -1033,16 +1091,6 @@ __device__ __forceinline__ float dot_ones(F16, uint4 u, float sum) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(pair_t, w[i]), one, sum, false);
     return sum;
-}
-
-// Eight numbers in the results' format.
-template <typename R>
-__device__ __forceinline__ void store8(char *to, const float (&v)[8]) {
-    if constexpr (R::BYTES == 4) {
-        *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4 *>(to + 16) = make_float4(v[4], v[5], v[6], v[7]);
-    } else
-        *reinterpret_cast<uint4 *>(to) = R::pack(v);
 }
 
 // dh: shares of the piece's entries x tiles of tokens x tiles of columns, one after the other; each adds to its own part.
@@ -1204,6 +1252,135 @@ __device__ __forceinline__ void weight_tasks(const BackwardArgs &a, const Piece 
     stream.done();
 }
 
+// ---------------------------------------------------------------- numbers that are far apart
+
+// Products of floats as they are (v_mfma_f32_32x32x2_f32), 64 x 64 results a wavefront, operands from memory straight to its registers: 16 products, 1024 clocks, to 16 loads.  An instruction's two
+// summed indices are four apart, so that four in a row are 16 bytes of d.  (Both directions with one token of 10^9 and without: 4096 x 50265 x 768 12.5 ms and 3.2, 385 x 32003 x 520 687 us and
+// 300, 32768 x 1000 x 64 603 and 188.)  load(k, a, b): index k + 4 (lane / 32) + q of 32 i + lane % 32, zeros of b or a behind the last; of a share at least one.
+template <typename Load, typename Seen>
+__device__ __forceinline__ void far_products(f32x16_t (&sums)[2][2], int first, int end, Load &&load, Seen &&seen) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sums[i][j][e] = 0.f;
+    float a[2][2][4], b[2][2][4];
+    auto form = [&](int at) {
+        seen(b[at]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) sums[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[at][i][q], b[at][j][q], sums[i][j], 0, 0, 0);
+    };
+    load(first, a[0], b[0]);
+    for (int k = first; k < end; k += 16) {
+        load(k + 8, a[1], b[1]);
+        form(0);
+        load(k + 16, a[0], b[0]);
+        form(1);
+    }
+}
+
+constexpr int FAR = 64, FAR_WAVES = COMPUTE_UNITS * THREADS / 64;
+
+// dh in the shares of hidden_tasks.
+template <typename F>
+__device__ __forceinline__ void far_hidden(const BackwardArgs &a, const Piece &p, int labelled, int piece, int unit) {
+    constexpr int STEPS_OF = STEP / F::PLANES;
+    const Sizes &s = a.o.s;
+    const int lane = threadIdx.x % 64, half = lane / 32, nt = (labelled + FAR - 1) / FAR, ht = (s.K + FAR - 1) / FAR;
+    const int wanted = *a.shares, length = (p.steps + 2 * wanted - 1) / (2 * wanted) * 2, steps = (p.width + STEPS_OF - 1) / STEPS_OF, tasks = (steps + length - 1) / length * nt * ht;
+    const float *const d = reinterpret_cast<const float *>(a.d);
+    for (int id = unit * (THREADS / 64) + threadIdx.x / 64; id < tasks; id += FAR_WAVES) {
+        const int share = id / ht / nt, n0 = id / ht % nt * FAR, h0 = id % ht * FAR, first = share * length * STEPS_OF, end = min(p.width, first + length * STEPS_OF);
+        f32x16_t sums[2][2];
+        far_products(sums, first, end, [&](int k, float (&x)[2][4], float (&w)[2][4]) {
+            const int v = k + 4 * half;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                // (behind the piece's last entry d has zeros up to a whole tile)
+                float4 of = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (v < end) of = *reinterpret_cast<const float4 *>(d + int64_t(min(n0 + 32 * i + lane % 32, labelled - 1)) * p.ld + v);
+                x[i][0] = of.x, x[i][1] = of.y, x[i][2] = of.z, x[i][3] = of.w;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float *const row = a.whole_weight + (p.v0 + min(v + q, p.width - 1)) * a.weight_stride;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) w[j][q] = row[min(h0 + 32 * j + lane % 32, s.K - 1)];
+            }
+        }, [](const float (&)[2][4]) {});
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int h = h0 + 32 * j + lane % 32;
+            if (h >= s.K) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int row = n0 + 32 * i + mfma_row(e, half);
+                    float *const at = a.parts + (int64_t(share) * labelled + row) * s.K + h;
+                    if (row < labelled) *at = piece == 0 ? sums[i][j][e] : *at + sums[i][j][e];
+                }
+        }
+    }
+}
+
+// dW in the shares of weight_tasks, and, with the first columns, db.
+template <typename F>
+__device__ __forceinline__ void far_weight(const BackwardArgs &a, const Piece &p, int labelled, int unit) {
+    constexpr int STEPS_OF = STEP / F::PLANES;
+    const Sizes &s = a.o.s;
+    const int lane = threadIdx.x % 64, half = lane / 32, vt = (p.width + FAR - 1) / FAR, ht = (s.K + FAR - 1) / FAR;
+    const TokenShares shares = TokenShares::of<F>(labelled, a.shares[2]);
+    const bool whole = shares.shares == 1;
+    const float factor = factor_of(a, labelled);
+    const float *const d = reinterpret_cast<const float *>(a.d);
+    for (int id = unit * (THREADS / 64) + threadIdx.x / 64; id < shares.shares * vt * ht; id += FAR_WAVES) {
+        const int share = id / ht / vt, v0 = id / ht % vt * FAR, h0 = id % ht * FAR, first = share * shares.length * STEPS_OF, end = min(labelled, first + shares.length * STEPS_OF);
+        const bool of_bias = h0 == 0 && a.grad_bias;
+        float bias[2] = {};
+        f32x16_t sums[2][2];
+        far_products(sums, first, end, [&](int k, float (&x)[2][4], float (&w)[2][4]) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = k + 4 * half + q, in = min(n, end - 1);
+                const float *const row = a.hidden + a.token[in] * a.hidden_stride, *const of = d + int64_t(in) * p.ld + v0 + lane % 32;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) x[i][q] = row[min(h0 + 32 * i + lane % 32, s.K - 1)];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) w[j][q] = n < end ? of[32 * j] : 0.f;
+            }
+        }, [&](const float (&w)[2][4]) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) bias[j] += (w[j][0] + w[j][1]) + (w[j][2] + w[j][3]);
+        });
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int in = v0 + 32 * j + lane % 32, v = p.v0 + in;
+            const float sum = (bias[j] + __shfl_xor(bias[j], 32)) * factor;
+            if (in >= p.width) continue;
+            if (of_bias && half == 0) {
+                if (!whole) a.bias_parts[int64_t(share) * s.V + v] = sum;
+                else put_bias(a, v, sum);
+            }
+            float *const row = whole ? static_cast<float *>(a.grad_weight) + int64_t(v) * s.K : a.weight_parts + (int64_t(share) * s.V + v) * s.K;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int h = h0 + 32 * i + 8 * g + 4 * half;
+                    if (h < s.K)
+                        *reinterpret_cast<float4 *>(row + h) =
+                            make_float4(sums[i][j][4 * g] * factor, sums[i][j][4 * g + 1] * factor, sums[i][j][4 * g + 2] * factor, sums[i][j][4 * g + 3] * factor);
+                }
+        }
+    }
+}
+
 // Both gradients of a piece.
 template <typename F, typename R>
 __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, int piece) {
@@ -1215,6 +1392,13 @@ __global__ __launch_bounds__(THREADS, 2) void gradients_kernel(BackwardArgs a, i
     if (p.width <= 0) return;
     // (COMPUTE_UNITS workgroups; the units of an XCD have neighbouring numbers)
     const int unit = blockIdx.x % XCDS * (COMPUTE_UNITS / XCDS) + blockIdx.x / XCDS;
+    if constexpr (F::PLANES == 2) {
+        if (far_apart(a.o)) {
+            if (a.grad_hidden) far_hidden<F>(a, p, labelled, piece, unit);
+            if (a.grad_weight) far_weight<F>(a, p, labelled, unit);
+            return;
+        }
+    }
     if (a.grad_hidden && labelled > NARROW) hidden_tasks<F, TILE>(a, p, labelled, piece, unit, lds);
     else if (a.grad_hidden && labelled) hidden_tasks<F, NARROW>(a, p, labelled, piece, unit, lds);
     if (a.grad_weight) weight_tasks<F, R>(a, p, labelled, unit, lds);
@@ -1248,7 +1432,7 @@ __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
     }
     if (t >= s.N) return;
     if (at >= 0) {
-        const float by = factor_of(a, labelled) * (F::PLANES == 2 ? __builtin_amdgcn_ldexpf(1.f, a.o.kept.head[2]) : 1.f);
+        const float by = factor_of(a, labelled) * (F::PLANES == 2 && !far_apart(a.o) ? __builtin_amdgcn_ldexpf(1.f, a.o.kept.head[2]) : 1.f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= by;
     }
@@ -1325,7 +1509,7 @@ Operands operands(const lffn_linear_cross_entropy &a, Carver &c, bool split) {
     o.bias = c.take<float>(o.s.Vp);
     o.weight = {static_cast<const char *>(a.weight), a.weight_stride * (planes == 2 ? 4 : 2), o.s.V, o.s.K};
     if (planes == 2) {
-        o.weight_scale = c.take<float>(o.s.Vp);          // (of few tokens: a workgroup's, and one of the tokens)
+        o.weight_scale = c.take<float>(o.s.Vp);          // (of few tokens: two a workgroup, and two of the tokens)
         o.row_scale = c.take<float>(Np);
     }
     if (split) {
@@ -1380,6 +1564,7 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     w.r.most = c.take<float>(a.reduction == 0 ? (a.tokens + CHUNK - 1) / CHUNK : 0);
     b.power = c.take<float>(1);
     b.shares = c.take<int32_t>(3);
+    if (planes == 2) b.token = w.r.token = c.take<int32_t>(Np);
     if (a.reduction != 0) b.coefficient = nullptr, w.r.most = nullptr;
     // as many launches as pieces if all tokens are labelled; with fewer the last ones find nothing
     const int64_t entries = a.tokens == 0 ? 0 : widest(b.d_bytes, Np, (int)planes);
@@ -1498,13 +1683,13 @@ extern "C" int lffn_linear_cross_entropy_fwd(const lffn_linear_cross_entropy *a,
     f.logits = kept ? f.f.o.kept.logits : nullptr;
     fill(f.r, *a, f.f.o);
     if (a->reduction == 0) f.j.loss = f.r.loss = loss, f.j.sums = nullptr;
-    // (workgroups that look for the largest scales behind those that join)
+    // (workgroups that look for the largest and the least scales behind those that join)
     const int looking = a->format == LFFN_ROWS_F32 ? 2 * LOOKING : 0;
     f.j.weight_scale = f.f.o.weight_scale, f.j.row_scale = f.f.o.row_scale;
     if (a->tokens > 0 && few_tokens(*a)) {
         const int done = a->format == LFFN_ROWS_F32 ? few<F32Row>(*a, f, st) : a->format == LFFN_ROWS_BF16 ? few<BF16>(*a, f, st) : few<F16>(*a, f, st);
         if (done != LFFN_OK) return done;
-        f.j.joining = int((a->tokens + 15) / 16), f.j.entries = f.j.tiles, f.j.few = 1;
+        f.j.joining = int((a->tokens + 15) / 16), f.j.entries = 2 * f.j.tiles, f.j.few = 1;
         join_kernel<<<dim3(f.j.joining + looking), dim3(256), 0, st>>>(f.j);
     } else if (a->tokens > 0) {
         if (a->tokens > COUNTED) {
@@ -1544,6 +1729,8 @@ extern "C" int lffn_linear_cross_entropy_bwd(const lffn_linear_cross_entropy *a,
     b.g_loss = g_loss;
     b.grad_hidden = grad_hidden, b.grad_weight = grad_weight, b.grad_bias = grad_bias;
     b.bias_format = a->bias_format, b.reduction = a->reduction;
+    b.hidden = static_cast<const float *>(a->hidden), b.whole_weight = static_cast<const float *>(a->weight);
+    b.hidden_stride = a->hidden_stride, b.weight_stride = a->weight_stride;
     fill(w.r, *a, b.o);
     w.r.g_loss = g_loss;
     launch_rows<true>(*a, w.r, st);

@@ -1742,7 +1742,7 @@ def _loss_kept_bytes(hidden, weight):
     """lffn_linear_cross_entropy_kept_bytes: how many tokens have a label, where a token is among them, and of those the label and two levels; of up to 64 tokens whose rows fit
     160 KB the logits, where they are no more than the weights."""
     (tokens, columns), vocabulary, size = hidden.shape, weight.shape[0], hidden.element_size()
-    kept = 16 + (tokens * 4 + 15) // 16 * 16 + (tokens + 255) // 256 * 256 * 12
+    kept = 32 + (tokens * 4 + 15) // 16 * 16 + (tokens + 255) // 256 * 256 * 12
     few = tokens <= 64 and (32 if tokens <= 32 else 64) * ((columns * size + 127) // 128 * 8 | 1) * 16 + 64 * 64 + 64 * 4 <= 160 * 1024
     return kept + (tokens * ((vocabulary + 31) // 32 * 32) * 4 if few and tokens * 4 <= columns * size else 0)
 
