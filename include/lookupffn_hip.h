@@ -1017,8 +1017,9 @@ int lffn_layer_norm_rows_bwd(const lffn_layer_norm_rows *a, const float *stats, 
  * as are the addresses); columns a multiple of 8, at most 65536; vocabulary at most 2^22, tokens at most 2^24, tokens * columns at most 2^32.  bias: [vocabulary] of bias_format, or NULL.
  * labels: [tokens], int64 where labels_64 is not 0, else int32.
  * reduction 0: loss is [tokens], zeros for the others; 1: their mean (0 of none), 2: their sum; [1].
- * format 0: products of two half-precision terms a number, fp32 accuracy; in the backward a number of hidden or weight is held to 2^-22 of the largest of its row.  Where labelled rows of
- * hidden, or rows of weight, are more than 2^16 apart, or logits may be 2^18, its products are of the floats as they are, at a quarter of the speed.
+ * format 0: products of two half-precision terms a number, fp32 accuracy; in the backward a number of hidden or weight is held to 2^-22 of the largest of its row,
+ * and a gradient of the logits to 2^-38 of the largest token's.  Where labelled rows of hidden, or rows of weight, are more than 2^16 apart, or logits may be 2^18, or tokens' gradients are more than
+ * 2^8 apart, its products are of the floats as they are, at a quarter of the speed.
  * 1 and 2: sums in fp32; in the backward the logits' gradients are rounded to the format.
  * kept: what the backward needs, of lffn_linear_cross_entropy_kept_bytes, 16-byte aligned, or NULL; of up to 64 tokens it may hold the logits.  workspace: 16-byte aligned.
  */

@@ -13,7 +13,7 @@
 // share adds to is its own: no atomics on results, the same bits on every call.
 //
 // fp32 in the backward: a sum's numbers have one power of two in common, so rows are laid by the largest of their array, and a row that is far below that would have few bits left.  Where rows,
-// or logits, are too far apart (far_apart) the rows are laid one by one, as in the forward, d stays a float, and both products are of the floats themselves (far_hidden, far_weight).
+// or logits, or tokens' gradients, are too far apart (far_apart) the rows are laid one by one, as in the forward, d stays a float, and both products are of the floats themselves (far_hidden, far_weight).
 #include "product_tiles.h"
 
 namespace {
@@ -57,14 +57,29 @@ struct Operands {
     float *bias;               // [Vp] fp32, -infinity behind the vocabulary
     float *weight_scale;       // two-term numbers: [Vp], [Np], by which sums are multiplied
     float *row_scale;
+    const float2 *range;       // the backward of losses by token: [RANGES] the largest and the least finite gradients of labelled tokens, zeros aside; else null
 };
+
+__device__ __forceinline__ float wave_most(float v) {
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) v = fmaxf(v, __shfl_xor(v, m));
+    return v;
+}
+
+__device__ __forceinline__ float wave_least(float v) { return -wave_most(-v); }
 
 // Whether two-term numbers cannot be laid by the largest of their arrays in the backward.  Rows whose largest is 2^-16 of the array's have 22 bits of it left, what a second term has at the
 // least.  And the logits that are formed of them must be those whose levels the forward left: laid either way they are off from each other by 2^-38 of the largest number of a row, of an
-// entry and the columns, which has to be no more than 2^-18.  (A row's largest is less than 2^14 times the power of two that it was divided by; kept logits are not formed again.)
-constexpr int ROWS_APART = 16, LOGITS_LARGEST = 20;
+// entry and the columns, which has to be no more than 2^-18.  (A row's largest is less than 2^14 times the power of two that it was divided by; kept logits are not formed again.)  d is scaled by
+// the largest of the tokens' gradients and held to 2^-38 of it: a token's at 2^-8 of that to 2^-30 of its own.  Called by whole wavefronts.
+constexpr int ROWS_APART = 16, LOGITS_LARGEST = 20, GRADIENTS_APART = 8, RANGES = 64;
 __device__ __forceinline__ bool far_apart(const Operands &o) {
     const int32_t *h = o.kept.head;
+    if (o.range) {
+        const float2 r = o.range[threadIdx.x % RANGES];
+        const float most = wave_most(r.x), least = wave_least(r.y);
+        if (most > 0.f && ilogbf(most) - ilogbf(least) > GRADIENTS_APART) return true;
+    }
     return max(h[1] - min(h[1], h[3]), h[2] - min(h[2], h[4])) > ROWS_APART || (!o.kept.logits && h[1] + h[2] + 28 + (32 - __clz(o.s.K - 1)) > LOGITS_LARGEST);
 }
 
@@ -84,8 +99,8 @@ struct RowsArgs {
     int parts;                                 // workgroups that lay a chunk's rows
     int32_t *token;                            // [labelled], or null
     float *loss;                               // [N]: zeros for the others, or null
-    const float *g_loss;                       // [N]
-    float *most;                               // the backward of losses by token: of a chunk's finite g_loss
+    const float *g_loss;                       // the backward of losses by token: [N]
+    float *coefficient, *power;                // and what becomes of it (BackwardArgs), or null
 };
 
 __device__ __forceinline__ int label_of(const void *labels, int wide, int64_t i, int64_t ignore, int V) {
@@ -111,14 +126,6 @@ __global__ __launch_bounds__(1024) void count_kernel(const void *labels, int wid
         groups[blockIdx.x] = sum;
     }
 }
-
-__device__ __forceinline__ float wave_most(float v) {
-#pragma unroll
-    for (int m = 32; m > 0; m /= 2) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
-}
-
-__device__ __forceinline__ float wave_least(float v) { return -wave_most(-v); }
 
 // A row of `columns` numbers as the products read it, zeros up to `padded`, by one wavefront.  Two-term numbers: scaled by the row's largest, or to `exponent` where that is
 // given; -> the power of two of the way back, 0 of a row of zeros (no sum of it is anything else) and of an infinite one (which is lost).
@@ -201,6 +208,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     }
     __shared__ int place[CHUNK], before[4];
     const int t0 = chunk * CHUNK;
+    const bool far = PLANES == 2 && BACKWARD && far_apart(a.o);
     int labelled = 0;              // up to and with this chunk
     if constexpr (!BACKWARD) {
         int n = 0;
@@ -234,15 +242,19 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
             const int at = t0 + lane < s.N ? k.pos[t0 + lane] : -1;
             place[lane] = at;
             if (a.token && part == 0 && at >= 0) a.token[at] = t0 + lane;
-            if (a.most && part == 0) {
-                const float g = at >= 0 ? fabsf(a.g_loss[t0 + lane]) : 0.f, most = wave_most(g < INFINITY ? g : 0.f);
-                if (lane == 0) a.most[chunk] = most;
+            if (a.coefficient && part == 0) {
+                // Tokens' own gradients by the power of two of their largest; far apart as they are, but for very large ones (d is lifted)
+                const float most = wave_most(a.o.range[lane].x);
+                int e = most > 0x1p100f ? 28 : 0;
+                const float scale = far ? __builtin_amdgcn_ldexpf(1.f, -e) : scale_to(most, 0, e);
+                if (at >= 0) a.coefficient[at] = a.g_loss[t0 + lane] * scale;
+                if (chunk == 0 && lane == 0) *a.power = __builtin_amdgcn_ldexpf(1.f / LIFT, e);
             }
         }
     }
     __syncthreads();
     const int64_t row_bytes = s.Kp * 2 * PLANES;
-    const int *const exponent = PLANES == 2 && BACKWARD && !far_apart(a.o) ? k.head + 1 : nullptr;
+    const int *const exponent = BACKWARD && !far ? k.head + 1 : nullptr;
     for (int i = part * 4 + wave; i < CHUNK; i += 4 * a.parts) {
         const int at = place[i];
         if (at < 0) continue;
@@ -901,26 +913,26 @@ __device__ __forceinline__ void put_shares(const BackwardArgs &a, int labelled, 
 
 // What both gradients' sums are multiplied with: of a sum or mean what all tokens' d are, else the power of two that their coefficients were divided by.
 __device__ __forceinline__ float factor_of(const BackwardArgs &a, int labelled) {
-    if (a.reduction == 0) return *a.power;
+    if (a.coefficient) return *a.power;
     return *a.g_loss / (a.reduction == 1 ? (float)max(labelled, 1) : 1.f) * (1.f / LIFT);
 }
 
-// Tokens' own gradients by the power of two of their largest, which is that of the chunks' largest ones.
-__global__ __launch_bounds__(1024) void coefficient_kernel(BackwardArgs a, const float *chunk_most) {
-    __shared__ float most[16];
-    const int tid = threadIdx.x, chunks = (a.o.s.N + CHUNK - 1) / CHUNK, n = blockIdx.x * 1024 + tid;
-    const int at = n < a.o.s.N ? a.o.kept.pos[n] : -1;
-    const float g = at >= 0 ? a.g_loss[n] : 0.f;
-    float v = 0.f;
-    for (int i = tid; i < chunks; i += 1024) v = fmaxf(v, chunk_most[i]);
-    v = wave_most(v);
-    if (tid % 64 == 0) most[tid / 64] = v;
+// The range of the tokens' own gradients, RANGES workgroups' shares of the tokens.
+__global__ __launch_bounds__(1024) void range_kernel(const int32_t *pos, const float *g_loss, int N, float2 *range) {
+    __shared__ float high[16], low[16];
+    const int tid = threadIdx.x;
+    float most = 0.f, least = INFINITY;
+#pragma unroll 4
+    for (int n = blockIdx.x * 1024 + tid; n < N; n += RANGES * 1024) {
+        const float g = pos[n] >= 0 ? fabsf(g_loss[n]) : 0.f;
+        if (g > 0.f && g < INFINITY) most = fmaxf(most, g), least = fminf(least, g);
+    }
+    most = wave_most(most), least = wave_least(least);
+    if (tid % 64 == 0) high[tid / 64] = most, low[tid / 64] = least;
     __syncthreads();
-    for (int i = 0; i < 16; ++i) v = fmaxf(v, most[i]);
-    int e;
-    const float scale = scale_to(v, 0, e);
-    if (at >= 0) a.coefficient[at] = g * scale;
-    if (n == 0) *a.power = __builtin_amdgcn_ldexpf(1.f / LIFT, e);
+    if (tid > 0) return;
+    for (int i = 1; i < 16; ++i) most = fmaxf(most, high[i]), least = fminf(least, low[i]);
+    range[blockIdx.x] = make_float2(most, least);
 }
 
 // A block's 32 numbers of each column, 16 a lane (mfma_row), packed: w[k] has 16 bytes of column 16 k + lane % 16, the piece_of_lane-th of its four.  Lanes 32 apart and then lanes 16 apart
@@ -1039,6 +1051,7 @@ template <typename F>
 __global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
     const int labelled = a.o.kept.head[0], n = blockIdx.y, V = a.o.s.V;
     const Piece p = piece_of<F>(a, labelled, piece);
+    const bool far = F::PLANES == 2 && far_apart(a.o);
     if (piece == 0 && n == FEW_ROWS - 1 && blockIdx.x == 0 && threadIdx.x < 64) put_shares<F>(a, labelled, p);
     const int in = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 8;
     if (in >= p.ld - APART || p.width <= 0) return;
@@ -1060,7 +1073,7 @@ __global__ __launch_bounds__(256) void few_d_kernel(BackwardArgs a, int piece) {
             }
         }
     }
-    if (F::PLANES == 2 && far_apart(a.o)) {
+    if (far) {
         store8<F32Row>(a.d + (int64_t(n) * p.ld + in) * 4, l);
         return;
     }
@@ -1413,6 +1426,7 @@ __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
     const int in = threadIdx.x % PLACES, part = threadIdx.x / PLACES, pieces = s.K / 8;
     const int64_t i = int64_t(blockIdx.x) * PLACES + in, t = i / pieces, c = i % pieces * 8;
     const int at = t < s.N ? a.o.kept.pos[t] : -1, labelled = a.o.kept.head[0];
+    const bool far = F::PLANES == 2 && far_apart(a.o);
     float v[8] = {};
     auto add = [&](const float4 &x, const float4 &y) { v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w; };
     if (at >= 0) {
@@ -1432,7 +1446,7 @@ __global__ __launch_bounds__(256) void hidden_kernel(BackwardArgs a) {
     }
     if (t >= s.N) return;
     if (at >= 0) {
-        const float by = factor_of(a, labelled) * (F::PLANES == 2 && !far_apart(a.o) ? __builtin_amdgcn_ldexpf(1.f, a.o.kept.head[2]) : 1.f);
+        const float by = factor_of(a, labelled) * (F::PLANES == 2 && !far ? __builtin_amdgcn_ldexpf(1.f, a.o.kept.head[2]) : 1.f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= by;
     }
@@ -1561,11 +1575,12 @@ int64_t carve(const lffn_linear_cross_entropy &a, char *base, Backward &w) {
     b.parts_bytes = one > PARTS_BYTES ? one : one * SHARES < PARTS_BYTES ? one * SHARES : PARTS_BYTES;
     b.parts = c.take<float>(b.parts_bytes / 4);
     b.coefficient = c.take<float>(a.reduction == 0 ? Np : 0);
-    w.r.most = c.take<float>(a.reduction == 0 ? (a.tokens + CHUNK - 1) / CHUNK : 0);
+    float2 *const range = c.take<float2>(a.reduction == 0 ? RANGES : 0);
     b.power = c.take<float>(1);
     b.shares = c.take<int32_t>(3);
     if (planes == 2) b.token = w.r.token = c.take<int32_t>(Np);
-    if (a.reduction != 0) b.coefficient = nullptr, w.r.most = nullptr;
+    if (a.reduction == 0) b.o.range = range, w.r.coefficient = b.coefficient, w.r.power = b.power;
+    else b.coefficient = nullptr;
     // as many launches as pieces if all tokens are labelled; with fewer the last ones find nothing
     const int64_t entries = a.tokens == 0 ? 0 : widest(b.d_bytes, Np, (int)planes);
     b.pieces = a.tokens == 0 ? 0 : int((a.vocabulary + entries - 1) / entries);
@@ -1733,8 +1748,8 @@ extern "C" int lffn_linear_cross_entropy_bwd(const lffn_linear_cross_entropy *a,
     b.hidden_stride = a->hidden_stride, b.weight_stride = a->weight_stride;
     fill(w.r, *a, b.o);
     w.r.g_loss = g_loss;
+    if (a->reduction == 0) range_kernel<<<dim3(RANGES), dim3(1024), 0, st>>>(b.o.kept.pos, g_loss, (int)a->tokens, const_cast<float2 *>(b.o.range));
     launch_rows<true>(*a, w.r, st);
-    if (a->reduction == 0) coefficient_kernel<<<dim3(unsigned((a->tokens + 1023) / 1024)), dim3(1024), 0, st>>>(b, w.r.most);
     const int done = a->format == LFFN_ROWS_F32    ? backward<F32Two, F32Row>(b, st)
                      : a->format == LFFN_ROWS_BF16 ? backward<BF16, BF16Row>(b, st)
                                                    : backward<F16, F16Row>(b, st);

@@ -89,8 +89,8 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
     "sum", or "none" (the shape of labels).
 
     float32: products of two half-precision terms a number, sums in float32, errors of the size of float32 products'; in the backward a number of hidden or
-    weight is held to 2^-22 of the largest of its row.  Where that is not to be had with one power of two for an array, because labelled rows of hidden, or rows of weight, are more than
-    2^16 apart, or logits may be 2^18, its products are of the floats as they are, at a quarter of the speed.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half:
+    weight is held to 2^-22 of the largest of its row, and a gradient of the logits to 2^-38 of the largest token's.  Where that would cost others their bits, because labelled rows of
+    hidden, or rows of weight, are more than 2^16 apart, or logits may be 2^18, or tokens' gradients are more than 2^8 apart, its products are of the floats as they are, at a quarter of the speed.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half:
     held to 2^-38 of the largest token's).
     Memory: of up to 64 tokens the logits are kept for the backward where they are no more bytes than weight.  The backward has a workspace of up to 1 GB for the
     logits' gradients (with more than some 250000 tokens 4.2 KB a token) and up to 0.75 GB for sums; float32 weights are laid out once more.

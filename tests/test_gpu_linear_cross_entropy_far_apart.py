@@ -1,4 +1,4 @@
-"""linear_cross_entropy where numbers are far apart: a token, or an entry of another size than the rest, logits that are large everywhere.  What one of them is must not
+"""linear_cross_entropy where numbers are far apart: a token, an entry or a token's gradient of another size than the rest, logits that are large everywhere.  What one of them is must not
 reach the others' gradients.  Against 64 bits."""
 import math
 
@@ -85,6 +85,17 @@ def test_large_logits_everywhere(N, V, K, dtype):
     """Logits of 10^8 and more: every token's softmax is one entry, and both directions have to see the same one at the same height."""
     h, w, y = (1e4 * _randn(N, K)).to(dtype), (1e4 * _randn(V, K, seed=1)).to(dtype), _labels(N, V)
     _check(h, w, None, y, torch.full((N,), 2.0 ** -6, device=DEV))
+
+
+@pytest.mark.parametrize("steps", [7, 30, 60])
+@pytest.mark.parametrize("N,V,K", SIZES)
+def test_tokens_gradients_of_many_sizes(N, V, K, steps):
+    """Each token's gradient as exact as if it were alone: sizes from 1 down to 2^-steps, both signs, zeros."""
+    h, w, b, y = _randn(N, K), 1.5 / math.sqrt(K) * _randn(V, K, seed=1), 0.5 * _randn(V, seed=2), _labels(N, V)
+    n = torch.arange(N, device=DEV)
+    g = 2.0 ** -(n * 7 % (steps + 1)).float() * torch.where(n % 2 == 0, 1.0, -1.0)
+    g[9] = 0
+    _check(h, w, b, y, g)
 
 
 def test_in_pieces_of_the_vocabulary():
