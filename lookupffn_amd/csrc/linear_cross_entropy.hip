@@ -911,10 +911,12 @@ __device__ __forceinline__ void put_shares(const BackwardArgs &a, int labelled, 
     if (threadIdx.x % 64 == 0) a.shares[0] = shares.vocabulary, a.shares[1] = p.pieces, a.shares[2] = shares.tokens;
 }
 
-// What both gradients' sums are multiplied with: of a sum or mean what all tokens' d are, else the power of two that their coefficients were divided by.
+// What both gradients' sums are multiplied with: of a sum or mean what all tokens' d are, nothing without any (whatever the loss's gradient is), else the power of two that their
+// coefficients were divided by.
 __device__ __forceinline__ float factor_of(const BackwardArgs &a, int labelled) {
+    if (labelled == 0) return 0.f;
     if (a.coefficient) return *a.power;
-    return *a.g_loss / (a.reduction == 1 ? (float)max(labelled, 1) : 1.f) * (1.f / LIFT);
+    return *a.g_loss / (a.reduction == 1 ? (float)labelled : 1.f) * (1.f / LIFT);
 }
 
 // The range of the tokens' own gradients, RANGES workgroups' shares of the tokens.

@@ -83,3 +83,15 @@ def test_gradients(N, V, K, dtype):
     grads = torch.autograd.grad(linear_cross_entropy(h, w, None, y, reduction="none"), leaves, g)
     want, bounds = reference(h, w, None, y, g)
     assert max(worst(got, want[i], bounds[i]) for i, got in enumerate(grads, 1)) <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [7, 300])
+def test_no_label_and_a_gradient_that_is_no_number(N, dtype):
+    """Tokens without a label have no part in anything, whatever the loss's gradient is."""
+    h, w, b = ((t / 8).to(dtype).requires_grad_() for t in (_randn(N, 64), _randn(200, 64, seed=1), _randn(200, seed=2)))
+    y = torch.full((N,), -100, device=DEV)
+    for g in (float("inf"), float("nan")):
+        for reduction in ("mean", "sum", "none"):
+            loss = linear_cross_entropy(h, w, b, y, reduction=reduction)
+            assert all((t == 0).all() for t in torch.autograd.grad(loss, (h, w, b), torch.full_like(loss, g)))
