@@ -323,7 +323,8 @@ class Lookup(nn.Module):
 class MaskedLMHead(nn.Module):
     """What the reference pre-trains its encoder by (src/roberta/tasks/mlm.py:33-112), behind the encoder: a projection, gelu and layer norm of the states, and the projection
     to the vocabulary by the word embeddings with a bias of its own.  With labels the loss, whose logits are not in memory as a whole and whose cost is that of the
-    labelled tokens (``linear_cross_entropy``); without, the logits.  GPU only; hidden_size a multiple of 8.
+    labelled tokens (``linear_cross_entropy``, GPU only; hidden_size a multiple of 8); without, the logits.  The norm is this package's ``layer_norm`` wherever it is the nn.LayerNorm
+    that the head was built with and nothing watches its calls, else what stands in its place.
 
     ``config``: hidden_size, vocab_size, layer_norm_eps."""
 
@@ -336,8 +337,11 @@ class MaskedLMHead(nn.Module):
     def forward(self, hidden_states, word_embeddings, labels=None, *, ignore_index=-100, reduction="mean"):
         """hidden_states [..., hidden], word_embeddings [vocabulary, hidden], labels [...] (ignore_index: not asked for) -> the loss, by ``reduction``; without labels
         the logits [..., vocabulary]."""
-        norm = self.LayerNorm
-        hidden = layer_norm(F.gelu(self.dense(hidden_states)), norm.weight, norm.bias, eps=norm.eps)
+        hidden, norm = F.gelu(self.dense(hidden_states)), self.LayerNorm
+        if _plain(norm, nn.LayerNorm) and hidden.is_cuda and norm.normalized_shape == hidden.shape[-1:]:
+            hidden = layer_norm(hidden, norm.weight, norm.bias, eps=norm.eps)
+        else:
+            hidden = norm(hidden)
         if labels is None:
             return F.linear(hidden, word_embeddings, self.bias)
         # (under autocast the states are 16 bits wide, and the projection is as any other's)
