@@ -58,7 +58,8 @@ class RobertaEmbeddings(nn.Module):
     (src/roberta/models/postnorm.py:6-28); positions are offset by pad_token_id + 1.
 
     kernels: the tables are read, and their gradients summed, by this package's ``embedding`` (the same numbers forward; gradients that cannot be
-    differentiated again) wherever a table is the nn.Embedding it was built with."""
+    differentiated again) wherever a table is the nn.Embedding it was built with, of float32, float16 or bfloat16.  There a word, type or position outside its table (a
+    sequence longer than max_position_embeddings) has a row of zeros and no gradient, where nn.Embedding fails."""
 
     def __init__(self, config, kernels=False):
         super().__init__()
@@ -71,8 +72,8 @@ class RobertaEmbeddings(nn.Module):
         self.dropout = nn.Dropout(config.hidden_dropout_prob)
 
     def _rows(self, table, ids):
-        if (self.kernels and _plain(table, nn.Embedding) and table.weight.is_cuda and table.max_norm is None and not table.sparse
-                and not table.scale_grad_by_freq):
+        if (self.kernels and _plain(table, nn.Embedding) and table.weight.is_cuda and ops.row_format(table.weight.dtype) is not None
+                and table.max_norm is None and not table.sparse and not table.scale_grad_by_freq):
             return embedding(ids, table.weight, padding_idx=table.padding_idx)
         return table(ids)
 
@@ -350,7 +351,8 @@ class MaskedLMHead(nn.Module):
 
 class LookupForMaskedLM(nn.Module):
     """``Lookup`` and ``MaskedLMHead``, which projects by the encoder's word embeddings: what the reference trains (src/roberta/tasks/mlm.py:33-112).  GPU only, as the
-    embeddings' kernels are; forward(..., labels) -> the mean loss of the labelled tokens, without labels the logits."""
+    embeddings' kernels are; forward(..., labels) -> the mean loss of the labelled tokens, without labels the logits.  Nothing is looked at on the host: numbers outside a table
+    are rows of zeros (``RobertaEmbeddings``), labels outside the vocabulary are as if not asked for (``linear_cross_entropy``)."""
 
     def __init__(self, config):
         super().__init__()
