@@ -92,8 +92,10 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
     weight is held to 2^-22 of the largest of its row, and a gradient of the logits to 2^-38 of the largest token's.  Where that would cost others their bits, because labelled rows of
     hidden, or rows of weight, are more than 2^16 apart, or logits may be 2^18, or tokens' gradients are more than 2^8 apart, its products are of the floats as they are, at a quarter of the speed.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half:
     held to 2^-38 of the largest token's).
-    Memory: of up to 64 tokens the logits are kept for the backward where they are no more bytes than weight.  The backward has a workspace of up to 1 GB for the
-    logits' gradients (with more than some 250000 tokens 4.2 KB a token) and up to 0.75 GB for sums; float32 weights are laid out once more.
+    Memory, beside 16 to 20 bytes a token: both directions lay hidden's rows out once more, in whole 128 columns, and float32 weights (not in the forward of few tokens).  The
+    forward has 8 bytes a token, labelled or not, for every 256 entries of the vocabulary (1.6 KB of 50265).  The backward has up to 1 GB for the logits' gradients, or, if that is more, 4.2 KB a
+    token (float32 8.4), up to 256 MB, or 4 bytes a number of hidden, for sums of hidden's gradient, and up to 512 MB for weight's, where that is small and the tokens are many.  Of up to 64 tokens the
+    logits are kept for it where they are no more bytes than weight.
     -> float32.  Gradients: hidden, weight and bias, the same bits on every call; none of theirs, and none in forward mode (an error); captured in graphs as ``cross_attention`` is."""
     host = _host()
     if host:
