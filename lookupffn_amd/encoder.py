@@ -61,6 +61,8 @@ class RobertaEmbeddings(nn.Module):
     differentiated again) wherever a table is the nn.Embedding it was built with, of float32, float16 or bfloat16.  There a word, type or position outside its table (a
     sequence longer than max_position_embeddings) has a row of zeros and no gradient, where nn.Embedding fails."""
 
+    kernels = False                      # (of a module that was pickled without)
+
     def __init__(self, config, kernels=False):
         super().__init__()
         self.kernels = kernels

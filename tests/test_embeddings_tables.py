@@ -1,4 +1,5 @@
 """Which tables RobertaEmbeddings reads by this package's kernels, and which are torch's; without a GPU, by tensors that have no memory."""
+import pickle
 from argparse import Namespace
 
 import pytest
@@ -26,3 +27,11 @@ def test_types(dtype, by_kernels, monkeypatch):
         ids = torch.zeros(2, 5, dtype=torch.int64, device="cuda")
         out = module(ids, ids, ids)
     assert len(calls) == by_kernels and out.shape == (2, 5, 64) and out.dtype == dtype
+
+
+def test_a_module_that_was_pickled_without_the_choice():
+    module = RobertaEmbeddings(CONFIG)
+    del module.__dict__["kernels"]
+    again = pickle.loads(pickle.dumps(module))
+    ids = torch.zeros(2, 5, dtype=torch.int64)
+    assert not again.kernels and torch.equal(again(ids, ids, ids), RobertaEmbeddings.forward(module, ids, ids, ids))
