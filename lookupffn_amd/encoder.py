@@ -341,7 +341,7 @@ class MaskedLMHead(nn.Module):
         """hidden_states [..., hidden], word_embeddings [vocabulary, hidden], labels [...] (ignore_index: not asked for) -> the loss, by ``reduction``; without labels
         the logits [..., vocabulary]."""
         hidden, norm = F.gelu(self.dense(hidden_states)), self.LayerNorm
-        if _plain(norm, nn.LayerNorm) and hidden.is_cuda and norm.normalized_shape == hidden.shape[-1:]:
+        if _plain(norm, nn.LayerNorm) and hidden.is_cuda and ops.row_format(hidden.dtype) is not None and norm.normalized_shape == hidden.shape[-1:]:
             hidden = layer_norm(hidden, norm.weight, norm.bias, eps=norm.eps)
         else:
             hidden = norm(hidden)

@@ -3,6 +3,7 @@ from argparse import Namespace
 
 import torch
 import torch.nn.functional as F
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from lookupffn_amd import MaskedLMHead
 
@@ -32,3 +33,15 @@ def test_another_norm_is_what_runs():
     head.LayerNorm = Shifted(64)
     want = F.layer_norm(F.gelu(head.dense(x)), (64,), head.LayerNorm.weight, head.LayerNorm.bias, 1e-5) + 1
     assert torch.equal(head(x, table), F.linear(want, table, head.bias))
+
+
+def test_logits_of_a_type_that_no_kernel_takes():
+    with FakeTensorMode():
+        torch.set_default_dtype(torch.float64)
+        try:
+            with torch.device("cuda"):
+                head, x, table = MaskedLMHead(CONFIG), torch.randn(3, 64), torch.randn(300, 64)
+        finally:
+            torch.set_default_dtype(torch.float32)
+        out = head(x, table)
+    assert out.shape == (3, 300) and out.dtype == torch.float64
