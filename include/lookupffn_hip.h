@@ -1020,7 +1020,7 @@ int lffn_layer_norm_rows_bwd(const lffn_layer_norm_rows *a, const float *stats, 
  * format 0: products of two half-precision terms a number, fp32 accuracy; in the backward a number of hidden or weight is held to 2^-22 of the largest of its row,
  * and a gradient of the logits to 2^-38 of the largest token's.  Where labelled rows of hidden, or rows of weight, are more than 2^16 apart, or logits may be 2^18, or tokens' gradients are more than
  * 2^8 apart, its products are of the floats as they are, at a quarter of the speed.
- * 1 and 2: sums in fp32; in the backward the logits' gradients are rounded to the format.
+ * 1 and 2: sums in fp32; in the backward the logits' gradients are rounded to the format (half's held to 2^-38 of the largest token's), also those that grad_bias adds up.
  * kept: what the backward needs, of lffn_linear_cross_entropy_kept_bytes, 16-byte aligned, or NULL; of up to 64 tokens it may hold the logits.  workspace: 16-byte aligned.
  */
 typedef struct lffn_linear_cross_entropy {

@@ -495,10 +495,12 @@ static_assert(NarrowLogits::M * NarrowLogits::TOKENS <= WAVES_M * TILE, "the par
 
 // ---------------------------------------------------------------- few tokens
 
-// Up to 64 tokens whose rows fit LDS, and whose logits are no more bytes than the weights: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a whole; a wavefront takes 32 entries of the vocabulary at a
-// time, whose rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, six such in flight.  Nothing is laid together before: a launch less.
-// fp32 is multiplied as it is (v_mfma_f32_32x32x2_f32): at 32 tokens a product takes as long as its weights' bytes (32 x 50265 x 840 64 us; splitting the weights to memory 71 and the tiles'
-// products 71).  The exponents that the backward's two-term numbers have in common are found on the way.
+// Up to 64 tokens whose rows fit LDS, and whose logits are no more bytes than the weights: reading the weights is all there is.  The labelled tokens' rows lie in every workgroup's LDS as a
+// whole; a wavefront takes 32 entries of the vocabulary at a time, whose rows go from memory straight to its registers as operands, 64 bytes a lane, half a line, six such in flight.  Nothing is
+// laid together before: a launch less.  (64 x 50265 x 768 bfloat16 22.7 us, 3.4 TB/s: 50265 entries are 1571 blocks for 2048 wavefronts, of which a quarter have none, and the others' single blocks
+// begin and end together.)
+// fp32 is multiplied as it is (v_mfma_f32_32x32x2_f32): 32 x 50265 x 840 64 us, where the weights' bytes are 33 and the products 17, but each wavefront's loads and products follow one another
+// (splitting the weights to memory took 71 and the tiles' products 71).  The exponents that the backward's two-term numbers have in common, and the least ones, are found on the way.
 constexpr int FEW = 64, LINE = 128;                                                            // bytes of a row that a step has
 constexpr int few_stride(int64_t row_bytes) { return int(up(row_bytes, LINE)) / 16 | 1; }      // 16-byte pieces of a row in LDS: odd, so that 16 rows meet every bank once
 constexpr int64_t few_lds(int64_t tokens, int64_t row_bytes) {
@@ -963,6 +965,9 @@ __device__ __forceinline__ void pieces_of(const float (&l)[16], uint4 (&w)[2]) {
 constexpr int FEW_ROWS = 2 * STEP;              // tokens that dW's sums over few have, at least
 static_assert(FEW_ROWS >= FEW && FEW_ROWS <= TILE && FEW_ROWS == 2 * NARROW, "two steps; twice a narrow tile");
 
+// d is rounded to the type of what it is multiplied with, as the matrix cores take operands of one type: two terms of it would be twice the products of both gradients.  What that costs is a
+// rounding of each summand, 2^-9 or 2^-12 of it and of either sign (32768 x 512 half, the largest error of hidden's gradient 3.6e-4 of its largest number; with d in fp32 and the result
+// rounded 2.4e-4).
 template <typename F, typename S>
 __device__ __forceinline__ void d_tiles(const BackwardArgs &a, const Piece &p, int labelled, uint32_t lds) {
     const Operands &o = a.o;

@@ -170,7 +170,8 @@ struct Sums {
 };
 
 // The products of one tile after the other.  The steps of all tiles are one stream: while a step's products are formed the next one is there, and the one behind it is on its way, also where
-// it is the next tile's, so that neither a tile's first copies nor what becomes of its results leave the matrix cores without operands.  In a step four chunks of operands are read from
+// it is the next tile's, so that a tile's first products have their operands when the last tile's results are done with.  (While those are, all eight wavefronts are at it and no products are
+// formed: for the loss's logits 8700 clocks a tile, of 29100 at 512 columns, for their gradients 12400 of 33000.)  In a step four chunks of operands are read from
 // LDS, each while the products of the chunk before are formed; with the last one in registers the buffer is free: the one barrier of a step stands there, before the last chunk's products.
 // Every tile has at least two steps.
 template <typename F, int MB, int NB, typename A, typename B>
