@@ -89,9 +89,11 @@ def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, red
     "sum", or "none" (the shape of labels).
 
     float32: products of two half-precision terms a number, sums in float32, errors of the size of float32 products'; in the backward a number of hidden or
-    weight is held to 2^-22 of the largest of its row, and a gradient of the logits to 2^-38 of the largest token's.  Where that would cost others their bits, because labelled rows of
-    hidden, or rows of weight, are more than 2^16 apart, or logits may be 2^18, or tokens' gradients are more than 2^8 apart, its products are of the floats as they are, at a quarter of the speed.  16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half:
-    held to 2^-38 of the largest token's), a float32 bias's gradient is the sum of those.
+    weight is held to 2^-22 of the largest of its row, and a gradient of the logits to 2^-38 of the largest token's.  Where that would cost others their bits
+    (labelled rows of hidden, or rows of weight, more than 2^16 apart, logits that may be 2^18, tokens' gradients more than 2^8 apart; zeros aside) its
+    products are of the floats as they are, at a quarter of the speed.
+    16 bits: sums in float32; in the backward the gradients of the logits are rounded to the type (half: held to 2^-38 of the largest token's), a float32
+    bias's gradient is the sum of those.
     Memory, beside 16 to 20 bytes a token: both directions lay hidden's rows out once more, in whole 128 columns, and float32 weights (not in the forward of few tokens).  The
     forward has 8 bytes a token, labelled or not, for every 256 entries of the vocabulary (1.6 KB of 50265).  The backward has up to 1 GB for the logits' gradients, or, if that is more, 4.2 KB a
     token (float32 8.4), up to 256 MB, or 4 bytes a number of hidden, for sums of hidden's gradient, and up to 512 MB for weight's, where that is small and the tokens are many.  Of up to 64 tokens the
